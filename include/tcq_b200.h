@@ -55,6 +55,7 @@ extern "C" {
 #define TCQ_E_NONFINITE_INPUT (-11) /* tcq_workspace_status: a weight of the last call was NaN or infinite */
 #define TCQ_E_DEVICE_TIMEOUT (-10) /* a bounded in-kernel wait gave up (tcq_workspace_status) */
 #define TCQ_E_TOO_MANY_TILES (-9) /* batch larger than tcq_encode_tb_static_max_tiles(K) */
+#define TCQ_E_BAD_FORMAT (-12)   /* microscaled format or element type unknown */
 
 /* Version of this ABI (bumped on any signature change). */
 TCQ_API int tcq_abi_version(void);
@@ -278,6 +279,62 @@ TCQ_API int tcq_pack_symbols(const int64_t *bits, int64_t n_tiles, int K, uint32
  * (src/trellis/qtip.py:59-66).   lut [65536] fp32
  */
 TCQ_API int tcq_codebook_lut(int codebook, float *lut, void *stream);
+
+/*
+ * 4-bit microscaled floating point (no counterpart in the reference): quantisation, its inverse, and products.
+ *
+ * A matrix of rows x k values is e2m1(code) * block scale [* row scale]:
+ *   TCQ_MS_MXFP4  blocks of 32 columns, scales 2^(byte - 127) (byte 255: NaN), no row scale
+ *   TCQ_MS_NVFP4  blocks of 16 columns, e4m3 scales, and one fp32 scale for each row
+ * and is held as
+ *   codes      [rows][tcq_ms_code_pitch(k)] bytes, 16-byte aligned: two codes a byte, the even column in the low half;
+ *              zeros behind column k
+ *   scales     tcq_ms_scale_bytes(rows, k, format) bytes, 16-byte aligned: [ceil(rows/128)][atoms][32][4][4], block b of
+ *              row r at [r/128][b/4][r%32][r%128/32][b%4], atoms = 2 (mxfp4) or 4 (nvfp4) for every 256 columns begun;
+ *              zeros behind column k.  Places of rows behind the last one may hold anything.
+ *   row_scale  [rows] fp32 (nvfp4), NULL (mxfp4)
+ */
+#define TCQ_MS_MXFP4 0
+#define TCQ_MS_NVFP4 1
+#define TCQ_F32 0
+#define TCQ_F16 1
+#define TCQ_BF16 2
+
+/* Sizes of the storage; 0 for a negative size or an unknown format. */
+TCQ_API size_t tcq_ms_code_pitch(int64_t k);
+TCQ_API size_t tcq_ms_scale_bytes(int64_t rows, int64_t k, int format);
+
+/*
+ * Quantise x [rows][ldx] (type dtype, k columns, ldx >= k).  mxfp4: block scale 2^(floor(log2 amax) - 2), clamped at
+ * 2^-127.  nvfp4: row scale the least 2^j, j >= -80, with amax(row) <= 2688 * 2^j (2^0 for a row of zeros), block scale
+ * e4m3(amax / (6 * row scale)).  Codes are the nearest of the real quotients (ties to the even code, beyond 6 to 6).
+ * A block that holds a NaN or an infinity gets the scale NaN and codes 0; the row scale is taken from the finite values.
+ * rotate = 16, 32, 64 or 128 (it must divide k): the columns are first multiplied by signs [k] (fp32, any factors) and
+ * every `rotate` of them transformed by the orthonormal Hadamard matrix (Sylvester order), in fp32; rotate = 0: neither,
+ * signs NULL.  The outputs are written whole (row_scale: nvfp4 only).
+ */
+TCQ_API int tcq_ms_quantize(const void *x, int dtype, int64_t rows, int64_t k, int64_t ldx, int format, int rotate,
+                            const float *signs, uint8_t *codes, uint8_t *scales, float *row_scale, void *stream);
+
+/* The values, rounded to dtype once: out [rows][ldo], ldo >= k. */
+TCQ_API int tcq_ms_dequantize(const uint8_t *codes, const uint8_t *scales, const float *row_scale, int64_t rows, int64_t k,
+                              int format, void *out, int dtype, int64_t ldo, void *stream);
+
+/*
+ * y[i][r] = sum_c x[i][c] * W[r][c]: x [m][ldx] of type dtype (not quantised), W n x k in 4 bits, y [m][ldy] of type dtype.
+ * Products and sums in fp32, rounded to dtype once; equal for equal inputs, run to run, and a row of y does not depend on
+ * what the other rows of x hold.  Columns of y behind n are left as they are.
+ */
+TCQ_API int tcq_ms_linear(const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t *codes, const uint8_t *scales,
+                          const float *row_scale, int64_t n, int64_t k, int format, void *y, int64_t ldy, void *stream);
+
+/*
+ * y[i][r] = sum_c X[i][c] * W[r][c] with both in 4 bits, of one format: X m x k, W n x k, y [m][ldy] of type dtype.
+ * As tcq_ms_linear otherwise.
+ */
+TCQ_API int tcq_ms_matmul(const uint8_t *x_codes, const uint8_t *x_scales, const float *x_row_scale, int64_t m,
+                          const uint8_t *codes, const uint8_t *scales, const float *row_scale, int64_t n, int64_t k,
+                          int format, void *y, int dtype, int64_t ldy, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,117 @@
+"""4-bit microscaled formats, what needs no GPU: refusals, the storage order, argument checks of the C ABI."""
+import ctypes
+
+import pytest
+import torch
+
+import ms_plain as P
+from trellis_b200 import _lib, microscale as ms, quant
+
+
+def test_plain_forms_round_as_torch_does():
+    """The tests' own e4m3 against torch's cast, and their e2m1 against the nearest of all values."""
+    t = torch.linspace(0, 448, 20001, dtype=torch.float64)
+    t = torch.cat((t, torch.ldexp(t, torch.full((t.numel(),), -12)), torch.arange(0, 449, 0.5, dtype=torch.float64)))
+    byte, v = P.nearest_e4m3(t)
+    want = t.float().to(torch.float8_e4m3fn)
+    assert torch.equal(byte, want.view(torch.uint8).long()) and torch.equal(v, want.double())
+    assert torch.equal(P.scale_values(byte, "nvfp4"), v)
+    q = torch.linspace(-7, 7, 5001, dtype=torch.float64)
+    code = P.nearest_e2m1(q)
+    val = P.values(code[None], torch.full((1, 313), 0x38), None, "nvfp4")[0]
+    grid = torch.tensor(sorted({s * x for x in P.VALUES for s in (1, -1)}), dtype=torch.float64)
+    assert torch.equal((val - q).abs(), (grid[None] - q[:, None]).abs().min(1).values)
+
+
+@pytest.mark.parametrize("fmt", ("mxfp4", "nvfp4"))
+@pytest.mark.parametrize("rows,k", ((1, 1), (3, 31), (130, 257), (256, 512)))
+def test_storage_of_given_blocks(fmt, rows, k):
+    gen = torch.Generator().manual_seed(rows + k)
+    codes, byte, row = P.random_matrix(rows, k, fmt, gen)
+    odd = torch.nn.functional.pad(codes, (0, k % 2), value=5)          # what a program left in the half behind an odd last column
+    q = ms.from_blocks((odd[:, 0::2] | (odd[:, 1::2] << 4)).to(torch.uint8), byte.to(torch.uint8), row, k, fmt)
+    got = P.unpack(q)
+    assert torch.equal(got[0], codes) and torch.equal(got[1], byte)
+    assert (row is None) == (got[2] is None) and (row is None or torch.equal(got[2], row.double()))
+    assert torch.equal(ms.block_scales(q).long(), byte)
+    assert q.codes.numel() == rows * _lib.lib().tcq_ms_code_pitch(k)
+    assert q.scales.numel() == _lib.lib().tcq_ms_scale_bytes(rows, k, ms.FORMATS[fmt])
+
+
+def test_given_blocks_are_checked():
+    c, s = torch.zeros(2, 16, dtype=torch.uint8), torch.zeros(2, 2, dtype=torch.uint8)
+    assert ms.from_blocks(c, s, 0.5, 32, "nvfp4").row_scale.tolist() == [0.5, 0.5]
+    for bad in ((c, s, None, 32, "nvfp4"), (c, s, 1.0, 32, "mxfp4"), (c, s, 1.0, 33, "nvfp4"), (c.int(), s, 1.0, 32, "nvfp4"),
+                (c, s[:1], 1.0, 32, "nvfp4"), (c, s, 1.0, 32, "fp4")):
+        with pytest.raises(ValueError):
+            ms.from_blocks(*bad)
+
+
+def test_refusals_before_touching_the_device():
+    x = torch.zeros(2, 32)
+    for bad in (dict(fmt="int4"), dict(rotate=8, signs=torch.ones(32)), dict(rotate=64, signs=torch.ones(32)), dict(rotate=16),
+                dict(signs=torch.ones(32))):
+        with pytest.raises(ValueError):
+            ms.quantize(x, **bad)
+    with pytest.raises(ValueError):
+        ms.quantize(torch.zeros(2, 2, 32))
+    with pytest.raises(ValueError):
+        ms.quantize(x.double())
+    with pytest.raises(ValueError, match="gradient"):
+        ms.quantize(x.requires_grad_())
+    with pytest.raises(ValueError):
+        ms.linear(x, x)
+    with pytest.raises(ValueError):
+        quant.MicroscaleQuantizer("int4")
+    with pytest.raises(ValueError):
+        quant.MicroscaleQuantizer("nvfp4", rotate=48)
+    with pytest.raises(ValueError):
+        quant.MicroscaledLinear(torch.zeros(2, 32), rotate=16)
+    assert quant.MicroscaleQuantizer("nvfp4").bpw == 4.5 and quant.MicroscaleQuantizer("mxfp4").bpw == 4.25
+    q = P.pack(*P.random_matrix(3, 40, "nvfp4", torch.Generator().manual_seed(0)), "nvfp4")
+    for bad in (q._replace(codes=q.codes[:, :16]), q._replace(scales=q.scales[:, :2]), q._replace(row_scale=None),
+                q._replace(shape=(4, 40)), q._replace(shape=(3, 300)), q._replace(fmt="mxfp4"), q._replace(codes=q.codes.int()),
+                q._replace(row_scale=q.row_scale.double()), q._replace(codes=q.codes.t().contiguous().t())):
+        with pytest.raises(ValueError):
+            ms.dequantize(bad)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="checks the behaviour on a box without a GPU")
+def test_no_cpu_fallback():
+    q = P.pack(*P.random_matrix(3, 40, "nvfp4", torch.Generator().manual_seed(0)), "nvfp4")
+    for call in (lambda: ms.quantize(torch.zeros(2, 32)), lambda: ms.dequantize(q), lambda: ms.linear(torch.zeros(1, 40), q), lambda: ms.matmul(q, q)):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            call()
+
+
+def test_argument_validation_needs_no_gpu():
+    L = _lib.lib()
+    buf = (ctypes.c_char * 4096)()
+    p = ctypes.addressof(buf)
+    p += (-p) % 256
+    Q, D, N, M = L.tcq_ms_quantize, L.tcq_ms_dequantize, L.tcq_ms_linear, L.tcq_ms_matmul
+    assert L.tcq_strerror(-12) and L.tcq_ms_code_pitch(33) == 32 and L.tcq_ms_scale_bytes(129, 1, 1) == 4096
+    assert L.tcq_ms_scale_bytes(1, 1, 2) == 0 and L.tcq_ms_scale_bytes(-1, 1, 0) == 0 and L.tcq_ms_code_pitch(-1) == 0
+    assert Q(p, 0, 1, 16, 16, 2, 0, None, p, p, p, None) == -12         # format
+    assert Q(p, 3, 1, 16, 16, 1, 0, None, p, p, p, None) == -12         # type
+    assert Q(p, 0, -1, 16, 16, 1, 0, None, p, p, p, None) == -3
+    assert Q(p, 0, 1, 16, 15, 1, 0, None, p, p, p, None) == -8          # row stride
+    assert Q(p, 0, 1, 48, 48, 1, 32, p, p, p, p, None) == -8            # rotation does not divide k
+    assert Q(p, 0, 1, 48, 48, 1, 48, p, p, p, p, None) == -8
+    assert Q(p, 0, 1, 48, 48, 1, 16, None, p, p, p, None) == -4         # signs missing
+    assert Q(p, 0, 1, 16, 16, 1, 0, None, p, p, None, None) == -4       # row scales missing
+    assert Q(p, 0, 1, 16, 16, 0, 0, None, p, p, p, None) == -4          # row scales where there are none
+    assert Q(p, 0, 1, 16, 16, 1, 0, None, p + 8, p, p, None) == -5
+    assert Q(p + 2, 0, 1, 16, 16, 1, 0, None, p, p, p, None) == -5
+    assert Q(p, 0, 0, 16, 16, 1, 0, None, None, None, None, None) == 0  # nothing to do
+    assert D(p, p, p, 1, 16, 1, p, 0, 15, None) == -8 and D(p, p, p, 1, 16, 1, None, 0, 16, None) == -4
+    assert D(p, p, p, 1, 1 << 31, 1, p, 0, 1 << 31, None) == -8
+    assert N(p, 2, 1, 16, p, p, p, 4, 16, 1, p, 3, None) == -8          # ldy < n
+    assert N(p, 2, 1, 15, p, p, p, 4, 16, 1, p, 4, None) == -8          # ldx < k
+    assert N(p, 2, 1, 16, p, p, p, 4, 0, 1, p, 4, None) == -8           # no columns
+    assert N(None, 2, 1, 16, p, p, p, 4, 16, 1, p, 4, None) == -4
+    assert N(p + 1, 2, 1, 16, p, p, p, 4, 16, 1, p, 4, None) == -5
+    assert N(p, 2, 0, 16, None, None, None, 4, 16, 1, None, 4, None) == 0
+    assert M(p, p, p, 1, p, p, None, 4, 16, 1, p, 2, 4, None) == -4
+    assert M(p, p, p, 1, p, p + 4, p, 4, 16, 1, p, 2, 4, None) == -5
+    assert M(p, p, p, -1, p, p, p, 4, 16, 1, p, 2, 4, None) == -3

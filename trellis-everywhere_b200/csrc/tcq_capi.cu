@@ -530,9 +530,12 @@ int encode_core(const EncodeIO& io, int K, int codebook, void* ws, size_t ws_byt
 
 size_t tcq::backpointer_workspace_bytes(long long n, int K) { return bp_ws_bytes(n, K); }
 
+// For the entry points of other files: keeps the text for tcq_last_cuda_error and gives the status.
+namespace tcq { int report_cuda_error(cudaError_t err, const char* where) { return cuda_fail(err, where); } }
+
 extern "C" {
 
-int tcq_abi_version(void) { return 4; }
+int tcq_abi_version(void) { return 5; }
 
 const char* tcq_strerror(int code) {
     switch (code) {
@@ -548,6 +551,7 @@ const char* tcq_strerror(int code) {
         case TCQ_E_NONFINITE_INPUT: return "a weight was NaN or infinite; the codes of its tile are meaningless";
         case TCQ_E_DEVICE_TIMEOUT: return "a bounded wait inside a kernel gave up; the outputs of that call are invalid";
         case TCQ_E_TOO_MANY_TILES: return "more tiles than the static scratch holds (see tcq_encode_tb_static_max_tiles)";
+        case TCQ_E_BAD_FORMAT: return "unknown microscaled format (0 = mxfp4, 1 = nvfp4) or element type (0 = fp32, 1 = fp16, 2 = bf16)";
         default: return "unknown error code";
     }
 }

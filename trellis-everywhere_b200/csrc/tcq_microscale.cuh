@@ -1,0 +1,97 @@
+// Shared definitions of the 4-bit microscaled formats: geometry of their storage, and the three small types as device functions.
+//
+// A matrix of rows x k values (value = e2m1(code) * block scale [* row scale]) is held as
+//   codes      [rows][pitch] bytes, pitch = 16 * ceil(k / 32): two e2m1 codes a byte, the even column in the low half; zeros behind column k
+//   scales     [ceil(rows / 128)][atoms][32][4][4] bytes: block b of row r at [r / 128][b / 4][r % 32][r % 128 / 32][b % 4].  512 bytes are
+//              what one tcgen05.cp of 32 x 128 bits takes to tensor memory for 128 rows; atoms = 4 (nvfp4) or 2 (mxfp4) for every 256
+//              columns begun, so that a tile of 256 columns always has all its scales.  Zeros behind column k; the places of rows
+//              behind the last one are never read for a result and are left as they are.
+//   row_scale  [rows] fp32 (nvfp4), none (mxfp4)
+#pragma once
+
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+namespace tcq {
+
+enum : int { kMxfp4 = 0, kNvfp4 = 1 };
+enum : int { kF32 = 0, kF16 = 1, kBf16 = 2 };
+
+constexpr int kMsTileK = 256;                            // columns that storage and kernels count in
+
+template <int FMT> struct Ms;
+template <> struct Ms<kMxfp4> { static constexpr int kBlock = 32, kAtoms = 2; };
+template <> struct Ms<kNvfp4> { static constexpr int kBlock = 16, kAtoms = 4; };
+
+inline long long ms_pitch(long long k) { return (k + 31) / 32 * 16; }
+inline long long ms_tiles_k(long long k) { return (k + kMsTileK - 1) / kMsTileK; }
+inline int ms_atoms(int fmt) { return fmt == kNvfp4 ? 4 : 2; }
+inline long long ms_scale_bytes(long long rows, long long k, int fmt) { return (rows + 127) / 128 * ms_tiles_k(k) * ms_atoms(fmt) * 512; }
+
+// Place of the scale of block b of row r, `atoms` = atoms of a row in all.
+__device__ __forceinline__ long long ms_scale_at(long long r, int b, long long atoms) {
+    return ((r >> 7) * atoms + (b >> 2)) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4 + (b & 3);
+}
+
+// Two e2m1 codes (low half first) as fp16 pairs; every value is exact.
+__device__ __forceinline__ uint32_t e2m1x2_to_f16x2(uint32_t byte) {
+    uint32_t r;
+    asm("{\n\t.reg .b8 b;\n\tcvt.u8.u32 b, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, b;\n\t}" : "=r"(r) : "r"(byte));
+    return r;
+}
+// Nearest e2m1 codes of two values (ties to the even code, beyond 6 to 6, the sign kept); lo in the low half of the byte.
+__device__ __forceinline__ uint32_t f32x2_to_e2m1x2(float lo, float hi) {
+    uint32_t r;
+    asm("{\n\t.reg .b8 b;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %2, %1;\n\tcvt.u32.u8 %0, b;\n\t}" : "=r"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+// Nearest e4m3 of one value (ties to even, NaN to 0x7F).
+__device__ __forceinline__ uint32_t f32_to_e4m3(float v) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.0f), "f"(v));
+    return r & 0xFFu;
+}
+__device__ __forceinline__ float e4m3_to_f32(uint32_t byte) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(uint16_t(byte)));
+    return __half2float(__ushort_as_half(uint16_t(r)));
+}
+// 2^(byte - 127); 255 is NaN.  Byte 0 is a denormal number.
+__device__ __forceinline__ float e8m0_to_f32(uint32_t byte) {
+    return __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7FC00000u : byte << 23);
+}
+template <int FMT> __device__ __forceinline__ float ms_scale_to_f32(uint32_t byte) {
+    if constexpr (FMT == kNvfp4) return e4m3_to_f32(byte);
+    else return e8m0_to_f32(byte);
+}
+
+template <typename T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+// Results are rounded here and nowhere before.
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// One operand in 4 bits, as the kernels take it.
+struct MsMatrix {
+    const uint8_t* codes;
+    const uint8_t* scales;
+    const float* row_scale;      // null for mxfp4
+    long long rows;
+};
+
+int report_cuda_error(cudaError_t err, const char* where);     // tcq_capi.cu
+
+cudaError_t launch_ms_quantize(const void* x, int dtype, long long rows, long long k, long long ldx, int fmt, int rotate, const float* signs,
+                               uint8_t* codes, uint8_t* scales, float* row_scale, cudaStream_t stream);
+cudaError_t launch_ms_dequantize(const MsMatrix& q, long long k, int fmt, void* out, int dtype, long long ldo, cudaStream_t stream);
+cudaError_t launch_ms_linear(const void* x, int dtype, long long m, long long ldx, const MsMatrix& w, long long k, int fmt, void* y,
+                             long long ldy, cudaStream_t stream);
+cudaError_t launch_ms_matmul(const MsMatrix& x, const MsMatrix& w, long long k, int fmt, void* y, int dtype, long long ldy, cudaStream_t stream);
+
+}  // namespace tcq

@@ -6,4 +6,4 @@ the reference imports ``trellis.qtip`` / ``trellis.ldlq``.
 """
 from . import _lib  # noqa: F401  (importing the package does not load the .so; the first call does)
 
-__all__ = ["qtip", "ldlq", "quant", "dist"]
+__all__ = ["qtip", "ldlq", "quant", "dist", "microscale"]

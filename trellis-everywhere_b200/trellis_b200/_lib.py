@@ -13,7 +13,7 @@ import subprocess
 _CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "csrc")
 LIB_PATH = os.path.join(_CSRC, "libtcq_b200.so")
 
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 # name -> (restype, argtypes); mirrors include/tcq_b200.h one to one
 _vp, _i64, _int, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t
@@ -42,6 +42,12 @@ SIGNATURES = {
     "tcq_ip_workspace_bytes": (_sz, [_i64, _i64]),
     "tcq_ip_forward": (_int, [_vp, _i64, _i64, _vp, _vp, ctypes.c_float, _int, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "tcq_ip_restore": (_int, [_vp, _int, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "tcq_ms_code_pitch": (_sz, [_i64]),
+    "tcq_ms_scale_bytes": (_sz, [_i64, _i64, _int]),
+    "tcq_ms_quantize": (_int, [_vp, _int, _i64, _i64, _i64, _int, _int, _vp, _vp, _vp, _vp, _vp]),
+    "tcq_ms_dequantize": (_int, [_vp, _vp, _vp, _i64, _i64, _int, _vp, _int, _i64, _vp]),
+    "tcq_ms_linear": (_int, [_vp, _int, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _int, _vp, _i64, _vp]),
+    "tcq_ms_matmul": (_int, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _int, _vp, _int, _i64, _vp]),
 }
 
 _lib = None

@@ -1,0 +1,246 @@
+"""4-bit microscaled floating point: quantisation, its inverse, and products (no counterpart in the reference).
+
+The trellis codes next door (``qtip``) store a matrix in 2 to 4 bits a weight and multiply by it one token at a time.
+These formats take 4.25 or 4.5 bits a weight and are what the tensor cores multiply directly, so they also serve
+prompts and activations:
+
+    quantize(x, fmt)        a matrix -> ``Microscaled`` (codes, block scales, row scales); optionally rotated first
+    dequantize(q, dtype)    its values
+    linear(x, w)            ``x @ W.T``, x in 16 or 32 bits (weight-only)
+    matmul(x, w)            ``X @ W.T``, both in 4 bits
+
+Every value is ``e2m1(code) * block scale``, e2m1 one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign:
+
+    "mxfp4"   blocks of 32 columns, scale 2^(floor(log2 amax) - 2)
+    "nvfp4"   blocks of 16 columns, scale e4m3(amax / (6 g)), times a row scale g: the least power of two, from
+              2^-80 on, with the row's largest magnitude <= 2688 g (2688 = 6 * 448)
+
+A row scale instead of one for the whole matrix keeps the codes of a token independent of the others in its batch.
+Codes are the nearest of the exact quotients, ties to the even code, magnitudes beyond 6 to 6.  A block that holds a
+NaN or an infinity becomes all NaN (its scale is), and nothing else changes by it.
+
+All tensors live on one CUDA device; calls are queued on its current stream, nothing synchronises, and every call can
+be captured into a graph.  Nothing here has a gradient: a call that would need one is refused.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional, Tuple
+
+import torch
+
+from . import _lib
+from .qtip import _call, _cuda_device
+
+FORMATS = {"mxfp4": 0, "nvfp4": 1}
+BLOCKS = {"mxfp4": 32, "nvfp4": 16}
+ROTATIONS = (0, 16, 32, 64, 128)
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+class Microscaled(NamedTuple):
+    """A ``shape`` = (rows, k) matrix in 4 bits, as the kernels read it.
+
+    ``codes``      uint8 ``[rows, 16 * ceil(k / 32)]``: two codes a byte, the even column in the low half; zeros behind column k
+    ``scales``     uint8 ``[ceil(rows / 128), atoms, 32, 4, 4]``: block b of row r at ``[r // 128, b // 4, r % 32, r % 128 // 32, b % 4]``;
+                   atoms = 2 (mxfp4) or 4 (nvfp4) for every 256 columns begun; zeros behind column k.  The places of rows
+                   behind the last one mean nothing (``block_scales`` leaves them out)
+    ``row_scale``  fp32 ``[rows]`` for nvfp4, None for mxfp4
+
+    A checkpoint's own codes and scales can be put in this form too (``from_blocks``); any positive row scales go with them.
+    """
+    codes: torch.Tensor
+    scales: torch.Tensor
+    row_scale: Optional[torch.Tensor]
+    shape: Tuple[int, int]
+    fmt: str
+
+
+def _storage(rows: int, k: int, fmt: str):
+    """Shapes of codes and scales."""
+    return (rows, 16 * -(-k // 32)), (-(-rows // 128), (4 if fmt == "nvfp4" else 2) * -(-k // 256), 32, 4, 4)
+
+
+def _check_fmt(fmt: str) -> int:
+    if fmt not in FORMATS:
+        raise ValueError(f"unknown microscaled format {fmt!r}; expected one of {sorted(FORMATS)}")
+    return FORMATS[fmt]
+
+
+def _check_dtype(dtype) -> int:
+    if dtype not in _DTYPES:
+        raise ValueError(f"float32, float16 or bfloat16 expected, not {dtype}")
+    return _DTYPES[dtype]
+
+
+def _check_q(q: Microscaled, name: str) -> torch.device:
+    """The device of a well-formed matrix; raises otherwise (the kernels trust its sizes)."""
+    if not isinstance(q, Microscaled):
+        raise ValueError(f"{name} must be a Microscaled matrix, got {type(q).__name__}")
+    _check_fmt(q.fmt)
+    rows, k = q.shape
+    codes, scales = _storage(rows, k, q.fmt)
+    dev = q.codes.device
+    for part, t, shape, dtype in (("codes", q.codes, codes, torch.uint8), ("scales", q.scales, scales, torch.uint8),
+                                  ("row_scale", q.row_scale, (rows,), torch.float32)):
+        if part == "row_scale" and q.fmt == "mxfp4":
+            if t is not None:
+                raise ValueError(f"{name}: mxfp4 has no row scales")
+            continue
+        if t is None or t.dtype != dtype or tuple(t.shape) != shape or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"{name}.{part} must be a contiguous {dtype} {list(shape)} tensor on {dev}")
+    if dev.type != "cuda":
+        _cuda_device()
+        raise ValueError(f"{name} must be on a CUDA device")
+    return dev
+
+
+def _check_x(x: torch.Tensor, name: str) -> Tuple[torch.Tensor, int]:
+    """A 2-d CUDA matrix with unit column stride, and its type's number."""
+    dt = _check_dtype(x.dtype)
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise ValueError(f"no gradient is defined here: detach {name} or call under torch.no_grad()")
+    if not x.is_cuda:
+        _cuda_device()
+        raise ValueError(f"{name} must be on a CUDA device")
+    if x.stride(-1) != 1 and x.shape[-1] > 1:
+        x = x.contiguous()
+    if x.shape[0] > 1 and x.stride(0) < x.shape[1]:          # rows that repeat or overlap (an expanded tensor)
+        x = x.contiguous()
+    return x, dt
+
+
+def _pitch(x: torch.Tensor) -> int:
+    return x.stride(0) if x.shape[0] > 1 else max(x.shape[1], 1)
+
+
+@torch.no_grad()
+def _quantize(x: torch.Tensor, dt: int, fmt: str, rotate: int, signs: Optional[torch.Tensor]) -> Microscaled:
+    rows, k = x.shape
+    codes_shape, scales_shape = _storage(rows, k, fmt)
+    dev = x.device
+    codes = torch.empty(codes_shape, dtype=torch.uint8, device=dev)
+    scales = torch.empty(scales_shape, dtype=torch.uint8, device=dev)
+    row = torch.empty(rows, dtype=torch.float32, device=dev) if fmt == "nvfp4" else None
+    if rows and k:
+        _call(dev, "tcq_ms_quantize", x.data_ptr(), dt, rows, k, _pitch(x), FORMATS[fmt], rotate,
+              signs.data_ptr() if signs is not None else None, codes.data_ptr(), scales.data_ptr(),
+              row.data_ptr() if row is not None else None)
+    elif row is not None:
+        row.fill_(1.0)                                       # rows without columns
+    return Microscaled(codes, scales, row, (rows, k), fmt)
+
+
+def quantize(x: torch.Tensor, fmt: str = "nvfp4", rotate: int = 0, signs: Optional[torch.Tensor] = None) -> Microscaled:
+    """``x [rows, k]`` (fp32, fp16 or bf16; any row stride) to 4 bits.
+
+    ``rotate`` = 16, 32, 64 or 128 (dividing k) first multiplies the columns by ``signs [k]`` (fp32) and transforms every
+    ``rotate`` of them by the orthonormal Hadamard matrix, in fp32 within the same kernel: incoherence processing of the input
+    axis (``qtip.block_hadamard``).  A product of two matrices rotated alike is the product of the matrices, and outliers
+    no longer set the scales.
+    """
+    _check_fmt(fmt)
+    if x.dim() != 2:
+        raise ValueError(f"expected a matrix, got {tuple(x.shape)}")
+    if rotate not in ROTATIONS or (rotate and x.shape[1] % rotate):
+        raise ValueError(f"rotate={rotate} must be one of {ROTATIONS} and divide the {x.shape[1]} columns")
+    if (signs is not None) != bool(rotate):
+        raise ValueError("signs go with rotate: give both or neither")
+    x, dt = _check_x(x, "x")
+    if signs is not None and (signs.dtype != torch.float32 or tuple(signs.shape) != (x.shape[1],) or signs.device != x.device
+                              or not signs.is_contiguous()):
+        raise ValueError(f"signs must be a contiguous float32 [{x.shape[1]}] tensor on {x.device}")
+    return _quantize(x, dt, fmt, rotate, signs)
+
+
+@torch.no_grad()
+def dequantize(q: Microscaled, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The ``[rows, k]`` values.  Of a matrix quantised here they are exact in fp32, and in bf16 as well; fp16 rounds those out of its range."""
+    dev, dt = _check_q(q, "q"), _check_dtype(dtype)
+    rows, k = q.shape
+    out = torch.empty((rows, k), dtype=dtype, device=dev)
+    if rows and k:
+        _call(dev, "tcq_ms_dequantize", *_parts(q), rows, k, FORMATS[q.fmt], out.data_ptr(), dt, k)
+    return out
+
+
+def _parts(q: Microscaled):
+    return q.codes.data_ptr(), q.scales.data_ptr(), q.row_scale.data_ptr() if q.row_scale is not None else None
+
+
+def linear(x: torch.Tensor, w: Microscaled) -> torch.Tensor:
+    """``x @ W.T``: ``x [..., k]`` (fp32, fp16 or bf16) times a 4-bit ``[n, k]`` matrix -> ``[..., n]`` of x's type.
+
+    Products with the weights' exact values, summed in fp32, rounded once.  A row of the result does not depend on what
+    the other rows of x hold, and equal calls give equal results.
+    """
+    dev = _check_q(w, "w")
+    n, k = w.shape
+    if x.dim() < 1 or x.shape[-1] != k:
+        raise ValueError(f"x must be [..., {k}], got {tuple(x.shape)}")
+    if x.device != dev:
+        raise ValueError(f"x must be on {dev}")
+    if not k:
+        _check_dtype(x.dtype)
+        return torch.zeros((*x.shape[:-1], n), dtype=x.dtype, device=dev)
+    flat, dt = _check_x(x.reshape(-1, k), "x")
+    return _linear(flat, dt, w).reshape(*x.shape[:-1], n)
+
+
+@torch.no_grad()
+def _linear(x: torch.Tensor, dt: int, w: Microscaled) -> torch.Tensor:
+    n, k = w.shape
+    y = torch.empty((x.shape[0], n), dtype=x.dtype, device=x.device)
+    if x.shape[0] and n:
+        _call(x.device, "tcq_ms_linear", x.data_ptr(), dt, x.shape[0], _pitch(x), *_parts(w), n, k, FORMATS[w.fmt], y.data_ptr(), n)
+    return y
+
+
+@torch.no_grad()
+def matmul(x: Microscaled, w: Microscaled, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``X @ W.T`` of two 4-bit matrices ``[m, k]`` and ``[n, k]`` of one format -> ``[m, n]`` of ``dtype``, summed in fp32, rounded once."""
+    dev, dt = _check_q(w, "w"), _check_dtype(dtype)
+    if _check_q(x, "x") != dev or x.fmt != w.fmt or x.shape[1] != w.shape[1]:
+        raise ValueError(f"x and w must have one format, device and number of columns: {x.fmt} {x.shape} on {x.codes.device}, "
+                         f"{w.fmt} {w.shape} on {dev}")
+    (m, k), n = x.shape, w.shape[0]
+    if not k:
+        return torch.zeros((m, n), dtype=dtype, device=dev)
+    y = torch.empty((m, n), dtype=dtype, device=dev)
+    if m and n:
+        _call(dev, "tcq_ms_matmul", *_parts(x), m, *_parts(w), n, k, FORMATS[w.fmt], y.data_ptr(), dt, n)
+    return y
+
+
+def block_scales(q: Microscaled) -> torch.Tensor:
+    """The scale bytes by row and block, uint8 ``[rows, ceil(k / block)]`` (e4m3 for nvfp4, exponents + 127 for mxfp4)."""
+    rows, k = q.shape
+    s = q.scales.permute(0, 3, 2, 1, 4).reshape(q.scales.shape[0] * 128, -1)
+    return s[:rows, :-(-k // BLOCKS[q.fmt])].contiguous()
+
+
+def from_blocks(codes: torch.Tensor, scales: torch.Tensor, row_scale: Optional[torch.Tensor], k: int, fmt: str) -> Microscaled:
+    """A matrix from row-major codes ``[rows, >= ceil(k / 2)]`` and scale bytes ``[rows, ceil(k / block)]``, as other programs store them.
+
+    ``row_scale``: fp32 ``[rows]`` or one number for all rows (nvfp4), None (mxfp4).  Done once per matrix, with torch.
+    """
+    _check_fmt(fmt)
+    if codes.dim() != 2 or scales.dim() != 2 or codes.dtype != torch.uint8 or codes.shape[1] < -(-k // 2) or k < 0:
+        raise ValueError(f"expected uint8 codes [rows, >= {-(-k // 2)}], got {codes.dtype} {tuple(codes.shape)}")
+    rows, nb = codes.shape[0], -(-k // BLOCKS[fmt])
+    if tuple(scales.shape) != (rows, nb) or scales.element_size() != 1:
+        raise ValueError(f"expected one-byte scales [{rows}, {nb}], got {scales.dtype} {tuple(scales.shape)}")
+    if (row_scale is None) != (fmt == "mxfp4"):
+        raise ValueError("row scales go with nvfp4, and only with it")
+    codes_shape, scales_shape = _storage(rows, k, fmt)
+    dev = codes.device
+    c = torch.zeros(codes_shape, dtype=torch.uint8, device=dev)
+    c[:, :-(-k // 2)] = codes[:, :-(-k // 2)]
+    if k % 2:
+        c[:, k // 2] &= 15                                   # the half behind the last column
+    full = torch.zeros((scales_shape[0] * 128, scales_shape[1] * 4), dtype=torch.uint8, device=dev)
+    full[:rows, :nb] = scales.to(dev).view(torch.uint8)
+    tiled = full.reshape(scales_shape[0], 4, 32, scales_shape[1], 4).permute(0, 3, 2, 1, 4).contiguous()
+    row = None
+    if row_scale is not None:
+        row = torch.as_tensor(row_scale, dtype=torch.float32, device=dev).expand(rows).contiguous()
+    return Microscaled(c, tiled, row, (rows, k), fmt)

@@ -2,7 +2,9 @@
 
 The reference's model-level drivers walk ``nn.Linear`` modules and call
 ``Quantizer.quantize_weight(w) -> w_fake``; ``TrellisQuantizer`` is that interface
-on top of the CUDA encoder, with or without LDLQ feedback.
+on top of the CUDA encoder, with or without LDLQ feedback.  ``MicroscaleQuantizer`` is the
+same for the 4-bit microscaled formats, and ``MicroscaledLinear`` / ``apply_microscaled`` keep
+the weights in 4 bits and multiply by them there (no counterpart in the reference).
 """
 from __future__ import annotations
 
@@ -12,8 +14,9 @@ from typing import Callable, Optional
 import torch
 import torch.nn as nn
 
+from . import microscale
 from .ldlq import tcq_quantize_weight_ldlq
-from .qtip import CodebookLike, tcq_quantize_weight
+from .qtip import CodebookLike, _cuda_device, block_hadamard, tcq_quantize_weight
 
 
 class Quantizer:
@@ -45,6 +48,81 @@ class TrellisQuantizer(Quantizer):
         return tcq_quantize_weight_ldlq(w, self.K, self.codebook, H, seed=s, sigma_reg=self.sigma_reg, backend="b200")
 
 
+def _signs(k: int, seed: int, device) -> torch.Tensor:
+    """+-1 for every input channel, from the CPU generator (as ``qtip.IPContext`` draws its signs)."""
+    gen = torch.Generator(device="cpu").manual_seed(seed)
+    return torch.empty(k, dtype=torch.float32).random_(0, 2, generator=gen).mul_(2).sub_(1).to(device)
+
+
+class MicroscaleQuantizer(Quantizer):
+    """4-bit microscaled floating point (``microscale.quantize``), optionally in a rotated space of the input channels.
+
+    ``rotate`` (16 to 128, dividing the matrix's input channels; 0: none) applies seeded signs and a block Hadamard
+    transform before the quantisation and takes them back after it.
+    """
+
+    def __init__(self, fmt: str = "nvfp4", rotate: int = 0, seed: int = 0):
+        if fmt not in microscale.FORMATS:
+            raise ValueError(f"unknown microscaled format {fmt!r}; expected one of {sorted(microscale.FORMATS)}")
+        if rotate not in microscale.ROTATIONS:
+            raise ValueError(f"rotate={rotate} must be one of {microscale.ROTATIONS}")
+        self.fmt, self.rotate, self.seed = fmt, rotate, seed
+        self.name = f"{fmt}-b200" + (f"-h{rotate}" if rotate else "")
+        self.bpw = 4.0 + 8.0 / microscale.BLOCKS[fmt]
+
+    @torch.no_grad()
+    def quantize_weight(self, w: torch.Tensor, seed: Optional[int] = None) -> torch.Tensor:
+        wd = w.to(_cuda_device(w))
+        if not self.rotate:
+            back = microscale.dequantize(microscale.quantize(wd, self.fmt), w.dtype)
+        else:
+            signs = _signs(w.shape[1], self.seed if seed is None else seed, wd.device)
+            z = microscale.dequantize(microscale.quantize(wd, self.fmt, self.rotate, signs))
+            back = block_hadamard(z, 1, self.rotate) * signs
+        return back.to(dtype=w.dtype, device=w.device)
+
+
+class MicroscaledLinear(nn.Module):
+    """``nn.Linear`` for inference with its weight in 4 bits.
+
+    ``activations=16``: inputs stay as they are (``microscale.linear``).  ``activations=4``: inputs are quantised token by
+    token (``microscale.quantize``) and both sides multiplied in 4 bits (``microscale.matmul``); ``rotate`` then puts both
+    sides in a rotated space of the input channels, which leaves the product what it is.
+    """
+
+    def __init__(self, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, fmt: str = "nvfp4", activations: int = 16,
+                 rotate: int = 0, seed: int = 0):
+        super().__init__()
+        if activations not in (4, 16):
+            raise ValueError("activations must be 4 or 16")
+        if rotate and activations == 16:
+            raise ValueError("rotate needs activations=4: inputs are rotated as they are quantised")
+        self.fmt, self.activations, self.rotate = fmt, activations, rotate
+        self.out_features, self.in_features = weight.shape
+        wd = weight.detach().to(_cuda_device(weight))
+        signs = _signs(self.in_features, seed, wd.device) if rotate else None
+        q = microscale.quantize(wd, fmt, rotate, signs)
+        for name, t in (("codes", q.codes), ("scales", q.scales), ("row_scale", q.row_scale), ("signs", signs),
+                        ("bias", None if bias is None else bias.detach().to(wd.device))):
+            self.register_buffer(name, t)
+
+    @property
+    def weight(self) -> "microscale.Microscaled":
+        return microscale.Microscaled(self.codes, self.scales, self.row_scale, (self.out_features, self.in_features), self.fmt)
+
+    @torch.no_grad()
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if self.activations == 16:
+            y = microscale.linear(x, self.weight)
+        else:
+            q = microscale.quantize(x.reshape(-1, self.in_features), self.fmt, self.rotate, self.signs)
+            y = microscale.matmul(q, self.weight, x.dtype).reshape(*x.shape[:-1], self.out_features)
+        return y if self.bias is None else y + self.bias.to(y.dtype)
+
+    def extra_repr(self) -> str:
+        return f"{self.in_features} -> {self.out_features}, {self.fmt}, activations={self.activations}, rotate={self.rotate}"
+
+
 def seed_from_name(name: str) -> int:
     """Per-matrix seed of the reference driver (``zlib.crc32(name)``, run_tcq_eval.py:115)."""
     return zlib.crc32(name.encode())
@@ -59,3 +137,15 @@ def apply_fake_quant(model: nn.Module, quantizer: Quantizer, skip: Callable[[str
             mod.weight.data = quantizer.quantize_weight(mod.weight.data).to(mod.weight.dtype)
             count += 1
     return count
+
+
+@torch.no_grad()
+def apply_microscaled(model: nn.Module, fmt: str = "nvfp4", activations: int = 16, rotate: int = 0,
+                      skip: Callable[[str], bool] = lambda n: False) -> int:
+    """Replace every ``nn.Linear`` by a ``MicroscaledLinear`` (seeds by name, as ``seed_from_name``). Returns the count."""
+    found = [(name, mod) for name, mod in model.named_modules() if isinstance(mod, nn.Linear) and name and not skip(name)]
+    for name, mod in found:
+        parent, _, leaf = name.rpartition(".")
+        setattr(model.get_submodule(parent), leaf,
+                MicroscaledLinear(mod.weight.data, mod.bias, fmt, activations, rotate, seed_from_name(name)))
+    return len(found)
