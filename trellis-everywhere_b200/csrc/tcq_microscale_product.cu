@@ -103,12 +103,4 @@ cudaError_t launch_ms_linear(const void* x, int dtype, long long m, long long ld
     }
 }
 
-cudaError_t launch_ms_matmul(const MsMatrix& x, const MsMatrix& w, long long k, int fmt, void* y, int dtype, long long ldy, cudaStream_t stream) {
-    switch (dtype) {
-        case kF32: return launch_product<void, float>(nullptr, 0, x.rows, x, w, k, fmt, y, ldy, stream);
-        case kF16: return launch_product<void, __half>(nullptr, 0, x.rows, x, w, k, fmt, y, ldy, stream);
-        default: return launch_product<void, __nv_bfloat16>(nullptr, 0, x.rows, x, w, k, fmt, y, ldy, stream);
-    }
-}
-
 }  // namespace tcq
