@@ -40,6 +40,13 @@ struct Tile {
     static_assert(kSmem > 114 * 1024 && kSmem <= 226 * 1024 && kStages >= 3);
 };
 
+}  // namespace
+
+// tcq_microscale_pair.cu: tiles of 256 tokens x nt rows of W on pairs of SMs.
+cudaError_t launch_ms_matmul_pair(const MsMatrix& x, const MsMatrix& w, long long k, int fmt, void* y, int dtype, long long ldy, int nt, int sms, cudaStream_t stream);
+
+namespace {
+
 struct MatmulArgs {
     const uint8_t* a_scales;
     const uint8_t* b_scales;
@@ -279,7 +286,7 @@ cudaError_t launch_fmt(const MsMatrix& x, const MsMatrix& w, long long k, void* 
         return launch<FMT, 64>(w, x, false, k, y, dtype, ldy, splits, stream);
     }
     const long long ta = (m + kRowsA - 1) / kRowsA;
-    if (ta * ((w.rows + 255) / 256) >= sm_count()) return launch<FMT, 256>(x, w, true, k, y, dtype, ldy, 1, stream);
+    if (m > 128) return launch_ms_matmul_pair(x, w, k, FMT, y, dtype, ldy, (m + 255) / 256 * ((w.rows + 255) / 256) * 2 >= sm_count() ? 256 : 128, sm_count(), stream);
     const long long tiles = ta * ((w.rows + 127) / 128);
     int splits = 1;
     while (splits < 8 && tiles * splits * 2 <= sm_count() && splits * 2 <= ms_tiles_k(k)) splits *= 2;
@@ -288,7 +295,9 @@ cudaError_t launch_fmt(const MsMatrix& x, const MsMatrix& w, long long k, void* 
 
 }  // namespace
 
-cudaError_t make_byte_map(CUtensorMap* map, const void* base, long long width, long long rows, long long pitch, int box_rows) {
+namespace {
+cudaError_t encode_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, cuuint64_t width, cuuint64_t rows, cuuint64_t pitch, cuuint32_t box_width,
+                       cuuint32_t box_rows, CUtensorMapSwizzle swizzle) {
     using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                                 CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
     static Encode encode = nullptr;
@@ -300,11 +309,20 @@ cudaError_t make_byte_map(CUtensorMap* map, const void* base, long long width, l
         if (found != cudaDriverEntryPointSuccess || fn == nullptr) return cudaErrorNotSupported;
         encode = reinterpret_cast<Encode>(fn);
     }
-    const cuuint64_t dims[2] = {cuuint64_t(width), cuuint64_t(rows)}, strides[1] = {cuuint64_t(pitch)};
-    const cuuint32_t box[2] = {128, cuuint32_t(box_rows)}, steps[2] = {1, 1};
-    const CUresult rc = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const cuuint64_t dims[2] = {width, rows}, strides[1] = {pitch};
+    const cuuint32_t box[2] = {box_width, box_rows}, steps[2] = {1, 1};
+    const CUresult rc = encode(map, type, 2, const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return rc == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+}  // namespace
+
+cudaError_t make_byte_map(CUtensorMap* map, const void* base, long long width, long long rows, long long pitch, int box_rows) {
+    return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, width, rows, pitch, 128, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+cudaError_t make_scale_map(CUtensorMap* map, const void* base, long long rows, int box_rows) {
+    return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, base, 128, rows, 512, 128, box_rows, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 cudaError_t launch_ms_matmul(const MsMatrix& x, const MsMatrix& w, long long k, int fmt, void* y, int dtype, long long ldy, cudaStream_t stream) {

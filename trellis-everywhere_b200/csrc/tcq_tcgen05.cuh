@@ -19,13 +19,21 @@ __device__ __forceinline__ uint64_t desc_rows16(uint32_t smem) {
     return uint64_t((smem & 0x3FFFFu) >> 4) | uint64_t(128 >> 4) << 32 | uint64_t(1) << 46;
 }
 
-// ---- tensor memory
+// ---- tensor memory.  CTAS = 2: the form for a pair of CTAs on neighbouring SMs (ranks 2i and 2i + 1 of a cluster); a kernel uses one form only.
+template <int CTAS = 1>
 __device__ __forceinline__ void tmem_alloc(uint32_t smem_to, uint32_t columns) {       // a whole warp
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_to), "r"(columns) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    if constexpr (CTAS == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_to), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_to), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
 }
+template <int CTAS = 1>
 __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t columns) {           // the same warp
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns));
+    if constexpr (CTAS == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns));
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns));
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -34,9 +42,16 @@ __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.
 __device__ __forceinline__ void tc_commit(uint32_t mbar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(mbar) : "memory");
 }
+// The pair's form: one arrival at the barrier of this place in both CTAs.
+__device__ __forceinline__ void tc_commit_pair(uint32_t mbar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(mbar), "h"(uint16_t(3)) : "memory");
+}
 // 512 bytes (32 rows of 16) to four columns of lanes 0-31, and again to the other three quarters of the lanes.
+// (pair: each CTA's own bytes to its own columns, asked for by the first CTA alone)
+template <int CTAS = 1>
 __device__ __forceinline__ void tc_copy_scales(uint32_t tmem, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+    if constexpr (CTAS == 1) asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+    else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
 }
 // N consecutive columns of this warp's 32 lanes.
 template <int N> __device__ __forceinline__ void tmem_load(uint32_t tmem, uint32_t (&v)[N]);
@@ -63,6 +78,11 @@ __device__ __forceinline__ void tma_load(uint32_t smem, const CUtensorMap* map, 
     asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                  ::"r"(smem), "l"(map), "r"(x), "r"(y), "r"(mbar) : "memory");
 }
+// To this CTA's memory, counted by a barrier of the pair's first CTA (a shared::cluster address).
+__device__ __forceinline__ void tma_load_pair(uint32_t smem, const CUtensorMap* map, int x, int y, uint32_t mbar) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(smem), "l"(map), "r"(x), "r"(y), "r"(mbar) : "memory");
+}
 __device__ __forceinline__ void bulk_load(uint32_t smem, const void* from, uint32_t bytes, uint32_t mbar) {
     asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(smem), "l"(from), "r"(bytes), "r"(mbar) : "memory");
@@ -74,6 +94,15 @@ __device__ __forceinline__ uint32_t cluster_size() { uint32_t r; asm volatile("m
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The address of this place in another CTA of the cluster.
+__device__ __forceinline__ uint32_t map_rank(uint32_t smem, uint32_t rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 __device__ __forceinline__ float ld_cluster_f32(uint32_t smem, uint32_t rank) {
     float v;
     asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}" : "=f"(v) : "r"(smem), "r"(rank) : "memory");
@@ -82,5 +111,8 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t smem, uint32_t rank) {
 
 // A map of [rows][width] bytes, `pitch` bytes a row (a multiple of 16), cut into boxes of [box_rows][128 bytes] in the 128-byte swizzle.
 cudaError_t make_byte_map(CUtensorMap* map, const void* base, long long width, long long rows, long long pitch, int box_rows);
+
+// A map of scales as rows of 512 bytes, cut into boxes of `box_rows` of them, one behind the other.
+cudaError_t make_scale_map(CUtensorMap* map, const void* base, long long rows, int box_rows);
 
 }  // namespace tcq
