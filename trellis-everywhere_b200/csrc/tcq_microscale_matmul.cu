@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_matmul_kernel(const __grid
     __shared__ uint32_t tmem_at;
     __shared__ unsigned int gave_up;
     const uint32_t smem = (smem_u32(raw) + 1023) & ~1023u;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xFFFFFFFFu, int(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank(), splits = cluster_size();
     const int first = int((long long)p.k_tiles * rank / splits), last = int((long long)p.k_tiles * (rank + 1) / splits);
     const int tiles = p.tiles_a * p.tiles_b, clusters = gridDim.x / splits;
@@ -105,70 +105,92 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_matmul_kernel(const __grid
     const uint32_t tmem = tmem_at, tmem_scales = tmem + T::kSumBuffers * T::kSumColumns;
     const long long atoms = (long long)p.k_tiles * T::kAtoms;
 
-    if (warp == 0 && lane == 0) {
-        // ---- loads
-        long long it = 0;
+    if (warp == 0) {
+        // ---- loads; the warp stays together, one lane issues
+        const bool one = elect_one();
+        uint32_t s = 0, phase = 1, loaded = 0;           // (the first wait for each stage is for the phase before the first)
         bool ok = true;
         const long long groups_b = (p.b_rows + 127) / 128;
         for (int t = blockIdx.x / splits; t < tiles && ok; t += clusters) {
             const int ta = t / p.tiles_b, tb = t % p.tiles_b;
-            for (int kt = first; kt < last; ++kt, ++it) {
-                const int s = int(it % T::kStages);
-                if (it >= T::kStages && !(ok = mbar_wait(smem_u32(&empty[s]), uint32_t(it / T::kStages - 1) & 1, &gave_up))) break;
-                const uint32_t to = smem + s * T::kStageBytes, bar = smem_u32(&full[s]);
-                mbar_expect(bar, T::kBytesA + T::kBytesB + T::kBytesSa + T::kBytesSb);
-                tma_load(to, &map_a, kt * 128, ta * kRowsA, bar);
-                tma_load(to + T::kBytesA, &map_b, kt * 128, tb * NT, bar);
-                bulk_load(to + T::kBytesA + T::kBytesB, p.a_scales + (ta * atoms + kt * T::kAtoms) * 512, T::kBytesSa, bar);
+            const uint8_t* const from_a = p.a_scales + ta * atoms * 512;
+            const uint8_t* from_b[T::kGroups];
 #pragma unroll
-                for (int g = 0; g < T::kGroups; ++g) {
-                    const long long group = (long long)tb * NT / 128 + g;             // one behind the last only has rows without results
-                    bulk_load(to + T::kBytesA + T::kBytesB + T::kBytesSa + g * T::kAtoms * 512,
-                              p.b_scales + ((group < groups_b ? group : groups_b - 1) * atoms + kt * T::kAtoms) * 512, T::kAtoms * 512, bar);
+            for (int g = 0; g < T::kGroups; ++g) {
+                const long long group = (long long)tb * NT / 128 + g;             // one behind the last only has rows without results
+                from_b[g] = p.b_scales + (group < groups_b ? group : groups_b - 1) * atoms * 512;
+            }
+            for (int kt = first; kt < last; ++kt) {
+                ok = mbar_wait(smem_u32(&empty[s]), phase, &gave_up);
+                ok = __all_sync(0xFFFFFFFFu, ok);        // every lane has seen this phase before the next can begin
+                if (!ok) break;
+                if (one) {
+                    const uint32_t to = smem + s * T::kStageBytes, bar = smem_u32(&full[s]);
+                    mbar_expect(bar, T::kBytesA + T::kBytesB + T::kBytesSa + T::kBytesSb);
+                    tma_load(to, &map_a, kt * 128, ta * kRowsA, bar);
+                    tma_load(to + T::kBytesA, &map_b, kt * 128, tb * NT, bar);
+                    bulk_load(to + T::kBytesA + T::kBytesB, from_a + (long long)kt * T::kBytesSa, T::kBytesSa, bar);
+#pragma unroll
+                    for (int g = 0; g < T::kGroups; ++g)
+                        bulk_load(to + T::kBytesA + T::kBytesB + T::kBytesSa + g * T::kAtoms * 512, from_b[g] + (long long)kt * T::kAtoms * 512, T::kAtoms * 512, bar);
                 }
+                __syncwarp();
+                if (++s == T::kStages) { s = 0; phase ^= 1; }
+                if (loaded < T::kStages) ++loaded;
             }
         }
-        // nothing may be on its way to this CTA's shared memory when it ends: after a failure nobody else has waited for these
-        if (gave_up)
-            for (long long i = it > T::kStages ? it - T::kStages : 0; i < it; ++i)
-                for (long long t0 = clock64(); !mbar_try_wait(smem_u32(&full[i % T::kStages]), uint32_t(i / T::kStages) & 1) && clock64() - t0 < kMbarWaitCycles;) {}
-    } else if (warp == 1 && lane == 0) {
-        // ---- products
+        if (gave_up)                                     // nothing may be on its way to this CTA's memory when it ends: the last loads of each stage
+            for (uint32_t i = 0; i < loaded; ++i) {
+                if (s == 0) phase ^= 1;
+                s = s == 0 ? T::kStages - 1 : s - 1;
+                for (long long t0 = clock64(); !mbar_try_wait(smem_u32(&full[s]), phase ^ 1) && clock64() - t0 < kMbarWaitCycles;) {}
+            }
+    } else if (warp == 1) {
+        // ---- products; likewise
         constexpr uint32_t kIdesc = 1u << 7 | 1u << 10 | uint32_t(NT >> 3) << 17 | (FMT == kMxfp4 ? 1u : 0u) << 23 | 1u << 27;
-        long long it = 0;
+        const bool one = elect_one();
+        uint32_t s = 0, phase = 0;
         int n = 0;
         bool ok = true;
         for (int t = blockIdx.x / splits; t < tiles && ok; t += clusters, ++n) {
             const int buf = n % T::kSumBuffers, use = n / T::kSumBuffers;
-            if (use > 0 && !(ok = mbar_wait(smem_u32(&sum_empty[buf]), uint32_t(use - 1) & 1, &gave_up))) break;
+            if (use > 0) ok = mbar_wait(smem_u32(&sum_empty[buf]), uint32_t(use - 1) & 1, &gave_up);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) break;
             tc_fence_after();
             const uint32_t d = tmem + buf * T::kSumColumns;
-            for (int kt = first; kt < last; ++kt, ++it) {
-                const int s = int(it % T::kStages);
-                if (!(ok = mbar_wait(smem_u32(&full[s]), uint32_t(it / T::kStages) & 1, &gave_up))) break;
+            for (int kt = first; kt < last; ++kt) {
+                ok = mbar_wait(smem_u32(&full[s]), phase, &gave_up);
+                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (!ok) break;
                 tc_fence_after();
                 const uint32_t at = smem + s * T::kStageBytes, sa = tmem_scales + s * T::kScaleColumns, sb = sa + T::kAtoms * 4;
-                const uint32_t from = at + T::kBytesA + T::kBytesB;
+                const uint64_t da = desc_rows128(at), db = desc_rows128(at + T::kBytesA), ds = desc_rows16(at + T::kBytesA + T::kBytesB);
+                if (one) {
 #pragma unroll
-                for (int j = 0; j < T::kAtoms; ++j) {
-                    tc_copy_scales(sa + 4 * j, desc_rows16(from + 512 * j));
+                    for (int j = 0; j < T::kAtoms; ++j) {
+                        tc_copy_scales(sa + 4 * j, ds + 32 * j);
 #pragma unroll
-                    for (int g = 0; g < T::kGroups; ++g)
-                        tc_copy_scales(sb + 4 * (j * T::kGroups + g), desc_rows16(from + T::kBytesSa + 512 * (g * T::kAtoms + j)));
+                        for (int g = 0; g < T::kGroups; ++g)
+                            tc_copy_scales(sb + 4 * (j * T::kGroups + g), ds + (T::kBytesSa >> 4) + 32 * (g * T::kAtoms + j));
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {            // 64 columns: 32 bytes of a row, one word of scales (nvfp4) or half a word (mxfp4)
+                        const int atom = FMT == kNvfp4 ? j : j / 2;
+                        const uint32_t id = FMT == kNvfp4 ? 0u : 2u * (j % 2);
+                        mma_block_scaled<FMT>(d, da + 2 * j, db + 2 * j, kIdesc | id << 4 | id << 29, sa + 4 * atom, sb + 4 * T::kGroups * atom, kt > first || j > 0);
+                    }
+                    tc_commit(smem_u32(&empty[s]));
                 }
-                const uint64_t da = desc_rows128(at), db = desc_rows128(at + T::kBytesA);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {                // 64 columns: 32 bytes of a row, one word of scales (nvfp4) or half a word (mxfp4)
-                    const int atom = FMT == kNvfp4 ? j : j / 2;
-                    const uint32_t id = FMT == kNvfp4 ? 0u : 2u * (j % 2);
-                    mma_block_scaled<FMT>(d, da + 2 * j, db + 2 * j, kIdesc | id << 4 | id << 29, sa + 4 * atom, sb + 4 * T::kGroups * atom, kt > first || j > 0);
-                }
-                tc_commit(smem_u32(&empty[s]));
+                __syncwarp();
+                if (++s == T::kStages) { s = 0; phase ^= 1; }
             }
-            if (ok) tc_commit(smem_u32(&sum_full[buf]));
+            if (ok && one) tc_commit(smem_u32(&sum_full[buf]));
+            __syncwarp();
         }
         if (!ok) {                                           // what was issued ends before the tensor memory goes
-            tc_commit(smem_u32(&drained));
+            if (one) tc_commit(smem_u32(&drained));
+            __syncwarp();
             for (long long t0 = clock64(); !mbar_try_wait(smem_u32(&drained), 0) && clock64() - t0 < kMbarWaitCycles;) {}
         }
     } else if (warp >= 2) {

@@ -75,55 +75,63 @@ __device__ __forceinline__ void store32(void* to, const uint32_t* v) {       // 
                  ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
 
-// 32 tokens (one a lane) x COLS columns out of tensor memory: scaled, rounded, the tensor memory handed back, stored.
+// What 32 tokens (one a lane) x COLS columns of results are scaled by; fetched while the products run.
+template <int FMT, int COLS>
+struct Factors {
+    float x, w[FMT == kNvfp4 ? COLS / 32 : 1];           // w: of column 32 q + lane
+    __device__ __forceinline__ Factors(const PairArgs& p, long long token0, long long col0) {
+        if constexpr (FMT == kNvfp4) {
+            const int lane = threadIdx.x & 31;
+            x = token0 + lane < p.m ? __ldg(p.x_row + token0 + lane) : 1.0f;
+#pragma unroll
+            for (int q = 0; q < COLS / 32; ++q) w[q] = col0 + 32 * q + lane < p.n ? __ldg(p.w_row + col0 + 32 * q + lane) : 1.0f;
+        }
+    }
+};
+
+// 32 tokens x COLS columns out of tensor memory, which is handed back at once; then scaled, rounded and stored.
 template <typename YT, int FMT, int COLS>
-__device__ __forceinline__ void results(const PairArgs& p, uint32_t tmem, uint32_t sum_empty, bool ok, long long token0, long long col0, uint32_t* turn) {
+__device__ __forceinline__ void results(const PairArgs& p, uint32_t tmem, uint32_t sum_empty, bool ok, long long token0, long long col0,
+                                        const Factors<FMT, COLS>& by, uint32_t* turn) {
     constexpr int kWords = sizeof(YT) == 4 ? 32 : 16;     // of 32 results
     const int lane = threadIdx.x & 31;
     const long long token = token0 + lane;
-    const float fx = FMT == kNvfp4 && token < p.m ? __ldg(p.x_row + token) : 1.0f;
-    uint32_t out[COLS / 32][kWords];
+    uint32_t v[COLS / 32][32];
 #pragma unroll
-    for (int q = 0; q < COLS / 32; ++q) {
-        uint32_t v[32];
-        tmem_load<32>(tmem + 32 * q, v);
-        const long long c = col0 + 32 * q + lane;
-        const float fw = FMT == kNvfp4 && c < p.n ? __ldg(p.w_row + c) : 1.0f;
-        tmem_wait_ld();
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            if constexpr (FMT == kNvfp4) v[i] = __float_as_uint(__uint_as_float(v[i]) * fx * __shfl_sync(0xFFFFFFFFu, fw, i));
-            if (!ok) v[i] = 0x7FC00000u;
-        }
-        if constexpr (sizeof(YT) == 4) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) out[q][i] = v[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) out[q][i] = pack<YT>(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-        }
-    }
+    for (int q = 0; q < COLS / 32; ++q) tmem_load<32>(tmem + 32 * q, v[q]);
+    tmem_wait_ld();
     tc_fence_before();
     __syncwarp();
     if (lane == 0) mbar_arrive_cluster(sum_empty);
     YT* const y = static_cast<YT*>(p.y);
-    if (p.aligned && col0 + COLS <= p.n) {
-        if (token < p.m) {
-            uint8_t* const to = reinterpret_cast<uint8_t*>(y + token * p.ldy + col0);
-#pragma unroll
-            for (int q = 0; q < COLS / 32; ++q)
-#pragma unroll
-                for (int i = 0; i < kWords; i += 8) store32(to + (q * kWords + i) * 4, &out[q][i]);
-        }
-        return;
-    }
-    // row by row, a result a lane; 32 columns at a time through shared memory
+    const bool direct = p.aligned && col0 + COLS <= p.n;
 #pragma unroll
     for (int q = 0; q < COLS / 32; ++q) {
+        uint32_t out[kWords];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            if constexpr (FMT == kNvfp4) v[q][i] = __float_as_uint(__uint_as_float(v[q][i]) * by.x * __shfl_sync(0xFFFFFFFFu, by.w[q], i));
+            if (!ok) v[q][i] = 0x7FC00000u;
+        }
+        if constexpr (sizeof(YT) == 4) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) out[i] = v[q][i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) out[i] = pack<YT>(__uint_as_float(v[q][2 * i]), __uint_as_float(v[q][2 * i + 1]));
+        }
+        if (direct) {
+            if (token < p.m) {
+                uint8_t* const to = reinterpret_cast<uint8_t*>(y + token * p.ldy + col0) + q * kWords * 4;
+#pragma unroll
+                for (int i = 0; i < kWords; i += 8) store32(to + 4 * i, out + i);
+            }
+            continue;
+        }
+        // a row at a time, a result a lane; 32 columns through shared memory
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < kWords; i += 4)
-            *reinterpret_cast<uint4*>(turn + lane * 36 + i) = make_uint4(out[q][i], out[q][i + 1], out[q][i + 2], out[q][i + 3]);
+        for (int i = 0; i < kWords; i += 4) *reinterpret_cast<uint4*>(turn + lane * 36 + i) = make_uint4(out[i], out[i + 1], out[i + 2], out[i + 3]);
         __syncwarp();
         const long long c = col0 + 32 * q + lane;
         if (c < p.n)
@@ -141,7 +149,7 @@ tcq_ms_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     __shared__ uint32_t tmem_at;
     __shared__ unsigned int gave_up;
     const uint32_t smem = (smem_u32(raw) + 1023) & ~1023u;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xFFFFFFFFu, int(threadIdx.x) >> 5, 0);
     const int rank = int(cluster_rank()), tiles = p.tiles_m * p.tiles_n, pair = blockIdx.x / 2, pairs = gridDim.x / 2;
 
     if (threadIdx.x == 0) {
@@ -156,69 +164,93 @@ tcq_ms_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     __syncthreads();
     cluster_sync();                                      // the neighbour's barriers are there
     tc_fence_after();
-    const uint32_t tmem = tmem_at, tmem_scales = tmem + T::kSumBuffers * NT;
+    const uint32_t tmem = tmem_at, tmem_scales = tmem + T::kSumBuffers * NT, full_first = map_rank(smem_u32(&full[0]), 0);
 
-    if (warp == 0 && lane == 0) {
-        // ---- loads of this CTA
-        long long it = 0;
+    if (warp == 0) {
+        // ---- loads of this CTA; the warp stays together, one lane issues
+        const bool one = elect_one();
+        uint32_t s = 0, phase = 1, loaded = 0;           // (the first wait for each stage is for the phase before the first)
         bool ok = true;
         for (int t = pair; t < tiles && ok; t += pairs) {
             const int tm = t % p.tiles_m, tn = t / p.tiles_m;
-            const int gx = min(2 * tm + rank, p.groups_m - 1);                  // (a group behind the last holds no results)
-            for (int kt = 0; kt < p.k_tiles; ++kt, ++it) {
-                const int s = int(it % T::kStages);
-                if (it >= T::kStages && !(ok = mbar_wait(smem_u32(&empty[s]), uint32_t(it / T::kStages - 1) & 1, &gave_up))) break;
-                const uint32_t to = smem + s * T::kStageBytes, bar = map_rank(smem_u32(&full[s]), 0);
-                if (rank == 0) mbar_expect(smem_u32(&full[s]), 2 * T::kLoaded);
-                tma_load_pair(to, &map_x, kt * 128, (2 * tm + rank) * 128, bar);
-                tma_load_pair(to + T::kBytesA, &map_w, kt * 128, tn * NT + rank * (NT / 2), bar);
-                tma_load_pair(to + T::kBytesA + T::kBytesB, &map_sx, 0, (gx * p.k_tiles + kt) * T::kAtoms, bar);
+            const int row_x = (2 * tm + rank) * 128, row_w = tn * NT + rank * (NT / 2);
+            int row_sx = min(2 * tm + rank, p.groups_m - 1) * p.k_tiles * T::kAtoms;             // (a group behind the last holds no results)
+            int row_sw[T::kGroups];
 #pragma unroll
-                for (int g = 0; g < T::kGroups; ++g)
-                    tma_load_pair(to + T::kBytesA + T::kBytesB + T::kBytesSa + g * T::kAtoms * 512, &map_sw, 0,
-                                  (min(tn * T::kGroups + g, p.groups_n - 1) * p.k_tiles + kt) * T::kAtoms, bar);
+            for (int g = 0; g < T::kGroups; ++g) row_sw[g] = min(tn * T::kGroups + g, p.groups_n - 1) * p.k_tiles * T::kAtoms;
+            for (int kt = 0; kt < p.k_tiles; ++kt) {
+                ok = mbar_wait(smem_u32(&empty[s]), phase, &gave_up);
+                ok = __all_sync(0xFFFFFFFFu, ok);        // every lane has seen this phase before the next can begin
+                if (!ok) break;
+                if (one) {
+                    const uint32_t to = smem + s * T::kStageBytes, bar = full_first + s * 8;
+                    if (rank == 0) mbar_expect(smem_u32(&full[s]), 2 * T::kLoaded);
+                    tma_load_pair(to, &map_x, kt * 128, row_x, bar);
+                    tma_load_pair(to + T::kBytesA, &map_w, kt * 128, row_w, bar);
+                    tma_load_pair(to + T::kBytesA + T::kBytesB, &map_sx, 0, row_sx + kt * T::kAtoms, bar);
+#pragma unroll
+                    for (int g = 0; g < T::kGroups; ++g)
+                        tma_load_pair(to + T::kBytesA + T::kBytesB + T::kBytesSa + g * T::kAtoms * 512, &map_sw, 0, row_sw[g] + kt * T::kAtoms, bar);
+                }
+                __syncwarp();
+                if (++s == T::kStages) { s = 0; phase ^= 1; }
+                if (loaded < T::kStages) ++loaded;
             }
         }
-        if (rank == 0 && gave_up)                        // nothing may be on its way to a CTA's memory when it ends
-            for (long long i = it > T::kStages ? it - T::kStages : 0; i < it; ++i)
-                for (long long t0 = clock64(); !mbar_try_wait(smem_u32(&full[i % T::kStages]), uint32_t(i / T::kStages) & 1) && clock64() - t0 < kMbarWaitCycles;) {}
-    } else if (warp == 1 && lane == 0 && rank == 0) {
-        // ---- products of the pair
+        if (rank == 0 && gave_up)                        // nothing may be on its way to a CTA's memory when it ends: the last loads of each stage
+            for (uint32_t i = 0; i < loaded; ++i) {
+                if (s == 0) phase ^= 1;
+                s = s == 0 ? T::kStages - 1 : s - 1;
+                for (long long t0 = clock64(); !mbar_try_wait(smem_u32(&full[s]), phase ^ 1) && clock64() - t0 < kMbarWaitCycles;) {}
+            }
+    } else if (warp == 1 && rank == 0) {
+        // ---- products of the pair; the warp stays together, one lane issues
         constexpr uint32_t kIdesc = 1u << 7 | 1u << 10 | uint32_t(NT >> 3) << 17 | (FMT == kMxfp4 ? 1u : 0u) << 23 | 2u << 27;
-        long long it = 0;
+        constexpr uint64_t kHigh128 = uint64_t(1024 >> 4) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61, kHigh16 = uint64_t(128 >> 4) << 32 | uint64_t(1) << 46;
+        const bool one = elect_one();
+        uint32_t s = 0, phase = 0;
         int n = 0;
         bool ok = true;
         for (int t = pair; t < tiles && ok; t += pairs, ++n) {
             const int buf = n % T::kSumBuffers, use = n / T::kSumBuffers;
-            if (use > 0 && !(ok = mbar_wait(smem_u32(&sum_empty[buf]), uint32_t(use - 1) & 1, &gave_up))) break;
+            if (use > 0) ok = mbar_wait(smem_u32(&sum_empty[buf]), uint32_t(use - 1) & 1, &gave_up);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) break;
             tc_fence_after();
             const uint32_t d = tmem + buf * NT;
-            for (int kt = 0; kt < p.k_tiles; ++kt, ++it) {
-                const int s = int(it % T::kStages);
-                if (!(ok = mbar_wait(smem_u32(&full[s]), uint32_t(it / T::kStages) & 1, &gave_up))) break;
+            for (int kt = 0; kt < p.k_tiles; ++kt) {
+                ok = mbar_wait(smem_u32(&full[s]), phase, &gave_up);
+                ok = __all_sync(0xFFFFFFFFu, ok);        // every lane has seen this phase before the stage can be loaded again
+                if (!ok) break;
                 tc_fence_after();
-                const uint32_t at = smem + s * T::kStageBytes, sa = tmem_scales + s * T::kScaleColumns, sb = sa + T::kAtoms * 4;
-                const uint32_t from = at + T::kBytesA + T::kBytesB;
+                const uint32_t at = (smem + s * T::kStageBytes) >> 4, sa = tmem_scales + s * T::kScaleColumns, sb = sa + T::kAtoms * 4;
+                const uint64_t da = kHigh128 | (at | 1u << 16), db = kHigh128 | ((at + (T::kBytesA >> 4)) | 1u << 16);
+                const uint64_t ds = kHigh16 | (at + ((T::kBytesA + T::kBytesB) >> 4));
+                if (one) {
 #pragma unroll
-                for (int j = 0; j < T::kAtoms; ++j) {
-                    tc_copy_scales<2>(sa + 4 * j, desc_rows16(from + 512 * j));
+                    for (int j = 0; j < T::kAtoms; ++j) {
+                        tc_copy_scales<2>(sa + 4 * j, ds + 32 * j);
 #pragma unroll
-                    for (int g = 0; g < T::kGroups; ++g)
-                        tc_copy_scales<2>(sb + 4 * (j * T::kGroups + g), desc_rows16(from + T::kBytesSa + 512 * (g * T::kAtoms + j)));
+                        for (int g = 0; g < T::kGroups; ++g)
+                            tc_copy_scales<2>(sb + 4 * (j * T::kGroups + g), ds + (T::kBytesSa >> 4) + 32 * (g * T::kAtoms + j));
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int atom = FMT == kNvfp4 ? j : j / 2;
+                        const uint32_t id = FMT == kNvfp4 ? 0u : 2u * (j % 2);
+                        mma_pair<FMT>(d, da + 2 * j, db + 2 * j, kIdesc | id << 4 | id << 29, sa + 4 * atom, sb + 4 * T::kGroups * atom, kt > 0 || j > 0);
+                    }
+                    tc_commit_pair(smem_u32(&empty[s]));
                 }
-                const uint64_t da = desc_rows128(at), db = desc_rows128(at + T::kBytesA);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {            // 64 columns: 32 bytes of a row, one word of scales (nvfp4) or half a word (mxfp4)
-                    const int atom = FMT == kNvfp4 ? j : j / 2;
-                    const uint32_t id = FMT == kNvfp4 ? 0u : 2u * (j % 2);
-                    mma_pair<FMT>(d, da + 2 * j, db + 2 * j, kIdesc | id << 4 | id << 29, sa + 4 * atom, sb + 4 * T::kGroups * atom, kt > 0 || j > 0);
-                }
-                tc_commit_pair(smem_u32(&empty[s]));
+                __syncwarp();
+                if (++s == T::kStages) { s = 0; phase ^= 1; }
             }
-            if (ok) tc_commit_pair(smem_u32(&sum_full[buf]));
+            if (ok && one) tc_commit_pair(smem_u32(&sum_full[buf]));
+            __syncwarp();
         }
         if (!ok) {                                       // what was issued ends before the tensor memory goes
-            tc_commit_pair(smem_u32(&drained));
+            if (one) tc_commit_pair(smem_u32(&drained));
+            __syncwarp();
             for (long long t0 = clock64(); !mbar_try_wait(smem_u32(&drained), 0) && clock64() - t0 < kMbarWaitCycles;) {}
         }
     } else if (warp >= 2) {
@@ -227,14 +259,14 @@ tcq_ms_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
         int n = 0;
         for (int t = pair; t < tiles; t += pairs, ++n) {
             const int buf = n % T::kSumBuffers, use = n / T::kSumBuffers;
-            const bool ok = mbar_wait(smem_u32(&sum_full[buf]), uint32_t(use) & 1, &gave_up);
-            __syncwarp();
+            const long long token0 = (long long)(t % p.tiles_m) * 256 + rank * 128 + 32 * quarter, col0 = (long long)(t / p.tiles_m) * NT + half * (NT / 2);
+            const Factors<FMT, NT / 2> by(p, token0, col0);
+            const bool ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sum_full[buf]), uint32_t(use) & 1, &gave_up));
             tc_fence_after();
             const uint32_t from = tmem + buf * NT + half * (NT / 2) + (uint32_t(32 * quarter) << 16), free_bar = map_rank(smem_u32(&sum_empty[buf]), 0);
-            const long long token0 = (long long)(t % p.tiles_m) * 256 + rank * 128 + 32 * quarter, col0 = (long long)(t / p.tiles_m) * NT + half * (NT / 2);
-            if (p.dtype == kF32) results<float, FMT, NT / 2>(p, from, free_bar, ok, token0, col0, turn);
-            else if (p.dtype == kF16) results<__half, FMT, NT / 2>(p, from, free_bar, ok, token0, col0, turn);
-            else results<__nv_bfloat16, FMT, NT / 2>(p, from, free_bar, ok, token0, col0, turn);
+            if (p.dtype == kF32) results<float, FMT, NT / 2>(p, from, free_bar, ok, token0, col0, by, turn);
+            else if (p.dtype == kF16) results<__half, FMT, NT / 2>(p, from, free_bar, ok, token0, col0, by, turn);
+            else results<__nv_bfloat16, FMT, NT / 2>(p, from, free_bar, ok, token0, col0, by, turn);
         }
     }
     __syncwarp();

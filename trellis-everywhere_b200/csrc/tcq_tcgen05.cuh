@@ -73,6 +73,14 @@ template <> __device__ __forceinline__ void tmem_load<32>(uint32_t tmem, uint32_
                    "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31]) : "r"(tmem));
 }
 
+// One lane of a whole warp, always the same.  A warp that loads or issues stays together and lets this lane do it: what the instructions
+// take is then known to be the same for the warp, and a stage of the products takes half the time to issue.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 // ---- bulk copies to shared memory, counted by an mbarrier
 __device__ __forceinline__ void tma_load(uint32_t smem, const CUtensorMap* map, int x, int y, uint32_t mbar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
