@@ -1,13 +1,13 @@
-// Products of two 4-bit microscaled matrices on the tensor cores: y[i][r] = sum_c X[i][c] * W[r][c].
+// Products of two 4-bit microscaled matrices, few tokens: y[i][r] = sum_c X[i][c] * W[r][c].
 //
-// tcgen05.mma (kind::mxf4nvf4, block scaled) multiplies 64 columns of 128 rows of one operand ("A") and NT rows of the other ("B"), with
-// the block scales in tensor memory; both operands come by TMA as they are stored, the scales by plain bulk copies, because
-// the storage order of the scales is the one that tcgen05.cp wants.  fp32 sums stay in tensor memory over the whole of k.
+// tcgen05.mma (kind::mxf4nvf4, block scaled) multiplies 64 columns of 128 rows of W and NT tokens, with the block scales in tensor memory;
+// codes come by TMA as they are stored, the scales by plain bulk copies, because the storage order of the scales is the one that
+// tcgen05.cp wants.  fp32 sums stay in tensor memory over the whole of k.
 //
-// Work split: one CTA per SM goes through tiles of 128 x NT results.  One thread loads stages of 256 columns, one issues copies of
-// scales and products, four warps take finished sums out of tensor memory (two buffers, where they fit), scale them by the row scales, round
-// and store.  With few tokens W's rows are the 128 and the tokens the NT: the weights are read once, and a cluster of S CTAs shares the
-// columns of a tile where there are fewer tiles than SMs; the S partial sums meet through distributed shared memory, in rank order.
+// Work split: one CTA per SM goes through tiles of 128 rows of W x NT tokens.  One warp loads stages of 256 columns, one issues copies of
+// scales and products, four take finished sums out of tensor memory (two buffers), scale them by the row scales, round and store.
+// W is read once; where there are fewer tiles than SMs, a cluster of S CTAs shares the columns of a tile, and the S partial sums meet
+// through distributed shared memory, in rank order.  Bound by the latency of one pass (few rows) or by what W's bytes take (many).
 //
 // A wait that runs out (kMbarWaitCycles) makes its CTA stop, and its results NaN.
 #include <algorithm>
@@ -20,24 +20,22 @@ namespace tcq {
 namespace {
 
 constexpr int kThreads = 192;                    // loader, issuer, four warps for the results
-constexpr int kRowsA = 128;
+constexpr int kRowsW = 128, kMostSplits = 8;
 
 template <int FMT, int NT>
 struct Tile {
     static constexpr int kAtoms = Ms<FMT>::kAtoms;
-    static constexpr int kGroups = (NT + 127) / 128;                          // 128-row groups of B's scales
-    static constexpr int kBytesA = kRowsA * 128, kBytesB = NT * 128, kBytesSa = kAtoms * 512, kBytesSb = kGroups * kAtoms * 512;
-    static constexpr int kStageBytes = (kBytesA + kBytesB + kBytesSa + kBytesSb + 1023) / 1024 * 1024;
-    static constexpr int kSumBuffers = NT <= 128 ? 2 : 1;
-    static constexpr int kSumColumns = NT < 32 ? 32 : NT;                     // of one buffer
-    static constexpr int kScaleColumns = kAtoms * 4 * (1 + kGroups);          // of one stage
+    static constexpr int kBytesW = kRowsW * 128, kBytesX = NT * 128, kBytesSw = kAtoms * 512, kBytesSx = kAtoms * 512;
+    static constexpr int kStageBytes = (kBytesW + kBytesX + kBytesSw + kBytesSx + 1023) / 1024 * 1024;
+    static constexpr int kSumColumns = NT < 32 ? 32 : NT;                     // of one of the two buffers of sums
+    static constexpr int kScaleColumns = kAtoms * 4 * 2;                      // of one stage
     // as many stages as fit in 216 KB and in what the sums leave of 512 columns of tensor memory
-    static constexpr int kBySmem = 216 * 1024 / kStageBytes, kByTmem = (512 - kSumBuffers * kSumColumns) / kScaleColumns;
+    static constexpr int kBySmem = 216 * 1024 / kStageBytes, kByTmem = (512 - 2 * kSumColumns) / kScaleColumns;
     static constexpr int kStages = std::min(std::min(kBySmem, kByTmem), 12);
-    static constexpr int kColumns = kSumBuffers * kSumColumns + kStages * kScaleColumns <= 256 ? 256 : 512;
+    static constexpr int kColumns = 2 * kSumColumns + kStages * kScaleColumns <= 256 ? 256 : 512;
     // over half of an SM's shared memory: two CTAs never share an SM, so that none waits for another's tensor memory
     static constexpr int kSmem = kStages * kStageBytes + 1024;
-    static_assert(kSmem > 114 * 1024 && kSmem <= 226 * 1024 && kStages >= 3);
+    static_assert(kSmem > 114 * 1024 && kSmem <= 226 * 1024 && kStages >= 3 && kStages * kStageBytes >= NT * kRowsW * 4);
 };
 
 }  // namespace
@@ -48,21 +46,33 @@ cudaError_t launch_ms_matmul_pair(const MsMatrix& x, const MsMatrix& w, long lon
 namespace {
 
 struct MatmulArgs {
-    const uint8_t* a_scales;
-    const uint8_t* b_scales;
-    const float* a_row;
-    const float* b_row;
-    long long a_rows, b_rows;
-    int tiles_a, tiles_b, k_tiles;
+    const uint8_t* w_scales;
+    const uint8_t* x_scales;
+    const float* w_row;
+    const float* x_row;
+    long long n, m;
+    int tiles_n, tiles_m, k_tiles;
     void* y;
-    long long step_a, step_b;                    // elements of y between neighbouring rows of A and of B
+    long long ldy;
     int dtype;
+    bool aligned;                                // y and ldy multiples of four elements
 };
 
 __device__ __forceinline__ void store(const MatmulArgs& p, long long at, float v) {
     if (p.dtype == kF32) static_cast<float*>(p.y)[at] = v;
     else if (p.dtype == kF16) static_cast<__half*>(p.y)[at] = __float2half_rn(v);
     else static_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(v);
+}
+__device__ __forceinline__ void store4(const MatmulArgs& p, long long at, float4 v) {
+    if (p.dtype == kF32) {
+        *reinterpret_cast<float4*>(static_cast<float*>(p.y) + at) = v;
+    } else if (p.dtype == kF16) {
+        const __half2 h[2] = {__floats2half2_rn(v.x, v.y), __floats2half2_rn(v.z, v.w)};
+        *reinterpret_cast<uint2*>(static_cast<__half*>(p.y) + at) = *reinterpret_cast<const uint2*>(h);
+    } else {
+        const __nv_bfloat162 h[2] = {__floats2bfloat162_rn(v.x, v.y), __floats2bfloat162_rn(v.z, v.w)};
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.y) + at) = *reinterpret_cast<const uint2*>(h);
+    }
 }
 
 template <int FMT>
@@ -78,67 +88,64 @@ __device__ __forceinline__ void mma_block_scaled(uint32_t d, uint64_t a, uint64_
 }
 
 template <int FMT, int NT>
-__global__ void __launch_bounds__(kThreads, 1) tcq_ms_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+__global__ void __launch_bounds__(kThreads, 1) tcq_ms_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                                                                     const __grid_constant__ MatmulArgs p) {
     using T = Tile<FMT, NT>;
     extern __shared__ uint8_t raw[];
-    __shared__ uint64_t full[T::kStages], empty[T::kStages], sum_full[T::kSumBuffers], sum_empty[T::kSumBuffers], drained;
+    __shared__ uint64_t full[T::kStages], empty[T::kStages], sum_full[2], sum_empty[2], drained;
     __shared__ uint32_t tmem_at;
     __shared__ unsigned int gave_up;
     const uint32_t smem = (smem_u32(raw) + 1023) & ~1023u;
     const int warp = __shfl_sync(0xFFFFFFFFu, int(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank(), splits = cluster_size();
     const int first = int((long long)p.k_tiles * rank / splits), last = int((long long)p.k_tiles * (rank + 1) / splits);
-    const int tiles = p.tiles_a * p.tiles_b, clusters = gridDim.x / splits;
+    const int tiles = p.tiles_n * p.tiles_m, clusters = gridDim.x / splits;
+    const long long atoms = (long long)p.k_tiles * T::kAtoms;
 
-    if (threadIdx.x == 0) {
-        gave_up = 0;
-        for (int s = 0; s < T::kStages; ++s) { mbar_init(smem_u32(&full[s]), 1); mbar_init(smem_u32(&empty[s]), 1); }
-        for (int s = 0; s < T::kSumBuffers; ++s) { mbar_init(smem_u32(&sum_full[s]), 1); mbar_init(smem_u32(&sum_empty[s]), 4); }
-        mbar_init(smem_u32(&drained), 1);
-        asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
+    auto load = [&](uint32_t s, int t, int kt) {
+        const int tn = t / p.tiles_m, tm = t % p.tiles_m;
+        const uint32_t to = smem + s * T::kStageBytes, bar = smem_u32(&full[s]);
+        mbar_expect(bar, T::kBytesW + T::kBytesX + T::kBytesSw + T::kBytesSx);
+        tma_load(to, &map_w, kt * 128, tn * kRowsW, bar);
+        tma_load(to + T::kBytesW, &map_x, kt * 128, tm * NT, bar);
+        bulk_load(to + T::kBytesW + T::kBytesX, p.w_scales + (tn * atoms + (long long)kt * T::kAtoms) * 512, T::kBytesSw, bar);
+        bulk_load(to + T::kBytesW + T::kBytesX + T::kBytesSw, p.x_scales + (tm * atoms + (long long)kt * T::kAtoms) * 512, T::kBytesSx, bar);
+    };
+    // The first tile's first stages are on their way before anything else: with few tokens a call is little more than its latencies.
+    const int ahead = min(T::kStages, last - first);
+    if (warp == 0) {
+        if (elect_one()) {
+            gave_up = 0;
+            for (int s = 0; s < T::kStages; ++s) { mbar_init(smem_u32(&full[s]), 1); mbar_init(smem_u32(&empty[s]), 1); }
+            for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&sum_full[s]), 1); mbar_init(smem_u32(&sum_empty[s]), 4); }
+            mbar_init(smem_u32(&drained), 1);
+            asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
+            for (int i = 0; i < ahead; ++i) load(i, blockIdx.x / splits, first + i);
+        }
+        __syncwarp();
     }
     if (warp == 1) tmem_alloc(smem_u32(&tmem_at), T::kColumns);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = tmem_at, tmem_scales = tmem + T::kSumBuffers * T::kSumColumns;
-    const long long atoms = (long long)p.k_tiles * T::kAtoms;
+    const uint32_t tmem = tmem_at, tmem_scales = tmem + 2 * T::kSumColumns;
 
     if (warp == 0) {
         // ---- loads; the warp stays together, one lane issues
         const bool one = elect_one();
-        uint32_t s = 0, phase = 1, loaded = 0;           // (the first wait for each stage is for the phase before the first)
+        uint32_t s = ahead % T::kStages, phase = ahead == T::kStages ? 0 : 1, loaded = ahead;    // (the first wait for a stage is for the phase before the first)
         bool ok = true;
-        const long long groups_b = (p.b_rows + 127) / 128;
-        for (int t = blockIdx.x / splits; t < tiles && ok; t += clusters) {
-            const int ta = t / p.tiles_b, tb = t % p.tiles_b;
-            const uint8_t* const from_a = p.a_scales + ta * atoms * 512;
-            const uint8_t* from_b[T::kGroups];
-#pragma unroll
-            for (int g = 0; g < T::kGroups; ++g) {
-                const long long group = (long long)tb * NT / 128 + g;             // one behind the last only has rows without results
-                from_b[g] = p.b_scales + (group < groups_b ? group : groups_b - 1) * atoms * 512;
-            }
-            for (int kt = first; kt < last; ++kt) {
+        int kt = first + ahead;
+        for (int t = blockIdx.x / splits; t < tiles && ok; t += clusters, kt = first)
+            for (; kt < last; ++kt) {
                 ok = mbar_wait(smem_u32(&empty[s]), phase, &gave_up);
                 ok = __all_sync(0xFFFFFFFFu, ok);        // every lane has seen this phase before the next can begin
                 if (!ok) break;
-                if (one) {
-                    const uint32_t to = smem + s * T::kStageBytes, bar = smem_u32(&full[s]);
-                    mbar_expect(bar, T::kBytesA + T::kBytesB + T::kBytesSa + T::kBytesSb);
-                    tma_load(to, &map_a, kt * 128, ta * kRowsA, bar);
-                    tma_load(to + T::kBytesA, &map_b, kt * 128, tb * NT, bar);
-                    bulk_load(to + T::kBytesA + T::kBytesB, from_a + (long long)kt * T::kBytesSa, T::kBytesSa, bar);
-#pragma unroll
-                    for (int g = 0; g < T::kGroups; ++g)
-                        bulk_load(to + T::kBytesA + T::kBytesB + T::kBytesSa + g * T::kAtoms * 512, from_b[g] + (long long)kt * T::kAtoms * 512, T::kAtoms * 512, bar);
-                }
+                if (one) load(s, t, kt);
                 __syncwarp();
                 if (++s == T::kStages) { s = 0; phase ^= 1; }
                 if (loaded < T::kStages) ++loaded;
             }
-        }
         if (gave_up)                                     // nothing may be on its way to this CTA's memory when it ends: the last loads of each stage
             for (uint32_t i = 0; i < loaded; ++i) {
                 if (s == 0) phase ^= 1;
@@ -153,8 +160,8 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_matmul_kernel(const __grid
         int n = 0;
         bool ok = true;
         for (int t = blockIdx.x / splits; t < tiles && ok; t += clusters, ++n) {
-            const int buf = n % T::kSumBuffers, use = n / T::kSumBuffers;
-            if (use > 0) ok = mbar_wait(smem_u32(&sum_empty[buf]), uint32_t(use - 1) & 1, &gave_up);
+            const int buf = n & 1;
+            if (n >= 2) ok = mbar_wait(smem_u32(&sum_empty[buf]), uint32_t(n / 2 - 1) & 1, &gave_up);
             ok = __all_sync(0xFFFFFFFFu, ok);
             if (!ok) break;
             tc_fence_after();
@@ -164,21 +171,19 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_matmul_kernel(const __grid
                 ok = __all_sync(0xFFFFFFFFu, ok);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t at = smem + s * T::kStageBytes, sa = tmem_scales + s * T::kScaleColumns, sb = sa + T::kAtoms * 4;
-                const uint64_t da = desc_rows128(at), db = desc_rows128(at + T::kBytesA), ds = desc_rows16(at + T::kBytesA + T::kBytesB);
+                const uint32_t at = smem + s * T::kStageBytes, sw = tmem_scales + s * T::kScaleColumns, sx = sw + T::kAtoms * 4;
+                const uint64_t dw = desc_rows128(at), dx = desc_rows128(at + T::kBytesW), ds = desc_rows16(at + T::kBytesW + T::kBytesX);
                 if (one) {
 #pragma unroll
                     for (int j = 0; j < T::kAtoms; ++j) {
-                        tc_copy_scales(sa + 4 * j, ds + 32 * j);
-#pragma unroll
-                        for (int g = 0; g < T::kGroups; ++g)
-                            tc_copy_scales(sb + 4 * (j * T::kGroups + g), ds + (T::kBytesSa >> 4) + 32 * (g * T::kAtoms + j));
+                        tc_copy_scales(sw + 4 * j, ds + 32 * j);
+                        tc_copy_scales(sx + 4 * j, ds + (T::kBytesSw >> 4) + 32 * j);
                     }
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {            // 64 columns: 32 bytes of a row, one word of scales (nvfp4) or half a word (mxfp4)
                         const int atom = FMT == kNvfp4 ? j : j / 2;
                         const uint32_t id = FMT == kNvfp4 ? 0u : 2u * (j % 2);
-                        mma_block_scaled<FMT>(d, da + 2 * j, db + 2 * j, kIdesc | id << 4 | id << 29, sa + 4 * atom, sb + 4 * T::kGroups * atom, kt > first || j > 0);
+                        mma_block_scaled<FMT>(d, dw + 2 * j, dx + 2 * j, kIdesc | id << 4 | id << 29, sw + 4 * atom, sx + 4 * atom, kt > first || j > 0);
                     }
                     tc_commit(smem_u32(&empty[s]));
                 }
@@ -193,54 +198,73 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_matmul_kernel(const __grid
             __syncwarp();
             for (long long t0 = clock64(); !mbar_try_wait(smem_u32(&drained), 0) && clock64() - t0 < kMbarWaitCycles;) {}
         }
-    } else if (warp >= 2) {
-        // ---- results: this warp's lanes are 32 rows of A
+    } else {
+        // ---- results: this warp's lanes are 32 rows of W, so that a store is 32 neighbours in y
         const int quarter = warp & 3;
         constexpr int kChunk = NT < 32 ? NT : 32;
         int n = 0;
         for (int t = blockIdx.x / splits; t < tiles; t += clusters, ++n) {
-            const int buf = n % T::kSumBuffers, use = n / T::kSumBuffers;
-            const bool ok = mbar_wait(smem_u32(&sum_full[buf]), uint32_t(use) & 1, &gave_up);
-            __syncwarp();
+            const int buf = n & 1;
+            const long long r = (long long)(t / p.tiles_m) * kRowsW + 32 * quarter + lane, i0 = (long long)(t % p.tiles_m) * NT;
+            const float fw = FMT == kNvfp4 && r < p.n ? p.w_row[r] : 1.0f;
+            const bool ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sum_full[buf]), uint32_t(n / 2) & 1, &gave_up));
             tc_fence_after();
-            const long long ra = (long long)(t / p.tiles_b) * kRowsA + 32 * quarter + lane, rb0 = (long long)(t % p.tiles_b) * NT;
-            const float fa = FMT == kNvfp4 && ra < p.a_rows ? p.a_row[ra] : 1.0f;
 #pragma unroll 1
             for (int c0 = 0; c0 < NT; c0 += kChunk) {
                 uint32_t v[kChunk];
                 tmem_load<kChunk>(tmem + buf * T::kSumColumns + c0 + (uint32_t(32 * quarter) << 16), v);
+                const float fx = FMT == kNvfp4 && i0 + c0 + lane < p.m ? __ldg(p.x_row + i0 + c0 + lane) : 1.0f;       // of column c0 + lane
                 tmem_wait_ld();
                 if (c0 + kChunk >= NT) {
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(smem_u32(&sum_empty[buf]));
                 }
+                if (splits > 1) {
+                    float* const part = reinterpret_cast<float*>(raw + (smem - smem_u32(raw)));
 #pragma unroll
-                for (int c = 0; c < kChunk; ++c) {
-                    float f = ok ? __uint_as_float(v[c]) : __uint_as_float(0x7FC00000u);
-                    const long long rb = rb0 + c0 + c;
-                    if (splits > 1) {
-                        reinterpret_cast<float*>(raw + (smem - smem_u32(raw)))[(c0 + c) * kRowsA + 32 * quarter + lane] = f;
-                    } else if (ra < p.a_rows && rb < p.b_rows) {
-                        if constexpr (FMT == kNvfp4) f = f * fa * p.b_row[rb];
-                        store(p, ra * p.step_a + rb * p.step_b, f);
+                    for (int c = 0; c < kChunk; ++c) part[(c0 + c) * kRowsW + 32 * quarter + lane] = ok ? __uint_as_float(v[c]) : __uint_as_float(0x7FC00000u);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < kChunk; ++c) {
+                        float f = ok ? __uint_as_float(v[c]) : __uint_as_float(0x7FC00000u);
+                        if constexpr (FMT == kNvfp4) f = f * fw * __shfl_sync(0xFFFFFFFFu, fx, c);
+                        if (r < p.n && i0 + c0 + c < p.m) store(p, (i0 + c0 + c) * p.ldy + r, f);
                     }
                 }
             }
         }
     }
     __syncwarp();
-    if (splits > 1) {                                        // one tile a cluster: add up the parts of it
+    if (splits > 1) {                                        // one tile a cluster: add up the parts of it, four neighbours a thread
         cluster_sync();
         const int t = blockIdx.x / splits;
-        const long long ra0 = (long long)(t / p.tiles_b) * kRowsA, rb0 = (long long)(t % p.tiles_b) * NT;
-        for (int i = int(rank) * kThreads + threadIdx.x; i < kRowsA * NT; i += int(splits) * kThreads) {
-            const long long ra = ra0 + i % kRowsA, rb = rb0 + i / kRowsA;
-            if (ra >= p.a_rows || rb >= p.b_rows) continue;
-            float f = 0.0f;
-            for (uint32_t q = 0; q < splits; ++q) f += ld_cluster_f32(smem + 4 * i, q);
-            if constexpr (FMT == kNvfp4) f = f * p.a_row[ra] * p.b_row[rb];
-            store(p, ra * p.step_a + rb * p.step_b, f);
+        const long long r0 = (long long)(t / p.tiles_m) * kRowsW, i0 = (long long)(t % p.tiles_m) * NT;
+        const int columns = int(min((long long)NT, p.m - i0));
+        for (int i = int(rank) * kThreads + threadIdx.x; i < kRowsW / 4 * columns; i += int(splits) * kThreads) {
+            const long long r = r0 + i % (kRowsW / 4) * 4, token = i0 + i / (kRowsW / 4);
+            if (r >= p.n) continue;
+            float4 part[kMostSplits];
+#pragma unroll
+            for (uint32_t q = 0; q < kMostSplits; ++q)
+                if (q < splits) part[q] = ld_cluster_f32x4(smem + 16 * i, q);
+            float4 f = part[0];
+#pragma unroll
+            for (uint32_t q = 1; q < kMostSplits; ++q)
+                if (q < splits) f = make_float4(f.x + part[q].x, f.y + part[q].y, f.z + part[q].z, f.w + part[q].w);
+            float* const e = &f.x;
+            if constexpr (FMT == kNvfp4) {
+                const float fx = p.x_row[token];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) e[j] = e[j] * (r + j < p.n ? p.w_row[r + j] : 1.0f) * fx;
+            }
+            if (p.aligned && r + 4 <= p.n) {
+                store4(p, token * p.ldy + r, f);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (r + j < p.n) store(p, token * p.ldy + r + j, e[j]);
+            }
         }
         cluster_sync();                                      // no CTA ends while another reads its part
     }
@@ -263,7 +287,7 @@ int sm_count() {
 }
 
 template <int FMT, int NT>
-cudaError_t launch(const MsMatrix& a, const MsMatrix& b, bool tokens_a, long long k, void* y, int dtype, long long ldy, int splits, cudaStream_t stream) {
+cudaError_t launch(const MsMatrix& x, const MsMatrix& w, long long k, void* y, int dtype, long long ldy, int splits, cudaStream_t stream) {
     using T = Tile<FMT, NT>;
     static bool ready[64] = {};
     int dev = 0;
@@ -273,13 +297,14 @@ cudaError_t launch(const MsMatrix& a, const MsMatrix& b, bool tokens_a, long lon
         if ((err = cudaFuncSetAttribute(tcq_ms_matmul_kernel<FMT, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem)) != cudaSuccess) return err;
         if (dev < 64) ready[dev] = true;
     }
-    CUtensorMap map_a, map_b;
+    CUtensorMap map_w, map_x;
     const long long pitch = ms_pitch(k);
-    if ((err = make_byte_map(&map_a, a.codes, pitch, a.rows, pitch, kRowsA)) != cudaSuccess) return err;
-    if ((err = make_byte_map(&map_b, b.codes, pitch, b.rows, pitch, NT)) != cudaSuccess) return err;
-    MatmulArgs p{a.scales, b.scales, a.row_scale, b.row_scale, a.rows, b.rows, int((a.rows + kRowsA - 1) / kRowsA), int((b.rows + NT - 1) / NT),
-                 int(ms_tiles_k(k)), y, tokens_a ? ldy : 1, tokens_a ? 1 : ldy, dtype};
-    const long long tiles = (long long)p.tiles_a * p.tiles_b;
+    if ((err = make_byte_map(&map_w, w.codes, pitch, w.rows, pitch, kRowsW)) != cudaSuccess) return err;
+    if ((err = make_byte_map(&map_x, x.codes, pitch, x.rows, pitch, NT)) != cudaSuccess) return err;
+    const size_t four = dtype == kF32 ? 16 : 8;
+    const MatmulArgs p{w.scales, x.scales, w.row_scale, x.row_scale, w.rows, x.rows, int((w.rows + kRowsW - 1) / kRowsW), int((x.rows + NT - 1) / NT),
+                       int(ms_tiles_k(k)), y, ldy, dtype, reinterpret_cast<uintptr_t>(y) % four == 0 && ldy % 4 == 0};
+    const long long tiles = (long long)p.tiles_n * p.tiles_m;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(splits > 1 ? tiles * splits : std::min<long long>(tiles, sm_count())));
     cfg.blockDim = dim3(kThreads);
@@ -291,28 +316,22 @@ cudaError_t launch(const MsMatrix& a, const MsMatrix& b, bool tokens_a, long lon
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, tcq_ms_matmul_kernel<FMT, NT>, map_a, map_b, p);
+    return cudaLaunchKernelEx(&cfg, tcq_ms_matmul_kernel<FMT, NT>, map_w, map_x, p);
 }
 
 template <int FMT>
 cudaError_t launch_fmt(const MsMatrix& x, const MsMatrix& w, long long k, void* y, int dtype, long long ldy, cudaStream_t stream) {
     const long long m = x.rows;
-    // Few tokens: W's rows are the 128.
-    if (m <= 64) {
-        const long long tiles = (w.rows + kRowsA - 1) / kRowsA;
-        int splits = 1;
-        while (splits < 8 && tiles * splits * 2 <= sm_count() && splits * 2 <= ms_tiles_k(k)) splits *= 2;
-        if (m <= 8) return launch<FMT, 8>(w, x, false, k, y, dtype, ldy, splits, stream);
-        if (m <= 16) return launch<FMT, 16>(w, x, false, k, y, dtype, ldy, splits, stream);
-        if (m <= 32) return launch<FMT, 32>(w, x, false, k, y, dtype, ldy, splits, stream);
-        return launch<FMT, 64>(w, x, false, k, y, dtype, ldy, splits, stream);
-    }
-    const long long ta = (m + kRowsA - 1) / kRowsA;
-    if (m > 128) return launch_ms_matmul_pair(x, w, k, FMT, y, dtype, ldy, (m + 255) / 256 * ((w.rows + 255) / 256) * 2 >= sm_count() ? 256 : 128, sm_count(), stream);
-    const long long tiles = ta * ((w.rows + 127) / 128);
+    const int sms = sm_count();
+    if (m > 128) return launch_ms_matmul_pair(x, w, k, FMT, y, dtype, ldy, (m + 255) / 256 * ((w.rows + 255) / 256) * 2 >= sms ? 256 : 128, sms, stream);
+    const long long tiles = (w.rows + kRowsW - 1) / kRowsW;
     int splits = 1;
-    while (splits < 8 && tiles * splits * 2 <= sm_count() && splits * 2 <= ms_tiles_k(k)) splits *= 2;
-    return launch<FMT, 128>(x, w, true, k, y, dtype, ldy, splits, stream);
+    while (splits < kMostSplits && tiles * splits * 2 <= sms && splits * 2 <= ms_tiles_k(k)) splits *= 2;
+    if (m <= 8) return launch<FMT, 8>(x, w, k, y, dtype, ldy, splits, stream);
+    if (m <= 16) return launch<FMT, 16>(x, w, k, y, dtype, ldy, splits, stream);
+    if (m <= 32) return launch<FMT, 32>(x, w, k, y, dtype, ldy, splits, stream);
+    if (m <= 64) return launch<FMT, 64>(x, w, k, y, dtype, ldy, splits, stream);
+    return launch<FMT, 128>(x, w, k, y, dtype, ldy, splits, stream);
 }
 
 }  // namespace

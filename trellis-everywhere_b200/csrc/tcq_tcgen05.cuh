@@ -111,9 +111,9 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t smem, uint32_t rank) {
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t smem, uint32_t rank) {
-    float v;
-    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}" : "=f"(v) : "r"(smem), "r"(rank) : "memory");
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t smem, uint32_t rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(map_rank(smem, rank)) : "memory");
     return v;
 }
 
