@@ -75,6 +75,19 @@ __device__ __forceinline__ void store4(const MatmulArgs& p, long long at, float4
     }
 }
 
+// Columns c0 .. c0 + N - 1 (tokens) of 32 rows of W, one a lane, scaled, rounded and stored: a store is 32 neighbours in y.
+template <typename YT, int FMT, int N>
+__device__ __forceinline__ void store_columns(const MatmulArgs& p, const uint32_t (&v)[N], long long r, long long token0, float fw, float fx) {
+    YT* to = static_cast<YT*>(p.y) + token0 * p.ldy + r;
+    const int columns = int(min((long long)N, p.m - token0));
+#pragma unroll
+    for (int c = 0; c < N; ++c, to += p.ldy) {
+        float f = __uint_as_float(v[c]);
+        if constexpr (FMT == kNvfp4) f = f * fw * __shfl_sync(0xFFFFFFFFu, fx, c);
+        if (r < p.n && c < columns) *to = from_f32<YT>(f);
+    }
+}
+
 template <int FMT>
 __device__ __forceinline__ void mma_block_scaled(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, bool add) {
     if constexpr (FMT == kNvfp4)
@@ -220,17 +233,19 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_matmul_kernel(const __grid
                     __syncwarp();
                     if (lane == 0) mbar_arrive(smem_u32(&sum_empty[buf]));
                 }
+#pragma unroll
+                for (int c = 0; c < kChunk; ++c)
+                    if (!ok) v[c] = 0x7FC00000u;
                 if (splits > 1) {
-                    float* const part = reinterpret_cast<float*>(raw + (smem - smem_u32(raw)));
+                    float* const part = reinterpret_cast<float*>(raw + (smem - smem_u32(raw))) + c0 * kRowsW + 32 * quarter + lane;
 #pragma unroll
-                    for (int c = 0; c < kChunk; ++c) part[(c0 + c) * kRowsW + 32 * quarter + lane] = ok ? __uint_as_float(v[c]) : __uint_as_float(0x7FC00000u);
+                    for (int c = 0; c < kChunk; ++c) part[c * kRowsW] = __uint_as_float(v[c]);
+                } else if (p.dtype == kF32) {
+                    store_columns<float, FMT>(p, v, r, i0 + c0, fw, fx);
+                } else if (p.dtype == kF16) {
+                    store_columns<__half, FMT>(p, v, r, i0 + c0, fw, fx);
                 } else {
-#pragma unroll
-                    for (int c = 0; c < kChunk; ++c) {
-                        float f = ok ? __uint_as_float(v[c]) : __uint_as_float(0x7FC00000u);
-                        if constexpr (FMT == kNvfp4) f = f * fw * __shfl_sync(0xFFFFFFFFu, fx, c);
-                        if (r < p.n && i0 + c0 + c < p.m) store(p, (i0 + c0 + c) * p.ldy + r, f);
-                    }
+                    store_columns<__nv_bfloat16, FMT>(p, v, r, i0 + c0, fw, fx);
                 }
             }
         }
@@ -319,14 +334,25 @@ cudaError_t launch(const MsMatrix& x, const MsMatrix& w, long long k, void* y, i
     return cudaLaunchKernelEx(&cfg, tcq_ms_matmul_kernel<FMT, NT>, map_w, map_x, p);
 }
 
+// Which form.  us on a B200, nvfp4 (mxfp4 is up to 15 % faster at the same choices):
+//   the columns shared by S CTAs while all run at once, at least two stages of 256 columns each, from eight stages on: one token, S = 1 / 2 / 4 / 8,
+//     4096 x 4096 7.5 / 6.8 / 5.7 / 11.9 (more CTAs than SMs), 1024 x 4096 7.5 / 6.8 / 5.4 / 5.0, 4096 x 1024 4.5 / 5.1 / 4.9
+//   one SM against a pair of SMs on 256 x 128 results: 64 tokens 8.8 and 10.9 (12288 x 4096), 7.8 and 7.6 (4096 x 4096); 128 tokens 10.5 and 11.5
+//     (12288 x 4096, every SM busy), 12.6 and 13.6 (4096 x 12288, S = 4), but 10.2 and 8.2 (4096 x 4096), 6.7 and 6.0 (4096 x 1024);
+//     256 tokens 14.9 and 11.8 (12288 x 4096)
+//   pairs: a tile of 256 x 256 takes 1.8 times as long as one of 256 x 128, which decides by the rounds that either needs: 512 tokens 12288 x 4096
+//     18.1 and 15.7, 2048 tokens 4096 x 12288 39.9 and 43.1
 template <int FMT>
 cudaError_t launch_fmt(const MsMatrix& x, const MsMatrix& w, long long k, void* y, int dtype, long long ldy, cudaStream_t stream) {
-    const long long m = x.rows;
+    const long long m = x.rows, k_tiles = ms_tiles_k(k), tiles = (w.rows + kRowsW - 1) / kRowsW;
     const int sms = sm_count();
-    if (m > 128) return launch_ms_matmul_pair(x, w, k, FMT, y, dtype, ldy, (m + 255) / 256 * ((w.rows + 255) / 256) * 2 >= sms ? 256 : 128, sms, stream);
-    const long long tiles = (w.rows + kRowsW - 1) / kRowsW;
+    if (m > 128 || (m > 64 && tiles <= sms / 2 && k_tiles < 32)) {
+        const long long pairs = sms / 2, tiles_m = (m + 255) / 256;
+        const long long rounds128 = (tiles_m * tiles + pairs - 1) / pairs, rounds256 = (tiles_m * ((w.rows + 255) / 256) + pairs - 1) / pairs;
+        return launch_ms_matmul_pair(x, w, k, FMT, y, dtype, ldy, 5 * rounds128 > 9 * rounds256 ? 256 : 128, sms, stream);
+    }
     int splits = 1;
-    while (splits < kMostSplits && tiles * splits * 2 <= sms && splits * 2 <= ms_tiles_k(k)) splits *= 2;
+    while (splits < kMostSplits && tiles * splits * 2 <= sms && splits * 4 <= k_tiles && k_tiles >= 8) splits *= 2;
     if (m <= 8) return launch<FMT, 8>(x, w, k, y, dtype, ldy, splits, stream);
     if (m <= 16) return launch<FMT, 16>(x, w, k, y, dtype, ldy, splits, stream);
     if (m <= 32) return launch<FMT, 32>(x, w, k, y, dtype, ldy, splits, stream);

@@ -159,12 +159,17 @@ tcq_ms_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
         mbar_init(smem_u32(&drained), 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 1) tmem_alloc<2>(smem_u32(&tmem_at), 512);
-    tc_fence_before();
-    __syncthreads();
-    cluster_sync();                                      // the neighbour's barriers are there
-    tc_fence_after();
-    const uint32_t tmem = tmem_at, tmem_scales = tmem + T::kSumBuffers * NT, full_first = map_rank(smem_u32(&full[0]), 0);
+    __syncwarp();
+    cluster_sync();                                      // the neighbour's barriers are there: the loads begin
+    uint32_t tmem = 0;
+    if (warp > 0) {
+        if (warp == 1) tmem_alloc<2>(smem_u32(&tmem_at), 512);
+        tc_fence_before();
+        asm volatile("bar.sync 1, %0;" ::"n"(kThreads - 32) : "memory");
+        tc_fence_after();
+        tmem = tmem_at;
+    }
+    const uint32_t tmem_scales = tmem + T::kSumBuffers * NT, full_first = map_rank(smem_u32(&full[0]), 0);
 
     if (warp == 0) {
         // ---- loads of this CTA; the warp stays together, one lane issues
