@@ -24,12 +24,13 @@ be captured into a graph.  Nothing here has a gradient: a call that would need o
 """
 from __future__ import annotations
 
+import math
 from typing import NamedTuple, Optional, Tuple
 
 import torch
 
 from . import _lib
-from .qtip import _call, _cuda_device
+from .qtip import _cuda_device
 
 FORMATS = {"mxfp4": 0, "nvfp4": 1}
 BLOCKS = {"mxfp4": 32, "nvfp4": 16}
@@ -72,8 +73,25 @@ def _check_dtype(dtype) -> int:
     return _DTYPES[dtype]
 
 
-def _check_q(q: Microscaled, name: str) -> torch.device:
-    """The device of a well-formed matrix; raises otherwise (the kernels trust its sizes)."""
+def _check_q(q: Microscaled, name: str) -> int:
+    """The CUDA device's number of a well-formed matrix; raises otherwise (the kernels trust its sizes).
+
+    The products of token generation last a few microseconds, so what leads up to them is kept short: one pass over the parts
+    where all is well, and the search for what is wrong elsewhere.
+    """
+    if type(q) is Microscaled:
+        codes, scales, row, (rows, k), fmt = q
+        dev = codes.get_device()
+        if (dev >= 0 and codes.dtype is torch.uint8 and scales.dtype is torch.uint8 and scales.get_device() == dev
+                and codes.shape == (rows, 16 * -(-k // 32)) and codes.is_contiguous() and scales.is_contiguous()
+                and (row.get_device() == dev and row.dtype is torch.float32 and row.shape == (rows,) and row.is_contiguous()
+                     and scales.shape == (-(-rows // 128), 4 * -(-k // 256), 32, 4, 4) if fmt == "nvfp4" and row is not None
+                     else fmt == "mxfp4" and row is None and scales.shape == (-(-rows // 128), 2 * -(-k // 256), 32, 4, 4))):
+            return dev
+    return _refuse_q(q, name)
+
+
+def _refuse_q(q, name: str) -> int:
     if not isinstance(q, Microscaled):
         raise ValueError(f"{name} must be a Microscaled matrix, got {type(q).__name__}")
     _check_fmt(q.fmt)
@@ -88,46 +106,45 @@ def _check_q(q: Microscaled, name: str) -> torch.device:
             continue
         if t is None or t.dtype != dtype or tuple(t.shape) != shape or t.device != dev or not t.is_contiguous():
             raise ValueError(f"{name}.{part} must be a contiguous {dtype} {list(shape)} tensor on {dev}")
-    if dev.type != "cuda":
-        _cuda_device()
-        raise ValueError(f"{name} must be on a CUDA device")
-    return dev
+    _cuda_device()
+    raise ValueError(f"{name} must be on a CUDA device")
 
 
-def _check_x(x: torch.Tensor, name: str) -> Tuple[torch.Tensor, int]:
-    """A 2-d CUDA matrix with unit column stride, and its type's number."""
-    dt = _check_dtype(x.dtype)
-    if torch.is_grad_enabled() and x.requires_grad:
+def _check_x(x: torch.Tensor, name: str) -> torch.Tensor:
+    """A matrix with unit column stride and rows that do not overlap, of a type the kernels take, on a CUDA device."""
+    if x.dtype not in _DTYPES:
+        _check_dtype(x.dtype)
+    if x.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"no gradient is defined here: detach {name} or call under torch.no_grad()")
     if not x.is_cuda:
         _cuda_device()
         raise ValueError(f"{name} must be on a CUDA device")
-    if x.stride(-1) != 1 and x.shape[-1] > 1:
-        x = x.contiguous()
-    if x.shape[0] > 1 and x.stride(0) < x.shape[1]:          # rows that repeat or overlap (an expanded tensor)
-        x = x.contiguous()
-    return x, dt
+    if x.is_contiguous():
+        return x
+    rows, k = x.shape
+    if (x.stride(1) != 1 and k > 1) or (x.stride(0) < k and rows > 1):
+        return x.detach().contiguous()
+    return x
 
 
 def _pitch(x: torch.Tensor) -> int:
-    return x.stride(0) if x.shape[0] > 1 else max(x.shape[1], 1)
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
-@torch.no_grad()
-def _quantize(x: torch.Tensor, dt: int, fmt: str, rotate: int, signs: Optional[torch.Tensor]) -> Microscaled:
-    rows, k = x.shape
-    codes_shape, scales_shape = _storage(rows, k, fmt)
-    dev = x.device
-    codes = torch.empty(codes_shape, dtype=torch.uint8, device=dev)
-    scales = torch.empty(scales_shape, dtype=torch.uint8, device=dev)
-    row = torch.empty(rows, dtype=torch.float32, device=dev) if fmt == "nvfp4" else None
-    if rows and k:
-        _call(dev, "tcq_ms_quantize", x.data_ptr(), dt, rows, k, _pitch(x), FORMATS[fmt], rotate,
-              signs.data_ptr() if signs is not None else None, codes.data_ptr(), scales.data_ptr(),
-              row.data_ptr() if row is not None else None)
-    elif row is not None:
-        row.fill_(1.0)                                       # rows without columns
-    return Microscaled(codes, scales, row, (rows, k), fmt)
+def _launch(dev: int, name: str, *args) -> None:
+    """``qtip._call`` for a device number, by the shortest way to the current device and stream."""
+    fn = getattr(_lib.lib(), name)
+    if torch._C._cuda_getDevice() == dev:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        _lib.check(rc, name)
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
 
 
 def quantize(x: torch.Tensor, fmt: str = "nvfp4", rotate: int = 0, signs: Optional[torch.Tensor] = None) -> Microscaled:
@@ -145,26 +162,33 @@ def quantize(x: torch.Tensor, fmt: str = "nvfp4", rotate: int = 0, signs: Option
         raise ValueError(f"rotate={rotate} must be one of {ROTATIONS} and divide the {x.shape[1]} columns")
     if (signs is not None) != bool(rotate):
         raise ValueError("signs go with rotate: give both or neither")
-    x, dt = _check_x(x, "x")
+    x = _check_x(x, "x")
     if signs is not None and (signs.dtype != torch.float32 or tuple(signs.shape) != (x.shape[1],) or signs.device != x.device
                               or not signs.is_contiguous()):
         raise ValueError(f"signs must be a contiguous float32 [{x.shape[1]}] tensor on {x.device}")
-    return _quantize(x, dt, fmt, rotate, signs)
+    rows, k = x.shape
+    dev = x.device
+    codes_shape, scales_shape = _storage(rows, k, fmt)
+    codes = torch.empty(codes_shape, dtype=torch.uint8, device=dev)
+    scales = torch.empty(scales_shape, dtype=torch.uint8, device=dev)
+    row = torch.empty(rows, dtype=torch.float32, device=dev) if fmt == "nvfp4" else None
+    if rows and k:
+        _launch(dev.index, "tcq_ms_quantize", x.data_ptr(), _DTYPES[x.dtype], rows, k, _pitch(x), FORMATS[fmt], rotate, _ptr(signs),
+                codes.data_ptr(), scales.data_ptr(), _ptr(row))
+    elif row is not None:
+        row.fill_(1.0)                                       # rows without columns
+    return Microscaled(codes, scales, row, (rows, k), fmt)
 
 
-@torch.no_grad()
 def dequantize(q: Microscaled, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The ``[rows, k]`` values.  Of a matrix quantised here they are exact in fp32, and in bf16 as well; fp16 rounds those out of its range."""
     dev, dt = _check_q(q, "q"), _check_dtype(dtype)
     rows, k = q.shape
-    out = torch.empty((rows, k), dtype=dtype, device=dev)
+    out = torch.empty((rows, k), dtype=dtype, device=q.codes.device)
     if rows and k:
-        _call(dev, "tcq_ms_dequantize", *_parts(q), rows, k, FORMATS[q.fmt], out.data_ptr(), dt, k)
+        _launch(dev, "tcq_ms_dequantize", q.codes.data_ptr(), q.scales.data_ptr(), _ptr(q.row_scale), rows, k, FORMATS[q.fmt],
+                out.data_ptr(), dt, k)
     return out
-
-
-def _parts(q: Microscaled):
-    return q.codes.data_ptr(), q.scales.data_ptr(), q.row_scale.data_ptr() if q.row_scale is not None else None
 
 
 def linear(x: torch.Tensor, w: Microscaled) -> torch.Tensor:
@@ -174,40 +198,37 @@ def linear(x: torch.Tensor, w: Microscaled) -> torch.Tensor:
     the other rows of x hold, and equal calls give equal results.
     """
     dev = _check_q(w, "w")
-    n, k = w.shape
-    if x.dim() < 1 or x.shape[-1] != k:
-        raise ValueError(f"x must be [..., {k}], got {tuple(x.shape)}")
-    if x.device != dev:
-        raise ValueError(f"x must be on {dev}")
-    if not k:
-        _check_dtype(x.dtype)
-        return torch.zeros((*x.shape[:-1], n), dtype=x.dtype, device=dev)
-    flat, dt = _check_x(x.reshape(-1, k), "x")
-    return _linear(flat, dt, w).reshape(*x.shape[:-1], n)
-
-
-@torch.no_grad()
-def _linear(x: torch.Tensor, dt: int, w: Microscaled) -> torch.Tensor:
-    n, k = w.shape
-    y = torch.empty((x.shape[0], n), dtype=x.dtype, device=x.device)
-    if x.shape[0] and n:
-        _call(x.device, "tcq_ms_linear", x.data_ptr(), dt, x.shape[0], _pitch(x), *_parts(w), n, k, FORMATS[w.fmt], y.data_ptr(), n)
+    codes, scales, row, (n, k), fmt = w
+    shape = x.shape
+    if not shape or shape[-1] != k:
+        raise ValueError(f"x must be [..., {k}], got {tuple(shape)}")
+    if x.get_device() != dev:
+        raise ValueError(f"x must be on {codes.device}")
+    flat = _check_x(x if len(shape) == 2 else x.reshape(math.prod(shape[:-1]), k), "x")
+    m = flat.shape[0]
+    y = torch.empty((m, n) if len(shape) == 2 else (*shape[:-1], n), dtype=flat.dtype, device=flat.device)
+    if m and n and k:
+        _launch(dev, "tcq_ms_linear", flat.data_ptr(), _DTYPES[flat.dtype], m, _pitch(flat), codes.data_ptr(), scales.data_ptr(), _ptr(row),
+                n, k, FORMATS[fmt], y.data_ptr(), n)
+    elif not k:
+        y.zero_()
     return y
 
 
-@torch.no_grad()
 def matmul(x: Microscaled, w: Microscaled, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``X @ W.T`` of two 4-bit matrices ``[m, k]`` and ``[n, k]`` of one format -> ``[m, n]`` of ``dtype``, summed in fp32, rounded once."""
     dev, dt = _check_q(w, "w"), _check_dtype(dtype)
-    if _check_q(x, "x") != dev or x.fmt != w.fmt or x.shape[1] != w.shape[1]:
+    codes, scales, row, (n, k), fmt = w
+    if _check_q(x, "x") != dev or x.fmt != fmt or x.shape[1] != k:
         raise ValueError(f"x and w must have one format, device and number of columns: {x.fmt} {x.shape} on {x.codes.device}, "
-                         f"{w.fmt} {w.shape} on {dev}")
-    (m, k), n = x.shape, w.shape[0]
-    if not k:
-        return torch.zeros((m, n), dtype=dtype, device=dev)
-    y = torch.empty((m, n), dtype=dtype, device=dev)
-    if m and n:
-        _call(dev, "tcq_ms_matmul", *_parts(x), m, *_parts(w), n, k, FORMATS[w.fmt], y.data_ptr(), dt, n)
+                         f"{fmt} {w.shape} on {codes.device}")
+    m = x.shape[0]
+    y = torch.empty((m, n), dtype=dtype, device=codes.device)
+    if m and n and k:
+        _launch(dev, "tcq_ms_matmul", x.codes.data_ptr(), x.scales.data_ptr(), _ptr(x.row_scale), m, codes.data_ptr(), scales.data_ptr(), _ptr(row),
+                n, k, FORMATS[fmt], y.data_ptr(), dt, n)
+    elif not k:
+        y.zero_()
     return y
 
 
