@@ -292,7 +292,8 @@ def test_results_leave_the_rest_of_their_buffer_alone(ms):
             for ldy in (n + 3, n + 8):
                 y = torch.full((m + 2, ldy), 77.0, dtype=torch.bfloat16, device="cuda")
                 xd = x.cuda()
-                assert lib.tcq_ms_linear(xd.data_ptr(), 2, m, k, w.codes.data_ptr(), w.scales.data_ptr(), w.row_scale.data_ptr(), n, k, 1, y.data_ptr(), ldy, stream) == 0
+                ws = torch.empty(lib.tcq_ms_linear_workspace_bytes(m, k, 2), dtype=torch.uint8, device="cuda")
+                assert lib.tcq_ms_linear(xd.data_ptr(), 2, m, k, w.codes.data_ptr(), w.scales.data_ptr(), w.row_scale.data_ptr(), n, k, 1, y.data_ptr(), ldy, ws.data_ptr(), ws.numel(), stream) == 0
                 assert torch.equal(y[:m, :n].cpu(), (x.double() @ wv.t()).to(torch.bfloat16))
                 assert (y[m:] == 77).all() and (y[:, n:] == 77).all()
                 y.fill_(77.0)

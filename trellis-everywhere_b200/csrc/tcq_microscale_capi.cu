@@ -62,17 +62,23 @@ int tcq_ms_dequantize(const uint8_t* codes, const uint8_t* scales, const float* 
     return err == cudaSuccess ? TCQ_OK : report_cuda_error(err, "ms_dequantize");
 }
 
+size_t tcq_ms_linear_workspace_bytes(int64_t m, int64_t k, int dtype) {
+    return check_ms(m, k, TCQ_MS_NVFP4, dtype) != TCQ_OK ? 0 : ms_linear_workspace_bytes(m, k, dtype);
+}
+
 int tcq_ms_linear(const void* x, int dtype, int64_t m, int64_t ldx, const uint8_t* codes, const uint8_t* scales,
-                  const float* row_scale, int64_t n, int64_t k, int format, void* y, int64_t ldy, void* stream) {
+                  const float* row_scale, int64_t n, int64_t k, int format, void* y, int64_t ldy, void* ws, size_t ws_bytes,
+                  void* stream) {
     int rc = check_ms(n, k, format, dtype);
     if (rc == TCQ_OK) rc = check_ms(m, k, format, dtype);
     if (rc != TCQ_OK) return rc;
     if (n == 0 || m == 0) return TCQ_OK;
     if (k == 0 || ldx < k || ldy < n) return TCQ_E_BAD_ARGUMENT;
-    if (x == nullptr || y == nullptr) return TCQ_E_NULL_POINTER;
+    if (x == nullptr || y == nullptr || ws == nullptr) return TCQ_E_NULL_POINTER;
     if ((rc = check_ms_matrix(codes, scales, row_scale, format)) != TCQ_OK) return rc;
-    if (misaligned(x, type_bytes(dtype)) || misaligned(y, type_bytes(dtype))) return TCQ_E_MISALIGNED;
-    cudaError_t err = launch_ms_linear(x, dtype, m, ldx, {codes, scales, row_scale, n}, k, format, y, ldy, static_cast<cudaStream_t>(stream));
+    if (misaligned(x, type_bytes(dtype)) || misaligned(y, type_bytes(dtype)) || misaligned(ws, 256)) return TCQ_E_MISALIGNED;
+    if (ws_bytes < ms_linear_workspace_bytes(m, k, dtype)) return TCQ_E_WORKSPACE;
+    cudaError_t err = launch_ms_linear(x, dtype, m, ldx, {codes, scales, row_scale, n}, k, format, y, ldy, ws, static_cast<cudaStream_t>(stream));
     return err == cudaSuccess ? TCQ_OK : report_cuda_error(err, "ms_linear");
 }
 

@@ -208,8 +208,11 @@ def linear(x: torch.Tensor, w: Microscaled) -> torch.Tensor:
     m = flat.shape[0]
     y = torch.empty((m, n) if len(shape) == 2 else (*shape[:-1], n), dtype=flat.dtype, device=flat.device)
     if m and n and k:
-        _launch(dev, "tcq_ms_linear", flat.data_ptr(), _DTYPES[flat.dtype], m, _pitch(flat), codes.data_ptr(), scales.data_ptr(), _ptr(row),
-                n, k, FORMATS[fmt], y.data_ptr(), n)
+        dt = _DTYPES[flat.dtype]
+        size = _lib.lib().tcq_ms_linear_workspace_bytes(m, k, dt)
+        ws = torch.empty(size, dtype=torch.uint8, device=flat.device)      # given back when the call is queued: the stream's later work comes after it
+        _launch(dev, "tcq_ms_linear", flat.data_ptr(), dt, m, _pitch(flat), codes.data_ptr(), scales.data_ptr(), _ptr(row),
+                n, k, FORMATS[fmt], y.data_ptr(), n, ws.data_ptr(), size)
     elif not k:
         y.zero_()
     return y
