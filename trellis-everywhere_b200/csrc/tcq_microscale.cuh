@@ -85,6 +85,7 @@ struct MsMatrix {
     long long rows;
 };
 
+int ms_sm_count();             // of the current device
 int report_cuda_error(cudaError_t err, const char* where);     // tcq_capi.cu
 
 cudaError_t launch_ms_quantize(const void* x, int dtype, long long rows, long long k, long long ldx, int fmt, int rotate, const float* signs,

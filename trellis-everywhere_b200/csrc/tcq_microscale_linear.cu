@@ -11,7 +11,7 @@
 // The 16 rows are 4 x 4: rows 4 i .. 4 i + 3 of each 32 in a group of 128, whose scales are 64 neighbouring bytes.
 // Warps of a CTA share the columns; partial sums meet in shared memory, in a fixed order.  Sums within a step are the tensor core's, steps are
 // added in fp32 with rounding to nearest.
-#include "tcq_microscale.cuh"
+#include "tcq_microscale_weights.cuh"
 
 namespace tcq {
 
@@ -30,33 +30,6 @@ struct LinearArgs {
     long long ldy;
     int warps_k;                 // warps that share a row group's columns: 1, 2, 4 or 8
 };
-
-// Four codes (the low 16 bits of w) as bf16 pairs, times the scale.
-__device__ __forceinline__ void four_weights(uint32_t w, __nv_bfloat162 scale, uint32_t& a, uint32_t& b) {
-    const uint32_t mag = w & 0x7777u;
-    const uint32_t lo = __byte_perm(0xC0800000u, 0xC0804000u, mag);                   // 0 .5 1 1.5 2 3 4 6: low bytes 00 00 80 C0 00 40 80 C0
-    uint32_t hi = __byte_perm(0x3F3F3F00u, 0x40404040u, mag);                         // high bytes 00 3F 3F 3F 40 40 40 40
-    uint32_t sign;
-    asm("prmt.b32 %0, %1, %2, 0x9D8C;" : "=r"(sign) : "r"(w), "r"(w << 4));           // the top bit of each code, over a whole byte
-    hi |= sign & 0x80808080u;
-    const uint32_t p = __byte_perm(lo, hi, 0x5140), q = __byte_perm(lo, hi, 0x7362);
-    const __nv_bfloat162 x = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&p), scale), y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&q), scale);
-    a = *reinterpret_cast<const uint32_t*>(&x);
-    b = *reinterpret_cast<const uint32_t*>(&y);
-}
-
-// The scale of 16 columns q of a lane's 64, twice; every one is a bf16 number.
-template <int FMT>
-__device__ __forceinline__ __nv_bfloat162 scale_of(uint32_t word, int q) {
-    if constexpr (FMT == kNvfp4) {
-        return __float2bfloat162_rn(e4m3_to_f32((word >> (8 * q)) & 0xFFu));
-    } else {
-        const uint32_t byte = (word >> (8 * (q / 2))) & 0xFFu;
-        const uint32_t bits = byte == 0 ? 0x0040u : byte == 255 ? 0x7FC0u : byte << 7;
-        const uint32_t two = bits << 16 | bits;
-        return *reinterpret_cast<const __nv_bfloat162*>(&two);
-    }
-}
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -191,17 +164,9 @@ cudaError_t launch(LinearArgs p, int sms, cudaStream_t stream) {
     return cudaGetLastError();
 }
 
-template <typename YT, int FMT, int P>
-cudaError_t launch_n(const LinearArgs& p, int sms, cudaStream_t stream) {
-    const long long virt = p.m * P;
-    if (virt <= 8 / P * P) return launch<YT, FMT, 1, P>(p, sms, stream);
-    if (virt <= 16 / P * P) return launch<YT, FMT, 2, P>(p, sms, stream);
-    return launch<YT, FMT, 4, P>(p, sms, stream);
-}
-
 template <typename YT, int P>
 cudaError_t launch_fmt(const LinearArgs& p, int fmt, int sms, cudaStream_t stream) {
-    return fmt == kNvfp4 ? launch_n<YT, kNvfp4, P>(p, sms, stream) : launch_n<YT, kMxfp4, P>(p, sms, stream);
+    return fmt == kNvfp4 ? launch<YT, kNvfp4, 1, P>(p, sms, stream) : launch<YT, kMxfp4, 1, P>(p, sms, stream);
 }
 
 template <typename T, int P>
@@ -212,6 +177,10 @@ cudaError_t split(const void* x, long long m, long long k, long long ldx, void* 
 
 }  // namespace
 
+// tcq_microscale_linear_many.cu: x as m * parts rows of bf16, `width` columns of them (the others zero), 16-byte aligned.
+cudaError_t launch_ms_linear_many(const __nv_bfloat16* x, long long ldx, long long width, long long m, int parts, int dtype, const MsMatrix& w, long long k,
+                                  int fmt, void* y, long long ldy, cudaStream_t stream);
+
 size_t ms_linear_workspace_bytes(long long m, long long k, int dtype) {
     return size_t(m) * size_t(ms_tiles_k(k) * kMsTileK) * 2 * (dtype == kF32 ? 3 : dtype == kF16 ? 2 : 1);
 }
@@ -219,14 +188,17 @@ size_t ms_linear_workspace_bytes(long long m, long long k, int dtype) {
 cudaError_t launch_ms_linear(const void* x, int dtype, long long m, long long ldx, const MsMatrix& w, long long k, int fmt, void* y,
                              long long ldy, void* ws, cudaStream_t stream) {
     const long long width = ms_tiles_k(k) * kMsTileK;
+    const int parts = dtype == kF32 ? 3 : dtype == kF16 ? 2 : 1;
     LinearArgs p{static_cast<const __nv_bfloat16*>(ws), width, m, w, ms_pitch(k), ms_tiles_k(k) * ms_atoms(fmt), int(ms_tiles_k(k)), y, ldy, 1};
+    const bool few = m * parts <= 8;
     cudaError_t err = cudaSuccess;
     if (dtype == kF32) err = split<float, 3>(x, m, k, ldx, ws, width, stream);
     else if (dtype == kF16) err = split<__half, 2>(x, m, k, ldx, ws, width, stream);
-    else if (k != width || reinterpret_cast<uintptr_t>(x) % 16 || ldx % 8) err = split<__nv_bfloat16, 1>(x, m, k, ldx, ws, width, stream);
+    else if ((few && k != width) || reinterpret_cast<uintptr_t>(x) % 16 || ldx % 8) err = split<__nv_bfloat16, 1>(x, m, k, ldx, ws, width, stream);
     else { p.x = static_cast<const __nv_bfloat16*>(x); p.ldx = ldx; }
     if (err != cudaSuccess) return err;
-    const int sms = 148;
+    if (!few) return launch_ms_linear_many(p.x, p.ldx, p.x == ws ? width : k, m, parts, dtype, w, k, fmt, y, ldy, stream);
+    const int sms = ms_sm_count();
     if (dtype == kF32) return launch_fmt<float, 3>(p, fmt, sms, stream);
     if (dtype == kF16) return launch_fmt<__half, 2>(p, fmt, sms, stream);
     return launch_fmt<__nv_bfloat16, 1>(p, fmt, sms, stream);

@@ -1,0 +1,377 @@
+// Products of 16- and 32-bit activations with a 4-bit microscaled matrix, many tokens: y[i][r] = sum_c x[i][c] * W[r][c].
+//
+// Every value of W is a bf16 number, and x comes as m * P rows of bf16 parts (tcq_microscale_linear.cu), so the products are those of a bf16
+// matrix product.  128 rows of W are the left operand, in tensor memory: eight warps read 64 columns of codes at a time from shared memory,
+// make bf16 numbers of them (a thread one row) and store them there, so that neither the bf16 weights nor their reading takes any of
+// shared memory's bandwidth.  NT rows of x are the right operand, by TMA.
+//
+// Work split: one CTA per SM goes through tiles of 128 rows of W x NT rows of x.  One warp loads (codes and scales of 256 columns, x of 64),
+// one issues products, eight make weights (two groups of four take turns), four take finished sums out of tensor memory.  With few tokens a
+// cluster of S CTAs shares the columns of a tile; the partial sums meet through distributed shared memory, in rank order.
+//
+// A wait that runs out (kMbarWaitCycles) makes its CTA stop, and its results NaN.
+#include <algorithm>
+
+#include "tcq_microscale_weights.cuh"
+#include "tcq_tcgen05.cuh"
+
+namespace tcq {
+
+namespace {
+
+constexpr int kThreads = 32 * 14;                // loader, issuer, four warps for the results, eight that make weights
+constexpr int kRows = 128, kStepK = 64;          // rows of W; columns of a step
+constexpr int kMostSplits = 8;
+
+template <int FMT, int NT>
+struct Tile {
+    static constexpr int kAtoms = Ms<FMT>::kAtoms;
+    static constexpr int kBytesW = kRows * 128, kBytesS = kAtoms * 512, kStageW = kBytesW + 2048, kStagesW = 3;      // 256 columns
+    static constexpr int kBytesX = NT * 128;                                                                        // 64 columns
+    static constexpr int kStagesX = std::min(8, (220 * 1024 - kStagesW * kStageW) / kBytesX);
+    static constexpr int kSumBuffers = NT <= 128 ? 2 : 1, kSumColumns = NT < 32 ? 32 : NT;
+    static constexpr int kStagesA = 4, kColumnsA = kStepK / 2;                                                      // weights in tensor memory
+    static constexpr int kColumns = 512;
+    static constexpr int kBytes = (kStagesW * kStageW + 1023) / 1024 * 1024 + kStagesX * kBytesX;
+    static constexpr int kSmem = std::max(kBytes, 115 * 1024) + 1024;                                               // two CTAs never share an SM
+    static_assert(kSumBuffers * kSumColumns + kStagesA * kColumnsA <= 512 && kSmem <= 226 * 1024 && kStagesX >= 4);
+    static_assert(kStagesX * kBytesX >= NT * kRows * 4 || NT > 64, "the parts of a tile");
+};
+
+struct ManyArgs {
+    MsMatrix w;
+    long long m;                                 // tokens
+    int tiles_n, tiles_m, steps;                 // steps of 64 columns
+    long long atoms;                             // of scales a row group
+    void* y;
+    long long ldy;
+};
+
+__device__ __forceinline__ void mma_from_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(add)) : "memory");
+}
+__device__ __forceinline__ void tmem_store32(uint32_t tmem, const uint32_t (&v)[32]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+                 "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+                 ::"r"(tmem), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+                   "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
+                   "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
+                   "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]) : "memory");
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t smem) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(smem));
+    return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t smem) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(smem));
+    return v;
+}
+
+// The parts of a token, smallest first, as its sum.
+template <int P>
+__device__ __forceinline__ float whole_of(const float* v) {
+    if constexpr (P == 1) return v[0];
+    else if constexpr (P == 2) return v[1] * 0x1p-8f + v[0];
+    else return v[2] * 0x1p-16f + v[1] * 0x1p-8f + v[0];
+}
+
+template <typename YT, int FMT, int NT, int P>
+__global__ void __launch_bounds__(kThreads, 1) tcq_ms_linear_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+                                                                         const __grid_constant__ ManyArgs p) {
+    using T = Tile<FMT, NT>;
+    constexpr int kTokens = NT / P;                      // of a tile
+    extern __shared__ uint8_t raw[];
+    __shared__ uint64_t w_full[T::kStagesW], w_empty[T::kStagesW], x_full[T::kStagesX], x_empty[T::kStagesX], a_full[T::kStagesA], a_empty[T::kStagesA],
+        sum_full[T::kSumBuffers], sum_empty[T::kSumBuffers], drained;
+    __shared__ uint32_t tmem_at;
+    __shared__ unsigned int gave_up;
+    const uint32_t smem_w = (smem_u32(raw) + 1023) & ~1023u, smem_x = smem_w + (T::kStagesW * T::kStageW + 1023) / 1024 * 1024;
+    const int warp = __shfl_sync(0xFFFFFFFFu, int(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank(), splits = cluster_size();
+    const int all_tiles_k = (p.steps + 3) / 4;           // columns are shared in whole 256s
+    const int first = 4 * int((long long)all_tiles_k * rank / splits), last = min(4 * int((long long)all_tiles_k * (rank + 1) / splits), p.steps);
+    const int tiles = p.tiles_n * p.tiles_m, clusters = gridDim.x / splits;
+
+    if (warp == 0 && elect_one()) {
+        gave_up = 0;
+        for (int s = 0; s < T::kStagesW; ++s) { mbar_init(smem_u32(&w_full[s]), 1); mbar_init(smem_u32(&w_empty[s]), 8); }
+        for (int s = 0; s < T::kStagesX; ++s) { mbar_init(smem_u32(&x_full[s]), 1); mbar_init(smem_u32(&x_empty[s]), 1); }
+        for (int s = 0; s < T::kStagesA; ++s) { mbar_init(smem_u32(&a_full[s]), 4); mbar_init(smem_u32(&a_empty[s]), 1); }
+        for (int s = 0; s < T::kSumBuffers; ++s) { mbar_init(smem_u32(&sum_full[s]), 1); mbar_init(smem_u32(&sum_empty[s]), 4); }
+        mbar_init(smem_u32(&drained), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncwarp();
+    if (warp == 1) tmem_alloc(smem_u32(&tmem_at), T::kColumns);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_at, tmem_a = tmem + T::kSumBuffers * T::kSumColumns;
+
+    if (warp == 0) {
+        // ---- loads; the warp stays together, one lane issues
+        const bool one = elect_one();
+        uint32_t sw = 0, pw = 1, sx = 0, px = 1, loaded_w = 0, loaded_x = 0;      // (the first waits are for the phase before the first)
+        bool ok = true;
+        for (int t = blockIdx.x / splits; t < tiles && ok; t += clusters) {
+            const int tn = t / p.tiles_m, tm = t % p.tiles_m;
+            for (int step = first; step < last; ++step) {
+                if (step % 4 == 0) {
+                    ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&w_empty[sw]), pw, &gave_up));
+                    if (!ok) break;
+                    if (one) {
+                        const uint32_t to = smem_w + sw * T::kStageW, bar = smem_u32(&w_full[sw]);
+                        mbar_expect(bar, T::kBytesW + T::kBytesS);
+                        tma_load(to, &map_w, step * 32, tn * kRows, bar);
+                        bulk_load(to + T::kBytesW, p.w.scales + (tn * p.atoms + (long long)(step / 4) * T::kAtoms) * 512, T::kBytesS, bar);
+                    }
+                    __syncwarp();
+                    if (++sw == T::kStagesW) { sw = 0; pw ^= 1; }
+                    if (loaded_w < T::kStagesW) ++loaded_w;
+                }
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&x_empty[sx]), px, &gave_up));
+                if (!ok) break;
+                if (one) {
+                    mbar_expect(smem_u32(&x_full[sx]), T::kBytesX);
+                    tma_load(smem_x + sx * T::kBytesX, &map_x, step * kStepK, tm * kTokens * P, smem_u32(&x_full[sx]));
+                }
+                __syncwarp();
+                if (++sx == T::kStagesX) { sx = 0; px ^= 1; }
+                if (loaded_x < T::kStagesX) ++loaded_x;
+            }
+        }
+        if (gave_up) {                                   // nothing may be on its way to this CTA's memory when it ends: the last loads of each stage
+            for (uint32_t i = 0; i < loaded_w; ++i) {
+                if (sw == 0) pw ^= 1;
+                sw = sw == 0 ? T::kStagesW - 1 : sw - 1;
+                for (long long t0 = clock64(); !mbar_try_wait(smem_u32(&w_full[sw]), pw ^ 1) && clock64() - t0 < kMbarWaitCycles;) {}
+            }
+            for (uint32_t i = 0; i < loaded_x; ++i) {
+                if (sx == 0) px ^= 1;
+                sx = sx == 0 ? T::kStagesX - 1 : sx - 1;
+                for (long long t0 = clock64(); !mbar_try_wait(smem_u32(&x_full[sx]), px ^ 1) && clock64() - t0 < kMbarWaitCycles;) {}
+            }
+        }
+    } else if (warp == 1) {
+        // ---- products; likewise
+        constexpr uint32_t kIdesc = 1u << 4 | 1u << 7 | 1u << 10 | uint32_t(NT >> 3) << 17 | uint32_t(kRows >> 4) << 24;      // bf16 x bf16, fp32 sums
+        const bool one = elect_one();
+        uint32_t sx = 0, px = 0, sa = 0, pa = 0;
+        int n = 0;
+        bool ok = true;
+        for (int t = blockIdx.x / splits; t < tiles && ok; t += clusters, ++n) {
+            const int buf = n % T::kSumBuffers, use = n / T::kSumBuffers;
+            if (use > 0) ok = mbar_wait(smem_u32(&sum_empty[buf]), uint32_t(use - 1) & 1, &gave_up);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t d = tmem + buf * T::kSumColumns;
+            for (int step = first; step < last; ++step) {
+                ok = mbar_wait(smem_u32(&x_full[sx]), px, &gave_up) && mbar_wait(smem_u32(&a_full[sa]), pa, &gave_up);
+                ok = __all_sync(0xFFFFFFFFu, ok);        // every lane has seen these phases before the stages can be filled again
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t db = desc_rows128(smem_x + sx * T::kBytesX);
+                const uint32_t a = tmem_a + sa * T::kColumnsA;
+                if (one) {
+#pragma unroll
+                    for (int j = 0; j < kStepK / 16; ++j) mma_from_tmem(d, a + 8 * j, db + 2 * j, kIdesc, step > first || j > 0);
+                    tc_commit(smem_u32(&x_empty[sx]));
+                    tc_commit(smem_u32(&a_empty[sa]));
+                }
+                __syncwarp();
+                if (++sx == T::kStagesX) { sx = 0; px ^= 1; }
+                if (++sa == T::kStagesA) { sa = 0; pa ^= 1; }
+            }
+            if (ok && one) tc_commit(smem_u32(&sum_full[buf]));
+            __syncwarp();
+        }
+        if (!ok) {                                       // what was issued ends before the tensor memory goes
+            if (one) tc_commit(smem_u32(&drained));
+            __syncwarp();
+            for (long long t0 = clock64(); !mbar_try_wait(smem_u32(&drained), 0) && clock64() - t0 < kMbarWaitCycles;) {}
+        }
+    } else if (warp >= 6) {
+        // ---- weights: lane = row of this warp's quarter; the two groups of four warps take every other step
+        const int quarter = warp & 3, mine = (warp - 6) >> 2;
+        const int row = 32 * quarter + lane;
+        uint32_t sw = 0, pw = 0, sa = 0, pa = 1;
+        bool ok = true;
+        for (int t = blockIdx.x / splits; t < tiles && ok; t += clusters)
+            for (int step = first; step < last && ok; ++step) {
+                if (step % 4 == 0) ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&w_full[sw]), pw, &gave_up));
+                if ((step & 1) == mine && ok) {
+                    const uint32_t from = smem_w + sw * T::kStageW + row * 128, sub = step % 4;
+                    uint32_t word;
+                    const uint32_t scales = smem_w + sw * T::kStageW + T::kBytesW + lane * 16 + quarter * 4;
+                    if constexpr (FMT == kNvfp4) word = lds32(scales + 512 * sub);
+                    else word = lds32(scales + 512 * (sub / 2)) >> (16 * (sub & 1));
+                    uint32_t v[32];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {        // 16 bytes: 32 columns; the swizzle has put piece c of row r at c ^ (r % 8)
+                        const uint4 c = lds128(from + (((2 * sub + i) ^ (row & 7)) << 4));
+                        const uint32_t cw[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const __nv_bfloat162 s = scale_of<FMT>(word, 2 * i + j / 2);
+                            four_weights(cw[j], s, v[16 * i + 4 * j], v[16 * i + 4 * j + 1]);
+                            four_weights(cw[j] >> 16, s, v[16 * i + 4 * j + 2], v[16 * i + 4 * j + 3]);
+                        }
+                    }
+                    ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&a_empty[sa]), pa, &gave_up));
+                    if (ok) {
+                        tc_fence_after();
+                        tmem_store32(tmem_a + sa * T::kColumnsA + (uint32_t(32 * quarter) << 16), v);
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(smem_u32(&a_full[sa]));
+                    }
+                }
+                if (++sa == T::kStagesA) { sa = 0; pa ^= 1; }
+                if (step % 4 == 3 || step + 1 == last) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&w_empty[sw]));
+                    if (++sw == T::kStagesW) { sw = 0; pw ^= 1; }
+                }
+            }
+    } else {
+        // ---- results: this warp's lanes are 32 rows of W, so that a store is 32 neighbours in y
+        const int quarter = warp & 3;
+        constexpr int kChunk = NT < 32 ? NT : 32, kUsed = kChunk / P * P;            // columns loaded, and columns of whole tokens
+        int n = 0;
+        for (int t = blockIdx.x / splits; t < tiles; t += clusters, ++n) {
+            const int buf = n % T::kSumBuffers, use = n / T::kSumBuffers;
+            const long long r = (long long)(t / p.tiles_m) * kRows + 32 * quarter + lane, token0 = (long long)(t % p.tiles_m) * kTokens;
+            const float fw = FMT == kNvfp4 && r < p.w.rows ? p.w.row_scale[r] : 1.0f;
+            const bool ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sum_full[buf]), uint32_t(use) & 1, &gave_up));
+            tc_fence_after();
+            const uint32_t from = tmem + buf * T::kSumColumns + (uint32_t(32 * quarter) << 16);
+#pragma unroll 1
+            for (int c0 = 0; c0 < kTokens * P; c0 += kUsed) {
+                uint32_t v[kChunk];
+                tmem_load<kChunk>(from + c0, v);         // (the last chunk may reach into columns behind the sums; they are not used)
+                tmem_wait_ld();
+                float f[kChunk];
+#pragma unroll
+                for (int c = 0; c < kChunk; ++c) f[c] = ok ? __uint_as_float(v[c]) : __uint_as_float(0x7FC00000u);
+                if (splits > 1) {
+                    float* const part = reinterpret_cast<float*>(raw + (smem_x - smem_u32(raw))) + c0 * kRows + 32 * quarter + lane;
+#pragma unroll
+                    for (int c = 0; c < kUsed; ++c)
+                        if (c0 + c < kTokens * P) part[c * kRows] = f[c];
+                } else {
+                    const long long token = token0 + c0 / P;
+                    const int here = int(min((long long)kTokens, p.m - token0)) - c0 / P;
+                    YT* to = static_cast<YT*>(p.y) + token * p.ldy + r;
+#pragma unroll
+                    for (int i = 0; i < kUsed / P; ++i, to += p.ldy) {
+                        float whole = whole_of<P>(f + i * P);
+                        if constexpr (FMT == kNvfp4) whole *= fw;
+                        if (r < p.w.rows && i < here) *to = from_f32<YT>(whole);
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sum_empty[buf]));
+        }
+    }
+    __syncwarp();
+    if (splits > 1) {                                    // one tile a cluster: add up the parts of it
+        cluster_sync();
+        const int t = blockIdx.x / splits;
+        const long long r0 = (long long)(t / p.tiles_m) * kRows, token0 = (long long)(t % p.tiles_m) * kTokens;
+        const int tokens = int(min((long long)kTokens, p.m - token0));
+        for (int i = int(rank) * kThreads + threadIdx.x; i < kRows / 4 * tokens; i += int(splits) * kThreads) {
+            const int r4 = i % (kRows / 4), token = i / (kRows / 4);
+            const long long r = r0 + 4 * r4;
+            if (r >= p.w.rows) continue;
+            float sum[4][P];
+#pragma unroll
+            for (int q = 0; q < P; ++q) {
+                float4 part[kMostSplits];
+#pragma unroll
+                for (uint32_t s = 0; s < kMostSplits; ++s)
+                    if (s < splits) part[s] = ld_cluster_f32x4(smem_x + 16 * ((token * P + q) * (kRows / 4) + r4), s);
+                float4 f = part[0];
+#pragma unroll
+                for (uint32_t s = 1; s < kMostSplits; ++s)
+                    if (s < splits) f = make_float4(f.x + part[s].x, f.y + part[s].y, f.z + part[s].z, f.w + part[s].w);
+                sum[0][q] = f.x; sum[1][q] = f.y; sum[2][q] = f.z; sum[3][q] = f.w;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (r + j < p.w.rows) {
+                    float whole = whole_of<P>(sum[j]);
+                    if constexpr (FMT == kNvfp4) whole *= p.w.row_scale[r + j];
+                    static_cast<YT*>(p.y)[(token0 + token) * p.ldy + r + j] = from_f32<YT>(whole);
+                }
+        }
+        cluster_sync();                                  // no CTA ends while another reads its part
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_free(tmem, T::kColumns);
+    }
+}
+
+template <typename YT, int FMT, int NT, int P>
+cudaError_t launch(const __nv_bfloat16* x, long long ldx, long long width, long long m, const MsMatrix& w, long long k, void* y, long long ldy, int splits,
+                   cudaStream_t stream) {
+    using T = Tile<FMT, NT>;
+    static bool ready[64] = {};
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
+    if (err != cudaSuccess) return err;
+    if (dev >= 64 || !ready[dev]) {
+        if ((err = cudaFuncSetAttribute(tcq_ms_linear_many_kernel<YT, FMT, NT, P>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem)) != cudaSuccess) return err;
+        if (dev < 64) ready[dev] = true;
+    }
+    CUtensorMap map_w, map_x;
+    const long long pitch = ms_pitch(k), tokens = NT / P;
+    if ((err = make_byte_map(&map_w, w.codes, pitch, w.rows, pitch, kRows)) != cudaSuccess) return err;
+    if ((err = make_bf16_map(&map_x, x, width, m * P, ldx, NT)) != cudaSuccess) return err;
+    const ManyArgs p{w, m, int((w.rows + kRows - 1) / kRows), int((m + tokens - 1) / tokens), int((k + kStepK - 1) / kStepK), ms_tiles_k(k) * T::kAtoms, y, ldy};
+    const long long tiles = (long long)p.tiles_n * p.tiles_m;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(splits > 1 ? tiles * splits : std::min<long long>(tiles, ms_sm_count())));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = T::kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = unsigned(splits);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, tcq_ms_linear_many_kernel<YT, FMT, NT, P>, map_w, map_x, p);
+}
+
+template <typename YT, int FMT, int P>
+cudaError_t launch_fmt(const __nv_bfloat16* x, long long ldx, long long width, long long m, const MsMatrix& w, long long k, void* y, long long ldy, cudaStream_t stream) {
+    const long long rows = m * P, tiles = (w.rows + kRows - 1) / kRows, k_tiles = ms_tiles_k(k);
+    int splits = 1;
+    while (splits < kMostSplits && tiles * splits * 2 <= ms_sm_count() && splits * 2 <= k_tiles) splits *= 2;
+    if (rows <= 16 / P * P) return launch<YT, FMT, 16, P>(x, ldx, width, m, w, k, y, ldy, splits, stream);
+    if (rows <= 32 / P * P) return launch<YT, FMT, 32, P>(x, ldx, width, m, w, k, y, ldy, splits, stream);
+    if (rows <= 64 / P * P) return launch<YT, FMT, 64, P>(x, ldx, width, m, w, k, y, ldy, splits, stream);
+    if (tiles * ((rows + 255) / 256) * 2 <= ms_sm_count()) return launch<YT, FMT, 128, P>(x, ldx, width, m, w, k, y, ldy, 1, stream);
+    return launch<YT, FMT, 256, P>(x, ldx, width, m, w, k, y, ldy, 1, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_ms_linear_many(const __nv_bfloat16* x, long long ldx, long long width, long long m, int parts, int dtype, const MsMatrix& w, long long k,
+                                  int fmt, void* y, long long ldy, cudaStream_t stream) {
+    if (dtype == kF32) return fmt == kNvfp4 ? launch_fmt<float, kNvfp4, 3>(x, ldx, width, m, w, k, y, ldy, stream) : launch_fmt<float, kMxfp4, 3>(x, ldx, width, m, w, k, y, ldy, stream);
+    if (dtype == kF16) return fmt == kNvfp4 ? launch_fmt<__half, kNvfp4, 2>(x, ldx, width, m, w, k, y, ldy, stream) : launch_fmt<__half, kMxfp4, 2>(x, ldx, width, m, w, k, y, ldy, stream);
+    return fmt == kNvfp4 ? launch_fmt<__nv_bfloat16, kNvfp4, 1>(x, ldx, width, m, w, k, y, ldy, stream) : launch_fmt<__nv_bfloat16, kMxfp4, 1>(x, ldx, width, m, w, k, y, ldy, stream);
+}
+
+}  // namespace tcq

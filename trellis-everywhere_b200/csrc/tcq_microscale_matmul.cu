@@ -291,16 +291,6 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_matmul_kernel(const __grid
     }
 }
 
-int sm_count() {
-    static int cache[64] = {};
-    int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return 148;
-    if (dev < 64 && cache[dev]) return cache[dev];
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
-    if (dev < 64) cache[dev] = n;
-    return n;
-}
-
 template <int FMT, int NT>
 cudaError_t launch(const MsMatrix& x, const MsMatrix& w, long long k, void* y, int dtype, long long ldy, int splits, cudaStream_t stream) {
     using T = Tile<FMT, NT>;
@@ -321,7 +311,7 @@ cudaError_t launch(const MsMatrix& x, const MsMatrix& w, long long k, void* y, i
                        int(ms_tiles_k(k)), y, ldy, dtype, reinterpret_cast<uintptr_t>(y) % four == 0 && ldy % 4 == 0};
     const long long tiles = (long long)p.tiles_n * p.tiles_m;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(splits > 1 ? tiles * splits : std::min<long long>(tiles, sm_count())));
+    cfg.gridDim = dim3(unsigned(splits > 1 ? tiles * splits : std::min<long long>(tiles, ms_sm_count())));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = T::kSmem;
     cfg.stream = stream;
@@ -345,7 +335,7 @@ cudaError_t launch(const MsMatrix& x, const MsMatrix& w, long long k, void* y, i
 template <int FMT>
 cudaError_t launch_fmt(const MsMatrix& x, const MsMatrix& w, long long k, void* y, int dtype, long long ldy, cudaStream_t stream) {
     const long long m = x.rows, k_tiles = ms_tiles_k(k), tiles = (w.rows + kRowsW - 1) / kRowsW;
-    const int sms = sm_count();
+    const int sms = ms_sm_count();
     if (m > 128 || (m > 64 && tiles <= sms / 2 && k_tiles < 32)) {
         const long long pairs = sms / 2, tiles_m = (m + 255) / 256;
         const long long rounds128 = (tiles_m * tiles + pairs - 1) / pairs, rounds256 = (tiles_m * ((w.rows + 255) / 256) + pairs - 1) / pairs;
@@ -361,6 +351,16 @@ cudaError_t launch_fmt(const MsMatrix& x, const MsMatrix& w, long long k, void* 
 }
 
 }  // namespace
+
+int ms_sm_count() {
+    static int cache[64] = {};
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+    if (dev < 64 && cache[dev]) return cache[dev];
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+    if (dev < 64) cache[dev] = n;
+    return n;
+}
 
 namespace {
 cudaError_t encode_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, cuuint64_t width, cuuint64_t rows, cuuint64_t pitch, cuuint32_t box_width,
@@ -386,6 +386,10 @@ cudaError_t encode_map(CUtensorMap* map, CUtensorMapDataType type, const void* b
 
 cudaError_t make_byte_map(CUtensorMap* map, const void* base, long long width, long long rows, long long pitch, int box_rows) {
     return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, width, rows, pitch, 128, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+cudaError_t make_bf16_map(CUtensorMap* map, const void* base, long long width, long long rows, long long ld, int box_rows) {
+    return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, width, rows, 2 * ld, 64, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 cudaError_t make_scale_map(CUtensorMap* map, const void* base, long long rows, int box_rows) {
