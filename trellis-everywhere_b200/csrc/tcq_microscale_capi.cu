@@ -74,10 +74,11 @@ int tcq_ms_linear(const void* x, int dtype, int64_t m, int64_t ldx, const uint8_
     if (rc != TCQ_OK) return rc;
     if (n == 0 || m == 0) return TCQ_OK;
     if (k == 0 || ldx < k || ldy < n) return TCQ_E_BAD_ARGUMENT;
-    if (x == nullptr || y == nullptr || ws == nullptr) return TCQ_E_NULL_POINTER;
+    const bool direct = ms_linear_direct(x, dtype, k, ldx);
+    if (x == nullptr || y == nullptr || (ws == nullptr && !direct)) return TCQ_E_NULL_POINTER;
     if ((rc = check_ms_matrix(codes, scales, row_scale, format)) != TCQ_OK) return rc;
     if (misaligned(x, type_bytes(dtype)) || misaligned(y, type_bytes(dtype)) || misaligned(ws, 256)) return TCQ_E_MISALIGNED;
-    if (ws_bytes < ms_linear_workspace_bytes(m, k, dtype)) return TCQ_E_WORKSPACE;
+    if (!direct && ws_bytes < ms_linear_workspace_bytes(m, k, dtype)) return TCQ_E_WORKSPACE;
     cudaError_t err = launch_ms_linear(x, dtype, m, ldx, {codes, scales, row_scale, n}, k, format, y, ldy, ws, static_cast<cudaStream_t>(stream));
     return err == cudaSuccess ? TCQ_OK : report_cuda_error(err, "ms_linear");
 }

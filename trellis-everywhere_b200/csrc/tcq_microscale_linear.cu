@@ -181,6 +181,10 @@ cudaError_t split(const void* x, long long m, long long k, long long ldx, void* 
 cudaError_t launch_ms_linear_many(const __nv_bfloat16* x, long long ldx, long long width, long long m, int parts, int dtype, const MsMatrix& w, long long k,
                                   int fmt, void* y, long long ldy, cudaStream_t stream);
 
+bool ms_linear_direct(const void* x, int dtype, long long k, long long ldx) {
+    return dtype == kBf16 && k % kMsTileK == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 8 == 0;
+}
+
 size_t ms_linear_workspace_bytes(long long m, long long k, int dtype) {
     return size_t(m) * size_t(ms_tiles_k(k) * kMsTileK) * 2 * (dtype == kF32 ? 3 : dtype == kF16 ? 2 : 1);
 }
@@ -190,14 +194,14 @@ cudaError_t launch_ms_linear(const void* x, int dtype, long long m, long long ld
     const long long width = ms_tiles_k(k) * kMsTileK;
     const int parts = dtype == kF32 ? 3 : dtype == kF16 ? 2 : 1;
     LinearArgs p{static_cast<const __nv_bfloat16*>(ws), width, m, w, ms_pitch(k), ms_tiles_k(k) * ms_atoms(fmt), int(ms_tiles_k(k)), y, ldy, 1};
-    const bool few = m * parts <= 8;
+    const bool few = m * parts <= 8, direct = ms_linear_direct(x, dtype, k, ldx);
     cudaError_t err = cudaSuccess;
-    if (dtype == kF32) err = split<float, 3>(x, m, k, ldx, ws, width, stream);
+    if (direct) { p.x = static_cast<const __nv_bfloat16*>(x); p.ldx = ldx; }
+    else if (dtype == kF32) err = split<float, 3>(x, m, k, ldx, ws, width, stream);
     else if (dtype == kF16) err = split<__half, 2>(x, m, k, ldx, ws, width, stream);
-    else if ((few && k != width) || reinterpret_cast<uintptr_t>(x) % 16 || ldx % 8) err = split<__nv_bfloat16, 1>(x, m, k, ldx, ws, width, stream);
-    else { p.x = static_cast<const __nv_bfloat16*>(x); p.ldx = ldx; }
+    else err = split<__nv_bfloat16, 1>(x, m, k, ldx, ws, width, stream);
     if (err != cudaSuccess) return err;
-    if (!few) return launch_ms_linear_many(p.x, p.ldx, p.x == ws ? width : k, m, parts, dtype, w, k, fmt, y, ldy, stream);
+    if (!few) return launch_ms_linear_many(p.x, p.ldx, direct ? k : width, m, parts, dtype, w, k, fmt, y, ldy, stream);
     const int sms = ms_sm_count();
     if (dtype == kF32) return launch_fmt<float, 3>(p, fmt, sms, stream);
     if (dtype == kF16) return launch_fmt<__half, 2>(p, fmt, sms, stream);

@@ -11,6 +11,7 @@
 //
 // A wait that runs out (kMbarWaitCycles) makes its CTA stop, and its results NaN.
 #include <algorithm>
+#include <type_traits>
 
 #include "tcq_microscale_weights.cuh"
 #include "tcq_tcgen05.cuh"
@@ -19,7 +20,9 @@ namespace tcq {
 
 namespace {
 
-constexpr int kThreads = 32 * 14;                // loader, issuer, four warps for the results, eight that make weights
+// Warps: loader, issuer, four for the results, and groups of four that make weights.
+template <int P> constexpr int kMakers = 2;
+template <int P> constexpr int kThreads = 32 * (6 + 4 * kMakers<P>);
 constexpr int kRows = 128, kStepK = 64;          // rows of W; columns of a step
 constexpr int kMostSplits = 8;
 
@@ -79,8 +82,12 @@ __device__ __forceinline__ float whole_of(const float* v) {
     else return v[2] * 0x1p-16f + v[1] * 0x1p-8f + v[0];
 }
 
+// Steps whose sums stay in tensor memory.  The tensor cores cut sums off where fp32 arithmetic rounds, which over 12288 columns comes to 2.2e-6 of a
+// result; where that is all the error there is (fp32 results), 256 columns at a time are added up in registers instead (4e-7).
+template <int P> constexpr int kStepsHeld = P == 3 ? 4 : 1 << 29;
+
 template <typename YT, int FMT, int NT, int P>
-__global__ void __launch_bounds__(kThreads, 1) tcq_ms_linear_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+__global__ void __launch_bounds__(kThreads<P>, 1) tcq_ms_linear_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                                                                          const __grid_constant__ ManyArgs p) {
     using T = Tile<FMT, NT>;
     constexpr int kTokens = NT / P;                      // of a tile
@@ -98,7 +105,7 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_linear_many_kernel(const _
 
     if (warp == 0 && elect_one()) {
         gave_up = 0;
-        for (int s = 0; s < T::kStagesW; ++s) { mbar_init(smem_u32(&w_full[s]), 1); mbar_init(smem_u32(&w_empty[s]), 8); }
+        for (int s = 0; s < T::kStagesW; ++s) { mbar_init(smem_u32(&w_full[s]), 1); mbar_init(smem_u32(&w_empty[s]), 4 * kMakers<P>); }
         for (int s = 0; s < T::kStagesX; ++s) { mbar_init(smem_u32(&x_full[s]), 1); mbar_init(smem_u32(&x_empty[s]), 1); }
         for (int s = 0; s < T::kStagesA; ++s) { mbar_init(smem_u32(&a_full[s]), 4); mbar_init(smem_u32(&a_empty[s]), 1); }
         for (int s = 0; s < T::kSumBuffers; ++s) { mbar_init(smem_u32(&sum_full[s]), 1); mbar_init(smem_u32(&sum_empty[s]), 4); }
@@ -163,32 +170,34 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_linear_many_kernel(const _
         uint32_t sx = 0, px = 0, sa = 0, pa = 0;
         int n = 0;
         bool ok = true;
-        for (int t = blockIdx.x / splits; t < tiles && ok; t += clusters, ++n) {
-            const int buf = n % T::kSumBuffers, use = n / T::kSumBuffers;
-            if (use > 0) ok = mbar_wait(smem_u32(&sum_empty[buf]), uint32_t(use - 1) & 1, &gave_up);
-            ok = __all_sync(0xFFFFFFFFu, ok);
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t d = tmem + buf * T::kSumColumns;
-            for (int step = first; step < last; ++step) {
-                ok = mbar_wait(smem_u32(&x_full[sx]), px, &gave_up) && mbar_wait(smem_u32(&a_full[sa]), pa, &gave_up);
-                ok = __all_sync(0xFFFFFFFFu, ok);        // every lane has seen these phases before the stages can be filled again
+        for (int t = blockIdx.x / splits; t < tiles && ok; t += clusters) {
+            for (int from = first; from < last && ok; from += kStepsHeld<P>, ++n) {
+                const int buf = n % T::kSumBuffers, use = n / T::kSumBuffers, to = P == 3 ? min(from + kStepsHeld<P>, last) : last;
+                if (use > 0) ok = mbar_wait(smem_u32(&sum_empty[buf]), uint32_t(use - 1) & 1, &gave_up);
+                ok = __all_sync(0xFFFFFFFFu, ok);
                 if (!ok) break;
                 tc_fence_after();
-                const uint64_t db = desc_rows128(smem_x + sx * T::kBytesX);
-                const uint32_t a = tmem_a + sa * T::kColumnsA;
-                if (one) {
+                const uint32_t d = tmem + buf * T::kSumColumns;
+                for (int step = from; step < to; ++step) {
+                    ok = mbar_wait(smem_u32(&x_full[sx]), px, &gave_up) && mbar_wait(smem_u32(&a_full[sa]), pa, &gave_up);
+                    ok = __all_sync(0xFFFFFFFFu, ok);    // every lane has seen these phases before the stages can be filled again
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t db = desc_rows128(smem_x + sx * T::kBytesX);
+                    const uint32_t a = tmem_a + sa * T::kColumnsA;
+                    if (one) {
 #pragma unroll
-                    for (int j = 0; j < kStepK / 16; ++j) mma_from_tmem(d, a + 8 * j, db + 2 * j, kIdesc, step > first || j > 0);
-                    tc_commit(smem_u32(&x_empty[sx]));
-                    tc_commit(smem_u32(&a_empty[sa]));
+                        for (int j = 0; j < kStepK / 16; ++j) mma_from_tmem(d, a + 8 * j, db + 2 * j, kIdesc, step > from || j > 0);
+                        tc_commit(smem_u32(&x_empty[sx]));
+                        tc_commit(smem_u32(&a_empty[sa]));
+                    }
+                    __syncwarp();
+                    if (++sx == T::kStagesX) { sx = 0; px ^= 1; }
+                    if (++sa == T::kStagesA) { sa = 0; pa ^= 1; }
                 }
+                if (ok && one) tc_commit(smem_u32(&sum_full[buf]));
                 __syncwarp();
-                if (++sx == T::kStagesX) { sx = 0; px ^= 1; }
-                if (++sa == T::kStagesA) { sa = 0; pa ^= 1; }
             }
-            if (ok && one) tc_commit(smem_u32(&sum_full[buf]));
-            __syncwarp();
         }
         if (!ok) {                                       // what was issued ends before the tensor memory goes
             if (one) tc_commit(smem_u32(&drained));
@@ -196,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_linear_many_kernel(const _
             for (long long t0 = clock64(); !mbar_try_wait(smem_u32(&drained), 0) && clock64() - t0 < kMbarWaitCycles;) {}
         }
     } else if (warp >= 6) {
-        // ---- weights: lane = row of this warp's quarter; the two groups of four warps take every other step
+        // ---- weights: lane = row of this warp's quarter; the groups of four warps take turns
         const int quarter = warp & 3, mine = (warp - 6) >> 2;
         const int row = 32 * quarter + lane;
         uint32_t sw = 0, pw = 0, sa = 0, pa = 1;
@@ -204,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_linear_many_kernel(const _
         for (int t = blockIdx.x / splits; t < tiles && ok; t += clusters)
             for (int step = first; step < last && ok; ++step) {
                 if (step % 4 == 0) ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&w_full[sw]), pw, &gave_up));
-                if ((step & 1) == mine && ok) {
+                if (step % kMakers<P> == mine && ok) {
                     const uint32_t from = smem_w + sw * T::kStageW + row * 128, sub = step % 4;
                     uint32_t word;
                     const uint32_t scales = smem_w + sw * T::kStageW + T::kBytesW + lane * 16 + quarter * 4;
@@ -243,41 +252,67 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_linear_many_kernel(const _
         const int quarter = warp & 3;
         constexpr int kChunk = NT < 32 ? NT : 32, kUsed = kChunk / P * P;            // columns loaded, and columns of whole tokens
         int n = 0;
-        for (int t = blockIdx.x / splits; t < tiles; t += clusters, ++n) {
-            const int buf = n % T::kSumBuffers, use = n / T::kSumBuffers;
+        for (int t = blockIdx.x / splits; t < tiles; t += clusters) {
             const long long r = (long long)(t / p.tiles_m) * kRows + 32 * quarter + lane, token0 = (long long)(t % p.tiles_m) * kTokens;
             const float fw = FMT == kNvfp4 && r < p.w.rows ? p.w.row_scale[r] : 1.0f;
-            const bool ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sum_full[buf]), uint32_t(use) & 1, &gave_up));
-            tc_fence_after();
-            const uint32_t from = tmem + buf * T::kSumColumns + (uint32_t(32 * quarter) << 16);
-#pragma unroll 1
-            for (int c0 = 0; c0 < kTokens * P; c0 += kUsed) {
-                uint32_t v[kChunk];
-                tmem_load<kChunk>(from + c0, v);         // (the last chunk may reach into columns behind the sums; they are not used)
-                tmem_wait_ld();
-                float f[kChunk];
-#pragma unroll
-                for (int c = 0; c < kChunk; ++c) f[c] = ok ? __uint_as_float(v[c]) : __uint_as_float(0x7FC00000u);
+            const int here = int(min((long long)kTokens, p.m - token0));
+            float* const part = reinterpret_cast<float*>(raw + (smem_x - smem_u32(raw))) + 32 * quarter + lane;
+            YT* const y = static_cast<YT*>(p.y) + token0 * p.ldy + r;
+            // the finished columns c0 .. c0 + N - 1
+            auto finish = [&](const float* f, int c0, auto count) {
+                constexpr int N = decltype(count)::value;
                 if (splits > 1) {
-                    float* const part = reinterpret_cast<float*>(raw + (smem_x - smem_u32(raw))) + c0 * kRows + 32 * quarter + lane;
 #pragma unroll
-                    for (int c = 0; c < kUsed; ++c)
-                        if (c0 + c < kTokens * P) part[c * kRows] = f[c];
+                    for (int c = 0; c < N; ++c)
+                        if (c0 + c < kTokens * P) part[(c0 + c) * kRows] = f[c];
                 } else {
-                    const long long token = token0 + c0 / P;
-                    const int here = int(min((long long)kTokens, p.m - token0)) - c0 / P;
-                    YT* to = static_cast<YT*>(p.y) + token * p.ldy + r;
+                    YT* to = y + c0 / P * p.ldy;
 #pragma unroll
-                    for (int i = 0; i < kUsed / P; ++i, to += p.ldy) {
+                    for (int i = 0; i < N / P; ++i, to += p.ldy) {
                         float whole = whole_of<P>(f + i * P);
                         if constexpr (FMT == kNvfp4) whole *= fw;
-                        if (r < p.w.rows && i < here) *to = from_f32<YT>(whole);
+                        if (r < p.w.rows && c0 / P + i < here) *to = from_f32<YT>(whole);
                     }
                 }
+            };
+            if constexpr (P == 3) {
+                float acc[NT] = {};
+                for (int step = first; step < last; step += kStepsHeld<P>, ++n) {
+                    const int buf = n % T::kSumBuffers;
+                    const bool ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sum_full[buf]), uint32_t(n / T::kSumBuffers) & 1, &gave_up));
+                    tc_fence_after();
+#pragma unroll
+                    for (int c0 = 0; c0 < NT; c0 += kChunk) {
+                        uint32_t v[kChunk];
+                        tmem_load<kChunk>(tmem + buf * T::kSumColumns + c0 + (uint32_t(32 * quarter) << 16), v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int c = 0; c < kChunk; ++c) acc[c0 + c] += ok ? __uint_as_float(v[c]) : __uint_as_float(0x7FC00000u);
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&sum_empty[buf]));
+                }
+                finish(acc, 0, std::integral_constant<int, NT / P * P>{});
+            } else {
+                const int buf = n % T::kSumBuffers;
+                const bool ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sum_full[buf]), uint32_t(n / T::kSumBuffers) & 1, &gave_up));
+                ++n;
+                tc_fence_after();
+#pragma unroll 1
+                for (int c0 = 0; c0 < kTokens * P; c0 += kUsed) {
+                    uint32_t v[kChunk];
+                    tmem_load<kChunk>(tmem + buf * T::kSumColumns + c0 + (uint32_t(32 * quarter) << 16), v);
+                    tmem_wait_ld();
+                    float f[kChunk];
+#pragma unroll
+                    for (int c = 0; c < kChunk; ++c) f[c] = ok ? __uint_as_float(v[c]) : __uint_as_float(0x7FC00000u);
+                    finish(f, c0, std::integral_constant<int, kUsed>{});
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sum_empty[buf]));
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&sum_empty[buf]));
         }
     }
     __syncwarp();
@@ -286,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_linear_many_kernel(const _
         const int t = blockIdx.x / splits;
         const long long r0 = (long long)(t / p.tiles_m) * kRows, token0 = (long long)(t % p.tiles_m) * kTokens;
         const int tokens = int(min((long long)kTokens, p.m - token0));
-        for (int i = int(rank) * kThreads + threadIdx.x; i < kRows / 4 * tokens; i += int(splits) * kThreads) {
+        for (int i = int(rank) * kThreads<P> + threadIdx.x; i < kRows / 4 * tokens; i += int(splits) * kThreads<P>) {
             const int r4 = i % (kRows / 4), token = i / (kRows / 4);
             const long long r = r0 + 4 * r4;
             if (r >= p.w.rows) continue;
@@ -341,7 +376,7 @@ cudaError_t launch(const __nv_bfloat16* x, long long ldx, long long width, long 
     const long long tiles = (long long)p.tiles_n * p.tiles_m;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(splits > 1 ? tiles * splits : std::min<long long>(tiles, ms_sm_count())));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(kThreads<P>);
     cfg.dynamicSmemBytes = T::kSmem;
     cfg.stream = stream;
     cudaLaunchAttribute attr{};
@@ -360,9 +395,14 @@ cudaError_t launch_fmt(const __nv_bfloat16* x, long long ldx, long long width, l
     while (splits < kMostSplits && tiles * splits * 2 <= ms_sm_count() && splits * 2 <= k_tiles) splits *= 2;
     if (rows <= 16 / P * P) return launch<YT, FMT, 16, P>(x, ldx, width, m, w, k, y, ldy, splits, stream);
     if (rows <= 32 / P * P) return launch<YT, FMT, 32, P>(x, ldx, width, m, w, k, y, ldy, splits, stream);
+    if constexpr (P == 3) {             // sums in registers: no more than 64 columns
+        const long long tiles_m = (rows + 62) / 63;
+        return launch<YT, FMT, 64, P>(x, ldx, width, m, w, k, y, ldy, tiles * tiles_m * splits <= ms_sm_count() ? splits : 1, stream);
+    } else {
     if (rows <= 64 / P * P) return launch<YT, FMT, 64, P>(x, ldx, width, m, w, k, y, ldy, splits, stream);
     if (tiles * ((rows + 255) / 256) * 2 <= ms_sm_count()) return launch<YT, FMT, 128, P>(x, ldx, width, m, w, k, y, ldy, 1, stream);
     return launch<YT, FMT, 256, P>(x, ldx, width, m, w, k, y, ldy, 1, stream);
+    }
 }
 
 }  // namespace
