@@ -211,6 +211,22 @@ def test_linear_keeps_24_bits_of_fp32(ms):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", (torch.float16, torch.bfloat16))
+@pytest.mark.parametrize("m", (1, 3, 8, 9, 70))
+def test_activations_of_any_range(ms, fmt, dtype, m):
+    """Numbers over a type's whole range next to each other, one nonzero product a result: each is the product, rounded once."""
+    k = 512
+    g = torch.Generator().manual_seed(m)
+    codes, byte = torch.zeros(k, k, dtype=torch.int64), torch.full((k, k // P.BLOCK[fmt]), 127 if fmt == "mxfp4" else 0x38)
+    codes[torch.arange(k), torch.arange(k)] = 3                  # 1.5 on the diagonal
+    w = P.pack(codes, byte, None if fmt == "mxfp4" else torch.ones(k), fmt, "cuda")
+    lo, hi = (-24, 15) if dtype == torch.float16 else (-133, 126)
+    x = (torch.rand(m, k, generator=g) * torch.ldexp(torch.ones(m, k), torch.randint(lo, hi, (m, k), generator=g))).to(dtype)
+    x[0, :4] = torch.tensor([torch.finfo(dtype).tiny, -torch.finfo(dtype).tiny / 2, torch.finfo(dtype).max / 2, 0.0])
+    assert torch.equal(ms.linear(x.cuda(), w).cpu(), (x.double() * 1.5).to(dtype))
+
+
+@pytest.mark.parametrize("fmt", FMTS)
 def test_scales_at_the_ends_of_their_range(ms, fmt):
     """The smallest and the largest scales of a format, in the weights and (products of both) in the activations."""
     k, n, m = 64, 24, 3

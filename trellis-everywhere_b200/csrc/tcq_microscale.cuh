@@ -93,7 +93,7 @@ cudaError_t launch_ms_quantize(const void* x, int dtype, long long rows, long lo
 cudaError_t launch_ms_dequantize(const MsMatrix& q, long long k, int fmt, void* out, int dtype, long long ldo, cudaStream_t stream);
 cudaError_t launch_ms_linear(const void* x, int dtype, long long m, long long ldx, const MsMatrix& w, long long k, int fmt, void* y,
                              long long ldy, void* ws, cudaStream_t stream);
-bool ms_linear_direct(const void* x, int dtype, long long k, long long ldx);     // x is taken as it lies: no scratch
+bool ms_linear_direct(const void* x, int dtype, long long m, long long ldx);     // x is taken as it lies: no scratch
 size_t ms_linear_workspace_bytes(long long m, long long k, int dtype);
 cudaError_t launch_ms_matmul(const MsMatrix& x, const MsMatrix& w, long long k, int fmt, void* y, int dtype, long long ldy, cudaStream_t stream);
 

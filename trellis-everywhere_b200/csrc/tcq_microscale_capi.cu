@@ -74,7 +74,7 @@ int tcq_ms_linear(const void* x, int dtype, int64_t m, int64_t ldx, const uint8_
     if (rc != TCQ_OK) return rc;
     if (n == 0 || m == 0) return TCQ_OK;
     if (k == 0 || ldx < k || ldy < n) return TCQ_E_BAD_ARGUMENT;
-    const bool direct = ms_linear_direct(x, dtype, k, ldx);
+    const bool direct = ms_linear_direct(x, dtype, m, ldx);
     if (x == nullptr || y == nullptr || (ws == nullptr && !direct)) return TCQ_E_NULL_POINTER;
     if ((rc = check_ms_matrix(codes, scales, row_scale, format)) != TCQ_OK) return rc;
     if (misaligned(x, type_bytes(dtype)) || misaligned(y, type_bytes(dtype)) || misaligned(ws, 256)) return TCQ_E_MISALIGNED;

@@ -1,129 +1,388 @@
-// Products of 16- and 32-bit activations with a 4-bit microscaled matrix, few tokens: y[i][r] = sum_c x[i][c] * W[r][c].
+// Products of 16- and 32-bit activations with a 4-bit microscaled matrix, up to eight tokens: y[i][r] = sum_c x[i][c] * W[r][c].
 //
-// Every value of W is a bf16 number (two bits of e2m1 times at most four of a scale), and an fp16 or fp32 activation is the sum of two or
-// three of them (8 significant bits each, cut off, not rounded; each held times 2^8 more than the one before).  So all products are exact on the tensor cores' bf16 path, and x enters
-// as m * P rows of bf16: P = 1 (bf16), 2 (fp16), 3 (fp32), the parts of a token next to each other, added up at the end.
+// Codes become fp16 numbers (one conversion instruction a pair), so the products are those of mma.sync on fp16.  nvfp4: times the e4m3 scale, still an
+// fp16 number.  mxfp4: scales can lie outside fp16, so the sums of 32 columns are scaled instead.  x is cut into fp16 parts, 256 columns of
+// a token at a time: a power of two brings the largest magnitude under 2^15, eleven bits are cut off as fp16, and what is left is the next
+// part's, until nothing is left.  fp16 and bf16 activations nearly always take one part (nothing is left of numbers within 2^-31 of the
+// largest), fp32 three (2^-37); more are further rounds over the same codes.  So every product is exact, whatever the range.
+// (bf16 weights need no such care but three times the instructions a pair, which was the bound: 4 tokens through 151936 x 4096 136 us.)
 //
-// A warp takes 16 rows of W x 256 columns a step (mma.sync m16n8k16): lane (g, t) holds columns 64 t .. 64 t + 63 of two rows, which are 32
-// bytes of codes and one word of scales each; the order of the columns within a product is free as long as W and x agree, so four
-// consecutive codes are a lane's share of a 16-column product.  Two byte permutations look the four magnitudes up as the bytes of bf16 numbers,
-// one spreads the signs, one multiplication per pair brings the scale in.
-// The 16 rows are 4 x 4: rows 4 i .. 4 i + 3 of each 32 in a group of 128, whose scales are 64 neighbouring bytes.
-// Warps of a CTA share the columns; partial sums meet in shared memory, in a fixed order.  Sums within a step are the tensor core's, steps are
-// added in fp32 with rounding to nearest.
-#include "tcq_microscale_weights.cuh"
+// Work split: a CTA takes 128 rows of W, eight warps 16 rows each; one more warp loads 256 columns of codes (TMA) and scales at a time into a ring
+// of stages.  ldmatrix gives lane (g, t) the t-th eight codes of 32 columns of rows g and g + 8, two products' share.  x is converted
+// once where all columns of a CTA fit beside the stages, else a token a warp, for the next stage while this one is multiplied.  Where there are few groups of 128 rows a cluster of S CTAs
+// shares the columns, and the partial sums meet through distributed shared memory, in rank order.
+//
+// A wait that runs out (kMbarWaitCycles) makes its CTA's results NaN.
+#include <algorithm>
+
+#include "tcq_common.cuh"
+#include "tcq_microscale.cuh"
+#include "tcq_tcgen05.cuh"
 
 namespace tcq {
 
 namespace {
 
-constexpr int kWarps = 8, kThreads = 32 * kWarps;
+constexpr int kConsumers = 256, kThreads = kConsumers + 32, kRows = 128, kMostSplits = 8, kTokens = 8;
+constexpr int kPitchX = 576;                     // bytes of a token's 256 columns: 512 and a step to other banks
 
-struct LinearArgs {
-    const __nv_bfloat16* x;      // [virtual tokens][ldx], zeros behind column k up to a multiple of 256; 16-byte aligned rows
-    long long ldx;
-    long long m;                 // tokens
-    MsMatrix w;
-    long long pitch, atoms;      // bytes of codes a row; atoms of scales a row group
-    int k_tiles;
-    void* y;
-    long long ldy;
-    int warps_k;                 // warps that share a row group's columns: 1, 2, 4 or 8
+template <int FMT, int PARTS>
+struct Tile {
+    static constexpr int kAtoms = Ms<FMT>::kAtoms;
+    static constexpr int kBytesW = kRows * 128, kBytesS = kAtoms * 512, kStage = kBytesW + 2048;
+    static constexpr int kStages = 3;
+    static constexpr int kRowsX = 88;                                         // rows of 256 columns held: at least two times eight tokens' parts
+    static constexpr int kBytesSum = kTokens * kRows * 4;
+    static constexpr int kSmem = kStages * kStage + (kRowsX + 1) * kPitchX + kBytesSum + 1024;
+    static_assert(kSmem <= 113 * 1024 && kRowsX >= 2 * PARTS * kTokens);      // two CTAs an SM
 };
 
-__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+struct FewArgs {
+    const void* x;
+    long long ldx;
+    int m;
+    bool wide;                                   // x in pieces of 16 bytes
+    long long k;
+    MsMatrix w;
+    long long atoms;
+    int tiles, k_tiles;
+    void* y;
+    long long ldy;
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t smem, uint32_t (&v)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(smem) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t smem) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(smem) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t smem) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(smem) : "memory");
+    return v;
+}
+__device__ __forceinline__ void sts128(uint32_t smem, const uint32_t (&v)[4]) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(smem), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// Eight codes as four pairs of fp16 numbers, in order.
+__device__ __forceinline__ void eight_codes(uint32_t w, uint32_t (&h)[4]) {
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\tmov.b32 {b0, b1, b2, b3}, %4;\n\tcvt.rn.f16x2.e2m1x2 %0, b0;\n\tcvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, b2;\n\tcvt.rn.f16x2.e2m1x2 %3, b3;\n\t}" : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
+}
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+// Two e8m0 scales as bf16 numbers (2^-127 a denormal one, 255 NaN).
+__device__ __forceinline__ uint32_t e8m0x2_to_bf16x2(uint16_t v) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.ue8m0x2 %0, %1;" : "=r"(r) : "h"(v));
+    return r;
+}
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }      // -126 <= e <= 127
 
-// NT: groups of eight virtual tokens; P: of them per token.
-template <typename YT, int FMT, int NT, int P>
-__global__ void __launch_bounds__(kThreads) tcq_ms_linear_kernel(const __grid_constant__ LinearArgs p) {
-    constexpr int kTokens = 8 * NT / P;                  // of a pass
-    __shared__ float part[kWarps][16][8 * NT + 1];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int wk = warp % p.warps_k, local = warp / p.warps_k, groups = kWarps / p.warps_k;
-    const long long token0 = (long long)blockIdx.y * kTokens;
-    const long long row_groups = (p.w.rows + 127) / 128 * 8;
-    const long long virt = (p.m - token0 < kTokens ? p.m - token0 : kTokens) * P;
+// The next part of eight of a token's 256 columns (a warp has them all): fp16 numbers times the factor returned; r becomes what is left.
+__device__ __forceinline__ float next_part(float (&r)[8], uint32_t (&h)[4], bool& left) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t b = __float_as_uint(r[i]) & 0x7FFFFFFFu;
+        most = max(most, b < 0x7F800000u ? b : 0u);
+    }
+    most = __reduce_max_sync(0xFFFFFFFFu, most);
+    const int e = max(int(most >> 23), 1) - 127, up = most == 0 ? 0 : 14 - e;                 // largest finite magnitude below 2^15; -113 <= up <= 140
+    const float f0 = pow2f(up / 2), f1 = pow2f(up - up / 2), g0 = pow2f(-(up / 2)), g1 = pow2f(up / 2 - up);
+    left = false;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const __half a = __float2half_rz(r[i] * f0 * f1), b = __float2half_rz(r[i + 1] * f0 * f1);
+        h[i / 2] = uint32_t(__half_as_ushort(a)) | uint32_t(__half_as_ushort(b)) << 16;
+        const bool fine_a = (__float_as_uint(r[i]) & 0x7F800000u) != 0x7F800000u, fine_b = (__float_as_uint(r[i + 1]) & 0x7F800000u) != 0x7F800000u;
+        r[i] = fine_a ? r[i] - __half2float(a) * g0 * g1 : 0.0f;                              // exact: the bits that were cut off
+        r[i + 1] = fine_b ? r[i + 1] - __half2float(b) * g0 * g1 : 0.0f;
+        left = left || r[i] != 0.0f || r[i + 1] != 0.0f;
+    }
+    return g0 * g1;
+}
 
-    for (long long rg0 = (long long)blockIdx.x * groups; rg0 < row_groups; rg0 += (long long)gridDim.x * groups) {
-        const long long rg = rg0 + local;
-        float acc[NT][4] = {};
-        if (rg < row_groups) {
-            const long long group = rg >> 3;
-            const int r32 = int(rg & 7) * 4 + (g & 3), q0 = g >> 2;               // row 128 group + 32 q + r32, q = q0 and q0 + 2
-            const long long row[2] = {group * 128 + 32 * q0 + r32, group * 128 + 32 * (q0 + 2) + r32};
-            const uint8_t* codes[2];
+// Whether any of the 256 threads says so; all of them have arrived.
+__device__ __forceinline__ bool any_of_consumers(bool mine) {
+    uint32_t r;
+    __syncwarp();
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.aligned.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(r) : "r"(uint32_t(mine)), "n"(kConsumers) : "memory");
+    return r != 0;
+}
+
+// PARTS of x held at a time.
+template <typename T, int FMT, int PARTS>
+__global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ FewArgs p) {
+    using G = Tile<FMT, PARTS>;
+    extern __shared__ uint8_t raw[];
+    __shared__ uint64_t full[G::kStages], empty[G::kStages];
+    __shared__ float factor[G::kRowsX];
+    __shared__ unsigned int gave_up;
+    const uint32_t smem = (smem_u32(raw) + 1023) & ~1023u, smem_x = smem + G::kStages * G::kStage, zeros = smem_x + G::kRowsX * kPitchX, smem_sum = zeros + kPitchX;
+    float* const sums = reinterpret_cast<float*>(raw + (smem_sum - smem_u32(raw)));
+    const int warp = __shfl_sync(0xFFFFFFFFu, int(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank(), splits = cluster_size();
+    const int first = int((long long)p.k_tiles * rank / splits), last = int((long long)p.k_tiles * (rank + 1) / splits);
+    const int clusters = gridDim.x / splits;
+
+    auto load = [&](uint32_t s, int t, int kt) {
+        const uint32_t to = smem + s * G::kStage, bar = smem_u32(&full[s]);
+        mbar_expect(bar, G::kBytesW + G::kBytesS);
+        tma_load(to, &map_w, kt * 128, t * kRows, bar);
+        bulk_load(to + G::kBytesW, p.w.scales + (t * p.atoms + (long long)kt * G::kAtoms) * 512, G::kBytesS, bar);
+    };
+    // The first stages are on their way before anything else: a small call is little more than its latencies.
+    const int ahead = min(G::kStages, last - first);
+    if (warp == 8) {
+        if (elect_one()) {
+            gave_up = 0;
+            for (int s = 0; s < G::kStages; ++s) { mbar_init(smem_u32(&full[s]), 1); mbar_init(smem_u32(&empty[s]), 8); }
+            asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
+            for (int i = 0; i < ahead; ++i) load(i, blockIdx.x / splits, first + i);
+        }
+        __syncwarp();
+    }
+    __syncthreads();
+
+    if (warp == 8) {
+        // ---- loads; the warp stays together, one lane issues
+        const bool one = elect_one();
+        uint32_t s = ahead % G::kStages, phase = ahead == G::kStages ? 0 : 1, loaded = ahead;    // (the first wait for a stage is for the phase before the first)
+        bool ok = true;
+        int kt = first + ahead;
+        for (int t = blockIdx.x / splits; t < p.tiles && ok; t += clusters, kt = first)
+            for (; kt < last; ++kt) {
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&empty[s]), phase, &gave_up));
+                if (!ok) break;
+                if (one) load(s, t, kt);
+                __syncwarp();
+                if (++s == G::kStages) { s = 0; phase ^= 1; }
+                if (loaded < G::kStages) ++loaded;
+            }
+        if (gave_up)                                     // nothing may be on its way to this CTA's memory when it ends: the last loads of each stage
+            for (uint32_t i = 0; i < loaded; ++i) {
+                if (s == 0) phase ^= 1;
+                s = s == 0 ? G::kStages - 1 : s - 1;
+                for (long long t0 = clock64(); !mbar_try_wait(smem_u32(&full[s]), phase ^ 1) && clock64() - t0 < kMbarWaitCycles;) {}
+            }
+    } else {
+        const int g = lane >> 2, t4 = lane & 3;
+        const bool converts = warp < p.m;                // a warp converts a token's columns, eight a lane
+        float next[8], r[8];
+        auto fetch = [&](int kt, int token) {
+            if (token >= p.m) return;
+            const T* const x = static_cast<const T*>(p.x) + token * p.ldx;
+            const long long c = (long long)kt * kMsTileK + 8 * lane;
+            if (p.wide && c + 8 <= p.k) {
+                uint4 u[sizeof(T) / 2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) codes[h] = p.w.codes + (row[h] < p.w.rows ? row[h] : p.w.rows - 1) * p.pitch;
-            const uint8_t* const scales = p.w.scales + group * p.atoms * 512 + r32 * 16 + q0 * 4;
-            for (int kt = wk; kt < p.k_tiles; kt += p.warps_k) {
-                uint4 c[2][2];
-                uint32_t s[2];
+                for (int i = 0; i < int(sizeof(T) / 2); ++i) u[i] = __ldg(reinterpret_cast<const uint4*>(x + c) + i);
+                const T* const v = reinterpret_cast<const T*>(u);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int i = 0; i < 8; ++i) next[i] = to_f32<T>(v[i]);
+            } else {
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const long long at = (long long)kt * 128 + 32 * t + 16 * i;
-                        c[h][i] = at < p.pitch ? __ldg(reinterpret_cast<const uint4*>(codes[h] + at)) : make_uint4(0, 0, 0, 0);
+                for (int i = 0; i < 8; ++i) next[i] = c + i < p.k ? to_f32<T>(x[c + i]) : 0.0f;
+            }
+        };
+        // The rows of x: part q of token i of the n-th 256 columns held is row (n * PARTS + q) * m + i.  PARTS more parts of r into the n-th; whether
+        // something is left.
+        auto convert_one = [&](int n, int token) {
+            bool left = false;
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q) {
+                uint32_t h[4];
+                const float f = next_part(r, h, left);
+                const int row = (n * PARTS + q) * p.m + token;
+                sts128(smem_x + row * kPitchX + 16 * lane, h);
+                if (lane == 0) factor[row] = f;
+            }
+            return left;
+        };
+        auto convert = [&](int n) { return any_of_consumers(converts && convert_one(n, warp)); };
+        // tokens that there are not: zeros
+        if (threadIdx.x < 32) {
+            const uint32_t zero[4] = {};
+            sts128(zeros + 16 * lane, zero);
+        }
+        uint32_t s = 0, phase = 0;
+        // ldmatrix: lane l gives the address of row l % 16 of this warp's, piece l / 16 of two
+        const int lrow = 16 * warp + (lane & 15);
+        const uint32_t from_w = lrow * 128, piece = lane >> 4, swizzle = lrow & 7;
+        const int srow = 16 * warp + g;                  // rows whose scales this lane needs: srow, srow + 8
+        const uint32_t from_s = G::kBytesW + (srow & 31) * 16 + (srow >> 5) * 4;
+
+        // Where all of this CTA's columns fit, they are converted once, by all warps; unless that leaves something, which takes further rounds.
+        bool held = (last - first) * PARTS * p.m <= G::kRowsX;
+        if (held) {
+            bool left = false;
+            for (int i = warp; i < (last - first) * p.m; i += 8) {
+                fetch(first + i / p.m, i % p.m);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) r[j] = next[j];
+                left = convert_one(i / p.m, i % p.m) || left;
+            }
+            held = !any_of_consumers(left);
+        }
+
+        for (int tile = blockIdx.x / splits; tile < p.tiles; tile += clusters) {
+            float acc[4] = {}, low[4] = {};              // rows g (0, 1) and g + 8, tokens 2 t4 and 2 t4 + 1; what the sums' rounding left
+            int buf = 0;
+            bool more = false;
+            if (!held) {
+                fetch(first, warp);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) r[i] = next[i];
+                more = convert(0);
+            }
+            for (int kt = first; kt < last; ++kt) {
+                if (!held && kt + 1 < last) fetch(kt + 1, warp);
+                const bool ok = mbar_wait(smem_u32(&full[s]), phase, &gave_up);
+                __syncwarp();
+                const uint32_t stage = smem + s * G::kStage;
+                for (;;) {
+                    float sum[PARTS][4] = {};            // of 256 columns
+                    f32x2 scaled[PARTS][2] = {}, by[PARTS];       // mxfp4: the same by columns of one scale; factors of this lane's two tokens
+                    uint32_t from_x[PARTS];
+#pragma unroll
+                    for (int q = 0; q < PARTS; ++q) {
+                        const int row = ((held ? kt - first : buf) * PARTS + q) * p.m;
+                        by[q] = pack2(2 * t4 < p.m ? factor[row + 2 * t4] : 0.0f, 2 * t4 + 1 < p.m ? factor[row + 2 * t4 + 1] : 0.0f);
+                        from_x[q] = (g < p.m ? smem_x + (row + g) * kPitchX : zeros) + 16 * t4;
                     }
-                    if constexpr (FMT == kNvfp4) s[h] = __ldg(reinterpret_cast<const uint32_t*>(scales + ((long long)kt * 4 + t) * 512 + 8 * h));
-                    else s[h] = __ldg(reinterpret_cast<const uint16_t*>(scales + ((long long)kt * 2 + t / 2) * 512 + 8 * h + 2 * (t & 1)));
-                }
-                float sum[NT][4] = {};
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {            // 16 columns of each lane
-                    const __nv_bfloat162 s0 = scale_of<FMT>(s[0], q), s1 = scale_of<FMT>(s[1], q);
-                    uint4 b[NT][2];
+                    for (int c = 0; c < 8; c += 2) {     // 64 columns
+                        uint32_t w[4];                   // columns 32 c: rows g and g + 8; columns 32 (c + 1)
+                        ldmatrix4(stage + from_w + ((c + piece) ^ swizzle) * 16, w);
+                        uint32_t scale[2][2];            // [piece][row]; nvfp4: fp16 pairs, of this lane's half of 32 columns; mxfp4: fp32
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        const uint4* const from = reinterpret_cast<const uint4*>(p.x + (token0 * P + 8 * n + g) * p.ldx + (long long)kt * 256 + 64 * t + 16 * q);
+                        for (int h = 0; h < 2; ++h) {
+                            if constexpr (FMT == kNvfp4) {
+                                const uint32_t word = lds32(stage + from_s + 512 * (c / 2) + 128 * h);
+                                const uint32_t two = __byte_perm(word, 0u, t4 < 2 ? 0x4420 : 0x4431);
+                                uint32_t f;
+                                asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(f) : "r"(two));
+                                scale[0][h] = __byte_perm(f, f, 0x1010);
+                                scale[1][h] = __byte_perm(f, f, 0x3232);
+                            } else {
+                                const uint32_t word = lds32(stage + from_s + 512 * (c / 4) + 128 * h);
+                                const uint32_t f = e8m0x2_to_bf16x2(uint16_t(c % 4 ? word >> 16 : word));
+                                scale[0][h] = f << 16;
+                                scale[1][h] = f & 0xFFFF0000u;
+                            }
+                        }
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) b[n][i] = 8 * n + g < virt ? __ldg(from + i) : make_uint4(0, 0, 0, 0);
-                    }
+                        for (int i = 0; i < 2; ++i) {
+                            uint32_t a0[4], a1[4];
+                            eight_codes(w[2 * i], a0);
+                            eight_codes(w[2 * i + 1], a1);
+                            if constexpr (FMT == kNvfp4) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {        // four of them are a lane's share of a product
-                        const int word = q % 2 * 2 + j / 2;
-                        uint32_t a[4];
-                        const uint4 c0 = c[0][q / 2], c1 = c[1][q / 2];
-                        const uint32_t w0 = word == 0 ? c0.x : word == 1 ? c0.y : word == 2 ? c0.z : c0.w;
-                        const uint32_t w1 = word == 0 ? c1.x : word == 1 ? c1.y : word == 2 ? c1.z : c1.w;
-                        four_weights(j & 1 ? w0 >> 16 : w0, s0, a[0], a[2]);
-                        four_weights(j & 1 ? w1 >> 16 : w1, s1, a[1], a[3]);
+                                for (int j = 0; j < 4; ++j) { a0[j] = mul_f16x2(a0[j], scale[i][0]); a1[j] = mul_f16x2(a1[j], scale[i][1]); }
+                            }
+                            const uint32_t lo[4] = {a0[0], a1[0], a0[1], a1[1]}, hi[4] = {a0[2], a1[2], a0[3], a1[3]};
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            const uint4 v = b[n][j / 2];
-                            mma_bf16(sum[n], a, j & 1 ? v.z : v.x, j & 1 ? v.w : v.y);
+                            for (int q = 0; q < PARTS; ++q) {
+                                const uint4 b = lds128(from_x[q] + 64 * (c + i));
+                                if constexpr (FMT == kNvfp4) {
+                                    mma_f16(sum[q], lo, b.x, b.y);
+                                    mma_f16(sum[q], hi, b.z, b.w);
+                                } else {
+                                    float d[4] = {};
+                                    mma_f16(d, lo, b.x, b.y);
+                                    mma_f16(d, hi, b.z, b.w);
+                                    const float s0 = __uint_as_float(scale[i][0]), s1 = __uint_as_float(scale[i][1]);
+                                    scaled[q][0] = fma2(mul2(pack2(d[0], d[1]), by[q]), pack2(s0, s0), scaled[q][0]);
+                                    scaled[q][1] = fma2(mul2(pack2(d[2], d[3]), by[q]), pack2(s1, s1), scaled[q][1]);
+                                }
+                            }
                         }
                     }
+                    // Parts of one number meet here: added with what each addition's rounding leaves, so that the number is whole again.
+#pragma unroll
+                    for (int q = 0; q < PARTS; ++q) {
+                        if constexpr (FMT == kNvfp4) {
+                            scaled[q][0] = mul2(pack2(sum[q][0], sum[q][1]), by[q]);
+                            scaled[q][1] = mul2(pack2(sum[q][2], sum[q][3]), by[q]);
+                        }
+                        float v[4];
+                        unpack2(scaled[q][0], v[0], v[1]);
+                        unpack2(scaled[q][1], v[2], v[3]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float total = acc[i] + v[i], was = total - acc[i];
+                            low[i] += (acc[i] - (total - was)) + (v[i] - was);
+                            acc[i] = total;
+                        }
+                    }
+                    if (!more) break;
+                    any_of_consumers(false);             // all have read this buffer: the next parts
+                    more = convert(buf);
                 }
+                if (!ok) acc[0] = acc[1] = acc[2] = acc[3] = __uint_as_float(0x7FC00000u);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&empty[s]));
+                if (++s == G::kStages) { s = 0; phase ^= 1; }
+                if (!held && kt + 1 < last) {
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                    for (int i = 0; i < 8; ++i) r[i] = next[i];
+                    buf ^= 1;
+                    more = convert(buf);
+                }
+            }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[n][i] += sum[n][i];
+            for (int i = 0; i < 4; ++i)                  // (an infinite or NaN sum leaves NaN behind)
+                sums[(2 * t4 + (i & 1)) * kRows + 16 * warp + g + 8 * (i >> 1)] = fabsf(low[i]) < __uint_as_float(0x7F800000u) ? acc[i] + low[i] : acc[i];
+            if (splits == 1) {
+                any_of_consumers(false);
+                for (int i = threadIdx.x; i < p.m * kRows; i += kConsumers) {
+                    const long long row = (long long)tile * kRows + i % kRows;
+                    if (row < p.w.rows) {
+                        float f = sums[i];
+                        if constexpr (FMT == kNvfp4) f *= p.w.row_scale[row];
+                        static_cast<T*>(p.y)[i / kRows * p.ldy + row] = from_f32<T>(f);
+                    }
+                }
+                any_of_consumers(false);                 // before the next rows' sums
             }
         }
-        __syncthreads();                                 // (the previous row groups' sums have been read)
+    }
+    __syncwarp();
+    if (splits > 1) {                                    // one group of rows a cluster: add up the parts of it
+        cluster_sync();
+        const long long row0 = (long long)(blockIdx.x / splits) * kRows;
+        for (int i = int(rank) * kThreads + threadIdx.x; i < p.m * (kRows / 4); i += int(splits) * kThreads) {
+            const long long row = row0 + 4 * (i % (kRows / 4));
+            if (row >= p.w.rows) continue;
+            float4 part[kMostSplits];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+            for (uint32_t q = 0; q < kMostSplits; ++q)
+                if (q < splits) part[q] = ld_cluster_f32x4(smem_sum + 16 * i, q);
+            float4 f = part[0];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) part[warp][g + 8 * (i >> 1)][8 * n + 2 * t + (i & 1)] = acc[n][i];
-        __syncthreads();
-        for (int i = threadIdx.x; i < groups * 16 * kTokens; i += kThreads) {
-            const int r16 = i & 15, token = i / 16 % kTokens, lg = i / 16 / kTokens;
-            const long long group_of = rg0 + lg, r = (group_of >> 3) * 128 + 32 * (r16 >> 2) + (group_of & 7) * 4 + (r16 & 3);
-            if (group_of >= row_groups || r >= p.w.rows || token0 + token >= p.m) continue;
-            float f = 0.0f;
+            for (uint32_t q = 1; q < kMostSplits; ++q)
+                if (q < splits) f = make_float4(f.x + part[q].x, f.y + part[q].y, f.z + part[q].z, f.w + part[q].w);
+            const float e[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
-            for (int q = P - 1; q >= 0; --q) {           // the smallest parts first
-                float one = 0.0f;
-                for (int v = 0; v < p.warps_k; ++v) one += part[lg * p.warps_k + v][r16][token * P + q];
-                f += q == 2 ? one * 0x1p-16f : q == 1 ? one * 0x1p-8f : one;
-            }
-            if constexpr (FMT == kNvfp4) f *= p.w.row_scale[r];
-            static_cast<YT*>(p.y)[(token0 + token) * p.ldy + r] = from_f32<YT>(f);
+            for (int j = 0; j < 4; ++j)
+                if (row + j < p.w.rows) {
+                    float one = e[j];
+                    if constexpr (FMT == kNvfp4) one *= p.w.row_scale[row + j];
+                    static_cast<T*>(p.y)[i / (kRows / 4) * p.ldy + row + j] = from_f32<T>(one);
+                }
         }
+        cluster_sync();                                  // no CTA ends while another reads its part
     }
 }
 
@@ -152,27 +411,52 @@ __global__ void __launch_bounds__(256) tcq_ms_parts_kernel(const T* __restrict__
     }
 }
 
-template <typename YT, int FMT, int NT, int P>
-cudaError_t launch(LinearArgs p, int sms, cudaStream_t stream) {
-    constexpr int kTokens = 8 * NT / P;
-    const long long row_groups = (p.w.rows + 127) / 128 * 8;
-    p.warps_k = 8;
-    while (p.warps_k > 1 && p.warps_k > p.k_tiles) p.warps_k /= 2;
-    const long long want = (row_groups + kWarps / p.warps_k - 1) / (kWarps / p.warps_k);
-    const dim3 grid(unsigned(want < 8ll * sms ? want : 8ll * sms), unsigned((p.m + kTokens - 1) / kTokens));
-    tcq_ms_linear_kernel<YT, FMT, NT, P><<<grid, kThreads, 0, stream>>>(p);
-    return cudaGetLastError();
-}
-
-template <typename YT, int P>
-cudaError_t launch_fmt(const LinearArgs& p, int fmt, int sms, cudaStream_t stream) {
-    return fmt == kNvfp4 ? launch<YT, kNvfp4, 1, P>(p, sms, stream) : launch<YT, kMxfp4, 1, P>(p, sms, stream);
-}
-
 template <typename T, int P>
 cudaError_t split(const void* x, long long m, long long k, long long ldx, void* ws, long long width, cudaStream_t stream) {
     tcq_ms_parts_kernel<T, P><<<unsigned((m * (width / 8) + 255) / 256), 256, 0, stream>>>(static_cast<const T*>(x), m, k, ldx, static_cast<__nv_bfloat16*>(ws), width);
     return cudaGetLastError();
+}
+
+template <typename T, int FMT, int PARTS>
+cudaError_t launch(FewArgs p, cudaStream_t stream) {
+    using G = Tile<FMT, PARTS>;
+    static bool ready[64] = {};
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
+    if (err != cudaSuccess) return err;
+    if (dev >= 64 || !ready[dev]) {
+        if ((err = cudaFuncSetAttribute(tcq_ms_linear_few_kernel<T, FMT, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmem)) != cudaSuccess) return err;
+        if (dev < 64) ready[dev] = true;
+    }
+    CUtensorMap map_w;
+    const long long pitch = ms_pitch(p.k);
+    if ((err = make_byte_map(&map_w, p.w.codes, pitch, p.w.rows, pitch, kRows)) != cudaSuccess) return err;
+    p.wide = reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && p.ldx * sizeof(T) % 16 == 0;
+    p.atoms = ms_tiles_k(p.k) * G::kAtoms;
+    p.tiles = int((p.w.rows + kRows - 1) / kRows);
+    p.k_tiles = int(ms_tiles_k(p.k));
+    // S, a power of two (clusters of three and five run 20 % longer than of two and four), while all CTAs run at once.  us, nvfp4, one token, S = 1 / 2 / 4 / 8:
+    // 4096 x 4096 14.2 / 9.1 / 6.8 / 6.5, 4096 x 12288 37.5 / 20.9 / 12.5 / 10.9, 12288 x 4096 14.6 / 12.9
+    const int slots = 2 * ms_sm_count();
+    int splits = 1;
+    while (splits < kMostSplits && splits * 2 <= p.k_tiles && p.tiles * splits * 2 <= slots) splits *= 2;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(splits > 1 ? p.tiles * splits : std::min(p.tiles, slots)));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = G::kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = unsigned(splits);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, tcq_ms_linear_few_kernel<T, FMT, PARTS>, map_w, p);
+}
+
+template <typename T, int PARTS>
+cudaError_t launch_fmt(const FewArgs& p, int fmt, cudaStream_t stream) {
+    return fmt == kNvfp4 ? launch<T, kNvfp4, PARTS>(p, stream) : launch<T, kMxfp4, PARTS>(p, stream);
 }
 
 }  // namespace
@@ -181,8 +465,9 @@ cudaError_t split(const void* x, long long m, long long k, long long ldx, void* 
 cudaError_t launch_ms_linear_many(const __nv_bfloat16* x, long long ldx, long long width, long long m, int parts, int dtype, const MsMatrix& w, long long k,
                                   int fmt, void* y, long long ldy, cudaStream_t stream);
 
-bool ms_linear_direct(const void* x, int dtype, long long k, long long ldx) {
-    return dtype == kBf16 && k % kMsTileK == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 8 == 0;
+// Whether x is taken as it lies, with no scratch: few tokens, or bf16 rows that a TMA load can start at.
+bool ms_linear_direct(const void* x, int dtype, long long m, long long ldx) {
+    return m <= kTokens || (dtype == kBf16 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 8 == 0);
 }
 
 size_t ms_linear_workspace_bytes(long long m, long long k, int dtype) {
@@ -191,21 +476,21 @@ size_t ms_linear_workspace_bytes(long long m, long long k, int dtype) {
 
 cudaError_t launch_ms_linear(const void* x, int dtype, long long m, long long ldx, const MsMatrix& w, long long k, int fmt, void* y,
                              long long ldy, void* ws, cudaStream_t stream) {
+    if (m <= kTokens) {
+        const FewArgs p{x, ldx, int(m), false, k, w, 0, 0, 0, y, ldy};
+        if (dtype == kF32) return launch_fmt<float, 3>(p, fmt, stream);
+        if (dtype == kF16) return launch_fmt<__half, 1>(p, fmt, stream);
+        return launch_fmt<__nv_bfloat16, 1>(p, fmt, stream);
+    }
     const long long width = ms_tiles_k(k) * kMsTileK;
     const int parts = dtype == kF32 ? 3 : dtype == kF16 ? 2 : 1;
-    LinearArgs p{static_cast<const __nv_bfloat16*>(ws), width, m, w, ms_pitch(k), ms_tiles_k(k) * ms_atoms(fmt), int(ms_tiles_k(k)), y, ldy, 1};
-    const bool few = m * parts <= 8, direct = ms_linear_direct(x, dtype, k, ldx);
-    cudaError_t err = cudaSuccess;
-    if (direct) { p.x = static_cast<const __nv_bfloat16*>(x); p.ldx = ldx; }
-    else if (dtype == kF32) err = split<float, 3>(x, m, k, ldx, ws, width, stream);
+    if (ms_linear_direct(x, dtype, m, ldx)) return launch_ms_linear_many(static_cast<const __nv_bfloat16*>(x), ldx, k, m, parts, dtype, w, k, fmt, y, ldy, stream);
+    cudaError_t err;
+    if (dtype == kF32) err = split<float, 3>(x, m, k, ldx, ws, width, stream);
     else if (dtype == kF16) err = split<__half, 2>(x, m, k, ldx, ws, width, stream);
     else err = split<__nv_bfloat16, 1>(x, m, k, ldx, ws, width, stream);
     if (err != cudaSuccess) return err;
-    if (!few) return launch_ms_linear_many(p.x, p.ldx, direct ? k : width, m, parts, dtype, w, k, fmt, y, ldy, stream);
-    const int sms = ms_sm_count();
-    if (dtype == kF32) return launch_fmt<float, 3>(p, fmt, sms, stream);
-    if (dtype == kF16) return launch_fmt<__half, 2>(p, fmt, sms, stream);
-    return launch_fmt<__nv_bfloat16, 1>(p, fmt, sms, stream);
+    return launch_ms_linear_many(static_cast<const __nv_bfloat16*>(ws), width, width, m, parts, dtype, w, k, fmt, y, ldy, stream);
 }
 
 }  // namespace tcq
