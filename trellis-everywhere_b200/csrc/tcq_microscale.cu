@@ -7,6 +7,9 @@
 // rounded, is on a border between two codes (a number of at most four bits) only where the real one is.  (For x near t d, both on
 // grids no finer than ulp(x), |x / d - t| >= ulp(x) / d, which is more than half an ulp of t.)  The same holds for amax / 6 and e4m3.
 // A block with a NaN or an infinity gets the scale NaN and codes 0, and counts for nothing in the row's largest value.
+#include <algorithm>
+
+#include "tcq_common.cuh"
 #include "tcq_microscale.cuh"
 
 namespace tcq {
@@ -37,11 +40,30 @@ __device__ __forceinline__ void load_run(const T* __restrict__ row, long long c0
     }
 }
 
+__device__ __forceinline__ void load_signs(const float* __restrict__ signs, long long c0, long long k, bool wide, float (&v)[kRun]) {
+    if (wide && c0 + kRun <= k) {
+#pragma unroll
+        for (int q = 0; q < kRun / 4; ++q) {
+            const float4 u = __ldg(reinterpret_cast<const float4*>(signs + c0) + q);
+            v[4 * q] = u.x; v[4 * q + 1] = u.y; v[4 * q + 2] = u.z; v[4 * q + 3] = u.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) v[i] = c0 + i < k ? signs[c0 + i] : 1.0f;
+    }
+}
+
+// One stage of the transform between lanes h apart.
+__device__ __forceinline__ void rotate_lanes(float (&v)[kRun], int h) {
+    const float sign = threadIdx.x & h ? -1.0f : 1.0f;
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) v[i] = __fmaf_rn(v[i], sign, __shfl_xor_sync(0xFFFFFFFFu, v[i], h));
+}
 // Signs, then the transform of every b = `rotate` columns: the first four stages within the thread, the others between neighbouring lanes.
 // b divides k, and all lanes of a group of b / 16 take part.
-__device__ __forceinline__ void rotate_run(float (&v)[kRun], const float* __restrict__ signs, long long c0, long long k, int rotate) {
+__device__ __forceinline__ void rotate_run(float (&v)[kRun], const float (&signs)[kRun], int rotate) {
 #pragma unroll
-    for (int i = 0; i < kRun; ++i) v[i] *= c0 + i < k ? signs[c0 + i] : 1.0f;
+    for (int i = 0; i < kRun; ++i) v[i] *= signs[i];
 #pragma unroll
     for (int h = 1; h < kRun; h *= 2)
 #pragma unroll
@@ -51,14 +73,9 @@ __device__ __forceinline__ void rotate_run(float (&v)[kRun], const float* __rest
                 v[i] = a + b;
                 v[i + h] = a - b;
             }
-    for (int h = 1; h < rotate / kRun; h *= 2) {
-        const bool upper = threadIdx.x & h;
-#pragma unroll
-        for (int i = 0; i < kRun; ++i) {
-            const float o = __shfl_xor_sync(0xFFFFFFFFu, v[i], h);
-            v[i] = upper ? o - v[i] : v[i] + o;
-        }
-    }
+    if (rotate >= 32) rotate_lanes(v, 1);
+    if (rotate >= 64) rotate_lanes(v, 2);
+    if (rotate >= 128) rotate_lanes(v, 4);
     const float scale = rotate == 16 ? 0.25f : rotate == 32 ? 0.17677669529663687f : rotate == 64 ? 0.125f : 0.08838834764831845f;
 #pragma unroll
     for (int i = 0; i < kRun; ++i) v[i] *= scale;
@@ -101,62 +118,179 @@ __device__ __forceinline__ uint2 codes_of(const float (&q)[kRun]) {
     return make_uint2(w[0], w[1]);
 }
 
-// One CTA a row (nvfp4 needs the row's largest value first); a thread takes 16 columns at a time.  Columns up to the next multiple of 256
-// are worked on as zeros, so that the storage behind column k is written.
+// A row's largest finite magnitude so far, as bits.
+__device__ __forceinline__ uint32_t row_largest(const float (&v)[kRun]) {
+    const uint32_t m = largest_bits(v);
+    return m < 0x7F800000u ? m : largest_finite_bits(v);
+}
+
+// A run's codes and scale byte out of its values; j: the row scale's exponent (nvfp4).  Lanes 2 i and 2 i + 1 have the halves of an mxfp4 block.
+// nvfp4's quotients, by s and by 6: one step from a product with the correctly rounded reciprocal, which gives the correctly rounded quotient
+// (Markstein; checked for all mantissas of x and all eight of s, 6 = 1.5 * 4 among them).
+template <int FMT>
+__device__ __forceinline__ uint2 quantize_run(float (&v)[kRun], int j, uint32_t& byte) {
+    uint32_t m = largest_bits(v);
+    if constexpr (FMT == kNvfp4) {
+        const float t = __uint_as_float(m) * pow2(-j), sixth = 0x1.555556p-3f, q6 = t * sixth;
+        byte = m < 0x7F800000u ? f32_to_e4m3(__fmaf_rn(__fmaf_rn(q6, -6.0f, t), sixth, q6)) : 0x7Fu;
+        const float s = e4m3_to_f32(byte), r = s > 0.0f ? __frcp_rn(s) * pow2(-j) : 0.0f, by = -s * pow2(j);
+        const f32x2 r2 = pack2(r, r), by2 = pack2(by, by);
+#pragma unroll
+        for (int i = 0; i < kRun; i += 2) {
+            const f32x2 x = pack2(v[i], v[i + 1]), q = mul2(x, r2);
+            float a, b;
+            unpack2(fma2(fma2(q, by2, x), r2, q), a, b);
+            v[i] = __uint_as_float(__float_as_uint(a) | (__float_as_uint(v[i]) & 0x80000000u));          // (the sum of two zeros has lost a sign)
+            v[i + 1] = __uint_as_float(__float_as_uint(b) | (__float_as_uint(v[i + 1]) & 0x80000000u));
+        }
+    } else {
+        m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+        const int e = m == 0 ? -127 : max(int(m >> 23) - 127 - 2, -127);
+        byte = m < 0x7F800000u ? uint32_t(e + 127) : 0xFFu;
+        const float inv = e <= -127 ? 1.7014118346046923e38f : pow2(-e);
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) v[i] *= inv;
+    }
+    if (m >= 0x7F800000u) {
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) v[i] = 0.0f;
+    }
+    return codes_of(v);
+}
+
+// Codes and scales of the run of columns c0 ... to their places.  The scales of four blocks are one word, which the first of their lanes stores.
+template <int FMT>
+__device__ __forceinline__ void store_run(long long r, bool row_is, long long c0, long long k, long long span, uint2 code, uint32_t byte, uint8_t* __restrict__ codes,
+                                          long long pitch, uint8_t* __restrict__ scales, long long atoms) {
+    constexpr int kLanes = FMT == kNvfp4 ? 1 : 2;        // of a block
+    uint32_t word = (c0 < k ? byte : 0u) << (8 * (threadIdx.x / kLanes & 3));
+    word |= __shfl_xor_sync(0xFFFFFFFFu, word, kLanes);
+    word |= __shfl_xor_sync(0xFFFFFFFFu, word, 2 * kLanes);
+    if (!row_is) return;
+    if (c0 < 2 * pitch) *reinterpret_cast<uint2*>(codes + r * pitch + c0 / 2) = code;
+    if (c0 < span && threadIdx.x % (4 * kLanes) == 0) *reinterpret_cast<uint32_t*>(scales + ms_scale_at(r, int(c0 / Ms<FMT>::kBlock), atoms)) = word;
+}
+
+struct QuantizeArgs {
+    long long rows, k, ldx;
+    bool wide;                                           // rows of x start on 16 bytes
+    int rotate;
+    const float* signs;
+    bool wide_signs;
+    uint8_t* codes;
+    long long pitch;
+    uint8_t* scales;
+    long long atoms;
+    float* row_scale;
+    int lanes;                                           // threads of a row
+};
+
+// `lanes` threads a row, RUNS runs of 16 columns each, blockDim / lanes rows a CTA at a time; a row is read once (the next one while this one is
+// worked on) and stays in registers.  Columns up to the next multiple of 256 are worked on as zeros, so that the storage behind column k is
+// written.  The factors of a rotation are a thread's own for all its rows.
+template <typename T, int FMT, int RUNS, bool ROTATED>
+__global__ void __launch_bounds__(1024) tcq_ms_quantize_kernel(const T* __restrict__ x, const __grid_constant__ QuantizeArgs p) {
+    constexpr int kPieces = sizeof(T);                   // of 16 bytes a run
+    __shared__ uint32_t part[2][32];
+    const int slot = threadIdx.x / p.lanes, lane = threadIdx.x - slot * p.lanes, slots = blockDim.x / p.lanes;
+    const long long span = (p.k + kMsTileK - 1) / kMsTileK * kMsTileK;
+    float signs[ROTATED ? RUNS : 1][kRun];
+    if constexpr (ROTATED)
+#pragma unroll
+        for (int q = 0; q < RUNS; ++q) load_signs(p.signs, ((long long)q * p.lanes + lane) * kRun, p.k, p.wide_signs, signs[q]);
+    uint4 next[RUNS][kPieces];
+    auto fetch = [&](long long r) {
+        const T* const row = x + (r < p.rows ? r : p.rows - 1) * p.ldx;
+#pragma unroll
+        for (int q = 0; q < RUNS; ++q) {
+            const long long c0 = ((long long)q * p.lanes + lane) * kRun;
+            if (p.wide && c0 + kRun <= p.k) {
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) next[q][i] = __ldg(reinterpret_cast<const uint4*>(row + c0) + i);
+            } else {
+                T* const v = reinterpret_cast<T*>(next[q]);
+#pragma unroll
+                for (int i = 0; i < kRun; ++i) v[i] = c0 + i < p.k ? row[c0 + i] : from_f32<T>(0.0f);
+            }
+        }
+    };
+    int turn = 0;
+    long long r0 = (long long)blockIdx.x * slots;
+    fetch(r0 + slot);
+    for (; r0 < p.rows; r0 += (long long)gridDim.x * slots, turn ^= 1) {
+        const long long r = r0 + slot;
+        const bool row_is = r < p.rows;
+        float v[RUNS][kRun];
+#pragma unroll
+        for (int q = 0; q < RUNS; ++q)
+#pragma unroll
+            for (int i = 0; i < kRun; ++i) v[q][i] = to_f32<T>(reinterpret_cast<const T*>(next[q])[i]);
+        if (r0 + (long long)gridDim.x * slots < p.rows) fetch(r + (long long)gridDim.x * slots);
+        if constexpr (ROTATED)
+#pragma unroll
+            for (int q = 0; q < RUNS; ++q) rotate_run(v[q], signs[q], p.rotate);
+        int j = 0;
+        if constexpr (FMT == kNvfp4) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int q = 0; q < RUNS; ++q) m = max(m, row_largest(v[q]));
+            if (p.lanes >= 32) {
+                m = __reduce_max_sync(0xFFFFFFFFu, m);
+                if (p.lanes > 32) {
+                    if ((threadIdx.x & 31) == 0) part[turn][threadIdx.x >> 5] = m;
+                    __syncthreads();                     // (the other turn's parts may still be read)
+                    const int from = slot * (p.lanes / 32);
+                    for (int w = 0; w < p.lanes / 32; ++w) m = max(m, part[turn][from + w]);
+                }
+            } else {
+                for (int h = 1; h < p.lanes; h *= 2) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, h));
+            }
+            j = row_exponent(m);
+            if (lane == 0 && row_is) p.row_scale[r] = pow2(j);
+        }
+#pragma unroll
+        for (int q = 0; q < RUNS; ++q) {
+            uint32_t byte;
+            const uint2 code = quantize_run<FMT>(v[q], j, byte);
+            store_run<FMT>(r, row_is, ((long long)q * p.lanes + lane) * kRun, p.k, span, code, byte, p.codes, p.pitch, p.scales, p.atoms);
+        }
+    }
+}
+
+// Rows too long for registers: one CTA a row, nvfp4's largest value in a pass of its own.
 template <typename T, int FMT>
-__global__ void __launch_bounds__(256) tcq_ms_quantize_kernel(const T* __restrict__ x, long long k, long long ldx, bool wide, int rotate,
-                                                              const float* __restrict__ signs, uint8_t* __restrict__ codes, long long pitch,
-                                                              uint8_t* __restrict__ scales, long long atoms, float* __restrict__ row_scale) {
-    const long long r = blockIdx.x;
-    const T* const row = x + r * ldx;
-    const long long span = (k + kMsTileK - 1) / kMsTileK * kMsTileK;
+__global__ void __launch_bounds__(256) tcq_ms_quantize_long_kernel(const T* __restrict__ x, const __grid_constant__ QuantizeArgs p) {
+    const long long r = blockIdx.x, span = (p.k + kMsTileK - 1) / kMsTileK * kMsTileK;
+    const T* const row = x + r * p.ldx;
+    float v[kRun], signs[kRun];
+    auto load = [&](long long c0) {
+        load_run(row, c0, p.k, p.wide, v);
+        if (p.rotate) {
+            load_signs(p.signs, c0, p.k, p.wide_signs, signs);
+            rotate_run(v, signs, p.rotate);
+        }
+    };
     int j = 0;
-    float v[kRun];
     if constexpr (FMT == kNvfp4) {
         __shared__ uint32_t part[8];
         uint32_t m = 0;
         for (long long c = 0; c < span; c += 256 * kRun) {
-            const long long c0 = c + (long long)threadIdx.x * kRun;
-            load_run(row, c0, k, wide, v);
-            if (rotate) rotate_run(v, signs, c0, k, rotate);
-            if (largest_bits(v) < 0x7F800000u) m = max(m, largest_bits(v));
-            else m = max(m, largest_finite_bits(v));
+            load(c + (long long)threadIdx.x * kRun);
+            m = max(m, row_largest(v));
         }
         m = __reduce_max_sync(0xFFFFFFFFu, m);
         if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
         __syncthreads();
         for (int w = 0; w < 8; ++w) m = max(m, part[w]);
         j = row_exponent(m);
-        if (threadIdx.x == 0) row_scale[r] = pow2(j);
+        if (threadIdx.x == 0) p.row_scale[r] = pow2(j);
     }
     for (long long c = 0; c < span; c += 256 * kRun) {
         const long long c0 = c + (long long)threadIdx.x * kRun;
-        load_run(row, c0, k, wide, v);
-        if (rotate) rotate_run(v, signs, c0, k, rotate);
-        uint32_t m = largest_bits(v), byte;
-        if constexpr (FMT == kNvfp4) {
-            const float inv = pow2(-j);
-            byte = m < 0x7F800000u ? f32_to_e4m3(__fdiv_rn(__uint_as_float(m) * inv, 6.0f)) : 0x7Fu;
-            const float s = e4m3_to_f32(byte);
-#pragma unroll
-            for (int i = 0; i < kRun; ++i) v[i] = s > 0.0f ? __fdiv_rn(v[i] * inv, s) : v[i] * 0.0f;
-        } else {
-            m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-            const int e = m == 0 ? -127 : max(int(m >> 23) - 127 - 2, -127);
-            byte = m < 0x7F800000u ? uint32_t(e + 127) : 0xFFu;
-            const float inv = e <= -127 ? 1.7014118346046923e38f : pow2(-e);
-#pragma unroll
-            for (int i = 0; i < kRun; ++i) v[i] *= inv;
-        }
-        if (m >= 0x7F800000u) {
-#pragma unroll
-            for (int i = 0; i < kRun; ++i) v[i] = 0.0f;
-        }
-        if (c0 < 2 * pitch) *reinterpret_cast<uint2*>(codes + r * pitch + c0 / 2) = codes_of(v);
-        if (c0 < span) {
-            if constexpr (FMT == kNvfp4) scales[ms_scale_at(r, int(c0 / 16), atoms)] = uint8_t(c0 < k ? byte : 0);
-            else if (!(threadIdx.x & 1)) scales[ms_scale_at(r, int(c0 / 32), atoms)] = uint8_t(c0 < k ? byte : 0);
-        }
+        load(c0);
+        uint32_t byte;
+        const uint2 code = quantize_run<FMT>(v, j, byte);
+        store_run<FMT>(r, true, c0, p.k, span, code, byte, p.codes, p.pitch, p.scales, p.atoms);
     }
 }
 
@@ -191,15 +325,35 @@ __global__ void __launch_bounds__(256) tcq_ms_dequantize_kernel(const uint8_t* _
     }
 }
 
+template <typename T, int FMT>
+cudaError_t quantize_fmt(const T* x, QuantizeArgs p, cudaStream_t stream) {
+    const long long runs = ms_tiles_k(p.k) * (kMsTileK / kRun);
+    if (runs > 2 * 1024) {
+        tcq_ms_quantize_long_kernel<T, FMT><<<unsigned(p.rows), 256, 0, stream>>>(x, p);
+        return cudaGetLastError();
+    }
+    // Up to 256 threads a row: a power of two of them, as many rows as make 256.  More: a CTA a row, up to 1024 threads of one run, then of two.
+    const int each = runs > 1024 ? 2 : 1;
+    int threads = 256;
+    p.lanes = 16;
+    while (p.lanes < runs && p.lanes < 256) p.lanes *= 2;
+    if (runs > 256) threads = p.lanes = int((runs / each + 31) / 32 * 32);
+    const long long ctas = (p.rows + threads / p.lanes - 1) / (threads / p.lanes);
+    const unsigned grid = unsigned(std::min<long long>(ctas, 2048ll / threads * ms_sm_count()));
+    if (each == 1 && p.rotate) tcq_ms_quantize_kernel<T, FMT, 1, true><<<grid, threads, 0, stream>>>(x, p);
+    else if (each == 1) tcq_ms_quantize_kernel<T, FMT, 1, false><<<grid, threads, 0, stream>>>(x, p);
+    else if (p.rotate) tcq_ms_quantize_kernel<T, FMT, 2, true><<<grid, threads, 0, stream>>>(x, p);
+    else tcq_ms_quantize_kernel<T, FMT, 2, false><<<grid, threads, 0, stream>>>(x, p);
+    return cudaGetLastError();
+}
+
 template <typename T>
 cudaError_t quantize_t(const void* x, long long rows, long long k, long long ldx, int fmt, int rotate, const float* signs, uint8_t* codes,
                        uint8_t* scales, float* row_scale, cudaStream_t stream) {
-    const bool wide = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * sizeof(T) % 16 == 0;
-    const long long atoms = ms_tiles_k(k) * ms_atoms(fmt);
-    const T* const p = static_cast<const T*>(x);
-    if (fmt == kNvfp4) tcq_ms_quantize_kernel<T, kNvfp4><<<unsigned(rows), 256, 0, stream>>>(p, k, ldx, wide, rotate, signs, codes, ms_pitch(k), scales, atoms, row_scale);
-    else tcq_ms_quantize_kernel<T, kMxfp4><<<unsigned(rows), 256, 0, stream>>>(p, k, ldx, wide, rotate, signs, codes, ms_pitch(k), scales, atoms, row_scale);
-    return cudaGetLastError();
+    const QuantizeArgs p{rows, k, ldx, reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * sizeof(T) % 16 == 0, rotate, signs,
+                         reinterpret_cast<uintptr_t>(signs) % 16 == 0, codes, ms_pitch(k), scales, ms_tiles_k(k) * ms_atoms(fmt), row_scale, 256};
+    const T* const from = static_cast<const T*>(x);
+    return fmt == kNvfp4 ? quantize_fmt<T, kNvfp4>(from, p, stream) : quantize_fmt<T, kMxfp4>(from, p, stream);
 }
 
 template <typename T>
