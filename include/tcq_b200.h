@@ -320,14 +320,14 @@ TCQ_API int tcq_ms_quantize(const void *x, int dtype, int64_t rows, int64_t k, i
 TCQ_API int tcq_ms_dequantize(const uint8_t *codes, const uint8_t *scales, const float *row_scale, int64_t rows, int64_t k,
                               int format, void *out, int dtype, int64_t ldo, void *stream);
 
-/* Scratch of tcq_ms_linear (activations as bf16 numbers, zeros behind column k); 0 for a negative size or an unknown type. */
-TCQ_API size_t tcq_ms_linear_workspace_bytes(int64_t m, int64_t k, int dtype);
+/* Scratch of tcq_ms_linear for x m x k and W n x k; 0 for a negative size or an unknown type or format. */
+TCQ_API size_t tcq_ms_linear_workspace_bytes(int64_t m, int64_t n, int64_t k, int dtype, int format);
 
 /*
  * y[i][r] = sum_c x[i][c] * W[r][c]: x [m][ldx] of type dtype (not quantised), W n x k in 4 bits, y [m][ldy] of type dtype.
  * Products and sums in fp32, rounded to dtype once; equal for equal inputs, run to run, and a row of y does not depend on
- * what the other rows of x hold.  ws: tcq_ms_linear_workspace_bytes(m, k, dtype) bytes,
- * 256-byte aligned; not used (may be NULL) for up to 8 rows of x, and where x is bf16, 16-byte aligned and ldx a multiple of 8.  Columns of y behind n are left as they are.
+ * what the other rows of x hold.  ws: tcq_ms_linear_workspace_bytes(...) bytes, 256-byte
+ * aligned; not used (may be NULL) for up to 8 rows of x, and where x is bf16 (or fp16 and W nvfp4), 16-byte aligned and ldx a multiple of 8.  Columns of y behind n are left as they are.
  */
 TCQ_API int tcq_ms_linear(const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t *codes, const uint8_t *scales,
                           const float *row_scale, int64_t n, int64_t k, int format, void *y, int64_t ldy, void *ws,

@@ -226,6 +226,27 @@ def test_activations_of_any_range(ms, fmt, dtype, m):
     assert torch.equal(ms.linear(x.cuda(), w).cpu(), (x.double() * 1.5).to(dtype))
 
 
+@pytest.mark.parametrize("m", (9, 70, 300))
+@pytest.mark.parametrize("apart", (36, 37, 100))
+def test_fp16_times_scales_far_apart(ms, m, apart):
+    """mxfp4 rows whose scales fp16 weights just hold, and just not; blocks of zeros with the smallest scale among them count for nothing."""
+    n, k = 200, 320
+    g = torch.Generator().manual_seed(apart)
+    codes = torch.randint(0, 16, (n, k), generator=g)
+    byte = torch.full((n, k // 32), 127)
+    byte[::3, 2:4], byte[::3, 4] = 127 - apart, 127 + 3
+    byte[::3, 2:4] += 3
+    for column, zero in ((1, 0), (7, 8)):
+        byte[:, column] = 0
+        codes[:, 32 * column:32 * column + 32] = torch.where(codes[:, 32 * column:32 * column + 32] > 7, zero, 0)
+    x = torch.zeros(m, k, dtype=torch.float16)
+    hot = torch.randint(0, k // 32, (m,), generator=g)                # whole numbers in one block of columns a token: exact sums
+    for i in range(m):
+        x[i, 32 * hot[i]:32 * hot[i] + 32] = torch.randint(-8, 9, (32,), generator=g) * (2.0 ** (10 if hot[i] in (2, 3) else 0))
+    want = x.double() @ P.values(codes, byte, None, "mxfp4").t()
+    assert torch.equal(ms.linear(x.cuda(), P.pack(codes, byte, None, "mxfp4", "cuda")).cpu(), want.half())
+
+
 @pytest.mark.parametrize("fmt", FMTS)
 def test_scales_at_the_ends_of_their_range(ms, fmt):
     """The smallest and the largest scales of a format, in the weights and (products of both) in the activations."""
@@ -308,7 +329,7 @@ def test_results_leave_the_rest_of_their_buffer_alone(ms):
             for ldy in (n + 3, n + 8):
                 y = torch.full((m + 2, ldy), 77.0, dtype=torch.bfloat16, device="cuda")
                 xd = x.cuda()
-                ws = torch.empty(lib.tcq_ms_linear_workspace_bytes(m, k, 2), dtype=torch.uint8, device="cuda")
+                ws = torch.empty(lib.tcq_ms_linear_workspace_bytes(m, n, k, 2, 1), dtype=torch.uint8, device="cuda")
                 assert lib.tcq_ms_linear(xd.data_ptr(), 2, m, k, w.codes.data_ptr(), w.scales.data_ptr(), w.row_scale.data_ptr(), n, k, 1, y.data_ptr(), ldy, ws.data_ptr(), ws.numel(), stream) == 0
                 assert torch.equal(y[:m, :n].cpu(), (x.double() @ wv.t()).to(torch.bfloat16))
                 assert (y[m:] == 77).all() and (y[:, n:] == 77).all()

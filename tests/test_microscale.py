@@ -112,8 +112,8 @@ def test_argument_validation_needs_no_gpu():
     assert N(p, 2, 1, 16, p, p, p, 4, 0, 1, p, 4, *ws) == -8            # no columns
     assert N(None, 2, 1, 16, p, p, p, 4, 16, 1, p, 4, *ws) == -4 and N(p, 0, 9, 16, p, p, p, 4, 16, 1, p, 4, None, 0, None) == -4
     assert N(p + 1, 2, 1, 16, p, p, p, 4, 16, 1, p, 4, *ws) == -5 and N(p, 2, 1, 16, p, p, p, 4, 16, 1, p, 4, p + 128, 4096, None) == -5
-    assert N(p, 0, 9, 16, p, p, p, 4, 16, 1, p, 4, p, L.tcq_ms_linear_workspace_bytes(9, 16, 0) - 1, None) == -6
-    assert L.tcq_ms_linear_workspace_bytes(1, 16, 3) == 0 and L.tcq_ms_linear_workspace_bytes(-1, 16, 0) == 0
+    assert N(p, 0, 9, 16, p, p, p, 4, 16, 1, p, 4, p, L.tcq_ms_linear_workspace_bytes(9, 4, 16, 0, 1) - 1, None) == -6
+    assert L.tcq_ms_linear_workspace_bytes(1, 1, 16, 3, 1) == 0 and L.tcq_ms_linear_workspace_bytes(-1, 1, 16, 0, 1) == 0 and L.tcq_ms_linear_workspace_bytes(1, 1, 16, 0, 2) == 0
     assert N(p, 2, 0, 16, None, None, None, 4, 16, 1, None, 4, None, 0, None) == 0
     assert M(p, p, p, 1, p, p, None, 4, 16, 1, p, 2, 4, None) == -4
     assert M(p, p, p, 1, p, p + 4, p, 4, 16, 1, p, 2, 4, None) == -5

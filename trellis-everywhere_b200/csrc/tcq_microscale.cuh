@@ -62,6 +62,16 @@ __device__ __forceinline__ float e4m3_to_f32(uint32_t byte) {
 __device__ __forceinline__ float e8m0_to_f32(uint32_t byte) {
     return __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7FC00000u : byte << 23);
 }
+// Eight codes as four pairs of fp16 numbers, in order.
+__device__ __forceinline__ void e2m1x8_to_f16(uint32_t w, uint32_t (&h)[4]) {
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\tmov.b32 {b0, b1, b2, b3}, %4;\n\tcvt.rn.f16x2.e2m1x2 %0, b0;\n\tcvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, b2;\n\tcvt.rn.f16x2.e2m1x2 %3, b3;\n\t}" : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
+}
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
 template <int FMT> __device__ __forceinline__ float ms_scale_to_f32(uint32_t byte) {
     if constexpr (FMT == kNvfp4) return e4m3_to_f32(byte);
     else return e8m0_to_f32(byte);
@@ -93,8 +103,8 @@ cudaError_t launch_ms_quantize(const void* x, int dtype, long long rows, long lo
 cudaError_t launch_ms_dequantize(const MsMatrix& q, long long k, int fmt, void* out, int dtype, long long ldo, cudaStream_t stream);
 cudaError_t launch_ms_linear(const void* x, int dtype, long long m, long long ldx, const MsMatrix& w, long long k, int fmt, void* y,
                              long long ldy, void* ws, cudaStream_t stream);
-bool ms_linear_direct(const void* x, int dtype, long long m, long long ldx);     // x is taken as it lies: no scratch
-size_t ms_linear_workspace_bytes(long long m, long long k, int dtype);
+bool ms_linear_direct(const void* x, int dtype, long long m, long long ldx, int fmt);      // needs no scratch
+size_t ms_linear_workspace_bytes(long long m, long long n, long long k, int dtype, int fmt);
 cudaError_t launch_ms_matmul(const MsMatrix& x, const MsMatrix& w, long long k, int fmt, void* y, int dtype, long long ldy, cudaStream_t stream);
 
 }  // namespace tcq

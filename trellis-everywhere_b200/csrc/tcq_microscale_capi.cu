@@ -62,8 +62,8 @@ int tcq_ms_dequantize(const uint8_t* codes, const uint8_t* scales, const float* 
     return err == cudaSuccess ? TCQ_OK : report_cuda_error(err, "ms_dequantize");
 }
 
-size_t tcq_ms_linear_workspace_bytes(int64_t m, int64_t k, int dtype) {
-    return check_ms(m, k, TCQ_MS_NVFP4, dtype) != TCQ_OK ? 0 : ms_linear_workspace_bytes(m, k, dtype);
+size_t tcq_ms_linear_workspace_bytes(int64_t m, int64_t n, int64_t k, int dtype, int format) {
+    return check_ms(m, k, format, dtype) != TCQ_OK || check_ms(n, k, format, dtype) != TCQ_OK ? 0 : ms_linear_workspace_bytes(m, n, k, dtype, format);
 }
 
 int tcq_ms_linear(const void* x, int dtype, int64_t m, int64_t ldx, const uint8_t* codes, const uint8_t* scales,
@@ -74,11 +74,11 @@ int tcq_ms_linear(const void* x, int dtype, int64_t m, int64_t ldx, const uint8_
     if (rc != TCQ_OK) return rc;
     if (n == 0 || m == 0) return TCQ_OK;
     if (k == 0 || ldx < k || ldy < n) return TCQ_E_BAD_ARGUMENT;
-    const bool direct = ms_linear_direct(x, dtype, m, ldx);
+    const bool direct = ms_linear_direct(x, dtype, m, ldx, format);
     if (x == nullptr || y == nullptr || (ws == nullptr && !direct)) return TCQ_E_NULL_POINTER;
     if ((rc = check_ms_matrix(codes, scales, row_scale, format)) != TCQ_OK) return rc;
     if (misaligned(x, type_bytes(dtype)) || misaligned(y, type_bytes(dtype)) || misaligned(ws, 256)) return TCQ_E_MISALIGNED;
-    if (!direct && ws_bytes < ms_linear_workspace_bytes(m, k, dtype)) return TCQ_E_WORKSPACE;
+    if (!direct && ws_bytes < ms_linear_workspace_bytes(m, n, k, dtype, format)) return TCQ_E_WORKSPACE;
     cudaError_t err = launch_ms_linear(x, dtype, m, ldx, {codes, scales, row_scale, n}, k, format, y, ldy, ws, static_cast<cudaStream_t>(stream));
     return err == cudaSuccess ? TCQ_OK : report_cuda_error(err, "ms_linear");
 }

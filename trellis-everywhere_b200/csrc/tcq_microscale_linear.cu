@@ -17,6 +17,7 @@
 
 #include "tcq_common.cuh"
 #include "tcq_microscale.cuh"
+#include "tcq_microscale_many.cuh"
 #include "tcq_tcgen05.cuh"
 
 namespace tcq {
@@ -69,16 +70,6 @@ __device__ __forceinline__ void sts128(uint32_t smem, const uint32_t (&v)[4]) {
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// Eight codes as four pairs of fp16 numbers, in order.
-__device__ __forceinline__ void eight_codes(uint32_t w, uint32_t (&h)[4]) {
-    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\tmov.b32 {b0, b1, b2, b3}, %4;\n\tcvt.rn.f16x2.e2m1x2 %0, b0;\n\tcvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %2, b2;\n\tcvt.rn.f16x2.e2m1x2 %3, b3;\n\t}" : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
-}
-__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
 }
 // Two e8m0 scales as bf16 numbers (2^-127 a denormal one, 255 NaN).
 __device__ __forceinline__ uint32_t e8m0x2_to_bf16x2(uint16_t v) {
@@ -285,8 +276,8 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             uint32_t a0[4], a1[4];
-                            eight_codes(w[2 * i], a0);
-                            eight_codes(w[2 * i + 1], a1);
+                            e2m1x8_to_f16(w[2 * i], a0);
+                            e2m1x8_to_f16(w[2 * i + 1], a1);
                             if constexpr (FMT == kNvfp4) {
 #pragma unroll
                                 for (int j = 0; j < 4; ++j) { a0[j] = mul_f16x2(a0[j], scale[i][0]); a1[j] = mul_f16x2(a1[j], scale[i][1]); }
@@ -390,7 +381,8 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
 // times 2^8 more than the one before, so that the last bits of the smallest numbers are still bf16 numbers.
 template <typename T, int P>
 __global__ void __launch_bounds__(256) tcq_ms_parts_kernel(const T* __restrict__ x, long long m, long long k, long long ldx, __nv_bfloat16* __restrict__ out,
-                                                           long long width) {
+                                                           long long width, const unsigned int* __restrict__ wide) {
+    if (wide != nullptr && *wide == 0) return;           // the fp16 form has run
     const long long id = (long long)blockIdx.x * 256 + threadIdx.x, runs = width / 8;
     if (id >= m * runs) return;
     const long long i = id / runs, c0 = (id - i * runs) * 8;
@@ -412,8 +404,8 @@ __global__ void __launch_bounds__(256) tcq_ms_parts_kernel(const T* __restrict__
 }
 
 template <typename T, int P>
-cudaError_t split(const void* x, long long m, long long k, long long ldx, void* ws, long long width, cudaStream_t stream) {
-    tcq_ms_parts_kernel<T, P><<<unsigned((m * (width / 8) + 255) / 256), 256, 0, stream>>>(static_cast<const T*>(x), m, k, ldx, static_cast<__nv_bfloat16*>(ws), width);
+cudaError_t split(const void* x, long long m, long long k, long long ldx, void* ws, long long width, const unsigned int* wide, cudaStream_t stream) {
+    tcq_ms_parts_kernel<T, P><<<unsigned((m * (width / 8) + 255) / 256), 256, 0, stream>>>(static_cast<const T*>(x), m, k, ldx, static_cast<__nv_bfloat16*>(ws), width, wide);
     return cudaGetLastError();
 }
 
@@ -461,17 +453,20 @@ cudaError_t launch_fmt(const FewArgs& p, int fmt, cudaStream_t stream) {
 
 }  // namespace
 
-// tcq_microscale_linear_many.cu: x as m * parts rows of bf16, `width` columns of them (the others zero), 16-byte aligned.
-cudaError_t launch_ms_linear_many(const __nv_bfloat16* x, long long ldx, long long width, long long m, int parts, int dtype, const MsMatrix& w, long long k,
-                                  int fmt, void* y, long long ldy, cudaStream_t stream);
+// Whether fp16 rows are multiplied as they lie, by fp16 weights: where a TMA load can start at them.
+static bool as_fp16(const void* x, int dtype, long long ldx) { return dtype == kF16 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 8 == 0; }
 
-// Whether x is taken as it lies, with no scratch: few tokens, or bf16 rows that a TMA load can start at.
-bool ms_linear_direct(const void* x, int dtype, long long m, long long ldx) {
-    return m <= kTokens || (dtype == kBf16 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 8 == 0);
+// Whether a call needs no scratch: few tokens, or rows that a TMA load can start at and weights that are numbers of x's type.
+bool ms_linear_direct(const void* x, int dtype, long long m, long long ldx, int fmt) {
+    return m <= kTokens || (dtype == kBf16 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 8 == 0) || (fmt == kNvfp4 && as_fp16(x, dtype, ldx));
 }
 
-size_t ms_linear_workspace_bytes(long long m, long long k, int dtype) {
+// The parts of x; behind them (fp16 and mxfp4) a word, and the largest scale of every row of W.
+static size_t parts_bytes(long long m, long long k, int dtype) {
     return size_t(m) * size_t(ms_tiles_k(k) * kMsTileK) * 2 * (dtype == kF32 ? 3 : dtype == kF16 ? 2 : 1);
+}
+size_t ms_linear_workspace_bytes(long long m, long long n, long long k, int dtype, int fmt) {
+    return parts_bytes(m, k, dtype) + (dtype == kF16 && fmt == kMxfp4 ? 256 + (size_t(n) + 127) / 128 * 128 : 0);
 }
 
 cudaError_t launch_ms_linear(const void* x, int dtype, long long m, long long ldx, const MsMatrix& w, long long k, int fmt, void* y,
@@ -483,14 +478,28 @@ cudaError_t launch_ms_linear(const void* x, int dtype, long long m, long long ld
         return launch_fmt<__nv_bfloat16, 1>(p, fmt, stream);
     }
     const long long width = ms_tiles_k(k) * kMsTileK;
-    const int parts = dtype == kF32 ? 3 : dtype == kF16 ? 2 : 1;
-    if (ms_linear_direct(x, dtype, m, ldx)) return launch_ms_linear_many(static_cast<const __nv_bfloat16*>(x), ldx, k, m, parts, dtype, w, k, fmt, y, ldy, stream);
+    ManyCall c{x, ldx, k, m, 1, dtype, w, k, fmt, y, ldy, false, nullptr, nullptr};
     cudaError_t err;
-    if (dtype == kF32) err = split<float, 3>(x, m, k, ldx, ws, width, stream);
-    else if (dtype == kF16) err = split<__half, 2>(x, m, k, ldx, ws, width, stream);
-    else err = split<__nv_bfloat16, 1>(x, m, k, ldx, ws, width, stream);
+    if (dtype == kBf16 && ms_linear_direct(x, dtype, m, ldx, fmt)) return launch_ms_linear_many(c, stream);
+    if (as_fp16(x, dtype, ldx) && (fmt == kNvfp4 || m > 128)) {
+        // fp16 weights: nvfp4's always are; mxfp4's where no row's scales are further apart than fp16 reaches, which the GPU finds out by itself: one of
+        // the two forms behind it runs (8 us of small launches: for many tokens; 1000 through 12288 x 4096 184 -> 88 us).
+        c.fp16 = true;
+        if (fmt == kNvfp4) return launch_ms_linear_many(c, stream);
+        c.wide = reinterpret_cast<unsigned int*>(static_cast<uint8_t*>(ws) + parts_bytes(m, k, dtype));
+        c.largest = reinterpret_cast<uint8_t*>(c.wide) + 256;
+        if ((err = launch_ms_scale_range(w, k, c.wide, c.largest, stream)) != cudaSuccess) return err;
+        if ((err = launch_ms_linear_many(c, stream)) != cudaSuccess) return err;
+        c.fp16 = false;
+    }
+    if (dtype == kF32) err = split<float, 3>(x, m, k, ldx, ws, width, c.wide, stream);
+    else if (dtype == kF16) err = split<__half, 2>(x, m, k, ldx, ws, width, c.wide, stream);
+    else err = split<__nv_bfloat16, 1>(x, m, k, ldx, ws, width, c.wide, stream);
     if (err != cudaSuccess) return err;
-    return launch_ms_linear_many(static_cast<const __nv_bfloat16*>(ws), width, width, m, parts, dtype, w, k, fmt, y, ldy, stream);
+    c.x = ws;
+    c.ldx = c.width = width;
+    c.parts = dtype == kF32 ? 3 : dtype == kF16 ? 2 : 1;
+    return launch_ms_linear_many(c, stream);
 }
 
 }  // namespace tcq

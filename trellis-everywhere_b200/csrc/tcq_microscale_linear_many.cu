@@ -1,7 +1,8 @@
 // Products of 16- and 32-bit activations with a 4-bit microscaled matrix, many tokens: y[i][r] = sum_c x[i][c] * W[r][c].
 //
-// Every value of W is a bf16 number, and x comes as m * P rows of bf16 parts (tcq_microscale_linear.cu), so the products are those of a bf16
-// matrix product.  128 rows of W are the left operand, in tensor memory: eight warps read 64 columns of codes at a time from shared memory,
+// Every value of W is a bf16 number, and x comes as m * P rows of bf16 parts (P = 1, 2, 3 for bf16, fp16, fp32, each the next eight
+// significant bits), so the products are exact ones of a bf16 matrix product.  fp16 x needs one part where the weights are fp16 numbers: nvfp4's are;
+// mxfp4's are, times a power of two for each row, unless a row's scales are more than 2^36 apart.  128 rows of W are the left operand, in tensor memory: eight warps read 64 columns of codes at a time from shared memory,
 // make bf16 numbers of them (a thread one row) and store them there, so that neither the bf16 weights nor their reading takes any of
 // shared memory's bandwidth.  NT rows of x are the right operand, by TMA.
 //
@@ -13,6 +14,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "tcq_microscale_many.cuh"
 #include "tcq_microscale_weights.cuh"
 #include "tcq_tcgen05.cuh"
 
@@ -48,6 +50,9 @@ struct ManyArgs {
     long long atoms;                             // of scales a row group
     void* y;
     long long ldy;
+    const unsigned int* wide;                    // run only if *wide is `run_if`
+    unsigned int run_if;
+    const uint8_t* largest;                      // fp16, mxfp4
 };
 
 __device__ __forceinline__ void mma_from_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
@@ -74,6 +79,15 @@ __device__ __forceinline__ uint32_t lds32(uint32_t smem) {
     return v;
 }
 
+// What a row's sums are multiplied by.
+template <int FMT, bool FP16>
+__device__ __forceinline__ float row_factor(const ManyArgs& p, long long r) {
+    if (r >= p.w.rows) return 1.0f;
+    if constexpr (FMT == kNvfp4) return p.w.row_scale[r];
+    else if constexpr (FP16) return __uint_as_float(uint32_t(p.largest[r]) << 23 | (p.largest[r] == 0 ? 0x00400000u : 0u)) * 0x1p-13f;      // (2^-127: a denormal number)
+    else return 1.0f;
+}
+
 // The parts of a token, smallest first, as its sum.
 template <int P>
 __device__ __forceinline__ float whole_of(const float* v) {
@@ -86,11 +100,19 @@ __device__ __forceinline__ float whole_of(const float* v) {
 // result; where that is all the error there is (fp32 results), 256 columns at a time are added up in registers instead (4e-7).
 template <int P> constexpr int kStepsHeld = P == 3 ? 4 : 1 << 29;
 
-template <typename YT, int FMT, int NT, int P>
+// fp16 scales of mxfp4: 2^13 over the row's largest scale (`most`, a byte), times the block's; 0 for what is too small for fp16 (blocks of zeros).
+__device__ __forceinline__ uint32_t relative_scale(uint32_t byte, uint32_t most) {
+    const int e = int(byte) - int(most) + 13;
+    const __half h = byte == 255 ? __ushort_as_half(0x7FFF) : e < -23 ? __ushort_as_half(0) : __float2half_rn(__uint_as_float(uint32_t(e + 127) << 23));
+    return uint32_t(__half_as_ushort(h)) * 0x10001u;
+}
+
+template <typename YT, int FMT, int NT, int P, bool FP16>
 __global__ void __launch_bounds__(kThreads<P>, 1) tcq_ms_linear_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                                                                          const __grid_constant__ ManyArgs p) {
     using T = Tile<FMT, NT>;
     constexpr int kTokens = NT / P;                      // of a tile
+    if (p.wide != nullptr && *p.wide != p.run_if) return;
     extern __shared__ uint8_t raw[];
     __shared__ uint64_t w_full[T::kStagesW], w_empty[T::kStagesW], x_full[T::kStagesX], x_empty[T::kStagesX], a_full[T::kStagesA], a_empty[T::kStagesA],
         sum_full[T::kSumBuffers], sum_empty[T::kSumBuffers], drained;
@@ -165,7 +187,7 @@ __global__ void __launch_bounds__(kThreads<P>, 1) tcq_ms_linear_many_kernel(cons
         }
     } else if (warp == 1) {
         // ---- products; likewise
-        constexpr uint32_t kIdesc = 1u << 4 | 1u << 7 | 1u << 10 | uint32_t(NT >> 3) << 17 | uint32_t(kRows >> 4) << 24;      // bf16 x bf16, fp32 sums
+        constexpr uint32_t kIdesc = 1u << 4 | (FP16 ? 0u : 1u << 7 | 1u << 10) | uint32_t(NT >> 3) << 17 | uint32_t(kRows >> 4) << 24;      // bf16 x bf16 (or fp16 x fp16), fp32 sums
         const bool one = elect_one();
         uint32_t sx = 0, px = 0, sa = 0, pa = 0;
         int n = 0;
@@ -210,7 +232,9 @@ __global__ void __launch_bounds__(kThreads<P>, 1) tcq_ms_linear_many_kernel(cons
         const int row = 32 * quarter + lane;
         uint32_t sw = 0, pw = 0, sa = 0, pa = 1;
         bool ok = true;
-        for (int t = blockIdx.x / splits; t < tiles && ok; t += clusters)
+        for (int t = blockIdx.x / splits; t < tiles && ok; t += clusters) {
+            uint32_t most = 0;
+            if constexpr (FP16 && FMT == kMxfp4) most = (long long)(t / p.tiles_m) * kRows + row < p.w.rows ? p.largest[(long long)(t / p.tiles_m) * kRows + row] : 0;
             for (int step = first; step < last && ok; ++step) {
                 if (step % 4 == 0) ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&w_full[sw]), pw, &gave_up));
                 if (step % kMakers<P> == mine && ok) {
@@ -224,11 +248,30 @@ __global__ void __launch_bounds__(kThreads<P>, 1) tcq_ms_linear_many_kernel(cons
                     for (int i = 0; i < 2; ++i) {        // 16 bytes: 32 columns; the swizzle has put piece c of row r at c ^ (r % 8)
                         const uint4 c = lds128(from + (((2 * sub + i) ^ (row & 7)) << 4));
                         const uint32_t cw[4] = {c.x, c.y, c.z, c.w};
+                        if constexpr (FP16) {
+                            uint32_t s[2];               // of the two halves
+                            if constexpr (FMT == kNvfp4) {
+                                uint32_t two;
+                                asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(two) : "r"(word >> (16 * i)));
+                                s[0] = __byte_perm(two, two, 0x1010);
+                                s[1] = __byte_perm(two, two, 0x3232);
+                            } else {
+                                s[0] = s[1] = relative_scale((word >> (8 * i)) & 0xFFu, most);
+                            }
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const __nv_bfloat162 s = scale_of<FMT>(word, 2 * i + j / 2);
-                            four_weights(cw[j], s, v[16 * i + 4 * j], v[16 * i + 4 * j + 1]);
-                            four_weights(cw[j] >> 16, s, v[16 * i + 4 * j + 2], v[16 * i + 4 * j + 3]);
+                            for (int j = 0; j < 4; ++j) {
+                                uint32_t h[4];
+                                e2m1x8_to_f16(cw[j], h);
+#pragma unroll
+                                for (int q = 0; q < 4; ++q) v[16 * i + 4 * j + q] = mul_f16x2(h[q], s[j / 2]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const __nv_bfloat162 s = scale_of<FMT>(word, 2 * i + j / 2);
+                                four_weights(cw[j], s, v[16 * i + 4 * j], v[16 * i + 4 * j + 1]);
+                                four_weights(cw[j] >> 16, s, v[16 * i + 4 * j + 2], v[16 * i + 4 * j + 3]);
+                            }
                         }
                     }
                     ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&a_empty[sa]), pa, &gave_up));
@@ -247,6 +290,7 @@ __global__ void __launch_bounds__(kThreads<P>, 1) tcq_ms_linear_many_kernel(cons
                     if (++sw == T::kStagesW) { sw = 0; pw ^= 1; }
                 }
             }
+        }
     } else {
         // ---- results: this warp's lanes are 32 rows of W, so that a store is 32 neighbours in y
         const int quarter = warp & 3;
@@ -254,7 +298,7 @@ __global__ void __launch_bounds__(kThreads<P>, 1) tcq_ms_linear_many_kernel(cons
         int n = 0;
         for (int t = blockIdx.x / splits; t < tiles; t += clusters) {
             const long long r = (long long)(t / p.tiles_m) * kRows + 32 * quarter + lane, token0 = (long long)(t % p.tiles_m) * kTokens;
-            const float fw = FMT == kNvfp4 && r < p.w.rows ? p.w.row_scale[r] : 1.0f;
+            const float fw = row_factor<FMT, FP16>(p, r);
             const int here = int(min((long long)kTokens, p.m - token0));
             float* const part = reinterpret_cast<float*>(raw + (smem_x - smem_u32(raw))) + 32 * quarter + lane;
             YT* const y = static_cast<YT*>(p.y) + token0 * p.ldy + r;
@@ -270,7 +314,7 @@ __global__ void __launch_bounds__(kThreads<P>, 1) tcq_ms_linear_many_kernel(cons
 #pragma unroll
                     for (int i = 0; i < N / P; ++i, to += p.ldy) {
                         float whole = whole_of<P>(f + i * P);
-                        if constexpr (FMT == kNvfp4) whole *= fw;
+                        if constexpr (FMT == kNvfp4 || FP16) whole *= fw;
                         if (r < p.w.rows && c0 / P + i < here) *to = from_f32<YT>(whole);
                     }
                 }
@@ -342,7 +386,7 @@ __global__ void __launch_bounds__(kThreads<P>, 1) tcq_ms_linear_many_kernel(cons
             for (int j = 0; j < 4; ++j)
                 if (r + j < p.w.rows) {
                     float whole = whole_of<P>(sum[j]);
-                    if constexpr (FMT == kNvfp4) whole *= p.w.row_scale[r + j];
+                    if constexpr (FMT == kNvfp4 || FP16) whole *= row_factor<FMT, FP16>(p, r + j);
                     static_cast<YT*>(p.y)[(token0 + token) * p.ldy + r + j] = from_f32<YT>(whole);
                 }
         }
@@ -356,23 +400,24 @@ __global__ void __launch_bounds__(kThreads<P>, 1) tcq_ms_linear_many_kernel(cons
     }
 }
 
-template <typename YT, int FMT, int NT, int P>
-cudaError_t launch(const __nv_bfloat16* x, long long ldx, long long width, long long m, const MsMatrix& w, long long k, void* y, long long ldy, int splits,
-                   cudaStream_t stream) {
+template <typename YT, int FMT, int NT, int P, bool FP16>
+cudaError_t launch(const ManyCall& c, int splits, cudaStream_t stream) {
     using T = Tile<FMT, NT>;
+    const auto kernel = tcq_ms_linear_many_kernel<YT, FMT, NT, P, FP16>;
     static bool ready[64] = {};
     int dev = 0;
     cudaError_t err = cudaGetDevice(&dev);
     if (err != cudaSuccess) return err;
     if (dev >= 64 || !ready[dev]) {
-        if ((err = cudaFuncSetAttribute(tcq_ms_linear_many_kernel<YT, FMT, NT, P>, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem)) != cudaSuccess) return err;
+        if ((err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem)) != cudaSuccess) return err;
         if (dev < 64) ready[dev] = true;
     }
     CUtensorMap map_w, map_x;
-    const long long pitch = ms_pitch(k), tokens = NT / P;
-    if ((err = make_byte_map(&map_w, w.codes, pitch, w.rows, pitch, kRows)) != cudaSuccess) return err;
-    if ((err = make_bf16_map(&map_x, x, width, m * P, ldx, NT)) != cudaSuccess) return err;
-    const ManyArgs p{w, m, int((w.rows + kRows - 1) / kRows), int((m + tokens - 1) / tokens), int((k + kStepK - 1) / kStepK), ms_tiles_k(k) * T::kAtoms, y, ldy};
+    const long long pitch = ms_pitch(c.k), tokens = NT / P;
+    if ((err = make_byte_map(&map_w, c.w.codes, pitch, c.w.rows, pitch, kRows)) != cudaSuccess) return err;
+    if ((err = make_16bit_map(&map_x, c.x, c.width, c.m * P, c.ldx, NT)) != cudaSuccess) return err;
+    const ManyArgs p{c.w, c.m, int((c.w.rows + kRows - 1) / kRows), int((c.m + tokens - 1) / tokens), int((c.k + kStepK - 1) / kStepK), ms_tiles_k(c.k) * T::kAtoms, c.y, c.ldy,
+                     c.wide, FP16 ? 0u : 1u, c.largest};
     const long long tiles = (long long)p.tiles_n * p.tiles_m;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(splits > 1 ? tiles * splits : std::min<long long>(tiles, ms_sm_count())));
@@ -385,33 +430,90 @@ cudaError_t launch(const __nv_bfloat16* x, long long ldx, long long width, long 
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, tcq_ms_linear_many_kernel<YT, FMT, NT, P>, map_w, map_x, p);
+    return cudaLaunchKernelEx(&cfg, kernel, map_w, map_x, p);
 }
 
-template <typename YT, int FMT, int P>
-cudaError_t launch_fmt(const __nv_bfloat16* x, long long ldx, long long width, long long m, const MsMatrix& w, long long k, void* y, long long ldy, cudaStream_t stream) {
-    const long long rows = m * P, tiles = (w.rows + kRows - 1) / kRows, k_tiles = ms_tiles_k(k);
+template <typename YT, int FMT, int P, bool FP16>
+cudaError_t launch_nt(const ManyCall& c, cudaStream_t stream) {
+    const long long rows = c.m * P, tiles = (c.w.rows + kRows - 1) / kRows, k_tiles = ms_tiles_k(c.k);
     int splits = 1;
     while (splits < kMostSplits && tiles * splits * 2 <= ms_sm_count() && splits * 2 <= k_tiles) splits *= 2;
-    if (rows <= 16 / P * P) return launch<YT, FMT, 16, P>(x, ldx, width, m, w, k, y, ldy, splits, stream);
-    if (rows <= 32 / P * P) return launch<YT, FMT, 32, P>(x, ldx, width, m, w, k, y, ldy, splits, stream);
-    if constexpr (P == 3) {             // sums in registers: no more than 64 columns
+    if (rows <= 16 / P * P) return launch<YT, FMT, 16, P, FP16>(c, splits, stream);
+    if (rows <= 32 / P * P) return launch<YT, FMT, 32, P, FP16>(c, splits, stream);
+    if constexpr (P == 3) {                              // sums in registers: no more than 64 columns
         const long long tiles_m = (rows + 62) / 63;
-        return launch<YT, FMT, 64, P>(x, ldx, width, m, w, k, y, ldy, tiles * tiles_m * splits <= ms_sm_count() ? splits : 1, stream);
+        return launch<YT, FMT, 64, P, FP16>(c, tiles * tiles_m * splits <= ms_sm_count() ? splits : 1, stream);
     } else {
-    if (rows <= 64 / P * P) return launch<YT, FMT, 64, P>(x, ldx, width, m, w, k, y, ldy, splits, stream);
-    if (tiles * ((rows + 255) / 256) * 2 <= ms_sm_count()) return launch<YT, FMT, 128, P>(x, ldx, width, m, w, k, y, ldy, 1, stream);
-    return launch<YT, FMT, 256, P>(x, ldx, width, m, w, k, y, ldy, 1, stream);
+        if (rows <= 64 / P * P) return launch<YT, FMT, 64, P, FP16>(c, splits, stream);
+        if (tiles * ((rows + 255) / 256) * 2 <= ms_sm_count()) return launch<YT, FMT, 128, P, FP16>(c, 1, stream);
+        return launch<YT, FMT, 256, P, FP16>(c, 1, stream);
     }
+}
+
+template <int FMT>
+cudaError_t launch_fmt(const ManyCall& c, cudaStream_t stream) {
+    if (c.dtype == kF32) return launch_nt<float, FMT, 3, false>(c, stream);
+    if (c.dtype == kBf16) return launch_nt<__nv_bfloat16, FMT, 1, false>(c, stream);
+    return c.fp16 ? launch_nt<__half, FMT, 1, true>(c, stream) : launch_nt<__half, FMT, 2, false>(c, stream);
+}
+
+// One CTA a group of 128 rows; a warp reads the 512 bytes of 128 columns at a time, a lane the four rows lane + 32 q.
+__global__ void __launch_bounds__(256) tcq_ms_scale_range_kernel(MsMatrix w, long long k, long long pitch, int atoms, unsigned int* wide, uint8_t* largest) {
+    __shared__ uint32_t part[8][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint4* const from = reinterpret_cast<const uint4*>(w.scales) + ((long long)blockIdx.x * atoms) * 32 + lane;
+    const int blocks = int((k + 31) / 32);
+    uint32_t most = 0;                                   // a byte a row
+    for (int a = warp; a < atoms; a += 8) {
+        const uint4 u = __ldg(from + a * 32);
+        const uint32_t v[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const uint32_t m = (most >> (8 * q)) & 0xFFu;
+            uint32_t b = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t s = (v[q] >> (8 * i)) & 0xFFu;
+                b = max(b, s == 255u ? 0u : s);          // (NaN: no size)
+            }
+            if (b > m) most = (most & ~(0xFFu << (8 * q))) | b << (8 * q);
+        }
+    }
+    part[warp][lane] = most;
+    __syncthreads();
+    most = part[0][lane];
+    for (int i = 1; i < 8; ++i) most = __vmaxu4(most, part[i][lane]);
+    if (warp < 4) {
+        const long long row = (long long)blockIdx.x * 128 + 32 * warp + lane;
+        if (row < w.rows) largest[row] = uint8_t(most >> (8 * warp));
+    }
+    bool far = false;
+    for (int a = warp; a < atoms; a += 8) {
+        const uint4 u = __ldg(from + a * 32);
+        const uint32_t v[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const long long row = (long long)blockIdx.x * 128 + 32 * q + lane;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (((v[q] >> (8 * i)) & 0xFFu) + 36 < ((most >> (8 * q)) & 0xFFu) && row < w.rows && 4 * a + i < blocks) {
+                    const uint4 c = __ldg(reinterpret_cast<const uint4*>(w.codes + row * pitch) + 4 * a + i);       // 32 codes
+                    far = far || ((c.x | c.y | c.z | c.w) & 0x77777777u) != 0;
+                }
+        }
+    }
+    if (far) atomicOr(wide, 1u);
 }
 
 }  // namespace
 
-cudaError_t launch_ms_linear_many(const __nv_bfloat16* x, long long ldx, long long width, long long m, int parts, int dtype, const MsMatrix& w, long long k,
-                                  int fmt, void* y, long long ldy, cudaStream_t stream) {
-    if (dtype == kF32) return fmt == kNvfp4 ? launch_fmt<float, kNvfp4, 3>(x, ldx, width, m, w, k, y, ldy, stream) : launch_fmt<float, kMxfp4, 3>(x, ldx, width, m, w, k, y, ldy, stream);
-    if (dtype == kF16) return fmt == kNvfp4 ? launch_fmt<__half, kNvfp4, 2>(x, ldx, width, m, w, k, y, ldy, stream) : launch_fmt<__half, kMxfp4, 2>(x, ldx, width, m, w, k, y, ldy, stream);
-    return fmt == kNvfp4 ? launch_fmt<__nv_bfloat16, kNvfp4, 1>(x, ldx, width, m, w, k, y, ldy, stream) : launch_fmt<__nv_bfloat16, kMxfp4, 1>(x, ldx, width, m, w, k, y, ldy, stream);
+cudaError_t launch_ms_linear_many(const ManyCall& c, cudaStream_t stream) { return c.fmt == kNvfp4 ? launch_fmt<kNvfp4>(c, stream) : launch_fmt<kMxfp4>(c, stream); }
+
+cudaError_t launch_ms_scale_range(const MsMatrix& w, long long k, unsigned int* wide, uint8_t* largest, cudaStream_t stream) {
+    cudaError_t err = cudaMemsetAsync(wide, 0, sizeof(unsigned int), stream);
+    if (err != cudaSuccess) return err;
+    tcq_ms_scale_range_kernel<<<unsigned((w.rows + 127) / 128), 256, 0, stream>>>(w, k, ms_pitch(k), int(ms_tiles_k(k)) * 2, wide, largest);
+    return cudaGetLastError();
 }
 
 }  // namespace tcq

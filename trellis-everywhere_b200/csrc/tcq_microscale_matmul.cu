@@ -388,8 +388,8 @@ cudaError_t make_byte_map(CUtensorMap* map, const void* base, long long width, l
     return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, width, rows, pitch, 128, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-cudaError_t make_bf16_map(CUtensorMap* map, const void* base, long long width, long long rows, long long ld, int box_rows) {
-    return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, width, rows, 2 * ld, 64, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+cudaError_t make_16bit_map(CUtensorMap* map, const void* base, long long width, long long rows, long long ld, int box_rows) {
+    return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, base, width, rows, 2 * ld, 64, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 cudaError_t make_scale_map(CUtensorMap* map, const void* base, long long rows, int box_rows) {

@@ -120,8 +120,8 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t smem, uint32_t rank)
 // A map of [rows][width] bytes, `pitch` bytes a row (a multiple of 16), cut into boxes of [box_rows][128 bytes] in the 128-byte swizzle.
 cudaError_t make_byte_map(CUtensorMap* map, const void* base, long long width, long long rows, long long pitch, int box_rows);
 
-// A map of [rows][width] bf16 numbers, `ld` from row to row (a multiple of 8), cut into boxes of [box_rows][64] in the same swizzle.
-cudaError_t make_bf16_map(CUtensorMap* map, const void* base, long long width, long long rows, long long ld, int box_rows);
+// A map of [rows][width] 16-bit numbers, `ld` from row to row (a multiple of 8), cut into boxes of [box_rows][64] in the same swizzle.
+cudaError_t make_16bit_map(CUtensorMap* map, const void* base, long long width, long long rows, long long ld, int box_rows);
 
 // A map of scales as rows of 512 bytes, cut into boxes of `box_rows` of them, one behind the other.
 cudaError_t make_scale_map(CUtensorMap* map, const void* base, long long rows, int box_rows);

@@ -46,7 +46,7 @@ SIGNATURES = {
     "tcq_ms_scale_bytes": (_sz, [_i64, _i64, _int]),
     "tcq_ms_quantize": (_int, [_vp, _int, _i64, _i64, _i64, _int, _int, _vp, _vp, _vp, _vp, _vp]),
     "tcq_ms_dequantize": (_int, [_vp, _vp, _vp, _i64, _i64, _int, _vp, _int, _i64, _vp]),
-    "tcq_ms_linear_workspace_bytes": (_sz, [_i64, _i64, _int]),
+    "tcq_ms_linear_workspace_bytes": (_sz, [_i64, _i64, _i64, _int, _int]),
     "tcq_ms_linear": (_int, [_vp, _int, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _int, _vp, _i64, _vp, _sz, _vp]),
     "tcq_ms_matmul": (_int, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _int, _vp, _int, _i64, _vp]),
 }

@@ -211,8 +211,8 @@ def linear(x: torch.Tensor, w: Microscaled) -> torch.Tensor:
     if m and n and k:
         dt, pitch, at = _DTYPES[flat.dtype], _pitch(flat), flat.data_ptr()
         ws = size = None
-        if m > 8 and (dt != 2 or at % 16 or pitch % 8):
-            size = _lib.lib().tcq_ms_linear_workspace_bytes(m, k, dt)
+        if m > 8 and (at % 16 or pitch % 8 or not (dt == 2 or (dt == 1 and fmt == "nvfp4"))):
+            size = _lib.lib().tcq_ms_linear_workspace_bytes(m, n, k, dt, FORMATS[fmt])
             ws = torch.empty(size, dtype=torch.uint8, device=flat.device)  # given back when the call is queued: the stream's later work comes after it
         _launch(dev, "tcq_ms_linear", at, dt, m, pitch, codes.data_ptr(), scales.data_ptr(), _ptr(row), n, k, FORMATS[fmt], y.data_ptr(), n,
                 _ptr(ws), size or 0)
