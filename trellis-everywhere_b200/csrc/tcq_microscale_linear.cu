@@ -403,10 +403,16 @@ __global__ void __launch_bounds__(256) tcq_ms_parts_kernel(const T* __restrict__
     }
 }
 
-template <typename T, int P>
-cudaError_t split(const void* x, long long m, long long k, long long ldx, void* ws, long long width, const unsigned int* wide, cudaStream_t stream) {
-    tcq_ms_parts_kernel<T, P><<<unsigned((m * (width / 8) + 255) / 256), 256, 0, stream>>>(static_cast<const T*>(x), m, k, ldx, static_cast<__nv_bfloat16*>(ws), width, wide);
-    return cudaGetLastError();
+// Rows of 16-bit numbers with zeros behind column k, for TMA loads that cannot start at them where they lie.
+__global__ void __launch_bounds__(256) tcq_ms_pad_kernel(const uint16_t* __restrict__ x, long long m, long long k, long long ldx, uint16_t* __restrict__ out, long long width) {
+    const long long id = (long long)blockIdx.x * 256 + threadIdx.x, runs = width / 8;
+    if (id >= m * runs) return;
+    const long long i = id / runs, c0 = (id - i * runs) * 8;
+    uint32_t w[4] = {};
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (c0 + j < k) w[j / 2] |= uint32_t(x[i * ldx + c0 + j]) << (16 * (j & 1));
+    *reinterpret_cast<uint4*>(out + i * width + c0) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 template <typename T, int FMT, int PARTS>
@@ -453,20 +459,20 @@ cudaError_t launch_fmt(const FewArgs& p, int fmt, cudaStream_t stream) {
 
 }  // namespace
 
-// Whether fp16 rows are multiplied as they lie, by fp16 weights: where a TMA load can start at them.
-static bool as_fp16(const void* x, int dtype, long long ldx) { return dtype == kF16 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 8 == 0; }
+// Whether a TMA load can start at the rows of x.
+static bool rows_aligned(const void* x, long long ldx) { return reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 8 == 0; }
 
-// Whether a call needs no scratch: few tokens, or rows that a TMA load can start at and weights that are numbers of x's type.
+// Whether a call needs no scratch: few tokens, or rows that a TMA load can start at, of a type that the weights are numbers of.
 bool ms_linear_direct(const void* x, int dtype, long long m, long long ldx, int fmt) {
-    return m <= kTokens || (dtype == kBf16 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 8 == 0) || (fmt == kNvfp4 && as_fp16(x, dtype, ldx));
+    return m <= kTokens || (rows_aligned(x, ldx) && (dtype == kBf16 || (dtype == kF16 && fmt == kNvfp4)));
 }
 
-// The parts of x; behind them (fp16 and mxfp4) a word, and the largest scale of every row of W.
-static size_t parts_bytes(long long m, long long k, int dtype) {
-    return size_t(m) * size_t(ms_tiles_k(k) * kMsTileK) * 2 * (dtype == kF32 ? 3 : dtype == kF16 ? 2 : 1);
-}
+// Rows of x, padded or in parts; for fp16 and mxfp4 both, a word, and the largest scale of every row of W.
+static size_t row_bytes(long long m, long long k) { return size_t(m) * size_t(ms_tiles_k(k) * kMsTileK) * 2; }
 size_t ms_linear_workspace_bytes(long long m, long long n, long long k, int dtype, int fmt) {
-    return parts_bytes(m, k, dtype) + (dtype == kF16 && fmt == kMxfp4 ? 256 + (size_t(n) + 127) / 128 * 128 : 0);
+    const size_t rows = row_bytes(m, k);
+    if (dtype == kF16 && fmt == kMxfp4) return 3 * rows + 256 + (size_t(n) + 127) / 128 * 128;
+    return dtype == kF32 ? 3 * rows : rows;
 }
 
 cudaError_t launch_ms_linear(const void* x, int dtype, long long m, long long ldx, const MsMatrix& w, long long k, int fmt, void* y,
@@ -478,27 +484,39 @@ cudaError_t launch_ms_linear(const void* x, int dtype, long long m, long long ld
         return launch_fmt<__nv_bfloat16, 1>(p, fmt, stream);
     }
     const long long width = ms_tiles_k(k) * kMsTileK;
+    const unsigned grid = unsigned((m * (width / 8) + 255) / 256);
+    uint8_t* const scratch = static_cast<uint8_t*>(ws);
     ManyCall c{x, ldx, k, m, 1, dtype, w, k, fmt, y, ldy, false, nullptr, nullptr};
     cudaError_t err;
-    if (dtype == kBf16 && ms_linear_direct(x, dtype, m, ldx, fmt)) return launch_ms_linear_many(c, stream);
-    if (as_fp16(x, dtype, ldx) && (fmt == kNvfp4 || m > 128)) {
+    if (dtype == kBf16 || (dtype == kF16 && (fmt == kNvfp4 || m > 128))) {
+        if (!rows_aligned(x, ldx)) {
+            tcq_ms_pad_kernel<<<grid, 256, 0, stream>>>(static_cast<const uint16_t*>(x), m, k, ldx, static_cast<uint16_t*>(ws), width);
+            if ((err = cudaGetLastError()) != cudaSuccess) return err;
+            c.x = ws;
+            c.ldx = c.width = width;
+        }
+        c.fp16 = dtype == kF16;
+        if (dtype == kBf16 || fmt == kNvfp4) return launch_ms_linear_many(c, stream);
         // fp16 weights: nvfp4's always are; mxfp4's where no row's scales are further apart than fp16 reaches, which the GPU finds out by itself: one of
         // the two forms behind it runs (8 us of small launches: for many tokens; 1000 through 12288 x 4096 184 -> 88 us).
-        c.fp16 = true;
-        if (fmt == kNvfp4) return launch_ms_linear_many(c, stream);
-        c.wide = reinterpret_cast<unsigned int*>(static_cast<uint8_t*>(ws) + parts_bytes(m, k, dtype));
+        c.wide = reinterpret_cast<unsigned int*>(scratch + 3 * row_bytes(m, k));
         c.largest = reinterpret_cast<uint8_t*>(c.wide) + 256;
         if ((err = launch_ms_scale_range(w, k, c.wide, c.largest, stream)) != cudaSuccess) return err;
         if ((err = launch_ms_linear_many(c, stream)) != cudaSuccess) return err;
         c.fp16 = false;
     }
-    if (dtype == kF32) err = split<float, 3>(x, m, k, ldx, ws, width, c.wide, stream);
-    else if (dtype == kF16) err = split<__half, 2>(x, m, k, ldx, ws, width, c.wide, stream);
-    else err = split<__nv_bfloat16, 1>(x, m, k, ldx, ws, width, c.wide, stream);
-    if (err != cudaSuccess) return err;
-    c.x = ws;
+    // x in parts of bf16 numbers
+    if (dtype == kF32) {
+        c.parts = 3;
+        c.x = ws;
+        tcq_ms_parts_kernel<float, 3><<<grid, 256, 0, stream>>>(static_cast<const float*>(x), m, k, ldx, static_cast<__nv_bfloat16*>(ws), width, nullptr);
+    } else {
+        c.parts = 2;
+        c.x = scratch + row_bytes(m, k);
+        tcq_ms_parts_kernel<__half, 2><<<grid, 256, 0, stream>>>(static_cast<const __half*>(x), m, k, ldx, reinterpret_cast<__nv_bfloat16*>(scratch + row_bytes(m, k)), width, c.wide);
+    }
+    if ((err = cudaGetLastError()) != cudaSuccess) return err;
     c.ldx = c.width = width;
-    c.parts = dtype == kF32 ? 3 : dtype == kF16 ? 2 : 1;
     return launch_ms_linear_many(c, stream);
 }
 
