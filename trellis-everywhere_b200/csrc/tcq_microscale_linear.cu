@@ -14,6 +14,7 @@
 //
 // A wait that runs out (kMbarWaitCycles) makes its CTA's results NaN.
 #include <algorithm>
+#include <type_traits>
 
 #include "tcq_common.cuh"
 #include "tcq_microscale.cuh"
@@ -79,28 +80,77 @@ __device__ __forceinline__ uint32_t e8m0x2_to_bf16x2(uint16_t v) {
 }
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }      // -126 <= e <= 127
 
-// The next part of eight of a token's 256 columns (a warp has them all): fp16 numbers times the factor returned; r becomes what is left.
-__device__ __forceinline__ float next_part(float (&r)[8], uint32_t (&h)[4], bool& left) {
+// The next PARTS parts of eight of a token's 256 columns (a warp has them all): fp16 numbers, times the factors given, which are 2^-11 apart; r
+// becomes what is left.  BITS: significant bits of the numbers at the start.
+template <int PARTS, int BITS>
+__device__ __forceinline__ bool next_parts(float (&r)[8], uint32_t (&h)[PARTS][4], float (&factor)[PARTS]) {
     uint32_t most = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint32_t b = __float_as_uint(r[i]) & 0x7FFFFFFFu;
-        most = max(most, b < 0x7F800000u ? b : 0u);
-    }
+    for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(r[i]) & 0x7FFFFFFFu);
     most = __reduce_max_sync(0xFFFFFFFFu, most);
-    const int e = max(int(most >> 23), 1) - 127, up = most == 0 ? 0 : 14 - e;                 // largest finite magnitude below 2^15; -113 <= up <= 140
-    const float f0 = pow2f(up / 2), f1 = pow2f(up - up / 2), g0 = pow2f(-(up / 2)), g1 = pow2f(up / 2 - up);
-    left = false;
+    bool left = false;
+    if (most >= 0x0C000000u && most < 0x7F800000u) {     // 2^-103 and more, and finite: all factors are normal numbers
+        const int up = 141 - int(most >> 23);            // largest magnitude below 2^15
+        if constexpr (PARTS == 1) {
+            const float f = pow2f(up);
+            factor[0] = pow2f(-up);
+            // the last of a number's bits is 2^-24 or more unless its exponent is below this: then it has been cut
+            const uint32_t least = uint32_t(127 - 24 + (BITS - 1) - up) << 23;
+            bool cut = false;
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-        const __half a = __float2half_rz(r[i] * f0 * f1), b = __float2half_rz(r[i + 1] * f0 * f1);
-        h[i / 2] = uint32_t(__half_as_ushort(a)) | uint32_t(__half_as_ushort(b)) << 16;
-        const bool fine_a = (__float_as_uint(r[i]) & 0x7F800000u) != 0x7F800000u, fine_b = (__float_as_uint(r[i + 1]) & 0x7F800000u) != 0x7F800000u;
-        r[i] = fine_a ? r[i] - __half2float(a) * g0 * g1 : 0.0f;                              // exact: the bits that were cut off
-        r[i + 1] = fine_b ? r[i + 1] - __half2float(b) * g0 * g1 : 0.0f;
-        left = left || r[i] != 0.0f || r[i + 1] != 0.0f;
+            for (int i = 0; i < 8; i += 2) {
+                asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(h[0][i / 2]) : "f"(r[i + 1] * f), "f"(r[i] * f));
+                cut = cut || (__float_as_uint(r[i]) & 0x7FFFFFFFu) - 1u < least - 1u || (__float_as_uint(r[i + 1]) & 0x7FFFFFFFu) - 1u < least - 1u;
+            }
+            if (!__any_sync(0xFFFFFFFFu, cut)) return false;
+        }
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q) {
+            const float f = pow2f(up + 11 * q), g = pow2f(-up - 11 * q);
+            const f32x2 f2 = pack2(f, f), minus = pack2(-g, -g);
+            factor[q] = g;
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                float a, b;
+                unpack2(mul2(pack2(r[i], r[i + 1]), f2), a, b);
+                asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(h[q][i / 2]) : "f"(b), "f"(a));
+                const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h[q][i / 2]));
+                unpack2(fma2(pack2(back.x, back.y), minus, pack2(r[i], r[i + 1])), r[i], r[i + 1]);      // exact: the bits that were cut off
+            }
+        }
+    } else {
+        // nothing left, tiny numbers, infinities or NaN: part by part, factors in two steps, what is not finite once and for all
+#pragma unroll 1
+        for (int q = 0; q < PARTS; ++q) {
+            uint32_t finite = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t b = __float_as_uint(r[i]) & 0x7FFFFFFFu;
+                finite = max(finite, b < 0x7F800000u ? b : 0u);
+            }
+            finite = __reduce_max_sync(0xFFFFFFFFu, finite);
+            const int up = finite == 0 ? 0 : 141 - max(int(finite >> 23), 1);                 // -113 <= up <= 140
+            const float f0 = pow2f(up / 2), f1 = pow2f(up - up / 2), g0 = pow2f(-(up / 2)), g1 = pow2f(up / 2 - up);
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(w[i / 2]) : "f"(r[i + 1] * f0 * f1), "f"(r[i] * f0 * f1));
+                const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&w[i / 2]));
+                r[i] = (__float_as_uint(r[i]) & 0x7F800000u) != 0x7F800000u ? r[i] - back.x * g0 * g1 : 0.0f;
+                r[i + 1] = (__float_as_uint(r[i + 1]) & 0x7F800000u) != 0x7F800000u ? r[i + 1] - back.y * g0 * g1 : 0.0f;
+            }
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p)
+                if (p == q) {
+                    factor[p] = g0 * g1;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) h[p][i] = w[i];
+                }
+        }
     }
-    return g0 * g1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) left = left || r[i] != 0.0f;
+    return left;
 }
 
 // Whether any of the 256 threads says so; all of them have arrived.
@@ -190,14 +240,15 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
         // The rows of x: part q of token i of the n-th 256 columns held is row (n * PARTS + q) * m + i.  PARTS more parts of r into the n-th; whether
         // something is left.
         auto convert_one = [&](int n, int token) {
-            bool left = false;
+            uint32_t h[PARTS][4];
+            float f[PARTS];
+            constexpr int kBits = std::is_same_v<T, float> ? 24 : std::is_same_v<T, __half> ? 11 : 8;
+            const bool left = next_parts<PARTS, kBits>(r, h, f);
 #pragma unroll
             for (int q = 0; q < PARTS; ++q) {
-                uint32_t h[4];
-                const float f = next_part(r, h, left);
                 const int row = (n * PARTS + q) * p.m + token;
-                sts128(smem_x + row * kPitchX + 16 * lane, h);
-                if (lane == 0) factor[row] = f;
+                sts128(smem_x + row * kPitchX + 16 * lane, h[q]);
+                if (lane == 0) factor[row] = f[q];
             }
             return left;
         };
