@@ -293,6 +293,7 @@ TCQ_API int tcq_codebook_lut(int codebook, float *lut, void *stream);
  *              row r at [r/128][b/4][r%32][r%128/32][b%4], atoms = 2 (mxfp4) or 4 (nvfp4) for every 256 columns begun;
  *              zeros behind column k.  Places of rows behind the last one may hold anything.
  *   row_scale  [rows] fp32 (nvfp4), NULL (mxfp4)
+ * Fewer than 2^31 rows, at most 2^24 columns.  Waits inside the products are bounded; results whose wait ran out are NaN.
  */
 #define TCQ_MS_MXFP4 0
 #define TCQ_MS_NVFP4 1

@@ -453,6 +453,24 @@ def test_model_in_four_bits(ms, fmt, activations, rotate):
     assert again == 1
 
 
+@pytest.mark.parametrize("activations,rotate", ((16, 0), (4, 64)))
+def test_module_given_another_type_keeps_its_scales(ms, activations, rotate):
+    from trellis_b200 import quant
+    torch.manual_seed(2)
+    model = torch.nn.Sequential(torch.nn.Linear(128, 40)).cuda()
+    assert quant.apply_microscaled(model, "nvfp4", activations, rotate) == 1
+    before = {k: v.clone() for k, v in model.state_dict().items()}
+    x = torch.randn(4, 128, device="cuda").half()
+    want = model(x)
+    model.half()
+    assert model[0].row_scale.dtype == torch.float32 and torch.equal(model(x), want)
+    other = torch.nn.Sequential(quant.MicroscaledLinear(torch.zeros(40, 128), torch.zeros(40), "nvfp4", activations, rotate))
+    other.load_state_dict(before)
+    assert torch.equal(other(x), want)
+    for name, t in other.to("cpu").state_dict().items():
+        assert t.device.type == "cpu" and torch.equal(t, before[name].cpu())
+
+
 def test_rotated_product_is_the_product(ms):
     """Both sides rotated: the product of the values is that of the unrotated ones, up to what 4 bits leave."""
     g = torch.Generator(device="cuda").manual_seed(3)

@@ -105,7 +105,7 @@ def test_argument_validation_needs_no_gpu():
     assert Q(p + 2, 0, 1, 16, 16, 1, 0, None, p, p, p, None) == -5
     assert Q(p, 0, 0, 16, 16, 1, 0, None, None, None, None, None) == 0  # nothing to do
     assert D(p, p, p, 1, 16, 1, p, 0, 15, None) == -8 and D(p, p, p, 1, 16, 1, None, 0, 16, None) == -4
-    assert D(p, p, p, 1, 1 << 31, 1, p, 0, 1 << 31, None) == -8
+    assert D(p, p, p, 1, (1 << 24) + 1, 1, p, 0, 1 << 31, None) == -8 and D(p, p, p, 1 << 31, 16, 1, p, 0, 16, None) == -8
     ws = (p, 4096, None)
     assert N(p, 2, 1, 16, p, p, p, 4, 16, 1, p, 3, *ws) == -8           # ldy < n
     assert N(p, 2, 1, 15, p, p, p, 4, 16, 1, p, 4, *ws) == -8           # ldx < k

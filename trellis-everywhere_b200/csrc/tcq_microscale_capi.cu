@@ -8,13 +8,14 @@ using namespace tcq;
 namespace {
 
 bool misaligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a != 0; }
-constexpr int64_t kMsMost = int64_t(1) << 31;            // rows and columns of a matrix: block numbers and grids fit 32 bits
+constexpr int64_t kMostRows = int64_t(1) << 31;          // grids and coordinates fit 32 bits
+constexpr int64_t kMostColumns = int64_t(1) << 24;       // a tile's products end well within the limit of a wait for them
 
 int check_ms(int64_t rows, int64_t k, int format, int dtype) {
     if (format != TCQ_MS_MXFP4 && format != TCQ_MS_NVFP4) return TCQ_E_BAD_FORMAT;
     if (dtype < TCQ_F32 || dtype > TCQ_BF16) return TCQ_E_BAD_FORMAT;
     if (rows < 0 || k < 0) return TCQ_E_BAD_COUNT;
-    return rows >= kMsMost || k >= kMsMost ? TCQ_E_BAD_ARGUMENT : TCQ_OK;
+    return rows >= kMostRows || k > kMostColumns ? TCQ_E_BAD_ARGUMENT : TCQ_OK;
 }
 // One matrix in 4 bits: what must be there, and aligned.
 int check_ms_matrix(const void* codes, const void* scales, const void* row_scale, int format) {

@@ -106,6 +106,16 @@ class MicroscaledLinear(nn.Module):
                         ("bias", None if bias is None else bias.detach().to(wd.device))):
             self.register_buffer(name, t)
 
+    def _apply(self, fn, recurse: bool = True):
+        """Moves with the module, but the scales and signs stay fp32 whatever type the module is given."""
+        kept = {name: t for name in ("row_scale", "signs") if (t := getattr(self, name)) is not None}
+        super()._apply(fn, recurse)
+        for name, t in kept.items():
+            now = getattr(self, name)
+            if now.dtype != torch.float32:
+                setattr(self, name, t.to(now.device))
+        return self
+
     @property
     def weight(self) -> "microscale.Microscaled":
         return microscale.Microscaled(self.codes, self.scales, self.row_scale, (self.out_features, self.in_features), self.fmt)
