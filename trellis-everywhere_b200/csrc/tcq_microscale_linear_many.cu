@@ -6,7 +6,7 @@
 // make bf16 numbers of them (a thread one row) and store them there, so that neither the bf16 weights nor their reading takes any of
 // shared memory's bandwidth.  NT rows of x are the right operand, by TMA.
 //
-// Work split: one CTA per SM goes through tiles of 128 rows of W x NT rows of x.  One warp loads (codes and scales of 256 columns, x of 64),
+// Work split: one CTA per SM, or two, goes through tiles of 128 rows of W x NT rows of x.  One warp loads (codes and scales of 256 columns, x of 64),
 // one issues products, eight make weights (two groups of four take turns), four take finished sums out of tensor memory.  With few tokens a
 // cluster of S CTAs shares the columns of a tile; the partial sums meet through distributed shared memory, in rank order.
 //
@@ -28,19 +28,23 @@ template <int P> constexpr int kThreads = 32 * (6 + 4 * kMakers<P>);
 constexpr int kRows = 128, kStepK = 64;          // rows of W; columns of a step
 constexpr int kMostSplits = 8;
 
-template <int FMT, int NT>
+template <int FMT, int NT, int P>
 struct Tile {
+    // Up to 64 rows of x two CTAs share an SM: making weights is what takes the time, and eight warps do not fill the SM
+    // (16 through 40960 x 4096: 67.4 -> 54.6 us, mxfp4 85.5 -> 66.2).
+    static constexpr int kCtas = NT <= 64 && P != 3 ? 2 : 1;
     static constexpr int kAtoms = Ms<FMT>::kAtoms;
     static constexpr int kBytesW = kRows * 128, kBytesS = kAtoms * 512, kStageW = kBytesW + 2048, kStagesW = 3;      // 256 columns
     static constexpr int kBytesX = NT * 128;                                                                        // 64 columns
-    static constexpr int kStagesX = std::min(8, (220 * 1024 - kStagesW * kStageW) / kBytesX);
+    static constexpr int kStagesX = std::min(8, ((kCtas == 2 ? 111 : 220) * 1024 - kStagesW * kStageW) / kBytesX);
     static constexpr int kSumBuffers = NT <= 128 ? 2 : 1, kSumColumns = NT < 32 ? 32 : NT;
     static constexpr int kStagesA = 4, kColumnsA = kStepK / 2;                                                      // weights in tensor memory
-    static constexpr int kColumns = 512;
+    static constexpr int kColumns = 512 / kCtas;
     static constexpr int kBytes = (kStagesW * kStageW + 1023) / 1024 * 1024 + kStagesX * kBytesX;
-    static constexpr int kSmem = std::max(kBytes, 115 * 1024) + 1024;                                               // two CTAs never share an SM
-    static_assert(kSumBuffers * kSumColumns + kStagesA * kColumnsA <= 512 && kSmem <= 226 * 1024 && kStagesX >= 4);
-    static_assert(kStagesX * kBytesX >= NT * kRows * 4 || NT > 64, "the parts of a tile");
+    // An SM (228 KB) holds two halves or one whole, so that no CTA waits for the tensor memory of another kernel's.
+    static constexpr int kSmem = kCtas == 2 ? 112 * 1024 : std::max(kBytes + 1024, 116 * 1024);
+    static_assert(kSumBuffers * kSumColumns + kStagesA * kColumnsA <= kColumns && kBytes + 1024 <= kSmem && kSmem <= 226 * 1024 && kStagesX >= 4);
+    static_assert(kStagesX * kBytesX >= NT * kRows * 4 || NT == 256, "the parts of a tile");
 };
 
 struct ManyArgs {
@@ -108,9 +112,9 @@ __device__ __forceinline__ uint32_t relative_scale(uint32_t byte, uint32_t most)
 }
 
 template <typename YT, int FMT, int NT, int P, bool FP16>
-__global__ void __launch_bounds__(kThreads<P>, 1) tcq_ms_linear_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+__global__ void __launch_bounds__(kThreads<P>, Tile<FMT, NT, P>::kCtas) tcq_ms_linear_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                                                                          const __grid_constant__ ManyArgs p) {
-    using T = Tile<FMT, NT>;
+    using T = Tile<FMT, NT, P>;
     constexpr int kTokens = NT / P;                      // of a tile
     if (p.wide != nullptr && *p.wide != p.run_if) return;
     extern __shared__ uint8_t raw[];
@@ -401,8 +405,8 @@ __global__ void __launch_bounds__(kThreads<P>, 1) tcq_ms_linear_many_kernel(cons
 }
 
 template <typename YT, int FMT, int NT, int P, bool FP16>
-cudaError_t launch(const ManyCall& c, int splits, cudaStream_t stream) {
-    using T = Tile<FMT, NT>;
+cudaError_t launch(const ManyCall& c, cudaStream_t stream) {
+    using T = Tile<FMT, NT, P>;
     const auto kernel = tcq_ms_linear_many_kernel<YT, FMT, NT, P, FP16>;
     static bool ready[64] = {};
     int dev = 0;
@@ -419,8 +423,17 @@ cudaError_t launch(const ManyCall& c, int splits, cudaStream_t stream) {
     const ManyArgs p{c.w, c.m, int((c.w.rows + kRows - 1) / kRows), int((c.m + tokens - 1) / tokens), int((c.k + kStepK - 1) / kStepK), ms_tiles_k(c.k) * T::kAtoms, c.y, c.ldy,
                      c.wide, FP16 ? 0u : 1u, c.largest};
     const long long tiles = (long long)p.tiles_n * p.tiles_m;
+    // How many CTAs share the columns of a tile: as many as leave every CTA an SM of its own (half an SM, where each still has 1024 columns:
+    // 4096 columns of 4096 rows by 8 instead of 4 costs 10.7 -> 11.7 us, 12288 of them 21.3 -> 20.2 us).
+    const int k_tiles = int(ms_tiles_k(c.k)), sms = ms_sm_count();
+    const auto fits = [&](int s) {
+        if (T::kCtas == 2) return tiles * s <= sms || (tiles * s <= 2 * sms && k_tiles >= 4 * s);
+        return tiles <= ms_most_clusters(reinterpret_cast<const void*>(kernel), kThreads<P>, T::kSmem, s);
+    };
+    int splits = 1;
+    while (NT <= 128 && splits < kMostSplits && 2 * splits <= k_tiles && fits(2 * splits)) splits *= 2;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(splits > 1 ? tiles * splits : std::min<long long>(tiles, ms_sm_count())));
+    cfg.gridDim = dim3(unsigned(splits > 1 ? tiles * splits : std::min<long long>(tiles, T::kCtas * ms_sm_count())));
     cfg.blockDim = dim3(kThreads<P>);
     cfg.dynamicSmemBytes = T::kSmem;
     cfg.stream = stream;
@@ -433,20 +446,19 @@ cudaError_t launch(const ManyCall& c, int splits, cudaStream_t stream) {
     return cudaLaunchKernelEx(&cfg, kernel, map_w, map_x, p);
 }
 
+// Rows of x in a tile: all of them up to 64; 128 where all tiles then run at once (100 through 4096 x 4096, its columns shared by four: 12.9 us,
+// not shared 26.4, tiles of 64 16.6); else 256, which makes the weights least often.
 template <typename YT, int FMT, int P, bool FP16>
 cudaError_t launch_nt(const ManyCall& c, cudaStream_t stream) {
-    const long long rows = c.m * P, tiles = (c.w.rows + kRows - 1) / kRows, k_tiles = ms_tiles_k(c.k);
-    int splits = 1;
-    while (splits < kMostSplits && tiles * splits * 2 <= ms_sm_count() && splits * 2 <= k_tiles) splits *= 2;
-    if (rows <= 16 / P * P) return launch<YT, FMT, 16, P, FP16>(c, splits, stream);
-    if (rows <= 32 / P * P) return launch<YT, FMT, 32, P, FP16>(c, splits, stream);
-    if constexpr (P == 3) {                              // sums in registers: no more than 64 columns
-        const long long tiles_m = (rows + 62) / 63;
-        return launch<YT, FMT, 64, P, FP16>(c, tiles * tiles_m * splits <= ms_sm_count() ? splits : 1, stream);
+    const long long rows = c.m * P;
+    if (rows <= 16 / P * P) return launch<YT, FMT, 16, P, FP16>(c, stream);
+    if (rows <= 32 / P * P) return launch<YT, FMT, 32, P, FP16>(c, stream);
+    if constexpr (P == 3) {
+        return launch<YT, FMT, 64, P, FP16>(c, stream);  // sums in registers: no more than 64 columns
     } else {
-        if (rows <= 64 / P * P) return launch<YT, FMT, 64, P, FP16>(c, splits, stream);
-        if (tiles * ((rows + 255) / 256) * 2 <= ms_sm_count()) return launch<YT, FMT, 128, P, FP16>(c, 1, stream);
-        return launch<YT, FMT, 256, P, FP16>(c, 1, stream);
+        if (rows <= 64 / P * P) return launch<YT, FMT, 64, P, FP16>(c, stream);
+        if ((c.w.rows + kRows - 1) / kRows * ((c.m + 128 / P - 1) / (128 / P)) <= ms_sm_count()) return launch<YT, FMT, 128, P, FP16>(c, stream);
+        return launch<YT, FMT, 256, P, FP16>(c, stream);
     }
 }
 

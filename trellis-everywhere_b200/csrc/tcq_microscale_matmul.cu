@@ -35,7 +35,7 @@ struct Tile {
     static constexpr int kColumns = 2 * kSumColumns + kStages * kScaleColumns <= 256 ? 256 : 512;
     // over half of an SM's shared memory: two CTAs never share an SM, so that none waits for another's tensor memory
     static constexpr int kSmem = kStages * kStageBytes + 1024;
-    static_assert(kSmem > 114 * 1024 && kSmem <= 226 * 1024 && kStages >= 3 && kStages * kStageBytes >= NT * kRowsW * 4);
+    static_assert(kSmem >= 116 * 1024 && kSmem <= 226 * 1024 && kStages >= 3 && kStages * kStageBytes >= NT * kRowsW * 4);
 };
 
 }  // namespace
@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_matmul_kernel(const __grid
 }
 
 template <int FMT, int NT>
-cudaError_t launch(const MsMatrix& x, const MsMatrix& w, long long k, void* y, int dtype, long long ldy, int splits, cudaStream_t stream) {
+cudaError_t launch(const MsMatrix& x, const MsMatrix& w, long long k, void* y, int dtype, long long ldy, cudaStream_t stream) {
     using T = Tile<FMT, NT>;
     static bool ready[64] = {};
     int dev = 0;
@@ -310,6 +310,9 @@ cudaError_t launch(const MsMatrix& x, const MsMatrix& w, long long k, void* y, i
     const MatmulArgs p{w.scales, x.scales, w.row_scale, x.row_scale, w.rows, x.rows, int((w.rows + kRowsW - 1) / kRowsW), int((x.rows + NT - 1) / NT),
                        int(ms_tiles_k(k)), y, ldy, dtype, reinterpret_cast<uintptr_t>(y) % four == 0 && ldy % 4 == 0};
     const long long tiles = (long long)p.tiles_n * p.tiles_m;
+    int splits = 1;
+    while (p.k_tiles >= 8 && splits < kMostSplits && splits * 4 <= p.k_tiles &&
+           tiles <= ms_most_clusters(reinterpret_cast<const void*>(tcq_ms_matmul_kernel<FMT, NT>), kThreads, T::kSmem, splits * 2)) splits *= 2;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(splits > 1 ? tiles * splits : std::min<long long>(tiles, ms_sm_count())));
     cfg.blockDim = dim3(kThreads);
@@ -341,13 +344,11 @@ cudaError_t launch_fmt(const MsMatrix& x, const MsMatrix& w, long long k, void* 
         const long long rounds128 = (tiles_m * tiles + pairs - 1) / pairs, rounds256 = (tiles_m * ((w.rows + 255) / 256) + pairs - 1) / pairs;
         return launch_ms_matmul_pair(x, w, k, FMT, y, dtype, ldy, 5 * rounds128 > 9 * rounds256 ? 256 : 128, sms, stream);
     }
-    int splits = 1;
-    while (splits < kMostSplits && tiles * splits * 2 <= sms && splits * 4 <= k_tiles && k_tiles >= 8) splits *= 2;
-    if (m <= 8) return launch<FMT, 8>(x, w, k, y, dtype, ldy, splits, stream);
-    if (m <= 16) return launch<FMT, 16>(x, w, k, y, dtype, ldy, splits, stream);
-    if (m <= 32) return launch<FMT, 32>(x, w, k, y, dtype, ldy, splits, stream);
-    if (m <= 64) return launch<FMT, 64>(x, w, k, y, dtype, ldy, splits, stream);
-    return launch<FMT, 128>(x, w, k, y, dtype, ldy, splits, stream);
+    if (m <= 8) return launch<FMT, 8>(x, w, k, y, dtype, ldy, stream);
+    if (m <= 16) return launch<FMT, 16>(x, w, k, y, dtype, ldy, stream);
+    if (m <= 32) return launch<FMT, 32>(x, w, k, y, dtype, ldy, stream);
+    if (m <= 64) return launch<FMT, 64>(x, w, k, y, dtype, ldy, stream);
+    return launch<FMT, 128>(x, w, k, y, dtype, ldy, stream);
 }
 
 }  // namespace
@@ -359,6 +360,30 @@ int ms_sm_count() {
     if (dev < 64 && cache[dev]) return cache[dev];
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
     if (dev < 64) cache[dev] = n;
+    return n;
+}
+
+int ms_most_clusters(const void* kernel, int threads, size_t smem, int size) {
+    static int cache[64][4] = {};                            // by log2(size); clusters of one CTA as well
+    const int slot = size >= 8 ? 3 : size / 2, sms = ms_sm_count();
+    int dev = 0, n = 0;
+    if (size == 1 || cudaGetDevice(&dev) != cudaSuccess) return sms / size;
+    if (dev < 64 && cache[dev][slot]) return cache[dev][slot];
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(size));
+    cfg.blockDim = dim3(unsigned(threads));
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = unsigned(size);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+        (void)cudaGetLastError();
+        return sms / size;
+    }
+    if (dev < 64) cache[dev][slot] = n;
     return n;
 }
 

@@ -34,7 +34,7 @@ struct Tile {
     static constexpr int kBySmem = (225 * 1024 - kTurnBytes) / kStageBytes, kByTmem = (512 - kSumBuffers * NT) / kScaleColumns;
     static constexpr int kStages = std::min(kBySmem, kByTmem);
     static constexpr int kSmem = kStages * kStageBytes + kTurnBytes + 1024;
-    static_assert(kSmem > 114 * 1024 && kSmem <= 226 * 1024 && kStages >= 4);
+    static_assert(kSmem >= 116 * 1024 && kSmem <= 226 * 1024 && kStages >= 4);
 };
 
 struct PairArgs {
