@@ -375,6 +375,44 @@ def test_calls_repeat_on_streams_and_in_graphs(ms, m):
         assert all(torch.equal(a, b) for a, b in zip(out, want[i])) and all(torch.equal(a, b) for a, b in zip(out2, want[i]))
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", ((1, 4600, 2304), (9, 2100, 2304), (30, 5000, 600), (42, 700, 4096), (60, 130, 8200), (100, 300, 4096), (128, 1000, 2111), (200, 130, 2048)))
+def test_shared_columns_within_rounding(ms, fmt, dtype, m, n, k):
+    """Sizes at which clusters of two, four and eight CTAs share the columns, in tiles of 8 to 128 rows of x, and two CTAs an SM."""
+    w = P.random_matrix(n, k, fmt, torch.Generator().manual_seed(n * k))
+    wq, wv = P.pack(*w, fmt, "cuda"), P.values(*w, fmt)
+    x = torch.randn(m, k, generator=torch.Generator().manual_seed(m)).to(dtype)
+    _close(ms.linear(x.cuda(), wq), x.double(), wv, k, dtype)
+    if m <= 128:
+        t = P.random_matrix(m, k, fmt, torch.Generator().manual_seed(m))
+        _close(ms.matmul(P.pack(*t, fmt, "cuda"), wq, dtype), P.values(*t, fmt), wv, k, dtype)
+
+
+def test_products_of_every_size_at_once(ms):
+    """Kernels that take a whole SM, half of one and no tensor memory, in clusters of several sizes, from six streams at once."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    n, k = 1300, 4096
+    calls = []
+    for fmt in FMTS:
+        w = P.pack(*P.random_matrix(n, k, fmt, torch.Generator().manual_seed(0)), fmt, "cuda")
+        for m in (1, 16, 60, 100, 300):
+            x = torch.randn(m, k, generator=g, device="cuda").to(torch.bfloat16)
+            xq = ms.quantize(x, fmt)
+            calls += [lambda x=x, w=w: ms.linear(x, w), lambda x=xq, w=w: ms.matmul(x, w), lambda x=x.half(), w=w: ms.linear(x, w), lambda x=x[:40].float(), w=w: ms.linear(x, w)]
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(6)]
+    got = {}
+    for turn in range(6):
+        for i in range(len(calls)):
+            with torch.cuda.stream(streams[(i + turn) % 6]):
+                got[turn, i] = calls[i]()
+    torch.cuda.synchronize()
+    for (turn, i), y in got.items():
+        assert torch.equal(y, want[i]), (turn, i)
+
+
 @pytest.mark.parametrize("m", (3, 130))
 def test_rows_do_not_depend_on_each_other(ms, m):
     w = P.pack(*P.random_matrix(200, 640, "nvfp4", torch.Generator().manual_seed(0)), "nvfp4", "cuda")

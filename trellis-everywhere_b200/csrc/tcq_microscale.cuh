@@ -96,8 +96,9 @@ struct MsMatrix {
 };
 
 int ms_sm_count();             // of the current device
-// How many clusters of `size` CTAs run at once where a CTA takes an SM for itself: fewer than SMs / size, since a cluster lies within a group of SMs.
-int ms_most_clusters(const void* kernel, int threads, size_t smem, int size);
+// How many clusters of `size` CTAs, `ctas` (1 or 2) of which an SM holds, run at once: fewer than SMs * ctas / size, since a cluster lies within a
+// group of SMs.
+int ms_most_clusters(const void* kernel, int threads, size_t smem, int ctas, int size);
 int report_cuda_error(cudaError_t err, const char* where);     // tcq_capi.cu
 
 cudaError_t launch_ms_quantize(const void* x, int dtype, long long rows, long long k, long long ldx, int fmt, int rotate, const float* signs,

@@ -486,11 +486,13 @@ cudaError_t launch(FewArgs p, cudaStream_t stream) {
     p.k_tiles = int(ms_tiles_k(p.k));
     // S, a power of two (clusters of three and five run 20 % longer than of two and four), while all CTAs run at once.  us, nvfp4, one token, S = 1 / 2 / 4 / 8:
     // 4096 x 4096 14.2 / 9.1 / 6.8 / 6.5, 4096 x 12288 37.5 / 20.9 / 12.5 / 10.9, 12288 x 4096 14.6 / 12.9
-    const int slots = 2 * ms_sm_count();
+    // (4600 x 4096, which 8 would give more clusters than run at once: 14.6 / 9.3 / 8.8 / 10.6)
+    const auto kernel = tcq_ms_linear_few_kernel<T, FMT, PARTS>;
     int splits = 1;
-    while (splits < kMostSplits && splits * 2 <= p.k_tiles && p.tiles * splits * 2 <= slots) splits *= 2;
+    while (splits < kMostSplits && splits * 2 <= p.k_tiles &&
+           p.tiles <= ms_most_clusters(reinterpret_cast<const void*>(kernel), kThreads, G::kSmem, 2, splits * 2)) splits *= 2;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(splits > 1 ? p.tiles * splits : std::min(p.tiles, slots)));
+    cfg.gridDim = dim3(unsigned(splits > 1 ? p.tiles * splits : std::min(p.tiles, 2 * ms_sm_count())));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = G::kSmem;
     cfg.stream = stream;
@@ -500,7 +502,7 @@ cudaError_t launch(FewArgs p, cudaStream_t stream) {
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, tcq_ms_linear_few_kernel<T, FMT, PARTS>, map_w, p);
+    return cudaLaunchKernelEx(&cfg, kernel, map_w, p);
 }
 
 template <typename T, int PARTS>

@@ -404,6 +404,8 @@ __global__ void __launch_bounds__(kThreads<P>, Tile<FMT, NT, P>::kCtas) tcq_ms_l
     }
 }
 
+__global__ void __launch_bounds__(256) tcq_ms_scale_range_kernel(MsMatrix w, long long k, long long pitch, int atoms, unsigned int* wide, uint8_t* largest);
+
 template <typename YT, int FMT, int NT, int P, bool FP16>
 cudaError_t launch(const ManyCall& c, cudaStream_t stream) {
     using T = Tile<FMT, NT, P>;
@@ -413,6 +415,8 @@ cudaError_t launch(const ManyCall& c, cudaStream_t stream) {
     cudaError_t err = cudaGetDevice(&dev);
     if (err != cudaSuccess) return err;
     if (dev >= 64 || !ready[dev]) {
+        // The count of clusters that run at once takes a kernel with tensor memory to be alone on its SM: two of them are counted as another kernel's.
+        if (T::kCtas == 2 && (err = cudaFuncSetAttribute(tcq_ms_scale_range_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem)) != cudaSuccess) return err;
         if ((err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem)) != cudaSuccess) return err;
         if (dev < 64) ready[dev] = true;
     }
@@ -427,8 +431,9 @@ cudaError_t launch(const ManyCall& c, cudaStream_t stream) {
     // 4096 columns of 4096 rows by 8 instead of 4 costs 10.7 -> 11.7 us, 12288 of them 21.3 -> 20.2 us).
     const int k_tiles = int(ms_tiles_k(c.k)), sms = ms_sm_count();
     const auto fits = [&](int s) {
-        if (T::kCtas == 2) return tiles * s <= sms || (tiles * s <= 2 * sms && k_tiles >= 4 * s);
-        return tiles <= ms_most_clusters(reinterpret_cast<const void*>(kernel), kThreads<P>, T::kSmem, s);
+        if (T::kCtas == 2 && tiles * s > sms && k_tiles < 4 * s) return false;
+        return tiles <= (T::kCtas == 2 ? ms_most_clusters(reinterpret_cast<const void*>(tcq_ms_scale_range_kernel), 256, T::kSmem, 2, s)
+                                       : ms_most_clusters(reinterpret_cast<const void*>(kernel), kThreads<P>, T::kSmem, 1, s));
     };
     int splits = 1;
     while (NT <= 128 && splits < kMostSplits && 2 * splits <= k_tiles && fits(2 * splits)) splits *= 2;

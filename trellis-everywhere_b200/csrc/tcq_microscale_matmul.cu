@@ -312,7 +312,7 @@ cudaError_t launch(const MsMatrix& x, const MsMatrix& w, long long k, void* y, i
     const long long tiles = (long long)p.tiles_n * p.tiles_m;
     int splits = 1;
     while (p.k_tiles >= 8 && splits < kMostSplits && splits * 4 <= p.k_tiles &&
-           tiles <= ms_most_clusters(reinterpret_cast<const void*>(tcq_ms_matmul_kernel<FMT, NT>), kThreads, T::kSmem, splits * 2)) splits *= 2;
+           tiles <= ms_most_clusters(reinterpret_cast<const void*>(tcq_ms_matmul_kernel<FMT, NT>), kThreads, T::kSmem, 1, splits * 2)) splits *= 2;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(splits > 1 ? tiles * splits : std::min<long long>(tiles, ms_sm_count())));
     cfg.blockDim = dim3(kThreads);
@@ -363,12 +363,12 @@ int ms_sm_count() {
     return n;
 }
 
-int ms_most_clusters(const void* kernel, int threads, size_t smem, int size) {
-    static int cache[64][4] = {};                            // by log2(size); clusters of one CTA as well
-    const int slot = size >= 8 ? 3 : size / 2, sms = ms_sm_count();
+int ms_most_clusters(const void* kernel, int threads, size_t smem, int ctas, int size) {
+    static int cache[64][2][4] = {};                         // by ctas - 1 and log2(size)
+    const int slot = size >= 8 ? 3 : size / 2, most = ctas * ms_sm_count() / size;
     int dev = 0, n = 0;
-    if (size == 1 || cudaGetDevice(&dev) != cudaSuccess) return sms / size;
-    if (dev < 64 && cache[dev][slot]) return cache[dev][slot];
+    if (size == 1 || cudaGetDevice(&dev) != cudaSuccess) return most;
+    if (dev < 64 && cache[dev][ctas - 1][slot]) return cache[dev][ctas - 1][slot];
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(size));
     cfg.blockDim = dim3(unsigned(threads));
@@ -381,9 +381,9 @@ int ms_most_clusters(const void* kernel, int threads, size_t smem, int size) {
     cfg.numAttrs = 1;
     if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
         (void)cudaGetLastError();
-        return sms / size;
+        return most;
     }
-    if (dev < 64) cache[dev][slot] = n;
+    if (dev < 64) cache[dev][ctas - 1][slot] = n;
     return n;
 }
 
