@@ -523,3 +523,34 @@ def test_rotated_product_is_the_product(ms):
         y = ms.matmul(ms.quantize(x, **a), ms.quantize(w, **a), torch.float32).double()
         err[r] = float((y - want).norm() / want.norm())
     assert err[128] < 0.25
+
+
+def test_layers_with_several_names_and_subclasses(ms):
+    from trellis_b200 import quant
+    torch.manual_seed(2)
+    shared = torch.nn.Linear(64, 64)
+    model = torch.nn.ModuleDict({"a": shared, "b": torch.nn.ModuleDict({"c": shared}), "attn": torch.nn.MultiheadAttention(64, 4), "d": torch.nn.Linear(64, 32)}).cuda()
+    assert quant.apply_microscaled(model) == 2
+    assert model["a"] is model["b"]["c"] and isinstance(model["a"], quant.MicroscaledLinear) and isinstance(model["d"], quant.MicroscaledLinear)
+    x = torch.randn(5, 2, 64, device="cuda")
+    y, _ = model["attn"](x, x, x)
+    assert torch.equal(ms.linear(x, model["d"].weight) + model["d"].bias, model["d"](x)) and y.shape == x.shape
+
+
+def test_a_model_is_replaced_whole_or_not_at_all(ms):
+    from trellis_b200 import quant
+    model = torch.nn.Sequential(torch.nn.Linear(64, 48), torch.nn.Linear(48, 8)).cuda()
+    with pytest.raises(ValueError):
+        quant.apply_microscaled(model, activations=4, rotate=64)
+    assert all(type(m) is torch.nn.Linear for m in model)
+
+
+@pytest.mark.parametrize("activations", (4, 16))
+def test_module_refuses_inputs_that_need_a_gradient(ms, activations):
+    from trellis_b200 import quant
+    layer = quant.MicroscaledLinear(torch.randn(16, 32), activations=activations)
+    x = torch.randn(3, 32, device="cuda", requires_grad=True)
+    with pytest.raises(ValueError):
+        layer(x)
+    with torch.no_grad():
+        assert layer(x).shape == (3, 16)

@@ -35,12 +35,6 @@ __device__ __forceinline__ long long ms_scale_at(long long r, int b, long long a
     return ((r >> 7) * atoms + (b >> 2)) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4 + (b & 3);
 }
 
-// Two e2m1 codes (low half first) as fp16 pairs; every value is exact.
-__device__ __forceinline__ uint32_t e2m1x2_to_f16x2(uint32_t byte) {
-    uint32_t r;
-    asm("{\n\t.reg .b8 b;\n\tcvt.u8.u32 b, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, b;\n\t}" : "=r"(r) : "r"(byte));
-    return r;
-}
 // Nearest e2m1 codes of two values (ties to the even code, beyond 6 to 6, the sign kept); lo in the low half of the byte.
 __device__ __forceinline__ uint32_t f32x2_to_e2m1x2(float lo, float hi) {
     uint32_t r;

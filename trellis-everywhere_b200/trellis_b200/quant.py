@@ -83,7 +83,7 @@ class MicroscaleQuantizer(Quantizer):
 
 
 class MicroscaledLinear(nn.Module):
-    """``nn.Linear`` for inference with its weight in 4 bits.
+    """``nn.Linear`` for inference with its weight in 4 bits (no gradient: inputs that need one are refused).
 
     ``activations=16``: inputs stay as they are (``microscale.linear``).  ``activations=4``: inputs are quantised token by
     token (``microscale.quantize``) and both sides multiplied in 4 bits (``microscale.matmul``); ``rotate`` then puts both
@@ -120,7 +120,6 @@ class MicroscaledLinear(nn.Module):
     def weight(self) -> "microscale.Microscaled":
         return microscale.Microscaled(self.codes, self.scales, self.row_scale, (self.out_features, self.in_features), self.fmt)
 
-    @torch.no_grad()
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if self.activations == 16:
             y = microscale.linear(x, self.weight)
@@ -152,10 +151,22 @@ def apply_fake_quant(model: nn.Module, quantizer: Quantizer, skip: Callable[[str
 @torch.no_grad()
 def apply_microscaled(model: nn.Module, fmt: str = "nvfp4", activations: int = 16, rotate: int = 0,
                       skip: Callable[[str], bool] = lambda n: False) -> int:
-    """Replace every ``nn.Linear`` by a ``MicroscaledLinear`` (seeds by name, as ``seed_from_name``). Returns the count."""
-    found = [(name, mod) for name, mod in model.named_modules() if isinstance(mod, nn.Linear) and name and not skip(name)]
+    """Replace every ``nn.Linear`` below ``model`` by a ``MicroscaledLinear`` (seeds by name, as ``seed_from_name``). Returns the count.
+
+    A layer that stands under several names is replaced under each that is not skipped, by one ``MicroscaledLinear``.  Subclasses of
+    ``nn.Linear`` stay: they may do more than its product, or their owner may read their weight (``nn.MultiheadAttention`` does).
+    All is checked before the first layer is replaced.
+    """
+    microscale._check_fmt(fmt)
+    found = [(name, mod) for name, mod in model.named_modules(remove_duplicate=False) if type(mod) is nn.Linear and name and not skip(name)]
     for name, mod in found:
+        if rotate and mod.in_features % rotate:
+            raise ValueError(f"{name}: rotate={rotate} does not divide its {mod.in_features} input channels")
+        microscale._check_dtype(mod.weight.dtype)
+    made = {}
+    for name, mod in found:
+        if mod not in made:
+            made[mod] = MicroscaledLinear(mod.weight.data, mod.bias, fmt, activations, rotate, seed_from_name(name))
         parent, _, leaf = name.rpartition(".")
-        setattr(model.get_submodule(parent), leaf,
-                MicroscaledLinear(mod.weight.data, mod.bias, fmt, activations, rotate, seed_from_name(name)))
-    return len(found)
+        setattr(model.get_submodule(parent), leaf, made[mod])
+    return len(made)
