@@ -389,6 +389,15 @@ def test_shared_columns_within_rounding(ms, fmt, dtype, m, n, k):
         _close(ms.matmul(P.pack(*t, fmt, "cuda"), wq, dtype), P.values(*t, fmt), wv, k, dtype)
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype,m,n,k", ((torch.float16, 7, 300, 32000), (torch.bfloat16, 8, 130, 32700), (torch.float32, 2, 260, 32000), (torch.float32, 8, 40000, 1000)))
+def test_few_tokens_beside_two_stages(ms, fmt, dtype, m, n, k):
+    """All of a CTA's columns of x are held where one stage less of the weights makes room for them."""
+    w = P.random_matrix(n, k, fmt, torch.Generator().manual_seed(n))
+    x = torch.randn(m, k, generator=torch.Generator().manual_seed(m)).to(dtype)
+    _close(ms.linear(x.cuda(), P.pack(*w, fmt, "cuda")), x.double(), P.values(*w, fmt), k, dtype)
+
+
 def test_products_of_every_size_at_once(ms):
     """Kernels that take a whole SM, half of one and no tensor memory, in clusters of several sizes, from six streams at once."""
     g = torch.Generator(device="cuda").manual_seed(1)

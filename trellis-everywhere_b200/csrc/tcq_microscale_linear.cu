@@ -26,17 +26,19 @@ namespace tcq {
 namespace {
 
 constexpr int kConsumers = 256, kThreads = kConsumers + 32, kRows = 128, kMostSplits = 8, kTokens = 8;
-constexpr int kPitchX = 576;                     // bytes of a token's 256 columns: 512 and a step to other banks
 
-template <int FMT, int PARTS>
+template <int FMT, int PARTS, int STAGES>
 struct Tile {
     static constexpr int kAtoms = Ms<FMT>::kAtoms;
     static constexpr int kBytesW = kRows * 128, kBytesS = kAtoms * 512, kStage = kBytesW + 2048;
-    static constexpr int kStages = 3;
-    static constexpr int kRowsX = 88;                                         // rows of 256 columns held: at least two times eight tokens' parts
     static constexpr int kBytesSum = kTokens * kRows * 4;
-    static constexpr int kSmem = kStages * kStage + (kRowsX + 1) * kPitchX + kBytesSum + 1024;
-    static_assert(kSmem <= 113 * 1024 && kRowsX >= 2 * PARTS * kTokens);      // two CTAs an SM
+    // A token's 256 columns: 512 bytes, for the banks either with odd tokens' pieces of 64 bytes swapped in twos or (three parts have no registers
+    // for that: 1.2 times the time) another 64 bytes.  So many of them are held beside three stages, and beside two.
+    static constexpr bool kSwapped = PARTS == 1;
+    static constexpr int kPitchX = kSwapped ? 512 : 576, kRowsX3 = kSwapped ? 100 : 88;
+    static constexpr int kRowsX = kRowsX3 + (3 - STAGES) * (kStage / kPitchX);
+    static constexpr int kSmem = 3 * kStage + (kRowsX3 + 1) * kPitchX + kBytesSum + 1024;
+    static_assert(kSmem <= 113 * 1024 && kRowsX3 >= 2 * PARTS * kTokens);      // two CTAs an SM; at least two times eight tokens' parts
 };
 
 struct FewArgs {
@@ -163,14 +165,14 @@ __device__ __forceinline__ bool any_of_consumers(bool mine) {
 }
 
 // PARTS of x held at a time.
-template <typename T, int FMT, int PARTS>
+template <typename T, int FMT, int PARTS, int STAGES>
 __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ FewArgs p) {
-    using G = Tile<FMT, PARTS>;
+    using G = Tile<FMT, PARTS, STAGES>;
     extern __shared__ uint8_t raw[];
-    __shared__ uint64_t full[G::kStages], empty[G::kStages];
+    __shared__ uint64_t full[STAGES], empty[STAGES];
     __shared__ float factor[G::kRowsX];
     __shared__ unsigned int gave_up;
-    const uint32_t smem = (smem_u32(raw) + 1023) & ~1023u, smem_x = smem + G::kStages * G::kStage, zeros = smem_x + G::kRowsX * kPitchX, smem_sum = zeros + kPitchX;
+    const uint32_t smem = (smem_u32(raw) + 1023) & ~1023u, smem_x = smem + STAGES * G::kStage, zeros = smem_x + G::kRowsX * G::kPitchX, smem_sum = zeros + G::kPitchX;
     float* const sums = reinterpret_cast<float*>(raw + (smem_sum - smem_u32(raw)));
     const int warp = __shfl_sync(0xFFFFFFFFu, int(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank(), splits = cluster_size();
@@ -184,11 +186,11 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
         bulk_load(to + G::kBytesW, p.w.scales + (t * p.atoms + (long long)kt * G::kAtoms) * 512, G::kBytesS, bar);
     };
     // The first stages are on their way before anything else: a small call is little more than its latencies.
-    const int ahead = min(G::kStages, last - first);
+    const int ahead = min(STAGES, last - first);
     if (warp == 8) {
         if (elect_one()) {
             gave_up = 0;
-            for (int s = 0; s < G::kStages; ++s) { mbar_init(smem_u32(&full[s]), 1); mbar_init(smem_u32(&empty[s]), 8); }
+            for (int s = 0; s < STAGES; ++s) { mbar_init(smem_u32(&full[s]), 1); mbar_init(smem_u32(&empty[s]), 8); }
             asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
             for (int i = 0; i < ahead; ++i) load(i, blockIdx.x / splits, first + i);
         }
@@ -199,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
     if (warp == 8) {
         // ---- loads; the warp stays together, one lane issues
         const bool one = elect_one();
-        uint32_t s = ahead % G::kStages, phase = ahead == G::kStages ? 0 : 1, loaded = ahead;    // (the first wait for a stage is for the phase before the first)
+        uint32_t s = ahead == STAGES ? 0 : ahead, phase = ahead == STAGES ? 0 : 1, loaded = ahead;    // (the first wait for a stage is for the phase before the first)
         bool ok = true;
         int kt = first + ahead;
         for (int t = blockIdx.x / splits; t < p.tiles && ok; t += clusters, kt = first)
@@ -208,17 +210,18 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
                 if (!ok) break;
                 if (one) load(s, t, kt);
                 __syncwarp();
-                if (++s == G::kStages) { s = 0; phase ^= 1; }
-                if (loaded < G::kStages) ++loaded;
+                if (++s == STAGES) { s = 0; phase ^= 1; }
+                if (loaded < STAGES) ++loaded;
             }
         if (gave_up)                                     // nothing may be on its way to this CTA's memory when it ends: the last loads of each stage
             for (uint32_t i = 0; i < loaded; ++i) {
                 if (s == 0) phase ^= 1;
-                s = s == 0 ? G::kStages - 1 : s - 1;
+                s = s == 0 ? STAGES - 1 : s - 1;
                 for (long long t0 = clock64(); !mbar_try_wait(smem_u32(&full[s]), phase ^ 1) && clock64() - t0 < kMbarWaitCycles;) {}
             }
     } else {
         const int g = lane >> 2, t4 = lane & 3;
+        const uint32_t odd = G::kSwapped ? 64 * (g & 1) : 0;
         const bool converts = warp < p.m;                // a warp converts a token's columns, eight a lane
         float next[8], r[8];
         auto fetch = [&](int kt, int token) {
@@ -247,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
 #pragma unroll
             for (int q = 0; q < PARTS; ++q) {
                 const int row = (n * PARTS + q) * p.m + token;
-                sts128(smem_x + row * kPitchX + 16 * lane, h[q]);
+                sts128(smem_x + row * G::kPitchX + ((16 * lane) ^ (G::kSwapped ? 64 * (token & 1) : 0)), h[q]);
                 if (lane == 0) factor[row] = f[q];
             }
             return left;
@@ -301,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
                     for (int q = 0; q < PARTS; ++q) {
                         const int row = ((held ? kt - first : buf) * PARTS + q) * p.m;
                         by[q] = pack2(2 * t4 < p.m ? factor[row + 2 * t4] : 0.0f, 2 * t4 + 1 < p.m ? factor[row + 2 * t4 + 1] : 0.0f);
-                        from_x[q] = (g < p.m ? smem_x + (row + g) * kPitchX : zeros) + 16 * t4;
+                        from_x[q] = (g < p.m ? smem_x + (row + g) * G::kPitchX : zeros) + 16 * t4;
                     }
 #pragma unroll
                     for (int c = 0; c < 8; c += 2) {     // 64 columns
@@ -336,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
                             const uint32_t lo[4] = {a0[0], a1[0], a0[1], a1[1]}, hi[4] = {a0[2], a1[2], a0[3], a1[3]};
 #pragma unroll
                             for (int q = 0; q < PARTS; ++q) {
-                                const uint4 b = lds128(from_x[q] + 64 * (c + i));
+                                const uint4 b = lds128((i ? from_x[q] - odd : from_x[q] + odd) + 64 * (c + i));
                                 if constexpr (FMT == kNvfp4) {
                                     mma_f16(sum[q], lo, b.x, b.y);
                                     mma_f16(sum[q], hi, b.z, b.w);
@@ -375,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
                 if (!ok) acc[0] = acc[1] = acc[2] = acc[3] = __uint_as_float(0x7FC00000u);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&empty[s]));
-                if (++s == G::kStages) { s = 0; phase ^= 1; }
+                if (++s == STAGES) { s = 0; phase ^= 1; }
                 if (!held && kt + 1 < last) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) r[i] = next[i];
@@ -468,13 +471,15 @@ __global__ void __launch_bounds__(256) tcq_ms_pad_kernel(const uint16_t* __restr
 
 template <typename T, int FMT, int PARTS>
 cudaError_t launch(FewArgs p, cudaStream_t stream) {
-    using G = Tile<FMT, PARTS>;
+    using G = Tile<FMT, PARTS, 3>;
+    const auto three = tcq_ms_linear_few_kernel<T, FMT, PARTS, 3>, two = tcq_ms_linear_few_kernel<T, FMT, PARTS, 2>;
     static bool ready[64] = {};
     int dev = 0;
     cudaError_t err = cudaGetDevice(&dev);
     if (err != cudaSuccess) return err;
     if (dev >= 64 || !ready[dev]) {
-        if ((err = cudaFuncSetAttribute(tcq_ms_linear_few_kernel<T, FMT, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmem)) != cudaSuccess) return err;
+        for (const auto kernel : {three, two})
+            if ((err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmem)) != cudaSuccess) return err;
         if (dev < 64) ready[dev] = true;
     }
     CUtensorMap map_w;
@@ -487,10 +492,12 @@ cudaError_t launch(FewArgs p, cudaStream_t stream) {
     // S, a power of two (clusters of three and five run 20 % longer than of two and four), while all CTAs run at once.  us, nvfp4, one token, S = 1 / 2 / 4 / 8:
     // 4096 x 4096 14.2 / 9.1 / 6.8 / 6.5, 4096 x 12288 37.5 / 20.9 / 12.5 / 10.9, 12288 x 4096 14.6 / 12.9
     // (4600 x 4096, which 8 would give more clusters than run at once: 14.6 / 9.3 / 8.8 / 10.6)
-    const auto kernel = tcq_ms_linear_few_kernel<T, FMT, PARTS>;
     int splits = 1;
     while (splits < kMostSplits && splits * 2 <= p.k_tiles &&
-           p.tiles <= ms_most_clusters(reinterpret_cast<const void*>(kernel), kThreads, G::kSmem, 2, splits * 2)) splits *= 2;
+           p.tiles <= ms_most_clusters(reinterpret_cast<const void*>(three), kThreads, G::kSmem, 2, splits * 2)) splits *= 2;
+    // One stage less where that makes room for all of x: eight tokens through 40960 x 4096 48.0 -> 41.4 us, 151936 x 4096 132 -> 91.5.
+    const int rows_x = (p.k_tiles + splits - 1) / splits * PARTS * p.m;
+    const auto kernel = rows_x > G::kRowsX && rows_x <= Tile<FMT, PARTS, 2>::kRowsX ? two : three;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(splits > 1 ? p.tiles * splits : std::min(p.tiles, 2 * ms_sm_count())));
     cfg.blockDim = dim3(kThreads);
