@@ -250,7 +250,8 @@ __global__ void __launch_bounds__(kThreads<P>, Tile<FMT, NT, P>::kCtas) tcq_ms_l
                     const uint32_t scales = smem_w + sw * T::kStageW + T::kBytesW + lane * 16 + quarter * 4;
                     if constexpr (FMT == kNvfp4) word = lds32(scales + 512 * sub);
                     else word = lds32(scales + 512 * (sub / 2)) >> (16 * (sub & 1));
-                    uint32_t v[32];
+                    uint32_t v[32], scales16[4];
+                    if constexpr (!FP16) four_scales<FMT>(word, scales16);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {        // 16 bytes: 32 columns; the swizzle has put piece c of row r at c ^ (r % 8)
                         const uint4 c = lds128(from + (((2 * sub + i) ^ (row & 7)) << 4));
@@ -275,9 +276,10 @@ __global__ void __launch_bounds__(kThreads<P>, Tile<FMT, NT, P>::kCtas) tcq_ms_l
                         } else {
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
-                                const __nv_bfloat162 s = scale_of<FMT>(word, 2 * i + j / 2);
-                                four_weights(cw[j], s, v[16 * i + 4 * j], v[16 * i + 4 * j + 1]);
-                                four_weights(cw[j] >> 16, s, v[16 * i + 4 * j + 2], v[16 * i + 4 * j + 3]);
+                                uint32_t h[4];
+                                eight_weights(cw[j], scales16[2 * i + j / 2], h);
+#pragma unroll
+                                for (int q = 0; q < 4; ++q) v[16 * i + 4 * j + q] = h[q];
                             }
                         }
                     }
