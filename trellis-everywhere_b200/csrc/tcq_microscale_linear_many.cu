@@ -237,6 +237,7 @@ __global__ void __launch_bounds__(kThreads<P>, Tile<FMT, NT, P>::kCtas) tcq_ms_l
         // ---- weights: lane = row of this warp's quarter; the groups of four warps take turns
         const int quarter = warp & 3, mine = (warp - 6) >> 2;
         const int row = 32 * quarter + lane;
+        const E2m1Bytes bytes;
         uint32_t sw = 0, pw = 0, sa = 0, pa = 1;
         bool ok = true;
         for (int t = blockIdx.x / splits; t < tiles && ok; t += clusters) {
@@ -277,7 +278,7 @@ __global__ void __launch_bounds__(kThreads<P>, Tile<FMT, NT, P>::kCtas) tcq_ms_l
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
                                 uint32_t h[4];
-                                eight_weights(cw[j], scales16[2 * i + j / 2], h);
+                                eight_weights(bytes, cw[j], scales16[2 * i + j / 2], h);
 #pragma unroll
                                 for (int q = 0; q < 4; ++q) v[16 * i + 4 * j + q] = h[q];
                             }

@@ -5,19 +5,29 @@
 
 namespace tcq {
 
+// The magnitudes 0 .5 1 1.5 2 3 4 6 as bf16 numbers: low bytes 00 00 80 C0 00 40 80 C0, high bytes 00 3F 3F 3F 40 40 40 40.  Made so that they stay in registers
+// (the compiler would put each anew before every use: a third more instructions).
+struct E2m1Bytes {
+    uint32_t low0, low1, high0, high1;
+    __device__ __forceinline__ E2m1Bytes() {
+        asm volatile("mov.b32 %0, 0xC0800000;\n\tmov.b32 %1, 0xC0804000;\n\tmov.b32 %2, 0x3F3F3F00;\n\tmov.b32 %3, 0x40404040;" : "=r"(low0), "=r"(low1), "=r"(high0), "=r"(high1));
+    }
+};
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t pick) {      // (__byte_perm masks what picks)
+    uint32_t r;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(pick));
+    return r;
+}
 // Eight codes as bf16 pairs in order, times the scale.  Two byte permutations look four magnitudes up as the bytes of bf16 numbers, one spreads the
 // signs; these half-rate instructions are what bounds it, so what can be shared by all eight is.
-__device__ __forceinline__ void eight_weights(uint32_t w, uint32_t scale, uint32_t (&out)[4]) {
+__device__ __forceinline__ void eight_weights(const E2m1Bytes& e, uint32_t w, uint32_t scale, uint32_t (&out)[4]) {
     const uint32_t mag = w & 0x77777777u, up = w << 4;
-    uint32_t sign[2];
-    asm("prmt.b32 %0, %1, %2, 0x9D8C;" : "=r"(sign[0]) : "r"(w), "r"(up));            // the top bit of each code, over a whole byte
-    asm("prmt.b32 %0, %1, %2, 0xBFAE;" : "=r"(sign[1]) : "r"(w), "r"(up));
+    const uint32_t sign[2] = {prmt(w, up, 0x9D8Cu), prmt(w, up, 0xBFAEu)};            // the top bit of each code, over a whole byte
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const uint32_t four = mag >> (16 * i);
-        const uint32_t lo = __byte_perm(0xC0800000u, 0xC0804000u, four);              // 0 .5 1 1.5 2 3 4 6: low bytes 00 00 80 C0 00 40 80 C0
-        const uint32_t hi = __byte_perm(0x3F3F3F00u, 0x40404040u, four) | (sign[i] & 0x80808080u);           // high bytes 00 3F 3F 3F 40 40 40 40
-        const uint32_t p = __byte_perm(lo, hi, 0x5140), q = __byte_perm(lo, hi, 0x7362);
+        const uint32_t lo = prmt(e.low0, e.low1, four), hi = prmt(e.high0, e.high1, four) | (sign[i] & 0x80808080u);
+        const uint32_t p = prmt(lo, hi, 0x5140u), q = prmt(lo, hi, 0x7362u);
         asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(out[2 * i]) : "r"(p), "r"(scale));
         asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(out[2 * i + 1]) : "r"(q), "r"(scale));
     }
