@@ -247,6 +247,50 @@ def test_fp16_times_scales_far_apart(ms, m, apart):
     assert torch.equal(ms.linear(x.cuda(), P.pack(codes, byte, None, "mxfp4", "cuda")).cpu(), want.half())
 
 
+@pytest.mark.parametrize("m,n", ((2000, 300), (200, 2500)))
+@pytest.mark.parametrize("apart", (36, 37, 100))
+def test_many_fp16_tokens_times_scales_far_apart(ms, m, n, apart):
+    """The same where there are enough tiles for fp16 weights: rows that these hold, and rows that they do not, with NaN blocks and rows at any address."""
+    k = 328
+    g = torch.Generator().manual_seed(apart)
+    codes = torch.randint(0, 16, (n, k), generator=g)
+    byte = torch.full((n, 11), 127)
+    byte[::3, 2:4], byte[::3, 4] = 127 - apart + 3, 127 + 3
+    byte[:, 1], codes[:, 32:64] = 0, 0
+    x = torch.zeros(m, k, dtype=torch.float16)
+    hot = torch.randint(0, 11, (m,), generator=g)                     # whole numbers in one block of columns a token: exact sums
+    for i in range(m):
+        part = x[i, 32 * hot[i]:32 * hot[i] + 32]
+        part.copy_(torch.randint(-8, 9, (len(part),), generator=g) * (2.0 ** (10 if hot[i] in (2, 3) else 0)))
+    want = (x.double() @ P.values(codes, byte, None, "mxfp4").t()).half()
+    w = P.pack(codes, byte, None, "mxfp4", "cuda")
+    wide = torch.full((m, k + 3), float("nan"), dtype=torch.float16, device="cuda")
+    for lo in (0, 1, 3):
+        wide.fill_(float("nan"))
+        wide[:, lo:lo + k] = x.cuda()
+        assert torch.equal(ms.linear(wide[:, lo:lo + k], w).cpu(), want)
+    held = x.cuda()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ms.linear(held, w)
+    for sign in (-1, 1):
+        held.copy_(x * sign)
+        graph.replay()
+        assert torch.equal(out.cpu(), want * sign)
+    byte[5, 6] = 255
+    got = ms.linear(x.cuda(), P.pack(codes, byte, None, "mxfp4", "cuda")).cpu()
+    assert torch.isnan(got[:, 5]).all()
+    got[:, 5], want[:, 5] = 0, 0
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("m,n,k", ((1300, 520, 768), (200, 2433, 257), (4800, 1, 64), (2401, 129, 31)))
+def test_many_fp16_tokens_times_whole_numbers(ms, m, n, k):
+    w = _whole_number_case(n, k, "mxfp4", n + k)
+    x = torch.randint(-8, 9, (m, k), generator=torch.Generator().manual_seed(m)).half()
+    assert torch.equal(ms.linear(x.cuda(), P.pack(*w, "mxfp4", "cuda")).cpu(), (x.double() @ P.values(*w, "mxfp4").t()).half())
+
+
 @pytest.mark.parametrize("fmt", FMTS)
 def test_scales_at_the_ends_of_their_range(ms, fmt):
     """The smallest and the largest scales of a format, in the weights and (products of both) in the activations."""

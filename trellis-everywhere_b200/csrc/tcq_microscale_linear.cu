@@ -550,14 +550,17 @@ cudaError_t launch_ms_linear(const void* x, int dtype, long long m, long long ld
     uint8_t* const scratch = static_cast<uint8_t*>(ws);
     ManyCall c{x, ldx, k, m, 1, dtype, w, k, fmt, y, ldy, false, nullptr, nullptr};
     cudaError_t err;
-    if (dtype == kBf16 || (dtype == kF16 && (fmt == kNvfp4 || m > 128))) {
+    // fp16 through mxfp4: up to 128 tokens, and while tiles of 64 leave half of the SMs free, two bf16 parts (200 through 1024 x 4096 15.4 us), else fp16
+    // weights (23.4; but through 4096 x 12288 52.5 instead of 69.5, 12288 x 4096 39 instead of 53).
+    const bool fp16 = dtype == kF16 && (fmt == kNvfp4 || (m > 128 && (w.rows + 127) / 128 * ((m + 63) / 64) * 2 > ms_sm_count()));
+    if (dtype == kBf16 || fp16) {
         if (!rows_aligned(x, ldx)) {
             tcq_ms_pad_kernel<<<grid, 256, 0, stream>>>(static_cast<const uint16_t*>(x), m, k, ldx, static_cast<uint16_t*>(ws), width);
             if ((err = cudaGetLastError()) != cudaSuccess) return err;
             c.x = ws;
             c.ldx = c.width = width;
         }
-        c.fp16 = dtype == kF16;
+        c.fp16 = fp16;
         if (dtype == kBf16 || fmt == kNvfp4) return launch_ms_linear_many(c, stream);
         // fp16 weights: nvfp4's always are; mxfp4's where no row's scales are further apart than fp16 reaches, which the GPU finds out by itself: one of
         // the two forms behind it runs (8 us of small launches: for many tokens; 1000 through 12288 x 4096 184 -> 88 us).

@@ -11,7 +11,7 @@
 // one issues products, eight make weights (two groups of four take turns), four take finished sums out of tensor memory.  With few tokens a
 // cluster of S CTAs shares the columns of a tile; the partial sums meet through distributed shared memory, in rank order.
 //
-// Bound by the making of weights, beside the tensor cores (57 % busy): 1000 tokens through 12288 x 4096 82 us (1.22 PFLOP/s), mxfp4 97; fp16 76 and 88.
+// Bound by the making of weights, beside the tensor cores (57 % busy): 1000 tokens through 12288 x 4096 82 us (1.22 PFLOP/s), mxfp4 83; fp16 76 and 88.
 //
 // A wait that runs out (kMbarWaitCycles) makes its CTA stop, and its results NaN.
 #include <algorithm>
@@ -34,7 +34,7 @@ constexpr int kMostSplits = 8;
 template <int FMT, int NT, int P>
 struct Tile {
     // Up to 64 rows of x two CTAs share an SM: making weights is what takes the time, and eight warps do not fill the SM
-    // (16 through 40960 x 4096: 67.4 -> 54.6 us, mxfp4 85.5 -> 66.2).
+    // (16 through 40960 x 4096 67.4 -> 54.6 us).
     static constexpr int kCtas = NT <= 64 && P != 3 ? 2 : 1;
     static constexpr int kAtoms = Ms<FMT>::kAtoms;
     static constexpr int kBytesW = kRows * 128, kBytesS = kAtoms * 512, kStageW = kBytesW + 2048, kStagesW = 3;      // 256 columns
