@@ -442,6 +442,19 @@ def test_few_tokens_beside_two_stages(ms, fmt, dtype, m, n, k):
     _close(ms.linear(x.cuda(), P.pack(*w, fmt, "cuda")), x.double(), P.values(*w, fmt), k, dtype)
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype,m,n,k", ((torch.bfloat16, 1, 40900, 1100), (torch.float16, 5, 77000, 600), (torch.float32, 3, 38000, 513), (torch.bfloat16, 8, 37900, 1300), (torch.float16, 2, 151936, 257)))
+def test_few_tokens_through_many_rows(ms, fmt, dtype, m, n, k):
+    """More groups of rows than CTAs: whole ones in turns, then the last ones shared."""
+    w = _whole_number_case(n, k, fmt, n + k)
+    x = torch.randint(-8, 9, (m, k), generator=torch.Generator().manual_seed(m)).to(dtype)
+    wq = P.pack(*w, fmt, "cuda")
+    got = ms.linear(x.cuda(), wq)
+    assert torch.equal(got.cpu(), (x.double() @ P.values(*w, fmt).t()).to(dtype))
+    again = [ms.linear(x.cuda(), wq) for _ in range(3)]
+    assert all(torch.equal(y, got) for y in again)
+
+
 def test_products_of_every_size_at_once(ms):
     """Kernels that take a whole SM, half of one and no tensor memory, in clusters of several sizes, from six streams at once."""
     g = torch.Generator(device="cuda").manual_seed(1)

@@ -9,10 +9,10 @@
 //
 // Work split: a CTA takes 128 rows of W, eight warps 16 rows each; one more warp loads 256 columns of codes (TMA) and scales at a time into a ring
 // of stages.  ldmatrix gives lane (g, t) the t-th eight codes of 32 columns of rows g and g + 8, two products' share.  x is converted
-// once where all columns of a CTA fit beside the stages, else a token a warp, for the next stage while this one is multiplied.  Where there are few groups of 128 rows a cluster of S CTAs
-// shares the columns, and the partial sums meet through distributed shared memory, in rank order.
+// once where all columns of a CTA fit beside the stages, else a token a warp, for the next stage while this one is multiplied.  Where there are few groups of 128 rows a
+// cluster of S CTAs shares the columns, and the partial sums meet through distributed shared memory, in rank order; of many groups, so are the last ones.
 //
-// Bound by instruction issue and its latencies (54 % of the slots): one token through 40960 x 4096 31.4 us (3.0 TB/s), mxfp4 28.8; eight 40.2 and 36.9.
+// Bound by instruction issue and its latencies (54 % of the slots): one token through 40960 x 4096 27.2 us (3.5 TB/s), mxfp4 23.3; eight 34.4 and 31.0.
 //
 // A wait that runs out (kMbarWaitCycles) makes its CTA's results NaN.
 #include <algorithm>
@@ -51,7 +51,7 @@ struct FewArgs {
     long long k;
     MsMatrix w;
     long long atoms;
-    int tiles, k_tiles;
+    int tiles, whole, k_tiles;                   // groups of 128 rows of W; how many of them a CTA does by itself
     void* y;
     long long ldy;
 };
@@ -178,8 +178,10 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
     float* const sums = reinterpret_cast<float*>(raw + (smem_sum - smem_u32(raw)));
     const int warp = __shfl_sync(0xFFFFFFFFu, int(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank(), splits = cluster_size();
-    const int first = int((long long)p.k_tiles * rank / splits), last = int((long long)p.k_tiles * (rank + 1) / splits);
-    const int clusters = gridDim.x / splits;
+    // What this CTA does: groups of rows blockIdx.x, blockIdx.x + gridDim.x ... of the first `whole`, and with its cluster, columns share .. until, one of the others.
+    const int share = int((long long)p.k_tiles * rank / splits), until = int((long long)p.k_tiles * (rank + 1) / splits);
+    const int together = p.whole + blockIdx.x / splits;
+    const int ends = p.whole + (splits > 1 && together < p.tiles ? int(gridDim.x) : 0);
 
     auto load = [&](uint32_t s, int t, int kt) {
         const uint32_t to = smem + s * G::kStage, bar = smem_u32(&full[s]);
@@ -188,13 +190,13 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
         bulk_load(to + G::kBytesW, p.w.scales + (t * p.atoms + (long long)kt * G::kAtoms) * 512, G::kBytesS, bar);
     };
     // The first stages are on their way before anything else: a small call is little more than its latencies.
-    const int ahead = min(STAGES, last - first);
+    const int ahead = min(STAGES, p.whole ? p.k_tiles : until - share);
     if (warp == 8) {
         if (elect_one()) {
             gave_up = 0;
             for (int s = 0; s < STAGES; ++s) { mbar_init(smem_u32(&full[s]), 1); mbar_init(smem_u32(&empty[s]), 8); }
             asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
-            for (int i = 0; i < ahead; ++i) load(i, blockIdx.x / splits, first + i);
+            for (int i = 0; i < ahead; ++i) load(i, p.whole ? blockIdx.x : together, (p.whole ? 0 : share) + i);
         }
         __syncwarp();
     }
@@ -205,12 +207,11 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
         const bool one = elect_one();
         uint32_t s = ahead == STAGES ? 0 : ahead, phase = ahead == STAGES ? 0 : 1, loaded = ahead;    // (the first wait for a stage is for the phase before the first)
         bool ok = true;
-        int kt = first + ahead;
-        for (int t = blockIdx.x / splits; t < p.tiles && ok; t += clusters, kt = first)
-            for (; kt < last; ++kt) {
+        for (int t = blockIdx.x, skip = ahead; t < ends && ok; t += gridDim.x, skip = 0)
+            for (int kt = (t < p.whole ? 0 : share) + skip; kt < (t < p.whole ? p.k_tiles : until); ++kt) {
                 ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&empty[s]), phase, &gave_up));
                 if (!ok) break;
-                if (one) load(s, t, kt);
+                if (one) load(s, t < p.whole ? t : together, kt);
                 __syncwarp();
                 if (++s == STAGES) { s = 0; phase ^= 1; }
                 if (loaded < STAGES) ++loaded;
@@ -271,11 +272,12 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
         const uint32_t from_s = G::kBytesW + (srow & 31) * 16 + (srow >> 5) * 4;
 
         // Where all of this CTA's columns fit, they are converted once, by all warps; unless that leaves something, which takes further rounds.
-        bool held = (last - first) * PARTS * p.m <= G::kRowsX;
+        const int base = p.whole ? 0 : share, span = p.whole ? p.k_tiles : until - share;
+        bool held = span * PARTS * p.m <= G::kRowsX;
         if (held) {
             bool left = false;
-            for (int i = warp; i < (last - first) * p.m; i += 8) {
-                fetch(first + i / p.m, i % p.m);
+            for (int i = warp; i < span * p.m; i += 8) {
+                fetch(base + i / p.m, i % p.m);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) r[j] = next[j];
                 left = convert_one(i / p.m, i % p.m) || left;
@@ -283,7 +285,8 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
             held = !any_of_consumers(left);
         }
 
-        for (int tile = blockIdx.x / splits; tile < p.tiles; tile += clusters) {
+        for (int t = blockIdx.x; t < ends; t += gridDim.x) {
+            const int first = t < p.whole ? 0 : share, last = t < p.whole ? p.k_tiles : until;
             float acc[4] = {}, low[4] = {};              // rows g (0, 1) and g + 8, tokens 2 t4 and 2 t4 + 1; what the sums' rounding left
             int buf = 0;
             bool more = false;
@@ -304,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
                     uint32_t from_x[PARTS];
 #pragma unroll
                     for (int q = 0; q < PARTS; ++q) {
-                        const int row = ((held ? kt - first : buf) * PARTS + q) * p.m;
+                        const int row = ((held ? kt - base : buf) * PARTS + q) * p.m;
                         by[q] = pack2(2 * t4 < p.m ? factor[row + 2 * t4] : 0.0f, 2 * t4 + 1 < p.m ? factor[row + 2 * t4 + 1] : 0.0f);
                         from_x[q] = (g < p.m ? smem_x + (row + g) * G::kPitchX : zeros) + 16 * t4;
                     }
@@ -391,10 +394,10 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
 #pragma unroll
             for (int i = 0; i < 4; ++i)                  // (an infinite or NaN sum leaves NaN behind)
                 sums[(2 * t4 + (i & 1)) * kRows + 16 * warp + g + 8 * (i >> 1)] = fabsf(low[i]) < __uint_as_float(0x7F800000u) ? acc[i] + low[i] : acc[i];
-            if (splits == 1) {
+            if (t < p.whole) {
                 any_of_consumers(false);
                 for (int i = threadIdx.x; i < p.m * kRows; i += kConsumers) {
-                    const long long row = (long long)tile * kRows + i % kRows;
+                    const long long row = (long long)t * kRows + i % kRows;
                     if (row < p.w.rows) {
                         float f = sums[i];
                         if constexpr (FMT == kNvfp4) f *= p.w.row_scale[row];
@@ -408,8 +411,8 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
     __syncwarp();
     if (splits > 1) {                                    // one group of rows a cluster: add up the parts of it
         cluster_sync();
-        const long long row0 = (long long)(blockIdx.x / splits) * kRows;
-        for (int i = int(rank) * kThreads + threadIdx.x; i < p.m * (kRows / 4); i += int(splits) * kThreads) {
+        const long long row0 = (long long)together * kRows;
+        for (int i = int(rank) * kThreads + threadIdx.x; together < p.tiles && i < p.m * (kRows / 4); i += int(splits) * kThreads) {
             const long long row = row0 + 4 * (i % (kRows / 4));
             if (row >= p.w.rows) continue;
             float4 part[kMostSplits];
@@ -498,10 +501,30 @@ cudaError_t launch(FewArgs p, cudaStream_t stream) {
     while (splits < kMostSplits && splits * 2 <= p.k_tiles &&
            p.tiles <= ms_most_clusters(reinterpret_cast<const void*>(three), kThreads, G::kSmem, 2, splits * 2)) splits *= 2;
     // One stage less where that makes room for all of x: eight tokens through 40960 x 4096 48.0 -> 41.4 us, 151936 x 4096 132 -> 91.5.
-    const int rows_x = (p.k_tiles + splits - 1) / splits * PARTS * p.m;
+    // More groups of rows than that: all of them whole, in turns of which the last may be a short one; or the last ones shared by clusters again, at once.
+    // The cost is counted in turns; a CTA alone on its SM takes 0.55 of one, an
+    // exchange 0.15.  (One token: 40960 x 4096 31.2 -> 27.2 us, 40960 x 12288 86.2 -> 72.3.)
+    int grid = splits > 1 ? p.tiles * splits : std::min(p.tiles, 2 * ms_sm_count());
+    p.whole = splits > 1 ? 0 : p.tiles;
+    if (splits == 1 && p.tiles > grid) {
+        const auto part = [](int ctas) { return ctas == 0 ? 0.0 : ctas <= ms_sm_count() ? 0.55 : 1.0; };
+        double least = p.tiles / grid + part(p.tiles % grid);
+        for (int share = 2; share <= 4 && share <= p.k_tiles; share *= 2) {
+            const int clusters = ms_most_clusters(reinterpret_cast<const void*>(three), kThreads, G::kSmem, 2, share), ctas = clusters * share;
+            const int left = p.tiles % ctas;
+            const double cost = p.tiles / ctas + part(left * share) / share + 0.15;
+            if (left <= clusters && cost < least) {
+                least = cost;
+                splits = share;
+                grid = ctas;
+                p.whole = p.tiles - left;
+            }
+        }
+    }
+    const int rows_x = (p.whole ? p.k_tiles : (p.k_tiles + splits - 1) / splits) * PARTS * p.m;
     const auto kernel = rows_x > G::kRowsX && rows_x <= Tile<FMT, PARTS, 2>::kRowsX ? two : three;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(splits > 1 ? p.tiles * splits : std::min(p.tiles, 2 * ms_sm_count())));
+    cfg.gridDim = dim3(unsigned(grid));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = G::kSmem;
     cfg.stream = stream;
@@ -540,7 +563,7 @@ size_t ms_linear_workspace_bytes(long long m, long long n, long long k, int dtyp
 cudaError_t launch_ms_linear(const void* x, int dtype, long long m, long long ldx, const MsMatrix& w, long long k, int fmt, void* y,
                              long long ldy, void* ws, cudaStream_t stream) {
     if (m <= kTokens) {
-        const FewArgs p{x, ldx, int(m), false, k, w, 0, 0, 0, y, ldy};
+        const FewArgs p{x, ldx, int(m), false, k, w, 0, 0, 0, 0, y, ldy};
         if (dtype == kF32) return launch_fmt<float, 3>(p, fmt, stream);
         if (dtype == kF16) return launch_fmt<__half, 1>(p, fmt, stream);
         return launch_fmt<__nv_bfloat16, 1>(p, fmt, stream);
