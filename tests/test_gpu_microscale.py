@@ -111,6 +111,29 @@ def test_quantize_row_strides_and_offsets(ms, fmt, dtype):
 
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k", ((1, 1023), (5, 257), (3, 4097), (37, 511), (9, 130), (2, 20001), (6, 8199)))
+def test_rows_at_any_address(ms, fmt, dtype, rows, k):
+    """Rows of both sides that start anywhere, and what lies around them: read as it must not count, left as it was."""
+    from trellis_b200 import _lib
+    stream, code = torch.cuda.current_stream().cuda_stream, {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype]
+    x = _matrix(rows, k, dtype, rows * 1000 + k)
+    want = _same(ms.quantize(x, fmt), x, fmt).to(dtype)
+    for pad, lo in ((0, 0), (1, 1), (3, 2), (16, 7), (11, 9)):
+        flat = torch.full((rows * (k + pad) + 32,), float("nan"), dtype=dtype, device="cuda")
+        view = flat[lo:lo + rows * (k + pad)].view(rows, k + pad)[:, :k]
+        view.copy_(x)
+        q = ms.quantize(view, fmt)
+        assert torch.equal(q.codes, ms.quantize(x, fmt).codes) and torch.equal(ms.dequantize(q, dtype).cpu(), want)
+        flat.fill_(77.0)
+        assert _lib.lib().tcq_ms_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), None if fmt == "mxfp4" else q.row_scale.data_ptr(), rows, k, FMTS.index(fmt),
+                                            view.data_ptr(), code, k + pad, stream) == 0
+        assert torch.equal(view.cpu(), want)
+        view.fill_(77.0)
+        assert (flat == 77).all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rotate,rows,k", ((16, 3, 48), (32, 5, 32), (32, 2, 4128), (64, 130, 192), (128, 7, 128), (128, 3, 12288)))
 def test_quantize_rotated(ms, fmt, dtype, rotate, rows, k):
     """Scales and codes are those of values within the transform's rounding: log2(b) + 1 fp32 operations on sums of at most sum |x|."""

@@ -18,8 +18,42 @@ namespace {
 
 constexpr int kRun = 16;         // consecutive values of a thread: one nvfp4 block, half an mxfp4 block
 
+// w[i] = the four bytes from byte 4 i + bytes on, 0 <= bytes < 16, as far as they are among the N words.
+template <int N>
+__device__ __forceinline__ void shift_words(uint32_t (&w)[N], uint32_t bytes) {
+#pragma unroll
+    for (int step = 2; step >= 1; --step)
+        if (bytes & (4 * step))
+#pragma unroll
+            for (int i = 0; i + step < N; ++i) w[i] = w[i + step];
+#pragma unroll
+    for (int i = 0; i + 1 < N; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 8 * (bytes & 3));
+}
+
+// The matrix in memory: from its first value to behind its last.
+struct Extent { const void *from, *to; };
+
+// kRun values at any address, by 16-byte pieces that start on 16 bytes: one more than they fill.  False where a piece would reach out of the matrix.
 template <typename T>
-__device__ __forceinline__ void load_run(const T* __restrict__ row, long long c0, long long k, bool wide, float (&v)[kRun]) {
+__device__ __forceinline__ bool load_pieces(const T* at, Extent x, uint4 (&out)[sizeof(T)]) {
+    constexpr int kPieces = sizeof(T);                   // of 16 bytes a run
+    const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(at)) & 15u;
+    const char* const base = reinterpret_cast<const char*>(at) - off;
+    if (base < x.from || base + 16 * (kPieces + 1) > x.to) return false;
+    uint32_t w[4 * (kPieces + 1)];
+#pragma unroll
+    for (int i = 0; i <= kPieces; ++i) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(base) + i);
+        w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
+    }
+    shift_words(w, off);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) out[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    return true;
+}
+
+template <typename T>
+__device__ __forceinline__ void load_run(const T* __restrict__ row, long long c0, long long k, bool wide, Extent x, float (&v)[kRun]) {
     if (c0 + kRun <= k) {
         if (wide) {
             constexpr int kPer = 16 / sizeof(T);
@@ -30,14 +64,17 @@ __device__ __forceinline__ void load_run(const T* __restrict__ row, long long c0
 #pragma unroll
                 for (int i = 0; i < kPer; ++i) v[q * kPer + i] = to_f32<T>(p[i]);
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kRun; ++i) v[i] = to_f32<T>(row[c0 + i]);
+            return;
         }
-    } else {
+        uint4 u[sizeof(T)];
+        if (load_pieces<T>(row + c0, x, u)) {
 #pragma unroll
-        for (int i = 0; i < kRun; ++i) v[i] = c0 + i < k ? to_f32<T>(row[c0 + i]) : 0.0f;
+            for (int i = 0; i < kRun; ++i) v[i] = to_f32<T>(reinterpret_cast<const T*>(u)[i]);
+            return;
+        }
     }
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) v[i] = c0 + i < k ? to_f32<T>(row[c0 + i]) : 0.0f;
 }
 
 __device__ __forceinline__ void load_signs(const float* __restrict__ signs, long long c0, long long k, bool wide, float (&v)[kRun]) {
@@ -199,6 +236,7 @@ __global__ void __launch_bounds__(1024) tcq_ms_quantize_kernel(const T* __restri
     if constexpr (ROTATED)
 #pragma unroll
         for (int q = 0; q < RUNS; ++q) load_signs(p.signs, ((long long)q * p.lanes + lane) * kRun, p.k, p.wide_signs, signs[q]);
+    const Extent extent{x, x + (p.rows - 1) * p.ldx + p.k};
     uint4 next[RUNS][kPieces];
     auto fetch = [&](long long r) {
         const T* const row = x + (r < p.rows ? r : p.rows - 1) * p.ldx;
@@ -208,7 +246,7 @@ __global__ void __launch_bounds__(1024) tcq_ms_quantize_kernel(const T* __restri
             if (p.wide && c0 + kRun <= p.k) {
 #pragma unroll
                 for (int i = 0; i < kPieces; ++i) next[q][i] = __ldg(reinterpret_cast<const uint4*>(row + c0) + i);
-            } else {
+            } else if (ROTATED || c0 + kRun > p.k || !load_pieces<T>(row + c0, extent, next[q])) {      // (rotated rows are nearly always aligned)
                 T* const v = reinterpret_cast<T*>(next[q]);
 #pragma unroll
                 for (int i = 0; i < kRun; ++i) v[i] = c0 + i < p.k ? row[c0 + i] : from_f32<T>(0.0f);
@@ -263,9 +301,10 @@ template <typename T, int FMT>
 __global__ void __launch_bounds__(256) tcq_ms_quantize_long_kernel(const T* __restrict__ x, const __grid_constant__ QuantizeArgs p) {
     const long long r = blockIdx.x, span = (p.k + kMsTileK - 1) / kMsTileK * kMsTileK;
     const T* const row = x + r * p.ldx;
+    const Extent extent{x, x + (p.rows - 1) * p.ldx + p.k};
     float v[kRun], signs[kRun];
     auto load = [&](long long c0) {
-        load_run(row, c0, p.k, p.wide, v);
+        load_run(row, c0, p.k, p.wide, extent, v);
         if (p.rotate) {
             load_signs(p.signs, c0, p.k, p.wide_signs, signs);
             rotate_run(v, signs, p.rotate);
@@ -297,35 +336,65 @@ __global__ void __launch_bounds__(256) tcq_ms_quantize_long_kernel(const T* __re
 
 // `lanes` threads a row, 16 columns each: 8 bytes of codes, one scale.  (A thread for several rows, one after the other, is 20 % slower.)
 // 12288 x 4096 to bf16 25.7 us (5.0 TB/s), to fp32 56.
-template <typename T, int FMT>
+template <typename T, int FMT, bool WIDE>
 __global__ void __launch_bounds__(256) tcq_ms_dequantize_kernel(const uint8_t* __restrict__ codes, long long pitch, const uint8_t* __restrict__ scales,
                                                                 long long atoms, const float* __restrict__ row_scale, long long rows,
-                                                                long long k, T* __restrict__ out, long long ldo, bool wide, int log_lanes) {
+                                                                long long k, T* __restrict__ out, long long ldo, int log_lanes) {
     const long long r = ((long long)blockIdx.x << (8 - log_lanes)) + (threadIdx.x >> log_lanes);
     const long long c0 = (((long long)blockIdx.y << log_lanes) + (threadIdx.x & ((1 << log_lanes) - 1))) * kRun;
-    if (r >= rows || c0 >= k) return;
-    const uint2 u = __ldg(reinterpret_cast<const uint2*>(codes + r * pitch + c0 / 2));
-    float s = ms_scale_to_f32<FMT>(__ldg(scales + ms_scale_at(r, int(c0 / Ms<FMT>::kBlock), atoms)));
-    if constexpr (FMT == kNvfp4) s *= __ldg(row_scale + r);
+    const bool is = r < rows && c0 < k;
+    if (WIDE && !is) return;
+    const long long rc = is ? r : 0, cc = is ? c0 : 0;
+    const uint2 u = __ldg(reinterpret_cast<const uint2*>(codes + rc * pitch + cc / 2));
+    float s = ms_scale_to_f32<FMT>(__ldg(scales + ms_scale_at(rc, int(cc / Ms<FMT>::kBlock), atoms)));
+    if constexpr (FMT == kNvfp4) s *= __ldg(row_scale + rc);
     uint32_t h[8];
     e2m1x8_to_f16(u.x, reinterpret_cast<uint32_t(&)[4]>(h[0]));
     e2m1x8_to_f16(u.y, reinterpret_cast<uint32_t(&)[4]>(h[4]));
-    T o[kRun];
+    constexpr int kPieces = sizeof(T), kWords = 4 * kPieces, kPer = 16 / sizeof(T);        // pieces of 16 bytes, words of a run; values of a piece
+    uint32_t w[4 + kWords];                              // four words of the lane before, then this lane's
+    T* const o = reinterpret_cast<T*>(w + 4);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
         o[2 * i] = from_f32<T>(f.x * s);
         o[2 * i + 1] = from_f32<T>(f.y * s);
     }
-    T* const to = out + r * ldo + c0;
-    if (wide && c0 + kRun <= k) {
+    T* const to = out + rc * ldo + cc;
+    const bool full = is && c0 + kRun <= k;
+    if constexpr (WIDE) {                                // rows of out start on 16 bytes
+        if (full) {
 #pragma unroll
-        for (int q = 0; q < int(kRun * sizeof(T) / 16); ++q) reinterpret_cast<uint4*>(to)[q] = reinterpret_cast<const uint4*>(o)[q];
-    } else {
+            for (int q = 0; q < kPieces; ++q) reinterpret_cast<uint4*>(to)[q] = make_uint4(w[4 + 4 * q], w[5 + 4 * q], w[6 + 4 * q], w[7 + 4 * q]);
+        } else if (is) {
 #pragma unroll
-        for (int i = 0; i < kRun; ++i)
-            if (c0 + i < k) to[i] = o[i];
+            for (int i = 0; i < kRun; ++i)
+                if (c0 + i < k) to[i] = o[i];
+        }
+        return;
     }
+    // Rows at any address: pieces that start on 16 bytes, the first of them with the end of the lane before (9300 x 12287 to bf16 622 -> 97 us).
+    const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(to)) & 15u;
+    const int lane = threadIdx.x & 31, lanes = min(32, 1 << log_lanes);
+    const bool before = (lane & (lanes - 1)) != 0, after = __shfl_down_sync(0xFFFFFFFFu, full, 1) && ((lane + 1) & (lanes - 1)) != 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __shfl_up_sync(0xFFFFFFFFu, w[kWords + i], 1);
+    if (!is) return;
+    const int spill = int(off / sizeof(T));              // this many values at the end are in the next lane's first piece
+#pragma unroll
+    for (int i = 0; i < kRun; ++i)
+        if (c0 + i < k && (!full || (i < kPer - spill && !before && spill) || (i >= kRun - spill && !after))) to[i] = o[i];
+    if (!full) return;
+    uint4* const pieces = reinterpret_cast<uint4*>(reinterpret_cast<char*>(to) - off);
+    if (off == 0) {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = w[4 + i];
+    } else {
+        shift_words(w, 16 - off);
+    }
+#pragma unroll
+    for (int q = 0; q < kPieces; ++q)
+        if (q > 0 || before || spill == 0) pieces[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
 }
 
 template <typename T, int FMT>
@@ -367,8 +436,9 @@ cudaError_t dequantize_t(const MsMatrix& q, long long k, int fmt, void* out, lon
     while ((1 << log_lanes) < runs && log_lanes < 8) ++log_lanes;
     const dim3 grid(unsigned((q.rows + (256 >> log_lanes) - 1) >> (8 - log_lanes)), unsigned((runs + (1 << log_lanes) - 1) >> log_lanes));
     T* const o = static_cast<T*>(out);
-    if (fmt == kNvfp4) tcq_ms_dequantize_kernel<T, kNvfp4><<<grid, 256, 0, stream>>>(q.codes, ms_pitch(k), q.scales, atoms, q.row_scale, q.rows, k, o, ldo, wide, log_lanes);
-    else tcq_ms_dequantize_kernel<T, kMxfp4><<<grid, 256, 0, stream>>>(q.codes, ms_pitch(k), q.scales, atoms, q.row_scale, q.rows, k, o, ldo, wide, log_lanes);
+    const auto kernel = fmt == kNvfp4 ? (wide ? tcq_ms_dequantize_kernel<T, kNvfp4, true> : tcq_ms_dequantize_kernel<T, kNvfp4, false>)
+                                      : (wide ? tcq_ms_dequantize_kernel<T, kMxfp4, true> : tcq_ms_dequantize_kernel<T, kMxfp4, false>);
+    kernel<<<grid, 256, 0, stream>>>(q.codes, ms_pitch(k), q.scales, atoms, q.row_scale, q.rows, k, o, ldo, log_lanes);
     return cudaGetLastError();
 }
 
