@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(256) tcq_ms_quantize_long_kernel(const T* __re
 }
 
 // `lanes` threads a row, 16 columns each: 8 bytes of codes, one scale.  (A thread for several rows, one after the other, is 20 % slower.)
-// 12288 x 4096 to bf16 25.7 us (5.0 TB/s), to fp32 41 (5.6 TB/s).
+// 12288 x 4096 to bf16 23.7 us (5.4 TB/s), to fp32 41 (5.6 TB/s).
 template <typename T, int FMT, bool WIDE>
 __global__ void __launch_bounds__(256) tcq_ms_dequantize_kernel(const uint8_t* __restrict__ codes, long long pitch, const uint8_t* __restrict__ scales,
                                                                 long long atoms, const float* __restrict__ row_scale, long long rows,
@@ -343,7 +343,6 @@ __global__ void __launch_bounds__(256) tcq_ms_dequantize_kernel(const uint8_t* _
     const long long r = ((long long)blockIdx.x << (8 - log_lanes)) + (threadIdx.x >> log_lanes);
     const long long c0 = (((long long)blockIdx.y << log_lanes) + (threadIdx.x & ((1 << log_lanes) - 1))) * kRun;
     const bool is = r < rows && c0 < k;
-    if (WIDE && sizeof(T) == 2 && !is) return;
     const long long rc = is ? r : 0, cc = is ? c0 : 0;
     const uint2 u = __ldg(reinterpret_cast<const uint2*>(codes + rc * pitch + cc / 2));
     float s = ms_scale_to_f32<FMT>(__ldg(scales + ms_scale_at(rc, int(cc / Ms<FMT>::kBlock), atoms)));
@@ -363,26 +362,23 @@ __global__ void __launch_bounds__(256) tcq_ms_dequantize_kernel(const uint8_t* _
     T* const to = out + rc * ldo + cc;
     const bool full = is && c0 + kRun <= k;
     if constexpr (WIDE) {                                // rows of out start on 16 bytes
-        bool stored = false;
-        if constexpr (sizeof(T) == 4) {
-            // Two neighbours swap two pieces each and write 32 bytes side by side, four times, instead of 16 bytes 64 apart (56 -> 41 us).
-            const bool odd = threadIdx.x & 1;
-            stored = __shfl_xor_sync(0xFFFFFFFFu, full, 1) && full && log_lanes > 0;
+        // Two neighbours swap half of their pieces and write 32 bytes side by side instead of 16 bytes 32 or 64 apart (12288 x 4096 to bf16 26.7 -> 23.7 us,
+        // to fp32 56 -> 41).
+        const bool odd = threadIdx.x & 1, stored = __shfl_xor_sync(0xFFFFFFFFu, full, 1) && full && log_lanes > 0;
 #pragma unroll
-            for (int q = 0; q < 4; q += 2)               // the even lane gives pieces 1 and 3, the odd one 0 and 2
+        for (int q = 0; q < kPieces; q += 2)             // the even lane gives its odd pieces, the odd one its even ones
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t got = __shfl_xor_sync(0xFFFFFFFFu, odd ? w[4 + 4 * q + i] : w[8 + 4 * q + i], 1);
-                    if (stored && odd) w[4 + 4 * q + i] = got;
-                    if (stored && !odd) w[8 + 4 * q + i] = got;
-                }
-            if (stored) {                                // E0 O0 E2 O2 in the even lane, E1 O1 E3 O3 in the odd one
-                uint4* const both = reinterpret_cast<uint4*>(to - (odd ? kRun : 0)) + odd;
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t got = __shfl_xor_sync(0xFFFFFFFFu, odd ? w[4 + 4 * q + i] : w[8 + 4 * q + i], 1);
+                if (stored && odd) w[4 + 4 * q + i] = got;
+                if (stored && !odd) w[8 + 4 * q + i] = got;
+            }
+        if (stored) {                                    // E0 O0 (E2 O2) in the even lane, E1 O1 (E3 O3) in the odd one
+            uint4* const both = reinterpret_cast<uint4*>(to - (odd ? kRun : 0)) + odd;
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int mine = q < 2 ? 2 * q : 2 * q - 3;
-                    both[2 * q] = make_uint4(w[4 + 4 * mine], w[5 + 4 * mine], w[6 + 4 * mine], w[7 + 4 * mine]);
-                }
+            for (int q = 0; q < kPieces; ++q) {
+                const int mine = kPieces == 2 ? q : q < 2 ? 2 * q : 2 * q - 3;
+                both[2 * q] = make_uint4(w[4 + 4 * mine], w[5 + 4 * mine], w[6 + 4 * mine], w[7 + 4 * mine]);
             }
         }
         if (full && !stored) {
