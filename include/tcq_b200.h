@@ -293,7 +293,8 @@ TCQ_API int tcq_codebook_lut(int codebook, float *lut, void *stream);
  *              row r at [r/128][b/4][r%32][r%128/32][b%4], atoms = 2 (mxfp4) or 4 (nvfp4) for every 256 columns begun;
  *              zeros behind column k.  Places of rows behind the last one may hold anything.
  *   row_scale  [rows] fp32 (nvfp4), NULL (mxfp4)
- * Fewer than 2^31 rows, at most 2^24 columns.  Waits inside the products are bounded; results whose wait ran out are NaN.
+ * Fewer than 2^31 rows, at most 2^24 columns.  Waits inside the products are bounded; where one runs out, the results of that CTA from there on,
+ * and those it shares with others, are NaN.
  */
 #define TCQ_MS_MXFP4 0
 #define TCQ_MS_NVFP4 1
@@ -341,6 +342,18 @@ TCQ_API int tcq_ms_linear(const void *x, int dtype, int64_t m, int64_t ldx, cons
 TCQ_API int tcq_ms_matmul(const uint8_t *x_codes, const uint8_t *x_scales, const float *x_row_scale, int64_t m,
                           const uint8_t *codes, const uint8_t *scales, const float *row_scale, int64_t n, int64_t k,
                           int format, void *y, int dtype, int64_t ldy, void *stream);
+
+/*
+ * Self-tests of the products' bounded waits: the same calls, in which every CTA stops loading after `loads` pieces of 256 columns (0 <= loads < 2^32 - 1).  What
+ * waits for more runs out after its time limit (about a quarter of a second), the kernel ends normally, and every result that needed more is NaN.
+ * Nothing faults, traps or spins without limit.
+ */
+TCQ_API int tcq_selftest_ms_linear_waits(int64_t loads, const void *x, int dtype, int64_t m, int64_t ldx, const uint8_t *codes,
+                                         const uint8_t *scales, const float *row_scale, int64_t n, int64_t k, int format, void *y,
+                                         int64_t ldy, void *ws, size_t ws_bytes, void *stream);
+TCQ_API int tcq_selftest_ms_matmul_waits(int64_t loads, const uint8_t *x_codes, const uint8_t *x_scales, const float *x_row_scale,
+                                         int64_t m, const uint8_t *codes, const uint8_t *scales, const float *row_scale, int64_t n,
+                                         int64_t k, int format, void *y, int dtype, int64_t ldy, void *stream);
 
 #ifdef __cplusplus
 }

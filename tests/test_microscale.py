@@ -118,3 +118,15 @@ def test_argument_validation_needs_no_gpu():
     assert M(p, p, p, 1, p, p, None, 4, 16, 1, p, 2, 4, None) == -4
     assert M(p, p, p, 1, p, p + 4, p, 4, 16, 1, p, 2, 4, None) == -5
     assert M(p, p, p, -1, p, p, p, 4, 16, 1, p, 2, 4, None) == -3
+
+
+def test_selftests_of_waits_check_their_arguments():
+    L = _lib.lib()
+    buf = (ctypes.c_char * 1024)()
+    p = ctypes.addressof(buf)
+    p += (-p) % 256
+    linear, matmul = (p, 2, 1, 16, p, p, p, 4, 16, 1, p, 4, p, 512, None), (p, p, p, 1, p, p, p, 4, 16, 1, p, 2, 4, None)
+    for loads in (-1, 2 ** 32 - 1, 2 ** 40):
+        assert L.tcq_selftest_ms_linear_waits(loads, *linear) == -3 and L.tcq_selftest_ms_matmul_waits(loads, *matmul) == -3
+    assert L.tcq_selftest_ms_linear_waits(0, None, *linear[1:]) == -4 and L.tcq_selftest_ms_matmul_waits(0, None, *matmul[1:]) == -4
+    assert L.tcq_selftest_ms_linear_waits(0, p, 2, 0, *linear[3:]) == 0

@@ -535,7 +535,7 @@ namespace tcq { int report_cuda_error(cudaError_t err, const char* where) { retu
 
 extern "C" {
 
-int tcq_abi_version(void) { return 5; }
+int tcq_abi_version(void) { return 6; }
 
 const char* tcq_strerror(int code) {
     switch (code) {

@@ -48,5 +48,22 @@ __device__ __forceinline__ bool mbar_wait(uint32_t mbar, uint32_t parity, volati
 __device__ __forceinline__ void mbar_arrive(uint32_t mbar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(mbar) : "memory");
 }
+// The end of a warp that fills a ring of STAGES: the last load of each of the `loaded` stages has landed, or does not come.  Nothing may be on its way to a
+// CTA's memory when the CTA ends, and a load that is late is seen to be missing (by whom it was for) only after this warp has issued its last one.
+// s, phase: the stage that would be next, and the parity of the wait for it to be empty.
+template <int STAGES>
+__device__ __forceinline__ void wait_for_loads(const uint64_t* full, uint32_t s, uint32_t phase, uint32_t loaded) {
+    for (uint32_t i = 0; i < loaded; ++i) {
+        if (s == 0) phase ^= 1;
+        s = s == 0 ? STAGES - 1 : s - 1;
+        for (long long t0 = clock64(); !mbar_try_wait(smem_u32(&full[s]), phase ^ 1) && clock64() - t0 < kMbarWaitCycles;) {}
+    }
+}
+// A failure is for good: behind a phase that never completes, a wait for the phase after the next is answered by the parity of the last complete one, at once
+// and wrongly.  So a warp whose wait ran out waits no more, and gives NaN from there on; who fills a ring stops, as an announcement for a stage that is not
+// complete would be counted into its open phase.
+__device__ __forceinline__ bool still_waits(bool ok, uint32_t mbar, uint32_t parity, volatile unsigned int* gave_up) {      // a whole warp, the same for all lanes
+    return ok && __all_sync(0xFFFFFFFFu, mbar_wait(mbar, parity, gave_up));
+}
 
 }  // namespace tcq

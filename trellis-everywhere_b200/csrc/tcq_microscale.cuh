@@ -98,10 +98,11 @@ int report_cuda_error(cudaError_t err, const char* where);     // tcq_capi.cu
 cudaError_t launch_ms_quantize(const void* x, int dtype, long long rows, long long k, long long ldx, int fmt, int rotate, const float* signs,
                                uint8_t* codes, uint8_t* scales, float* row_scale, cudaStream_t stream);
 cudaError_t launch_ms_dequantize(const MsMatrix& q, long long k, int fmt, void* out, int dtype, long long ldo, cudaStream_t stream);
+constexpr unsigned kMsAllLoads = 0xFFFFFFFFu;     // `loads` of the products: how many stages a CTA loads before it stops (a self-test's limit)
 cudaError_t launch_ms_linear(const void* x, int dtype, long long m, long long ldx, const MsMatrix& w, long long k, int fmt, void* y,
-                             long long ldy, void* ws, cudaStream_t stream);
+                             long long ldy, void* ws, unsigned loads, cudaStream_t stream);
 bool ms_linear_direct(const void* x, int dtype, long long m, long long ldx, int fmt);      // needs no scratch
 size_t ms_linear_workspace_bytes(long long m, long long n, long long k, int dtype, int fmt);
-cudaError_t launch_ms_matmul(const MsMatrix& x, const MsMatrix& w, long long k, int fmt, void* y, int dtype, long long ldy, cudaStream_t stream);
+cudaError_t launch_ms_matmul(const MsMatrix& x, const MsMatrix& w, long long k, int fmt, void* y, int dtype, long long ldy, unsigned loads, cudaStream_t stream);
 
 }  // namespace tcq

@@ -24,6 +24,39 @@ int check_ms_matrix(const void* codes, const void* scales, const void* row_scale
 }
 size_t type_bytes(int dtype) { return dtype == TCQ_F32 ? 4 : 2; }
 
+int linear_core(const void* x, int dtype, int64_t m, int64_t ldx, const uint8_t* codes, const uint8_t* scales, const float* row_scale, int64_t n, int64_t k,
+                int format, void* y, int64_t ldy, void* ws, size_t ws_bytes, unsigned loads, void* stream) {
+    int rc = check_ms(n, k, format, dtype);
+    if (rc == TCQ_OK) rc = check_ms(m, k, format, dtype);
+    if (rc != TCQ_OK) return rc;
+    if (n == 0 || m == 0) return TCQ_OK;
+    if (k == 0 || ldx < k || ldy < n) return TCQ_E_BAD_ARGUMENT;
+    const bool direct = ms_linear_direct(x, dtype, m, ldx, format);
+    if (x == nullptr || y == nullptr || (ws == nullptr && !direct)) return TCQ_E_NULL_POINTER;
+    if ((rc = check_ms_matrix(codes, scales, row_scale, format)) != TCQ_OK) return rc;
+    if (misaligned(x, type_bytes(dtype)) || misaligned(y, type_bytes(dtype)) || misaligned(ws, 256)) return TCQ_E_MISALIGNED;
+    if (!direct && ws_bytes < ms_linear_workspace_bytes(m, n, k, dtype, format)) return TCQ_E_WORKSPACE;
+    cudaError_t err = launch_ms_linear(x, dtype, m, ldx, {codes, scales, row_scale, n}, k, format, y, ldy, ws, loads, static_cast<cudaStream_t>(stream));
+    return err == cudaSuccess ? TCQ_OK : report_cuda_error(err, "ms_linear");
+}
+
+int matmul_core(const uint8_t* x_codes, const uint8_t* x_scales, const float* x_row_scale, int64_t m, const uint8_t* codes, const uint8_t* scales,
+                const float* row_scale, int64_t n, int64_t k, int format, void* y, int dtype, int64_t ldy, unsigned loads, void* stream) {
+    int rc = check_ms(n, k, format, dtype);
+    if (rc == TCQ_OK) rc = check_ms(m, k, format, dtype);
+    if (rc != TCQ_OK) return rc;
+    if (n == 0 || m == 0) return TCQ_OK;
+    if (k == 0 || ldy < n) return TCQ_E_BAD_ARGUMENT;
+    if (y == nullptr) return TCQ_E_NULL_POINTER;
+    if ((rc = check_ms_matrix(x_codes, x_scales, x_row_scale, format)) != TCQ_OK) return rc;
+    if ((rc = check_ms_matrix(codes, scales, row_scale, format)) != TCQ_OK) return rc;
+    if (misaligned(y, type_bytes(dtype))) return TCQ_E_MISALIGNED;
+    cudaError_t err = launch_ms_matmul({x_codes, x_scales, x_row_scale, m}, {codes, scales, row_scale, n}, k, format, y, dtype, ldy, loads,
+                                       static_cast<cudaStream_t>(stream));
+    return err == cudaSuccess ? TCQ_OK : report_cuda_error(err, "ms_matmul");
+}
+bool bad_loads(int64_t loads) { return loads < 0 || loads >= int64_t(kMsAllLoads); }
+
 }  // namespace
 
 extern "C" {
@@ -70,35 +103,27 @@ size_t tcq_ms_linear_workspace_bytes(int64_t m, int64_t n, int64_t k, int dtype,
 int tcq_ms_linear(const void* x, int dtype, int64_t m, int64_t ldx, const uint8_t* codes, const uint8_t* scales,
                   const float* row_scale, int64_t n, int64_t k, int format, void* y, int64_t ldy, void* ws, size_t ws_bytes,
                   void* stream) {
-    int rc = check_ms(n, k, format, dtype);
-    if (rc == TCQ_OK) rc = check_ms(m, k, format, dtype);
-    if (rc != TCQ_OK) return rc;
-    if (n == 0 || m == 0) return TCQ_OK;
-    if (k == 0 || ldx < k || ldy < n) return TCQ_E_BAD_ARGUMENT;
-    const bool direct = ms_linear_direct(x, dtype, m, ldx, format);
-    if (x == nullptr || y == nullptr || (ws == nullptr && !direct)) return TCQ_E_NULL_POINTER;
-    if ((rc = check_ms_matrix(codes, scales, row_scale, format)) != TCQ_OK) return rc;
-    if (misaligned(x, type_bytes(dtype)) || misaligned(y, type_bytes(dtype)) || misaligned(ws, 256)) return TCQ_E_MISALIGNED;
-    if (!direct && ws_bytes < ms_linear_workspace_bytes(m, n, k, dtype, format)) return TCQ_E_WORKSPACE;
-    cudaError_t err = launch_ms_linear(x, dtype, m, ldx, {codes, scales, row_scale, n}, k, format, y, ldy, ws, static_cast<cudaStream_t>(stream));
-    return err == cudaSuccess ? TCQ_OK : report_cuda_error(err, "ms_linear");
+    return linear_core(x, dtype, m, ldx, codes, scales, row_scale, n, k, format, y, ldy, ws, ws_bytes, kMsAllLoads, stream);
 }
 
 int tcq_ms_matmul(const uint8_t* x_codes, const uint8_t* x_scales, const float* x_row_scale, int64_t m, const uint8_t* codes,
                   const uint8_t* scales, const float* row_scale, int64_t n, int64_t k, int format, void* y, int dtype,
                   int64_t ldy, void* stream) {
-    int rc = check_ms(n, k, format, dtype);
-    if (rc == TCQ_OK) rc = check_ms(m, k, format, dtype);
-    if (rc != TCQ_OK) return rc;
-    if (n == 0 || m == 0) return TCQ_OK;
-    if (k == 0 || ldy < n) return TCQ_E_BAD_ARGUMENT;
-    if (y == nullptr) return TCQ_E_NULL_POINTER;
-    if ((rc = check_ms_matrix(x_codes, x_scales, x_row_scale, format)) != TCQ_OK) return rc;
-    if ((rc = check_ms_matrix(codes, scales, row_scale, format)) != TCQ_OK) return rc;
-    if (misaligned(y, type_bytes(dtype))) return TCQ_E_MISALIGNED;
-    cudaError_t err = launch_ms_matmul({x_codes, x_scales, x_row_scale, m}, {codes, scales, row_scale, n}, k, format, y, dtype, ldy,
-                                       static_cast<cudaStream_t>(stream));
-    return err == cudaSuccess ? TCQ_OK : report_cuda_error(err, "ms_matmul");
+    return matmul_core(x_codes, x_scales, x_row_scale, m, codes, scales, row_scale, n, k, format, y, dtype, ldy, kMsAllLoads, stream);
+}
+
+int tcq_selftest_ms_linear_waits(int64_t loads, const void* x, int dtype, int64_t m, int64_t ldx, const uint8_t* codes, const uint8_t* scales,
+                                 const float* row_scale, int64_t n, int64_t k, int format, void* y, int64_t ldy, void* ws, size_t ws_bytes,
+                                 void* stream) {
+    return bad_loads(loads) ? TCQ_E_BAD_COUNT
+                            : linear_core(x, dtype, m, ldx, codes, scales, row_scale, n, k, format, y, ldy, ws, ws_bytes, unsigned(loads), stream);
+}
+
+int tcq_selftest_ms_matmul_waits(int64_t loads, const uint8_t* x_codes, const uint8_t* x_scales, const float* x_row_scale, int64_t m,
+                                 const uint8_t* codes, const uint8_t* scales, const float* row_scale, int64_t n, int64_t k, int format,
+                                 void* y, int dtype, int64_t ldy, void* stream) {
+    return bad_loads(loads) ? TCQ_E_BAD_COUNT
+                            : matmul_core(x_codes, x_scales, x_row_scale, m, codes, scales, row_scale, n, k, format, y, dtype, ldy, unsigned(loads), stream);
 }
 
 }  // extern "C"

@@ -14,7 +14,7 @@
 //
 // Bound by instruction issue and its latencies (54 % of the slots): one token through 40960 x 4096 27.2 us (3.5 TB/s), mxfp4 23.3; eight 34.4 and 31.0.
 //
-// A wait that runs out (kMbarWaitCycles) makes its CTA's results NaN.
+// A wait that runs out (kMbarWaitCycles) makes its CTA's results from there on NaN, and those of its cluster.
 #include <algorithm>
 #include <type_traits>
 
@@ -54,6 +54,7 @@ struct FewArgs {
     int tiles, whole, k_tiles;                   // groups of 128 rows of W; how many of them a CTA does by itself
     void* y;
     long long ldy;
+    unsigned loads;                              // stages that a CTA loads, at most (a self-test's limit)
 };
 
 __device__ __forceinline__ void ldmatrix4(uint32_t smem, uint32_t (&v)[4]) {
@@ -190,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
         bulk_load(to + G::kBytesW, p.w.scales + (t * p.atoms + (long long)kt * G::kAtoms) * 512, G::kBytesS, bar);
     };
     // The first stages are on their way before anything else: a small call is little more than its latencies.
-    const int ahead = min(STAGES, p.whole ? p.k_tiles : until - share);
+    const int ahead = min(min(unsigned(STAGES), unsigned(p.whole ? p.k_tiles : until - share)), p.loads);
     if (warp == 8) {
         if (elect_one()) {
             gave_up = 0;
@@ -206,22 +207,18 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
         // ---- loads; the warp stays together, one lane issues
         const bool one = elect_one();
         uint32_t s = ahead == STAGES ? 0 : ahead, phase = ahead == STAGES ? 0 : 1, loaded = ahead;    // (the first wait for a stage is for the phase before the first)
+        unsigned left = p.loads - ahead;
         bool ok = true;
         for (int t = blockIdx.x, skip = ahead; t < ends && ok; t += gridDim.x, skip = 0)
             for (int kt = (t < p.whole ? 0 : share) + skip; kt < (t < p.whole ? p.k_tiles : until); ++kt) {
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&empty[s]), phase, &gave_up));
+                ok = still_waits(left-- > 0, smem_u32(&empty[s]), phase, &gave_up) && !__any_sync(0xFFFFFFFFu, gave_up);      // (who gave up arrives all the same)
                 if (!ok) break;
                 if (one) load(s, t < p.whole ? t : together, kt);
                 __syncwarp();
                 if (++s == STAGES) { s = 0; phase ^= 1; }
                 if (loaded < STAGES) ++loaded;
             }
-        if (gave_up)                                     // nothing may be on its way to this CTA's memory when it ends: the last loads of each stage
-            for (uint32_t i = 0; i < loaded; ++i) {
-                if (s == 0) phase ^= 1;
-                s = s == 0 ? STAGES - 1 : s - 1;
-                for (long long t0 = clock64(); !mbar_try_wait(smem_u32(&full[s]), phase ^ 1) && clock64() - t0 < kMbarWaitCycles;) {}
-            }
+        wait_for_loads<STAGES>(full, s, phase, loaded);
     } else {
         const int g = lane >> 2, t4 = lane & 3;
         const uint32_t odd = G::kSwapped ? 64 * (g & 1) : 0;
@@ -298,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
             }
             for (int kt = first; kt < last; ++kt) {
                 if (!held && kt + 1 < last) fetch(kt + 1, warp);
-                const bool ok = mbar_wait(smem_u32(&full[s]), phase, &gave_up);
+                mbar_wait(smem_u32(&full[s]), phase, &gave_up);
                 __syncwarp();
                 const uint32_t stage = smem + s * G::kStage;
                 for (;;) {
@@ -380,7 +377,6 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
                     any_of_consumers(false);             // all have read this buffer: the next parts
                     more = convert(buf);
                 }
-                if (!ok) acc[0] = acc[1] = acc[2] = acc[3] = __uint_as_float(0x7FC00000u);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&empty[s]));
                 if (++s == STAGES) { s = 0; phase ^= 1; }
@@ -391,6 +387,8 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
                     more = convert(buf);
                 }
             }
+            // A wait that ran out is for good, here as well: waits for later phases of that stage may have been answered by the parity of an earlier one.
+            if (*static_cast<volatile unsigned int*>(&gave_up)) acc[0] = acc[1] = acc[2] = acc[3] = __uint_as_float(0x7FC00000u);
 #pragma unroll
             for (int i = 0; i < 4; ++i)                  // (an infinite or NaN sum leaves NaN behind)
                 sums[(2 * t4 + (i & 1)) * kRows + 16 * warp + g + 8 * (i >> 1)] = fabsf(low[i]) < __uint_as_float(0x7F800000u) ? acc[i] + low[i] : acc[i];
@@ -561,9 +559,9 @@ size_t ms_linear_workspace_bytes(long long m, long long n, long long k, int dtyp
 }
 
 cudaError_t launch_ms_linear(const void* x, int dtype, long long m, long long ldx, const MsMatrix& w, long long k, int fmt, void* y,
-                             long long ldy, void* ws, cudaStream_t stream) {
+                             long long ldy, void* ws, unsigned loads, cudaStream_t stream) {
     if (m <= kTokens) {
-        const FewArgs p{x, ldx, int(m), false, k, w, 0, 0, 0, 0, y, ldy};
+        const FewArgs p{x, ldx, int(m), false, k, w, 0, 0, 0, 0, y, ldy, loads};
         if (dtype == kF32) return launch_fmt<float, 3>(p, fmt, stream);
         if (dtype == kF16) return launch_fmt<__half, 1>(p, fmt, stream);
         return launch_fmt<__nv_bfloat16, 1>(p, fmt, stream);
@@ -571,7 +569,7 @@ cudaError_t launch_ms_linear(const void* x, int dtype, long long m, long long ld
     const long long width = ms_tiles_k(k) * kMsTileK;
     const unsigned grid = unsigned((m * (width / 8) + 255) / 256);
     uint8_t* const scratch = static_cast<uint8_t*>(ws);
-    ManyCall c{x, ldx, k, m, 1, dtype, w, k, fmt, y, ldy, false, nullptr, nullptr};
+    ManyCall c{x, ldx, k, m, 1, dtype, w, k, fmt, y, ldy, false, nullptr, nullptr, loads};
     cudaError_t err;
     // fp16 through mxfp4: up to 128 tokens, and while tiles of 64 leave half of the SMs free, two bf16 parts (200 through 1024 x 4096 15.4 us), else fp16
     // weights (23.4; but through 4096 x 12288 52.5 instead of 69.5, 12288 x 4096 39 instead of 53).

@@ -13,7 +13,7 @@
 //
 // Bound by the making of weights, beside the tensor cores (57 % busy): 1000 tokens through 12288 x 4096 82 us (1.22 PFLOP/s), mxfp4 83; fp16 76 and 88.
 //
-// A wait that runs out (kMbarWaitCycles) makes its CTA stop, and its results NaN.
+// A wait that runs out (kMbarWaitCycles) makes its CTA stop, and its results from there on NaN, as those of its cluster.
 #include <algorithm>
 #include <type_traits>
 
@@ -60,6 +60,7 @@ struct ManyArgs {
     const unsigned int* wide;                    // run only if *wide is `run_if`
     unsigned int run_if;
     const uint8_t* largest;                      // fp16, mxfp4
+    unsigned loads;                              // stages of W that a CTA loads, at most (a self-test's limit)
 };
 
 __device__ __forceinline__ void mma_from_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
@@ -152,12 +153,13 @@ __global__ void __launch_bounds__(kThreads<P>, Tile<FMT, NT, P>::kCtas) tcq_ms_l
         // ---- loads; the warp stays together, one lane issues
         const bool one = elect_one();
         uint32_t sw = 0, pw = 1, sx = 0, px = 1, loaded_w = 0, loaded_x = 0;      // (the first waits are for the phase before the first)
+        unsigned left = p.loads;
         bool ok = true;
         for (int t = blockIdx.x / splits; t < tiles && ok; t += clusters) {
             const int tn = t / p.tiles_m, tm = t % p.tiles_m;
             for (int step = first; step < last; ++step) {
                 if (step % 4 == 0) {
-                    ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&w_empty[sw]), pw, &gave_up));
+                    ok = still_waits(left-- > 0, smem_u32(&w_empty[sw]), pw, &gave_up) && !__any_sync(0xFFFFFFFFu, gave_up);
                     if (!ok) break;
                     if (one) {
                         const uint32_t to = smem_w + sw * T::kStageW, bar = smem_u32(&w_full[sw]);
@@ -169,7 +171,7 @@ __global__ void __launch_bounds__(kThreads<P>, Tile<FMT, NT, P>::kCtas) tcq_ms_l
                     if (++sw == T::kStagesW) { sw = 0; pw ^= 1; }
                     if (loaded_w < T::kStagesW) ++loaded_w;
                 }
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&x_empty[sx]), px, &gave_up));
+                ok = still_waits(ok, smem_u32(&x_empty[sx]), px, &gave_up);
                 if (!ok) break;
                 if (one) {
                     mbar_expect(smem_u32(&x_full[sx]), T::kBytesX);
@@ -180,18 +182,10 @@ __global__ void __launch_bounds__(kThreads<P>, Tile<FMT, NT, P>::kCtas) tcq_ms_l
                 if (loaded_x < T::kStagesX) ++loaded_x;
             }
         }
-        if (gave_up) {                                   // nothing may be on its way to this CTA's memory when it ends: the last loads of each stage
-            for (uint32_t i = 0; i < loaded_w; ++i) {
-                if (sw == 0) pw ^= 1;
-                sw = sw == 0 ? T::kStagesW - 1 : sw - 1;
-                for (long long t0 = clock64(); !mbar_try_wait(smem_u32(&w_full[sw]), pw ^ 1) && clock64() - t0 < kMbarWaitCycles;) {}
-            }
-            for (uint32_t i = 0; i < loaded_x; ++i) {
-                if (sx == 0) px ^= 1;
-                sx = sx == 0 ? T::kStagesX - 1 : sx - 1;
-                for (long long t0 = clock64(); !mbar_try_wait(smem_u32(&x_full[sx]), px ^ 1) && clock64() - t0 < kMbarWaitCycles;) {}
-            }
-        }
+        wait_for_loads<T::kStagesW>(w_full, sw, pw, loaded_w);
+        wait_for_loads<T::kStagesX>(x_full, sx, px, loaded_x);
+        if (splits > 1 && gave_up)                       // a load that was late may lie over the NaN of this CTA's part
+            for (int i = lane; i < kTokens * P * kRows; i += 32) reinterpret_cast<uint32_t*>(raw + (smem_x - smem_u32(raw)))[i] = 0x7FC00000u;
     } else if (warp == 1) {
         // ---- products; likewise
         constexpr uint32_t kIdesc = 1u << 4 | (FP16 ? 0u : 1u << 7 | 1u << 10) | uint32_t(NT >> 3) << 17 | uint32_t(kRows >> 4) << 24;      // bf16 x bf16 (or fp16 x fp16), fp32 sums
@@ -306,6 +300,7 @@ __global__ void __launch_bounds__(kThreads<P>, Tile<FMT, NT, P>::kCtas) tcq_ms_l
         const int quarter = warp & 3;
         constexpr int kChunk = NT < 32 ? NT : 32, kUsed = kChunk / P * P;            // columns loaded, and columns of whole tokens
         int n = 0;
+        bool ok = true;
         for (int t = blockIdx.x / splits; t < tiles; t += clusters) {
             const long long r = (long long)(t / p.tiles_m) * kRows + 32 * quarter + lane, token0 = (long long)(t % p.tiles_m) * kTokens;
             const float fw = row_factor<FMT, FP16>(p, r);
@@ -333,7 +328,7 @@ __global__ void __launch_bounds__(kThreads<P>, Tile<FMT, NT, P>::kCtas) tcq_ms_l
                 float acc[NT] = {};
                 for (int step = first; step < last; step += kStepsHeld<P>, ++n) {
                     const int buf = n % T::kSumBuffers;
-                    const bool ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sum_full[buf]), uint32_t(n / T::kSumBuffers) & 1, &gave_up));
+                    ok = still_waits(ok, smem_u32(&sum_full[buf]), uint32_t(n / T::kSumBuffers) & 1, &gave_up);
                     tc_fence_after();
 #pragma unroll
                     for (int c0 = 0; c0 < NT; c0 += kChunk) {
@@ -350,7 +345,7 @@ __global__ void __launch_bounds__(kThreads<P>, Tile<FMT, NT, P>::kCtas) tcq_ms_l
                 finish(acc, 0, std::integral_constant<int, NT / P * P>{});
             } else {
                 const int buf = n % T::kSumBuffers;
-                const bool ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sum_full[buf]), uint32_t(n / T::kSumBuffers) & 1, &gave_up));
+                ok = still_waits(ok, smem_u32(&sum_full[buf]), uint32_t(n / T::kSumBuffers) & 1, &gave_up);
                 ++n;
                 tc_fence_after();
 #pragma unroll 1
@@ -431,7 +426,7 @@ cudaError_t launch(const ManyCall& c, cudaStream_t stream) {
     if ((err = make_byte_map(&map_w, c.w.codes, pitch, c.w.rows, pitch, kRows)) != cudaSuccess) return err;
     if ((err = make_16bit_map(&map_x, c.x, c.width, c.m * P, c.ldx, NT)) != cudaSuccess) return err;
     const ManyArgs p{c.w, c.m, int((c.w.rows + kRows - 1) / kRows), int((c.m + tokens - 1) / tokens), int((c.k + kStepK - 1) / kStepK), ms_tiles_k(c.k) * T::kAtoms, c.y, c.ldy,
-                     c.wide, FP16 ? 0u : 1u, c.largest};
+                     c.wide, FP16 ? 0u : 1u, c.largest, c.loads};
     const long long tiles = (long long)p.tiles_n * p.tiles_m;
     // How many CTAs share the columns of a tile: as many as leave every CTA an SM of its own (half an SM, where each still has 1024 columns:
     // 4096 columns of 4096 rows by 8 instead of 4 costs 10.7 -> 11.7 us, 12288 of them 21.3 -> 20.2 us).

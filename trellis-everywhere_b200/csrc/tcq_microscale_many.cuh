@@ -19,6 +19,7 @@ struct ManyCall {
     bool fp16;                   // x and weights as fp16 numbers; mxfp4's weights times 2^13 over the row's largest scale
     unsigned int* wide;          // mxfp4: whether some row's scales are too far apart for that, which decides on the GPU which form runs; or NULL
     uint8_t* largest;            // mxfp4, fp16: the byte of the largest scale of every row
+    unsigned loads;              // stages of W that a CTA loads, at most
 };
 
 cudaError_t launch_ms_linear_many(const ManyCall& c, cudaStream_t stream);

@@ -10,7 +10,7 @@
 // through distributed shared memory, in rank order.  Bound by the latency of one pass (few rows: one token,
 // 4096 x 4096 5.7 us) or by what W's bytes take (many: 40960 x 4096 16.4 us, 5.8 TB/s; mxfp4 14.5, 6.5 TB/s).
 //
-// A wait that runs out (kMbarWaitCycles) makes its CTA stop, and its results NaN.
+// A wait that runs out (kMbarWaitCycles) makes its CTA stop, and its results from there on NaN, as those of its cluster.
 #include <algorithm>
 
 #include "tcq_microscale.cuh"
@@ -42,7 +42,8 @@ struct Tile {
 }  // namespace
 
 // tcq_microscale_pair.cu: tiles of 256 tokens x nt rows of W on pairs of SMs.
-cudaError_t launch_ms_matmul_pair(const MsMatrix& x, const MsMatrix& w, long long k, int fmt, void* y, int dtype, long long ldy, int nt, int sms, cudaStream_t stream);
+cudaError_t launch_ms_matmul_pair(const MsMatrix& x, const MsMatrix& w, long long k, int fmt, void* y, int dtype, long long ldy, int nt, int sms, unsigned loads,
+                                  cudaStream_t stream);
 
 namespace {
 
@@ -57,6 +58,7 @@ struct MatmulArgs {
     long long ldy;
     int dtype;
     bool aligned;                                // y and ldy multiples of four elements
+    unsigned loads;                              // stages that a CTA loads, at most (a self-test's limit)
 };
 
 __device__ __forceinline__ void store(const MatmulArgs& p, long long at, float v) {
@@ -126,7 +128,7 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_matmul_kernel(const __grid
         bulk_load(to + T::kBytesW + T::kBytesX + T::kBytesSw, p.x_scales + (tm * atoms + (long long)kt * T::kAtoms) * 512, T::kBytesSx, bar);
     };
     // The first tile's first stages are on their way before anything else: with few tokens a call is little more than its latencies.
-    const int ahead = min(T::kStages, last - first);
+    const int ahead = min(min(unsigned(T::kStages), unsigned(last - first)), p.loads);
     if (warp == 0) {
         if (elect_one()) {
             gave_up = 0;
@@ -148,24 +150,21 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_matmul_kernel(const __grid
         // ---- loads; the warp stays together, one lane issues
         const bool one = elect_one();
         uint32_t s = ahead % T::kStages, phase = ahead == T::kStages ? 0 : 1, loaded = ahead;    // (the first wait for a stage is for the phase before the first)
+        unsigned left = p.loads - ahead;
         bool ok = true;
         int kt = first + ahead;
         for (int t = blockIdx.x / splits; t < tiles && ok; t += clusters, kt = first)
             for (; kt < last; ++kt) {
-                ok = mbar_wait(smem_u32(&empty[s]), phase, &gave_up);
-                ok = __all_sync(0xFFFFFFFFu, ok);        // every lane has seen this phase before the next can begin
+                ok = still_waits(left-- > 0, smem_u32(&empty[s]), phase, &gave_up);      // every lane has seen this phase before the next can begin
                 if (!ok) break;
                 if (one) load(s, t, kt);
                 __syncwarp();
                 if (++s == T::kStages) { s = 0; phase ^= 1; }
                 if (loaded < T::kStages) ++loaded;
             }
-        if (gave_up)                                     // nothing may be on its way to this CTA's memory when it ends: the last loads of each stage
-            for (uint32_t i = 0; i < loaded; ++i) {
-                if (s == 0) phase ^= 1;
-                s = s == 0 ? T::kStages - 1 : s - 1;
-                for (long long t0 = clock64(); !mbar_try_wait(smem_u32(&full[s]), phase ^ 1) && clock64() - t0 < kMbarWaitCycles;) {}
-            }
+        wait_for_loads<T::kStages>(full, s, phase, loaded);
+        if (splits > 1 && gave_up)                       // a load that was late may lie over the NaN of this CTA's part
+            for (int i = lane; i < NT * kRowsW; i += 32) reinterpret_cast<uint32_t*>(raw + (smem - smem_u32(raw)))[i] = 0x7FC00000u;
     } else if (warp == 1) {
         // ---- products; likewise
         constexpr uint32_t kIdesc = 1u << 7 | 1u << 10 | uint32_t(NT >> 3) << 17 | (FMT == kMxfp4 ? 1u : 0u) << 23 | 1u << 27;
@@ -217,11 +216,12 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_matmul_kernel(const __grid
         const int quarter = warp & 3;
         constexpr int kChunk = NT < 32 ? NT : 32;
         int n = 0;
+        bool ok = true;
         for (int t = blockIdx.x / splits; t < tiles; t += clusters, ++n) {
             const int buf = n & 1;
             const long long r = (long long)(t / p.tiles_m) * kRowsW + 32 * quarter + lane, i0 = (long long)(t % p.tiles_m) * NT;
             const float fw = FMT == kNvfp4 && r < p.n ? p.w_row[r] : 1.0f;
-            const bool ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sum_full[buf]), uint32_t(n / 2) & 1, &gave_up));
+            ok = still_waits(ok, smem_u32(&sum_full[buf]), uint32_t(n / 2) & 1, &gave_up);
             tc_fence_after();
 #pragma unroll 1
             for (int c0 = 0; c0 < NT; c0 += kChunk) {
@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_matmul_kernel(const __grid
 }
 
 template <int FMT, int NT>
-cudaError_t launch(const MsMatrix& x, const MsMatrix& w, long long k, void* y, int dtype, long long ldy, cudaStream_t stream) {
+cudaError_t launch(const MsMatrix& x, const MsMatrix& w, long long k, void* y, int dtype, long long ldy, unsigned loads, cudaStream_t stream) {
     using T = Tile<FMT, NT>;
     static bool ready[64] = {};
     int dev = 0;
@@ -309,7 +309,7 @@ cudaError_t launch(const MsMatrix& x, const MsMatrix& w, long long k, void* y, i
     if ((err = make_byte_map(&map_x, x.codes, pitch, x.rows, pitch, NT)) != cudaSuccess) return err;
     const size_t four = dtype == kF32 ? 16 : 8;
     const MatmulArgs p{w.scales, x.scales, w.row_scale, x.row_scale, w.rows, x.rows, int((w.rows + kRowsW - 1) / kRowsW), int((x.rows + NT - 1) / NT),
-                       int(ms_tiles_k(k)), y, ldy, dtype, reinterpret_cast<uintptr_t>(y) % four == 0 && ldy % 4 == 0};
+                       int(ms_tiles_k(k)), y, ldy, dtype, reinterpret_cast<uintptr_t>(y) % four == 0 && ldy % 4 == 0, loads};
     const long long tiles = (long long)p.tiles_n * p.tiles_m;
     int splits = 1;
     while (p.k_tiles >= 8 && splits < kMostSplits && splits * 4 <= p.k_tiles &&
@@ -337,19 +337,19 @@ cudaError_t launch(const MsMatrix& x, const MsMatrix& w, long long k, void* y, i
 //   pairs: a tile of 256 x 256 takes 1.8 times as long as one of 256 x 128, which decides by the rounds that either needs: 512 tokens 12288 x 4096
 //     18.1 and 15.7, 2048 tokens 4096 x 12288 39.9 and 43.1
 template <int FMT>
-cudaError_t launch_fmt(const MsMatrix& x, const MsMatrix& w, long long k, void* y, int dtype, long long ldy, cudaStream_t stream) {
+cudaError_t launch_fmt(const MsMatrix& x, const MsMatrix& w, long long k, void* y, int dtype, long long ldy, unsigned loads, cudaStream_t stream) {
     const long long m = x.rows, k_tiles = ms_tiles_k(k), tiles = (w.rows + kRowsW - 1) / kRowsW;
     const int sms = ms_sm_count();
     if (m > 128 || (m > 64 && tiles <= sms / 2 && k_tiles < 32)) {
         const long long pairs = sms / 2, tiles_m = (m + 255) / 256;
         const long long rounds128 = (tiles_m * tiles + pairs - 1) / pairs, rounds256 = (tiles_m * ((w.rows + 255) / 256) + pairs - 1) / pairs;
-        return launch_ms_matmul_pair(x, w, k, FMT, y, dtype, ldy, 5 * rounds128 > 9 * rounds256 ? 256 : 128, sms, stream);
+        return launch_ms_matmul_pair(x, w, k, FMT, y, dtype, ldy, 5 * rounds128 > 9 * rounds256 ? 256 : 128, sms, loads, stream);
     }
-    if (m <= 8) return launch<FMT, 8>(x, w, k, y, dtype, ldy, stream);
-    if (m <= 16) return launch<FMT, 16>(x, w, k, y, dtype, ldy, stream);
-    if (m <= 32) return launch<FMT, 32>(x, w, k, y, dtype, ldy, stream);
-    if (m <= 64) return launch<FMT, 64>(x, w, k, y, dtype, ldy, stream);
-    return launch<FMT, 128>(x, w, k, y, dtype, ldy, stream);
+    if (m <= 8) return launch<FMT, 8>(x, w, k, y, dtype, ldy, loads, stream);
+    if (m <= 16) return launch<FMT, 16>(x, w, k, y, dtype, ldy, loads, stream);
+    if (m <= 32) return launch<FMT, 32>(x, w, k, y, dtype, ldy, loads, stream);
+    if (m <= 64) return launch<FMT, 64>(x, w, k, y, dtype, ldy, loads, stream);
+    return launch<FMT, 128>(x, w, k, y, dtype, ldy, loads, stream);
 }
 
 }  // namespace
@@ -422,8 +422,8 @@ cudaError_t make_scale_map(CUtensorMap* map, const void* base, long long rows, i
     return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, base, 128, rows, 512, 128, box_rows, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
-cudaError_t launch_ms_matmul(const MsMatrix& x, const MsMatrix& w, long long k, int fmt, void* y, int dtype, long long ldy, cudaStream_t stream) {
-    return fmt == kNvfp4 ? launch_fmt<kNvfp4>(x, w, k, y, dtype, ldy, stream) : launch_fmt<kMxfp4>(x, w, k, y, dtype, ldy, stream);
+cudaError_t launch_ms_matmul(const MsMatrix& x, const MsMatrix& w, long long k, int fmt, void* y, int dtype, long long ldy, unsigned loads, cudaStream_t stream) {
+    return fmt == kNvfp4 ? launch_fmt<kNvfp4>(x, w, k, y, dtype, ldy, loads, stream) : launch_fmt<kMxfp4>(x, w, k, y, dtype, ldy, loads, stream);
 }
 
 }  // namespace tcq

@@ -13,7 +13,7 @@
 // Bound by power in long runs (1000 W: 1.5 to 1.7 GHz), then by the copies of scales to tensor memory, which nvfp4 has twice as many of: 8192 tokens
 // through 12288 x 4096 162 us (5.1 PFLOP/s), mxfp4 149 (5.5); 2048 tokens 46.4 and 42.2.
 //
-// A wait that runs out (kMbarWaitCycles) makes its CTA stop, and its results NaN.
+// A wait that runs out (kMbarWaitCycles) makes its CTA stop, and its results from there on NaN.
 #include <algorithm>
 
 #include "tcq_microscale.cuh"
@@ -49,6 +49,7 @@ struct PairArgs {
     long long ldy;
     int dtype;
     bool aligned;                                        // rows of y start on 32 bytes
+    unsigned loads;                                      // stages that a CTA loads, at most (a self-test's limit)
 };
 
 template <int FMT>
@@ -178,6 +179,7 @@ tcq_ms_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
         // ---- loads of this CTA; the warp stays together, one lane issues
         const bool one = elect_one();
         uint32_t s = 0, phase = 1, loaded = 0;           // (the first wait for each stage is for the phase before the first)
+        unsigned left = p.loads;
         bool ok = true;
         for (int t = pair; t < tiles && ok; t += pairs) {
             const int tm = t % p.tiles_m, tn = t / p.tiles_m;
@@ -187,8 +189,7 @@ tcq_ms_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
 #pragma unroll
             for (int g = 0; g < T::kGroups; ++g) row_sw[g] = min(tn * T::kGroups + g, p.groups_n - 1) * p.k_tiles * T::kAtoms;
             for (int kt = 0; kt < p.k_tiles; ++kt) {
-                ok = mbar_wait(smem_u32(&empty[s]), phase, &gave_up);
-                ok = __all_sync(0xFFFFFFFFu, ok);        // every lane has seen this phase before the next can begin
+                ok = still_waits(left-- > 0, smem_u32(&empty[s]), phase, &gave_up);      // every lane has seen this phase before the next can begin
                 if (!ok) break;
                 if (one) {
                     const uint32_t to = smem + s * T::kStageBytes, bar = full_first + s * 8;
@@ -205,12 +206,7 @@ tcq_ms_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
                 if (loaded < T::kStages) ++loaded;
             }
         }
-        if (rank == 0 && gave_up)                        // nothing may be on its way to a CTA's memory when it ends: the last loads of each stage
-            for (uint32_t i = 0; i < loaded; ++i) {
-                if (s == 0) phase ^= 1;
-                s = s == 0 ? T::kStages - 1 : s - 1;
-                for (long long t0 = clock64(); !mbar_try_wait(smem_u32(&full[s]), phase ^ 1) && clock64() - t0 < kMbarWaitCycles;) {}
-            }
+        if (rank == 0) wait_for_loads<T::kStages>(full, s, phase, loaded);       // (of both CTAs)
     } else if (warp == 1 && rank == 0) {
         // ---- products of the pair; the warp stays together, one lane issues
         constexpr uint32_t kIdesc = 1u << 7 | 1u << 10 | uint32_t(NT >> 3) << 17 | (FMT == kMxfp4 ? 1u : 0u) << 23 | 2u << 27;
@@ -265,11 +261,12 @@ tcq_ms_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
         const int quarter = warp & 3, half = (warp - 2) >> 2;
         uint32_t* const turn = reinterpret_cast<uint32_t*>(raw + (smem - smem_u32(raw)) + T::kStages * T::kStageBytes) + (warp - 2) * 32 * 36;
         int n = 0;
+        bool ok = true;
         for (int t = pair; t < tiles; t += pairs, ++n) {
             const int buf = n % T::kSumBuffers, use = n / T::kSumBuffers;
             const long long token0 = (long long)(t % p.tiles_m) * 256 + rank * 128 + 32 * quarter, col0 = (long long)(t / p.tiles_m) * NT + half * (NT / 2);
             const Factors<FMT, NT / 2> by(p, token0, col0);
-            const bool ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&sum_full[buf]), uint32_t(use) & 1, &gave_up));
+            ok = still_waits(ok, smem_u32(&sum_full[buf]), uint32_t(use) & 1, &gave_up);
             tc_fence_after();
             const uint32_t from = tmem + buf * NT + half * (NT / 2) + (uint32_t(32 * quarter) << 16), free_bar = map_rank(smem_u32(&sum_empty[buf]), 0);
             if (p.dtype == kF32) results<float, FMT, NT / 2>(p, from, free_bar, ok, token0, col0, by, turn);
@@ -287,7 +284,7 @@ tcq_ms_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
 }
 
 template <int FMT, int NT>
-cudaError_t launch(const MsMatrix& x, const MsMatrix& w, long long k, void* y, int dtype, long long ldy, int sms, cudaStream_t stream) {
+cudaError_t launch(const MsMatrix& x, const MsMatrix& w, long long k, void* y, int dtype, long long ldy, int sms, unsigned loads, cudaStream_t stream) {
     using T = Tile<FMT, NT>;
     static bool ready[64] = {};
     int dev = 0;
@@ -305,7 +302,7 @@ cudaError_t launch(const MsMatrix& x, const MsMatrix& w, long long k, void* y, i
     if ((err = make_scale_map(&map_sw, w.scales, gw * k_tiles * T::kAtoms, T::kAtoms)) != cudaSuccess) return err;
     const size_t bytes = dtype == kF32 ? 4 : 2;
     const PairArgs p{x.row_scale, w.row_scale, x.rows, w.rows, int((x.rows + 255) / 256), int((w.rows + NT - 1) / NT), int(k_tiles), int(gx), int(gw),
-                     y, ldy, dtype, reinterpret_cast<uintptr_t>(y) % 32 == 0 && ldy * bytes % 32 == 0};
+                     y, ldy, dtype, reinterpret_cast<uintptr_t>(y) % 32 == 0 && ldy * bytes % 32 == 0, loads};
     const long long tiles = (long long)p.tiles_m * p.tiles_n;
     tcq_ms_pair_kernel<FMT, NT><<<unsigned(2 * std::min<long long>(tiles, sms / 2)), kThreads, T::kSmem, stream>>>(map_x, map_w, map_sx, map_sw, p);
     return cudaGetLastError();
@@ -313,9 +310,10 @@ cudaError_t launch(const MsMatrix& x, const MsMatrix& w, long long k, void* y, i
 
 }  // namespace
 
-cudaError_t launch_ms_matmul_pair(const MsMatrix& x, const MsMatrix& w, long long k, int fmt, void* y, int dtype, long long ldy, int nt, int sms, cudaStream_t stream) {
-    if (fmt == kNvfp4) return nt == 256 ? launch<kNvfp4, 256>(x, w, k, y, dtype, ldy, sms, stream) : launch<kNvfp4, 128>(x, w, k, y, dtype, ldy, sms, stream);
-    return nt == 256 ? launch<kMxfp4, 256>(x, w, k, y, dtype, ldy, sms, stream) : launch<kMxfp4, 128>(x, w, k, y, dtype, ldy, sms, stream);
+cudaError_t launch_ms_matmul_pair(const MsMatrix& x, const MsMatrix& w, long long k, int fmt, void* y, int dtype, long long ldy, int nt, int sms, unsigned loads,
+                                  cudaStream_t stream) {
+    if (fmt == kNvfp4) return nt == 256 ? launch<kNvfp4, 256>(x, w, k, y, dtype, ldy, sms, loads, stream) : launch<kNvfp4, 128>(x, w, k, y, dtype, ldy, sms, loads, stream);
+    return nt == 256 ? launch<kMxfp4, 256>(x, w, k, y, dtype, ldy, sms, loads, stream) : launch<kMxfp4, 128>(x, w, k, y, dtype, ldy, sms, loads, stream);
 }
 
 }  // namespace tcq

@@ -13,7 +13,7 @@ import subprocess
 _CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "csrc")
 LIB_PATH = os.path.join(_CSRC, "libtcq_b200.so")
 
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 # name -> (restype, argtypes); mirrors include/tcq_b200.h one to one
 _vp, _i64, _int, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t
@@ -49,6 +49,8 @@ SIGNATURES = {
     "tcq_ms_linear_workspace_bytes": (_sz, [_i64, _i64, _i64, _int, _int]),
     "tcq_ms_linear": (_int, [_vp, _int, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _int, _vp, _i64, _vp, _sz, _vp]),
     "tcq_ms_matmul": (_int, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _int, _vp, _int, _i64, _vp]),
+    "tcq_selftest_ms_linear_waits": (_int, [_i64, _vp, _int, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _int, _vp, _i64, _vp, _sz, _vp]),
+    "tcq_selftest_ms_matmul_waits": (_int, [_i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _int, _vp, _int, _i64, _vp]),
 }
 
 _lib = None
