@@ -107,7 +107,11 @@ __device__ __forceinline__ bool next_parts(float (&r)[8], uint32_t (&h)[PARTS][4
                 asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(h[0][i / 2]) : "f"(r[i + 1] * f), "f"(r[i] * f));
                 cut = cut || (__float_as_uint(r[i]) & 0x7FFFFFFFu) - 1u < least - 1u || (__float_as_uint(r[i + 1]) & 0x7FFFFFFFu) - 1u < least - 1u;
             }
-            if (!__any_sync(0xFFFFFFFFu, cut)) return false;
+            if (!__any_sync(0xFFFFFFFFu, cut)) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) r[i] = 0.0f;   // another token may have further rounds, in which this one adds nothing
+                return false;
+            }
         }
 #pragma unroll
         for (int q = 0; q < PARTS; ++q) {
