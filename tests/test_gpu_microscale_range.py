@@ -1,0 +1,112 @@
+"""Products and values at the ends of the types' ranges, where each factor is far from 1 and their product is not.
+
+Weights are e2m1 x block scale x row scale, and any of the three may be large where another is small.  A result is finite where the sum of the
+products' magnitudes is, whatever the parts of a product are by themselves.
+
+Tolerances.  One product a result (six bits of a weight, up to 24 of x; row scales powers of two): fp32 parts are added with roundings of at most 2^-8 of
+half a step, then the result's rounding, half a step; results below the smallest normal number are rounded to the type's smallest steps, once in fp32 and once in
+the type, half a step each.  Dense sums: (k + 16) 2^-23 of the sum of magnitudes, as anywhere, and the result's rounding.
+"""
+import pytest
+import torch
+
+import ms_plain as P
+
+pytestmark = pytest.mark.gpu
+FMTS = ("mxfp4", "nvfp4")
+DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+@pytest.fixture(scope="module")
+def ms():
+    from trellis_b200 import microscale
+    return microscale
+
+
+def _near(got, ref, tol, dtype):
+    got = got.cpu().double()
+    most = torch.finfo(dtype).max * (1 + torch.finfo(dtype).eps / 4)
+    over = torch.isinf(got) & (torch.sign(got) == torch.sign(ref)) & (ref.abs() + tol >= most)
+    off = torch.where(over, torch.zeros_like(ref), (got - ref).abs())
+    assert (off <= tol).all(), f"{int((~(off <= tol)).sum())} of {off.numel()} off, {(off / tol).nan_to_num(1e30).max():.3g} of the tolerance"
+
+
+def _rounding(ref, dtype):
+    f = torch.finfo(dtype)
+    return f.eps / 2 * ref.abs() * (1 + 2.0 ** -7) + f.smallest_normal * f.eps
+
+
+def _diagonal(k, fmt, seed, byte_span, row_span):
+    """A matrix with one value a row, on the diagonal: any code, block scales and row scales over the given powers of two."""
+    g = torch.Generator().manual_seed(seed)
+    codes = torch.zeros(k, k, dtype=torch.int64)
+    codes[torch.arange(k), torch.arange(k)] = torch.randint(1, 8, (k,), generator=g) + 8 * torch.randint(0, 2, (k,), generator=g)
+    nb = k // P.BLOCK[fmt]
+    if fmt == "mxfp4":
+        return codes, 127 + torch.randint(byte_span[0], byte_span[1] + 1, (k, nb), generator=g), None
+    return codes, torch.randint(1, 0x7F, (k, nb), generator=g), torch.ldexp(torch.ones(k), torch.randint(row_span[0], row_span[1] + 1, (k,), generator=g))
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m", (1, 8))
+@pytest.mark.parametrize("spans", (((-30, 0), (-17, -17)), ((-110, -80), (-110, -60)), ((0, 30), (1, 12)), ((70, 100), (60, 117))))
+def test_few_tokens_of_any_size_times_weights_of_any_size(ms, fmt, dtype, m, spans):
+    _products(ms, fmt, dtype, m, spans)
+
+
+def _products(ms, fmt, dtype, m, spans):
+    k = 512
+    w = _diagonal(k, fmt, m, *spans)
+    v = P.values(*w, fmt).diagonal()
+    g = torch.Generator().manual_seed(m + 1)
+    lo, hi = {torch.float16: (-24, 15), torch.bfloat16: (-133, 127), torch.float32: (-149, 127)}[dtype]
+    x = ((1 + torch.rand(m, k, generator=g, dtype=torch.float64)) * torch.ldexp(torch.ones(m, k, dtype=torch.float64), torch.randint(lo, hi, (m, k), generator=g))).to(dtype)
+    x[:, ::7] = torch.finfo(dtype).max
+    x[:, 3::7] = -torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    ref = x.double() * v
+    _near(ms.linear(x.cuda(), P.pack(*w, fmt, "cuda")), ref, _rounding(ref, dtype), dtype)
+
+
+def _dense(ms, fmt, m, n, k, dtype, x_exp, w_exp, seed):
+    g = torch.Generator().manual_seed(seed)
+    w = (torch.randn(n, k, generator=g) * 2.0 ** w_exp).cuda()
+    x = (torch.randn(m, k, generator=g).double() * 2.0 ** x_exp).to(dtype).cuda()
+    q = ms.quantize(w, fmt)
+    return x, q, P.values(*P.unpack(q), fmt)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+@pytest.mark.parametrize("x_exp,w_exp", ((120, -6), (125, -40), (124, -60), (-120, 100), (-60, 60)))
+@pytest.mark.parametrize("m,n,k", ((2, 140, 1024), (8, 300, 4096), (1, 40000, 300)))
+def test_few_tokens_sums_far_from_one(ms, fmt, dtype, x_exp, w_exp, m, n, k):
+    _sums(ms, fmt, dtype, x_exp, w_exp, m, n, k)
+
+
+def _sums(ms, fmt, dtype, x_exp, w_exp, m, n, k):
+    x, q, wv = _dense(ms, fmt, m, n, k, dtype, x_exp, w_exp, m + n)
+    xv = x.cpu().double()
+    ref, bound = xv @ wv.t(), xv.abs() @ wv.abs().t()
+    _near(ms.linear(x, q), ref, (k + 16) * 2.0 ** -23 * bound + _rounding(ref, dtype), dtype)
+
+
+def test_few_tokens_row_scales_of_any_number(ms):
+    """Row scales that are not powers of two, and the smallest and the largest numbers."""
+    k = 256
+    codes, byte, _ = _diagonal(k, "nvfp4", 5, None, (0, 0))
+    row = torch.rand(k, generator=torch.Generator().manual_seed(6)) + 0.5
+    row[::5] *= 2.0 ** -120
+    row[1::5] = 1e-45
+    row[2::5] = 3e38
+    v = P.values(codes, byte, row, "nvfp4").diagonal()
+    w = P.pack(codes, byte, row, "nvfp4", "cuda")
+    for dtype in (torch.float32, torch.bfloat16):
+        for m in (1, 5):
+            x = torch.randn(m, k, generator=torch.Generator().manual_seed(m))
+            x[:, 2::5] *= 2.0 ** -20
+            x[:, 1::5] *= 2.0 ** 120
+            x = x.to(dtype)
+            ref = x.double() * v
+            # the row scale's 24 bits: one more rounding in fp32
+            _near(ms.linear(x.cuda(), w), ref, _rounding(ref, dtype) + 2.0 ** -23 * ref.abs(), dtype)

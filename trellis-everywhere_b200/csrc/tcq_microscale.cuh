@@ -71,6 +71,13 @@ template <int FMT> __device__ __forceinline__ float ms_scale_to_f32(uint32_t byt
     else return e8m0_to_f32(byte);
 }
 
+// A row scale g as power * rest: a power of two, within 2^-90 and 2^90, that goes into the products or into parts of their sum, which then are of the size of the
+// result, and what the sum is multiplied by at the end (1 to 2 where g is within those bounds).
+__device__ __forceinline__ float row_power(float g) {
+    return fminf(fmaxf(__uint_as_float(__float_as_uint(g) & 0x7F800000u), 0x1p-90f), 0x1p90f);
+}
+__device__ __forceinline__ float row_rest(float g) { return g * __uint_as_float(0x7F000000u - __float_as_uint(row_power(g))); }      // exact: divided by it
+
 template <typename T> __device__ __forceinline__ float to_f32(T v);
 template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
 template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }

@@ -4,7 +4,9 @@
 // fp16 number.  mxfp4: scales can lie outside fp16, so the sums of 32 columns are scaled instead.  x is cut into fp16 parts, 256 columns of
 // a token at a time: a power of two brings the largest magnitude under 2^15, eleven bits are cut off as fp16, and what is left is the next
 // part's, until nothing is left.  fp16 and bf16 activations nearly always take one part (nothing is left of numbers within 2^-31 of the
-// largest), fp32 three (2^-37); more are further rounds over the same codes.  So every product is exact, whatever the range.
+// largest), fp32 three (2^-37); more are further rounds over the same codes.  So every product is exact.  Sums of 32 columns (mxfp4) take the block's scale, sums
+// of 256 (nvfp4) the power of two in the row's scale, before x's factor: what is then added up is of the size of the results, whatever that of x and of W alone.
+// (Only a block scale above 2^104, of weights above 10^31, may take a sum out of range that x would bring back.)
 // (bf16 weights need no such care but three times the instructions a pair, which was the bound: 4 tokens through 151936 x 4096 136 us.)
 //
 // Work split: a CTA takes 128 rows of W, eight warps 16 rows each; one more warp loads 256 columns of codes (TMA) and scales at a time into a ring
@@ -271,6 +273,15 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
         const uint32_t from_w = lrow * 128, piece = lane >> 4, swizzle = lrow & 7;
         const int srow = 16 * warp + g;                  // rows whose scales this lane needs: srow, srow + 8
         const uint32_t from_s = G::kBytesW + (srow & 31) * 16 + (srow >> 5) * 4;
+        float power[2] = {1.0f, 1.0f};                   // nvfp4: the powers of two in these rows' scales; the first ones on their way while x is converted
+        auto fetch_power = [&](int t) {
+            if constexpr (FMT == kNvfp4) {
+                const long long row = (long long)(t < p.whole ? t : together) * kRows + srow;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) power[h] = row_power(row + 8 * h < p.w.rows ? __ldg(p.w.row_scale + row + 8 * h) : 1.0f);
+            }
+        };
+        fetch_power(blockIdx.x);
 
         // Where all of this CTA's columns fit, they are converted once, by all warps; unless that leaves something, which takes further rounds.
         const int base = p.whole ? 0 : share, span = p.whole ? p.k_tiles : until - share;
@@ -288,6 +299,7 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
 
         for (int t = blockIdx.x; t < ends; t += gridDim.x) {
             const int first = t < p.whole ? 0 : share, last = t < p.whole ? p.k_tiles : until;
+            if (t != int(blockIdx.x)) fetch_power(t);
             float acc[4] = {}, low[4] = {};              // rows g (0, 1) and g + 8, tokens 2 t4 and 2 t4 + 1; what the sums' rounding left
             int buf = 0;
             bool more = false;
@@ -354,8 +366,8 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
                                     mma_f16(d, lo, b.x, b.y);
                                     mma_f16(d, hi, b.z, b.w);
                                     const float s0 = __uint_as_float(scale[i][0]), s1 = __uint_as_float(scale[i][1]);
-                                    scaled[q][0] = fma2(mul2(pack2(d[0], d[1]), by[q]), pack2(s0, s0), scaled[q][0]);
-                                    scaled[q][1] = fma2(mul2(pack2(d[2], d[3]), by[q]), pack2(s1, s1), scaled[q][1]);
+                                    scaled[q][0] = fma2(mul2(pack2(d[0], d[1]), pack2(s0, s0)), by[q], scaled[q][0]);
+                                    scaled[q][1] = fma2(mul2(pack2(d[2], d[3]), pack2(s1, s1)), by[q], scaled[q][1]);
                                 }
                             }
                         }
@@ -364,8 +376,8 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
 #pragma unroll
                     for (int q = 0; q < PARTS; ++q) {
                         if constexpr (FMT == kNvfp4) {
-                            scaled[q][0] = mul2(pack2(sum[q][0], sum[q][1]), by[q]);
-                            scaled[q][1] = mul2(pack2(sum[q][2], sum[q][3]), by[q]);
+                            scaled[q][0] = mul2(mul2(pack2(sum[q][0], sum[q][1]), pack2(power[0], power[0])), by[q]);
+                            scaled[q][1] = mul2(mul2(pack2(sum[q][2], sum[q][3]), pack2(power[1], power[1])), by[q]);
                         }
                         float v[4];
                         unpack2(scaled[q][0], v[0], v[1]);
@@ -402,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
                     const long long row = (long long)t * kRows + i % kRows;
                     if (row < p.w.rows) {
                         float f = sums[i];
-                        if constexpr (FMT == kNvfp4) f *= p.w.row_scale[row];
+                        if constexpr (FMT == kNvfp4) f *= row_rest(p.w.row_scale[row]);
                         static_cast<T*>(p.y)[i / kRows * p.ldy + row] = from_f32<T>(f);
                     }
                 }
@@ -430,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
             for (int j = 0; j < 4; ++j)
                 if (row + j < p.w.rows) {
                     float one = e[j];
-                    if constexpr (FMT == kNvfp4) one *= p.w.row_scale[row + j];
+                    if constexpr (FMT == kNvfp4) one *= row_rest(p.w.row_scale[row + j]);
                     static_cast<T*>(p.y)[i / (kRows / 4) * p.ldy + row + j] = from_f32<T>(one);
                 }
         }
