@@ -91,17 +91,22 @@ __device__ __forceinline__ uint32_t lds32(uint32_t smem) {
 template <int FMT, bool FP16>
 __device__ __forceinline__ float row_factor(const ManyArgs& p, long long r) {
     if (r >= p.w.rows) return 1.0f;
-    if constexpr (FMT == kNvfp4) return p.w.row_scale[r];
+    if constexpr (FMT == kNvfp4) return FP16 ? p.w.row_scale[r] : row_rest(p.w.row_scale[r]);
     else if constexpr (FP16) return __uint_as_float(uint32_t(p.largest[r]) << 23 | (p.largest[r] == 0 ? 0x00400000u : 0u)) * 0x1p-13f;      // (2^-127: a denormal number)
     else return 1.0f;
 }
+
+// Weights as bf16 numbers carry the power of two of nvfp4's row scale: their sums, of activations of up to 2^128, are of the size of the results.  (fp16 activations
+// are small, and take the row scale at the end.)  Where x is in three parts, of which a later one may be up to four times the first before its 2^-8 or 2^-16, weights are
+// a quarter of what they are: still bf16 numbers, down to half of 2^-127.  (fp32 results below 2^-124 are then multiples of 2^-147, not of 2^-149.)
+template <int P> constexpr float kWeightPower = P == 3 ? 0x1p-2f : 1.0f;
 
 // The parts of a token, smallest first, as its sum.
 template <int P>
 __device__ __forceinline__ float whole_of(const float* v) {
     if constexpr (P == 1) return v[0];
     else if constexpr (P == 2) return v[1] * 0x1p-8f + v[0];
-    else return v[2] * 0x1p-16f + v[1] * 0x1p-8f + v[0];
+    else return v[2] * (0x1p-16f / kWeightPower<P>) + v[1] * (0x1p-8f / kWeightPower<P>) + v[0] / kWeightPower<P>;
 }
 
 // Steps whose sums stay in tensor memory.  The tensor cores cut sums off where fp32 arithmetic rounds, which over 12288 columns comes to 2.2e-6 of a
@@ -236,7 +241,11 @@ __global__ void __launch_bounds__(kThreads<P>, Tile<FMT, NT, P>::kCtas) tcq_ms_l
         bool ok = true;
         for (int t = blockIdx.x / splits; t < tiles && ok; t += clusters) {
             uint32_t most = 0;
-            if constexpr (FP16 && FMT == kMxfp4) most = (long long)(t / p.tiles_m) * kRows + row < p.w.rows ? p.largest[(long long)(t / p.tiles_m) * kRows + row] : 0;
+            const long long r = (long long)(t / p.tiles_m) * kRows + row;
+            float power = kWeightPower<P>;
+            if constexpr (!FP16 && FMT == kNvfp4) power *= row_power(r < p.w.rows ? __ldg(p.w.row_scale + r) : 1.0f);
+            const uint32_t power2 = (__float_as_uint(power) >> 16) * 0x10001u;               // twice, as a bf16 number
+            if constexpr (FP16 && FMT == kMxfp4) most = r < p.w.rows ? p.largest[r] : 0;
             for (int step = first; step < last && ok; ++step) {
                 if (step % 4 == 0) ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&w_full[sw]), pw, &gave_up));
                 if (step % kMakers<P> == mine && ok) {
@@ -247,6 +256,10 @@ __global__ void __launch_bounds__(kThreads<P>, Tile<FMT, NT, P>::kCtas) tcq_ms_l
                     else word = lds32(scales + 512 * (sub / 2)) >> (16 * (sub & 1));
                     uint32_t v[32], scales16[4];
                     if constexpr (!FP16) four_scales<FMT>(word, scales16);
+                    if constexpr (!FP16 && (FMT == kNvfp4 || P == 3)) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(scales16[q]) : "r"(power2));
+                    }
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {        // 16 bytes: 32 columns; the swizzle has put piece c of row r at c ^ (r % 8)
                         const uint4 c = lds128(from + (((2 * sub + i) ^ (row & 7)) << 4));
