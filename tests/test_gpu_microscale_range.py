@@ -141,3 +141,30 @@ def test_fp32_results_just_below_the_largest_number(ms, fmt, m):
     g = torch.Generator().manual_seed(m)
     x = torch.finfo(torch.float32).max / 6 * (1 - torch.rand(m, k, generator=g) * 0.4)
     assert torch.equal(ms.linear(x.cuda(), w).cpu(), (x.double() * 6).float())
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+@pytest.mark.parametrize("m,n,k", ((1, 40, 64), (20, 300, 2304), (100, 200, 512), (150, 140, 272), (300, 520, 768)))
+@pytest.mark.parametrize("x_exp,w_exp", ((122, -20), (-20, 122), (124, -70), (-60, 123), (-75, 90), (110, -110)))
+def test_matmul_of_sides_far_apart(ms, dtype, m, n, k, x_exp, w_exp):
+    """One side's row scales huge, the other's tiny: the sum of both sides' codes times one of them leaves the range, the result does not."""
+    g = torch.Generator().manual_seed(m)
+    x, w = (ms.quantize((torch.randn(r, k, generator=g) * 2.0 ** e).cuda(), "nvfp4") for r, e in ((m, x_exp), (n, w_exp)))
+    xv, wv = P.values(*P.unpack(x), "nvfp4"), P.values(*P.unpack(w), "nvfp4")
+    ref = xv @ wv.t()
+    # (both scales, powers of two, are exact)
+    _near(ms.matmul(x, w, dtype), ref, (k + 16) * 2.0 ** -23 * (xv.abs() @ wv.abs().t()) + _rounding(ref, dtype), dtype)
+
+
+def test_matmul_of_row_scales_of_any_number(ms):
+    g = torch.Generator().manual_seed(1)
+    for m in (3, 70, 150):
+        k, n = 320, 64
+        x, w = ([*P.random_matrix(r, k, "nvfp4", g)] for r in (m, n))
+        for q, rows in ((x, m), (w, n)):
+            q[2] = (torch.rand(rows, generator=g) + 0.5) * torch.ldexp(torch.ones(rows), torch.randint(-63, 64, (rows,), generator=g))
+            q[2][::7] = 1e-44
+        ref, bound = P.values(*x, "nvfp4") @ P.values(*w, "nvfp4").t(), P.values(*x, "nvfp4").abs() @ P.values(*w, "nvfp4").abs().t()
+        got = ms.matmul(P.pack(*x, "nvfp4", "cuda"), P.pack(*w, "nvfp4", "cuda"), torch.float32)
+        # three roundings by scales of 24 bits
+        _near(got, ref, (k + 16) * 2.0 ** -23 * bound + 3 * 2.0 ** -24 * ref.abs() + _rounding(ref, torch.float32), torch.float32)

@@ -78,6 +78,11 @@ __device__ __forceinline__ float row_power(float g) {
 }
 __device__ __forceinline__ float row_rest(float g) { return g * __uint_as_float(0x7F000000u - __float_as_uint(row_power(g))); }      // exact: divided by it
 
+// For products of both sides' scales: g as inner * outer, the inner one within 2^-60 and 2^60.  A sum of 4-bit products (2^-20 to 2^47) times one side's inner
+// part, the other side's scale and then the outer part leaves the range of fp32 only where the result does; the outer part is 1 unless g is extreme.
+__device__ __forceinline__ float inner_part(float g) { return g > 0x1p60f ? 0x1p60f : g < 0x1p-60f ? 0x1p-60f : g; }
+__device__ __forceinline__ float outer_part(float g) { return g > 0x1p60f ? g * 0x1p-60f : g < 0x1p-60f ? g * 0x1p60f : 1.0f; }
+
 template <typename T> __device__ __forceinline__ float to_f32(T v);
 template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
 template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }

@@ -80,14 +80,21 @@ __device__ __forceinline__ void store4(const MatmulArgs& p, long long at, float4
 
 // Columns c0 .. c0 + N - 1 (tokens) of 32 rows of W, one a lane, scaled, rounded and stored: a store is 32 neighbours in y.
 template <typename YT, int FMT, int N>
-__device__ __forceinline__ void store_columns(const MatmulArgs& p, const uint32_t (&v)[N], long long r, long long token0, float fw, float fx) {
+__device__ __forceinline__ void store_columns(const MatmulArgs& p, uint32_t (&v)[N], long long r, long long token0, float fw, float fx) {
     YT* to = static_cast<YT*>(p.y) + token0 * p.ldy + r;
     const int columns = int(min((long long)N, p.m - token0));
+    if constexpr (FMT == kNvfp4) {
+        const float inner = inner_part(fw), outer = outer_part(fw);
+#pragma unroll
+        for (int c = 0; c < N; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * inner * __shfl_sync(0xFFFFFFFFu, fx, c));
+        if (__any_sync(0xFFFFFFFFu, outer != 1.0f)) {
+#pragma unroll
+            for (int c = 0; c < N; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * outer);
+        }
+    }
 #pragma unroll
     for (int c = 0; c < N; ++c, to += p.ldy) {
-        float f = __uint_as_float(v[c]);
-        if constexpr (FMT == kNvfp4) f = f * fw * __shfl_sync(0xFFFFFFFFu, fx, c);
-        if (r < p.n && c < columns) *to = from_f32<YT>(f);
+        if (r < p.n && c < columns) *to = from_f32<YT>(__uint_as_float(v[c]));
     }
 }
 
@@ -272,7 +279,10 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_matmul_kernel(const __grid
             if constexpr (FMT == kNvfp4) {
                 const float fx = p.x_row[token];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) e[j] = e[j] * (r + j < p.n ? p.w_row[r + j] : 1.0f) * fx;
+                for (int j = 0; j < 4; ++j) {
+                    const float fw = r + j < p.n ? p.w_row[r + j] : 1.0f;
+                    e[j] = e[j] * inner_part(fw) * fx * outer_part(fw);
+                }
             }
             if (p.aligned && r + 4 <= p.n) {
                 store4(p, token * p.ldy + r, f);

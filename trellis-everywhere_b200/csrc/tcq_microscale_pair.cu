@@ -82,11 +82,13 @@ __device__ __forceinline__ void store32(void* to, const uint32_t* v) {       // 
 // What 32 tokens (one a lane) x COLS columns of results are scaled by; fetched while the products run.
 template <int FMT, int COLS>
 struct Factors {
-    float x, w[FMT == kNvfp4 ? COLS / 32 : 1];           // w: of column 32 q + lane
+    float x, outer, w[FMT == kNvfp4 ? COLS / 32 : 1];    // w: of column 32 q + lane
     __device__ __forceinline__ Factors(const PairArgs& p, long long token0, long long col0) {
         if constexpr (FMT == kNvfp4) {
             const int lane = threadIdx.x & 31;
-            x = token0 + lane < p.m ? __ldg(p.x_row + token0 + lane) : 1.0f;
+            const float g = token0 + lane < p.m ? __ldg(p.x_row + token0 + lane) : 1.0f;
+            x = inner_part(g);
+            outer = outer_part(g);
 #pragma unroll
             for (int q = 0; q < COLS / 32; ++q) w[q] = col0 + 32 * q + lane < p.n ? __ldg(p.w_row + col0 + 32 * q + lane) : 1.0f;
         }
@@ -116,6 +118,10 @@ __device__ __forceinline__ void results(const PairArgs& p, uint32_t tmem, uint32
         for (int i = 0; i < 32; ++i) {
             if constexpr (FMT == kNvfp4) v[q][i] = __float_as_uint(__uint_as_float(v[q][i]) * by.x * __shfl_sync(0xFFFFFFFFu, by.w[q], i));
             if (!ok) v[q][i] = 0x7FC00000u;
+        }
+        if (FMT == kNvfp4 && __any_sync(0xFFFFFFFFu, by.outer != 1.0f)) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[q][i] = __float_as_uint(__uint_as_float(v[q][i]) * by.outer);
         }
         if constexpr (sizeof(YT) == 4) {
 #pragma unroll
