@@ -168,3 +168,20 @@ def test_matmul_of_row_scales_of_any_number(ms):
         got = ms.matmul(P.pack(*x, "nvfp4", "cuda"), P.pack(*w, "nvfp4", "cuda"), torch.float32)
         # three roundings by scales of 24 bits
         _near(got, ref, (k + 16) * 2.0 ** -23 * bound + 3 * 2.0 ** -24 * ref.abs() + _rounding(ref, torch.float32), torch.float32)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+@pytest.mark.parametrize("rotate,k", ((16, 48), (32, 96), (64, 192), (128, 256), (128, 33024)))
+def test_rotation_of_the_largest_numbers(ms, fmt, dtype, rotate, k):
+    """Sums of `rotate` numbers leave the range where the orthonormal transform does not: the codes are those of the same numbers 2^-20 times as large."""
+    g = torch.Generator().manual_seed(rotate)
+    top = torch.finfo(dtype).max / rotate ** 0.5
+    x = (torch.randint(-2, 3, (5, k), generator=g) / 2.0 * top).to(dtype).cuda()
+    signs = (torch.randint(0, 2, (k,), generator=g) * 2.0 - 1).cuda()
+    a, b = ms.quantize(x, fmt, rotate, signs), ms.quantize(x * 2.0 ** -20, fmt, rotate, signs)
+    ca, sa, ra = P.unpack(a)
+    cb, sb, rb = P.unpack(b)
+    assert torch.equal(ca, cb) and torch.equal(sa, sb if fmt == "nvfp4" else torch.where(sb > 0, sb + 20, sb))
+    assert ra is None or torch.equal(ra, rb * 2.0 ** 20)
+    assert not torch.isnan(ms.dequantize(b)).any() and not ((sa == (255 if fmt == "mxfp4" else 0x7F)).any())

@@ -77,6 +77,7 @@ __device__ __forceinline__ void load_run(const T* __restrict__ row, long long c0
     for (int i = 0; i < kRun; ++i) v[i] = c0 + i < k ? to_f32<T>(row[c0 + i]) : 0.0f;
 }
 
+// Times 2^-7, so that no sum of 128 leaves the range of fp32 before it is multiplied by 128^(-1/2) (exact but for numbers below 2^-119).
 __device__ __forceinline__ void load_signs(const float* __restrict__ signs, long long c0, long long k, bool wide, float (&v)[kRun]) {
     if (wide && c0 + kRun <= k) {
 #pragma unroll
@@ -88,6 +89,8 @@ __device__ __forceinline__ void load_signs(const float* __restrict__ signs, long
 #pragma unroll
         for (int i = 0; i < kRun; ++i) v[i] = c0 + i < k ? signs[c0 + i] : 1.0f;
     }
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) v[i] *= 0x1p-7f;
 }
 
 // One stage of the transform between lanes h apart.
@@ -113,7 +116,7 @@ __device__ __forceinline__ void rotate_run(float (&v)[kRun], const float (&signs
     if (rotate >= 32) rotate_lanes(v, 1);
     if (rotate >= 64) rotate_lanes(v, 2);
     if (rotate >= 128) rotate_lanes(v, 4);
-    const float scale = rotate == 16 ? 0.25f : rotate == 32 ? 0.17677669529663687f : rotate == 64 ? 0.125f : 0.08838834764831845f;
+    const float scale = rotate == 16 ? 32.0f : rotate == 32 ? 0.17677669529663687f * 128 : rotate == 64 ? 16.0f : 0.08838834764831845f * 128;     // 2^7 b^(-1/2)
 #pragma unroll
     for (int i = 0; i < kRun; ++i) v[i] *= scale;
 }
