@@ -318,7 +318,7 @@ TCQ_API size_t tcq_ms_scale_bytes(int64_t rows, int64_t k, int format);
 TCQ_API int tcq_ms_quantize(const void *x, int dtype, int64_t rows, int64_t k, int64_t ldx, int format, int rotate,
                             const float *signs, uint8_t *codes, uint8_t *scales, float *row_scale, void *stream);
 
-/* The values, rounded to dtype once: out [rows][ldo], ldo >= k. */
+/* The values: exact in fp32 but for the rounding by a row scale of more than 18 bits, then rounded to dtype.  out [rows][ldo], ldo >= k. */
 TCQ_API int tcq_ms_dequantize(const uint8_t *codes, const uint8_t *scales, const float *row_scale, int64_t rows, int64_t k,
                               int format, void *out, int dtype, int64_t ldo, void *stream);
 

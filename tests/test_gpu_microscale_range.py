@@ -185,3 +185,18 @@ def test_rotation_of_the_largest_numbers(ms, fmt, dtype, rotate, k):
     assert torch.equal(ca, cb) and torch.equal(sa, sb if fmt == "nvfp4" else torch.where(sb > 0, sb + 20, sb))
     assert ra is None or torch.equal(ra, rb * 2.0 ** 20)
     assert not torch.isnan(ms.dequantize(b)).any() and not ((sa == (255 if fmt == "mxfp4" else 0x7F)).any())
+
+
+def test_values_with_row_scales_of_any_number(ms):
+    """Code times block scale is exact in fp32, so a row scale rounds once, and a zero stays one however large the scales are."""
+    g = torch.Generator().manual_seed(3)
+    rows, k = 96, 321
+    codes, byte, _ = P.random_matrix(rows, k, "nvfp4", g, spread=6)
+    byte[:, 3], byte[:, 4] = 0x7E, 1
+    codes[::2, 50:60] = torch.randint(0, 2, (rows // 2, 10), generator=g) * 8
+    row = (torch.rand(rows, generator=g) + 0.5) * torch.ldexp(torch.ones(rows), torch.randint(-126, 127, (rows,), generator=g))
+    row[:3] = torch.tensor((3.4e38, 1e-45, 2.9e-39))
+    v = P.values(codes, byte, row, "nvfp4")                      # (exact in fp64)
+    w = P.pack(codes, byte, row, "nvfp4", "cuda")
+    for dtype in DTYPES:
+        assert torch.equal(ms.dequantize(w, dtype).cpu(), v.float().to(dtype)), dtype

@@ -348,8 +348,9 @@ __global__ void __launch_bounds__(256) tcq_ms_dequantize_kernel(const uint8_t* _
     const bool is = r < rows && c0 < k;
     const long long rc = is ? r : 0, cc = is ? c0 : 0;
     const uint2 u = __ldg(reinterpret_cast<const uint2*>(codes + rc * pitch + cc / 2));
-    float s = ms_scale_to_f32<FMT>(__ldg(scales + ms_scale_at(rc, int(cc / Ms<FMT>::kBlock), atoms)));
-    if constexpr (FMT == kNvfp4) s *= __ldg(row_scale + rc);
+    const float s = ms_scale_to_f32<FMT>(__ldg(scales + ms_scale_at(rc, int(cc / Ms<FMT>::kBlock), atoms)));
+    float row = 1.0f;
+    if constexpr (FMT == kNvfp4) row = __ldg(row_scale + rc);
     uint32_t h[8];
     e2m1x8_to_f16(u.x, reinterpret_cast<uint32_t(&)[4]>(h[0]));
     e2m1x8_to_f16(u.y, reinterpret_cast<uint32_t(&)[4]>(h[4]));
@@ -359,8 +360,9 @@ __global__ void __launch_bounds__(256) tcq_ms_dequantize_kernel(const uint8_t* _
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
-        o[2 * i] = from_f32<T>(f.x * s);
-        o[2 * i + 1] = from_f32<T>(f.y * s);
+        // (the first product is exact; nvfp4's row scale, which may be any number, rounds once in fp32)
+        o[2 * i] = from_f32<T>(FMT == kNvfp4 ? f.x * s * row : f.x * s);
+        o[2 * i + 1] = from_f32<T>(FMT == kNvfp4 ? f.y * s * row : f.y * s);
     }
     T* const to = out + rc * ldo + cc;
     const bool full = is && c0 + kRun <= k;
