@@ -1,0 +1,36 @@
+"""Calls of the microscaled operators that go beyond plain matrices: gradients that are asked for, and other programs' matrices."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+import ms_plain as P
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ms():
+    from trellis_b200 import microscale
+    return microscale
+
+
+def test_inputs_that_need_a_gradient_on_the_device(ms):
+    w = P.pack(*P.random_matrix(20, 64, "nvfp4", torch.Generator().manual_seed(0)), "nvfp4", "cuda")
+    x = torch.randn(3, 64, device="cuda")
+    q, grown = ms.quantize(x), w._replace(row_scale=w.row_scale.clone().requires_grad_())
+    signs = torch.ones(64, device="cuda", requires_grad=True)
+    calls = (lambda: ms.quantize(x, rotate=16, signs=signs), lambda: ms.linear(x, grown), lambda: ms.matmul(q, grown), lambda: ms.matmul(grown, q), lambda: ms.dequantize(grown))
+    for call in calls:
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+    with torch.no_grad():
+        for call in calls:
+            call()
+        assert torch.equal(ms.linear(x, grown), ms.linear(x, w))
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        row = w._replace(row_scale=forward_ad.make_dual(w.row_scale, torch.ones_like(w.row_scale)))
+        for call in (lambda: ms.quantize(dual), lambda: ms.linear(dual, w), lambda: ms.linear(x, row), lambda: ms.dequantize(row), lambda: ms.matmul(q, row)):
+            with pytest.raises(ValueError, match="gradient"):
+                call()
+        assert torch.equal(ms.linear(x, w), ms.linear(x.clone(), w))

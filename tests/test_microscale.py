@@ -130,3 +130,28 @@ def test_selftests_of_waits_check_their_arguments():
         assert L.tcq_selftest_ms_linear_waits(loads, *linear) == -3 and L.tcq_selftest_ms_matmul_waits(loads, *matmul) == -3
     assert L.tcq_selftest_ms_linear_waits(0, None, *linear[1:]) == -4 and L.tcq_selftest_ms_matmul_waits(0, None, *matmul[1:]) == -4
     assert L.tcq_selftest_ms_linear_waits(0, p, 2, 0, *linear[3:]) == 0
+
+
+def test_every_input_that_needs_a_gradient_is_refused():
+    """Backward and forward ones, of the input, the signs and the row scales; none where gradients are off."""
+    from torch.autograd import forward_ad
+    x = torch.zeros(2, 32)
+    q = P.pack(*P.random_matrix(3, 32, "nvfp4", torch.Generator().manual_seed(0)), "nvfp4")
+    grown = q._replace(row_scale=q.row_scale.clone().requires_grad_())
+    for call in (lambda: ms.quantize(x, rotate=16, signs=torch.ones(32, requires_grad=True)), lambda: ms.linear(x, grown), lambda: ms.matmul(q, grown),
+                 lambda: ms.dequantize(grown)):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(Exception) as refused:
+            call()
+        assert "gradient" not in str(refused.value)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones(2, 32))
+        row = q._replace(row_scale=forward_ad.make_dual(q.row_scale, torch.ones(3)))
+        signs = forward_ad.make_dual(torch.ones(32), torch.ones(32))
+        for call in (lambda: ms.quantize(dual), lambda: ms.quantize(x, rotate=16, signs=signs), lambda: ms.dequantize(row), lambda: ms.linear(x, row)):
+            with pytest.raises(ValueError, match="gradient"):
+                call()
+        with pytest.raises(Exception) as refused:
+            ms.quantize(x)
+        assert "gradient" not in str(refused.value)

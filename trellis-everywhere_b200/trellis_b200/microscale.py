@@ -20,7 +20,8 @@ Codes are the nearest of the exact quotients, ties to the even code, magnitudes 
 NaN or an infinity becomes all NaN (its scale is), and nothing else changes by it.
 
 All tensors live on one CUDA device; calls are queued on its current stream, nothing synchronises, and every call can
-be captured into a graph.  Nothing here has a gradient: a call that would need one is refused.
+be captured into a graph.  Nothing here has a gradient: a call that would need one, of the input, the signs or the row scales, backward or
+forward, is refused.
 """
 from __future__ import annotations
 
@@ -28,6 +29,7 @@ import math
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .qtip import _cuda_device
@@ -73,6 +75,13 @@ def _check_dtype(dtype) -> int:
     return _DTYPES[dtype]
 
 
+def _no_gradient(t: torch.Tensor, name: str) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"no gradient is defined here: detach {name} or call under torch.no_grad()")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"no gradient is defined here, forward ones neither: {name} has a tangent")
+
+
 def _check_q(q: Microscaled, name: str) -> int:
     """The CUDA device's number of a well-formed matrix; raises otherwise (the kernels trust its sizes).
 
@@ -88,6 +97,8 @@ def _check_q(q: Microscaled, name: str) -> int:
                 and (row.get_device() == dev and row.dtype is torch.float32 and row.shape == (rows,) and row.is_contiguous()
                      and scales.shape == (-(-rows // 128), 4 * -(-k // 256), 32, 4, 4) if fmt == "nvfp4" and row is not None
                      else fmt == "mxfp4" and row is None and scales.shape == (-(-rows // 128), 2 * -(-k // 256), 32, 4, 4))):
+            if row is not None:
+                _no_gradient(row, f"{name}.row_scale")
             return dev
     return _refuse_q(q, name)
 
@@ -107,6 +118,8 @@ def _refuse_q(q, name: str) -> int:
             continue
         if t is None or t.dtype != dtype or tuple(t.shape) != shape or t.device != dev or not t.is_contiguous():
             raise ValueError(f"{name}.{part} must be a contiguous {dtype} {list(shape)} tensor on {dev}")
+    if q.row_scale is not None:
+        _no_gradient(q.row_scale, f"{name}.row_scale")
     _cuda_device()
     raise ValueError(f"{name} must be on a CUDA device")
 
@@ -115,8 +128,7 @@ def _check_x(x: torch.Tensor, name: str) -> torch.Tensor:
     """A matrix with unit column stride and rows that do not overlap, of a type the kernels take, on a CUDA device."""
     if x.dtype not in _DTYPES:
         _check_dtype(x.dtype)
-    if x.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"no gradient is defined here: detach {name} or call under torch.no_grad()")
+    _no_gradient(x, name)
     if not x.is_cuda:
         _cuda_device()
         raise ValueError(f"{name} must be on a CUDA device")
@@ -163,6 +175,8 @@ def quantize(x: torch.Tensor, fmt: str = "nvfp4", rotate: int = 0, signs: Option
         raise ValueError(f"rotate={rotate} must be one of {ROTATIONS} and divide the {x.shape[1]} columns")
     if (signs is not None) != bool(rotate):
         raise ValueError("signs go with rotate: give both or neither")
+    if signs is not None:
+        _no_gradient(signs, "signs")
     x = _check_x(x, "x")
     if signs is not None and (signs.dtype != torch.float32 or tuple(signs.shape) != (x.shape[1],) or signs.device != x.device
                               or not signs.is_contiguous()):
