@@ -34,3 +34,16 @@ def test_inputs_that_need_a_gradient_on_the_device(ms):
             with pytest.raises(ValueError, match="gradient"):
                 call()
         assert torch.equal(ms.linear(x, w), ms.linear(x.clone(), w))
+
+
+def test_a_subclass_is_a_matrix_too(ms):
+    class Named(ms.Microscaled):
+        pass
+
+    for fmt in ("mxfp4", "nvfp4"):
+        w = P.pack(*P.random_matrix(20, 64, fmt, torch.Generator().manual_seed(0)), fmt, "cuda")
+        x = torch.randn(3, 64, device="cuda")
+        q, named = ms.quantize(x, fmt), Named(*w)
+        assert torch.equal(ms.linear(x, named), ms.linear(x, w)) and torch.equal(ms.matmul(q, named), ms.matmul(q, w)) and torch.equal(ms.dequantize(named), ms.dequantize(w))
+        with pytest.raises(ValueError, match="codes"):
+            ms.dequantize(named._replace(codes=w.codes[:, :16]))

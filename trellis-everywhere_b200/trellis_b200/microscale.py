@@ -89,7 +89,7 @@ def _check_q(q: Microscaled, name: str) -> int:
     where all is well, and the search for what is wrong elsewhere (and results by ``torch.empty_strided``, which is a microsecond
     faster than ``torch.empty``).
     """
-    if type(q) is Microscaled:
+    if isinstance(q, Microscaled):
         codes, scales, row, (rows, k), fmt = q
         dev = codes.get_device()
         if (dev >= 0 and codes.dtype is torch.uint8 and scales.dtype is torch.uint8 and scales.get_device() == dev
