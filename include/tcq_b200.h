@@ -285,7 +285,7 @@ TCQ_API int tcq_codebook_lut(int codebook, float *lut, void *stream);
  *
  * A matrix of rows x k values is e2m1(code) * block scale [* row scale]:
  *   TCQ_MS_MXFP4  blocks of 32 columns, scales 2^(byte - 127) (byte 255: NaN), no row scale
- *   TCQ_MS_NVFP4  blocks of 16 columns, e4m3 scales, and one fp32 scale for each row
+ *   TCQ_MS_NVFP4  blocks of 16 columns, e4m3 scales (no sign: 0x00 to 0x7E, 0x7F: NaN), and one fp32 scale for each row
  * and is held as
  *   codes      [rows][tcq_ms_code_pitch(k)] bytes, 16-byte aligned: two codes a byte, the even column in the low half;
  *              zeros behind column k

@@ -47,3 +47,19 @@ def test_a_subclass_is_a_matrix_too(ms):
         assert torch.equal(ms.linear(x, named), ms.linear(x, w)) and torch.equal(ms.matmul(q, named), ms.matmul(q, w)) and torch.equal(ms.dequantize(named), ms.dequantize(w))
         with pytest.raises(ValueError, match="codes"):
             ms.dequantize(named._replace(codes=w.codes[:, :16]))
+
+
+@pytest.mark.parametrize("m", (1, 20, 150))
+def test_products_of_scales_with_a_sign(ms, m):
+    """Scales of another program's matrix that carry a sign: all products take it alike."""
+    gen = torch.Generator().manual_seed(m)
+    n, k = 70, 96
+    codes = torch.randint(0, 16, (n, k), generator=gen)
+    byte, sign = torch.full((n, k // 16), 0x38), torch.randint(0, 2, (n, k // 16), generator=gen)
+    w = ms.from_blocks((codes[:, 0::2] | (codes[:, 1::2] << 4)).to(torch.uint8).cuda(), (byte + 128 * sign).to(torch.uint8).cuda(), 0.5, k, "nvfp4")
+    wv = P.values(codes, byte, torch.full((n,), 0.5), "nvfp4") * (1 - 2 * sign).repeat_interleave(16, 1)
+    x = torch.randint(-4, 5, (m, k), generator=gen).float()      # whole numbers: exact sums, and exact 4-bit values
+    q = ms.quantize(x.cuda(), "nvfp4")
+    assert torch.equal(ms.dequantize(w).cpu().double(), wv)
+    assert torch.equal(ms.linear(x.cuda(), w).cpu().double(), x.double() @ wv.t())
+    assert torch.equal(ms.matmul(q, w, torch.float32).cpu().double(), ms.dequantize(q).cpu().double() @ wv.t())

@@ -155,3 +155,30 @@ def test_every_input_that_needs_a_gradient_is_refused():
         with pytest.raises(Exception) as refused:
             ms.quantize(x)
         assert "gradient" not in str(refused.value)
+
+
+@pytest.mark.parametrize("rows,k", ((1, 1), (3, 31), (130, 257), (7, 80)))
+def test_scales_with_a_sign_go_to_the_codes(rows, k):
+    gen = torch.Generator().manual_seed(rows * k)
+    codes, byte, row = P.random_matrix(rows, k, "nvfp4", gen)
+    sign = torch.randint(0, 2, byte.shape, generator=gen)
+    odd = torch.nn.functional.pad(codes, (0, k % 2), value=5)
+    packed = (odd[:, 0::2] | (odd[:, 1::2] << 4)).to(torch.uint8)
+    want = P.values(codes, byte, row, "nvfp4") * (1 - 2 * sign).repeat_interleave(16, 1)[:, :k]
+    for scales in ((byte + 128 * sign).to(torch.uint8), (byte + 128 * sign).to(torch.uint8).view(torch.float8_e4m3fn)):
+        q = ms.from_blocks(packed, scales, row, k, "nvfp4")
+        got = P.unpack(q)                                        # (checks that nothing stands behind column k)
+        assert torch.equal(got[1], byte) and torch.equal(P.values(*got, "nvfp4"), want)
+    nan = ms.from_blocks(packed, torch.full_like(byte, 0xFF, dtype=torch.uint8), row, k, "nvfp4")
+    assert (ms.block_scales(nan) == 0x7F).all()
+
+
+def test_scales_of_another_type_are_refused():
+    c = torch.zeros(2, 16, dtype=torch.uint8)
+    for fmt, row, nb, own, other in (("nvfp4", 1.0, 2, torch.float8_e4m3fn, torch.float8_e8m0fnu), ("mxfp4", None, 1, torch.float8_e8m0fnu, torch.float8_e4m3fn)):
+        s = torch.zeros(2, nb, dtype=torch.uint8)
+        for good in (s, s.view(torch.int8), s.view(own)):
+            assert not ms.block_scales(ms.from_blocks(c, good, row, 32, fmt)).any()
+        for bad in (s.view(other), s.view(torch.float8_e5m2), s.bool()):
+            with pytest.raises(ValueError, match="scales"):
+                ms.from_blocks(c, bad, row, 32, fmt)

@@ -262,24 +262,30 @@ def block_scales(q: Microscaled) -> torch.Tensor:
 def from_blocks(codes: torch.Tensor, scales: torch.Tensor, row_scale: Optional[torch.Tensor], k: int, fmt: str) -> Microscaled:
     """A matrix from row-major codes ``[rows, >= ceil(k / 2)]`` and scale bytes ``[rows, ceil(k / block)]``, as other programs store them.
 
-    ``row_scale``: fp32 ``[rows]`` or one number for all rows (nvfp4), None (mxfp4).  Done once per matrix, with torch.
+    ``row_scale``: fp32 ``[rows]`` or one number for all rows (nvfp4), None (mxfp4).  Done once per matrix, with torch.  Scales are bytes or
+    of their own type (float8_e4m3fn, float8_e8m0fnu); the tensor cores take them without a sign, so that of an e4m3 scale goes to its codes.
     """
     _check_fmt(fmt)
     if codes.dim() != 2 or scales.dim() != 2 or codes.dtype != torch.uint8 or codes.shape[1] < -(-k // 2) or k < 0:
         raise ValueError(f"expected uint8 codes [rows, >= {-(-k // 2)}], got {codes.dtype} {tuple(codes.shape)}")
     rows, nb = codes.shape[0], -(-k // BLOCKS[fmt])
-    if tuple(scales.shape) != (rows, nb) or scales.element_size() != 1:
-        raise ValueError(f"expected one-byte scales [{rows}, {nb}], got {scales.dtype} {tuple(scales.shape)}")
+    own = torch.float8_e4m3fn if fmt == "nvfp4" else torch.float8_e8m0fnu
+    if tuple(scales.shape) != (rows, nb) or scales.dtype not in (torch.uint8, torch.int8, own):
+        raise ValueError(f"expected scales [{rows}, {nb}] of bytes or {own}, got {scales.dtype} {tuple(scales.shape)}")
     if (row_scale is None) != (fmt == "mxfp4"):
         raise ValueError("row scales go with nvfp4, and only with it")
     codes_shape, scales_shape = _storage(rows, k, fmt)
     dev = codes.device
     c = torch.zeros(codes_shape, dtype=torch.uint8, device=dev)
     c[:, :-(-k // 2)] = codes[:, :-(-k // 2)]
+    scales = scales.to(dev).view(torch.uint8)
+    if fmt == "nvfp4":
+        c[:, :-(-k // 2)] ^= ((scales >> 7) * 0x88).repeat_interleave(8, 1)[:, :-(-k // 2)]
+        scales = scales & 0x7F
     if k % 2:
         c[:, k // 2] &= 15                                   # the half behind the last column
     full = torch.zeros((scales_shape[0] * 128, scales_shape[1] * 4), dtype=torch.uint8, device=dev)
-    full[:rows, :nb] = scales.to(dev).view(torch.uint8)
+    full[:rows, :nb] = scales
     tiled = full.reshape(scales_shape[0], 4, 32, scales_shape[1], 4).permute(0, 3, 2, 1, 4).contiguous()
     row = None
     if row_scale is not None:
