@@ -155,7 +155,7 @@ def apply_microscaled(model: nn.Module, fmt: str = "nvfp4", activations: int = 1
 
     A layer that stands under several names is replaced under each that is not skipped, by one ``MicroscaledLinear``.  Subclasses of
     ``nn.Linear`` stay: they may do more than its product, or their owner may read their weight (``nn.MultiheadAttention`` does).
-    All is checked before the first layer is replaced.
+    A layer's mode (``training``) goes to its replacement.  All is checked before the first layer is replaced.
     """
     microscale._check_fmt(fmt)
     found = [(name, mod) for name, mod in model.named_modules(remove_duplicate=False) if type(mod) is nn.Linear and name and not skip(name)]
@@ -166,7 +166,7 @@ def apply_microscaled(model: nn.Module, fmt: str = "nvfp4", activations: int = 1
     made = {}
     for name, mod in found:
         if mod not in made:
-            made[mod] = MicroscaledLinear(mod.weight.data, mod.bias, fmt, activations, rotate, seed_from_name(name))
+            made[mod] = MicroscaledLinear(mod.weight.data, mod.bias, fmt, activations, rotate, seed_from_name(name)).train(mod.training)
         parent, _, leaf = name.rpartition(".")
         setattr(model.get_submodule(parent), leaf, made[mod])
     return len(made)
