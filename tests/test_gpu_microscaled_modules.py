@@ -22,3 +22,37 @@ def test_replacements_keep_the_mode_of_their_layers(quant):
     assert not model[0].training and model[1][0].training and not model[2].training
     model.train()
     assert model[0].training
+
+
+def test_forward_hooks_go_with_the_layer(quant):
+    model = nn.Sequential(nn.Linear(32, 48), nn.Linear(48, 16)).cuda()
+    seen = []
+    handle = model[0].register_forward_hook(lambda mod, args, out: seen.append(out.shape))
+    model[1].register_forward_pre_hook(lambda mod, args: (args[0] * 0,))
+    model[1].register_forward_hook(lambda mod, args, kwargs, out: out + 1, with_kwargs=True)
+    bias = model[1].bias.data.clone()
+    assert quant.apply_microscaled(model) == 2
+    with torch.no_grad():
+        y = model(torch.randn(3, 32, device="cuda"))
+    assert seen == [(3, 48)] and torch.equal(y, (bias + 1).expand(3, 16))
+    handle.remove()
+    with torch.no_grad():
+        model(torch.randn(3, 32, device="cuda"))
+    assert len(seen) == 1
+
+
+@pytest.mark.parametrize("change", ("norm", "prune", "forward", "state"))
+def test_layers_that_are_more_than_their_weight_are_refused(quant, change):
+    from torch.nn.utils import prune, weight_norm
+    model = nn.Sequential(nn.Linear(32, 48), nn.Linear(48, 16)).cuda()
+    if change == "norm":
+        weight_norm(model[1])
+    elif change == "prune":
+        prune.random_unstructured(model[1], "weight", 0.3)
+    elif change == "forward":
+        model[1].forward = lambda x: x
+    else:
+        model[1].register_state_dict_pre_hook(lambda *a: None)
+    with pytest.raises(ValueError, match="^1: "):
+        quant.apply_microscaled(model)
+    assert type(model[0]) is nn.Linear and quant.apply_microscaled(model, skip=lambda name: name == "1") == 1

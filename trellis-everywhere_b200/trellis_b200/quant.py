@@ -148,6 +148,16 @@ def apply_fake_quant(model: nn.Module, quantizer: Quantizer, skip: Callable[[str
     return count
 
 
+_FORWARD_HOOKS = ("_forward_hooks", "_forward_hooks_with_kwargs", "_forward_hooks_always_called", "_forward_pre_hooks", "_forward_pre_hooks_with_kwargs")
+_STATE_HOOKS = ("_state_dict_hooks", "_state_dict_pre_hooks", "_load_state_dict_pre_hooks", "_load_state_dict_post_hooks")
+
+
+def _check_replaceable(name: str, layer: nn.Linear) -> None:
+    """Refuses a layer that is more than its weight and bias (backward hooks are left out: no gradient passes its replacement)."""
+    if "weight" not in layer._parameters or "forward" in layer.__dict__ or any(getattr(layer, h) for h in _STATE_HOOKS):
+        raise ValueError(f"{name}: its weight is computed, its forward is its own or hooks read its state: take that off first, or skip it")
+
+
 @torch.no_grad()
 def apply_microscaled(model: nn.Module, fmt: str = "nvfp4", activations: int = 16, rotate: int = 0,
                       skip: Callable[[str], bool] = lambda n: False) -> int:
@@ -155,7 +165,8 @@ def apply_microscaled(model: nn.Module, fmt: str = "nvfp4", activations: int = 1
 
     A layer that stands under several names is replaced under each that is not skipped, by one ``MicroscaledLinear``.  Subclasses of
     ``nn.Linear`` stay: they may do more than its product, or their owner may read their weight (``nn.MultiheadAttention`` does).
-    A layer's mode (``training``) goes to its replacement.  All is checked before the first layer is replaced.
+    A layer's mode (``training``) and its forward hooks go to its replacement; a layer with a computed weight (weight norm, pruning),
+    a forward of its own or hooks on its state is refused.  All is checked before the first layer is replaced.
     """
     microscale._check_fmt(fmt)
     found = [(name, mod) for name, mod in model.named_modules(remove_duplicate=False) if type(mod) is nn.Linear and name and not skip(name)]
@@ -163,10 +174,13 @@ def apply_microscaled(model: nn.Module, fmt: str = "nvfp4", activations: int = 1
         if rotate and mod.in_features % rotate:
             raise ValueError(f"{name}: rotate={rotate} does not divide its {mod.in_features} input channels")
         microscale._check_dtype(mod.weight.dtype)
+        _check_replaceable(name, mod)
     made = {}
     for name, mod in found:
         if mod not in made:
             made[mod] = MicroscaledLinear(mod.weight.data, mod.bias, fmt, activations, rotate, seed_from_name(name)).train(mod.training)
+            for hooks in _FORWARD_HOOKS:                 # (the same dict: a handle from the layer still removes its hook)
+                setattr(made[mod], hooks, getattr(mod, hooks))
         parent, _, leaf = name.rpartition(".")
         setattr(model.get_submodule(parent), leaf, made[mod])
     return len(made)
