@@ -169,18 +169,23 @@ def apply_microscaled(model: nn.Module, fmt: str = "nvfp4", activations: int = 1
     a forward of its own or hooks on its state is refused.  All is checked before the first layer is replaced.
     """
     microscale._check_fmt(fmt)
-    found = [(name, mod) for name, mod in model.named_modules(remove_duplicate=False) if type(mod) is nn.Linear and name and not skip(name)]
-    for name, mod in found:
+    layers = {}                                              # layer -> its names
+    for name, mod in model.named_modules(remove_duplicate=False):
+        if type(mod) is nn.Linear and name and not skip(name):
+            layers.setdefault(mod, []).append(name)
+    for mod, names in layers.items():
         if rotate and mod.in_features % rotate:
-            raise ValueError(f"{name}: rotate={rotate} does not divide its {mod.in_features} input channels")
+            raise ValueError(f"{names[0]}: rotate={rotate} does not divide its {mod.in_features} input channels")
         microscale._check_dtype(mod.weight.dtype)
-        _check_replaceable(name, mod)
-    made = {}
-    for name, mod in found:
-        if mod not in made:
-            made[mod] = MicroscaledLinear(mod.weight.data, mod.bias, fmt, activations, rotate, seed_from_name(name)).train(mod.training)
-            for hooks in _FORWARD_HOOKS:                 # (the same dict: a handle from the layer still removes its hook)
-                setattr(made[mod], hooks, getattr(mod, hooks))
-        parent, _, leaf = name.rpartition(".")
-        setattr(model.get_submodule(parent), leaf, made[mod])
-    return len(made)
+        _check_replaceable(names[0], mod)
+    count = len(layers)
+    while layers:                                            # a layer's own weight goes before the next one's 4 bits are made
+        mod = next(iter(layers))
+        names = layers.pop(mod)
+        new = MicroscaledLinear(mod.weight.data, mod.bias, fmt, activations, rotate, seed_from_name(names[0])).train(mod.training)
+        for hooks in _FORWARD_HOOKS:                         # (the same dict: a handle from the layer still removes its hook)
+            setattr(new, hooks, getattr(mod, hooks))
+        for name in names:
+            parent, _, leaf = name.rpartition(".")
+            setattr(model.get_submodule(parent), leaf, new)
+    return count
