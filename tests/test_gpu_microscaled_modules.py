@@ -56,3 +56,39 @@ def test_layers_that_are_more_than_their_weight_are_refused(quant, change):
     with pytest.raises(ValueError, match="^1: "):
         quant.apply_microscaled(model)
     assert type(model[0]) is nn.Linear and quant.apply_microscaled(model, skip=lambda name: name == "1") == 1
+
+
+@pytest.mark.parametrize("batch_first", (True, False))
+@pytest.mark.parametrize("mode", ("train", "eval", "no_grad", "padded"))
+def test_transformer_layers_that_read_their_weights(quant, batch_first, mode):
+    """In evaluation torch's encoder hands its layers' weights to one fused function, unless they are not plain tensors."""
+    torch.manual_seed(0)
+    layer = nn.TransformerEncoderLayer(64, 4, 128, dropout=0.0, batch_first=batch_first, device="cuda")
+    model = nn.TransformerEncoder(layer, 2)
+    assert quant.apply_microscaled(model) == 4
+    for m in model.layers:
+        assert isinstance(m.linear1, quant.MicroscaledLinear)
+    model.requires_grad_(False).train(mode == "train")
+    x = torch.randn(2, 5, 64, device="cuda")
+    mask = torch.tensor([[False] * 5, [False] * 3 + [True] * 2], device="cuda") if mode == "padded" and batch_first else None
+    with torch.set_grad_enabled(mode in ("train", "eval")):
+        y = model(x, src_key_padding_mask=mask)
+    # the same layers with the values of their 4-bit weights, on torch's plain path
+    from trellis_b200 import microscale as ms
+    plain = nn.TransformerEncoder(nn.TransformerEncoderLayer(64, 4, 128, dropout=0.0, batch_first=batch_first, device="cuda"), 2).double()
+    state = {n: t.double() for n, t in model.state_dict().items() if "linear" not in n}
+    for i, m in enumerate(model.layers):
+        for name in ("linear1", "linear2"):
+            state[f"layers.{i}.{name}.weight"] = ms.dequantize(getattr(m, name).weight).double()
+            state[f"layers.{i}.{name}.bias"] = getattr(m, name).bias.double()
+    plain.load_state_dict(state)
+    want = plain.requires_grad_(False).train()(x.double(), src_key_padding_mask=mask)
+    # two layers, each three sums of at most 128 products of fp32 numbers and a normalisation: 1e-3 is a hundred times what their roundings can add up to
+    off = (y.double() - want).abs()
+    assert (off if mask is None else off[~mask]).max() < 1e-3
+
+
+def test_torch_functions_refuse_a_matrix_in_four_bits(quant):
+    layer = quant.MicroscaledLinear(torch.randn(16, 32))
+    with pytest.raises(TypeError):
+        nn.functional.linear(torch.randn(3, 32, device="cuda"), layer.weight)

@@ -57,6 +57,12 @@ class Microscaled(NamedTuple):
     shape: Tuple[int, int]
     fmt: str
 
+    @classmethod
+    def __torch_function__(cls, func, types, args=(), kwargs=None):
+        """torch's functions do not take such a matrix: owners of a layer that look (``nn.TransformerEncoderLayer`` in evaluation) then call the
+        layer instead of handing its weight to a function, and those that do not look get a TypeError."""
+        return NotImplemented
+
 
 def _storage(rows: int, k: int, fmt: str):
     """Shapes of codes and scales."""
