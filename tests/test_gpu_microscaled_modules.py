@@ -92,3 +92,16 @@ def test_torch_functions_refuse_a_matrix_in_four_bits(quant):
     layer = quant.MicroscaledLinear(torch.randn(16, 32))
     with pytest.raises(TypeError):
         nn.functional.linear(torch.randn(3, 32, device="cuda"), layer.weight)
+
+
+@pytest.mark.parametrize("activations", (4, 16))
+def test_inputs_of_every_width_and_none(quant, activations):
+    layer = quant.MicroscaledLinear(torch.randn(16, 32), torch.randn(16), activations=activations)
+    with torch.no_grad():
+        for shape in ((0, 32), (2, 0, 32), (32,), (1, 1, 1, 32)):
+            assert layer(torch.randn(shape, device="cuda")).shape == (*shape[:-1], 16)
+        for shape in ((0, 64), (4, 16), (2, 64), (), (16, 2)):
+            with pytest.raises(ValueError, match="32"):
+                layer(torch.randn(shape, device="cuda"))
+        none = quant.MicroscaledLinear(torch.zeros(5, 0), torch.arange(5.0), activations=activations)
+        assert torch.equal(none(torch.zeros(3, 0, device="cuda")).cpu(), torch.arange(5.0).expand(3, 5))

@@ -8,6 +8,7 @@ the weights in 4 bits and multiply by them there (no counterpart in the referenc
 """
 from __future__ import annotations
 
+import math
 import zlib
 from typing import Callable, Optional
 
@@ -124,7 +125,9 @@ class MicroscaledLinear(nn.Module):
         if self.activations == 16:
             y = microscale.linear(x, self.weight)
         else:
-            q = microscale.quantize(x.reshape(-1, self.in_features), self.fmt, self.rotate, self.signs)
+            if not x.dim() or x.shape[-1] != self.in_features:
+                raise ValueError(f"x must be [..., {self.in_features}], got {tuple(x.shape)}")
+            q = microscale.quantize(x.reshape(math.prod(x.shape[:-1]), self.in_features), self.fmt, self.rotate, self.signs)
             y = microscale.matmul(q, self.weight, x.dtype).reshape(*x.shape[:-1], self.out_features)
         return y if self.bias is None else y + self.bias.to(y.dtype)
 
