@@ -9,6 +9,7 @@
 //   row_scale  [rows] fp32 (nvfp4), none (mxfp4)
 #pragma once
 
+#include <atomic>
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -102,9 +103,10 @@ struct MsMatrix {
 };
 
 int ms_sm_count();             // of the current device
-// How many clusters of `size` CTAs, `ctas` (1 or 2) of which an SM holds, run at once: fewer than SMs * ctas / size, since a cluster lies within a
-// group of SMs.
-int ms_most_clusters(const void* kernel, int threads, size_t smem, int ctas, int size);
+// How many clusters of `size` CTAs of a kernel, `ctas` (1 or 2) of which an SM holds, run at once: fewer than SMs * ctas / size, since a cluster lies within a
+// group of SMs.  `kept`: this kernel's answers so far, by device and log2(size).  (Statics of calls are atomic: two threads may make their first calls at once.)
+struct MostClusters { std::atomic<int> of[64][4]; };
+int ms_most_clusters(MostClusters& kept, const void* kernel, int threads, size_t smem, int ctas, int size);
 int report_cuda_error(cudaError_t err, const char* where);     // tcq_capi.cu
 
 cudaError_t launch_ms_quantize(const void* x, int dtype, long long rows, long long k, long long ldx, int fmt, int rotate, const float* signs,

@@ -492,7 +492,8 @@ template <typename T, int FMT, int PARTS>
 cudaError_t launch(FewArgs p, cudaStream_t stream) {
     using G = Tile<FMT, PARTS, 3>;
     const auto three = tcq_ms_linear_few_kernel<T, FMT, PARTS, 3>, two = tcq_ms_linear_few_kernel<T, FMT, PARTS, 2>;
-    static bool ready[64] = {};
+    static std::atomic<bool> ready[64];
+    static MostClusters kept;
     int dev = 0;
     cudaError_t err = cudaGetDevice(&dev);
     if (err != cudaSuccess) return err;
@@ -513,7 +514,7 @@ cudaError_t launch(FewArgs p, cudaStream_t stream) {
     // (4600 x 4096, which 8 would give more clusters than run at once: 14.6 / 9.3 / 8.8 / 10.6)
     int splits = 1;
     while (splits < kMostSplits && splits * 2 <= p.k_tiles &&
-           p.tiles <= ms_most_clusters(reinterpret_cast<const void*>(three), kThreads, G::kSmem, 2, splits * 2)) splits *= 2;
+           p.tiles <= ms_most_clusters(kept, reinterpret_cast<const void*>(three), kThreads, G::kSmem, 2, splits * 2)) splits *= 2;
     // One stage less where that makes room for all of x: eight tokens through 40960 x 4096 48.0 -> 41.4 us, 151936 x 4096 132 -> 91.5.
     // More groups of rows than that: all of them whole, in turns of which the last may be a short one; or the last ones shared by clusters again, at once.
     // The cost is counted in turns; a CTA alone on its SM takes 0.55 of one, an
@@ -524,7 +525,7 @@ cudaError_t launch(FewArgs p, cudaStream_t stream) {
         const auto part = [](int ctas) { return ctas == 0 ? 0.0 : ctas <= ms_sm_count() ? 0.55 : 1.0; };
         double least = p.tiles / grid + part(p.tiles % grid);
         for (int share = 2; share <= 4 && share <= p.k_tiles; share *= 2) {
-            const int clusters = ms_most_clusters(reinterpret_cast<const void*>(three), kThreads, G::kSmem, 2, share), ctas = clusters * share;
+            const int clusters = ms_most_clusters(kept, reinterpret_cast<const void*>(three), kThreads, G::kSmem, 2, share), ctas = clusters * share;
             const int left = p.tiles % ctas;
             const double cost = p.tiles / ctas + part(left * share) / share + 0.15;
             if (left <= clusters && cost < least) {

@@ -424,7 +424,8 @@ template <typename YT, int FMT, int NT, int P, bool FP16>
 cudaError_t launch(const ManyCall& c, cudaStream_t stream) {
     using T = Tile<FMT, NT, P>;
     const auto kernel = tcq_ms_linear_many_kernel<YT, FMT, NT, P, FP16>;
-    static bool ready[64] = {};
+    static std::atomic<bool> ready[64];
+    static MostClusters kept;
     int dev = 0;
     cudaError_t err = cudaGetDevice(&dev);
     if (err != cudaSuccess) return err;
@@ -446,8 +447,8 @@ cudaError_t launch(const ManyCall& c, cudaStream_t stream) {
     const int k_tiles = int(ms_tiles_k(c.k)), sms = ms_sm_count();
     const auto fits = [&](int s) {
         if (T::kCtas == 2 && tiles * s > sms && k_tiles < 4 * s) return false;
-        return tiles <= (T::kCtas == 2 ? ms_most_clusters(reinterpret_cast<const void*>(tcq_ms_scale_range_kernel), 256, T::kSmem, 2, s)
-                                       : ms_most_clusters(reinterpret_cast<const void*>(kernel), kThreads<P>, T::kSmem, 1, s));
+        return tiles <= (T::kCtas == 2 ? ms_most_clusters(kept, reinterpret_cast<const void*>(tcq_ms_scale_range_kernel), 256, T::kSmem, 2, s)
+                                       : ms_most_clusters(kept, reinterpret_cast<const void*>(kernel), kThreads<P>, T::kSmem, 1, s));
     };
     int splits = 1;
     while (NT <= 128 && splits < kMostSplits && 2 * splits <= k_tiles && fits(2 * splits)) splits *= 2;

@@ -305,7 +305,8 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_matmul_kernel(const __grid
 template <int FMT, int NT>
 cudaError_t launch(const MsMatrix& x, const MsMatrix& w, long long k, void* y, int dtype, long long ldy, unsigned loads, cudaStream_t stream) {
     using T = Tile<FMT, NT>;
-    static bool ready[64] = {};
+    static std::atomic<bool> ready[64];
+    static MostClusters kept;
     int dev = 0;
     cudaError_t err = cudaGetDevice(&dev);
     if (err != cudaSuccess) return err;
@@ -323,7 +324,7 @@ cudaError_t launch(const MsMatrix& x, const MsMatrix& w, long long k, void* y, i
     const long long tiles = (long long)p.tiles_n * p.tiles_m;
     int splits = 1;
     while (p.k_tiles >= 8 && splits < kMostSplits && splits * 4 <= p.k_tiles &&
-           tiles <= ms_most_clusters(reinterpret_cast<const void*>(tcq_ms_matmul_kernel<FMT, NT>), kThreads, T::kSmem, 1, splits * 2)) splits *= 2;
+           tiles <= ms_most_clusters(kept, reinterpret_cast<const void*>(tcq_ms_matmul_kernel<FMT, NT>), kThreads, T::kSmem, 1, splits * 2)) splits *= 2;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(splits > 1 ? tiles * splits : std::min<long long>(tiles, ms_sm_count())));
     cfg.blockDim = dim3(kThreads);
@@ -365,21 +366,20 @@ cudaError_t launch_fmt(const MsMatrix& x, const MsMatrix& w, long long k, void* 
 }  // namespace
 
 int ms_sm_count() {
-    static int cache[64] = {};
+    static std::atomic<int> cache[64];
     int dev = 0, n = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return 148;
-    if (dev < 64 && cache[dev]) return cache[dev];
+    if (dev < 64 && (n = cache[dev]) != 0) return n;
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
     if (dev < 64) cache[dev] = n;
     return n;
 }
 
-int ms_most_clusters(const void* kernel, int threads, size_t smem, int ctas, int size) {
-    static int cache[64][2][4] = {};                         // by ctas - 1 and log2(size)
+int ms_most_clusters(MostClusters& kept, const void* kernel, int threads, size_t smem, int ctas, int size) {
     const int slot = size >= 8 ? 3 : size / 2, most = ctas * ms_sm_count() / size;
     int dev = 0, n = 0;
     if (size == 1 || cudaGetDevice(&dev) != cudaSuccess) return most;
-    if (dev < 64 && cache[dev][ctas - 1][slot]) return cache[dev][ctas - 1][slot];
+    if (dev < 64 && (n = kept.of[dev][slot]) != 0) return n;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(size));
     cfg.blockDim = dim3(unsigned(threads));
@@ -394,7 +394,7 @@ int ms_most_clusters(const void* kernel, int threads, size_t smem, int ctas, int
         (void)cudaGetLastError();
         return most;
     }
-    if (dev < 64) cache[dev][ctas - 1][slot] = n;
+    if (dev < 64) kept.of[dev][slot] = n;
     return n;
 }
 
@@ -403,14 +403,15 @@ cudaError_t encode_map(CUtensorMap* map, CUtensorMapDataType type, const void* b
                        cuuint32_t box_rows, CUtensorMapSwizzle swizzle) {
     using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                                 CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-    static Encode encode = nullptr;
+    static std::atomic<Encode> kept{nullptr};
+    Encode encode = kept;
     if (encode == nullptr) {
         void* fn = nullptr;
         cudaDriverEntryPointQueryResult found{};
         const cudaError_t err = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found);
         if (err != cudaSuccess) return err;
         if (found != cudaDriverEntryPointSuccess || fn == nullptr) return cudaErrorNotSupported;
-        encode = reinterpret_cast<Encode>(fn);
+        kept = encode = reinterpret_cast<Encode>(fn);
     }
     const cuuint64_t dims[2] = {width, rows}, strides[1] = {pitch};
     const cuuint32_t box[2] = {box_width, box_rows}, steps[2] = {1, 1};

@@ -292,7 +292,7 @@ tcq_ms_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
 template <int FMT, int NT>
 cudaError_t launch(const MsMatrix& x, const MsMatrix& w, long long k, void* y, int dtype, long long ldy, int sms, unsigned loads, cudaStream_t stream) {
     using T = Tile<FMT, NT>;
-    static bool ready[64] = {};
+    static std::atomic<bool> ready[64];
     int dev = 0;
     cudaError_t err = cudaGetDevice(&dev);
     if (err != cudaSuccess) return err;
