@@ -273,15 +273,15 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
         const uint32_t from_w = lrow * 128, piece = lane >> 4, swizzle = lrow & 7;
         const int srow = 16 * warp + g;                  // rows whose scales this lane needs: srow, srow + 8
         const uint32_t from_s = G::kBytesW + (srow & 31) * 16 + (srow >> 5) * 4;
-        float power[2] = {1.0f, 1.0f};                   // nvfp4: the powers of two in these rows' scales; the first ones on their way while x is converted
-        auto fetch_power = [&](int t) {
+        float g2[2] = {1.0f, 1.0f};                      // nvfp4: these rows' scales; the first ones are on their way while x is converted
+        auto fetch_scales = [&](int t) {
             if constexpr (FMT == kNvfp4) {
                 const long long row = (long long)(t < p.whole ? t : together) * kRows + srow;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) power[h] = row_power(row + 8 * h < p.w.rows ? __ldg(p.w.row_scale + row + 8 * h) : 1.0f);
+                for (int h = 0; h < 2; ++h) g2[h] = row + 8 * h < p.w.rows ? __ldg(p.w.row_scale + row + 8 * h) : 1.0f;
             }
         };
-        fetch_power(blockIdx.x);
+        fetch_scales(blockIdx.x);
 
         // Where all of this CTA's columns fit, they are converted once, by all warps; unless that leaves something, which takes further rounds.
         const int base = p.whole ? 0 : share, span = p.whole ? p.k_tiles : until - share;
@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
 
         for (int t = blockIdx.x; t < ends; t += gridDim.x) {
             const int first = t < p.whole ? 0 : share, last = t < p.whole ? p.k_tiles : until;
-            if (t != int(blockIdx.x)) fetch_power(t);
+            if (t != int(blockIdx.x)) fetch_scales(t);
             float acc[4] = {}, low[4] = {};              // rows g (0, 1) and g + 8, tokens 2 t4 and 2 t4 + 1; what the sums' rounding left
             int buf = 0;
             bool more = false;
@@ -376,6 +376,7 @@ __global__ void __launch_bounds__(kThreads, 2) tcq_ms_linear_few_kernel(const __
 #pragma unroll
                     for (int q = 0; q < PARTS; ++q) {
                         if constexpr (FMT == kNvfp4) {
+                            const float power[2] = {row_power(g2[0]), row_power(g2[1])};
                             scaled[q][0] = mul2(mul2(pack2(sum[q][0], sum[q][1]), pack2(power[0], power[0])), by[q]);
                             scaled[q][1] = mul2(mul2(pack2(sum[q][2], sum[q][3]), pack2(power[1], power[1])), by[q]);
                         }
