@@ -237,13 +237,21 @@ __global__ void __launch_bounds__(kThreads<P>, Tile<FMT, NT, P>::kCtas) tcq_ms_l
         const int quarter = warp & 3, mine = (warp - 6) >> 2;
         const int row = 32 * quarter + lane;
         const E2m1Bytes bytes;
+        const auto scale_of = [&](int t) {               // of this lane's row; fetched a tile ahead
+            const long long r = (long long)(t / p.tiles_m) * kRows + row;
+            return !FP16 && FMT == kNvfp4 && t < tiles && r < p.w.rows ? __ldg(p.w.row_scale + r) : 1.0f;
+        };
+        float next = scale_of(blockIdx.x / splits);
         uint32_t sw = 0, pw = 0, sa = 0, pa = 1;
         bool ok = true;
         for (int t = blockIdx.x / splits; t < tiles && ok; t += clusters) {
             uint32_t most = 0;
             const long long r = (long long)(t / p.tiles_m) * kRows + row;
             float power = kWeightPower<P>;
-            if constexpr (!FP16 && FMT == kNvfp4) power *= row_power(r < p.w.rows ? __ldg(p.w.row_scale + r) : 1.0f);
+            if constexpr (!FP16 && FMT == kNvfp4) {
+                power *= row_power(next);
+                next = scale_of(t + clusters);
+            }
             const uint32_t power2 = (__float_as_uint(power) >> 16) * 0x10001u;               // twice, as a bf16 number
             if constexpr (FP16 && FMT == kMxfp4) most = r < p.w.rows ? p.largest[r] : 0;
             for (int step = first; step < last && ok; ++step) {
