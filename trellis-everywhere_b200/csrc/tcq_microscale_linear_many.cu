@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(kThreads<P>, Tile<FMT, NT, P>::kCtas) tcq_ms_l
         // ---- weights: lane = row of this warp's quarter; the groups of four warps take turns
         const int quarter = warp & 3, mine = (warp - 6) >> 2;
         const int row = 32 * quarter + lane;
-        const E2m1Bytes bytes;
+        const E2m1Bytes<P == 3> bytes;
         const auto scale_of = [&](int t) {               // of this lane's row; fetched a tile ahead
             const long long r = (long long)(t / p.tiles_m) * kRows + row;
             return !FP16 && FMT == kNvfp4 && t < tiles && r < p.w.rows ? __ldg(p.w.row_scale + r) : 1.0f;
@@ -247,9 +247,9 @@ __global__ void __launch_bounds__(kThreads<P>, Tile<FMT, NT, P>::kCtas) tcq_ms_l
         for (int t = blockIdx.x / splits; t < tiles && ok; t += clusters) {
             uint32_t most = 0;
             const long long r = (long long)(t / p.tiles_m) * kRows + row;
-            float power = kWeightPower<P>;
+            float power = 1.0f;
             if constexpr (!FP16 && FMT == kNvfp4) {
-                power *= row_power(next);
+                power = row_power(next);
                 next = scale_of(t + clusters);
             }
             const uint32_t power2 = (__float_as_uint(power) >> 16) * 0x10001u;               // twice, as a bf16 number
@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(kThreads<P>, Tile<FMT, NT, P>::kCtas) tcq_ms_l
                     else word = lds32(scales + 512 * (sub / 2)) >> (16 * (sub & 1));
                     uint32_t v[32], scales16[4];
                     if constexpr (!FP16) four_scales<FMT>(word, scales16);
-                    if constexpr (!FP16 && (FMT == kNvfp4 || P == 3)) {
+                    if constexpr (!FP16 && FMT == kNvfp4) {
 #pragma unroll
                         for (int q = 0; q < 4; ++q) asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(scales16[q]) : "r"(power2));
                     }

@@ -6,11 +6,13 @@
 namespace tcq {
 
 // The magnitudes 0 .5 1 1.5 2 3 4 6 as bf16 numbers: low bytes 00 00 80 C0 00 40 80 C0, high bytes 00 3F 3F 3F 40 40 40 40.  Made so that they stay in registers
-// (the compiler would put each anew before every use: a third more instructions).
+// (the compiler would put each anew before every use: a third more instructions).  QUARTER: a fourth of them, high bytes 00 3E 3E 3E 3F 3F 3F 3F.
+template <bool QUARTER>
 struct E2m1Bytes {
     uint32_t low0, low1, high0, high1;
     __device__ __forceinline__ E2m1Bytes() {
-        asm volatile("mov.b32 %0, 0xC0800000;\n\tmov.b32 %1, 0xC0804000;\n\tmov.b32 %2, 0x3F3F3F00;\n\tmov.b32 %3, 0x40404040;" : "=r"(low0), "=r"(low1), "=r"(high0), "=r"(high1));
+        asm volatile("mov.b32 %0, 0xC0800000;\n\tmov.b32 %1, 0xC0804000;\n\tmov.b32 %2, %4;\n\tmov.b32 %3, %5;"
+                     : "=r"(low0), "=r"(low1), "=r"(high0), "=r"(high1) : "n"(QUARTER ? 0x3E3E3E00 : 0x3F3F3F00), "n"(QUARTER ? 0x3F3F3F3F : 0x40404040));
     }
 };
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t pick) {      // (__byte_perm masks what picks)
@@ -20,7 +22,8 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t pick) 
 }
 // Eight codes as bf16 pairs in order, times the scale.  Two byte permutations look four magnitudes up as the bytes of bf16 numbers, one spreads the
 // signs; these half-rate instructions are what bounds it, so what can be shared by all eight is.
-__device__ __forceinline__ void eight_weights(const E2m1Bytes& e, uint32_t w, uint32_t scale, uint32_t (&out)[4]) {
+template <bool QUARTER>
+__device__ __forceinline__ void eight_weights(const E2m1Bytes<QUARTER>& e, uint32_t w, uint32_t scale, uint32_t (&out)[4]) {
     const uint32_t mag = w & 0x77777777u, up = w << 4;
     const uint32_t sign[2] = {prmt(w, up, 0x9D8Cu), prmt(w, up, 0xBFAEu)};            // the top bit of each code, over a whole byte
 #pragma unroll
