@@ -587,7 +587,7 @@ cudaError_t launch_ms_linear(const void* x, int dtype, long long m, long long ld
     const long long width = ms_tiles_k(k) * kMsTileK;
     const unsigned grid = unsigned((m * (width / 8) + 255) / 256);
     uint8_t* const scratch = static_cast<uint8_t*>(ws);
-    ManyCall c{x, ldx, k, m, 1, dtype, w, k, fmt, y, ldy, false, nullptr, nullptr, loads};
+    ManyCall c{x, ldx, k, m, dtype, w, k, fmt, y, ldy, false, nullptr, nullptr, loads};
     cudaError_t err;
     // fp16 through mxfp4: up to 128 tokens, and while tiles of 64 leave half of the SMs free, two bf16 parts (200 through 1024 x 4096 15.4 us), else fp16
     // weights (23.4; but through 4096 x 12288 52.5 instead of 69.5, 12288 x 4096 39 instead of 53).
@@ -611,11 +611,9 @@ cudaError_t launch_ms_linear(const void* x, int dtype, long long m, long long ld
     }
     // x in parts of bf16 numbers
     if (dtype == kF32) {
-        c.parts = 3;
         c.x = ws;
         tcq_ms_parts_kernel<float, 3><<<grid, 256, 0, stream>>>(static_cast<const float*>(x), m, k, ldx, static_cast<__nv_bfloat16*>(ws), width, nullptr);
     } else {
-        c.parts = 2;
         c.x = scratch + row_bytes(m, k);
         tcq_ms_parts_kernel<__half, 2><<<grid, 256, 0, stream>>>(static_cast<const __half*>(x), m, k, ldx, reinterpret_cast<__nv_bfloat16*>(scratch + row_bytes(m, k)), width, c.wide);
     }

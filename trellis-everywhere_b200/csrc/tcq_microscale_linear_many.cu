@@ -26,8 +26,8 @@ namespace tcq {
 namespace {
 
 // Warps: loader, issuer, four for the results, and groups of four that make weights.
-template <int P> constexpr int kMakers = 2;
-template <int P> constexpr int kThreads = 32 * (6 + 4 * kMakers<P>);
+constexpr int kMakers = 2;
+constexpr int kThreads = 32 * (6 + 4 * kMakers);
 constexpr int kRows = 128, kStepK = 64;          // rows of W; columns of a step
 constexpr int kMostSplits = 8;
 
@@ -121,7 +121,7 @@ __device__ __forceinline__ uint32_t relative_scale(uint32_t byte, uint32_t most)
 }
 
 template <typename YT, int FMT, int NT, int P, bool FP16>
-__global__ void __launch_bounds__(kThreads<P>, Tile<FMT, NT, P>::kCtas) tcq_ms_linear_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+__global__ void __launch_bounds__(kThreads, Tile<FMT, NT, P>::kCtas) tcq_ms_linear_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                                                                          const __grid_constant__ ManyArgs p) {
     using T = Tile<FMT, NT, P>;
     constexpr int kTokens = NT / P;                      // of a tile
@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(kThreads<P>, Tile<FMT, NT, P>::kCtas) tcq_ms_l
 
     if (warp == 0 && elect_one()) {
         gave_up = 0;
-        for (int s = 0; s < T::kStagesW; ++s) { mbar_init(smem_u32(&w_full[s]), 1); mbar_init(smem_u32(&w_empty[s]), 4 * kMakers<P>); }
+        for (int s = 0; s < T::kStagesW; ++s) { mbar_init(smem_u32(&w_full[s]), 1); mbar_init(smem_u32(&w_empty[s]), 4 * kMakers); }
         for (int s = 0; s < T::kStagesX; ++s) { mbar_init(smem_u32(&x_full[s]), 1); mbar_init(smem_u32(&x_empty[s]), 1); }
         for (int s = 0; s < T::kStagesA; ++s) { mbar_init(smem_u32(&a_full[s]), 4); mbar_init(smem_u32(&a_empty[s]), 1); }
         for (int s = 0; s < T::kSumBuffers; ++s) { mbar_init(smem_u32(&sum_full[s]), 1); mbar_init(smem_u32(&sum_empty[s]), 4); }
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(kThreads<P>, Tile<FMT, NT, P>::kCtas) tcq_ms_l
             if constexpr (FP16 && FMT == kMxfp4) most = r < p.w.rows ? p.largest[r] : 0;
             for (int step = first; step < last && ok; ++step) {
                 if (step % 4 == 0) ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&w_full[sw]), pw, &gave_up));
-                if (step % kMakers<P> == mine && ok) {
+                if (step % kMakers == mine && ok) {
                     const uint32_t from = smem_w + sw * T::kStageW + row * 128, sub = step % 4;
                     uint32_t word;
                     const uint32_t scales = smem_w + sw * T::kStageW + T::kBytesW + lane * 16 + quarter * 4;
@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(kThreads<P>, Tile<FMT, NT, P>::kCtas) tcq_ms_l
         const int t = blockIdx.x / splits;
         const long long r0 = (long long)(t / p.tiles_m) * kRows, token0 = (long long)(t % p.tiles_m) * kTokens;
         const int tokens = int(min((long long)kTokens, p.m - token0));
-        for (int i = int(rank) * kThreads<P> + threadIdx.x; i < kRows / 4 * tokens; i += int(splits) * kThreads<P>) {
+        for (int i = int(rank) * kThreads + threadIdx.x; i < kRows / 4 * tokens; i += int(splits) * kThreads) {
             const int r4 = i % (kRows / 4), token = i / (kRows / 4);
             const long long r = r0 + 4 * r4;
             if (r >= p.w.rows) continue;
@@ -456,13 +456,13 @@ cudaError_t launch(const ManyCall& c, cudaStream_t stream) {
     const auto fits = [&](int s) {
         if (T::kCtas == 2 && tiles * s > sms && k_tiles < 4 * s) return false;
         return tiles <= (T::kCtas == 2 ? ms_most_clusters(kept, reinterpret_cast<const void*>(tcq_ms_scale_range_kernel), 256, T::kSmem, 2, s)
-                                       : ms_most_clusters(kept, reinterpret_cast<const void*>(kernel), kThreads<P>, T::kSmem, 1, s));
+                                       : ms_most_clusters(kept, reinterpret_cast<const void*>(kernel), kThreads, T::kSmem, 1, s));
     };
     int splits = 1;
     while (NT <= 128 && splits < kMostSplits && 2 * splits <= k_tiles && fits(2 * splits)) splits *= 2;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(splits > 1 ? tiles * splits : std::min<long long>(tiles, T::kCtas * ms_sm_count())));
-    cfg.blockDim = dim3(kThreads<P>);
+    cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = T::kSmem;
     cfg.stream = stream;
     cudaLaunchAttribute attr{};
@@ -479,12 +479,16 @@ cudaError_t launch(const ManyCall& c, cudaStream_t stream) {
 template <typename YT, int FMT, int P, bool FP16>
 cudaError_t launch_nt(const ManyCall& c, cudaStream_t stream) {
     const long long rows = c.m * P;
-    if (rows <= 16 / P * P) return launch<YT, FMT, 16, P, FP16>(c, stream);
-    if (rows <= 32 / P * P) return launch<YT, FMT, 32, P, FP16>(c, stream);
+    constexpr bool kMany = FP16 && FMT == kMxfp4;        // called from 129 tokens on; the others from nine
+    if constexpr (!kMany && P == 1)
+        if (rows <= 16) return launch<YT, FMT, 16, P, FP16>(c, stream);
+    if constexpr (!kMany)
+        if (rows <= 32 / P * P) return launch<YT, FMT, 32, P, FP16>(c, stream);
     if constexpr (P == 3) {
         return launch<YT, FMT, 64, P, FP16>(c, stream);  // sums in registers: no more than 64 columns
     } else {
-        if (rows <= 64 / P * P) return launch<YT, FMT, 64, P, FP16>(c, stream);
+        if constexpr (!kMany)
+            if (rows <= 64 / P * P) return launch<YT, FMT, 64, P, FP16>(c, stream);
         if ((c.w.rows + kRows - 1) / kRows * ((c.m + 128 / P - 1) / (128 / P)) <= ms_sm_count()) return launch<YT, FMT, 128, P, FP16>(c, stream);
         return launch<YT, FMT, 256, P, FP16>(c, stream);
     }
@@ -494,7 +498,9 @@ template <int FMT>
 cudaError_t launch_fmt(const ManyCall& c, cudaStream_t stream) {
     if (c.dtype == kF32) return launch_nt<float, FMT, 3, false>(c, stream);
     if (c.dtype == kBf16) return launch_nt<__nv_bfloat16, FMT, 1, false>(c, stream);
-    return c.fp16 ? launch_nt<__half, FMT, 1, true>(c, stream) : launch_nt<__half, FMT, 2, false>(c, stream);
+    if constexpr (FMT == kMxfp4)
+        if (!c.fp16) return launch_nt<__half, FMT, 2, false>(c, stream);
+    return launch_nt<__half, FMT, 1, true>(c, stream);   // nvfp4's weights are fp16 numbers
 }
 
 // One CTA a group of 128 rows; a warp reads the 512 bytes of 128 columns at a time, a lane the four rows lane + 32 q.

@@ -6,10 +6,9 @@
 namespace tcq {
 
 struct ManyCall {
-    const void* x;               // m * parts rows of bf16 (or m of fp16), 16-byte aligned, `width` columns of them (the others zero)
+    const void* x;               // the parts of m tokens (1 for bf16, 2 for fp16, 3 for fp32) as rows of bf16, or m rows of fp16, 16-byte aligned, `width` columns of them (the others zero)
     long long ldx, width;
     long long m;
-    int parts;                   // of a token: 1 (bf16), 2 (fp16), 3 (fp32)
     int dtype;                   // of y
     MsMatrix w;
     long long k;
