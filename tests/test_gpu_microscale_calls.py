@@ -63,3 +63,18 @@ def test_products_of_scales_with_a_sign(ms, m):
     assert torch.equal(ms.dequantize(w).cpu().double(), wv)
     assert torch.equal(ms.linear(x.cuda(), w).cpu().double(), x.double() @ wv.t())
     assert torch.equal(ms.matmul(q, w, torch.float32).cpu().double(), ms.dequantize(q).cpu().double() @ wv.t())
+
+
+@pytest.mark.parametrize("fmt", ("mxfp4", "nvfp4"))
+def test_outliers_do_not_set_the_scales_of_a_rotated_matrix(ms, fmt):
+    """One channel of 100 among values of at most 1.  Unrotated it is its block's largest value, 100; rotated by 128 no value is above (100 + 127) / 128^(1/2) = 20.1,
+    so that the largest scale falls from 2^4 to 2^2 at most (mxfp4), or from at least 100 / 6 (1 - 2^-4) to at most 20.1 / 6 (1 + 2^-4) (nvfp4)."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.rand(200, 512, generator=g, device="cuda") * 2 - 1
+    x[:, 17] = 100.0
+    signs = torch.randint(0, 2, (512,), generator=g, device="cuda").float() * 2 - 1
+    top = []
+    for q in (ms.quantize(x, fmt), ms.quantize(x, fmt, 128, signs)):
+        s = P.scale_values(ms.block_scales(q).long().cpu(), fmt)
+        top.append((s if q.row_scale is None else s * q.row_scale.cpu().double()[:, None]).amax(1))
+    assert (top[1] <= top[0] / 4).all()
