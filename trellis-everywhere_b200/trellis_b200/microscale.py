@@ -103,7 +103,7 @@ def _check_q(q: Microscaled, name: str) -> int:
                 and (row.get_device() == dev and row.dtype is torch.float32 and row.shape == (rows,) and row.is_contiguous()
                      and scales.shape == (-(-rows // 128), 4 * -(-k // 256), 32, 4, 4) if fmt == "nvfp4" and row is not None
                      else fmt == "mxfp4" and row is None and scales.shape == (-(-rows // 128), 2 * -(-k // 256), 32, 4, 4))):
-            if row is not None:
+            if row is not None and (row.requires_grad or forward_ad._current_level >= 0):
                 _no_gradient(row, f"{name}.row_scale")
             return dev
     return _refuse_q(q, name)
@@ -134,7 +134,8 @@ def _check_x(x: torch.Tensor, name: str) -> torch.Tensor:
     """A matrix with unit column stride and rows that do not overlap, of a type the kernels take, on a CUDA device."""
     if x.dtype not in _DTYPES:
         _check_dtype(x.dtype)
-    _no_gradient(x, name)
+    if x.requires_grad or forward_ad._current_level >= 0:
+        _no_gradient(x, name)
     if not x.is_cuda:
         _cuda_device()
         raise ValueError(f"{name} must be on a CUDA device")
