@@ -47,3 +47,11 @@ def test_nothing_is_replaced_where_a_later_layer_is_refused(standin):
         with pytest.raises(ValueError):
             quant.apply_microscaled(model, activations=4, rotate=64)
         assert not standin.made and all(type(m) is nn.Linear for m in model)
+
+
+def test_layers_without_values_are_refused_before_any_is_replaced(standin):
+    standin.watched = []
+    model = nn.Sequential(nn.Linear(64, 48), nn.Linear(48, 8, device="meta"))
+    with pytest.raises(ValueError, match="^1: "):
+        quant.apply_microscaled(model)
+    assert not standin.made and type(model[0]) is nn.Linear

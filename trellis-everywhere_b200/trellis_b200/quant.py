@@ -159,6 +159,8 @@ def _check_replaceable(name: str, layer: nn.Linear) -> None:
     """Refuses a layer that is more than its weight and bias (backward hooks are left out: no gradient passes its replacement)."""
     if "weight" not in layer._parameters or "forward" in layer.__dict__ or any(getattr(layer, h) for h in _STATE_HOOKS):
         raise ValueError(f"{name}: its weight is computed, its forward is its own or hooks read its state: take that off first, or skip it")
+    if layer.weight.is_meta or (layer.bias is not None and layer.bias.is_meta):
+        raise ValueError(f"{name}: its weight or bias has no values yet (meta device)")
 
 
 @torch.no_grad()
