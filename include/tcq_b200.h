@@ -327,7 +327,8 @@ TCQ_API size_t tcq_ms_linear_workspace_bytes(int64_t m, int64_t n, int64_t k, in
 
 /*
  * y[i][r] = sum_c x[i][c] * W[r][c]: x [m][ldx] of type dtype (not quantised), W n x k in 4 bits, y [m][ldy] of type dtype.
- * Products and sums in fp32, rounded to dtype once; equal for equal inputs, run to run, and a row of y does not depend on
+ * Products exact, sums in fp32 (cut off by the tensor cores, not rounded, for 16-bit x of more than 8 rows), rounded to dtype once; finite wherever the sum of the
+ * products' magnitudes is (for mxfp4 block scales up to 2^104); equal for equal inputs, run to run, and a row of y does not depend on
  * what the other rows of x hold.  ws: tcq_ms_linear_workspace_bytes(...) bytes, 256-byte
  * aligned; not used (may be NULL) for up to 8 rows of x, and where x is bf16 (or fp16 and W nvfp4), 16-byte aligned and ldx a multiple of 8.  Columns of y behind n are left as they are.
  */
@@ -337,7 +338,7 @@ TCQ_API int tcq_ms_linear(const void *x, int dtype, int64_t m, int64_t ldx, cons
 
 /*
  * y[i][r] = sum_c X[i][c] * W[r][c] with both in 4 bits, of one format: X m x k, W n x k, y [m][ldy] of type dtype.
- * As tcq_ms_linear otherwise.
+ * As tcq_ms_linear otherwise; the sum over all of k is the tensor cores', which cut fp32 sums off where fp32 arithmetic rounds.
  */
 TCQ_API int tcq_ms_matmul(const uint8_t *x_codes, const uint8_t *x_scales, const float *x_row_scale, int64_t m,
                           const uint8_t *codes, const uint8_t *scales, const float *row_scale, int64_t n, int64_t k,

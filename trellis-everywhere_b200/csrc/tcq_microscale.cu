@@ -6,7 +6,7 @@
 // Every code is the nearest of the real quotient: divisors are powers of two times at most four bits, so that an fp32 quotient, correctly
 // rounded, is on a border between two codes (a number of at most four bits) only where the real one is.  (For x near t d, both on
 // grids no finer than ulp(x), |x / d - t| >= ulp(x) / d, which is more than half an ulp of t.)  The same holds for amax / 6 and e4m3.
-// A block with a NaN or an infinity gets the scale NaN and codes 0, and counts for nothing in the row's largest value.
+// A block with a NaN or an infinity gets the scale NaN and codes 0; its finite values count in the row's largest value.
 #include <algorithm>
 
 #include "tcq_common.cuh"
@@ -226,9 +226,9 @@ struct QuantizeArgs {
 };
 
 // `lanes` threads a row, RUNS runs of 16 columns each, blockDim / lanes rows a CTA at a time; a row is read once (the next one while this one is
-// worked on) and stays in registers.  Columns up to the next multiple of 256 are worked on as zeros, so that the storage behind column k is
+// worked on) and stays with its threads: in registers, but for 32 to 520 bytes a thread that spill at two runs (16385 to 32768 columns).  Columns up to the next multiple of 256 are worked on as zeros, so that the storage behind column k is
 // written.  The factors of a rotation are a thread's own for all its rows.  Bound by instruction issue (70 to 77 % of the slots), not by memory:
-// 12288 x 4096 bf16 25.9 us (mxfp4, 5.0 TB/s of x and codes), 38.5 (nvfp4, for its quotients); rotated by 128 44.7 and 60.5; fp32 35.4 and 43.9.
+// 12288 x 4096 bf16 25.9 us (mxfp4, 5.0 TB/s of x and codes), 39 (nvfp4, for its quotients); rotated by 128 46.4 and 60.9; fp32 35.8 and 44.5.
 template <typename T, int FMT, int RUNS, bool ROTATED>
 __global__ void __launch_bounds__(1024) tcq_ms_quantize_kernel(const T* __restrict__ x, const __grid_constant__ QuantizeArgs p) {
     constexpr int kPieces = sizeof(T);                   // of 16 bytes a run

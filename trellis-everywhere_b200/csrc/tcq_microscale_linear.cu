@@ -4,17 +4,19 @@
 // fp16 number.  mxfp4: scales can lie outside fp16, so the sums of 32 columns are scaled instead.  x is cut into fp16 parts, 256 columns of
 // a token at a time: a power of two brings the largest magnitude under 2^15, eleven bits are cut off as fp16, and what is left is the next
 // part's, until nothing is left.  fp16 and bf16 activations nearly always take one part (nothing is left of numbers within 2^-31 of the
-// largest), fp32 three (2^-37); more are further rounds over the same codes.  So every product is exact.  Sums of 32 columns (mxfp4) take the block's scale, sums
-// of 256 (nvfp4) the power of two in the row's scale, before x's factor: what is then added up is of the size of the results, whatever that of x and of W alone.
-// (Only a block scale above 2^104, of weights above 10^31, may take a sum out of range that x would bring back.)
-// (bf16 weights need no such care but three times the instructions a pair, which was the bound: 4 tokens through 151936 x 4096 136 us.)
+// largest), fp32 three (2^-37); more are further rounds over the same codes.  So every product is exact.  (bf16 weights need no such care but three
+// times the instructions a pair, which was the bound: 4 tokens through 151936 x 4096 136 us.)
+// Sums of 32 columns (mxfp4) take the block's scale, sums of 256 (nvfp4) the power of two in the row's scale, before x's factor: what is then added up is of the
+// size of the results, whatever that of x and of W alone.  (Only a block scale above 2^104, of weights above 10^31, may take a sum out of range that x would bring back.)
 //
 // Work split: a CTA takes 128 rows of W, eight warps 16 rows each; one more warp loads 256 columns of codes (TMA) and scales at a time into a ring
 // of stages.  ldmatrix gives lane (g, t) the t-th eight codes of 32 columns of rows g and g + 8, two products' share.  x is converted
 // once where all columns of a CTA fit beside the stages, else a token a warp, for the next stage while this one is multiplied.  Where there are few groups of 128 rows a
 // cluster of S CTAs shares the columns, and the partial sums meet through distributed shared memory, in rank order; of many groups, so are the last ones.
 //
-// Bound by instruction issue and its latencies (54 % of the slots): one token through 40960 x 4096 27.2 us (3.5 TB/s), mxfp4 23.3; eight 34.4 and 31.0.
+// Bound by latency (51 to 56 % of the issue slots, 18 warps an SM; nvfp4's products of a stage are one chain of sums): one token through 40960 x 4096 26.6 us
+// (3.5 TB/s), mxfp4 26.2; eight 36.8 and 32.5.  Three parts of x spill (184 bytes a thread, mxfp4 384, at the 96 registers that nine warps leave): seven fp32 tokens
+// through 4096 x 12288 23.6 us, mxfp4 26.7.
 //
 // A wait that runs out (kMbarWaitCycles) makes its CTA's results from there on NaN, and those of its cluster.
 #include <algorithm>

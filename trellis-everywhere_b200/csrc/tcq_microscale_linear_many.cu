@@ -11,7 +11,8 @@
 // one issues products, eight make weights (two groups of four take turns), four take finished sums out of tensor memory.  With few tokens a
 // cluster of S CTAs shares the columns of a tile; the partial sums meet through distributed shared memory, in rank order.
 //
-// Bound by the making of weights, beside the tensor cores (57 % busy): 1000 tokens through 12288 x 4096 82 us (1.22 PFLOP/s), mxfp4 83; fp16 76 and 88.
+// Bound by the making of weights, beside the tensor cores (57 % busy): 1000 tokens through 12288 x 4096 81 us (1.24 PFLOP/s), mxfp4 79; fp16 75 and 90 (mxfp4 as
+// called, with a scan of the scales and a form that ends at once, 105).  fp32 tokens, 21 to a tile at most: 40 through 4096 x 4096 19 us, 100 (mxfp4) 50.
 //
 // A wait that runs out (kMbarWaitCycles) makes its CTA stop, and its results from there on NaN, as those of its cluster.
 #include <algorithm>

@@ -8,7 +8,7 @@
 // scales and products, four take finished sums out of tensor memory (two buffers), scale them by the row scales, round and store.
 // W is read once; where there are fewer tiles than SMs, a cluster of S CTAs shares the columns of a tile, and the S partial sums meet
 // through distributed shared memory, in rank order.  Bound by the latency of one pass (few rows: one token,
-// 4096 x 4096 5.7 us) or by what W's bytes take (many: 40960 x 4096 16.4 us, 5.8 TB/s; mxfp4 14.5, 6.5 TB/s).
+// 4096 x 4096 5.4 us) or by what W's bytes take (many: 40960 x 4096 17.2 us, 5.5 TB/s; mxfp4 14.9, 6.3 TB/s).
 //
 // A wait that runs out (kMbarWaitCycles) makes its CTA stop, and its results from there on NaN, as those of its cluster.
 #include <algorithm>

@@ -11,7 +11,7 @@
 // NT = 256 there is one buffer of sums, at 128 two.
 //
 // Bound by power in long runs (1000 W: 1.5 to 1.7 GHz), then by the copies of scales to tensor memory, which nvfp4 has twice as many of: 8192 tokens
-// through 12288 x 4096 162 us (5.1 PFLOP/s), mxfp4 149 (5.5); 2048 tokens 46.4 and 42.2.
+// through 12288 x 4096 back to back 190 us (4.3 PFLOP/s); a dozen calls at full clocks 160 to 164 (5.1), mxfp4 146 to 150 (5.6); 2048 tokens 47.4 and 42.6.
 //
 // A wait that runs out (kMbarWaitCycles) makes its CTA stop, and its results from there on NaN.
 #include <algorithm>

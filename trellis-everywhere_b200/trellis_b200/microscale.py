@@ -216,8 +216,10 @@ def dequantize(q: Microscaled, dtype: torch.dtype = torch.float32) -> torch.Tens
 def linear(x: torch.Tensor, w: Microscaled) -> torch.Tensor:
     """``x @ W.T``: ``x [..., k]`` (fp32, fp16 or bf16) times a 4-bit ``[n, k]`` matrix -> ``[..., n]`` of x's type.
 
-    Products with the weights' exact values, summed in fp32, rounded once.  A row of the result does not depend on what
-    the other rows of x hold, and equal calls give equal results.
+    Products with the weights' exact values, summed in fp32, rounded once (16-bit results of more than eight rows are summed
+    by the tensor cores, which cut fp32 sums off instead of rounding them).  Finite wherever the sum of the products' magnitudes
+    is, whatever the size of x and of the weights (mxfp4 block scales up to 2^104).  A row of the result does not depend
+    on what the other rows of x hold, and equal calls give equal results.
     """
     dev = _check_q(w, "w")
     codes, scales, row, (n, k), fmt = w
@@ -243,7 +245,11 @@ def linear(x: torch.Tensor, w: Microscaled) -> torch.Tensor:
 
 
 def matmul(x: Microscaled, w: Microscaled, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """``X @ W.T`` of two 4-bit matrices ``[m, k]`` and ``[n, k]`` of one format -> ``[m, n]`` of ``dtype``, summed in fp32, rounded once."""
+    """``X @ W.T`` of two 4-bit matrices ``[m, k]`` and ``[n, k]`` of one format -> ``[m, n]`` of ``dtype``, rounded once.
+
+    The sum is the tensor cores': in fp32 over all of k, cut off where fp32 arithmetic rounds (exact for Gaussian matrices of up to
+    12288 columns, whose products have few bits; otherwise up to 2^-23 of the sum of magnitudes a term).
+    """
     dev, dt = _check_q(w, "w"), _check_dtype(dtype)
     codes, scales, row, (n, k), fmt = w
     if _check_q(x, "x") != dev or x.fmt != fmt or x.shape[1] != k:
