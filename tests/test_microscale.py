@@ -182,3 +182,11 @@ def test_scales_of_another_type_are_refused():
         for bad in (s.view(other), s.view(torch.float8_e5m2), s.bool()):
             with pytest.raises(ValueError, match="scales"):
                 ms.from_blocks(c, bad, row, 32, fmt)
+
+
+@pytest.mark.parametrize("fmt", ("mxfp4", "nvfp4"))
+def test_blocks_of_matrices_without_rows_or_columns(fmt):
+    for rows, k in ((0, 40), (3, 0), (0, 0)):
+        nb = -(-k // ms.BLOCKS[fmt])
+        q = ms.from_blocks(torch.zeros(rows, -(-k // 2), dtype=torch.uint8), torch.zeros(rows, nb, dtype=torch.uint8), None if fmt == "mxfp4" else 1.0, k, fmt)
+        assert ms.block_scales(q).shape == (rows, nb)

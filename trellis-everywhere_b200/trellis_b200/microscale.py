@@ -268,7 +268,7 @@ def matmul(x: Microscaled, w: Microscaled, dtype: torch.dtype = torch.bfloat16) 
 def block_scales(q: Microscaled) -> torch.Tensor:
     """The scale bytes by row and block, uint8 ``[rows, ceil(k / block)]`` (e4m3 for nvfp4, exponents + 127 for mxfp4)."""
     rows, k = q.shape
-    s = q.scales.permute(0, 3, 2, 1, 4).reshape(q.scales.shape[0] * 128, -1)
+    s = q.scales.permute(0, 3, 2, 1, 4).reshape(q.scales.shape[0] * 128, q.scales.shape[1] * 4)
     return s[:rows, :-(-k // BLOCKS[q.fmt])].contiguous()
 
 
