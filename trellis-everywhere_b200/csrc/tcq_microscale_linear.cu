@@ -98,7 +98,8 @@ __device__ __forceinline__ bool next_parts(float (&r)[8], uint32_t (&h)[PARTS][4
     for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(r[i]) & 0x7FFFFFFFu);
     most = __reduce_max_sync(0xFFFFFFFFu, most);
     bool left = false;
-    if (most >= 0x0C000000u && most < 0x7F800000u) {     // 2^-103 and more, and finite: all factors are normal numbers
+    // 2^-103 and more (2^-90 for three parts, the last of which takes 2^22 more), and finite: all factors are normal numbers
+    if (most >= uint32_t(PARTS == 1 ? 24 : 15 + 11 * (PARTS - 1)) << 23 && most < 0x7F800000u) {
         const int up = 141 - int(most >> 23);            // largest magnitude below 2^15
         if constexpr (PARTS == 1) {
             const float f = pow2f(up);
