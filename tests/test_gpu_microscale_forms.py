@@ -151,3 +151,33 @@ def test_the_tables_name_the_kernels_that_run(ms):
 def _zeros(ms, rows, k, f):
     q = torch.zeros(rows, -(-k // 2), dtype=torch.uint8, device="cuda")
     return ms.from_blocks(q, torch.zeros(rows, -(-k // BLOCK[NAMES[f]]), dtype=torch.uint8, device="cuda"), None if f == MX else 1.0, k, NAMES[f])
+
+
+@pytest.mark.parametrize("f", (MX, NV))
+@pytest.mark.parametrize("op,m,n,k", (("matmul", 300, 9728, 515), ("matmul", 2100, 12288, 300), ("matmul", 100, 20000, 515), ("matmul", 5, 76000, 300), ("matmul", 20, 1024, 2304),
+                                      ("linear", 300, 20000, 515), ("linear", 140, 6016, 330), ("linear", 50, 76000, 300), ("linear", 7, 76000, 300), ("linear", 40, 1024, 2304)))
+def test_rows_of_results_with_room_behind_them(ms, f, op, m, n, k):
+    """Results by the C entries, rows of any length and start: what lies behind column n and row m stays."""
+    from trellis_b200 import _lib
+    lib, stream, code = _lib.lib(), torch.cuda.current_stream().cuda_stream, {F32: 0, F16: 1, BF16: 2}
+    w, wv = whole_matrix(n, k, NAMES[f], n)
+    ptr = lambda t: None if t is None else t.data_ptr()
+    weights = (w.codes.data_ptr(), w.scales.data_ptr(), ptr(w.row_scale))
+    if op == "matmul":
+        x, xv = whole_matrix(m, k, NAMES[f], m)
+        want = xv @ wv.t()
+    for dtype in (F32, F16, BF16):
+        if op == "linear":
+            x = whole_tokens(m, k, dtype, m)
+            want = x.double() @ wv.t()
+            ws = torch.empty(lib.tcq_ms_linear_workspace_bytes(m, n, k, code[dtype], f), dtype=torch.uint8, device="cuda")
+        for ldy, start in ((n, 0), (n + 3, 1), (n + 8, 8), (n + 32, 0)):
+            flat = torch.full((start + (m + 2) * ldy,), 77.0, dtype=dtype, device="cuda")
+            y = flat[start:].view(m + 2, ldy)
+            if op == "matmul":
+                rc = lib.tcq_ms_matmul(x.codes.data_ptr(), x.scales.data_ptr(), ptr(x.row_scale), m, *weights, n, k, f, y.data_ptr(), code[dtype], ldy, stream)
+            else:
+                rc = lib.tcq_ms_linear(x.data_ptr(), code[dtype], m, k, *weights, n, k, f, y.data_ptr(), ldy, ws.data_ptr(), ws.numel(), stream)
+            assert rc == 0 and torch.equal(y[:m, :n], _exact(want, dtype)), (dtype, ldy, start)
+            y[:m, :n] = 77.0
+            assert (flat == 77).all()
