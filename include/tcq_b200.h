@@ -345,6 +345,65 @@ TCQ_API int tcq_ms_matmul(const uint8_t *x_codes, const uint8_t *x_scales, const
                           int format, void *y, int dtype, int64_t ldy, void *stream);
 
 /*
+ * Rows in groups times a 4-bit matrix each, with an epilogue (no counterpart in the reference): with h[i][r] = sum_c x[t(i)][c] * W[g(i)][r][c] + bias[g(i)][r],
+ *   y[i][r] = act(h[i][r]) + residual[i][r], and for the gated activations y[i][j] = act(h[i][2 j]) * h[i][2 j + 1] + residual[i][j], n / 2 columns.
+ *   x         [x_rows][ldx] of type dtype (TCQ_F16 or TCQ_BF16), k columns;  t(i) = tokens[i] (int32 [rows]; a row outside x gives NaN), or i where tokens is NULL (x_rows >= rows)
+ *   offsets   int32 [groups + 1] on the device: rows offsets[g] .. offsets[g + 1] - 1 are group g's; NULL: one group of all rows.  Rows of no group are left as they are.
+ *             Offsets that fall or leave 0 .. rows are taken as far as they do not.
+ *   codes, scales, row_scale   `groups` matrices n x k one behind the other, each as above: codes [groups][n][pitch], scales [groups][tcq_ms_scale_bytes(n, k, format)],
+ *             row_scale [groups][n]
+ *   bias      [groups][n] of type bias_dtype, or NULL;  residual [rows][ldr] of y's type, or NULL;  y [rows][ldy] of type y_dtype.  y may be the residual.
+ * Sums, bias, activation and residual in fp32, one rounding.  x is multiplied as sums of six 4-bit parts: exact down to 2^-10 (fp16: 2^-7) of the largest of each 16 (nvfp4)
+ * or 32 (mxfp4) columns, 2^-18 of that off at most elsewhere (nvfp4: or 2^-20 of the row's largest).  A row of x with a NaN or an infinity gives NaN.  At most 1024 groups and 2^30 rows;
+ * 1 <= k.  A row of y does not depend on the other rows' values; equal calls give equal results.
+ *   ws        tcq_ms_grouped_linear_workspace_bytes(...) bytes, 256-byte aligned
+ */
+#define TCQ_ACT_NONE 0
+#define TCQ_ACT_RELU 1
+#define TCQ_ACT_GELU 2          /* h (1 + erf(h / sqrt 2)) / 2 */
+#define TCQ_ACT_GELU_TANH 3     /* h (1 + tanh(sqrt(2 / pi) (h + 0.044715 h^3))) / 2 */
+#define TCQ_ACT_SILU 4          /* h / (1 + exp(-h)) */
+#define TCQ_ACT_GEGLU 5         /* gated by GELU */
+#define TCQ_ACT_SWIGLU 6        /* gated by SiLU */
+TCQ_API size_t tcq_ms_grouped_linear_workspace_bytes(int64_t rows, int64_t groups, int64_t n, int64_t k, int dtype, int format);
+TCQ_API int tcq_ms_grouped_linear(const void *x, int dtype, int64_t x_rows, int64_t ldx, const int32_t *tokens, const int32_t *offsets, int64_t groups,
+                                  int64_t rows, const uint8_t *codes, const uint8_t *scales, const float *row_scale, int64_t n, int64_t k, int format,
+                                  const void *bias, int bias_dtype, int activation, const void *residual, int64_t ldr, void *y, int y_dtype, int64_t ldy,
+                                  void *ws, size_t ws_bytes, void *stream);
+
+/* The epilogue by itself, of sums h [rows][n] in fp32 (one behind the other); the other arguments as above. */
+TCQ_API int tcq_ms_epilogue(const float *h, int64_t rows, int64_t n, const void *bias, int bias_dtype, int activation, const void *residual, int64_t ldr, void *y,
+                            int y_dtype, int64_t ldy, void *stream);
+
+/*
+ * Routing of tokens to experts.  Of each row of logits [tokens][ld] (type dtype) the `top` largest are chosen, one after the other; of equal ones the lower number; -infinity never
+ * (so a token may get fewer, or none), a NaN first.
+ *   weights [tokens][top] fp32: score 0: exp of the logit over the sum of all (normalize = 0) or of the chosen (1); score 1: sigmoid, normalize = 1: over the sum of the chosen
+ *   chosen  [tokens][top] int32, -1 where there is none (weight 0)
+ *   places  [tokens][top] int32: the row of each choice when all are in order of experts (of one expert in order of tokens), -1 where there is none
+ *   order   [tokens * top] int32: the token of each row; -1 behind the last;  offsets [experts + 1] int32: where each expert's rows begin, and where the last end
+ * 1 <= top <= 32, top <= experts <= 1024, tokens * top < 2^31.  ws: tcq_route_workspace_bytes(...) bytes, 4-byte aligned (0 for few tokens).
+ */
+#define TCQ_SCORE_SOFTMAX 0
+#define TCQ_SCORE_SIGMOID 1
+TCQ_API size_t tcq_route_workspace_bytes(int64_t tokens, int64_t experts);
+TCQ_API int tcq_route(const void *logits, int dtype, int64_t tokens, int64_t ld, int64_t experts, int64_t top, int score, int normalize, float *weights,
+                      int32_t *chosen, int32_t *places, int32_t *order, int32_t *offsets, void *ws, size_t ws_bytes, void *stream);
+
+/*
+ * out[t][c] = sum_j weights[t][j] * y[places[t][j]][c] + residual[t][c]: sums in fp32, j ascending, one rounding.  Places outside 0 .. rows - 1 add nothing.
+ * y [rows][ldy] of type dtype; out and residual (or NULL) [tokens][ldo], [tokens][ldr] of type out_dtype.  out may be the residual.
+ */
+TCQ_API int tcq_combine(const void *y, int dtype, int64_t rows, int64_t ldy, int64_t n, const float *weights, const int32_t *places, int64_t tokens, int64_t top,
+                        const void *residual, int64_t ldr, void *out, int out_dtype, int64_t ldo, void *stream);
+
+/* Self-test of the grouped products' bounded waits, as below. */
+TCQ_API int tcq_selftest_ms_grouped_waits(int64_t loads, const void *x, int dtype, int64_t x_rows, int64_t ldx, const int32_t *tokens, const int32_t *offsets,
+                                          int64_t groups, int64_t rows, const uint8_t *codes, const uint8_t *scales, const float *row_scale, int64_t n, int64_t k,
+                                          int format, const void *bias, int bias_dtype, int activation, const void *residual, int64_t ldr, void *y, int y_dtype,
+                                          int64_t ldy, void *ws, size_t ws_bytes, void *stream);
+
+/*
  * Self-tests of the products' bounded waits: the same calls, in which every CTA stops loading after `loads` pieces of 256 columns (0 <= loads < 2^32 - 1).  What
  * waits for more runs out after its time limit (about a quarter of a second), the kernel ends normally, and every result that needed more is NaN.
  * Nothing faults, traps or spins without limit.

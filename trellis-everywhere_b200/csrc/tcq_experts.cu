@@ -1,0 +1,377 @@
+// Mixtures of experts around the products: routing, and the sum of a token's results.
+//
+// Routing: a warp chooses a token's experts, a round of two warp reductions each: the largest logit (as an integer of the same order), then the lowest number that has it.
+// The rows are put in order of experts by counting: how many tokens before, by chunks of tokens, then by warps of a chunk, then within 32 neighbours; so
+// rows of one expert keep the order of their tokens, whatever runs first.  Up to kOneChunk tokens are one CTA's and one launch; more take two.
+//
+// The sum: a thread has eight neighbouring columns of one token, its rows' loads are in flight together.  Bound by memory.
+#include <algorithm>
+
+#include "tcq_experts.cuh"
+
+namespace tcq {
+
+namespace {
+
+constexpr int kOneChunk = 64;                    // tokens of the form that is one launch
+constexpr int kMostChunks = 256;
+constexpr int kWarps = 16, kThreads = 32 * kWarps;
+
+// Integers in the order of the numbers: -0 as 0, every NaN above infinity; 0 stands for -infinity, which is never chosen.
+__device__ __forceinline__ uint32_t ordered(float v) {
+    if (v != v) return 0xFFFFFFFFu;
+    const uint32_t b = __float_as_uint(v + 0.0f);
+    return v == -INFINITY ? 0u : b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float sum_of_warp(float v) {
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
+    return v;
+}
+
+// One token by one warp; lane l has logits l, l + 32 ...; EACH: of them.
+template <int EACH>
+__device__ void choose(const RouteCall& c, int token) {
+    const int lane = threadIdx.x & 31;
+    const long long row = token * c.ld;
+    uint32_t key[EACH];
+    float v[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        const int e = lane + 32 * i;
+        v[i] = e < c.experts ? load_as_f32(c.logits, c.dtype, row + e) : -INFINITY;
+        key[i] = ordered(v[i]);
+    }
+    float value = 0.0f;                                  // lane j: the j-th chosen
+    int expert = -1, found = 0;
+    for (int j = 0; j < c.top; ++j) {
+        uint32_t best = 0;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) best = max(best, key[i]);
+        best = __reduce_max_sync(0xFFFFFFFFu, best);
+        if (best == 0) break;                            // nothing is left
+        uint32_t at = 0xFFFFFFFFu;
+#pragma unroll
+        for (int i = EACH - 1; i >= 0; --i)
+            if (key[i] == best) at = lane + 32 * i;
+        at = __reduce_min_sync(0xFFFFFFFFu, at);
+        float mine = 0.0f;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i)
+            if (at == uint32_t(lane + 32 * i)) {
+                mine = v[i];
+                key[i] = 0;
+            }
+        mine = __shfl_sync(0xFFFFFFFFu, mine, at & 31);
+        if (lane == j) {
+            value = mine;
+            expert = int(at);
+        }
+        ++found;
+    }
+    float w;
+    if (c.score == kScoreSoftmax) {
+        const float most = __shfl_sync(0xFFFFFFFFu, value, 0);
+        w = lane < found ? expf(value - most) : 0.0f;
+        float sum = 0.0f;
+        if (c.normalize) {
+            sum = w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < EACH; ++i)
+                if (found > 0 && v[i] != -INFINITY) sum += expf(v[i] - most);
+        }
+        sum = sum_of_warp(sum);
+        w = lane < found ? w / sum : 0.0f;
+    } else {
+        // (far below zero a sigmoid is the exponential, and a quotient of two of them needs neither: nothing underflows)
+        const float most = __shfl_sync(0xFFFFFFFFu, value, 0);
+        w = lane >= found ? 0.0f : c.normalize && most < -30.0f ? expf(value - most) : 1.0f / (1.0f + expf(-value));
+        if (c.normalize) {
+            const float sum = sum_of_warp(w);
+            w = lane < found ? w / sum : 0.0f;
+        }
+    }
+    if (lane < c.top) {
+        c.weights[(long long)token * c.top + lane] = w;
+        c.chosen[(long long)token * c.top + lane] = expert;
+    }
+}
+__device__ __forceinline__ void choose_any(const RouteCall& c, int token) {
+    if (c.experts <= 64) choose<2>(c, token);
+    else if (c.experts <= 128) choose<4>(c, token);
+    else if (c.experts <= 256) choose<8>(c, token);
+    else choose<32>(c, token);
+}
+
+// The chunk's rows in order: `mine`, the chunk's first entry; offsets of experts and counts of the chunks before are in base[].
+// hist: [kWarps][experts] in shared memory.
+__device__ void place_chunk(const RouteCall& c, long long first, int entries, const int* base, int* hist) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int per = ((entries + kWarps - 1) / kWarps + 31) / 32 * 32, from = warp * per, to = min(entries, from + per);
+    for (int i = threadIdx.x; i < kWarps * c.experts; i += kThreads) hist[i] = 0;
+    __syncthreads();
+    for (int i = from + lane; i < to; i += 32) {
+        const int e = c.chosen[first + i];
+        if (e >= 0) atomicAdd(&hist[warp * c.experts + e], 1);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < c.experts; e += kThreads) {
+        int sum = base[e];
+        for (int w = 0; w < kWarps; ++w) {
+            const int mine = hist[w * c.experts + e];
+            hist[w * c.experts + e] = sum;
+            sum += mine;
+        }
+    }
+    __syncthreads();
+    for (int i = from; i < to; i += 32) {
+        const int e = i + lane < to ? c.chosen[first + i + lane] : -1;
+        const unsigned same = __match_any_sync(0xFFFFFFFFu, e);
+        int place = -1;
+        if (e >= 0) place = hist[warp * c.experts + e] + __popc(same & ((1u << lane) - 1));
+        __syncwarp();
+        if (e >= 0 && (same & ((1u << lane) - 1)) == 0) hist[warp * c.experts + e] += __popc(same);
+        __syncwarp();
+        if (i + lane < to) {
+            c.places[first + i + lane] = place;
+            if (place >= 0) c.order[place] = int((first + i + lane) / c.top);
+        }
+    }
+}
+
+// base[e] from counts in it to where experts begin, by one warp; the end of all.
+__device__ int scan_experts(int experts, int* base) {
+    const int lane = threadIdx.x & 31;
+    int sum = 0;
+    for (int at = 0; at < experts; at += 32) {
+        const int mine = at + lane < experts ? base[at + lane] : 0;
+        int v = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int other = __shfl_up_sync(0xFFFFFFFFu, v, d);
+            if (lane >= d) v += other;
+        }
+        if (at + lane < experts) base[at + lane] = sum + v - mine;
+        sum += __shfl_sync(0xFFFFFFFFu, v, 31);
+    }
+    return sum;
+}
+
+// All of few tokens.
+__global__ void __launch_bounds__(kThreads) tcq_route_kernel(const __grid_constant__ RouteCall c) {
+    extern __shared__ int hist[];
+    __shared__ int base[kMostExperts];
+    const int warp = threadIdx.x >> 5, entries = c.tokens * c.top;
+    for (int e = threadIdx.x; e < c.experts; e += kThreads) base[e] = 0;
+    for (int t = warp; t < c.tokens; t += kWarps) choose_any(c, t);
+    __syncthreads();
+    for (int i = threadIdx.x; i < entries; i += kThreads) {
+        const int e = c.chosen[i];
+        if (e >= 0) atomicAdd(&base[e], 1);
+    }
+    __syncthreads();
+    if (warp == 0) {
+        const int end = scan_experts(c.experts, base);
+        if (threadIdx.x == 0) c.offsets[c.experts] = end;
+        for (int i = end + int(threadIdx.x); i < entries; i += 32) c.order[i] = -1;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < c.experts; e += kThreads) c.offsets[e] = base[e];
+    place_chunk(c, 0, entries, base, hist);
+}
+
+// A chunk of many: its experts, and how many of each.
+__global__ void __launch_bounds__(kThreads) tcq_route_choose_kernel(const __grid_constant__ RouteCall c, int chunk) {
+    __shared__ int count[kMostExperts];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int warp = threadIdx.x >> 5, t0 = blockIdx.x * chunk, t1 = min(c.tokens, t0 + chunk);
+    for (int e = threadIdx.x; e < c.experts; e += kThreads) count[e] = 0;
+    for (int t = t0 + warp; t < t1; t += kWarps) choose_any(c, t);
+    __syncthreads();
+    for (int i = t0 * c.top + threadIdx.x; i < t1 * c.top; i += kThreads) {
+        const int e = c.chosen[i];
+        if (e >= 0) atomicAdd(&count[e], 1);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < c.experts; e += kThreads) c.counts[(long long)blockIdx.x * c.experts + e] = count[e];
+}
+
+// The chunk's rows in order, from the counts of all chunks.
+__global__ void __launch_bounds__(kThreads) tcq_route_place_kernel(const __grid_constant__ RouteCall c, int chunk) {
+    extern __shared__ int hist[];
+    __shared__ int base[kMostExperts], before[kMostExperts];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int warp = threadIdx.x >> 5;
+    for (int e = threadIdx.x; e < c.experts; e += kThreads) base[e] = before[e] = 0;
+    __syncthreads();
+    // neighbouring threads take neighbouring experts, groups of threads a share of the chunks each
+    const int wide = min(kThreads, (c.experts + 31) / 32 * 32), groups = kThreads / wide, group = threadIdx.x / wide;
+    for (int e = threadIdx.x % wide; e < c.experts && group < groups; e += wide) {
+        int all = 0, lower = 0;
+#pragma unroll 4
+        for (int q = group; q < int(gridDim.x); q += groups) {
+            const int n = c.counts[(long long)q * c.experts + e];
+            all += n;
+            if (q < int(blockIdx.x)) lower += n;
+        }
+        atomicAdd(&base[e], all);
+        atomicAdd(&before[e], lower);
+    }
+    __syncthreads();
+    if (warp == 0) {
+        const int end = scan_experts(c.experts, base);
+        if (blockIdx.x == 0) {
+            if (threadIdx.x == 0) c.offsets[c.experts] = end;
+            for (int e = threadIdx.x; e < c.experts; e += 32) c.offsets[e] = base[e];
+        }
+        // the rows that nobody has, a share each
+        for (long long i = end + (long long)blockIdx.x * 32 + threadIdx.x; i < (long long)c.tokens * c.top; i += 32ll * gridDim.x) c.order[i] = -1;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < c.experts; e += kThreads) base[e] += before[e];
+    __syncthreads();
+    const int t0 = blockIdx.x * chunk, t1 = min(c.tokens, t0 + chunk);
+    place_chunk(c, (long long)t0 * c.top, (t1 - t0) * c.top, base, hist);
+}
+
+// N neighbouring numbers, as one load where `wide`.
+template <typename T, int N>
+__device__ __forceinline__ void load_run(const T* p, bool wide, int there, float (&v)[N]) {
+    if (wide) {
+        constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+        for (int q = 0; q < N / kPer; ++q) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4*>(p) + q);
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) v[q * kPer + i] = to_f32<T>(reinterpret_cast<const T*>(&u)[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = i < there ? to_f32<T>(p[i]) : 0.0f;
+    }
+}
+
+// Y: of the rows, O: of what comes out.  RUN = 8: a thread eight neighbours in pieces of 16 bytes; 1: a thread one column, a warp 32 neighbours.
+template <typename Y, typename O, int RUN>
+__global__ void __launch_bounds__(256) tcq_combine_kernel(const __grid_constant__ CombineCall c, unsigned runs) {
+    const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long token = id / runs, c0 = (id - token * runs) * RUN;
+    if (token >= c.tokens) return;
+    float sum[RUN] = {};
+    const bool wide = RUN == 8;
+    if (c.residual != nullptr) load_run<O, RUN>(static_cast<const O*>(c.residual) + token * c.ldr + c0, wide, RUN, sum);
+    float out[RUN] = {};
+    for (int j0 = 0; j0 < c.top; j0 += 4) {
+        float v[4][RUN], w[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int j = j0 + q;
+            const int place = j < c.top ? __ldg(c.places + token * c.top + j) : -1;
+            w[q] = 0.0f;
+            if (place >= 0 && place < c.rows) {
+                w[q] = __ldg(c.weights + token * c.top + j);
+                load_run<Y, RUN>(static_cast<const Y*>(c.y) + place * c.ldy + c0, wide, RUN, v[q]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < RUN; ++i) v[q][i] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int i = 0; i < RUN; ++i) out[i] = __fmaf_rn(v[q][i], w[q], out[i]);
+    }
+    O* const to = static_cast<O*>(c.out) + token * c.ldo + c0;
+    if constexpr (RUN == 8) {
+        alignas(16) O r[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] = from_f32<O>(out[i] + sum[i]);
+#pragma unroll
+        for (int q = 0; q < int(sizeof(O) / 2); ++q) reinterpret_cast<uint4*>(to)[q] = reinterpret_cast<const uint4*>(r)[q];
+    } else {
+        *to = from_f32<O>(out[0] + sum[0]);
+    }
+}
+
+template <typename Y, typename O>
+cudaError_t combine(const CombineCall& c, cudaStream_t stream) {
+    const auto rows_of_16 = [](const void* p, long long ld, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * bytes % 16 == 0; };
+    const bool wide = c.n % 8 == 0 && rows_of_16(c.y, c.ldy, sizeof(Y)) && rows_of_16(c.out, c.ldo, sizeof(O)) &&
+                      (c.residual == nullptr || rows_of_16(c.residual, c.ldr, sizeof(O)));
+    const long long runs = wide ? c.n / 8 : c.n, blocks = (c.tokens * runs + 255) / 256;
+    if (blocks > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
+    if (wide) tcq_combine_kernel<Y, O, 8><<<unsigned(blocks), 256, 0, stream>>>(c, unsigned(runs));
+    else tcq_combine_kernel<Y, O, 1><<<unsigned(blocks), 256, 0, stream>>>(c, unsigned(runs));
+    return cudaGetLastError();
+}
+template <typename Y>
+cudaError_t combine_to(const CombineCall& c, cudaStream_t stream) {
+    if (c.out_dtype == kF32) return combine<Y, float>(c, stream);
+    return c.out_dtype == kF16 ? combine<Y, __half>(c, stream) : combine<Y, __nv_bfloat16>(c, stream);
+}
+
+__global__ void __launch_bounds__(256) tcq_epilogue_kernel(const float* h, long long rows, long long n, const __grid_constant__ Epilogue e) {
+    const long long fours = (n + 3) / 4, id = (long long)blockIdx.x * 256 + threadIdx.x, row = id / fours, r = (id - row * fours) * 4;
+    if (row >= rows) return;
+    float v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        v[j] = r + j < n ? h[row * n + r + j] : 0.0f;
+        if (e.bias != nullptr && r + j < n) v[j] += load_as_f32(e.bias, e.bias_dtype, r + j);
+    }
+    finish_four(e, v, row, r, n);
+}
+
+}  // namespace
+
+int route_chunks(int tokens) {
+    if (tokens <= kOneChunk) return 1;
+    const int chunk = std::max(32, (tokens + kMostChunks - 1) / kMostChunks);
+    return (tokens + chunk - 1) / chunk;
+}
+
+cudaError_t launch_route(const RouteCall& c, cudaStream_t stream) {
+    const int chunks = route_chunks(c.tokens), smem = kWarps * c.experts * int(sizeof(int));
+    static std::atomic<bool> ready[64];
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
+    if (err != cudaSuccess) return err;
+    if (dev >= 64 || !ready[dev]) {
+        for (const void* kernel : {reinterpret_cast<const void*>(tcq_route_kernel), reinterpret_cast<const void*>(tcq_route_place_kernel)})
+            if ((err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kWarps * kMostExperts * int(sizeof(int)))) != cudaSuccess) return err;
+        if (dev < 64) ready[dev] = true;
+    }
+    if (chunks == 1) {
+        tcq_route_kernel<<<1, kThreads, smem, stream>>>(c);
+        return cudaGetLastError();
+    }
+    const int chunk = std::max(32, (c.tokens + kMostChunks - 1) / kMostChunks);
+    tcq_route_choose_kernel<<<unsigned(chunks), kThreads, 0, stream>>>(c, chunk);
+    if ((err = cudaGetLastError()) != cudaSuccess) return err;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(chunks));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = size_t(smem);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, tcq_route_place_kernel, c, chunk);
+}
+
+cudaError_t launch_combine(const CombineCall& c, cudaStream_t stream) {
+    if (c.dtype == kF32) return combine_to<float>(c, stream);
+    return c.dtype == kF16 ? combine_to<__half>(c, stream) : combine_to<__nv_bfloat16>(c, stream);
+}
+
+cudaError_t launch_epilogue(const float* h, long long rows, long long n, const Epilogue& e, cudaStream_t stream) {
+    const long long blocks = (rows * ((n + 3) / 4) + 255) / 256;
+    if (blocks > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
+    tcq_epilogue_kernel<<<unsigned(blocks), 256, 0, stream>>>(h, rows, n, e);
+    return cudaGetLastError();
+}
+
+}  // namespace tcq

@@ -13,7 +13,7 @@ import subprocess
 _CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "csrc")
 LIB_PATH = os.path.join(_CSRC, "libtcq_b200.so")
 
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 # name -> (restype, argtypes); mirrors include/tcq_b200.h one to one
 _vp, _i64, _int, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t
@@ -51,6 +51,15 @@ SIGNATURES = {
     "tcq_ms_matmul": (_int, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _int, _vp, _int, _i64, _vp]),
     "tcq_selftest_ms_linear_waits": (_int, [_i64, _vp, _int, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _int, _vp, _i64, _vp, _sz, _vp]),
     "tcq_selftest_ms_matmul_waits": (_int, [_i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _int, _vp, _int, _i64, _vp]),
+    "tcq_ms_grouped_linear_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _int, _int]),
+    "tcq_ms_grouped_linear": (_int, [_vp, _int, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _int, _vp, _int, _int, _vp, _i64, _vp, _int, _i64,
+                                     _vp, _sz, _vp]),
+    "tcq_ms_epilogue": (_int, [_vp, _i64, _i64, _vp, _int, _int, _vp, _i64, _vp, _int, _i64, _vp]),
+    "tcq_route_workspace_bytes": (_sz, [_i64, _i64]),
+    "tcq_route": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _int, _int, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "tcq_combine": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _int, _i64, _vp]),
+    "tcq_selftest_ms_grouped_waits": (_int, [_i64, _vp, _int, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _int, _vp, _int, _int, _vp, _i64, _vp, _int,
+                                             _i64, _vp, _sz, _vp]),
 }
 
 _lib = None

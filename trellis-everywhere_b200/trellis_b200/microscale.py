@@ -6,7 +6,7 @@ prompts and activations:
 
     quantize(x, fmt)        a matrix -> ``Microscaled`` (codes, block scales, row scales); optionally rotated first
     dequantize(q, dtype)    its values
-    linear(x, w)            ``x @ W.T``, x in 16 or 32 bits (weight-only)
+    linear(x, w)            ``x @ W.T``, x in 16 or 32 bits (weight-only); with bias, activation and residual in the same call
     matmul(x, w)            ``X @ W.T``, both in 4 bits
 
 Every value is ``e2m1(code) * block scale``, e2m1 one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign:
@@ -38,6 +38,8 @@ FORMATS = {"mxfp4": 0, "nvfp4": 1}
 BLOCKS = {"mxfp4": 32, "nvfp4": 16}
 ROTATIONS = (0, 16, 32, 64, 128)
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4, "geglu": 5, "swiglu": 6}
+GATED = ("geglu", "swiglu")
 
 
 class Microscaled(NamedTuple):
@@ -213,14 +215,22 @@ def dequantize(q: Microscaled, dtype: torch.dtype = torch.float32) -> torch.Tens
     return out
 
 
-def linear(x: torch.Tensor, w: Microscaled) -> torch.Tensor:
-    """``x @ W.T``: ``x [..., k]`` (fp32, fp16 or bf16) times a 4-bit ``[n, k]`` matrix -> ``[..., n]`` of x's type.
+def linear(x: torch.Tensor, w: Microscaled, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
+           residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``act(x @ W.T + bias) + residual``: ``x [..., k]`` (fp32, fp16 or bf16) times a 4-bit ``[n, k]`` matrix -> ``[..., n]`` of x's type.
 
-    Products with the weights' exact values, summed in fp32, rounded once (16-bit results of more than eight rows are summed
+    Without an epilogue: products with the weights' exact values, summed in fp32, rounded once (16-bit results of more than eight rows are summed
     by the tensor cores, which cut fp32 sums off instead of rounding them).  Finite wherever the sum of the products' magnitudes
     is, whatever the size of x and of the weights (mxfp4 block scales up to 2^104).  A row of the result does not depend
     on what the other rows of x hold, and equal calls give equal results.
+
+    ``bias [n]`` (fp32, fp16 or bf16), ``activation`` and ``residual [..., n]`` of x's type are applied to the fp32 sums, before the one rounding.
+    ``activation``: "relu", "gelu" (with erf), "gelu_tanh", "silu", or gated, "geglu" or "swiglu": rows 2 j and 2 j + 1 of W are the gate and
+    the value of result j (``interleave``), ``act(h[2 j]) * h[2 j + 1]``, and n / 2 results come out.  Products of 16-bit x with an epilogue are those of
+    ``experts.grouped_linear`` (x exact down to 2^-10 of a block's largest magnitude in bf16, 2^-7 in fp16; an infinity in x gives NaN).
     """
+    if bias is not None or activation is not None or residual is not None:
+        return _linear_epilogue(x, w, bias, activation, residual)
     dev = _check_q(w, "w")
     codes, scales, row, (n, k), fmt = w
     shape = x.shape
@@ -242,6 +252,71 @@ def linear(x: torch.Tensor, w: Microscaled) -> torch.Tensor:
     elif not k:
         y.zero_()
     return y if len(shape) == 2 else y.view(*shape[:-1], n)
+
+
+def _check_act(activation: Optional[str], n: int) -> Tuple[int, int]:
+    """The activation's number, and how many results come of n sums."""
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"unknown activation {activation!r}; expected one of {sorted(a for a in ACTIVATIONS if a)} or None")
+    if activation not in GATED:
+        return ACTIVATIONS[activation], n
+    if n % 2:
+        raise ValueError(f"{activation} takes rows of W in pairs of gate and value: {n} is odd")
+    return ACTIVATIONS[activation], n // 2
+
+
+def _check_bias(bias: Optional[torch.Tensor], shape: Tuple[int, ...], device) -> Optional[torch.Tensor]:
+    if bias is None:
+        return None
+    if bias.shape != shape or bias.dtype not in _DTYPES or bias.device != device:
+        raise ValueError(f"bias must be a float32, float16 or bfloat16 {list(shape)} tensor on {device}")
+    _no_gradient(bias, "bias")
+    return bias if bias.is_contiguous() else bias.detach().contiguous()
+
+
+def _grouped(dev: int, flat: torch.Tensor, tokens, offsets, groups: int, rows: int, codes, scales, row, n: int, k: int, fmt: str, bias, act: int, residual, y: torch.Tensor) -> None:
+    """``tcq_ms_grouped_linear`` with its workspace, given back when the call is queued: the stream's later work comes after it."""
+    dt, f = _DTYPES[flat.dtype], FORMATS[fmt]
+    size = _lib.lib().tcq_ms_grouped_linear_workspace_bytes(rows, groups, n, k, dt, f)
+    ws = torch.empty(size, dtype=torch.uint8, device=flat.device)
+    _launch(dev, "tcq_ms_grouped_linear", flat.data_ptr(), dt, flat.shape[0], _pitch(flat), _ptr(tokens), _ptr(offsets), groups, rows, codes.data_ptr(), scales.data_ptr(),
+            _ptr(row), n, k, f, _ptr(bias), 0 if bias is None else _DTYPES[bias.dtype], act, _ptr(residual), 0 if residual is None else _pitch(residual),
+            y.data_ptr(), _DTYPES[y.dtype], y.shape[1], ws.data_ptr(), size)
+
+
+def _linear_epilogue(x: torch.Tensor, w: Microscaled, bias, activation, residual) -> torch.Tensor:
+    dev = _check_q(w, "w")
+    codes, scales, row, (n, k), fmt = w
+    shape = x.shape
+    act, out = _check_act(activation, n)
+    if not shape or shape[-1] != k:
+        raise ValueError(f"x must be [..., {k}], got {tuple(shape)}")
+    if x.get_device() != dev:
+        raise ValueError(f"x must be on {codes.device}")
+    m = math.prod(shape[:-1])
+    flat = _check_x(x if len(shape) == 2 else x.reshape(m, k), "x")
+    bias = _check_bias(bias, (n,), codes.device)
+    if residual is not None:
+        if residual.shape != (*shape[:-1], out) or residual.dtype != flat.dtype or residual.get_device() != dev:
+            raise ValueError(f"residual must be a {flat.dtype} {[*shape[:-1], out]} tensor on {codes.device}")
+        residual = _check_x(residual if len(shape) == 2 else residual.reshape(m, out), "residual")
+    if m and n and k and flat.dtype is not torch.float32:
+        y = torch.empty_strided((m, out), (out, 1), dtype=flat.dtype, device=flat.device)
+        _grouped(dev, flat, None, None, 1, m, codes, scales, row, n, k, fmt, bias, act, residual, y)
+    else:                                                    # fp32 sums as they are, then the epilogue by itself
+        h = linear(flat.float() if not k else flat, w)
+        y = h if out == n and h.dtype is flat.dtype else torch.empty_strided((m, out), (out, 1), dtype=flat.dtype, device=flat.device)
+        if m and n:
+            _launch(dev, "tcq_ms_epilogue", h.data_ptr(), m, n, _ptr(bias), 0 if bias is None else _DTYPES[bias.dtype], act,
+                    _ptr(residual), 0 if residual is None else _pitch(residual), y.data_ptr(), _DTYPES[y.dtype], out)
+    return y if len(shape) == 2 else y.view(*shape[:-1], out)
+
+
+def interleave(gate: torch.Tensor, value: torch.Tensor) -> torch.Tensor:
+    """``[..., 2 n, k]`` from two ``[..., n, k]``: rows in turn, as the gated activations take them (a bias ``[..., n]``: with ``k`` = 1 columns added and taken off)."""
+    if gate.shape != value.shape or gate.dim() < 2:
+        raise ValueError(f"gate and value must be matrices of one shape, got {tuple(gate.shape)} and {tuple(value.shape)}")
+    return torch.stack((gate, value), dim=-2).flatten(-3, -2)
 
 
 def matmul(x: Microscaled, w: Microscaled, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
