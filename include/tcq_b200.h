@@ -354,9 +354,9 @@ TCQ_API int tcq_ms_matmul(const uint8_t *x_codes, const uint8_t *x_scales, const
  *             row_scale [groups][n]
  *   bias      [groups][n] of type bias_dtype, or NULL;  residual [rows][ldr] of y's type, or NULL;  y [rows][ldy] of type y_dtype.  y may be the residual.
  * Sums, bias, activation and residual in fp32, one rounding.  x is multiplied as sums of six 4-bit parts: exact down to 2^-10 (fp16: 2^-7) of the largest of each 16 (nvfp4)
- * or 32 (mxfp4) columns, 2^-18 of that off at most elsewhere (nvfp4: or 2^-20 of the row's largest).  A row of x with a NaN or an infinity gives NaN.  At most 1024 groups and 2^30 rows;
+ * or 32 (mxfp4) columns, 2^-18 of that off at most elsewhere (nvfp4: or 2^-20 of the row's largest).  A row of x with a NaN gives NaN, one with an infinity NaN or what its sums have.  At most 1024 groups and 2^30 rows;
  * 1 <= k.  A row of y does not depend on the other rows' values; equal calls give equal results.
- *   ws        tcq_ms_grouped_linear_workspace_bytes(...) bytes, 256-byte aligned
+ *   ws        tcq_ms_grouped_linear_workspace_bytes(...) bytes, 256-byte aligned (may be 0); in_order: tokens is NULL, x 16-byte aligned and ldx a multiple of 8
  */
 #define TCQ_ACT_NONE 0
 #define TCQ_ACT_RELU 1
@@ -365,7 +365,7 @@ TCQ_API int tcq_ms_matmul(const uint8_t *x_codes, const uint8_t *x_scales, const
 #define TCQ_ACT_SILU 4          /* h / (1 + exp(-h)) */
 #define TCQ_ACT_GEGLU 5         /* gated by GELU */
 #define TCQ_ACT_SWIGLU 6        /* gated by SiLU */
-TCQ_API size_t tcq_ms_grouped_linear_workspace_bytes(int64_t rows, int64_t groups, int64_t n, int64_t k, int dtype, int format);
+TCQ_API size_t tcq_ms_grouped_linear_workspace_bytes(int64_t rows, int64_t groups, int64_t n, int64_t k, int dtype, int format, int in_order);
 TCQ_API int tcq_ms_grouped_linear(const void *x, int dtype, int64_t x_rows, int64_t ldx, const int32_t *tokens, const int32_t *offsets, int64_t groups,
                                   int64_t rows, const uint8_t *codes, const uint8_t *scales, const float *row_scale, int64_t n, int64_t k, int format,
                                   const void *bias, int bias_dtype, int activation, const void *residual, int64_t ldr, void *y, int y_dtype, int64_t ldy,

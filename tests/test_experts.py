@@ -113,8 +113,8 @@ def test_grouped_calls_of_nothing():
     L = _lib.lib()
     assert L.tcq_ms_grouped_linear(*{**GROUPED, "rows": 0}.values()) == 0 and L.tcq_ms_grouped_linear(*{**GROUPED, "n": 0}.values()) == 0
     assert L.tcq_selftest_ms_grouped_waits(-1, *GROUPED.values()) == BAD_COUNT
-    assert L.tcq_ms_grouped_linear_workspace_bytes(0, 3, 8, 64, 2, 1) == 0 and L.tcq_ms_grouped_linear_workspace_bytes(10, 3, 8, 64, 0, 1) == 0
-    assert L.tcq_ms_grouped_linear_workspace_bytes(10, 3, 8, 64, 2, 1) > 0
+    assert L.tcq_ms_grouped_linear_workspace_bytes(0, 3, 8, 64, 2, 1, 1) == 0 and L.tcq_ms_grouped_linear_workspace_bytes(10, 3, 8, 64, 0, 1, 1) == 0
+    assert L.tcq_ms_grouped_linear_workspace_bytes(10, 3, 8, 64, 2, 1, 1) > 0
 
 
 EPILOGUE = dict(h=at(), rows=4, n=8, bias=at(), bias_dtype=0, activation=5, residual=at(), ldr=4, y=at(), y_dtype=0, ldy=4, stream=None)

@@ -274,8 +274,8 @@ def test_waits_that_run_out(rows, counts, fmt):
     want = experts.grouped_linear(x, w, offsets)
     L = _lib.lib()
     f = 0 if fmt == "mxfp4" else 1
-    size = L.tcq_ms_grouped_linear_workspace_bytes(rows, len(counts), n, k, 2, f)
-    ws = torch.empty(size, dtype=torch.uint8, device=DEV)
+    size = L.tcq_ms_grouped_linear_workspace_bytes(rows, len(counts), n, k, 2, f, 1)
+    ws = torch.empty(max(size, 1), dtype=torch.uint8, device=DEV)
     for loads in (0, 1, 3):                                       # of eight stages, which four CTAs share at most: one load is too few for any of them
         y = torch.zeros(rows, n, dtype=torch.bfloat16, device=DEV)
         rc = L.tcq_selftest_ms_grouped_waits(loads, x.data_ptr(), 2, rows, k, None, offsets.data_ptr(), len(counts), rows, w.codes.data_ptr(), w.scales.data_ptr(),

@@ -112,6 +112,21 @@ def test_not_finite_rows(m, fmt):
 
 
 @pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+def test_not_finite_rows_of_many(fmt):
+    """The same among many tokens, where an infinity may also give what its sums have."""
+    from trellis_b200 import microscale as ms
+    x, w, b, _ = case(300, 200, 300, fmt, torch.bfloat16, None, torch.float32, False)
+    want = ms.linear(x, w, b)
+    y = x.clone()
+    y[1, 37], y[40, 299], y[299, 0] = float("nan"), float("inf"), -float("inf")
+    got = ms.linear(y, w, b)
+    exact = y[[40, 299]].double() @ ms.dequantize(w).double().t() + b.double()
+    assert bool(got[1].isnan().all()) and bool((got[[40, 299]].isnan() | (got[[40, 299]] == exact)).all())
+    keep = [i for i in range(300) if i not in (1, 40, 299)]
+    assert torch.equal(got[keep], want[keep])
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
 @pytest.mark.parametrize("power", [-100, -30, 30, 100])
 def test_size_of_activations(power, fmt):
     """A power of two in x is one in the results, exactly."""

@@ -43,10 +43,12 @@ int grouped_core(const void* x, int dtype, int64_t x_rows, int64_t ldx, const in
     if (rows == 0 || n == 0) return TCQ_OK;
     if (k == 0 || ldx < k || x_rows >= int64_t(1) << 31 || (tokens == nullptr && x_rows < rows)) return TCQ_E_BAD_ARGUMENT;
     if ((rc = check_epilogue(n, bias, bias_dtype, activation, residual, ldr, y, y_dtype, ldy)) != TCQ_OK) return rc;
-    if ((x == nullptr && x_rows > 0) || codes == nullptr || scales == nullptr || (format == TCQ_MS_NVFP4) != (row_scale != nullptr) || ws == nullptr) return TCQ_E_NULL_POINTER;
+    if ((x == nullptr && x_rows > 0) || codes == nullptr || scales == nullptr || (format == TCQ_MS_NVFP4) != (row_scale != nullptr)) return TCQ_E_NULL_POINTER;
     if (misaligned(x, 2) || misaligned(codes, 16) || misaligned(scales, 16) || misaligned(row_scale, 4) || misaligned(tokens, 4) || misaligned(offsets, 4) || misaligned(ws, 256))
         return TCQ_E_MISALIGNED;
-    if (ws_bytes < ms_grouped_workspace_bytes(rows, groups, n, k, dtype, format)) return TCQ_E_WORKSPACE;
+    const size_t need = ms_grouped_workspace_bytes(rows, groups, n, k, dtype, format, tokens == nullptr && ms_rows_aligned(x, ldx));
+    if (need && ws == nullptr) return TCQ_E_NULL_POINTER;
+    if (ws_bytes < need) return TCQ_E_WORKSPACE;
     const GroupedCall c{x, dtype, x_rows, ldx, tokens, {offsets, int(groups), int(rows)}, {codes, scales, row_scale, n}, k, format,
                         {bias, bias_dtype, activation, residual, ldr, y, y_dtype, ldy}, loads};
     const cudaError_t err = launch_ms_grouped(c, ws, static_cast<cudaStream_t>(stream));
@@ -57,9 +59,9 @@ int grouped_core(const void* x, int dtype, int64_t x_rows, int64_t ldx, const in
 
 extern "C" {
 
-size_t tcq_ms_grouped_linear_workspace_bytes(int64_t rows, int64_t groups, int64_t n, int64_t k, int dtype, int format) {
+size_t tcq_ms_grouped_linear_workspace_bytes(int64_t rows, int64_t groups, int64_t n, int64_t k, int dtype, int format, int in_order) {
     if (check_grouped(rows, groups, n, k, dtype, format) != TCQ_OK || rows == 0) return 0;
-    return ms_grouped_workspace_bytes(rows, groups, n, k, dtype, format);
+    return ms_grouped_workspace_bytes(rows, groups, n, k, dtype, format, in_order != 0);
 }
 
 int tcq_ms_grouped_linear(const void* x, int dtype, int64_t x_rows, int64_t ldx, const int32_t* tokens, const int32_t* offsets, int64_t groups, int64_t rows,

@@ -21,16 +21,24 @@ struct Epilogue {
 
 __host__ __device__ constexpr bool act_gated(int act) { return act >= kActGeglu; }
 
-// A call, so that what erf and tanh take of registers and instructions is there once, beside loops that need theirs.
-static __device__ __noinline__ float activate(int act, float h) {
-    if (act == kActRelu) return h < 0.0f ? 0.0f : h;                              // (NaN stays)
-    if (act == kActGelu || act == kActGeglu) return 0.5f * h * (1.0f + erff(h * 0.70710678118654752f));
-    if (act == kActGeluTanh) {
-        const float t = tanhf(0.79788456080286536f * (h + 0.044715f * h * h * h));
-        return 0.5f * h * (1.0f + t);
+// N activations at once: one branch for all of them.  The fast exponential and quotient are within a few ulp where results are rounded to 16 bits or follow an fp32 sum
+// that is further off; -h far above 88 gives 1 / infinity, the limit.
+__device__ __forceinline__ float sigmoid(float h) { return __fdividef(1.0f, 1.0f + __expf(-h)); }
+template <int N>
+__device__ __forceinline__ void activate(int act, float (&h)[N]) {
+    if (act == kActRelu) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) h[i] = h[i] < 0.0f ? 0.0f : h[i];             // (NaN stays)
+    } else if (act == kActSilu || act == kActSwiglu) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) h[i] *= sigmoid(h[i]);
+    } else if (act == kActGeluTanh) {                                             // (1 + tanh z) / 2 = sigmoid(2 z)
+#pragma unroll
+        for (int i = 0; i < N; ++i) h[i] *= sigmoid(1.5957691216057308f * __fmaf_rn(0.044715f * h[i] * h[i], h[i], h[i]));
+    } else if (act == kActGelu || act == kActGeglu) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) h[i] *= 0.5f + 0.5f * erff(h[i] * 0.70710678118654752f);
     }
-    if (act == kActSilu || act == kActSwiglu) return h / (1.0f + expf(-h));
-    return h;
 }
 
 __device__ __forceinline__ float load_as_f32(const void* p, int dtype, long long at) {
@@ -38,55 +46,75 @@ __device__ __forceinline__ float load_as_f32(const void* p, int dtype, long long
     if (dtype == kF16) return __half2float(__ldg(static_cast<const __half*>(p) + at));
     return __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p) + at));
 }
-__device__ __forceinline__ void store_f32(void* p, int dtype, long long at, float v) {
-    if (dtype == kF32) static_cast<float*>(p)[at] = v;
-    else if (dtype == kF16) static_cast<__half*>(p)[at] = __float2half_rn(v);
-    else static_cast<__nv_bfloat16*>(p)[at] = __float2bfloat16_rn(v);
-}
-
-// One result: residual and rounding.  (y may be the residual: read and written by the same thread.)
-__device__ __forceinline__ void finish_one(const Epilogue& e, long long row, long long column, float v) {
-    if (e.residual != nullptr) {
-        const long long at = row * e.ldr + column;
-        if (e.dtype == kF32) v += static_cast<const float*>(e.residual)[at];
-        else if (e.dtype == kF16) v += __half2float(static_cast<const __half*>(e.residual)[at]);
-        else v += __bfloat162float(static_cast<const __nv_bfloat16*>(e.residual)[at]);
+// N results of one column, in rows row, row + step ...: residual, rounding, stores.  (y may be the residual: read and written by the same thread.)
+template <typename YT, int N>
+__device__ __forceinline__ void store_rows_as(const Epilogue& e, const float (&v)[N], long long row, int step, int rows, long long column) {
+    YT* to = static_cast<YT*>(e.y) + row * e.ldy + column;
+    if (e.residual == nullptr) {
+#pragma unroll
+        for (int i = 0; i < N; ++i, to += step * e.ldy)
+            if (i < rows) *to = from_f32<YT>(v[i]);
+    } else {
+        const YT* from = static_cast<const YT*>(e.residual) + row * e.ldr + column;
+        YT r[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i, from += step * e.ldr)
+            if (i < rows) r[i] = *from;
+#pragma unroll
+        for (int i = 0; i < N; ++i, to += step * e.ldy)
+            if (i < rows) *to = from_f32<YT>(v[i] + to_f32<YT>(r[i]));
     }
-    store_f32(e.y, e.dtype, row * e.ldy + column, v);
+}
+template <int N>
+__device__ __forceinline__ void store_rows(const Epilogue& e, const float (&v)[N], long long row, int step, int rows, long long column) {
+    if (e.dtype == kBf16) store_rows_as<__nv_bfloat16>(e, v, row, step, rows, column);
+    else if (e.dtype == kF16) store_rows_as<__half>(e, v, row, step, rows, column);
+    else store_rows_as<float>(e, v, row, step, rows, column);
 }
 
 // N rows of results of column r of h, one column a lane (lanes are 32 neighbours, lane 0 an even one); the whole warp.  h: sums with the bias in; there: whether
 // column r exists; rows row0 .. row0 + rows - 1 do.
 // Gated: neighbours hold gate and value of the same result, so the even lane takes every other row and the odd lane those between.
 template <int N>
-__device__ __forceinline__ void finish_rows(const Epilogue& e, const float (&h)[N], long long row0, int rows, long long r, bool there) {
+__device__ __forceinline__ void finish_rows(const Epilogue& e, float (&h)[N], long long row0, int rows, long long r, bool there) {
     if (!act_gated(e.act)) {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (there && i < rows) finish_one(e, row0 + i, r, e.act == kActNone ? h[i] : activate(e.act, h[i]));
+        activate(e.act, h);
+        store_rows(e, h, row0, 1, there ? rows : 0, r);
     } else {
+        constexpr int kPairs = (N + 1) / 2;
         const bool odd = r & 1;
+        float gate[kPairs], value[kPairs];
 #pragma unroll
         for (int i = 0; i < N; i += 2) {
             const float second = i + 1 < N ? h[i + 1 < N ? i + 1 : i] : 0.0f;
             const float got = __shfl_xor_sync(0xFFFFFFFFu, odd ? h[i] : second, 1);
-            const float gate = odd ? got : h[i], value = odd ? second : got;
-            const int row = i + (odd ? 1 : 0);
-            if (there && row < rows && row < N) finish_one(e, row0 + row, r >> 1, activate(e.act, gate) * value);
+            gate[i / 2] = odd ? got : h[i];
+            value[i / 2] = odd ? second : got;
         }
+        activate(e.act, gate);
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) gate[i] *= value[i];
+        store_rows(e, gate, row0 + odd, 2, there ? (min(rows, N) + 1 - odd) / 2 : 0, r >> 1);
     }
 }
 
 // Four neighbouring columns r .. r + 3 of one row, sums with the bias in; r a multiple of four, `n` columns in all (an even number where gated).
-__device__ __forceinline__ void finish_four(const Epilogue& e, const float (&h)[4], long long row, long long r, long long n) {
+__device__ __forceinline__ void finish_four(const Epilogue& e, float (&h)[4], long long row, long long r, long long n) {
     if (!act_gated(e.act)) {
+        activate(e.act, h);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (r + j < n) finish_one(e, row, r + j, e.act == kActNone ? h[j] : activate(e.act, h[j]));
+        for (int j = 0; j < 4; ++j) {
+            const float one[1] = {h[j]};
+            if (r + j < n) store_rows(e, one, row, 1, 1, r + j);
+        }
     } else {
+        float gate[2] = {h[0], h[2]};
+        activate(e.act, gate);
 #pragma unroll
-        for (int j = 0; j < 4; j += 2)
-            if (r + j < n) finish_one(e, row, (r + j) >> 1, activate(e.act, h[j]) * h[j + 1]);
+        for (int j = 0; j < 2; ++j) {
+            const float one[1] = {gate[j] * h[2 * j + 1]};
+            if (r + 2 * j < n) store_rows(e, one, row, 1, 1, (r >> 1) + j);
+        }
     }
 }
 

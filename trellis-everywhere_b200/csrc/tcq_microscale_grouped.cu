@@ -471,7 +471,7 @@ cudaError_t launch(const GroupedCall& c, void* ws, cudaStream_t stream) {
     const long long tiles = most_tiles(c.groups.rows, c.groups.groups, T::kRowsX);
     uint8_t* const records = static_cast<uint8_t*>(ws) + (tiles * T::kRowsX * 4 + 255) / 256 * 256;
     const PartsArgs parts{c.x, c.x_rows, c.ldx, c.tokens, c.groups, c.k, k_tiles, T::kRowsX, (long long)record_bytes(FMT, NT),
-                          reinterpret_cast<uintptr_t>(c.x) % 16 == 0 && c.ldx % 8 == 0, records, static_cast<float*>(ws)};
+                          ms_rows_aligned(c.x, c.ldx), records, static_cast<float*>(ws)};
     err = c.dtype == kF16 ? launch_parts<__half>(c, parts, stream) : launch_parts<__nv_bfloat16>(c, parts, stream);
     if (err != cudaSuccess) return err;
     const GroupedArgs p{c.w, c.groups, int((n + kRowsW - 1) / kRowsW), k_tiles, records, static_cast<const float*>(ws), c.out, c.loads};
@@ -508,13 +508,20 @@ cudaError_t launch_nt(const GroupedCall& c, void* ws, cudaStream_t stream) {
 
 }  // namespace
 
-size_t ms_grouped_workspace_bytes(long long rows, long long groups, long long n, long long k, int dtype, int fmt) {
-    (void)n, (void)dtype;
+// Whether weights as 16-bit numbers pay: they are made once for up to 256 rows, where parts of x take six columns a row.
+static bool many_rows(long long rows, long long groups, int dtype, int fmt) { return rows > 90 * std::min(groups, rows) && ms_grouped_many_takes(dtype, fmt); }
+
+size_t ms_grouped_workspace_bytes(long long rows, long long groups, long long n, long long k, int dtype, int fmt, bool in_order) {
+    (void)n;
+    if (many_rows(rows, groups, dtype, fmt)) return in_order ? 0 : ms_grouped_many_workspace_bytes(rows, k);
     const int nt = columns_for(rows, groups), per = nt / kPartsX;
     const long long tiles = most_tiles(rows, groups, per);
     return size_t((tiles * per * 4 + 255) / 256 * 256) + size_t(tiles) * size_t(ms_tiles_k(k)) * record_bytes(fmt, nt);
 }
 
-cudaError_t launch_ms_grouped(const GroupedCall& c, void* ws, cudaStream_t stream) { return c.fmt == kNvfp4 ? launch_nt<kNvfp4>(c, ws, stream) : launch_nt<kMxfp4>(c, ws, stream); }
+cudaError_t launch_ms_grouped(const GroupedCall& c, void* ws, cudaStream_t stream) {
+    if (many_rows(c.groups.rows, c.groups.groups, c.dtype, c.fmt)) return launch_ms_grouped_many(c, ws, stream);
+    return c.fmt == kNvfp4 ? launch_nt<kNvfp4>(c, ws, stream) : launch_nt<kMxfp4>(c, ws, stream);
+}
 
 }  // namespace tcq

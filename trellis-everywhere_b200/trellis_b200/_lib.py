@@ -51,7 +51,7 @@ SIGNATURES = {
     "tcq_ms_matmul": (_int, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _int, _vp, _int, _i64, _vp]),
     "tcq_selftest_ms_linear_waits": (_int, [_i64, _vp, _int, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _int, _vp, _i64, _vp, _sz, _vp]),
     "tcq_selftest_ms_matmul_waits": (_int, [_i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _int, _vp, _int, _i64, _vp]),
-    "tcq_ms_grouped_linear_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _int, _int]),
+    "tcq_ms_grouped_linear_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _int, _int, _int]),
     "tcq_ms_grouped_linear": (_int, [_vp, _int, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _int, _vp, _int, _int, _vp, _i64, _vp, _int, _i64,
                                      _vp, _sz, _vp]),
     "tcq_ms_epilogue": (_int, [_vp, _i64, _i64, _vp, _int, _int, _vp, _i64, _vp, _int, _i64, _vp]),

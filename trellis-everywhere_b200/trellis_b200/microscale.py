@@ -227,7 +227,7 @@ def linear(x: torch.Tensor, w: Microscaled, bias: Optional[torch.Tensor] = None,
     ``bias [n]`` (fp32, fp16 or bf16), ``activation`` and ``residual [..., n]`` of x's type are applied to the fp32 sums, before the one rounding.
     ``activation``: "relu", "gelu" (with erf), "gelu_tanh", "silu", or gated, "geglu" or "swiglu": rows 2 j and 2 j + 1 of W are the gate and
     the value of result j (``interleave``), ``act(h[2 j]) * h[2 j + 1]``, and n / 2 results come out.  Products of 16-bit x with an epilogue are those of
-    ``experts.grouped_linear`` (x exact down to 2^-10 of a block's largest magnitude in bf16, 2^-7 in fp16; an infinity in x gives NaN).
+    ``experts.grouped_linear`` (x exact down to 2^-10 of a block's largest magnitude in bf16, 2^-7 in fp16; an infinity in x may give NaN where its sums have an infinity).
     """
     if bias is not None or activation is not None or residual is not None:
         return _linear_epilogue(x, w, bias, activation, residual)
@@ -276,12 +276,12 @@ def _check_bias(bias: Optional[torch.Tensor], shape: Tuple[int, ...], device) ->
 
 def _grouped(dev: int, flat: torch.Tensor, tokens, offsets, groups: int, rows: int, codes, scales, row, n: int, k: int, fmt: str, bias, act: int, residual, y: torch.Tensor) -> None:
     """``tcq_ms_grouped_linear`` with its workspace, given back when the call is queued: the stream's later work comes after it."""
-    dt, f = _DTYPES[flat.dtype], FORMATS[fmt]
-    size = _lib.lib().tcq_ms_grouped_linear_workspace_bytes(rows, groups, n, k, dt, f)
-    ws = torch.empty(size, dtype=torch.uint8, device=flat.device)
-    _launch(dev, "tcq_ms_grouped_linear", flat.data_ptr(), dt, flat.shape[0], _pitch(flat), _ptr(tokens), _ptr(offsets), groups, rows, codes.data_ptr(), scales.data_ptr(),
+    dt, f, at, pitch = _DTYPES[flat.dtype], FORMATS[fmt], flat.data_ptr(), _pitch(flat)
+    size = _lib.lib().tcq_ms_grouped_linear_workspace_bytes(rows, groups, n, k, dt, f, tokens is None and not (at % 16 or pitch % 8))
+    ws = torch.empty(size, dtype=torch.uint8, device=flat.device) if size else None
+    _launch(dev, "tcq_ms_grouped_linear", at, dt, flat.shape[0], pitch, _ptr(tokens), _ptr(offsets), groups, rows, codes.data_ptr(), scales.data_ptr(),
             _ptr(row), n, k, f, _ptr(bias), 0 if bias is None else _DTYPES[bias.dtype], act, _ptr(residual), 0 if residual is None else _pitch(residual),
-            y.data_ptr(), _DTYPES[y.dtype], y.shape[1], ws.data_ptr(), size)
+            y.data_ptr(), _DTYPES[y.dtype], y.shape[1], _ptr(ws), size)
 
 
 def _linear_epilogue(x: torch.Tensor, w: Microscaled, bias, activation, residual) -> torch.Tensor:
