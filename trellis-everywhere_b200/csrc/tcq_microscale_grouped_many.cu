@@ -5,8 +5,10 @@
 // x are the right operand, by TMA; an item takes as many columns as it has rows.  Rows that are gathered are put in order first.  (TMA loads of four rows of any numbers each took twice as long
 // for all.)
 //
-// Work split: one CTA per SM goes through items of 128 rows of a matrix x up to NT rows of its group.  One warp loads (codes and scales of 256 columns, x of 64), one issues
-// products, kMakers groups of four make weights in turn, four take finished sums out of tensor memory.
+// Work split: one CTA per SM goes through items of 128 rows of a matrix x up to 256 rows of its group.  One warp loads (codes and scales of 256 columns, x of 64), one issues
+// products, two groups of four make weights in turn, eight take finished sums out of tensor memory.  The sums of 128 rows are a buffer, of which there are three: the next item
+// begins when the first half of the last one's sums has been taken.  x and weights of 64 columns are one stage of one ring, with one barrier that says that both are there and one
+// that they are no longer needed: what a stage takes beside its products is waits and arrivals (0.3 us with neither products nor weights made; a third group of makers makes it longer).
 //
 // A wait that runs out (kMbarWaitCycles) makes its CTA stop, and its results from there on NaN.
 #include <algorithm>
@@ -19,20 +21,20 @@ namespace tcq {
 
 namespace {
 
-constexpr int kMakers = 3;
-constexpr int kThreads = 32 * (6 + 4 * kMakers);
-constexpr int kRows = 128, kStepK = 64, kNt = 256;
+constexpr int kMakers = 2, kTakers = 2;          // groups of four warps
+constexpr int kFirstTaker = 2, kFirstMaker = 2 + 4 * kTakers, kThreads = 32 * (2 + 4 * kTakers + 4 * kMakers);
+constexpr int kRows = 128, kStepK = 64, kNt = 256, kHalf = 128;
 constexpr int kBoxRows = 32;
 
 template <int FMT>
 struct Tile {
     static constexpr int kAtoms = Ms<FMT>::kAtoms;
-    static constexpr int kBytesW = kRows * 128, kBytesS = kAtoms * 512, kStageW = kBytesW + 2048, kStagesW = 3;      // 256 columns
-    static constexpr int kBytesX = kNt * 128, kStagesX = 5;                                                          // 64 columns
-    static constexpr int kStagesA = 4, kColumnsA = kStepK / 2;                                                       // weights in tensor memory
+    static constexpr int kBytesW = kRows * 128, kBytesS = kAtoms * 512, kStageW = kBytesW + 2048, kStagesW = 4;      // 256 columns
+    static constexpr int kBytesX = kNt * 128, kStages = 4;                                                           // 64 columns
+    static constexpr int kSums = 3, kColumnsA = kStepK / 2;                                                          // weights in tensor memory
     static constexpr int kColumns = 512;
-    static constexpr int kSmem = (kStagesW * kStageW + 1023) / 1024 * 1024 + kStagesX * kBytesX + 1024;
-    static_assert(kNt + kStagesA * kColumnsA <= kColumns && kSmem + sizeof(GroupPlan) + 1024 <= 227 * 1024);
+    static constexpr int kSmem = (kStagesW * kStageW + 1023) / 1024 * 1024 + kStages * kBytesX + 1024;
+    static_assert(kSums * kHalf + kStages * kColumnsA <= kColumns && kSmem + sizeof(GroupPlan) + 1024 <= 227 * 1024 && kSmem >= 116 * 1024);
 };
 
 struct ManyArgs {
@@ -81,7 +83,7 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_many_kernel(const 
     using T = Tile<FMT>;
     extern __shared__ uint8_t raw[];
     __shared__ GroupPlan plan;
-    __shared__ uint64_t w_full[T::kStagesW], w_empty[T::kStagesW], x_full[T::kStagesX], x_empty[T::kStagesX], a_full[T::kStagesA], a_empty[T::kStagesA], sum_full, sum_empty, drained;
+    __shared__ uint64_t w_full[T::kStagesW], w_empty[T::kStagesW], full[T::kStages], empty[T::kStages], sum_full[T::kSums], sum_empty[T::kSums], drained;
     __shared__ uint32_t tmem_at;
     __shared__ unsigned int gave_up;
     const uint32_t smem_w = (smem_u32(raw) + 1023) & ~1023u, smem_x = smem_w + (T::kStagesW * T::kStageW + 1023) / 1024 * 1024;
@@ -90,10 +92,8 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_many_kernel(const 
     if (warp == 0 && elect_one()) {
         gave_up = 0;
         for (int s = 0; s < T::kStagesW; ++s) { mbar_init(smem_u32(&w_full[s]), 1); mbar_init(smem_u32(&w_empty[s]), 4 * kMakers); }
-        for (int s = 0; s < T::kStagesX; ++s) { mbar_init(smem_u32(&x_full[s]), 1); mbar_init(smem_u32(&x_empty[s]), 1); }
-        for (int s = 0; s < T::kStagesA; ++s) { mbar_init(smem_u32(&a_full[s]), 4); mbar_init(smem_u32(&a_empty[s]), 1); }
-        mbar_init(smem_u32(&sum_full), 1);
-        mbar_init(smem_u32(&sum_empty), 4);
+        for (int s = 0; s < T::kStages; ++s) { mbar_init(smem_u32(&full[s]), 1 + 4); mbar_init(smem_u32(&empty[s]), 1); }
+        for (int s = 0; s < T::kSums; ++s) { mbar_init(smem_u32(&sum_full[s]), 1); mbar_init(smem_u32(&sum_empty[s]), 4 * kTakers); }
         mbar_init(smem_u32(&drained), 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -103,14 +103,14 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_many_kernel(const 
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = tmem_at, tmem_a = tmem + kNt;
+    const uint32_t tmem = tmem_at, tmem_a = tmem + T::kSums * kHalf;
     const int items = plan.tile[p.groups.groups] * p.tiles_n;
     const auto item_of = [&](int i) { return group_item(plan, p.groups.groups, p.tiles_n, kNt, i); };
 
     if (warp == 0) {
         // ---- loads; the warp stays together, one lane issues
         const bool one = elect_one();
-        uint32_t sw = 0, pw = 1, sx = 0, px = 1, loaded_w = 0, loaded_x = 0;      // (the first waits are for the phase before the first)
+        uint32_t sw = 0, pw = 1, s = 0, phase = 1, loaded_w = 0, loaded = 0;      // (the first waits are for the phase before the first)
         unsigned left = p.loads;
         bool ok = true;
         for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
@@ -130,61 +130,73 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_many_kernel(const 
                     if (++sw == T::kStagesW) { sw = 0; pw ^= 1; }
                     if (loaded_w < T::kStagesW) ++loaded_w;
                 }
-                ok = still_waits(ok, smem_u32(&x_empty[sx]), px, &gave_up);
+                ok = still_waits(ok, smem_u32(&empty[s]), phase, &gave_up);
                 if (!ok) break;
-                const uint32_t to = smem_x + sx * T::kBytesX, bar = smem_u32(&x_full[sx]);
                 if (one) {
+                    const uint32_t to = smem_x + s * T::kBytesX, bar = smem_u32(&full[s]);
                     mbar_expect(bar, boxes * kBoxRows * 128);
                     for (int b = 0; b < boxes; ++b) tma_load(to + b * kBoxRows * 128, &map_x, step * kStepK, t.row0 + b * kBoxRows, bar);
                 }
                 __syncwarp();
-                if (++sx == T::kStagesX) { sx = 0; px ^= 1; }
-                if (loaded_x < T::kStagesX) ++loaded_x;
+                if (++s == T::kStages) { s = 0; phase ^= 1; }
+                if (loaded < T::kStages) ++loaded;
             }
         }
         wait_for_loads<T::kStagesW>(w_full, sw, pw, loaded_w);
-        wait_for_loads<T::kStagesX>(x_full, sx, px, loaded_x);
+        wait_for_loads<T::kStages>(full, s, phase, loaded);
     } else if (warp == 1) {
         // ---- products; likewise
         constexpr uint32_t kIdesc = 1u << 4 | (FP16 ? 0u : 1u << 7 | 1u << 10) | uint32_t(kRows >> 4) << 24;      // bf16 x bf16 (or fp16 x fp16), fp32 sums
         const bool one = elect_one();
-        uint32_t sx = 0, px = 0, sa = 0, pa = 0;
-        int n = 0;
+        uint32_t s = 0, phase = 0;
+        int n = 0;                                       // buffers of sums taken so far
         bool ok = true;
-        for (int i = blockIdx.x; i < items && ok; i += gridDim.x, ++n) {
-            const uint32_t idesc = kIdesc | uint32_t((item_of(i).rows + 15) / 16 * 2) << 17;
-            if (n > 0) ok = mbar_wait(smem_u32(&sum_empty), uint32_t(n - 1) & 1, &gave_up);
+        for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
+            const int rows = item_of(i).rows, halves = rows > kHalf ? 2 : 1;
+            const auto idesc_of = [](int columns) { return kIdesc | uint32_t((columns + 15) / 16 * 2) << 17; };
+            const uint32_t idesc[2] = {idesc_of(min(rows, kHalf)), idesc_of(rows - kHalf)};
+            uint32_t d[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int buf = (n + h) % T::kSums, use = (n + h) / T::kSums;
+                d[h] = tmem + buf * kHalf;
+                if (h < halves && use > 0) ok = ok && mbar_wait(smem_u32(&sum_empty[buf]), uint32_t(use - 1) & 1, &gave_up);
+            }
             ok = __all_sync(0xFFFFFFFFu, ok);
             if (!ok) break;
             tc_fence_after();
             for (int step = 0; step < p.steps; ++step) {
-                ok = mbar_wait(smem_u32(&x_full[sx]), px, &gave_up) && mbar_wait(smem_u32(&a_full[sa]), pa, &gave_up);
-                ok = __all_sync(0xFFFFFFFFu, ok);        // every lane has seen these phases before the stages can be filled again
+                ok = mbar_wait(smem_u32(&full[s]), phase, &gave_up);
+                ok = __all_sync(0xFFFFFFFFu, ok);        // every lane has seen this phase before the stage can be filled again
                 if (!ok) break;
                 tc_fence_after();
-                const uint64_t db = desc_rows128(smem_x + sx * T::kBytesX);
-                const uint32_t a = tmem_a + sa * T::kColumnsA;
+                const uint64_t db = desc_rows128(smem_x + s * T::kBytesX);
+                const uint32_t a = tmem_a + s * T::kColumnsA;
                 if (one) {
 #pragma unroll
-                    for (int j = 0; j < kStepK / 16; ++j) mma_from_tmem(tmem, a + 8 * j, db + 2 * j, idesc, step > 0 || j > 0);
-                    tc_commit(smem_u32(&x_empty[sx]));
-                    tc_commit(smem_u32(&a_empty[sa]));
+                    for (int j = 0; j < kStepK / 16; ++j) mma_from_tmem(d[0], a + 8 * j, db + 2 * j, idesc[0], step > 0 || j > 0);
+                    if (halves > 1) {
+#pragma unroll
+                        for (int j = 0; j < kStepK / 16; ++j) mma_from_tmem(d[1], a + 8 * j, db + (kHalf * 128 >> 4) + 2 * j, idesc[1], step > 0 || j > 0);
+                    }
+                    tc_commit(smem_u32(&empty[s]));
                 }
                 __syncwarp();
-                if (++sx == T::kStagesX) { sx = 0; px ^= 1; }
-                if (++sa == T::kStagesA) { sa = 0; pa ^= 1; }
+                if (++s == T::kStages) { s = 0; phase ^= 1; }
             }
-            if (ok && one) tc_commit(smem_u32(&sum_full));
+            if (ok && one)
+                for (int h = 0; h < halves; ++h) tc_commit(smem_u32(&sum_full[(n + h) % T::kSums]));
             __syncwarp();
+            n += halves;
         }
         if (!ok) {                                       // what was issued ends before the tensor memory goes
             if (one) tc_commit(smem_u32(&drained));
             __syncwarp();
             for (long long t0 = clock64(); !mbar_try_wait(smem_u32(&drained), 0) && clock64() - t0 < kMbarWaitCycles;) {}
         }
-    } else if (warp >= 6) {
+    } else if (warp >= kFirstMaker) {
         // ---- weights: lane = row of this warp's quarter; the groups of four warps take turns
-        const int quarter = warp & 3, mine = (warp - 6) >> 2;
+        const int quarter = warp & 3, mine = (warp - kFirstMaker) >> 2;
         const int row = 32 * quarter + lane;
         const E2m1Bytes<false> bytes;
         const auto scale_of = [&](int i) {               // of this lane's row; fetched an item ahead
@@ -194,7 +206,7 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_many_kernel(const 
             return r < p.w.rows ? __ldg(p.w.row_scale + t.group * p.w.rows + r) : 1.0f;
         };
         float next = scale_of(blockIdx.x);
-        uint32_t sw = 0, pw = 0, sa = 0, pa = 1;
+        uint32_t sw = 0, pw = 0, s = 0, phase = 1;
         int turn = 0;                                    // whose step it is
         bool ok = true;
         for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
@@ -244,17 +256,17 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_many_kernel(const 
                             }
                         }
                     }
-                    ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&a_empty[sa]), pa, &gave_up));
+                    ok = __all_sync(0xFFFFFFFFu, mbar_wait(smem_u32(&empty[s]), phase, &gave_up));
                     if (ok) {
                         tc_fence_after();
-                        tmem_store32(tmem_a + sa * T::kColumnsA + (uint32_t(32 * quarter) << 16), v);
+                        tmem_store32(tmem_a + s * T::kColumnsA + (uint32_t(32 * quarter) << 16), v);
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(smem_u32(&a_full[sa]));
+                        if (lane == 0) mbar_arrive(smem_u32(&full[s]));
                     }
                 }
                 if (++turn == kMakers) turn = 0;
-                if (++sa == T::kStagesA) { sa = 0; pa ^= 1; }
+                if (++s == T::kStages) { s = 0; phase ^= 1; }
                 if (step % 4 == 3 || step + 1 == p.steps) {
                     __syncwarp();
                     if (lane == 0) mbar_arrive(smem_u32(&w_empty[sw]));
@@ -264,36 +276,42 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_many_kernel(const 
         }
     } else {
         // ---- results: this warp's lanes are 32 rows of W, so that a store is 32 neighbours in y
-        const int quarter = warp & 3;
-        constexpr int kChunk = 16;
+        const int quarter = warp & 3, mine = (warp - kFirstTaker) >> 2;
+        constexpr int kChunk = 16, kShare = kHalf / kTakers;                     // columns of a buffer that are this warp's
         int n = 0;
         bool ok = true;
-        for (int i = blockIdx.x; i < items; i += gridDim.x, ++n) {
+        for (int i = blockIdx.x; i < items; i += gridDim.x) {
             const GroupItem t = item_of(i);
             const long long r = (long long)t.tn * kRows + 32 * quarter + lane, column = t.group * p.w.rows + r;
             const bool there = r < p.w.rows;
             const float fw = there ? row_factor<FMT, FP16>(p, column) : 1.0f;
             const float bias = p.out.bias != nullptr && there ? load_as_f32(p.out.bias, p.out.bias_dtype, column) : 0.0f;
-            ok = still_waits(ok, smem_u32(&sum_full), uint32_t(n) & 1, &gave_up);
-            tc_fence_after();
+            for (int half = 0; half < t.rows; half += kHalf, ++n) {
+                const int buf = n % T::kSums;
+                ok = still_waits(ok, smem_u32(&sum_full[buf]), uint32_t(n / T::kSums) & 1, &gave_up);
+                tc_fence_after();
+                const int first = mine * kShare, last = min(first + kShare, t.rows - half);
 #pragma unroll 1
-            for (int c0 = 0; c0 < t.rows; c0 += kChunk) {
-                uint32_t v[kChunk];
-                tmem_load<kChunk>(tmem + c0 + (uint32_t(32 * quarter) << 16), v);
-                tmem_wait_ld();
-                if (c0 + kChunk >= t.rows) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&sum_empty));
-                }
-                float h[kChunk];
+                for (int c0 = first; c0 < last; c0 += kChunk) {
+                    uint32_t v[kChunk];
+                    tmem_load<kChunk>(tmem + buf * kHalf + c0 + (uint32_t(32 * quarter) << 16), v);
+                    tmem_wait_ld();
+                    float h[kChunk];
 #pragma unroll
-                for (int c = 0; c < kChunk; ++c) {
-                    float f = __uint_as_float(v[c]);
-                    if constexpr (FMT == kNvfp4) f *= fw;
-                    h[c] = ok ? f + bias : __uint_as_float(0x7FC00000u);
+                    for (int c = 0; c < kChunk; ++c) {
+                        float f = __uint_as_float(v[c]);
+                        if constexpr (FMT == kNvfp4) f *= fw;
+                        h[c] = ok ? f + bias : __uint_as_float(0x7FC00000u);
+                    }
+                    if (c0 + kChunk >= last) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(smem_u32(&sum_empty[buf]));
+                    }
+                    finish_rows(p.out, h, t.row0 + half + c0, last - c0, r, there);
                 }
-                finish_rows(p.out, h, t.row0 + c0, t.rows - c0, r, there);
+                if (first >= last && lane == 0) mbar_arrive(smem_u32(&sum_empty[buf]));       // fewer rows than reach this warp's columns
+                __syncwarp();
             }
         }
     }
