@@ -21,15 +21,15 @@ def activate(h, act):
 
 
 def sums_bound(x, w, fmt):
-    """Of fp32 sums of x's 4-bit parts times w (fp64 [m, k], [n, k]): 2^-18 of each block's largest for what the parts leave (nvfp4: and 2^-20 of the row's), and for
-    every 64 columns 2^-22 of the sum of the parts' magnitudes, which is at most 1.6 times that of the blocks' largest (the parts of x: |x| + s / 2, then s / 2, s / 16 ... with
-    s <= amax / 2)."""
+    """Of fp32 sums of x's 4-bit parts times w (fp64 [m, k], [n, k]).  With s of a block, 1.7 s <= amax: x / s is rounded to 15 binary places, 2^-16 s <= 2^-16.7 amax off.  nvfp4
+    leaves digits out whose scale is below 2^-17 of the row's largest scale S, 1.7 S <= the row's largest: 4 (1/8 + 1/64 + ...) 2^-17 S <= 0.572 2^-17 / 1.7 = 2^-18.5 of the row's largest.
+    For every 64 columns 2^-22 of the sum of the parts' magnitudes: the first is |x| + 0.572 s at most and the others 0.572 s together, |x| + 1.15 s <= 1.7 amax."""
     b, k = BLOCK[fmt], x.shape[1]
     amax = torch.nn.functional.pad(x.abs(), (0, -k % b)).reshape(x.shape[0], -1, b).amax(2).repeat_interleave(b, 1)[:, :k]
     a = amax @ w.abs().t()
-    bound = a * (2.0 ** -18 + 1.6 * (k / 64 + 8) * 2.0 ** -22)
+    bound = a * (2.0 ** -16.7 + 1.7 * (k / 64 + 8) * 2.0 ** -22)
     if fmt == "nvfp4":
-        bound = bound + 2.0 ** -20 * x.abs().amax(1, keepdim=True) * w.abs().sum(1)[None]
+        bound = bound + 2.0 ** -18.5 * x.abs().amax(1, keepdim=True) * w.abs().sum(1)[None]
     return bound
 
 

@@ -4,7 +4,7 @@
 // The rows are put in order of experts by counting: how many tokens before, by chunks of tokens, then by warps of a chunk, then within 32 neighbours; so
 // rows of one expert keep the order of their tokens, whatever runs first.  Up to kOneChunk tokens are one CTA's and one launch; more take two.
 //
-// The sum: a thread has eight neighbouring columns of one token, its rows' loads are in flight together.  Bound by memory.
+// The sum: a thread has eight columns of one token, and the loads of four of its rows are in flight together.  Bound by memory.
 #include <algorithm>
 
 #include "tcq_experts.cuh"
@@ -235,74 +235,123 @@ __global__ void __launch_bounds__(kThreads) tcq_route_place_kernel(const __grid_
     place_chunk(c, (long long)t0 * c.top, (t1 - t0) * c.top, base, hist);
 }
 
-// N neighbouring numbers, as one load where `wide`.
-template <typename T, int N>
-__device__ __forceinline__ void load_run(const T* p, bool wide, int there, float (&v)[N]) {
-    if (wide) {
-        constexpr int kPer = 16 / sizeof(T);
+// Eight neighbouring numbers as they lie in memory.
+template <typename T> struct Eight { uint4 u[sizeof(T) / 2]; };
+template <typename T>
+__device__ __forceinline__ void to_floats(const Eight<T>& e, float (&v)[8]) {
 #pragma unroll
-        for (int q = 0; q < N / kPer; ++q) {
-            const uint4 u = __ldg(reinterpret_cast<const uint4*>(p) + q);
+    for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(reinterpret_cast<const T*>(e.u)[i]);
+}
+// At any address: pieces of 16 bytes that start on 16 bytes, one more than they fill, and a shift; single numbers where a piece would reach out of from .. to.  `there` of them exist.
+template <typename T>
+__device__ __forceinline__ Eight<T> load_eight(const T* p, bool aligned, int there, const void* from, const void* to) {
+    constexpr int kPieces = sizeof(T) / 2;
+    Eight<T> e;
+    if (aligned) {
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) v[q * kPer + i] = to_f32<T>(reinterpret_cast<const T*>(&u)[i]);
+        for (int q = 0; q < kPieces; ++q) e.u[q] = __ldg(reinterpret_cast<const uint4*>(p) + q);
+        return e;
+    }
+    const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(p)) & 15u;
+    const char* const base = reinterpret_cast<const char*>(p) - off;
+    if (there >= 8 && base >= from && base + 16 * (kPieces + 1) <= to) {
+        uint32_t w[4 * (kPieces + 1)];
+#pragma unroll
+        for (int q = 0; q <= kPieces; ++q) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4*>(base) + q);
+            w[4 * q] = u.x; w[4 * q + 1] = u.y; w[4 * q + 2] = u.z; w[4 * q + 3] = u.w;
         }
+#pragma unroll
+        for (int step = 2; step >= 1; --step)
+            if (off & (4 * step))
+#pragma unroll
+                for (int i = 0; i + step < 4 * (kPieces + 1); ++i) w[i] = w[i + step];
+#pragma unroll
+        for (int i = 0; i < 4 * kPieces; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 8 * (off & 3));
+#pragma unroll
+        for (int q = 0; q < kPieces; ++q) e.u[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = i < there ? to_f32<T>(p[i]) : 0.0f;
+        for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(e.u)[i] = i < there ? p[i] : from_f32<T>(0.0f);
     }
+    return e;
 }
 
-// Y: of the rows, O: of what comes out.  RUN = 8: a thread eight neighbours in pieces of 16 bytes; 1: a thread one column, a warp 32 neighbours.
-template <typename Y, typename O, int RUN>
-__global__ void __launch_bounds__(256) tcq_combine_kernel(const __grid_constant__ CombineCall c, unsigned runs) {
-    const long long id = (long long)blockIdx.x * 256 + threadIdx.x;
-    const long long token = id / runs, c0 = (id - token * runs) * RUN;
-    if (token >= c.tokens) return;
-    float sum[RUN] = {};
-    const bool wide = RUN == 8;
-    if (c.residual != nullptr) load_run<O, RUN>(static_cast<const O*>(c.residual) + token * c.ldr + c0, wide, RUN, sum);
-    float out[RUN] = {};
-    for (int j0 = 0; j0 < c.top; j0 += 4) {
-        float v[4][RUN], w[4];
+// Y: of the rows, O: of what comes out.  Threads in x: eight columns of a token each; in y: tokens.  ALIGNED: all rows start on 16 bytes, and n is a multiple of eight.
+template <typename Y, typename O, bool ALIGNED>
+__global__ void __launch_bounds__(256, !ALIGNED ? 3 : sizeof(Y) == 2 ? 5 : 4) tcq_combine_kernel(const __grid_constant__ CombineCall c) {
+    __shared__ uint4 turn[ALIGNED ? 1 : 8][ALIGNED ? 1 : 32 * (sizeof(O) / 2)];      // results of a warp, which stores neighbours
+    const int n = int(c.n), lane = threadIdx.x & 31;
+    const long long stride = (long long)gridDim.x * blockDim.y;
+    for (long long token = (long long)blockIdx.x * blockDim.y + threadIdx.y; token < c.tokens; token += stride) {
+        const int* const places = c.places + token * c.top;
+        const float* const weights = c.weights + token * c.top;
+        for (int c0 = 8 * threadIdx.x; c0 - 8 * lane < n; c0 += 8 * blockDim.x) {     // (whole warps stay together)
+            const int there = n - c0;
+            float out[8] = {};
+            Eight<O> res;
+            if (c.residual != nullptr && there > 0) {
+                const O* const at = static_cast<const O*>(c.residual) + token * c.ldr + c0;
+                res = load_eight<O>(at, ALIGNED, there, c.residual, static_cast<const O*>(c.residual) + (c.tokens - 1) * c.ldr + n);
+            }
+            for (int j0 = 0; j0 < c.top; j0 += 4) {
+                Eight<Y> v[4];
+                float w[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int j = j0 + q;
-            const int place = j < c.top ? __ldg(c.places + token * c.top + j) : -1;
-            w[q] = 0.0f;
-            if (place >= 0 && place < c.rows) {
-                w[q] = __ldg(c.weights + token * c.top + j);
-                load_run<Y, RUN>(static_cast<const Y*>(c.y) + place * c.ldy + c0, wide, RUN, v[q]);
+                for (int q = 0; q < 4; ++q) {
+                    const int place = j0 + q < c.top ? __ldg(places + j0 + q) : -1;
+                    const bool some = place >= 0 && place < c.rows && there > 0;
+                    w[q] = some ? __ldg(weights + j0 + q) : 0.0f;
+                    v[q] = {};
+                    if (some) v[q] = load_eight<Y>(static_cast<const Y*>(c.y) + place * c.ldy + c0, ALIGNED, there, c.y, static_cast<const Y*>(c.y) + (c.rows - 1) * c.ldy + n);
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    float f[8];
+                    to_floats(v[q], f);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) out[i] = __fmaf_rn(f[i], w[q], out[i]);
+                }
+            }
+            if (c.residual != nullptr && there > 0) {
+                float f[8];
+                to_floats(res, f);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) out[i] += f[i];
+            }
+            Eight<O> r;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) reinterpret_cast<O*>(r.u)[i] = from_f32<O>(out[i]);
+            O* const to = static_cast<O*>(c.out) + token * c.ldo + c0;
+            if constexpr (ALIGNED) {
+                if (there > 0)
+#pragma unroll
+                    for (int q = 0; q < int(sizeof(O) / 2); ++q) reinterpret_cast<uint4*>(to)[q] = r.u[q];
             } else {
+                uint4* const mine = turn[threadIdx.y * (blockDim.x / 32) + threadIdx.x / 32];
 #pragma unroll
-                for (int i = 0; i < RUN; ++i) v[q][i] = 0.0f;
+                for (int q = 0; q < int(sizeof(O) / 2); ++q) mine[lane * (sizeof(O) / 2) + q] = r.u[q];
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (c0 - 8 * lane + lane + 32 * i < n) to[lane + 32 * i - 8 * lane] = reinterpret_cast<const O*>(mine)[lane + 32 * i];
+                __syncwarp();
             }
         }
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-            for (int i = 0; i < RUN; ++i) out[i] = __fmaf_rn(v[q][i], w[q], out[i]);
-    }
-    O* const to = static_cast<O*>(c.out) + token * c.ldo + c0;
-    if constexpr (RUN == 8) {
-        alignas(16) O r[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) r[i] = from_f32<O>(out[i] + sum[i]);
-#pragma unroll
-        for (int q = 0; q < int(sizeof(O) / 2); ++q) reinterpret_cast<uint4*>(to)[q] = reinterpret_cast<const uint4*>(r)[q];
-    } else {
-        *to = from_f32<O>(out[0] + sum[0]);
     }
 }
 
 template <typename Y, typename O>
 cudaError_t combine(const CombineCall& c, cudaStream_t stream) {
     const auto rows_of_16 = [](const void* p, long long ld, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * bytes % 16 == 0; };
-    const bool wide = c.n % 8 == 0 && rows_of_16(c.y, c.ldy, sizeof(Y)) && rows_of_16(c.out, c.ldo, sizeof(O)) &&
-                      (c.residual == nullptr || rows_of_16(c.residual, c.ldr, sizeof(O)));
-    const long long runs = wide ? c.n / 8 : c.n, blocks = (c.tokens * runs + 255) / 256;
-    if (blocks > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
-    if (wide) tcq_combine_kernel<Y, O, 8><<<unsigned(blocks), 256, 0, stream>>>(c, unsigned(runs));
-    else tcq_combine_kernel<Y, O, 1><<<unsigned(blocks), 256, 0, stream>>>(c, unsigned(runs));
+    const bool aligned = c.n % 8 == 0 && rows_of_16(c.y, c.ldy, sizeof(Y)) && rows_of_16(c.out, c.ldo, sizeof(O)) &&
+                         (c.residual == nullptr || rows_of_16(c.residual, c.ldr, sizeof(O)));
+    const long long runs = (c.n + 7) / 8;
+    dim3 block(32, 8);
+    while (block.x < 256 && block.x < runs) { block.x *= 2; block.y /= 2; }
+    const unsigned grid = unsigned(std::min<long long>((c.tokens + block.y - 1) / block.y, 1 << 20));
+    if (aligned) tcq_combine_kernel<Y, O, true><<<grid, block, 0, stream>>>(c);
+    else tcq_combine_kernel<Y, O, false><<<grid, block, 0, stream>>>(c);
     return cudaGetLastError();
 }
 template <typename Y>

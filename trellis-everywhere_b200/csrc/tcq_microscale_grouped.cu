@@ -1,10 +1,10 @@
 // Rows of 16-bit activations in groups, each group times a 4-bit microscaled matrix of its own, few rows a group: y[i] = act(W[g(i)] x[i] + bias) + residual.
 //
-// The tensor cores multiply 4-bit numbers as they lie in memory, so that a weight costs nothing but its bytes; it is x that is cut up.  With s = 2^(floor(log2
-// amax) - 1) of a block of 16 (nvfp4) or 32 (mxfp4) columns, x / s is below 4 in magnitude; the nearest e2m1 number is off by half at most, and what is left, times
-// eight, is below 4 again.  So x = s (q0 + q1 / 8 + q2 / 64 + ...), each part a row of 4-bit numbers with block scales s, s / 8, s / 64 ..., and the product is that of
-// tcgen05.mma with kPartsX columns for each row of x, added up at the end.  Six parts hold every bit of bf16 numbers down to 2^-10 of their block's
-// largest (fp16: 2^-7) and are off by 2^-18 of that at most elsewhere; nvfp4's scales, of a token as of a matrix, end 2^-17 below the token's largest one (2^-20 of its largest number).
+// The tensor cores multiply 4-bit numbers as they lie in memory, so that a weight costs nothing but its bytes; it is x that is cut up.  With s a power of two, 1.7 s <= amax < 3.4 s for
+// the largest magnitude of a block of 16 (nvfp4) or 32 (mxfp4) columns, x / s rounded to 15 binary places is a number of six digits of base 8, each of -4 .. 3, all of which are e2m1 numbers:
+// x = s (d0 + d1 / 8 + ... + d5 / 8^5).  Each digit is a row of 4-bit numbers with block scales s, s / 8, s / 64 ..., and the product is that of tcgen05.mma with kPartsX columns for
+// each row of x, added up at the end.  Six digits hold every bit of bf16 numbers down to 2^-8 of their block's largest (fp16: 2^-5) and are off by 2^-16.7 of that at most elsewhere;
+// nvfp4's scales, of a token as of a matrix, end 2^-17 below the token's largest one: digits below that are left out (2^-18.5 of its largest number at most).
 //
 // Work split: one small kernel finds each row's group and place, cuts it up and leaves it as the stages that the products load (codes swizzled as the tensor cores
 // read them, scales in the order of tcgen05.cp).  The other goes through items of 128 rows of a matrix x NT / kPartsX rows of its group, one CTA per SM, and begins
@@ -71,8 +71,52 @@ __device__ __forceinline__ uint32_t largest(const float* v) {
     return m;
 }
 
-// The exponent of a block's first scale: floor(log2 amax) - 1, no lower than leaves the last part a scale of its own.
-__device__ __forceinline__ int first_exponent(uint32_t amax_bits) { return max(int(amax_bits >> 23) - 128, -127 + 3 * (kPartsX - 1)); }
+// The exponent of a block's first scale s, no lower than leaves the last digit a scale of its own.
+__device__ __forceinline__ int first_exponent(uint32_t amax_bits) { return max(int((amax_bits + 0x266667u) >> 23) - 128, -127 + 3 * (kPartsX - 1)); }
+
+// A block's first scale as an exponent over 2^base.  nvfp4, base the exponent of the row's scale: digits that would have a scale below 2^-9, the least, are left out, so that the
+// last one is to have this very scale.
+template <int FMT>
+__device__ __forceinline__ int block_exponent(uint32_t amax_bits, int base) {
+    const int e = first_exponent(amax_bits) - base;
+    if (FMT == kMxfp4 || e >= 3 * (kPartsX - 1) - 9) return e;
+    return (max(e + 9, 0) + 2) / 3 * 3 - 9;
+}
+struct Up {                                              // times 2^(15 - e), in two steps: e may be -135
+    float a, b;
+    __device__ __forceinline__ Up(int e) : a(pow2f((15 - e) / 2)), b(pow2f(15 - e - (15 - e) / 2)) {}
+    __device__ __forceinline__ float operator()(float v) const { return v * a * b; }
+};
+
+// The six digits of v 2^-15, |v| < 3.4 * 2^15, as codes: the first in nibble 5.  Bits 24 and up mean nothing.
+// An addition rounds to a whole number and makes digits 0 .. 7 of -4 .. 3; three bits are spread to four, and all six are looked up as functions of their bits.
+__device__ __forceinline__ uint32_t digit_codes(float v) {
+    constexpr float kZero = 12582912.0f + 4.0f * (1 + 8 + 64 + 512 + 4096 + 32768);       // 3 * 2^22, and a digit 4 in every place
+    const uint32_t u = __float_as_uint(v + kZero), two = (u & 0x1FFu) | ((u << 3) & ~0x1FFu);
+    uint32_t d = (two & 0x007007u) | ((two << 1) & ~0x007007u);
+    d = (d & 0x077077u) | ((two << 2) & ~0x077077u);
+    const uint32_t b1 = d >> 1, b2 = d >> 2;
+    const uint32_t c0 = d & ~(b1 ^ b2), c1 = (b2 & ~b1 & d) | (~b2 & ~(b1 ^ d)), c2 = (b2 & b1) | (~b2 & ~(b1 & d));      // 4 3 2 1 0 -1 .. as 6 5 4 2 0 and the sign
+    uint32_t r = (c0 & 0x111111u) | ((c1 << 1) & ~0x111111u);
+    r = (r & 0x333333u) | ((c2 << 2) & ~0x333333u);
+    return (r & 0x777777u) | (~(d << 1) & ~0x777777u);
+}
+// The codes of two columns side by side: of part 5 - 2 b in byte b of `even`, of part 4 - 2 b in byte b of `odd`.
+struct TwoColumns { uint32_t even, odd; };
+__device__ __forceinline__ TwoColumns two_columns(float a, float b) {
+    const uint32_t x = digit_codes(a), y = digit_codes(b);
+    return {(x & 0x0F0F0Fu) | ((y << 4) & ~0x0F0F0Fu), ((x >> 4) & 0x0F0F0Fu) | (y & ~0x0F0F0Fu)};
+}
+__device__ __forceinline__ uint32_t of_part(const TwoColumns& t, int part) { return part & 1 ? t.even : t.odd; }      // (byte (5 - part) / 2 of it)
+
+// The byte of the scale of a part, and whether its codes count.  e: exponent of the block's first scale (nvfp4: over the row's scale); nan: the block is not finite.
+template <int FMT>
+__device__ __forceinline__ uint32_t part_scale(int e, bool nan, int part, bool& gone) {
+    const int at = e - 3 * part;
+    gone = FMT == kNvfp4 && at < -9;                     // below the least scale
+    if constexpr (FMT == kNvfp4) return nan ? 0x7Fu : at >= -6 ? uint32_t(at + 7) << 3 : gone ? 0u : 1u << (at + 9);
+    else return nan ? 0xFFu : uint32_t(at + 127);
+}
 
 // One CTA takes rows blockIdx.x, blockIdx.x + gridDim.x ...; a thread 32 columns at a time.
 template <typename T, int FMT>
@@ -125,53 +169,42 @@ __global__ void __launch_bounds__(256) tcq_ms_row_parts_kernel(const __grid_cons
         }
         for (int j = threadIdx.x; j < chunks; j += blockDim.x) {
             if (j != int(threadIdx.x) && inside) load32(row, 32ll * j, p.k, p.wide, v);
-            constexpr int kBlocks = 32 / Ms<FMT>::kBlock, kBlock = Ms<FMT>::kBlock;
-            int e[kBlocks];
-            bool nan[kBlocks];
+            uint32_t m[2] = {largest<16>(v), largest<16>(v + 16)};
+            if constexpr (FMT == kMxfp4) m[0] = m[1] = max(m[0], m[1]);           // one block
+            int e[2];
+            bool nan[2];
+            TwoColumns two[16];
 #pragma unroll
-            for (int b = 0; b < kBlocks; ++b) {
-                const uint32_t m = largest<kBlock>(v + b * kBlock);
-                nan[b] = !inside || m >= 0x7F800000u;
-                e[b] = first_exponent(m);
-                const float down0 = pow2f(-(e[b] / 2)), down1 = pow2f(e[b] / 2 - e[b]);      // in two steps: -112 <= e <= 126
+            for (int h = 0; h < 2; ++h) {
+                nan[h] = !inside || m[h] >= 0x7F800000u;
+                e[h] = nan[h] ? 0 : block_exponent<FMT>(m[h], base);
+                const Up up(e[h] + base);
 #pragma unroll
-                for (int q = 0; q < kBlock; ++q) v[b * kBlock + q] = nan[b] ? 0.0f : v[b * kBlock + q] * down0 * down1;
+                for (int q = 0; q < 8; ++q) {
+                    const int c = 16 * h + 2 * q;
+                    two[8 * h + q] = two_columns(nan[h] ? 0.0f : up(v[c]), nan[h] ? 0.0f : up(v[c + 1]));
+                }
             }
             uint8_t* const record = p.out + ((long long)tile * p.k_tiles + j / 8) * p.record;
             const int jj = j % 8;
 #pragma unroll
             for (int part = 0; part < kPartsX; ++part) {
-                uint32_t words[4] = {};
-                uint32_t scale = 0;
+                const uint32_t byte = (5 - part) / 2, pick = byte | (4 + byte) << 4;
+                uint32_t w[4], scale[2];
+                bool gone[2];
 #pragma unroll
-                for (int b = 0; b < kBlocks; ++b) {
-                    uint32_t byte;
-                    bool gone = false;                   // nvfp4: its scale would be below the least
-                    if constexpr (FMT == kNvfp4) {
-                        const int to = e[b] - 3 * part - base;                    // at most 8
-                        gone = to < -9;
-                        byte = nan[b] ? 0x7Fu : to >= -6 ? uint32_t(to + 7) << 3 : gone ? 0u : 1u << (to + 9);
-                    } else {
-                        byte = nan[b] ? 0xFFu : uint32_t(e[b] - 3 * part + 127);
-                    }
-                    scale |= byte << (8 * b);
+                for (int h = 0; h < 2; ++h) scale[h] = part_scale<FMT>(e[h], nan[h], part, gone[h]);
 #pragma unroll
-                    for (int q = 0; q < kBlock; q += 2) {
-                        const int at2 = b * kBlock + q;
-                        const uint32_t code = f32x2_to_e2m1x2(v[at2], v[at2 + 1]);
-                        uint32_t h;
-                        asm("{\n\t.reg .b8 b0;\n\tcvt.u8.u32 b0, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, b0;\n\t}" : "=r"(h) : "r"(code));
-                        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h));
-                        v[at2] = (v[at2] - back.x) * 8.0f;                        // exact
-                        v[at2 + 1] = (v[at2 + 1] - back.y) * 8.0f;
-                        words[at2 / 8] |= (gone ? 0u : code) << (4 * (at2 % 8));
-                    }
+                for (int q = 0; q < 4; ++q) {
+                    const TwoColumns* const t = two + 4 * q;
+                    w[q] = __byte_perm(__byte_perm(of_part(t[0], part), of_part(t[1], part), pick), __byte_perm(of_part(t[2], part), of_part(t[3], part), pick), 0x5410);
+                    if (gone[q / 2]) w[q] = 0;
                 }
                 const int c = place * kPartsX + part;    // column of the tile
-                *reinterpret_cast<uint4*>(record + kBytesScales<FMT> + c * 128 + ((jj ^ (c & 7)) << 4)) = make_uint4(words[0], words[1], words[2], words[3]);
+                *reinterpret_cast<uint4*>(record + kBytesScales<FMT> + c * 128 + ((jj ^ (c & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
                 uint8_t* const s = record + (c & 31) * 16 + (c >> 5) * 4;
-                if constexpr (FMT == kNvfp4) *reinterpret_cast<uint16_t*>(s + (jj / 2) * 512 + 2 * (jj & 1)) = uint16_t(scale);
-                else s[(jj / 4) * 512 + (jj & 3)] = uint8_t(scale);
+                if constexpr (FMT == kNvfp4) *reinterpret_cast<uint16_t*>(s + (jj / 2) * 512 + 2 * (jj & 1)) = uint16_t(scale[0] | scale[1] << 8);
+                else s[(jj / 4) * 512 + (jj & 3)] = uint8_t(scale[0]);
             }
         }
     }
@@ -219,6 +252,28 @@ __device__ __forceinline__ void mma_block_scaled(uint32_t d, uint64_t a, uint64_
                      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(uint32_t(add)) : "memory");
 }
 
+// The sums of one item out of the parts that the CTAs of a cluster have in shared memory ([rows][128] at smem_sum of each), in rank order; four neighbours a thread.
+__device__ __forceinline__ void add_up_parts(const Epilogue& out, const GroupItem& t, long long n, uint32_t smem_sum, uint32_t rank, uint32_t splits, int threads) {
+    for (int i = int(rank) * threads + int(threadIdx.x); i < kRowsW / 4 * t.rows; i += int(splits) * threads) {
+        const long long r = (long long)t.tn * kRowsW + i % (kRowsW / 4) * 4;
+        if (r >= n) continue;
+        float4 part[kMostSplits];
+#pragma unroll
+        for (uint32_t q = 0; q < kMostSplits; ++q)
+            if (q < splits) part[q] = ld_cluster_f32x4(smem_sum + 16 * i, q);
+        float4 f = part[0];
+#pragma unroll
+        for (uint32_t q = 1; q < kMostSplits; ++q)
+            if (q < splits) f = make_float4(f.x + part[q].x, f.y + part[q].y, f.z + part[q].z, f.w + part[q].w);
+        float h[4] = {f.x, f.y, f.z, f.w};
+        if (out.bias != nullptr)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (r + j < n) h[j] += load_as_f32(out.bias, out.bias_dtype, (long long)t.group * n + r + j);
+        finish_four(out, h, t.row0 + i / (kRowsW / 4), r, n);
+    }
+}
+
 template <int FMT, int NT>
 __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ GroupedArgs p) {
     using T = Tile<FMT, NT>;
@@ -231,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_kernel(const __gri
     float* const sums = reinterpret_cast<float*>(raw + (smem_sum - smem_u32(raw)));
     const int warp = __shfl_sync(0xFFFFFFFFu, int(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank(), splits = cluster_size();
-    const int first = int((long long)p.k_tiles * rank / splits), last = int((long long)p.k_tiles * (rank + 1) / splits);
+    const int first = int(uint32_t(p.k_tiles) * rank / splits), last = int(uint32_t(p.k_tiles) * (rank + 1) / splits);      // (at most 2^16 times 8)
     const int start = blockIdx.x / splits, clusters = gridDim.x / splits;
     const long long atoms = (long long)p.k_tiles * T::kAtoms;
     constexpr long long kRecord = T::kBytesS + NT * 128;
@@ -403,28 +458,321 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_kernel(const __gri
     __syncwarp();
     if (splits > 1) {                                        // one item a cluster: add up the parts of it, four neighbours a thread
         cluster_sync();
-        if (start < items) {
-            const GroupItem t = item_of(start);
-            for (int i = int(rank) * kThreads + threadIdx.x; i < kRowsW / 4 * t.rows; i += int(splits) * kThreads) {
-                const long long r = (long long)t.tn * kRowsW + i % (kRowsW / 4) * 4;
-                if (r >= p.w.rows) continue;
-                float4 part[kMostSplits];
+        if (start < items) add_up_parts(p.out, item_of(start), p.w.rows, smem_sum, rank, splits, kThreads);
+        cluster_sync_relaxed();                              // no CTA ends while another reads its part
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_free(tmem, T::kColumns);
+    }
+}
+
+// One or two rows an item, cut up by the CTA that multiplies them: one launch, and x goes from global memory to what the tensor cores read without a way round.  What a CTA's columns of x
+// become stays in shared memory while its items are of the same rows.
+template <int FMT, int NT>
+struct FewTile {
+    static constexpr int kAtoms = Ms<FMT>::kAtoms, kRowsX = NT / kPartsX;
+    static constexpr int kBytesW = kRowsW * 128, kBytesS = kAtoms * 512, kStageBytes = (kBytesW + kBytesS + 1023) / 1024 * 1024, kStages = 6;
+    static constexpr int kRecord = (kBytesS + NT * 128 + 1023) / 1024 * 1024;
+    static constexpr int kHeld = 88 * 1024 / kRecord;                         // pieces of 256 columns of x
+    static constexpr int kSumColumns = 32, kScaleColumns = kAtoms * 4 * 2, kScales = 6;      // scales in tensor memory: of kScales stages
+    static constexpr int kColumns = 512;
+    static constexpr int kBytesSum = kRowsX * kRowsW * 4;
+    static constexpr int kSmem = kStages * kStageBytes + kHeld * kRecord + kBytesSum + 1024;
+    static_assert(kSmem >= 116 * 1024 && kSmem <= 216 * 1024 && kStages <= kScales && 2 * kSumColumns + kScales * kScaleColumns <= kColumns && NT <= 16);
+};
+constexpr int kFewWarps = 10, kFewThreads = 32 * kFewWarps, kCutters = 8;        // loader, issuer, eight that cut x up, four of which take the results
+
+struct FewArgs {
+    const void* x;
+    long long x_rows, ldx;
+    const int* tokens;
+    bool wide;                                   // x in pieces of 16 bytes
+    MsMatrix w;
+    Groups groups;
+    long long k;
+    int tiles_n, k_tiles;
+    Epilogue out;
+    unsigned loads;
+};
+
+template <typename XT, int FMT, int NT>
+__global__ void __launch_bounds__(kFewThreads, 1) tcq_ms_grouped_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ FewArgs p) {
+    using T = FewTile<FMT, NT>;
+    extern __shared__ uint8_t raw[];
+    __shared__ GroupPlan plan;
+    __shared__ uint64_t full[T::kStages], empty[T::kStages], sum_full[2], sum_empty[2], x_there, drained;
+    __shared__ uint32_t tmem_at, most[2][T::kRowsX][kCutters];
+    __shared__ unsigned int gave_up;
+    const uint32_t smem = (smem_u32(raw) + 1023) & ~1023u, smem_x = smem + T::kStages * T::kStageBytes, smem_sum = smem_x + T::kHeld * T::kRecord;
+    float* const sums = reinterpret_cast<float*>(raw + (smem_sum - smem_u32(raw)));
+    const int warp = __shfl_sync(0xFFFFFFFFu, int(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank(), splits = cluster_size();
+    const int first = int(uint32_t(p.k_tiles) * rank / splits), last = int(uint32_t(p.k_tiles) * (rank + 1) / splits);      // (at most 2^16 times 8)
+    const int start = blockIdx.x / splits, clusters = gridDim.x / splits;
+    const long long atoms = (long long)p.k_tiles * T::kAtoms;
+
+    const auto load = [&](uint32_t s, const GroupItem& t, int kt) {
+        const uint32_t to = smem + s * T::kStageBytes, bar = smem_u32(&full[s]);
+        mbar_expect(bar, T::kBytesW + T::kBytesS);
+        tma_load(to, &map_w, kt * 128, int(t.group * p.w.rows + t.tn * kRowsW), bar);
+        bulk_load(to + T::kBytesW, p.w.scales + (((long long)t.group * p.tiles_n + t.tn) * atoms + (long long)kt * T::kAtoms) * 512, T::kBytesS, bar);
+    };
+    const int runs = (last - first) * 64;                // of four columns of a row that this CTA has: whole warps
+    constexpr int kRun = 4, kRuns = 4, kApart = 32 * kCutters;                    // a thread takes four of them at a time, kApart apart: their loads are in flight together
+    // Four columns of x's row `token` (one that x has not: NaN), zeros behind the last column.  Loads stay where they stand.
+    const auto fetch = [&](int token, int j, float (&v)[kRun]) {
+        const int q = j >= runs ? 1 : 0;
+        const long long c0 = (long long)first * kMsTileK + 4 * (j - q * runs);
+        const XT* const from = static_cast<const XT*>(p.x) + token * p.ldx + c0;
+        if (token < 0 || token >= p.x_rows) {
+            v[0] = v[1] = v[2] = v[3] = __uint_as_float(0x7FC00000u);
+        } else if (p.wide && c0 + 4 <= p.k) {
+            uint2 u;
+            asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(u.x), "=r"(u.y) : "l"(from));
 #pragma unroll
-                for (uint32_t q = 0; q < kMostSplits; ++q)
-                    if (q < splits) part[q] = ld_cluster_f32x4(smem_sum + 16 * i, q);
-                float4 f = part[0];
+            for (int h = 0; h < 4; ++h) v[h] = to_f32<XT>(reinterpret_cast<const XT*>(&u)[h]);
+        } else {
 #pragma unroll
-                for (uint32_t q = 1; q < kMostSplits; ++q)
-                    if (q < splits) f = make_float4(f.x + part[q].x, f.y + part[q].y, f.z + part[q].z, f.w + part[q].w);
-                float h[4] = {f.x, f.y, f.z, f.w};
-                if (p.out.bias != nullptr)
+            for (int h = 0; h < 4; ++h) v[h] = c0 + h < p.k ? to_f32<XT>(from[h]) : 0.0f;
+        }
+    };
+    float v[kRuns][kRun];
+    int token[T::kRowsX] = {};                           // x's rows of the item's rows
+    const auto fetch_tokens = [&](int row0, int rows) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (r + j < p.w.rows) h[j] += load_as_f32(p.out.bias, p.out.bias_dtype, (long long)t.group * p.w.rows + r + j);
-                finish_four(p.out, h, t.row0 + i / (kRowsW / 4), r, p.w.rows);
+        for (int q = 0; q < T::kRowsX; ++q) token[q] = p.tokens != nullptr && q < rows ? __ldg(p.tokens + row0 + q) : row0 + q;
+    };
+    const auto fetch_all = [&](int j0, int all) {
+#pragma unroll
+        for (int u = 0; u < kRuns; ++u)
+            if (j0 + u * kApart < all) fetch(token[j0 + u * kApart >= runs ? T::kRowsX - 1 : 0], j0 + u * kApart, v[u]);
+    };
+    // One group: whose rows they are is known, and x is on its way before the barriers are there.
+    const bool early = p.groups.offsets == nullptr && start < p.tiles_n;
+    if (early && warp >= 2) {
+        fetch_tokens(0, p.groups.rows);
+        fetch_all(int(threadIdx.x) - 64, min(p.groups.rows, T::kRowsX) * runs);
+    }
+    if (warp == 0) {
+        if (elect_one()) {
+            gave_up = 0;
+            for (int s = 0; s < T::kStages; ++s) { mbar_init(smem_u32(&full[s]), 1); mbar_init(smem_u32(&empty[s]), 1); }
+            for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&sum_full[s]), 1); mbar_init(smem_u32(&sum_empty[s]), 4); }
+            mbar_init(smem_u32(&x_there), kCutters);
+            mbar_init(smem_u32(&drained), 1);
+            asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
+        }
+        __syncwarp();
+        plan_groups(p.groups, T::kRowsX, plan);
+    }
+    if (warp == 1) tmem_alloc(smem_u32(&tmem_at), T::kColumns);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_at, tmem_scales = tmem + 2 * T::kSumColumns;
+    const int items = plan.tile[p.groups.groups] * p.tiles_n;
+    const auto item_of = [&](int i) { return group_item(plan, p.groups.groups, p.tiles_n, T::kRowsX, i); };
+
+    if (warp == 0) {
+        // ---- loads; the warp stays together, one lane issues
+        const bool one = elect_one();
+        uint32_t s = 0, phase = 1, loaded = 0;           // (the first wait for a stage is for the phase before the first)
+        unsigned left = p.loads;
+        bool ok = true;
+        for (int i = start; i < items && ok; i += clusters) {
+            const GroupItem t = item_of(i);
+            for (int kt = first; kt < last; ++kt) {
+                ok = still_waits(left-- > 0, smem_u32(&empty[s]), phase, &gave_up);      // every lane has seen this phase before the next can begin
+                if (!ok) break;
+                if (one) load(s, t, kt);
+                __syncwarp();
+                if (++s == T::kStages) { s = 0; phase ^= 1; }
+                if (loaded < T::kStages) ++loaded;
             }
         }
-        cluster_sync();                                      // no CTA ends while another reads its part
+        wait_for_loads<T::kStages>(full, s, phase, loaded);
+    } else if (warp == 1) {
+        // ---- products; likewise
+        constexpr uint32_t kIdesc = 1u << 7 | 1u << 10 | (FMT == kMxfp4 ? 1u : 0u) << 23 | 1u << 27;
+        const bool one = elect_one();
+        uint32_t s = 0, phase = 0;
+        int n = 0, tile = -1, cut = 0;                       // rows of x that are there; how often x has been cut up
+        bool ok = true;
+        for (int i = start; i < items && ok; i += clusters, ++n) {
+            const GroupItem t = item_of(i);
+            const uint32_t idesc0 = kIdesc | uint32_t((t.rows * kPartsX + 7) / 8) << 17;
+            const int buf = n & 1;
+            if (n >= 2) ok = mbar_wait(smem_u32(&sum_empty[buf]), uint32_t(n / 2 - 1) & 1, &gave_up);
+            if (t.tile != tile) {
+                ok = ok && mbar_wait(smem_u32(&x_there), uint32_t(cut) & 1, &gave_up);
+                ++cut;
+                tile = t.tile;
+            }
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t d = tmem + buf * T::kSumColumns;
+            for (int kt = first; kt < last; ++kt) {
+                ok = mbar_wait(smem_u32(&full[s]), phase, &gave_up);
+                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t at = smem + s * T::kStageBytes, x = smem_x + (kt - first) * T::kRecord, sw = tmem_scales + s * T::kScaleColumns, sx = sw + T::kAtoms * 4;
+                const uint64_t dw = desc_rows128(at), dx = desc_rows128(x), ds = desc_rows16(at + T::kBytesW), dsx = desc_rows16(x + NT * 128);
+                if (one) {
+#pragma unroll
+                    for (int j = 0; j < T::kAtoms; ++j) {
+                        tc_copy_scales(sw + 4 * j, ds + 32 * j);
+                        tc_copy_scales(sx + 4 * j, dsx + 32 * j);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {            // 64 columns: 32 bytes of a row, one word of scales (nvfp4) or half a word (mxfp4)
+                        const int atom = FMT == kNvfp4 ? j : j / 2;
+                        const uint32_t id = FMT == kNvfp4 ? 0u : 2u * (j % 2);
+                        mma_block_scaled<FMT>(d, dw + 2 * j, dx + 2 * j, idesc0 | id << 4 | id << 29, sw + 4 * atom, sx + 4 * atom, kt > first || j > 0);
+                    }
+                    tc_commit(smem_u32(&empty[s]));
+                }
+                __syncwarp();
+                if (++s == T::kStages) { s = 0; phase ^= 1; }
+            }
+            if (ok && one) tc_commit(smem_u32(&sum_full[buf]));
+            __syncwarp();
+        }
+        if (!ok) {                                           // what was issued ends before the tensor memory goes
+            if (one) tc_commit(smem_u32(&drained));
+            __syncwarp();
+            for (long long t0 = clock64(); !mbar_try_wait(smem_u32(&drained), 0) && clock64() - t0 < kMbarWaitCycles;) {}
+        }
+    } else {
+        // ---- x, by all eight warps, four columns a thread; results, by the first four: lanes are 32 rows of W, so that a store is 32 neighbours in y
+        constexpr int kLanes = Ms<FMT>::kBlock / kRun;                            // that share a block
+        const int id = threadIdx.x - 64, quarter = warp & 3;
+        const bool takes = warp < 6;
+        float fx[T::kRowsX];
+        int n = 0, tile = -1, cut = 0;
+        bool ok = true;
+        for (int i = start; i < items; i += clusters, ++n) {
+            const GroupItem t = item_of(i);
+            const int buf = n & 1;
+            if (t.tile != tile) {
+                tile = t.tile;                               // (every warp here has waited for the sums of the item before: its x is no longer read)
+                const int all = t.rows * runs;
+                int base[T::kRowsX] = {};                    // nvfp4: exponent of the scale of this CTA's columns of each row
+                if (i != start || !early) {
+                    fetch_tokens(t.row0, t.rows);
+                    fetch_all(id, all);
+                }
+                if constexpr (FMT == kNvfp4) {
+                    uint32_t m[T::kRowsX] = {};              // the largest finite magnitudes
+#pragma unroll 1
+                    for (int j0 = id; j0 < all; j0 += kRuns * kApart) {
+                        if (j0 != id) fetch_all(j0, all);
+#pragma unroll
+                        for (int u = 0; u < kRuns; ++u) {
+                            const int j = j0 + u * kApart;
+                            uint32_t r = 0;
+#pragma unroll
+                            for (int h = 0; h < kRun; ++h) {
+                                const uint32_t b = __float_as_uint(v[u][h]) & 0x7FFFFFFFu;
+                                r = max(r, b < 0x7F800000u ? b : 0u);
+                            }
+#pragma unroll
+                            for (int q = 0; q < T::kRowsX; ++q)
+                                if (j >= q * runs && j < min(all, (q + 1) * runs)) m[q] = max(m[q], r);
+                        }
+                    }
+                    if (all > kRuns * kApart) fetch_all(id, all);
+#pragma unroll
+                    for (int q = 0; q < T::kRowsX; ++q) {
+                        m[q] = __reduce_max_sync(0xFFFFFFFFu, m[q]);
+                        if (lane == 0) most[cut & 1][q][warp - 2] = m[q];        // (two turns of them: who writes these has seen that all have read the ones before)
+                    }
+                    asm volatile("bar.sync 1, %0;" ::"n"(kApart) : "memory");
+#pragma unroll
+                    for (int q = 0; q < T::kRowsX; ++q) {
+#pragma unroll
+                        for (int h = 0; h < kCutters; ++h) m[q] = max(m[q], most[cut & 1][q][h]);
+                        base[q] = max(first_exponent(m[q]) - 8, -126);           // the largest block's scale is 2^8
+                        fx[q] = pow2f(base[q]);
+                    }
+                }
+                ++cut;
+                // (as little code as there may be: a small call is over before code that is run once has been fetched)
+#pragma unroll 1
+                for (int j0 = id; j0 < all; j0 += kRuns * kApart) {
+                    if (j0 != id) fetch_all(j0, all);
+#pragma unroll 1
+                    for (int u = 0; u < kRuns; ++u) {
+                        const int j = j0 + u * kApart, q = j >= runs ? 1 : 0, run = j - q * runs;
+                        if (j >= all) break;
+                        uint32_t m = largest<kRun>(v[0]);
+#pragma unroll
+                        for (int d = 1; d < kLanes; d *= 2) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+                        const bool nan = m >= 0x7F800000u;
+                        const int of_row = q ? base[T::kRowsX - 1] : base[0], from = nan ? 0 : block_exponent<FMT>(m, of_row), block = (run & 63) / kLanes;
+                        const Up up(from + of_row);
+                        const TwoColumns lo = two_columns(nan ? 0.0f : up(v[0][0]), nan ? 0.0f : up(v[0][1])), hi = two_columns(nan ? 0.0f : up(v[0][2]), nan ? 0.0f : up(v[0][3]));
+                        const uint32_t record = smem_x + run / 64 * T::kRecord;
+#pragma unroll
+                        for (int part = 0; part < kPartsX; ++part) {
+                            const int c = q * kPartsX + part, byte = (5 - part) / 2;
+                            bool gone;
+                            const uint32_t scale = part_scale<FMT>(from, nan, part, gone);
+                            const uint32_t codes = __byte_perm(of_part(lo, part), of_part(hi, part), byte | (4 + byte) << 4);
+                            asm volatile("st.shared.u16 [%0], %1;" ::"r"(record + c * 128 + ((((run & 63) >> 3) ^ (c & 7)) << 4) + 2 * (run & 7)), "h"(uint16_t(gone ? 0u : codes)) : "memory");
+                            if (lane % kLanes == 0)
+                                asm volatile("st.shared.u8 [%0], %1;" ::"r"(record + NT * 128 + c * 16 + (block / 4) * 512 + (block & 3)), "r"(scale) : "memory");
+                        }
+#pragma unroll
+                        for (int h = 0; h + 1 < kRuns; ++h)
+#pragma unroll
+                            for (int f = 0; f < kRun; ++f) v[h][f] = v[h + 1][f];     // the next run's
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&x_there));
+            }
+            if (!takes) {
+                ok = still_waits(ok, smem_u32(&sum_full[buf]), uint32_t(n / 2) & 1, &gave_up);
+                continue;
+            }
+            const long long r = (long long)t.tn * kRowsW + 32 * quarter + lane;
+            const bool there = r < p.w.rows;
+            const long long column = (long long)t.group * p.w.rows + r;
+            const float fw = FMT == kNvfp4 && there ? __ldg(p.w.row_scale + column) : 1.0f;
+            const float bias = p.out.bias != nullptr && there ? load_as_f32(p.out.bias, p.out.bias_dtype, column) : 0.0f;
+            ok = still_waits(ok, smem_u32(&sum_full[buf]), uint32_t(n / 2) & 1, &gave_up);
+            tc_fence_after();
+            uint32_t sum_of[NT];
+            tmem_load<NT>(tmem + buf * T::kSumColumns + (uint32_t(32 * quarter) << 16), sum_of);
+            tmem_wait_ld();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sum_empty[buf]));
+            float h[T::kRowsX];
+#pragma unroll
+            for (int q = 0; q < T::kRowsX; ++q) {
+                float sum = __uint_as_float(sum_of[q * kPartsX + kPartsX - 1]);
+#pragma unroll
+                for (int part = kPartsX - 2; part >= 0; --part) sum += __uint_as_float(sum_of[q * kPartsX + part]);   // smallest first
+                if constexpr (FMT == kNvfp4) sum = sum * inner_part(fw) * fx[q] * outer_part(fw);
+                h[q] = ok ? sum : __uint_as_float(0x7FC00000u);
+                if (splits > 1) sums[q * kRowsW + 32 * quarter + lane] = h[q];
+                else h[q] += bias;
+            }
+            if (splits == 1) finish_rows(p.out, h, t.row0, t.rows, r, there);
+        }
+    }
+    __syncwarp();
+    if (splits > 1) {                                        // one item a cluster: add up the parts of it, four neighbours a thread
+        cluster_sync();
+        if (start < items) add_up_parts(p.out, item_of(start), p.w.rows, smem_sum, rank, splits, kFewThreads);
+        cluster_sync_relaxed();                              // no CTA ends while another reads its part
     }
     tc_fence_before();
     __syncthreads();
@@ -449,6 +797,13 @@ cudaError_t launch_parts(const GroupedCall& c, const PartsArgs& p, cudaStream_t 
     if (c.fmt == kNvfp4) tcq_ms_row_parts_kernel<T, kNvfp4><<<grid, threads, 0, stream>>>(p);
     else tcq_ms_row_parts_kernel<T, kMxfp4><<<grid, threads, 0, stream>>>(p);
     return cudaGetLastError();
+}
+
+// How many CTAs share the columns of an item: as many as leave each an SM of its own, and two pieces of 256 columns or more.
+int splits_for(MostClusters& kept, const void* kernel, int threads, size_t smem, long long items, int k_tiles) {
+    int splits = 1;
+    while (splits < kMostSplits && splits * 4 <= k_tiles && items <= ms_most_clusters(kept, kernel, threads, smem, 1, splits * 2)) splits *= 2;
+    return splits;
 }
 
 template <int FMT, int NT>
@@ -476,9 +831,7 @@ cudaError_t launch(const GroupedCall& c, void* ws, cudaStream_t stream) {
     if (err != cudaSuccess) return err;
     const GroupedArgs p{c.w, c.groups, int((n + kRowsW - 1) / kRowsW), k_tiles, records, static_cast<const float*>(ws), c.out, c.loads};
     const long long items = tiles * p.tiles_n;
-    int splits = 1;
-    while (splits < kMostSplits && splits * 4 <= k_tiles &&
-           items <= ms_most_clusters(kept, reinterpret_cast<const void*>(kernel), kThreads, T::kSmem, 1, splits * 2)) splits *= 2;
+    const int splits = splits_for(kept, reinterpret_cast<const void*>(kernel), kThreads, T::kSmem, items, k_tiles);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(splits > 1 ? items * splits : std::min<long long>(items, ms_sm_count())));
     cfg.blockDim = dim3(kThreads);
@@ -493,6 +846,54 @@ cudaError_t launch(const GroupedCall& c, void* ws, cudaStream_t stream) {
     cfg.attrs = attrs;
     cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, kernel, map_w, p);
+}
+
+template <typename XT, int FMT, int NT>
+cudaError_t launch_few(const GroupedCall& c, cudaStream_t stream) {
+    using T = FewTile<FMT, NT>;
+    const auto kernel = tcq_ms_grouped_few_kernel<XT, FMT, NT>;
+    static std::atomic<bool> ready[64];
+    static MostClusters kept;
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
+    if (err != cudaSuccess) return err;
+    if (dev >= 64 || !ready[dev]) {
+        if ((err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem)) != cudaSuccess) return err;
+        if (dev < 64) ready[dev] = true;
+    }
+    CUtensorMap map_w;
+    const long long pitch = ms_pitch(c.k), n = c.w.rows;
+    if ((err = make_byte_map(&map_w, c.w.codes, pitch, n * c.groups.groups, pitch, kRowsW)) != cudaSuccess) return err;
+    const FewArgs p{c.x, c.x_rows, c.ldx, c.tokens, ms_rows_aligned(c.x, c.ldx), c.w, c.groups, c.k, int((n + kRowsW - 1) / kRowsW), int(ms_tiles_k(c.k)), c.out, c.loads};
+    const long long items = most_tiles(c.groups.rows, c.groups.groups, T::kRowsX) * p.tiles_n;
+    const int splits = splits_for(kept, reinterpret_cast<const void*>(kernel), kFewThreads, T::kSmem, items, p.k_tiles);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(splits > 1 ? items * splits : std::min<long long>(items, ms_sm_count())));
+    cfg.blockDim = dim3(kFewThreads);
+    cfg.dynamicSmemBytes = T::kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = unsigned(splits);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, map_w, p);
+}
+
+// Whether x is cut up where it is multiplied: one or two rows an item, its columns held by a CTA whatever the split, and few enough items, or only those of the same rows.
+bool cut_in_place(long long rows, long long groups, long long n, long long k, int fmt) {
+    const int nt = columns_for(rows, groups);
+    if (nt > 16) return false;
+    const int per = nt / kPartsX, held = fmt == kNvfp4 ? (nt == 8 ? FewTile<kNvfp4, 8>::kHeld : FewTile<kNvfp4, 16>::kHeld) : (nt == 8 ? FewTile<kMxfp4, 8>::kHeld : FewTile<kMxfp4, 16>::kHeld);
+    return ms_tiles_k(k) <= held && (rows <= per || most_tiles(rows, groups, per) * ((n + kRowsW - 1) / kRowsW) <= 2 * ms_sm_count());
+}
+
+template <int FMT>
+cudaError_t launch_cut(const GroupedCall& c, cudaStream_t stream) {
+    const bool eight = columns_for(c.groups.rows, c.groups.groups) == 8;
+    if (c.dtype == kF16) return eight ? launch_few<__half, FMT, 8>(c, stream) : launch_few<__half, FMT, 16>(c, stream);
+    return eight ? launch_few<__nv_bfloat16, FMT, 8>(c, stream) : launch_few<__nv_bfloat16, FMT, 16>(c, stream);
 }
 
 template <int FMT>
@@ -512,8 +913,8 @@ cudaError_t launch_nt(const GroupedCall& c, void* ws, cudaStream_t stream) {
 static bool many_rows(long long rows, long long groups, int dtype, int fmt) { return rows > 90 * std::min(groups, rows) && ms_grouped_many_takes(dtype, fmt); }
 
 size_t ms_grouped_workspace_bytes(long long rows, long long groups, long long n, long long k, int dtype, int fmt, bool in_order) {
-    (void)n;
     if (many_rows(rows, groups, dtype, fmt)) return in_order ? 0 : ms_grouped_many_workspace_bytes(rows, k);
+    if (cut_in_place(rows, groups, n, k, fmt)) return 0;
     const int nt = columns_for(rows, groups), per = nt / kPartsX;
     const long long tiles = most_tiles(rows, groups, per);
     return size_t((tiles * per * 4 + 255) / 256 * 256) + size_t(tiles) * size_t(ms_tiles_k(k)) * record_bytes(fmt, nt);
@@ -521,6 +922,7 @@ size_t ms_grouped_workspace_bytes(long long rows, long long groups, long long n,
 
 cudaError_t launch_ms_grouped(const GroupedCall& c, void* ws, cudaStream_t stream) {
     if (many_rows(c.groups.rows, c.groups.groups, c.dtype, c.fmt)) return launch_ms_grouped_many(c, ws, stream);
+    if (cut_in_place(c.groups.rows, c.groups.groups, c.w.rows, c.k, c.fmt)) return c.fmt == kNvfp4 ? launch_cut<kNvfp4>(c, stream) : launch_cut<kMxfp4>(c, stream);
     return c.fmt == kNvfp4 ? launch_nt<kNvfp4>(c, ws, stream) : launch_nt<kMxfp4>(c, ws, stream);
 }
 

@@ -30,31 +30,52 @@ __device__ __forceinline__ void plan_groups(const Groups& g, int per, GroupPlan&
         __syncwarp();
         return;
     }
-    int most = 0;                                        // of the offsets before these 32
-    for (int at = 0; at <= g.groups; at += 32) {
-        int v = at + lane <= g.groups ? min(max(__ldg(g.offsets + at + lane), 0), g.rows) : 0;
+    int most = 0, sum = 0;                               // of the offsets and the tiles before these
+    for (int at = 0; at <= g.groups; at += 128) {        // a lane has four neighbours, whose loads are in flight together
+        const int mine = at + 4 * lane;
+        int v[5];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = mine + q <= g.groups ? __ldg(g.offsets + mine + q) : 0;
+        v[4] = at + 128 <= g.groups ? __ldg(g.offsets + at + 128) : 0;            // what the last lane needs of the next ones
+#pragma unroll
+        for (int q = 0; q < 5; ++q) v[q] = min(max(v[q], 0), g.rows);
+#pragma unroll
+        for (int q = 1; q < 4; ++q) v[q] = max(v[q], v[q - 1]);
+        int before = v[3];
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
-            const int other = __shfl_up_sync(0xFFFFFFFFu, v, d);
-            if (lane >= d) v = max(v, other);
+            const int other = __shfl_up_sync(0xFFFFFFFFu, before, d);
+            if (lane >= d) before = max(before, other);
         }
-        v = max(v, most);
-        if (at + lane <= g.groups) plan.begin[at + lane] = v;
-        most = __shfl_sync(0xFFFFFFFFu, v, 31);
-    }
-    __syncwarp();
-    int sum = 0;
-    for (int at = 0; at <= g.groups; at += 32) {
-        const int i = at + lane;
-        const int mine = i < g.groups ? (plan.begin[i + 1] - plan.begin[i] + per - 1) / per : 0;
-        int v = mine;
+        const int last = __shfl_sync(0xFFFFFFFFu, before, 31);
+        before = __shfl_up_sync(0xFFFFFFFFu, before, 1);
+        before = max(lane == 0 ? 0 : before, most);
+        most = max(most, last);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = max(v[q], before);
+        const int next = __shfl_down_sync(0xFFFFFFFFu, v[0], 1);
+        v[4] = lane == 31 ? max(v[4], v[3]) : next;
+        int tiles[4], all = 0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            tiles[q] = all;
+            all += mine + q < g.groups ? (v[q + 1] - v[q] + per - 1) / per : 0;
+        }
+        int first = all;
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
-            const int other = __shfl_up_sync(0xFFFFFFFFu, v, d);
-            if (lane >= d) v += other;
+            const int other = __shfl_up_sync(0xFFFFFFFFu, first, d);
+            if (lane >= d) first += other;
         }
-        if (i <= g.groups) plan.tile[i] = sum + v - mine;
-        sum += __shfl_sync(0xFFFFFFFFu, v, 31);
+        const int end = __shfl_sync(0xFFFFFFFFu, first, 31);
+        first += sum - all;
+        sum += end;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (mine + q <= g.groups) {
+                plan.begin[mine + q] = v[q];
+                plan.tile[mine + q] = first + tiles[q];
+            }
     }
     __syncwarp();
 }
@@ -86,7 +107,7 @@ __device__ __forceinline__ GroupItem group_item(const GroupPlan& plan, int group
     return t;
 }
 
-// No more tiles than this, whatever the offsets.
-inline long long most_tiles(long long rows, long long groups, int per) { return rows / per + (groups < rows ? groups : rows); }
+// No more tiles than this, whatever the offsets: every group that has rows may have all but one of another tile's.
+inline long long most_tiles(long long rows, long long groups, int per) { return (rows + (groups < rows ? groups : rows) * (per - 1)) / per; }
 
 }  // namespace tcq

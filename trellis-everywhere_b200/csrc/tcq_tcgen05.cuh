@@ -102,6 +102,10 @@ __device__ __forceinline__ uint32_t cluster_size() { uint32_t r; asm volatile("m
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The same for threads that have read all that they will read of one another's memory, and written nothing: no store is waited for.
+__device__ __forceinline__ void cluster_sync_relaxed() {
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
 // The address of this place in another CTA of the cluster.
 __device__ __forceinline__ uint32_t map_rank(uint32_t smem, uint32_t rank) {
     uint32_t a;
