@@ -18,6 +18,7 @@ All tensors live on one CUDA device; calls are queued on its current stream.  No
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
@@ -107,6 +108,21 @@ def expert(w: ExpertMatrices, i: int) -> Microscaled:
 
 def _check_e(w: ExpertMatrices, name: str) -> int:
     """The CUDA device's number of well-formed matrices; raises otherwise (the kernels trust their sizes)."""
+    if isinstance(w, ExpertMatrices):                        # one short pass where all is well
+        codes, scales, row, (e, n, k), fmt = w
+        dev = codes.get_device()
+        if (dev >= 0 and codes.dtype is torch.uint8 and scales.dtype is torch.uint8 and scales.get_device() == dev and codes.shape == (e, n, 16 * -(-k // 32))
+                and codes.is_contiguous() and scales.is_contiguous()
+                and (row.get_device() == dev and row.dtype is torch.float32 and row.shape == (e, n) and row.is_contiguous()
+                     and scales.shape == (e, -(-n // 128), 4 * -(-k // 256), 32, 4, 4) if fmt == "nvfp4" and row is not None
+                     else fmt == "mxfp4" and row is None and scales.shape == (e, -(-n // 128), 2 * -(-k // 256), 32, 4, 4))):
+            if row is not None:
+                _no_gradient(row, f"{name}.row_scale")
+            return dev
+    return _refuse_e(w, name)
+
+
+def _refuse_e(w, name: str) -> int:
     if not isinstance(w, ExpertMatrices):
         raise ValueError(f"{name} must be ExpertMatrices, got {type(w).__name__}")
     _check_fmt(w.fmt)
@@ -122,10 +138,8 @@ def _check_e(w: ExpertMatrices, name: str) -> int:
             raise ValueError(f"{name}.{part} must be a contiguous {dtype} {list(shape)} tensor on {dev}")
     if w.row_scale is not None:
         _no_gradient(w.row_scale, f"{name}.row_scale")
-    if dev.type != "cuda":
-        _cuda_device()
-        raise ValueError(f"{name} must be on a CUDA device")
-    return dev.index
+    _cuda_device()
+    raise ValueError(f"{name} must be on a CUDA device")
 
 
 def _check_ints(t: torch.Tensor, name: str, shape: Tuple[int, ...], dev: int) -> None:
@@ -158,11 +172,16 @@ def route(logits: torch.Tensor, top_k: int, score: str = "softmax", normalize: b
     places = torch.empty_strided((t, top_k), (top_k, 1), dtype=torch.int32, device=dev)
     tokens = torch.empty_strided((t * top_k,), (1,), dtype=torch.int32, device=dev)
     offsets = torch.empty_strided((e + 1,), (1,), dtype=torch.int32, device=dev)
-    size = _lib.lib().tcq_route_workspace_bytes(t, e)
-    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    size = _route_workspace(t, e)
+    ws = torch.empty_strided((size,), (1,), dtype=torch.uint8, device=dev) if size else None
     _launch(dev.index, "tcq_route", logits.data_ptr(), _DTYPES[logits.dtype], t, _pitch(logits), e, top_k, SCORES[score], int(normalize), weights.data_ptr(),
             chosen.data_ptr(), places.data_ptr(), tokens.data_ptr(), offsets.data_ptr(), _ptr(ws), size)
     return Routing(weights, chosen, places, tokens, offsets)
+
+
+@functools.lru_cache(maxsize=4096)
+def _route_workspace(t: int, e: int) -> int:
+    return _lib.lib().tcq_route_workspace_bytes(t, e)
 
 
 def grouped_linear(x: torch.Tensor, w: ExpertMatrices, offsets: torch.Tensor, tokens: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,

@@ -25,6 +25,7 @@ forward, is refused.
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import NamedTuple, Optional, Tuple
 
@@ -274,10 +275,15 @@ def _check_bias(bias: Optional[torch.Tensor], shape: Tuple[int, ...], device) ->
     return bias if bias.is_contiguous() else bias.detach().contiguous()
 
 
+@functools.lru_cache(maxsize=4096)
+def _grouped_workspace(rows: int, groups: int, n: int, k: int, dt: int, f: int, in_order: bool) -> int:
+    return _lib.lib().tcq_ms_grouped_linear_workspace_bytes(rows, groups, n, k, dt, f, in_order)
+
+
 def _grouped(dev: int, flat: torch.Tensor, tokens, offsets, groups: int, rows: int, codes, scales, row, n: int, k: int, fmt: str, bias, act: int, residual, y: torch.Tensor) -> None:
     """``tcq_ms_grouped_linear`` with its workspace, given back when the call is queued: the stream's later work comes after it."""
     dt, f, at, pitch = _DTYPES[flat.dtype], FORMATS[fmt], flat.data_ptr(), _pitch(flat)
-    size = _lib.lib().tcq_ms_grouped_linear_workspace_bytes(rows, groups, n, k, dt, f, tokens is None and not (at % 16 or pitch % 8))
+    size = _grouped_workspace(rows, groups, n, k, dt, f, tokens is None and not (at % 16 or pitch % 8))
     ws = torch.empty(size, dtype=torch.uint8, device=flat.device) if size else None
     _launch(dev, "tcq_ms_grouped_linear", at, dt, flat.shape[0], pitch, _ptr(tokens), _ptr(offsets), groups, rows, codes.data_ptr(), scales.data_ptr(),
             _ptr(row), n, k, f, _ptr(bias), 0 if bias is None else _DTYPES[bias.dtype], act, _ptr(residual), 0 if residual is None else _pitch(residual),
