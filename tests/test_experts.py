@@ -84,6 +84,22 @@ def test_arguments():
         torch.zeros(3) + stack()
 
 
+def test_the_short_way_leaves_what_it_does_not_take():
+    """On the CPU it takes nothing: the Python functions say what is wrong, with it as without it."""
+    short = _lib.short()
+    assert short, "tcq_torch.so is not built"
+    x, w, e = torch.zeros(2, 32, dtype=torch.bfloat16), matrix(), stack()
+    r = experts.Routing(torch.ones(2, 1), *[torch.zeros(2, 1, dtype=torch.int32)] * 4)
+    for got in (short.linear(x, w, None, "relu", None), short.linear(None, w, None, "relu", None), short.linear(x, (1, 2), None, None, x), short.linear(x, w, None, "tanh", None),
+                short.linear(x, w), short.grouped_linear(x, e, torch.zeros(4, dtype=torch.int32), None, None, None, None), short.grouped_linear(x, w, None, None, None, None, None),
+                short.grouped_linear(), short.route(torch.zeros(2, 4), 2, "softmax", True), short.route(torch.zeros(2, 4), 1 << 70, "softmax", True), short.route(3, 2, "softmax", True),
+                short.combine(x, r, None, None), short.combine(x, None, None, None), short.combine(x, r, None, 7),
+                short.linear(x, w._replace(shape=(1 << 80, 32)), None, "relu", None), short.linear(x, w._replace(shape=("a", 32)), None, "relu", None)):
+        assert got is None
+    with pytest.raises(TypeError):
+        short.bind(1, 2)
+
+
 # ------------------------------------------------------------------------------------------------ the C ABI
 BAD_COUNT, NULL, MISALIGNED, WORKSPACE, BAD, FORMAT = -3, -4, -5, -6, -8, -12
 

@@ -7,11 +7,15 @@ codec fails with an error that says how to build it.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import subprocess
+import sys
 
 _CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "csrc")
 LIB_PATH = os.path.join(_CSRC, "libtcq_b200.so")
+SHORT_PATH = os.path.join(_CSRC, "tcq_torch.so")
 
 ABI_VERSION = 7
 
@@ -71,7 +75,7 @@ class TcqError(RuntimeError):
 
 def build(verbose: bool = False, jobs: int = 8) -> str:
     """Compile the CUDA sources for sm_100a with nvcc (``make`` in ``csrc/``)."""
-    cmd = ["make", "-C", _CSRC, f"-j{jobs}", "libtcq_b200.so"]
+    cmd = ["make", "-C", _CSRC, f"-j{jobs}", "libtcq_b200.so", "tcq_torch.so", f"PYTHON={sys.executable}"]
     subprocess.check_call(cmd, stdout=None if verbose else subprocess.DEVNULL)
     return LIB_PATH
 
@@ -95,6 +99,27 @@ def lib() -> ctypes.CDLL:
             raise ImportError(f"libtcq_b200.so has ABI version {got}, this package needs {ABI_VERSION}: rebuild it")
         _lib = handle
     return _lib
+
+
+_short = None
+SHORT_BINDS = ("tcq_ms_grouped_linear_workspace_bytes", "tcq_ms_grouped_linear", "tcq_route_workspace_bytes", "tcq_route", "tcq_combine")
+
+
+def short():
+    """The extension that takes the small calls where all is well (``csrc/tcq_torch.cpp``), bound to the library; False where it was not built: the same calls then go
+    through ctypes, which takes twice as long."""
+    global _short
+    if _short is None:
+        handle = lib()
+        if os.path.exists(SHORT_PATH):
+            loader = importlib.machinery.ExtensionFileLoader("tcq_torch", SHORT_PATH)
+            module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("tcq_torch", SHORT_PATH, loader=loader))
+            loader.exec_module(module)
+            module.bind(*(ctypes.cast(getattr(handle, name), ctypes.c_void_p).value for name in SHORT_BINDS))
+            _short = module
+        else:
+            _short = False
+    return _short
 
 
 def check(code: int, what: str) -> None:

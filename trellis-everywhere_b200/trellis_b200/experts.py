@@ -156,6 +156,10 @@ def route(logits: torch.Tensor, top_k: int, score: str = "softmax", normalize: b
     ``score``: "softmax", weights exp(logit) over their sum over all experts, or with ``normalize`` over the chosen ones; "sigmoid", weights
     1 / (1 + exp(-logit)), with ``normalize`` over their sum.  In fp32.
     """
+    short = _lib.short()
+    parts = short.route(logits, top_k, score, normalize) if short else None
+    if parts is not None:
+        return Routing(*parts)
     if score not in SCORES:
         raise ValueError(f"unknown score {score!r}; expected one of {sorted(SCORES)}")
     if logits.dim() != 2:
@@ -196,6 +200,10 @@ def grouped_linear(x: torch.Tensor, w: ExpertMatrices, offsets: torch.Tensor, to
     of the largest of its block of 16 (nvfp4) or 32 (mxfp4) columns (fp16: 2^-5), and 2^-16.7 of that off at most elsewhere (nvfp4: or 2^-18.5 of the
     row's largest).  A row of x with a NaN gives NaN, one with an infinity NaN or what its sums have.  A row's result does not depend on what the others hold, and equal calls give equal results.
     """
+    short = _lib.short()
+    y = short.grouped_linear(x, w, offsets, tokens, bias, activation, dtype) if short and isinstance(w, ExpertMatrices) else None
+    if y is not None:
+        return y
     dev = _check_e(w, "w")
     e, n, k = w.shape
     act, out = _check_act(activation, n)
@@ -225,6 +233,10 @@ def combine(y: torch.Tensor, routing: Routing, residual: Optional[torch.Tensor] 
 
     ``y [rows, n]`` and ``residual [T, n]`` in fp32, fp16 or bf16; a choice without an expert adds nothing.
     """
+    short = _lib.short()
+    out = short.combine(y, routing, residual, dtype) if short else None
+    if out is not None:
+        return out
     if y.dim() != 2:
         raise ValueError(f"y must be [rows, n], got {tuple(y.shape)}")
     y = _check_x(y, "y")

@@ -231,7 +231,9 @@ def linear(x: torch.Tensor, w: Microscaled, bias: Optional[torch.Tensor] = None,
     ``experts.grouped_linear`` (bf16 x exact down to 2^-8 of a block's largest magnitude, fp16 x to 2^-5, the rest to 2^-16.7 of that; an infinity in x may give NaN where its sums have an infinity).
     """
     if bias is not None or activation is not None or residual is not None:
-        return _linear_epilogue(x, w, bias, activation, residual)
+        short = _lib.short()
+        y = short.linear(x, w, bias, activation, residual) if short and isinstance(w, Microscaled) else None
+        return _linear_epilogue(x, w, bias, activation, residual) if y is None else y
     dev = _check_q(w, "w")
     codes, scales, row, (n, k), fmt = w
     shape = x.shape
