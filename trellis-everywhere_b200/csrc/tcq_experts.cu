@@ -13,9 +13,10 @@ namespace tcq {
 
 namespace {
 
-constexpr int kOneChunk = 64;                    // tokens of the form that is one launch
-constexpr int kMostChunks = 256;
-constexpr int kWarps = 16, kThreads = 32 * kWarps;
+constexpr int kOneChunk = 32;                    // tokens of the form that is one launch: one a warp
+constexpr int kMostChunks = 148;
+constexpr int kWarps = 32, kThreads = 32 * kWarps;
+constexpr int kFewEntries = 128;                 // that one warp puts in order in less time than all count
 
 // Integers in the order of the numbers: -0 as 0, every NaN above infinity; 0 stands for -infinity, which is never chosen.
 __device__ __forceinline__ uint32_t ordered(float v) {
@@ -23,6 +24,7 @@ __device__ __forceinline__ uint32_t ordered(float v) {
     const uint32_t b = __float_as_uint(v + 0.0f);
     return v == -INFINITY ? 0u : b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float number_of(uint32_t key) { return __uint_as_float(key == 0xFFFFFFFFu ? 0x7FC00000u : key & 0x80000000u ? key & 0x7FFFFFFFu : ~key); }
 __device__ __forceinline__ float sum_of_warp(float v) {
 #pragma unroll
     for (int d = 16; d > 0; d /= 2) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
@@ -55,16 +57,11 @@ __device__ void choose(const RouteCall& c, int token) {
         for (int i = EACH - 1; i >= 0; --i)
             if (key[i] == best) at = lane + 32 * i;
         at = __reduce_min_sync(0xFFFFFFFFu, at);
-        float mine = 0.0f;
 #pragma unroll
         for (int i = 0; i < EACH; ++i)
-            if (at == uint32_t(lane + 32 * i)) {
-                mine = v[i];
-                key[i] = 0;
-            }
-        mine = __shfl_sync(0xFFFFFFFFu, mine, at & 31);
+            if (at == uint32_t(lane + 32 * i)) key[i] = 0;
         if (lane == j) {
-            value = mine;
+            value = number_of(best);
             expert = int(at);
         }
         ++found;
@@ -135,7 +132,29 @@ __device__ void place_chunk(const RouteCall& c, long long first, int entries, co
         __syncwarp();
         if (i + lane < to) {
             c.places[first + i + lane] = place;
-            if (place >= 0) c.order[place] = int((first + i + lane) / c.top);
+            if (place >= 0) c.order[place] = int(uint32_t(first + i + lane) / uint32_t(c.top));
+        }
+    }
+}
+
+// The same of few entries, by one warp: base[] counts on.
+__device__ void place_few(const RouteCall& c, long long first, int entries, int* base) {
+    const int lane = threadIdx.x & 31;
+    int all[kFewEntries / 32];                           // loads in flight together
+#pragma unroll
+    for (int u = 0; u < kFewEntries / 32; ++u) all[u] = 32 * u + lane < entries ? c.chosen[first + 32 * u + lane] : -1;
+#pragma unroll
+    for (int u = 0; u < kFewEntries / 32; ++u) {
+        if (32 * u >= entries) break;
+        const int e = all[u], i = 32 * u + lane;
+        const unsigned same = __match_any_sync(0xFFFFFFFFu, e), before = same & ((1u << lane) - 1);
+        const int place = e >= 0 ? base[e] + __popc(before) : -1;
+        __syncwarp();
+        if (e >= 0 && before == 0) base[e] += __popc(same);
+        __syncwarp();
+        if (i < entries) {
+            c.places[first + i] = place;
+            if (place >= 0) c.order[place] = int(uint32_t(first + i) / uint32_t(c.top));
         }
     }
 }
@@ -178,7 +197,12 @@ __global__ void __launch_bounds__(kThreads) tcq_route_kernel(const __grid_consta
     }
     __syncthreads();
     for (int e = threadIdx.x; e < c.experts; e += kThreads) c.offsets[e] = base[e];
-    place_chunk(c, 0, entries, base, hist);
+    if (entries <= kFewEntries) {
+        __syncthreads();                                 // offsets are read before base[] counts on
+        if (warp == 0) place_few(c, 0, entries, base);
+    } else {
+        place_chunk(c, 0, entries, base, hist);
+    }
 }
 
 // A chunk of many: its experts, and how many of each.
@@ -209,7 +233,7 @@ __global__ void __launch_bounds__(kThreads) tcq_route_place_kernel(const __grid_
     const int wide = min(kThreads, (c.experts + 31) / 32 * 32), groups = kThreads / wide, group = threadIdx.x / wide;
     for (int e = threadIdx.x % wide; e < c.experts && group < groups; e += wide) {
         int all = 0, lower = 0;
-#pragma unroll 4
+#pragma unroll 8
         for (int q = group; q < int(gridDim.x); q += groups) {
             const int n = c.counts[(long long)q * c.experts + e];
             all += n;
@@ -231,8 +255,9 @@ __global__ void __launch_bounds__(kThreads) tcq_route_place_kernel(const __grid_
     __syncthreads();
     for (int e = threadIdx.x; e < c.experts; e += kThreads) base[e] += before[e];
     __syncthreads();
-    const int t0 = blockIdx.x * chunk, t1 = min(c.tokens, t0 + chunk);
-    place_chunk(c, (long long)t0 * c.top, (t1 - t0) * c.top, base, hist);
+    const int t0 = blockIdx.x * chunk, t1 = min(c.tokens, t0 + chunk), entries = (t1 - t0) * c.top;
+    if (entries > kFewEntries) place_chunk(c, (long long)t0 * c.top, entries, base, hist);
+    else if (warp == 0) place_few(c, (long long)t0 * c.top, entries, base);
 }
 
 // Eight neighbouring numbers as they lie in memory.
@@ -242,9 +267,10 @@ __device__ __forceinline__ void to_floats(const Eight<T>& e, float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(reinterpret_cast<const T*>(e.u)[i]);
 }
-// At any address: pieces of 16 bytes that start on 16 bytes, one more than they fill, and a shift; single numbers where a piece would reach out of from .. to.  `there` of them exist.
+// At any address: pieces of 16 bytes that start on 16 bytes, one more than they fill, and a shift; single numbers where fewer than eight exist, or in the first and the last row (`inner`
+// is false), where a piece could reach out of the matrix.
 template <typename T>
-__device__ __forceinline__ Eight<T> load_eight(const T* p, bool aligned, int there, const void* from, const void* to) {
+__device__ __forceinline__ Eight<T> load_eight(const T* p, bool aligned, int there, bool inner) {
     constexpr int kPieces = sizeof(T) / 2;
     Eight<T> e;
     if (aligned) {
@@ -254,7 +280,7 @@ __device__ __forceinline__ Eight<T> load_eight(const T* p, bool aligned, int the
     }
     const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(p)) & 15u;
     const char* const base = reinterpret_cast<const char*>(p) - off;
-    if (there >= 8 && base >= from && base + 16 * (kPieces + 1) <= to) {
+    if (there >= 8 && inner) {
         uint32_t w[4 * (kPieces + 1)];
 #pragma unroll
         for (int q = 0; q <= kPieces; ++q) {
@@ -292,7 +318,7 @@ __global__ void __launch_bounds__(256, !ALIGNED ? 3 : sizeof(Y) == 2 ? 5 : 4) tc
             Eight<O> res;
             if (c.residual != nullptr && there > 0) {
                 const O* const at = static_cast<const O*>(c.residual) + token * c.ldr + c0;
-                res = load_eight<O>(at, ALIGNED, there, c.residual, static_cast<const O*>(c.residual) + (c.tokens - 1) * c.ldr + n);
+                res = load_eight<O>(at, ALIGNED, there, token > 0 && token + 1 < c.tokens);
             }
             for (int j0 = 0; j0 < c.top; j0 += 4) {
                 Eight<Y> v[4];
@@ -303,7 +329,7 @@ __global__ void __launch_bounds__(256, !ALIGNED ? 3 : sizeof(Y) == 2 ? 5 : 4) tc
                     const bool some = place >= 0 && place < c.rows && there > 0;
                     w[q] = some ? __ldg(weights + j0 + q) : 0.0f;
                     v[q] = {};
-                    if (some) v[q] = load_eight<Y>(static_cast<const Y*>(c.y) + place * c.ldy + c0, ALIGNED, there, c.y, static_cast<const Y*>(c.y) + (c.rows - 1) * c.ldy + n);
+                    if (some) v[q] = load_eight<Y>(static_cast<const Y*>(c.y) + place * c.ldy + c0, ALIGNED, there, place > 0 && place + 1 < c.rows);
                 }
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {

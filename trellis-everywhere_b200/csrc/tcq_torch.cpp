@@ -26,6 +26,9 @@ decltype(&tcq_ms_grouped_linear) grouped_linear = nullptr;
 decltype(&tcq_route_workspace_bytes) route_bytes = nullptr;
 decltype(&tcq_route) route = nullptr;
 decltype(&tcq_combine) combine = nullptr;
+decltype(&tcq_ms_linear_workspace_bytes) linear_bytes = nullptr;
+decltype(&tcq_ms_linear) ms_linear = nullptr;
+decltype(&tcq_ms_epilogue) epilogue = nullptr;
 
 int type_of(at::ScalarType t) {
     switch (t) {
@@ -123,14 +126,28 @@ bool queue_grouped(const at::Tensor& x, const Rows& r, const int32_t* tokens, co
                           c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(m.dev)).stream()) == TCQ_OK;
 }
 
-// linear(x, w, bias, activation, residual), x in 16 bits
+// fp32 x: the product, then the epilogue behind it, in place where nothing is gated.
+at::Tensor queue_fp32(const at::Tensor& x, const Rows& r, const Matrices& m, const at::Tensor* bias, int act, const at::Tensor* residual, int64_t ldr, at::IntArrayRef sizes, int64_t out) {
+    at::Tensor y = empty(sizes, at::kFloat, m.dev), h = out == m.n ? y : empty({r.rows, m.n}, at::kFloat, m.dev), ws;
+    const size_t size = linear_bytes(r.rows, m.n, m.k, TCQ_F32, m.fmt);
+    if (r.rows > 8) ws = empty({int64_t(size)}, at::kByte, m.dev);
+    const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(m.dev));
+    void* const stream = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(m.dev)).stream();
+    if (ms_linear(address(&x), TCQ_F32, r.rows, r.ld, static_cast<const uint8_t*>(address(m.codes)), static_cast<const uint8_t*>(address(m.scales)), static_cast<const float*>(address(m.row)),
+                  m.n, m.k, m.fmt, h.mutable_data_ptr(), m.n, r.rows > 8 ? ws.mutable_data_ptr() : nullptr, size, stream) != TCQ_OK ||
+        epilogue(h.const_data_ptr<float>(), r.rows, m.n, address(bias), bias ? type_of(bias->scalar_type()) : 0, act, address(residual), ldr, y.mutable_data_ptr(), TCQ_F32, out, stream) != TCQ_OK)
+        return {};
+    return y;
+}
+
+// linear(x, w, bias, activation, residual)
 PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t count) {
     HANDLE_TH_ERRORS
     Matrices m;
     const int act = count == 5 ? activation_of(a[3]) : -1;
     if (act < 0 || !usual_mode() || !matrices(a[1], false, m) || (gated(act) && m.n % 2)) Py_RETURN_NONE;
     const at::Tensor* const x = plain(a[0]);
-    if (!on(x, m.dev) || (x->scalar_type() != at::kHalf && x->scalar_type() != at::kBFloat16)) Py_RETURN_NONE;
+    if (!on(x, m.dev) || type_of(x->scalar_type()) < 0) Py_RETURN_NONE;
     const Rows r = rows_of(*x, m.k);
     if (!r.ok || r.rows == 0 || m.n == 0) Py_RETURN_NONE;
     const int64_t out = gated(act) ? m.n / 2 : m.n;
@@ -152,6 +169,11 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t count) {
     }
     c10::SmallVector<int64_t, 4> sizes(x->sizes().begin(), x->sizes().end());
     sizes.back() = out;
+    if (x->scalar_type() == at::kFloat) {
+        at::Tensor y = queue_fp32(*x, r, m, bias, act, residual, ldr, sizes, out);
+        if (!y.defined()) Py_RETURN_NONE;
+        return THPVariable_Wrap(std::move(y));
+    }
     at::Tensor y = empty(sizes, x->scalar_type(), m.dev);
     if (!queue_grouped(*x, r, nullptr, nullptr, r.rows, m, bias, act, residual, ldr, y, out)) Py_RETURN_NONE;
     return THPVariable_Wrap(std::move(y));
@@ -264,14 +286,15 @@ PyObject* py_combine(PyObject*, PyObject* const* a, Py_ssize_t count) {
     END_HANDLE_TH_ERRORS
 }
 
-// bind(address of tcq_ms_grouped_linear_workspace_bytes, tcq_ms_grouped_linear, tcq_route_workspace_bytes, tcq_route, tcq_combine)
+// bind(addresses of tcq_ms_grouped_linear_workspace_bytes, tcq_ms_grouped_linear, tcq_route_workspace_bytes, tcq_route, tcq_combine, tcq_ms_linear_workspace_bytes, tcq_ms_linear,
+// tcq_ms_epilogue)
 PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t count) {
-    if (count != 5) {
-        PyErr_SetString(PyExc_TypeError, "five addresses expected");
+    if (count != 8) {
+        PyErr_SetString(PyExc_TypeError, "eight addresses expected");
         return nullptr;
     }
-    void* at[5];
-    for (int i = 0; i < 5; ++i)
+    void* at[8];
+    for (int i = 0; i < 8; ++i)
         if ((at[i] = PyLong_AsVoidPtr(a[i])) == nullptr) {
             if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "an address is NULL");
             return nullptr;
@@ -281,6 +304,9 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t count) {
     route_bytes = reinterpret_cast<decltype(route_bytes)>(at[2]);
     route = reinterpret_cast<decltype(route)>(at[3]);
     combine = reinterpret_cast<decltype(combine)>(at[4]);
+    linear_bytes = reinterpret_cast<decltype(linear_bytes)>(at[5]);
+    ms_linear = reinterpret_cast<decltype(ms_linear)>(at[6]);
+    epilogue = reinterpret_cast<decltype(epilogue)>(at[7]);
     Py_RETURN_NONE;
 }
 

@@ -102,7 +102,8 @@ def lib() -> ctypes.CDLL:
 
 
 _short = None
-SHORT_BINDS = ("tcq_ms_grouped_linear_workspace_bytes", "tcq_ms_grouped_linear", "tcq_route_workspace_bytes", "tcq_route", "tcq_combine")
+SHORT_BINDS = ("tcq_ms_grouped_linear_workspace_bytes", "tcq_ms_grouped_linear", "tcq_route_workspace_bytes", "tcq_route", "tcq_combine", "tcq_ms_linear_workspace_bytes", "tcq_ms_linear",
+               "tcq_ms_epilogue")
 
 
 def short():
