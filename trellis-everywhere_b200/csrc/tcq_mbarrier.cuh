@@ -48,17 +48,18 @@ __device__ __forceinline__ bool mbar_wait(uint32_t mbar, uint32_t parity, volati
 __device__ __forceinline__ void mbar_arrive(uint32_t mbar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(mbar) : "memory");
 }
-// The end of a warp that fills a ring of STAGES: the last load of each of the `loaded` stages has landed, or does not come.  Nothing may be on its way to a
+// The end of a warp that fills a ring of `stages`: the last load of each of the `loaded` stages has landed, or does not come.  Nothing may be on its way to a
 // CTA's memory when the CTA ends, and a load that is late is seen to be missing (by whom it was for) only after this warp has issued its last one.
 // s, phase: the stage that would be next, and the parity of the wait for it to be empty.
-template <int STAGES>
-__device__ __forceinline__ void wait_for_loads(const uint64_t* full, uint32_t s, uint32_t phase, uint32_t loaded) {
+__device__ __forceinline__ void wait_for_loads(const uint64_t* full, uint32_t stages, uint32_t s, uint32_t phase, uint32_t loaded) {
     for (uint32_t i = 0; i < loaded; ++i) {
         if (s == 0) phase ^= 1;
-        s = s == 0 ? STAGES - 1 : s - 1;
+        s = s == 0 ? stages - 1 : s - 1;
         for (long long t0 = clock64(); !mbar_try_wait(smem_u32(&full[s]), phase ^ 1) && clock64() - t0 < kMbarWaitCycles;) {}
     }
 }
+template <int STAGES>
+__device__ __forceinline__ void wait_for_loads(const uint64_t* full, uint32_t s, uint32_t phase, uint32_t loaded) { wait_for_loads(full, STAGES, s, phase, loaded); }
 // A failure is for good: behind a phase that never completes, a wait for the phase after the next is answered by the parity of the last complete one, at once
 // and wrongly.  So a warp whose wait ran out waits no more, and gives NaN from there on; who fills a ring stops, as an announcement for a stage that is not
 // complete would be counted into its open phase.

@@ -101,22 +101,24 @@ __device__ __forceinline__ uint32_t digit_codes(float v) {
     r = (r & 0x333333u) | ((c2 << 2) & ~0x333333u);
     return (r & 0x777777u) | (~(d << 1) & ~0x777777u);
 }
-// The codes of two columns side by side: of part 5 - 2 b in byte b of `even`, of part 4 - 2 b in byte b of `odd`.
+// The codes of two columns side by side: of part 5 - 2 b in byte b of `even`, of part 4 - 2 b in byte b of `odd`.  kept: of the codes' nibbles.
 struct TwoColumns { uint32_t even, odd; };
-__device__ __forceinline__ TwoColumns two_columns(float a, float b) {
-    const uint32_t x = digit_codes(a), y = digit_codes(b);
+__device__ __forceinline__ TwoColumns two_columns(float a, float b, uint32_t kept) {
+    const uint32_t x = digit_codes(a) & kept, y = digit_codes(b) & kept;
     return {(x & 0x0F0F0Fu) | ((y << 4) & ~0x0F0F0Fu), ((x >> 4) & 0x0F0F0Fu) | (y & ~0x0F0F0Fu)};
 }
 __device__ __forceinline__ uint32_t of_part(const TwoColumns& t, int part) { return part & 1 ? t.even : t.odd; }      // (byte (5 - part) / 2 of it)
 
-// The byte of the scale of a part, and whether its codes count.  e: exponent of the block's first scale (nvfp4: over the row's scale); nan: the block is not finite.
+// The byte of the scale of a part.  e: exponent of the block's first scale (nvfp4: over the row's scale); nan: the block is not finite.
 template <int FMT>
-__device__ __forceinline__ uint32_t part_scale(int e, bool nan, int part, bool& gone) {
+__device__ __forceinline__ uint32_t part_scale(int e, bool nan, int part) {
     const int at = e - 3 * part;
-    gone = FMT == kNvfp4 && at < -9;                     // below the least scale
-    if constexpr (FMT == kNvfp4) return nan ? 0x7Fu : at >= -6 ? uint32_t(at + 7) << 3 : gone ? 0u : 1u << (at + 9);
+    if constexpr (FMT == kNvfp4) return nan ? 0x7Fu : at >= -6 ? uint32_t(at + 7) << 3 : at < -9 ? 0u : 1u << (at + 9);
     else return nan ? 0xFFu : uint32_t(at + 127);
 }
+// The nibbles of digits whose scale is no less than the least (all of them but nvfp4's for blocks that are small beside their row's largest).
+template <int FMT>
+__device__ __forceinline__ uint32_t kept_digits(int e) { return FMT == kMxfp4 || e >= 3 * (kPartsX - 1) - 9 ? 0xFFFFFFu : 0xFFFFFFu << (4 * (kPartsX - 1) - (e + 9) / 3 * 4); }
 
 // One CTA takes rows blockIdx.x, blockIdx.x + gridDim.x ...; a thread 32 columns at a time.
 template <typename T, int FMT>
@@ -179,10 +181,11 @@ __global__ void __launch_bounds__(256) tcq_ms_row_parts_kernel(const __grid_cons
                 nan[h] = !inside || m[h] >= 0x7F800000u;
                 e[h] = nan[h] ? 0 : block_exponent<FMT>(m[h], base);
                 const Up up(e[h] + base);
+                const uint32_t kept = kept_digits<FMT>(e[h]);
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
                     const int c = 16 * h + 2 * q;
-                    two[8 * h + q] = two_columns(nan[h] ? 0.0f : up(v[c]), nan[h] ? 0.0f : up(v[c + 1]));
+                    two[8 * h + q] = two_columns(nan[h] ? 0.0f : up(v[c]), nan[h] ? 0.0f : up(v[c + 1]), kept);
                 }
             }
             uint8_t* const record = p.out + ((long long)tile * p.k_tiles + j / 8) * p.record;
@@ -191,14 +194,12 @@ __global__ void __launch_bounds__(256) tcq_ms_row_parts_kernel(const __grid_cons
             for (int part = 0; part < kPartsX; ++part) {
                 const uint32_t byte = (5 - part) / 2, pick = byte | (4 + byte) << 4;
                 uint32_t w[4], scale[2];
-                bool gone[2];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) scale[h] = part_scale<FMT>(e[h], nan[h], part, gone[h]);
+                for (int h = 0; h < 2; ++h) scale[h] = part_scale<FMT>(e[h], nan[h], part);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const TwoColumns* const t = two + 4 * q;
                     w[q] = __byte_perm(__byte_perm(of_part(t[0], part), of_part(t[1], part), pick), __byte_perm(of_part(t[2], part), of_part(t[3], part), pick), 0x5410);
-                    if (gone[q / 2]) w[q] = 0;
                 }
                 const int c = place * kPartsX + part;    // column of the tile
                 *reinterpret_cast<uint4*>(record + kBytesScales<FMT> + c * 128 + ((jj ^ (c & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -250,6 +251,18 @@ __device__ __forceinline__ void mma_block_scaled(uint32_t d, uint64_t a, uint64_
         asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
                      "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
                      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(uint32_t(add)) : "memory");
+}
+
+// What add_up_parts reads of global memory is on its way while the parts are waited for.
+__device__ __forceinline__ void prefetch_parts(const Epilogue& out, const GroupItem& t, long long n, uint32_t rank, uint32_t splits, int threads) {
+    const int i = int(rank) * threads + int(threadIdx.x);
+    const long long r = (long long)t.tn * kRowsW + i % (kRowsW / 4) * 4;
+    if (i >= kRowsW / 4 * t.rows || r >= n) return;
+    const auto prefetch = [](const void* base, int dtype, long long at) {
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(static_cast<const char*>(base) + at * (dtype == kF32 ? 4 : 2)));
+    };
+    if (out.bias != nullptr) prefetch(out.bias, out.bias_dtype, (long long)t.group * n + r);
+    if (out.residual != nullptr) prefetch(out.residual, out.dtype, (t.row0 + i / (kRowsW / 4)) * out.ldr + (act_gated(out.act) ? r >> 1 : r));
 }
 
 // The sums of one item out of the parts that the CTAs of a cluster have in shared memory ([rows][128] at smem_sum of each), in rank order; four neighbours a thread.
@@ -457,6 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_kernel(const __gri
     }
     __syncwarp();
     if (splits > 1) {                                        // one item a cluster: add up the parts of it, four neighbours a thread
+        if (start < items) prefetch_parts(p.out, item_of(start), p.w.rows, rank, splits, kThreads);
         cluster_sync();
         if (start < items) add_up_parts(p.out, item_of(start), p.w.rows, smem_sum, rank, splits, kThreads);
         cluster_sync_relaxed();                              // no CTA ends while another reads its part
@@ -474,14 +488,15 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_kernel(const __gri
 template <int FMT, int NT>
 struct FewTile {
     static constexpr int kAtoms = Ms<FMT>::kAtoms, kRowsX = NT / kPartsX;
-    static constexpr int kBytesW = kRowsW * 128, kBytesS = kAtoms * 512, kStageBytes = (kBytesW + kBytesS + 1023) / 1024 * 1024, kStages = 6;
+    static constexpr int kBytesW = kRowsW * 128, kBytesS = kAtoms * 512, kStageBytes = (kBytesW + kBytesS + 1023) / 1024 * 1024, kMostStages = 10;
     static constexpr int kRecord = (kBytesS + NT * 128 + 1023) / 1024 * 1024;
-    static constexpr int kHeld = 88 * 1024 / kRecord;                         // pieces of 256 columns of x
-    static constexpr int kSumColumns = 32, kScaleColumns = kAtoms * 4 * 2, kScales = 6;      // scales in tensor memory: of kScales stages
+    static constexpr int kSumColumns = 32, kScaleColumns = kAtoms * 4 * 2;   // scales in tensor memory: of one stage
     static constexpr int kColumns = 512;
     static constexpr int kBytesSum = kRowsX * kRowsW * 4;
-    static constexpr int kSmem = kStages * kStageBytes + kHeld * kRecord + kBytesSum + 1024;
-    static_assert(kSmem >= 116 * 1024 && kSmem <= 216 * 1024 && kStages <= kScales && 2 * kSumColumns + kScales * kScaleColumns <= kColumns && NT <= 16);
+    // What x leaves is stages of W, four at least: with few columns all of them are on their way at once (eight experts of 2048 x 2048, six stages 9.7 us).
+    static constexpr int kSmem = 206 * 1024, kRoom = (kSmem - 1024 - kBytesSum) / 1024 * 1024, kHeld = (kRoom - 4 * kStageBytes) / kRecord;      // pieces of 256 columns of x
+    static constexpr int stages(int held) { return std::min(kMostStages, (kRoom - held * kRecord) / kStageBytes); }
+    static_assert(2 * kSumColumns + kMostStages * kScaleColumns <= kColumns && NT <= 16 && stages(kHeld) >= 4);
 };
 constexpr int kFewWarps = 10, kFewThreads = 32 * kFewWarps, kCutters = 8;        // loader, issuer, eight that cut x up, four of which take the results
 
@@ -494,6 +509,7 @@ struct FewArgs {
     Groups groups;
     long long k;
     int tiles_n, k_tiles;
+    int held, stages;                            // pieces of x that a CTA has room for, and stages of W
     Epilogue out;
     unsigned loads;
 };
@@ -503,10 +519,10 @@ __global__ void __launch_bounds__(kFewThreads, 1) tcq_ms_grouped_few_kernel(cons
     using T = FewTile<FMT, NT>;
     extern __shared__ uint8_t raw[];
     __shared__ GroupPlan plan;
-    __shared__ uint64_t full[T::kStages], empty[T::kStages], sum_full[2], sum_empty[2], x_there, drained;
+    __shared__ uint64_t full[T::kMostStages], empty[T::kMostStages], sum_full[2], sum_empty[2], x_there, drained;
     __shared__ uint32_t tmem_at, most[2][T::kRowsX][kCutters];
     __shared__ unsigned int gave_up;
-    const uint32_t smem = (smem_u32(raw) + 1023) & ~1023u, smem_x = smem + T::kStages * T::kStageBytes, smem_sum = smem_x + T::kHeld * T::kRecord;
+    const uint32_t stages = p.stages, smem_x = (smem_u32(raw) + 1023) & ~1023u, smem = smem_x + p.held * T::kRecord, smem_sum = smem_x + T::kRoom;
     float* const sums = reinterpret_cast<float*>(raw + (smem_sum - smem_u32(raw)));
     const int warp = __shfl_sync(0xFFFFFFFFu, int(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank(), splits = cluster_size();
@@ -540,26 +556,32 @@ __global__ void __launch_bounds__(kFewThreads, 1) tcq_ms_grouped_few_kernel(cons
         }
     };
     float v[kRuns][kRun];
-    int token[T::kRowsX] = {};                           // x's rows of the item's rows
+    int token[T::kRowsX] = {}, ahead = 0;                // x's rows of the item's rows; of all rows, a lane one, where there are no more than lanes
+    if (p.tokens != nullptr && lane < p.groups.rows && p.groups.rows <= 32) asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(ahead) : "l"(p.tokens + lane));
     const auto fetch_tokens = [&](int row0, int rows) {
 #pragma unroll
-        for (int q = 0; q < T::kRowsX; ++q) token[q] = p.tokens != nullptr && q < rows ? __ldg(p.tokens + row0 + q) : row0 + q;
+        for (int q = 0; q < T::kRowsX; ++q) {
+            const int known = __shfl_sync(0xFFFFFFFFu, ahead, (row0 + q) & 31);
+            token[q] = p.tokens == nullptr ? row0 + q : p.groups.rows <= 32 ? known : q < rows ? __ldg(p.tokens + row0 + q) : 0;
+        }
     };
     const auto fetch_all = [&](int j0, int all) {
 #pragma unroll
         for (int u = 0; u < kRuns; ++u)
             if (j0 + u * kApart < all) fetch(token[j0 + u * kApart >= runs ? T::kRowsX - 1 : 0], j0 + u * kApart, v[u]);
     };
-    // One group: whose rows they are is known, and x is on its way before the barriers are there.
-    const bool early = p.groups.offsets == nullptr && start < p.tiles_n;
+    // x is on its way before the barriers are there, and before it is known whose rows they are: of one group, or with one row an item and a first group that begins with the first row, the
+    // item's rows are these.
+    const int guess = start / p.tiles_n * T::kRowsX, guessed = p.groups.offsets == nullptr ? min(p.groups.rows, T::kRowsX) : 1;
+    const bool early = (p.groups.offsets == nullptr || T::kRowsX == 1) && guess < p.groups.rows;
     if (early && warp >= 2) {
-        fetch_tokens(0, p.groups.rows);
-        fetch_all(int(threadIdx.x) - 64, min(p.groups.rows, T::kRowsX) * runs);
+        fetch_tokens(guess, guessed);
+        fetch_all(int(threadIdx.x) - 64, guessed * runs);
     }
     if (warp == 0) {
         if (elect_one()) {
             gave_up = 0;
-            for (int s = 0; s < T::kStages; ++s) { mbar_init(smem_u32(&full[s]), 1); mbar_init(smem_u32(&empty[s]), 1); }
+            for (uint32_t s = 0; s < stages; ++s) { mbar_init(smem_u32(&full[s]), 1); mbar_init(smem_u32(&empty[s]), 1); }
             for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&sum_full[s]), 1); mbar_init(smem_u32(&sum_empty[s]), 4); }
             mbar_init(smem_u32(&x_there), kCutters);
             mbar_init(smem_u32(&drained), 1);
@@ -589,11 +611,11 @@ __global__ void __launch_bounds__(kFewThreads, 1) tcq_ms_grouped_few_kernel(cons
                 if (!ok) break;
                 if (one) load(s, t, kt);
                 __syncwarp();
-                if (++s == T::kStages) { s = 0; phase ^= 1; }
-                if (loaded < T::kStages) ++loaded;
+                if (++s == stages) { s = 0; phase ^= 1; }
+                if (loaded < stages) ++loaded;
             }
         }
-        wait_for_loads<T::kStages>(full, s, phase, loaded);
+        wait_for_loads(full, stages, s, phase, loaded);
     } else if (warp == 1) {
         // ---- products; likewise
         constexpr uint32_t kIdesc = 1u << 7 | 1u << 10 | (FMT == kMxfp4 ? 1u : 0u) << 23 | 1u << 27;
@@ -637,7 +659,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tcq_ms_grouped_few_kernel(cons
                     tc_commit(smem_u32(&empty[s]));
                 }
                 __syncwarp();
-                if (++s == T::kStages) { s = 0; phase ^= 1; }
+                if (++s == stages) { s = 0; phase ^= 1; }
             }
             if (ok && one) tc_commit(smem_u32(&sum_full[buf]));
             __syncwarp();
@@ -662,7 +684,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tcq_ms_grouped_few_kernel(cons
                 tile = t.tile;                               // (every warp here has waited for the sums of the item before: its x is no longer read)
                 const int all = t.rows * runs;
                 int base[T::kRowsX] = {};                    // nvfp4: exponent of the scale of this CTA's columns of each row
-                if (i != start || !early) {
+                if (i != start || !early || t.row0 != guess) {
                     fetch_tokens(t.row0, t.rows);
                     fetch_all(id, all);
                 }
@@ -715,18 +737,20 @@ __global__ void __launch_bounds__(kFewThreads, 1) tcq_ms_grouped_few_kernel(cons
                         const bool nan = m >= 0x7F800000u;
                         const int of_row = q ? base[T::kRowsX - 1] : base[0], from = nan ? 0 : block_exponent<FMT>(m, of_row), block = (run & 63) / kLanes;
                         const Up up(from + of_row);
-                        const TwoColumns lo = two_columns(nan ? 0.0f : up(v[0][0]), nan ? 0.0f : up(v[0][1])), hi = two_columns(nan ? 0.0f : up(v[0][2]), nan ? 0.0f : up(v[0][3]));
-                        const uint32_t record = smem_x + run / 64 * T::kRecord;
+                        const uint32_t kept = kept_digits<FMT>(from);
+                        const TwoColumns lo = two_columns(nan ? 0.0f : up(v[0][0]), nan ? 0.0f : up(v[0][1]), kept), hi = two_columns(nan ? 0.0f : up(v[0][2]), nan ? 0.0f : up(v[0][3]), kept);
+                        const uint32_t record = smem_x + run / 64 * T::kRecord + q * kPartsX * 128 + 2 * (run & 7), turn = (run & 63) >> 3;
 #pragma unroll
                         for (int part = 0; part < kPartsX; ++part) {
-                            const int c = q * kPartsX + part, byte = (5 - part) / 2;
-                            bool gone;
-                            const uint32_t scale = part_scale<FMT>(from, nan, part, gone);
+                            const int byte = (5 - part) / 2;
                             const uint32_t codes = __byte_perm(of_part(lo, part), of_part(hi, part), byte | (4 + byte) << 4);
-                            asm volatile("st.shared.u16 [%0], %1;" ::"r"(record + c * 128 + ((((run & 63) >> 3) ^ (c & 7)) << 4) + 2 * (run & 7)), "h"(uint16_t(gone ? 0u : codes)) : "memory");
-                            if (lane % kLanes == 0)
-                                asm volatile("st.shared.u8 [%0], %1;" ::"r"(record + NT * 128 + c * 16 + (block / 4) * 512 + (block & 3)), "r"(scale) : "memory");
+                            asm volatile("st.shared.u16 [%0], %1;" ::"r"(record + part * 128 + (((turn ^ (q * kPartsX + part)) & 7) << 4)), "h"(uint16_t(codes)) : "memory");
                         }
+                        // the scales: a part or two each of the lanes that share a block
+                        const uint32_t scales = smem_x + run / 64 * T::kRecord + NT * 128 + q * kPartsX * 16 + (block / 4) * 512 + (block & 3);
+#pragma unroll
+                        for (int part = lane % kLanes; part < kPartsX; part += kLanes)
+                            asm volatile("st.shared.u8 [%0], %1;" ::"r"(scales + part * 16), "r"(part_scale<FMT>(from, nan, part)) : "memory");
 #pragma unroll
                         for (int h = 0; h + 1 < kRuns; ++h)
 #pragma unroll
@@ -770,6 +794,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tcq_ms_grouped_few_kernel(cons
     }
     __syncwarp();
     if (splits > 1) {                                        // one item a cluster: add up the parts of it, four neighbours a thread
+        if (start < items) prefetch_parts(p.out, item_of(start), p.w.rows, rank, splits, kFewThreads);
         cluster_sync();
         if (start < items) add_up_parts(p.out, item_of(start), p.w.rows, smem_sum, rank, splits, kFewThreads);
         cluster_sync_relaxed();                              // no CTA ends while another reads its part
@@ -865,9 +890,11 @@ cudaError_t launch_few(const GroupedCall& c, cudaStream_t stream) {
     CUtensorMap map_w;
     const long long pitch = ms_pitch(c.k), n = c.w.rows;
     if ((err = make_byte_map(&map_w, c.w.codes, pitch, n * c.groups.groups, pitch, kRowsW)) != cudaSuccess) return err;
-    const FewArgs p{c.x, c.x_rows, c.ldx, c.tokens, ms_rows_aligned(c.x, c.ldx), c.w, c.groups, c.k, int((n + kRowsW - 1) / kRowsW), int(ms_tiles_k(c.k)), c.out, c.loads};
+    FewArgs p{c.x, c.x_rows, c.ldx, c.tokens, ms_rows_aligned(c.x, c.ldx), c.w, c.groups, c.k, int((n + kRowsW - 1) / kRowsW), int(ms_tiles_k(c.k)), 0, 0, c.out, c.loads};
     const long long items = most_tiles(c.groups.rows, c.groups.groups, T::kRowsX) * p.tiles_n;
     const int splits = splits_for(kept, reinterpret_cast<const void*>(kernel), kFewThreads, T::kSmem, items, p.k_tiles);
+    p.held = (p.k_tiles + splits - 1) / splits;
+    p.stages = T::stages(p.held);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(splits > 1 ? items * splits : std::min<long long>(items, ms_sm_count())));
     cfg.blockDim = dim3(kFewThreads);
