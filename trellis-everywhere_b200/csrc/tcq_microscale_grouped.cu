@@ -13,6 +13,8 @@
 //
 // A wait that runs out (kMbarWaitCycles) makes its CTA stop, and its results from there on NaN, as those of its cluster.
 #include <algorithm>
+#include <cmath>
+#include <type_traits>
 
 #include "tcq_microscale_grouped.cuh"
 #include "tcq_tcgen05.cuh"
@@ -47,19 +49,40 @@ struct PartsArgs {
 
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }      // -126 <= e <= 127
 
-// 32 columns of x from c0 on, zeros behind the last.
+// Eight columns of x from c0 on as they are, zeros behind the last.
 template <typename T>
-__device__ __forceinline__ void load32(const T* row, long long c0, long long k, bool wide, float (&v)[32]) {
-    if (wide && c0 + 32 <= k) {
-        uint4 u[4];
+__device__ __forceinline__ uint4 load8(const T* row, long long c0, long long k, bool wide) {
+    if (wide && c0 + 8 <= k) return __ldg(reinterpret_cast<const uint4*>(row + c0));
+    uint32_t w[4] = {};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) u[i] = __ldg(reinterpret_cast<const uint4*>(row + c0) + i);
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = to_f32<T>(reinterpret_cast<const T*>(u)[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = c0 + i < k ? to_f32<T>(row[c0 + i]) : 0.0f;
+    for (int i = 0; i < 8; ++i)
+        if (c0 + i < k) w[i / 2] |= uint32_t(reinterpret_cast<const uint16_t*>(row)[c0 + i]) << (16 * (i & 1));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// Their largest magnitude, as bits of 16; a NaN or an infinity is kInfinite<T> or more.
+template <typename T> constexpr uint32_t kInfinite = std::is_same_v<T, __half> ? 0x7C00u : 0x7F80u;
+__device__ __forceinline__ uint32_t largest8(const uint4& u) {
+    const uint32_t m = __vmaxu2(__vmaxu2(u.x & 0x7FFF7FFFu, u.y & 0x7FFF7FFFu), __vmaxu2(u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu));
+    return max(m & 0xFFFFu, m >> 16);
+}
+// The same of the finite ones.
+template <typename T>
+__device__ __forceinline__ uint32_t largest_finite8(const uint4& u) {
+    uint32_t m = largest8(u);
+    if (m >= kInfinite<T>) {                             // (seldom: one by one)
+        m = 0;
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t b = (i < 2 ? u.x : i < 4 ? u.y : i < 6 ? u.z : u.w) >> (16 * (i & 1)) & 0x7FFFu;
+            if (b < kInfinite<T>) m = max(m, b);
+        }
     }
+    return m;
+}
+// 16 bits of a magnitude as those of the fp32 number.
+template <typename T>
+__device__ __forceinline__ uint32_t as_f32_bits(uint32_t m) {
+    if constexpr (std::is_same_v<T, __half>) return __float_as_uint(__half2float(__ushort_as_half(uint16_t(m))));
+    else return m << 16;
 }
 
 // Bits of the largest magnitude of v[from .. from + N - 1]; a NaN or an infinity counts as 0x7F800000 and more.
@@ -82,10 +105,12 @@ __device__ __forceinline__ int block_exponent(uint32_t amax_bits, int base) {
     if (FMT == kMxfp4 || e >= 3 * (kPartsX - 1) - 9) return e;
     return (max(e + 9, 0) + 2) / 3 * 3 - 9;
 }
-struct Up {                                              // times 2^(15 - e), in two steps: e may be -135
+// Times 2^(15 - e); FAR: in two steps, where e may be below -112 (down to -135: nvfp4, for numbers of fp32's range).
+template <bool FAR>
+struct Up {
     float a, b;
-    __device__ __forceinline__ Up(int e) : a(pow2f((15 - e) / 2)), b(pow2f(15 - e - (15 - e) / 2)) {}
-    __device__ __forceinline__ float operator()(float v) const { return v * a * b; }
+    __device__ __forceinline__ Up(int e) : a(pow2f(FAR ? (15 - e) / 2 : 15 - e)), b(FAR ? pow2f(15 - e - (15 - e) / 2) : 1.0f) {}
+    __device__ __forceinline__ float operator()(float v) const { return FAR ? v * a * b : v * a; }
 };
 
 // The six digits of v 2^-15, |v| < 3.4 * 2^15, as codes: the first in nibble 5.  Bits 24 and up mean nothing.
@@ -113,29 +138,30 @@ __device__ __forceinline__ uint32_t of_part(const TwoColumns& t, int part) { ret
 template <int FMT>
 __device__ __forceinline__ uint32_t part_scale(int e, bool nan, int part) {
     const int at = e - 3 * part;
-    if constexpr (FMT == kNvfp4) return nan ? 0x7Fu : at >= -6 ? uint32_t(at + 7) << 3 : at < -9 ? 0u : 1u << (at + 9);
+    if constexpr (FMT == kNvfp4) return nan ? 0x7Fu : f32_to_e4m3(pow2f(max(at, -20)));       // (below 2^-10: 0)
     else return nan ? 0xFFu : uint32_t(at + 127);
 }
 // The nibbles of digits whose scale is no less than the least (all of them but nvfp4's for blocks that are small beside their row's largest).
 template <int FMT>
 __device__ __forceinline__ uint32_t kept_digits(int e) { return FMT == kMxfp4 || e >= 3 * (kPartsX - 1) - 9 ? 0xFFFFFFu : 0xFFFFFFu << (4 * (kPartsX - 1) - (e + 9) / 3 * 4); }
 
-// One CTA takes rows blockIdx.x, blockIdx.x + gridDim.x ...; a thread 32 columns at a time.
+// One CTA takes rows blockIdx.x, blockIdx.x + gridDim.x ...; a thread eight columns at a time (32 of them take a row of 4096 three times as long, and all of many rows no less).
+constexpr int kPartsThreads = 512;
 template <typename T, int FMT>
-__global__ void __launch_bounds__(256) tcq_ms_row_parts_kernel(const __grid_constant__ PartsArgs p) {
+__global__ void __launch_bounds__(kPartsThreads) tcq_ms_row_parts_kernel(const __grid_constant__ PartsArgs p) {
     __shared__ GroupPlan plan;
-    __shared__ uint32_t most[8];
+    __shared__ uint32_t most[2][kPartsThreads / 32];
+    constexpr int kRun = 8, kLanes = Ms<FMT>::kBlock / kRun;       // lanes that share a block
     launch_dependents();
-    const int chunks = p.k_tiles * 8;
+    const int runs = p.k_tiles * (kMsTileK / kRun);      // whole warps of them
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     bool planned = false;
-    for (int i = blockIdx.x; i < p.groups.rows; i += gridDim.x) {
+    for (int i = blockIdx.x, turn = 0; i < p.groups.rows; i += gridDim.x) {
         const int token = p.tokens != nullptr ? __ldg(p.tokens + i) : i;
         const bool inside = token >= 0 && token < p.x_rows;
         const T* const row = static_cast<const T*>(p.x) + (inside ? token : 0) * p.ldx;
-        float v[32];
-        const bool mine = int(threadIdx.x) < chunks;
-        if (mine && inside) load32(row, 32ll * threadIdx.x, p.k, p.wide, v);     // on their way while the groups are counted
+        uint4 u = {};
+        if (int(threadIdx.x) < runs && inside) u = load8(row, (long long)kRun * threadIdx.x, p.k, p.wide);       // on their way while the groups are counted
         if (!planned) {
             if (warp == 0) plan_groups(p.groups, p.per, plan);
             __syncthreads();
@@ -143,69 +169,50 @@ __global__ void __launch_bounds__(256) tcq_ms_row_parts_kernel(const __grid_cons
         }
         if (i < plan.begin[0] || i >= plan.begin[p.groups.groups]) continue;     // no group's
         const int g = last_not_above(plan.begin, p.groups.groups, i), at = i - plan.begin[g];
-        const int tile = plan.tile[g] + at / p.per, place = at % p.per;
+        const int before = at / p.per, tile = plan.tile[g] + before, place = at - before * p.per;
         int base = 0;                                    // nvfp4: exponent of the token's row scale
         if constexpr (FMT == kNvfp4) {
-            uint32_t m = 0;
-            for (int j = threadIdx.x; j < chunks && inside; j += blockDim.x) {
-                float w[32];
-                if (j == int(threadIdx.x)) {
-#pragma unroll
-                    for (int q = 0; q < 32; ++q) w[q] = v[q];
-                } else {
-                    load32(row, 32ll * j, p.k, p.wide, w);
-                }
-#pragma unroll
-                for (int q = 0; q < 32; ++q) {
-                    const uint32_t b = __float_as_uint(w[q]) & 0x7FFFFFFFu;
-                    m = max(m, b < 0x7F800000u ? b : 0u);
-                }
-            }
+            uint32_t m = largest_finite8<T>(u);
+            for (int j = threadIdx.x + blockDim.x; j < runs && inside; j += blockDim.x) m = max(m, largest_finite8<T>(load8(row, (long long)kRun * j, p.k, p.wide)));
             m = __reduce_max_sync(0xFFFFFFFFu, m);
-            __syncthreads();                             // the row before has been read from `most`
-            if (lane == 0) most[warp] = m;
+            if (lane == 0) most[turn][warp] = m;         // (two turns of them: who writes these has seen that all have read the ones before)
             __syncthreads();
-            for (int q = 0; q < int(blockDim.x) / 32; ++q) m = max(m, most[q]);
-            base = max(first_exponent(m) - 8, -126);     // the largest block's scale is 2^8
+            for (int q = 0; q < int(blockDim.x) / 32; ++q) m = max(m, most[turn][q]);
+            turn ^= 1;
+            base = max(first_exponent(as_f32_bits<T>(m)) - 8, -126);             // the largest block's scale is 2^8
             if (threadIdx.x == 0) p.row_scale[(long long)tile * p.per + place] = pow2f(base);
         }
-        for (int j = threadIdx.x; j < chunks; j += blockDim.x) {
-            if (j != int(threadIdx.x) && inside) load32(row, 32ll * j, p.k, p.wide, v);
-            uint32_t m[2] = {largest<16>(v), largest<16>(v + 16)};
-            if constexpr (FMT == kMxfp4) m[0] = m[1] = max(m[0], m[1]);           // one block
-            int e[2];
-            bool nan[2];
-            TwoColumns two[16];
+        uint8_t* const records = p.out + (long long)tile * p.k_tiles * p.record;
+        const uint32_t column = place * kPartsX;         // of the tile: the first part's
+        for (int j = threadIdx.x; j < runs; j += blockDim.x) {
+            if (j != int(threadIdx.x) && inside) u = load8(row, (long long)kRun * j, p.k, p.wide);
+            uint32_t m = inside ? largest8(u) : kInfinite<T>;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                nan[h] = !inside || m[h] >= 0x7F800000u;
-                e[h] = nan[h] ? 0 : block_exponent<FMT>(m[h], base);
-                const Up up(e[h] + base);
-                const uint32_t kept = kept_digits<FMT>(e[h]);
+            for (int d = 1; d < kLanes; d *= 2) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+            const bool nan = m >= kInfinite<T>;
+            if (nan) u = {};
+            const int e = nan ? 0 : block_exponent<FMT>(as_f32_bits<T>(m), base);
+            const Up<FMT == kNvfp4 && !std::is_same_v<T, __half>> up(e + base);
+            const uint32_t kept = kept_digits<FMT>(e), w[4] = {u.x, u.y, u.z, u.w};
+            TwoColumns two[4];
 #pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    const int c = 16 * h + 2 * q;
-                    two[8 * h + q] = two_columns(nan[h] ? 0.0f : up(v[c]), nan[h] ? 0.0f : up(v[c + 1]), kept);
-                }
+            for (int q = 0; q < 4; ++q) {
+                const T* const pair = reinterpret_cast<const T*>(&w[q]);
+                two[q] = two_columns(up(to_f32<T>(pair[0])), up(to_f32<T>(pair[1])), kept);
             }
-            uint8_t* const record = p.out + ((long long)tile * p.k_tiles + j / 8) * p.record;
-            const int jj = j % 8;
+            uint8_t* const record = records + (j / 32) * p.record;
+            const uint32_t jj = j % 32, block = jj / kLanes, from = kBytesScales<FMT> + column * 128 + 4 * (jj & 3);       // of the 256 columns
 #pragma unroll
             for (int part = 0; part < kPartsX; ++part) {
                 const uint32_t byte = (5 - part) / 2, pick = byte | (4 + byte) << 4;
-                uint32_t w[4], scale[2];
+                *reinterpret_cast<uint32_t*>(record + (from + 128 * part + (((jj >> 2) ^ ((column + part) & 7)) << 4))) =
+                    __byte_perm(__byte_perm(of_part(two[0], part), of_part(two[1], part), pick), __byte_perm(of_part(two[2], part), of_part(two[3], part), pick), 0x5410);
+            }
+            // the scales: some parts each of the lanes that share a block
 #pragma unroll
-                for (int h = 0; h < 2; ++h) scale[h] = part_scale<FMT>(e[h], nan[h], part);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const TwoColumns* const t = two + 4 * q;
-                    w[q] = __byte_perm(__byte_perm(of_part(t[0], part), of_part(t[1], part), pick), __byte_perm(of_part(t[2], part), of_part(t[3], part), pick), 0x5410);
-                }
-                const int c = place * kPartsX + part;    // column of the tile
-                *reinterpret_cast<uint4*>(record + kBytesScales<FMT> + c * 128 + ((jj ^ (c & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                uint8_t* const s = record + (c & 31) * 16 + (c >> 5) * 4;
-                if constexpr (FMT == kNvfp4) *reinterpret_cast<uint16_t*>(s + (jj / 2) * 512 + 2 * (jj & 1)) = uint16_t(scale[0] | scale[1] << 8);
-                else s[(jj / 4) * 512 + (jj & 3)] = uint8_t(scale[0]);
+            for (int part = lane % kLanes; part < kPartsX; part += kLanes) {
+                const uint32_t c = column + part;
+                record[(block / 4) * 512 + (c & 31) * 16 + (c >> 5) * 4 + (block & 3)] = uint8_t(part_scale<FMT>(e, nan, part));
             }
         }
     }
@@ -736,7 +743,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tcq_ms_grouped_few_kernel(cons
                         for (int d = 1; d < kLanes; d *= 2) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
                         const bool nan = m >= 0x7F800000u;
                         const int of_row = q ? base[T::kRowsX - 1] : base[0], from = nan ? 0 : block_exponent<FMT>(m, of_row), block = (run & 63) / kLanes;
-                        const Up up(from + of_row);
+                        const Up<FMT == kNvfp4 && !std::is_same_v<XT, __half>> up(from + of_row);
                         const uint32_t kept = kept_digits<FMT>(from);
                         const TwoColumns lo = two_columns(nan ? 0.0f : up(v[0][0]), nan ? 0.0f : up(v[0][1]), kept), hi = two_columns(nan ? 0.0f : up(v[0][2]), nan ? 0.0f : up(v[0][3]), kept);
                         const uint32_t record = smem_x + run / 64 * T::kRecord + q * kPartsX * 128 + 2 * (run & 7), turn = (run & 63) >> 3;
@@ -818,8 +825,11 @@ int columns_for(long long rows, long long groups) {
 
 template <typename T>
 cudaError_t launch_parts(const GroupedCall& c, const PartsArgs& p, cudaStream_t stream) {
-    const int threads = int(std::min<long long>(256, (p.k_tiles * 8 + 31) / 32 * 32));
-    const unsigned grid = unsigned(std::min<long long>(c.groups.rows, ms_sm_count() * 8));
+    // Threads of a row: all of its runs at once while there are few rows; fewer where many rows fill the SMs, since what a row takes of every thread (its group and place, its largest
+    // number) is as much as eight columns do (8192 rows of 2048 columns: 256 threads 73 us).
+    const int rows = c.groups.rows, sms = ms_sm_count();
+    const int threads = std::min(rows <= sms ? 512 : rows <= 4 * sms ? 256 : rows <= 16 * sms ? 128 : 64, p.k_tiles * 32);
+    const unsigned grid = unsigned(std::min<long long>(rows, sms * 1536ll / threads));
     if (c.fmt == kNvfp4) tcq_ms_row_parts_kernel<T, kNvfp4><<<grid, threads, 0, stream>>>(p);
     else tcq_ms_row_parts_kernel<T, kMxfp4><<<grid, threads, 0, stream>>>(p);
     return cudaGetLastError();
@@ -937,11 +947,24 @@ cudaError_t launch_nt(const GroupedCall& c, void* ws, cudaStream_t stream) {
 
 }  // namespace
 
-// Whether weights as 16-bit numbers pay: they are made once for up to 256 rows, where parts of x take six columns a row.
-static bool many_rows(long long rows, long long groups, int dtype, int fmt) { return rows > 90 * std::min(groups, rows) && ms_grouped_many_takes(dtype, fmt); }
+// Whether weights as 16-bit numbers pay: they are made once for up to 256 rows, where digits take six columns a row, and are made anew for each row.  Both forms' times as measured, us: a
+// step of 64 columns of 128 rows of W takes 0.33 to 0.5 with 16-bit weights; 256 columns 0.29 (mxfp4) or 0.35 with digits, which cost 3.2 for a million numbers of x.  (64 rows a group, 2816 x
+// 2048: 132 and 143 in nvfp4, 134 and 123 in mxfp4; 100 rows through 4096 x 4096: 27 and 15, as 16-bit weights have only 32 SMs busy.)
+static bool many_rows(long long rows, long long groups, long long n, long long k, int dtype, int fmt) {
+    if (!ms_grouped_many_takes(dtype, fmt) || rows <= 32 * std::min(groups, rows)) return false;
+    const double filled = double(std::min(groups, rows)), sms = ms_sm_count(), across = double((n + kRowsW - 1) / kRowsW);
+    const int per = columns_for(rows, groups) / kPartsX;
+    const auto turns = [&](int per_item) {
+        if (groups == 1) return std::ceil(double((rows + per_item - 1) / per_item) * across / sms);
+        return std::max(filled, double(rows) / per_item + 0.5 * filled) * across / sms + 0.5;
+    };
+    const double many = 6.0 + turns(256) * double((k + 63) / 64) * (0.33 + 0.17 * std::min(1.0, double(rows) / filled / 256));
+    const double digits = 8.0 + turns(per) * double(ms_tiles_k(k)) * (fmt == kNvfp4 ? 0.35 : 0.29) + 3.2e-6 * double(rows) * double(k);
+    return many < digits;
+}
 
 size_t ms_grouped_workspace_bytes(long long rows, long long groups, long long n, long long k, int dtype, int fmt, bool in_order) {
-    if (many_rows(rows, groups, dtype, fmt)) return in_order ? 0 : ms_grouped_many_workspace_bytes(rows, k);
+    if (many_rows(rows, groups, n, k, dtype, fmt)) return in_order ? 0 : ms_grouped_many_workspace_bytes(rows, k);
     if (cut_in_place(rows, groups, n, k, fmt)) return 0;
     const int nt = columns_for(rows, groups), per = nt / kPartsX;
     const long long tiles = most_tiles(rows, groups, per);
@@ -949,7 +972,7 @@ size_t ms_grouped_workspace_bytes(long long rows, long long groups, long long n,
 }
 
 cudaError_t launch_ms_grouped(const GroupedCall& c, void* ws, cudaStream_t stream) {
-    if (many_rows(c.groups.rows, c.groups.groups, c.dtype, c.fmt)) return launch_ms_grouped_many(c, ws, stream);
+    if (many_rows(c.groups.rows, c.groups.groups, c.w.rows, c.k, c.dtype, c.fmt)) return launch_ms_grouped_many(c, ws, stream);
     if (cut_in_place(c.groups.rows, c.groups.groups, c.w.rows, c.k, c.fmt)) return c.fmt == kNvfp4 ? launch_cut<kNvfp4>(c, stream) : launch_cut<kMxfp4>(c, stream);
     return c.fmt == kNvfp4 ? launch_nt<kNvfp4>(c, ws, stream) : launch_nt<kMxfp4>(c, ws, stream);
 }
