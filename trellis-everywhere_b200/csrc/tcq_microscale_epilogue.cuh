@@ -48,25 +48,29 @@ __device__ __forceinline__ float load_as_f32(const void* p, int dtype, long long
 }
 // N results of one column, in rows row, row + step ...: residual, rounding, stores.  (y may be the residual: read and written by the same thread.)
 template <typename YT, int N>
-__device__ __forceinline__ void store_rows_as(const Epilogue& e, const float (&v)[N], long long row, int step, int rows, long long column) {
+__device__ __forceinline__ void store_rows_as(const Epilogue& e, float (&v)[N], long long row, int step, int rows, long long column) {
     YT* to = static_cast<YT*>(e.y) + row * e.ldy + column;
-    if (e.residual == nullptr) {
-#pragma unroll
-        for (int i = 0; i < N; ++i, to += step * e.ldy)
-            if (i < rows) *to = from_f32<YT>(v[i]);
-    } else {
+    const long long apart = step * e.ldy;
+    if (e.residual != nullptr) {
         const YT* from = static_cast<const YT*>(e.residual) + row * e.ldr + column;
         YT r[N];
 #pragma unroll
         for (int i = 0; i < N; ++i, from += step * e.ldr)
             if (i < rows) r[i] = *from;
 #pragma unroll
-        for (int i = 0; i < N; ++i, to += step * e.ldy)
-            if (i < rows) *to = from_f32<YT>(v[i] + to_f32<YT>(r[i]));
+        for (int i = 0; i < N; ++i) v[i] += to_f32<YT>(r[i]);
+    }
+    if (rows >= N) {
+#pragma unroll
+        for (int i = 0; i < N; ++i, to += apart) *to = from_f32<YT>(v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i, to += apart)
+            if (i < rows) *to = from_f32<YT>(v[i]);
     }
 }
 template <int N>
-__device__ __forceinline__ void store_rows(const Epilogue& e, const float (&v)[N], long long row, int step, int rows, long long column) {
+__device__ __forceinline__ void store_rows(const Epilogue& e, float (&v)[N], long long row, int step, int rows, long long column) {
     if (e.dtype == kBf16) store_rows_as<__nv_bfloat16>(e, v, row, step, rows, column);
     else if (e.dtype == kF16) store_rows_as<__half>(e, v, row, step, rows, column);
     else store_rows_as<float>(e, v, row, step, rows, column);
@@ -104,7 +108,7 @@ __device__ __forceinline__ void finish_four(const Epilogue& e, float (&h)[4], lo
         activate(e.act, h);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float one[1] = {h[j]};
+            float one[1] = {h[j]};
             if (r + j < n) store_rows(e, one, row, 1, 1, r + j);
         }
     } else {
@@ -112,7 +116,7 @@ __device__ __forceinline__ void finish_four(const Epilogue& e, float (&h)[4], lo
         activate(e.act, gate);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const float one[1] = {gate[j] * h[2 * j + 1]};
+            float one[1] = {gate[j] * h[2 * j + 1]};
             if (r + 2 * j < n) store_rows(e, one, row, 1, 1, (r >> 1) + j);
         }
     }

@@ -290,6 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_many_kernel(const 
                 const int buf = n % T::kSums;
                 ok = still_waits(ok, smem_u32(&sum_full[buf]), uint32_t(n / T::kSums) & 1, &gave_up);
                 tc_fence_after();
+                const float plus = ok ? bias : __uint_as_float(0x7FC00000u);
                 const int first = mine * kShare, last = min(first + kShare, t.rows - half);
 #pragma unroll 1
                 for (int c0 = first; c0 < last; c0 += kChunk) {
@@ -298,11 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_many_kernel(const 
                     tmem_wait_ld();
                     float h[kChunk];
 #pragma unroll
-                    for (int c = 0; c < kChunk; ++c) {
-                        float f = __uint_as_float(v[c]);
-                        if constexpr (FMT == kNvfp4) f *= fw;
-                        h[c] = ok ? f + bias : __uint_as_float(0x7FC00000u);
-                    }
+                    for (int c = 0; c < kChunk; ++c) h[c] = FMT == kNvfp4 ? __fmaf_rn(__uint_as_float(v[c]), fw, plus) : __uint_as_float(v[c]) + plus;
                     if (c0 + kChunk >= last) {
                         tc_fence_before();
                         __syncwarp();
