@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_many_kernel(const 
     tc_fence_after();
     const uint32_t tmem = tmem_at, tmem_a = tmem + T::kSums * kHalf;
     const int items = plan.tile[p.groups.groups] * p.tiles_n;
-    const auto item_of = [&](int i) { return group_item(plan, p.groups.groups, p.tiles_n, kNt, i); };
+    const auto item_of = [&](int i) { return group_item<true>(plan, p.groups.groups, p.tiles_n, kNt, i); };
 
     if (warp == 0) {
         // ---- loads; the warp stays together, one lane issues

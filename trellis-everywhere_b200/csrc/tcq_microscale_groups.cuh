@@ -95,6 +95,8 @@ __device__ __forceinline__ int last_not_above(const int* at, int groups, int v) 
 struct GroupItem {
     int group, tile, tn, row0, rows;                     // tile: among all tiles; tn: which 128 rows of the matrix; row0, rows: of x and y
 };
+// EVEN: a group's rows are shared by its tiles evenly, so that items are of more equal size; else all but its last one are full.
+template <bool EVEN = false>
 __device__ __forceinline__ GroupItem group_item(const GroupPlan& plan, int groups, int tiles_n, int per, int i) {
     GroupItem t;
     t.group = last_not_above(plan.tile, groups, i / tiles_n);
@@ -102,8 +104,15 @@ __device__ __forceinline__ GroupItem group_item(const GroupPlan& plan, int group
     t.tn = local / count;
     const int turn = local - t.tn * count;
     t.tile = first + turn;
-    t.row0 = plan.begin[t.group] + turn * per;
-    t.rows = min(per, plan.begin[t.group + 1] - t.row0);
+    const int begin = plan.begin[t.group], all = plan.begin[t.group + 1] - begin;
+    if (EVEN) {
+        const int share = all / count, more = all - share * count;       // the first `more` have one more (at most per, at least one)
+        t.row0 = begin + turn * share + min(turn, more);
+        t.rows = share + (turn < more);
+    } else {
+        t.row0 = begin + turn * per;
+        t.rows = min(per, all - turn * per);
+    }
     return t;
 }
 
