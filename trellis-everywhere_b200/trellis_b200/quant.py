@@ -4,7 +4,7 @@ The reference's model-level drivers walk ``nn.Linear`` modules and call
 ``Quantizer.quantize_weight(w) -> w_fake``; ``TrellisQuantizer`` is that interface
 on top of the CUDA encoder, with or without LDLQ feedback.  ``MicroscaleQuantizer`` is the
 same for the 4-bit microscaled formats, and ``MicroscaledLinear`` / ``apply_microscaled`` keep
-the weights in 4 bits and multiply by them there (no counterpart in the reference).
+the weights in 4 bits and multiply by them there, ``MicroscaledExperts`` those of a mixture of experts (no counterpart in the reference).
 """
 from __future__ import annotations
 
@@ -15,7 +15,7 @@ from typing import Callable, Optional
 import torch
 import torch.nn as nn
 
-from . import microscale
+from . import experts, microscale
 from .ldlq import tcq_quantize_weight_ldlq
 from .qtip import CodebookLike, _cuda_device, block_hadamard, tcq_quantize_weight
 
@@ -83,22 +83,39 @@ class MicroscaleQuantizer(Quantizer):
         return back.to(dtype=w.dtype, device=w.device)
 
 
+def _apply_in_fp32(module: nn.Module, names, apply) -> nn.Module:
+    """``nn.Module._apply`` of a module whose buffers of these names stay fp32 whatever type it is given."""
+    kept = {name: t for name in names if (t := getattr(module, name)) is not None}
+    apply()
+    for name, t in kept.items():
+        now = getattr(module, name)
+        if now.dtype != torch.float32:
+            setattr(module, name, t.to(now.device))
+    return module
+
+
 class MicroscaledLinear(nn.Module):
     """``nn.Linear`` for inference with its weight in 4 bits (no gradient: inputs that need one are refused).
 
     ``activations=16``: inputs stay as they are (``microscale.linear``).  ``activations=4``: inputs are quantised token by
     token (``microscale.quantize``) and both sides multiplied in 4 bits (``microscale.matmul``); ``rotate`` then puts both
     sides in a rotated space of the input channels, which leaves the product what it is.
+
+    ``activation`` ("relu", "gelu", "gelu_tanh", "silu", or gated by pairs of rows, "geglu", "swiglu": ``microscale.linear``) and the ``residual`` that ``forward`` may be given are
+    applied to the sums of the product, bias included, before they are rounded (``activations=16``).
     """
 
     def __init__(self, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, fmt: str = "nvfp4", activations: int = 16,
-                 rotate: int = 0, seed: int = 0):
+                 rotate: int = 0, seed: int = 0, activation: Optional[str] = None):
         super().__init__()
         if activations not in (4, 16):
             raise ValueError("activations must be 4 or 16")
         if rotate and activations == 16:
             raise ValueError("rotate needs activations=4: inputs are rotated as they are quantised")
-        self.fmt, self.activations, self.rotate = fmt, activations, rotate
+        if activation is not None and activations == 4:
+            raise ValueError("an activation in the product needs activations=16")
+        microscale._check_act(activation, weight.shape[0])
+        self.fmt, self.activations, self.rotate, self.activation = fmt, activations, rotate, activation
         self.out_features, self.in_features = weight.shape
         wd = weight.detach().to(_cuda_device(weight))
         signs = _signs(self.in_features, seed, wd.device) if rotate else None
@@ -109,19 +126,17 @@ class MicroscaledLinear(nn.Module):
 
     def _apply(self, fn, recurse: bool = True):
         """Moves with the module, but the scales and signs stay fp32 whatever type the module is given."""
-        kept = {name: t for name in ("row_scale", "signs") if (t := getattr(self, name)) is not None}
-        super()._apply(fn, recurse)
-        for name, t in kept.items():
-            now = getattr(self, name)
-            if now.dtype != torch.float32:
-                setattr(self, name, t.to(now.device))
-        return self
+        return _apply_in_fp32(self, ("row_scale", "signs"), lambda: super(MicroscaledLinear, self)._apply(fn, recurse))
 
     @property
     def weight(self) -> "microscale.Microscaled":
         return microscale.Microscaled(self.codes, self.scales, self.row_scale, (self.out_features, self.in_features), self.fmt)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if self.activation is not None or residual is not None:
+            if self.activations == 4:
+                raise ValueError("a residual in the product needs activations=16")
+            return microscale.linear(x, self.weight, self.bias, self.activation, residual)
         if self.activations == 16:
             y = microscale.linear(x, self.weight)
         else:
@@ -132,7 +147,79 @@ class MicroscaledLinear(nn.Module):
         return y if self.bias is None else y + self.bias.to(y.dtype)
 
     def extra_repr(self) -> str:
-        return f"{self.in_features} -> {self.out_features}, {self.fmt}, activations={self.activations}, rotate={self.rotate}"
+        then = "" if self.activation is None else f", {self.activation}"
+        return f"{self.in_features} -> {self.out_features}, {self.fmt}, activations={self.activations}, rotate={self.rotate}{then}"
+
+
+class MicroscaledExperts(nn.Module):
+    """A mixture of experts for inference with its matrices in 4 bits: ``sum_e weight_e * (act(x @ gate_e.T) * (x @ up_e.T)) @ down_e.T`` over each token's ``top_k`` experts.
+
+    ``up [E, n, k]`` and ``down [E, k_out, n]``; ``gate`` like ``up`` with a gated ``activation`` ("swiglu", "geglu"), None with another (``act(x @ up_e.T)``).  Biases ``[E, n]``,
+    ``[E, n]``, ``[E, k_out]`` or None.  The experts and their weights come of logits (``experts.route`` with ``score`` and ``normalize``): ``router(x)``, where one is given, or what
+    ``forward`` is handed.  Sums between the products stay fp32 but for the rounding of the second one's input to x's type.
+    """
+
+    def __init__(self, up: torch.Tensor, down: torch.Tensor, top_k: int, gate: Optional[torch.Tensor] = None, fmt: str = "nvfp4", activation: str = "swiglu",
+                 score: str = "softmax", normalize: bool = True, router: Optional[nn.Module] = None, up_bias: Optional[torch.Tensor] = None,
+                 gate_bias: Optional[torch.Tensor] = None, down_bias: Optional[torch.Tensor] = None):
+        super().__init__()
+        if up.dim() != 3 or down.dim() != 3 or down.shape[0] != up.shape[0] or down.shape[2] != up.shape[1]:
+            raise ValueError(f"up must be [experts, n, k] and down [experts, k_out, n], got {tuple(up.shape)} and {tuple(down.shape)}")
+        if (gate is not None) != (activation in microscale.GATED):
+            raise ValueError(f"activation {activation!r} {'takes' if gate is None else 'does not take'} a gate")
+        if gate is not None and gate.shape != up.shape:
+            raise ValueError(f"gate must be like up, {list(up.shape)}, got {list(gate.shape)}")
+        if gate_bias is not None and (gate is None or up_bias is None) or (gate is not None and up_bias is not None and gate_bias is None):
+            raise ValueError("gate_bias goes with a gate and up_bias, and up_bias of a gated layer with gate_bias")
+        microscale._check_act(activation, 2)
+        if score not in experts.SCORES or not 1 <= top_k <= min(up.shape[0], experts.MOST_CHOSEN):
+            raise ValueError(f"score={score!r}, top_k={top_k}: expected one of {sorted(experts.SCORES)} and 1 to {min(up.shape[0], experts.MOST_CHOSEN)}")
+        self.fmt, self.activation, self.top_k, self.score, self.normalize, self.router = fmt, activation, top_k, score, normalize, router
+        self.shape = tuple(up.shape) + (down.shape[1],)     # experts, inner, in and out features
+        dev = _cuda_device(up)
+        with torch.no_grad():
+            first = up.detach().to(dev)
+            if gate is not None:
+                first = microscale.interleave(gate.detach().to(dev), first)
+            q, r = experts.quantize_experts(first, fmt), experts.quantize_experts(down.detach().to(dev), fmt)
+            del first
+            if gate_bias is not None:
+                up_bias = torch.stack((gate_bias.detach(), up_bias.detach()), -1).flatten(-2)
+        for name, t in (("up_codes", q.codes), ("up_scales", q.scales), ("up_row_scale", q.row_scale), ("down_codes", r.codes), ("down_scales", r.scales), ("down_row_scale", r.row_scale),
+                        ("up_bias", None if up_bias is None else up_bias.detach().to(dev)), ("down_bias", None if down_bias is None else down_bias.detach().to(dev))):
+            self.register_buffer(name, t)
+
+    def _apply(self, fn, recurse: bool = True):
+        """Moves with the module, but the row scales stay fp32 whatever type the module is given."""
+        return _apply_in_fp32(self, ("up_row_scale", "down_row_scale"), lambda: super(MicroscaledExperts, self)._apply(fn, recurse))
+
+    @property
+    def up(self) -> "experts.ExpertMatrices":
+        e, n, k, _ = self.shape
+        return experts.ExpertMatrices(self.up_codes, self.up_scales, self.up_row_scale, (e, 2 * n if self.activation in microscale.GATED else n, k), self.fmt)
+
+    @property
+    def down(self) -> "experts.ExpertMatrices":
+        e, n, _, out = self.shape
+        return experts.ExpertMatrices(self.down_codes, self.down_scales, self.down_row_scale, (e, out, n), self.fmt)
+
+    def forward(self, x: torch.Tensor, logits: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``x [..., k]`` in fp16 or bf16, ``logits [..., E]`` where there is no router, ``residual [..., k_out]`` of x's type added in the same pass."""
+        e, _, k, out = self.shape
+        if not x.dim() or x.shape[-1] != k:
+            raise ValueError(f"x must be [..., {k}], got {tuple(x.shape)}")
+        if (logits is None) == (self.router is None):
+            raise ValueError("logits come either from the router or with the call")
+        tokens = math.prod(x.shape[:-1])
+        flat = x.reshape(tokens, k)
+        r = experts.route((self.router(flat) if logits is None else logits).reshape(tokens, e), self.top_k, self.score, self.normalize)
+        h = experts.grouped_linear(flat, self.up, r.offsets, r.tokens, self.up_bias, self.activation)
+        y = experts.grouped_linear(h, self.down, r.offsets, bias=self.down_bias, dtype=torch.float32)
+        return experts.combine(y, r, None if residual is None else residual.reshape(tokens, out), x.dtype).reshape(*x.shape[:-1], out)
+
+    def extra_repr(self) -> str:
+        e, n, k, out = self.shape
+        return f"{e} experts, {self.top_k} a token, {k} -> {n} -> {out}, {self.activation}, {self.fmt}"
 
 
 def seed_from_name(name: str) -> int:
