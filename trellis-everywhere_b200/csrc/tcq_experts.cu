@@ -8,6 +8,7 @@
 #include <algorithm>
 
 #include "tcq_experts.cuh"
+#include "tcq_programmatic.cuh"
 
 namespace tcq {
 
@@ -182,6 +183,8 @@ __global__ void __launch_bounds__(kThreads) tcq_route_kernel(const __grid_consta
     extern __shared__ int hist[];
     __shared__ int base[kMostExperts];
     const int warp = threadIdx.x >> 5, entries = c.tokens * c.top;
+    wait_for_kernel_before();
+    launch_dependents();
     for (int e = threadIdx.x; e < c.experts; e += kThreads) base[e] = 0;
     for (int t = warp; t < c.tokens; t += kWarps) choose_any(c, t);
     __syncthreads();
@@ -208,7 +211,8 @@ __global__ void __launch_bounds__(kThreads) tcq_route_kernel(const __grid_consta
 // A chunk of many: its experts, and how many of each.
 __global__ void __launch_bounds__(kThreads) tcq_route_choose_kernel(const __grid_constant__ RouteCall c, int chunk) {
     __shared__ int count[kMostExperts];
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    wait_for_kernel_before();
+    launch_dependents();
     const int warp = threadIdx.x >> 5, t0 = blockIdx.x * chunk, t1 = min(c.tokens, t0 + chunk);
     for (int e = threadIdx.x; e < c.experts; e += kThreads) count[e] = 0;
     for (int t = t0 + warp; t < t1; t += kWarps) choose_any(c, t);
@@ -225,7 +229,8 @@ __global__ void __launch_bounds__(kThreads) tcq_route_choose_kernel(const __grid
 __global__ void __launch_bounds__(kThreads) tcq_route_place_kernel(const __grid_constant__ RouteCall c, int chunk) {
     extern __shared__ int hist[];
     __shared__ int base[kMostExperts], before[kMostExperts];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    wait_for_kernel_before();
+    launch_dependents();
     const int warp = threadIdx.x >> 5;
     for (int e = threadIdx.x; e < c.experts; e += kThreads) base[e] = before[e] = 0;
     __syncthreads();
@@ -308,6 +313,8 @@ template <typename Y, typename O, bool ALIGNED>
 __global__ void __launch_bounds__(256, !ALIGNED ? 3 : sizeof(Y) == 2 ? 5 : 4) tcq_combine_kernel(const __grid_constant__ CombineCall c) {
     __shared__ uint4 turn[ALIGNED ? 1 : 8][ALIGNED ? 1 : 32 * (sizeof(O) / 2)];      // results of a warp, which stores neighbours
     const int n = int(c.n), lane = threadIdx.x & 31;
+    wait_for_kernel_before();
+    launch_dependents();
     const long long stride = (long long)gridDim.x * blockDim.y;
     for (long long token = (long long)blockIdx.x * blockDim.y + threadIdx.y; token < c.tokens; token += stride) {
         const int* const places = c.places + token * c.top;
@@ -376,9 +383,7 @@ cudaError_t combine(const CombineCall& c, cudaStream_t stream) {
     dim3 block(32, 8);
     while (block.x < 256 && block.x < runs) { block.x *= 2; block.y /= 2; }
     const unsigned grid = unsigned(std::min<long long>((c.tokens + block.y - 1) / block.y, 1 << 20));
-    if (aligned) tcq_combine_kernel<Y, O, true><<<grid, block, 0, stream>>>(c);
-    else tcq_combine_kernel<Y, O, false><<<grid, block, 0, stream>>>(c);
-    return cudaGetLastError();
+    return launch_programmatic(aligned ? tcq_combine_kernel<Y, O, true> : tcq_combine_kernel<Y, O, false>, dim3(grid), block, 0, 0, stream, c);
 }
 template <typename Y>
 cudaError_t combine_to(const CombineCall& c, cudaStream_t stream) {
@@ -387,6 +392,8 @@ cudaError_t combine_to(const CombineCall& c, cudaStream_t stream) {
 }
 
 __global__ void __launch_bounds__(256) tcq_epilogue_kernel(const float* h, long long rows, long long n, const __grid_constant__ Epilogue e) {
+    wait_for_kernel_before();
+    launch_dependents();
     const long long fours = (n + 3) / 4, id = (long long)blockIdx.x * 256 + threadIdx.x, row = id / fours, r = (id - row * fours) * 4;
     if (row >= rows) return;
     float v[4];
@@ -418,23 +425,11 @@ cudaError_t launch_route(const RouteCall& c, cudaStream_t stream) {
         if (dev < 64) ready[dev] = true;
     }
     if (chunks == 1) {
-        tcq_route_kernel<<<1, kThreads, smem, stream>>>(c);
-        return cudaGetLastError();
+        return launch_programmatic(tcq_route_kernel, dim3(1), dim3(kThreads), smem, 0, stream, c);
     }
     const int chunk = std::max(32, (c.tokens + kMostChunks - 1) / kMostChunks);
-    tcq_route_choose_kernel<<<unsigned(chunks), kThreads, 0, stream>>>(c, chunk);
-    if ((err = cudaGetLastError()) != cudaSuccess) return err;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(chunks));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = size_t(smem);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, tcq_route_place_kernel, c, chunk);
+    if ((err = launch_programmatic(tcq_route_choose_kernel, dim3(unsigned(chunks)), dim3(kThreads), 0, 0, stream, c, chunk)) != cudaSuccess) return err;
+    return launch_programmatic(tcq_route_place_kernel, dim3(unsigned(chunks)), dim3(kThreads), size_t(smem), 0, stream, c, chunk);
 }
 
 cudaError_t launch_combine(const CombineCall& c, cudaStream_t stream) {
@@ -445,8 +440,7 @@ cudaError_t launch_combine(const CombineCall& c, cudaStream_t stream) {
 cudaError_t launch_epilogue(const float* h, long long rows, long long n, const Epilogue& e, cudaStream_t stream) {
     const long long blocks = (rows * ((n + 3) / 4) + 255) / 256;
     if (blocks > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
-    tcq_epilogue_kernel<<<unsigned(blocks), 256, 0, stream>>>(h, rows, n, e);
-    return cudaGetLastError();
+    return launch_programmatic(tcq_epilogue_kernel, dim3(unsigned(blocks)), dim3(256), 0, 0, stream, h, rows, n, e);
 }
 
 }  // namespace tcq

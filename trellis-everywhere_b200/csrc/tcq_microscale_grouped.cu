@@ -17,6 +17,7 @@
 #include <type_traits>
 
 #include "tcq_microscale_grouped.cuh"
+#include "tcq_programmatic.cuh"
 #include "tcq_tcgen05.cuh"
 
 namespace tcq {
@@ -26,9 +27,6 @@ namespace {
 constexpr int kPartsX = 6;
 constexpr int kThreads = 192;                    // loader, issuer, four warps for the results
 constexpr int kRowsW = 128, kMostSplits = 8;
-
-__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_kernel_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // What a stage of a tile holds of x: block scales of up to 128 columns (parts of rows), then a row of 128 bytes of codes a column.
 template <int FMT> constexpr int kBytesScales = Ms<FMT>::kAtoms * 512;
@@ -152,6 +150,7 @@ __global__ void __launch_bounds__(kPartsThreads) tcq_ms_row_parts_kernel(const _
     __shared__ GroupPlan plan;
     __shared__ uint32_t most[2][kPartsThreads / 32];
     constexpr int kRun = 8, kLanes = Ms<FMT>::kBlock / kRun;       // lanes that share a block
+    wait_for_kernel_before();
     launch_dependents();
     const int runs = p.k_tiles * (kMsTileK / kRun);      // whole warps of them
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -352,7 +351,8 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_kernel(const __gri
     if (warp == 0) {
         // ---- loads; the warp stays together, one lane issues
         const bool one = elect_one();
-        wait_for_kernel_before();                        // x's parts are there
+        wait_for_kernel_before();                        // x's digits are there
+        launch_dependents();
         asm volatile("fence.proxy.async;" ::: "memory");
         uint32_t s = ahead % T::kStages, phase = ahead == T::kStages ? 0 : 1, loaded = ahead;    // (the first wait for a stage is for the phase before the first)
         unsigned left = p.loads - ahead;
@@ -562,6 +562,18 @@ __global__ void __launch_bounds__(kFewThreads, 1) tcq_ms_grouped_few_kernel(cons
             for (int h = 0; h < 4; ++h) v[h] = c0 + h < p.k ? to_f32<XT>(from[h]) : 0.0f;
         }
     };
+    if (warp == 0 && elect_one()) {
+        gave_up = 0;
+        for (uint32_t s = 0; s < stages; ++s) { mbar_init(smem_u32(&full[s]), 1); mbar_init(smem_u32(&empty[s]), 1); }
+        for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&sum_full[s]), 1); mbar_init(smem_u32(&sum_empty[s]), 4); }
+        mbar_init(smem_u32(&x_there), kCutters);
+        mbar_init(smem_u32(&drained), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncwarp();
+    if (warp == 1) tmem_alloc(smem_u32(&tmem_at), T::kColumns);
+    wait_for_kernel_before();
+    launch_dependents();
     float v[kRuns][kRun];
     int token[T::kRowsX] = {}, ahead = 0;                // x's rows of the item's rows; of all rows, a lane one, where there are no more than lanes
     if (p.tokens != nullptr && lane < p.groups.rows && p.groups.rows <= 32) asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(ahead) : "l"(p.tokens + lane));
@@ -577,7 +589,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tcq_ms_grouped_few_kernel(cons
         for (int u = 0; u < kRuns; ++u)
             if (j0 + u * kApart < all) fetch(token[j0 + u * kApart >= runs ? T::kRowsX - 1 : 0], j0 + u * kApart, v[u]);
     };
-    // x is on its way before the barriers are there, and before it is known whose rows they are: of one group, or with one row an item and a first group that begins with the first row, the
+    // x is on its way before it is known whose rows they are: of one group, or with one row an item and a first group that begins with the first row, the
     // item's rows are these.
     const int guess = start / p.tiles_n * T::kRowsX, guessed = p.groups.offsets == nullptr ? min(p.groups.rows, T::kRowsX) : 1;
     const bool early = (p.groups.offsets == nullptr || T::kRowsX == 1) && guess < p.groups.rows;
@@ -585,19 +597,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tcq_ms_grouped_few_kernel(cons
         fetch_tokens(guess, guessed);
         fetch_all(int(threadIdx.x) - 64, guessed * runs);
     }
-    if (warp == 0) {
-        if (elect_one()) {
-            gave_up = 0;
-            for (uint32_t s = 0; s < stages; ++s) { mbar_init(smem_u32(&full[s]), 1); mbar_init(smem_u32(&empty[s]), 1); }
-            for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&sum_full[s]), 1); mbar_init(smem_u32(&sum_empty[s]), 4); }
-            mbar_init(smem_u32(&x_there), kCutters);
-            mbar_init(smem_u32(&drained), 1);
-            asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
-        }
-        __syncwarp();
-        plan_groups(p.groups, T::kRowsX, plan);
-    }
-    if (warp == 1) tmem_alloc(smem_u32(&tmem_at), T::kColumns);
+    if (warp == 0) plan_groups(p.groups, T::kRowsX, plan);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -830,9 +830,7 @@ cudaError_t launch_parts(const GroupedCall& c, const PartsArgs& p, cudaStream_t 
     const int rows = c.groups.rows, sms = ms_sm_count();
     const int threads = std::min(rows <= sms ? 512 : rows <= 4 * sms ? 256 : rows <= 16 * sms ? 128 : 64, p.k_tiles * 32);
     const unsigned grid = unsigned(std::min<long long>(rows, sms * 1536ll / threads));
-    if (c.fmt == kNvfp4) tcq_ms_row_parts_kernel<T, kNvfp4><<<grid, threads, 0, stream>>>(p);
-    else tcq_ms_row_parts_kernel<T, kMxfp4><<<grid, threads, 0, stream>>>(p);
-    return cudaGetLastError();
+    return launch_programmatic(c.fmt == kNvfp4 ? tcq_ms_row_parts_kernel<T, kNvfp4> : tcq_ms_row_parts_kernel<T, kMxfp4>, dim3(grid), dim3(threads), 0, 0, stream, p);
 }
 
 // How many CTAs share the columns of an item: as many as leave each an SM of its own, and two pieces of 256 columns or more.
@@ -868,20 +866,8 @@ cudaError_t launch(const GroupedCall& c, void* ws, cudaStream_t stream) {
     const GroupedArgs p{c.w, c.groups, int((n + kRowsW - 1) / kRowsW), k_tiles, records, static_cast<const float*>(ws), c.out, c.loads};
     const long long items = tiles * p.tiles_n;
     const int splits = splits_for(kept, reinterpret_cast<const void*>(kernel), kThreads, T::kSmem, items, k_tiles);
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(splits > 1 ? items * splits : std::min<long long>(items, ms_sm_count())));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = T::kSmem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attrs[2] = {};
-    attrs[0].id = cudaLaunchAttributeClusterDimension;
-    attrs[0].val.clusterDim.x = unsigned(splits);
-    attrs[0].val.clusterDim.y = attrs[0].val.clusterDim.z = 1;
-    attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;      // begins beside the kernel that makes the parts, and waits for it where it needs them
-    attrs[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attrs;
-    cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, kernel, map_w, p);
+    // (begins beside the kernel that makes the digits, and waits for it where it needs them)
+    return launch_programmatic(kernel, dim3(unsigned(splits > 1 ? items * splits : std::min<long long>(items, ms_sm_count()))), dim3(kThreads), T::kSmem, splits, stream, map_w, p);
 }
 
 template <typename XT, int FMT, int NT>
@@ -905,18 +891,7 @@ cudaError_t launch_few(const GroupedCall& c, cudaStream_t stream) {
     const int splits = splits_for(kept, reinterpret_cast<const void*>(kernel), kFewThreads, T::kSmem, items, p.k_tiles);
     p.held = (p.k_tiles + splits - 1) / splits;
     p.stages = T::stages(p.held);
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(splits > 1 ? items * splits : std::min<long long>(items, ms_sm_count())));
-    cfg.blockDim = dim3(kFewThreads);
-    cfg.dynamicSmemBytes = T::kSmem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = unsigned(splits);
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, map_w, p);
+    return launch_programmatic(kernel, dim3(unsigned(splits > 1 ? items * splits : std::min<long long>(items, ms_sm_count()))), dim3(kFewThreads), T::kSmem, splits, stream, map_w, p);
 }
 
 // Whether x is cut up where it is multiplied: one or two rows an item, its columns held by a CTA whatever the split, and few enough items, or only those of the same rows.

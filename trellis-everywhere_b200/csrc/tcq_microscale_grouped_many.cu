@@ -15,6 +15,7 @@
 
 #include "tcq_microscale_grouped.cuh"
 #include "tcq_microscale_weights.cuh"
+#include "tcq_programmatic.cuh"
 #include "tcq_tcgen05.cuh"
 
 namespace tcq {
@@ -99,6 +100,8 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_many_kernel(const 
     }
     __syncwarp();
     if (warp == 1) tmem_alloc(smem_u32(&tmem_at), T::kColumns);
+    wait_for_kernel_before();
+    launch_dependents();
     if (warp == 2) plan_groups(p.groups, kNt, plan);
     tc_fence_before();
     __syncthreads();
@@ -324,6 +327,8 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_many_kernel(const 
 // Rows of 16-bit numbers in order, zeros up to a multiple of eight columns; rows that x has not are NaN.
 __global__ void __launch_bounds__(256) tcq_ms_grouped_rows_kernel(const uint16_t* __restrict__ x, long long x_rows, long long k, long long ldx, const int* __restrict__ tokens,
                                                                   long long rows, uint16_t* __restrict__ out, long long runs, bool wide) {
+    wait_for_kernel_before();
+    launch_dependents();
     for (long long id = (long long)blockIdx.x * 256 + threadIdx.x; id < rows * runs; id += (long long)gridDim.x * 256) {
         const long long i = id / runs, c0 = (id - i * runs) * 8, token = tokens != nullptr ? __ldg(tokens + i) : i;
         const bool there = token >= 0 && token < x_rows;
@@ -358,8 +363,7 @@ cudaError_t launch(const GroupedCall& c, cudaStream_t stream) {
     if ((err = make_16bit_map(&map_x, c.x, c.k, c.x_rows, c.ldx, kBoxRows)) != cudaSuccess) return err;
     const ManyArgs p{c.w, c.groups, int((n + kRows - 1) / kRows), int((c.k + kStepK - 1) / kStepK), ms_tiles_k(c.k) * T::kAtoms, c.out, c.loads};
     const long long items = most_tiles(c.groups.rows, c.groups.groups, kNt) * p.tiles_n;
-    kernel<<<unsigned(std::min<long long>(items, ms_sm_count())), kThreads, T::kSmem, stream>>>(map_w, map_x, p);
-    return cudaGetLastError();
+    return launch_programmatic(kernel, dim3(unsigned(std::min<long long>(items, ms_sm_count()))), dim3(kThreads), T::kSmem, 0, stream, map_w, map_x, p);
 }
 
 }  // namespace
@@ -370,9 +374,9 @@ cudaError_t launch_ms_grouped_many(const GroupedCall& call, void* ws, cudaStream
     GroupedCall c = call;
     if (c.tokens != nullptr || !ms_rows_aligned(c.x, c.ldx)) {      // in order, where TMA loads can start
         const long long runs = (c.k + 7) / 8;
-        tcq_ms_grouped_rows_kernel<<<unsigned(std::min<long long>((c.groups.rows * runs + 255) / 256, 1 << 20)), 256, 0, stream>>>(
-            static_cast<const uint16_t*>(c.x), c.x_rows, c.k, c.ldx, c.tokens, c.groups.rows, static_cast<uint16_t*>(ws), runs, c.k % 8 == 0 && ms_rows_aligned(c.x, c.ldx));
-        const cudaError_t err = cudaGetLastError();
+        const cudaError_t err = launch_programmatic(tcq_ms_grouped_rows_kernel, dim3(unsigned(std::min<long long>((c.groups.rows * runs + 255) / 256, 1 << 20))), dim3(256), 0, 0, stream,
+                                                    static_cast<const uint16_t*>(c.x), c.x_rows, c.k, c.ldx, c.tokens, (long long)c.groups.rows, static_cast<uint16_t*>(ws), runs,
+                                                    c.k % 8 == 0 && ms_rows_aligned(c.x, c.ldx));
         if (err != cudaSuccess) return err;
         c.x = ws;
         c.x_rows = c.groups.rows;
