@@ -6,6 +6,7 @@
 //
 // The sum: a thread has eight columns of one token, and the loads of four of its rows are in flight together.  Bound by memory.
 #include <algorithm>
+#include <type_traits>
 
 #include "tcq_experts.cuh"
 #include "tcq_programmatic.cuh"
@@ -272,45 +273,61 @@ __device__ __forceinline__ void to_floats(const Eight<T>& e, float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(reinterpret_cast<const T*>(e.u)[i]);
 }
-// At any address: pieces of 16 bytes that start on 16 bytes, one more than they fill, and a shift; single numbers where fewer than eight exist, or in the first and the last row (`inner`
-// is false), where a piece could reach out of the matrix.
+__device__ __forceinline__ void load_if(bool there, const void* p, uint4& u) {       // without a branch, so that loads behind it are in flight with it
+    asm("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\t@p ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+        : "+r"(u.x), "+r"(u.y), "+r"(u.z), "+r"(u.w) : "l"(p), "r"(uint32_t(there)));
+}
 template <typename T>
-__device__ __forceinline__ Eight<T> load_eight(const T* p, bool aligned, int there, bool inner) {
-    constexpr int kPieces = sizeof(T) / 2;
+__device__ __forceinline__ Eight<T> load_eight(const T* p) {
     Eight<T> e;
-    if (aligned) {
 #pragma unroll
-        for (int q = 0; q < kPieces; ++q) e.u[q] = __ldg(reinterpret_cast<const uint4*>(p) + q);
-        return e;
-    }
-    const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(p)) & 15u;
-    const char* const base = reinterpret_cast<const char*>(p) - off;
-    if (there >= 8 && inner) {
-        uint32_t w[4 * (kPieces + 1)];
-#pragma unroll
-        for (int q = 0; q <= kPieces; ++q) {
-            const uint4 u = __ldg(reinterpret_cast<const uint4*>(base) + q);
-            w[4 * q] = u.x; w[4 * q + 1] = u.y; w[4 * q + 2] = u.z; w[4 * q + 3] = u.w;
-        }
-#pragma unroll
-        for (int step = 2; step >= 1; --step)
-            if (off & (4 * step))
-#pragma unroll
-                for (int i = 0; i + step < 4 * (kPieces + 1); ++i) w[i] = w[i + step];
-#pragma unroll
-        for (int i = 0; i < 4 * kPieces; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 8 * (off & 3));
-#pragma unroll
-        for (int q = 0; q < kPieces; ++q) e.u[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(e.u)[i] = i < there ? p[i] : from_f32<T>(0.0f);
-    }
+    for (int q = 0; q < int(sizeof(T) / 2); ++q) e.u[q] = __ldg(reinterpret_cast<const uint4*>(p) + q);
     return e;
 }
+// Eight numbers at any address: pieces of 16 bytes that start on 16 bytes, one more than they fill, and a shift; single numbers where fewer than eight exist, or in
+// the first and the last row (`inner` is false), where a piece could reach out of the matrix.
+template <typename T>
+struct EightAt {
+    static constexpr int kPieces = sizeof(T) / 2 + 1;
+    const T* p;
+    uint4 u[kPieces];
+    bool whole;
+    __device__ __forceinline__ void load(const T* at, bool some, int there, bool inner) {
+        p = at;
+        whole = some && there >= 8 && inner;
+        const char* const base = reinterpret_cast<const char*>(reinterpret_cast<uintptr_t>(at) & ~uintptr_t(15));
+#pragma unroll
+        for (int q = 0; q < kPieces; ++q) {
+            u[q] = make_uint4(0, 0, 0, 0);
+            load_if(whole, base + 16 * q, u[q]);
+        }
+    }
+    __device__ __forceinline__ Eight<T> get(bool some, int there) const {
+        Eight<T> e;
+        if (whole || !some) {
+            const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(p)) & 15u;
+            uint32_t w[4 * kPieces];
+#pragma unroll
+            for (int q = 0; q < kPieces; ++q) { w[4 * q] = u[q].x; w[4 * q + 1] = u[q].y; w[4 * q + 2] = u[q].z; w[4 * q + 3] = u[q].w; }
+#pragma unroll
+            for (int step = 2; step >= 1; --step)
+#pragma unroll
+                for (int i = 0; i + step < 4 * kPieces; ++i) w[i] = off & (4 * step) ? w[i + step] : w[i];
+#pragma unroll
+            for (int i = 0; i + 1 < 4 * kPieces; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 8 * (off & 3));
+#pragma unroll
+            for (int q = 0; q + 1 < kPieces; ++q) e.u[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(e.u)[i] = i < there ? p[i] : from_f32<T>(0.0f);
+        }
+        return e;
+    }
+};
 
 // Y: of the rows, O: of what comes out.  Threads in x: eight columns of a token each; in y: tokens.  ALIGNED: all rows start on 16 bytes, and n is a multiple of eight.
 template <typename Y, typename O, bool ALIGNED>
-__global__ void __launch_bounds__(256, !ALIGNED ? 3 : sizeof(Y) == 2 ? 5 : 4) tcq_combine_kernel(const __grid_constant__ CombineCall c) {
+__global__ void __launch_bounds__(256, 3) tcq_combine_kernel(const __grid_constant__ CombineCall c) {
     __shared__ uint4 turn[ALIGNED ? 1 : 8][ALIGNED ? 1 : 32 * (sizeof(O) / 2)];      // results of a warp, which stores neighbours
     const int n = int(c.n), lane = threadIdx.x & 31;
     wait_for_kernel_before();
@@ -322,33 +339,46 @@ __global__ void __launch_bounds__(256, !ALIGNED ? 3 : sizeof(Y) == 2 ? 5 : 4) tc
         for (int c0 = 8 * threadIdx.x; c0 - 8 * lane < n; c0 += 8 * blockDim.x) {     // (whole warps stay together)
             const int there = n - c0;
             float out[8] = {};
-            Eight<O> res;
-            if (c.residual != nullptr && there > 0) {
-                const O* const at = static_cast<const O*>(c.residual) + token * c.ldr + c0;
-                res = load_eight<O>(at, ALIGNED, there, token > 0 && token + 1 < c.tokens);
+            const bool add = c.residual != nullptr && there > 0;
+            const O* const from = static_cast<const O*>(c.residual) + token * c.ldr + c0;
+            using Residual = std::conditional_t<ALIGNED, Eight<O>, EightAt<O>>;
+            using Row = std::conditional_t<ALIGNED, Eight<Y>, EightAt<Y>>;
+            Residual res;
+            if constexpr (ALIGNED) {
+                if (add) res = load_eight<O>(from);
+            } else {
+                res.load(from, add, there, token > 0 && token + 1 < c.tokens);
             }
             for (int j0 = 0; j0 < c.top; j0 += 4) {
-                Eight<Y> v[4];
+                Row v[4];
                 float w[4];
+                bool some[4];
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const int place = j0 + q < c.top ? __ldg(places + j0 + q) : -1;
-                    const bool some = place >= 0 && place < c.rows && there > 0;
-                    w[q] = some ? __ldg(weights + j0 + q) : 0.0f;
-                    v[q] = {};
-                    if (some) v[q] = load_eight<Y>(static_cast<const Y*>(c.y) + place * c.ldy + c0, ALIGNED, there, place > 0 && place + 1 < c.rows);
+                    some[q] = place >= 0 && place < c.rows && there > 0;
+                    w[q] = some[q] ? __ldg(weights + j0 + q) : 0.0f;
+                    const Y* const row = static_cast<const Y*>(c.y) + place * c.ldy + c0;
+                    if constexpr (ALIGNED) {
+                        v[q] = {};
+                        if (some[q]) v[q] = load_eight<Y>(row);
+                    } else {
+                        v[q].load(row, some[q], there, place > 0 && place + 1 < c.rows);
+                    }
                 }
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     float f[8];
-                    to_floats(v[q], f);
+                    if constexpr (ALIGNED) to_floats(v[q], f);
+                    else to_floats(v[q].get(some[q], there), f);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) out[i] = __fmaf_rn(f[i], w[q], out[i]);
                 }
             }
-            if (c.residual != nullptr && there > 0) {
+            if (add) {
                 float f[8];
-                to_floats(res, f);
+                if constexpr (ALIGNED) to_floats(res, f);
+                else to_floats(res.get(add, there), f);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) out[i] += f[i];
             }

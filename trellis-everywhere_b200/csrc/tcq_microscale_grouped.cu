@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_kernel(const __gri
         // ---- loads; the warp stays together, one lane issues
         const bool one = elect_one();
         wait_for_kernel_before();                        // x's digits are there
-        launch_dependents();
+        // (the next kernel begins when this one has ended: its warps beside these cost 800 rows of 32 groups of 2000 x 2048 6 %)
         asm volatile("fence.proxy.async;" ::: "memory");
         uint32_t s = ahead % T::kStages, phase = ahead == T::kStages ? 0 : 1, loaded = ahead;    // (the first wait for a stage is for the phase before the first)
         unsigned left = p.loads - ahead;
