@@ -172,3 +172,66 @@ def test_calls_in_turn_on_one_stream():
             graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, y)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("n", [3850, 3970, 4096])
+@pytest.mark.parametrize("rows,counts", [(100, [25, 25, 25, 25]), (100, [0, 1, 60, 39]), (100, [100, 0, 0, 0]), (100, [18, 21, 22, 39])])
+def test_matrices_of_many_rows(rows, counts, n, fmt, dtype):
+    """More items than SMs, in halves of 128 rows of a matrix, its last one alone or not whole, with rows of x gathered and not."""
+    from trellis_b200 import experts
+    w, x = case(4, rows, n, 296, fmt, dtype=dtype)
+    offsets = torch.tensor([0, *counts], device=DEV).cumsum(0).int()
+    y, back = experts.grouped_linear(x, w, offsets, dtype=torch.float32), torch.arange(rows - 1, -1, -1, device=DEV).int()
+    assert torch.equal(experts.grouped_linear(x[back.long()], w, offsets, back, dtype=torch.float32), y)
+    bias, gated = torch.randn(4, n, device=DEV), experts.grouped_linear(x, w, offsets, activation="swiglu")
+    with_bias = experts.grouped_linear(x, w, offsets, bias=bias)
+    at = offsets.tolist()
+    for e in range(4):
+        i, j = at[e], at[e + 1]
+        from trellis_b200 import microscale as ms
+        one, xd = ms.dequantize(experts.expert(w, e)).double(), x[i:j].double()
+        if i == j:
+            continue
+        h, b = xd @ one.t(), plain.sums_bound(xd, one, fmt)
+        for got, bi, act, dt in ((y, None, None, torch.float32), (gated, None, "swiglu", dtype), (with_bias, bias[e], None, dtype)):
+            want, bound = plain.epilogue(h, b, bi, act, None, dt)
+            assert bool(((got[i:j].double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+def test_many_items_for_each_sm(fmt):
+    """Every group's result is that of its rows alone: sums of 64 columns, so that no form adds them in another order."""
+    from trellis_b200 import experts
+    e, rows, n = 96, 1500, 1182
+    w, x = case(e, rows, n, 64, fmt)
+    g = torch.Generator(device=DEV).manual_seed(3)
+    offsets = torch.cat([torch.zeros(1, device=DEV), torch.randint(0, e, (rows,), generator=g, device=DEV).bincount(minlength=e).cumsum(0)]).int()
+    y, at = experts.grouped_linear(x, w, offsets, dtype=torch.float32), offsets.tolist()
+    for i in range(e):
+        if at[i] < at[i + 1]:
+            mine = w._replace(codes=w.codes[i:i + 1], scales=w.scales[i:i + 1], row_scale=None if w.row_scale is None else w.row_scale[i:i + 1], shape=(1, n, 64))
+            assert torch.equal(experts.grouped_linear(x[at[i]:at[i + 1]], mine, torch.tensor([0, at[i + 1] - at[i]], device=DEV).int(), dtype=torch.float32), y[at[i]:at[i + 1]])
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+def test_waits_for_matrices_of_many_rows_that_run_out(fmt):
+    """Loads that never come where a CTA has several items: the kernel ends, and what needed them is NaN; the next call is right."""
+    from trellis_b200 import _lib, experts
+    e, rows, n, k = 8, 200, 4000, 512
+    w, x = case(e, rows, n, k, fmt)
+    offsets = torch.arange(0, rows + 1, rows // e, device=DEV).int()
+    want = experts.grouped_linear(x, w, offsets)
+    L, f = _lib.lib(), 0 if fmt == "mxfp4" else 1
+    size = L.tcq_ms_grouped_linear_workspace_bytes(rows, e, n, k, 2, f, 1)
+    ws = torch.empty(size, dtype=torch.uint8, device=DEV)
+    for loads in (0, 1, 2, 3):                                    # two a first item
+        y = torch.zeros(rows, n, dtype=torch.bfloat16, device=DEV)
+        rc = L.tcq_selftest_ms_grouped_waits(loads, x.data_ptr(), 2, rows, k, None, offsets.data_ptr(), e, rows, w.codes.data_ptr(), w.scales.data_ptr(),
+                                             None if w.row_scale is None else w.row_scale.data_ptr(), n, k, f, None, 0, 0, None, 0, y.data_ptr(), 2, n, ws.data_ptr(), size,
+                                             torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        torch.cuda.synchronize()
+        assert bool((y.isnan() | (y == want)).all()) and bool(y.isnan().any()) and (loads < 2 or bool((y == want).any()))
+    assert torch.equal(experts.grouped_linear(x, w, offsets), want)

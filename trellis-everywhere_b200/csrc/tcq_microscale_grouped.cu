@@ -293,6 +293,23 @@ __device__ __forceinline__ void add_up_parts(const Epilogue& out, const GroupIte
     }
 }
 
+// N rows' sums out of tensor memory, six columns each from `from` on in PIECES pieces of eight: added up, smallest first, and scaled.  fx: the scale of row `lane`.
+template <int FMT, int N, int PIECES>
+__device__ __forceinline__ void take_rows(uint32_t from, float fx, float inner, float outer, bool ok, float (&h)[N]) {
+    uint32_t v[PIECES][8];
+#pragma unroll
+    for (int q = 0; q < PIECES; ++q) tmem_load<8>(from + 8 * q, v[q]);
+    tmem_wait_ld();
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+        float sum = __uint_as_float(v[(q * kPartsX + kPartsX - 1) / 8][(q * kPartsX + kPartsX - 1) % 8]);
+#pragma unroll
+        for (int part = kPartsX - 2; part >= 0; --part) sum += __uint_as_float(v[(q * kPartsX + part) / 8][(q * kPartsX + part) % 8]);
+        if constexpr (FMT == kNvfp4) sum = sum * inner * __shfl_sync(0xFFFFFFFFu, fx, q) * outer;
+        h[q] = ok ? sum : __uint_as_float(0x7FC00000u);
+    }
+}
+
 template <int FMT, int NT>
 __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ GroupedArgs p) {
     using T = Tile<FMT, NT>;
@@ -444,24 +461,13 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_kernel(const __gri
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < t.rows; c += T::kTake) {
-                uint32_t v[T::kPieces][8];
-#pragma unroll
-                for (int q = 0; q < T::kPieces; ++q) tmem_load<8>(tmem + buf * T::kSumColumns + c * kPartsX + 8 * q + (uint32_t(32 * quarter) << 16), v[q]);
-                const float fx = FMT == kNvfp4 && lane < T::kTake && c + lane < t.rows ? p.x_row[(long long)t.tile * T::kRowsX + c + lane] : 1.0f;
-                tmem_wait_ld();
+                float h[T::kTake];
+                take_rows<FMT, T::kTake, T::kPieces>(tmem + buf * T::kSumColumns + c * kPartsX + (uint32_t(32 * quarter) << 16),
+                                                     FMT == kNvfp4 && lane < T::kTake && c + lane < t.rows ? p.x_row[(long long)t.tile * T::kRowsX + c + lane] : 1.0f, inner, outer, ok, h);
                 if (c + T::kTake >= t.rows) {
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(smem_u32(&sum_empty[buf]));
-                }
-                float h[T::kTake];
-#pragma unroll
-                for (int q = 0; q < T::kTake; ++q) {
-                    float sum = __uint_as_float(v[(q * kPartsX + kPartsX - 1) / 8][(q * kPartsX + kPartsX - 1) % 8]);
-#pragma unroll
-                    for (int part = kPartsX - 2; part >= 0; --part) sum += __uint_as_float(v[(q * kPartsX + part) / 8][(q * kPartsX + part) % 8]);      // smallest first
-                    if constexpr (FMT == kNvfp4) sum = sum * inner * __shfl_sync(0xFFFFFFFFu, fx, q) * outer;
-                    h[q] = ok ? sum : __uint_as_float(0x7FC00000u);
                 }
                 if (splits > 1) {
 #pragma unroll
@@ -487,6 +493,185 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_kernel(const __gri
     if (warp == 1) {
         tc_fence_after();
         tmem_free(tmem, T::kColumns);
+    }
+}
+
+// More rows an item than a few, and many items: 256 rows of W an item, two halves of which share a stage's digits of x.  What binds the form above there is what comes out of L2 (9 to 10 TB/s:
+// 17 KB of W and as many of x for 524 clocks of products); here x is read half as often.  Of the sums' buffers there are three, a half of an item each.
+// (256 tokens to 8 of 64 experts, 2048 x 2816 with SwiGLU: mxfp4 71.7 -> 63.4 us, nvfp4, whose x is read for 18 rows an item where the form above has 21, 80.5 -> 78.0.)
+template <int FMT>
+struct WideTile {
+    static constexpr int kNt = FMT == kMxfp4 ? 128 : 112, kRowsX = kNt / kPartsX;      // (nvfp4's scales take twice the tensor memory)
+    static constexpr int kAtoms = Ms<FMT>::kAtoms, kBytesW = kRowsW * 128, kBytesS = kAtoms * 512;
+    static constexpr int kStageBytes = (2 * kBytesW + 3 * kBytesS + kNt * 128 + 1023) / 1024 * 1024, kStages = FMT == kMxfp4 ? 4 : 3;
+    static constexpr int kSums = 3, kScaleColumns = kAtoms * 4 * 3;
+    static constexpr int kSmem = kStages * kStageBytes + 1024;
+    static_assert(kSums * kNt + kStages * kScaleColumns <= 512 && kSmem >= 116 * 1024 && kSmem + sizeof(GroupPlan) + 1024 <= 227 * 1024 && (3 * kBytesS) % 1024 == 0);
+    static constexpr int kTake = 4, kPieces = (kTake * kPartsX + 7) / 8;
+};
+constexpr int kWideThreads = 320;                // loader, issuer, four warps for the results of each half
+
+template <int FMT>
+__global__ void __launch_bounds__(kWideThreads, 1) tcq_ms_grouped_wide_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ GroupedArgs p) {
+    using T = WideTile<FMT>;
+    extern __shared__ uint8_t raw[];
+    __shared__ GroupPlan plan;
+    __shared__ uint64_t full[T::kStages], empty[T::kStages], sum_full[2][T::kSums], sum_empty[T::kSums], drained;
+    __shared__ uint32_t tmem_at;
+    __shared__ unsigned int gave_up;
+    const uint32_t smem = (smem_u32(raw) + 1023) & ~1023u;
+    const int warp = __shfl_sync(0xFFFFFFFFu, int(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
+    const long long atoms = (long long)p.k_tiles * T::kAtoms;
+    constexpr long long kRecord = T::kBytesS + T::kNt * 128;
+    const int tiles_n2 = (p.tiles_n + 1) / 2;
+
+    const auto columns_of = [](const GroupItem& t) { return (t.rows * kPartsX + 7) & ~7; };
+    const auto halves_of = [&](const GroupItem& t) { return 2 * t.tn + 1 < p.tiles_n ? 2 : 1; };
+    if (warp == 0) {
+        if (elect_one()) {
+            gave_up = 0;
+            for (int s = 0; s < T::kStages; ++s) { mbar_init(smem_u32(&full[s]), 1); mbar_init(smem_u32(&empty[s]), 1); }
+            for (int s = 0; s < T::kSums; ++s) { mbar_init(smem_u32(&sum_full[0][s]), 1); mbar_init(smem_u32(&sum_full[1][s]), 1); mbar_init(smem_u32(&sum_empty[s]), 4); }
+            mbar_init(smem_u32(&drained), 1);
+            asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
+        }
+        __syncwarp();
+        plan_groups(p.groups, T::kRowsX, plan);
+    }
+    if (warp == 1) tmem_alloc(smem_u32(&tmem_at), 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_at, tmem_scales = tmem + T::kSums * T::kNt;
+    const int items = plan.tile[p.groups.groups] * tiles_n2;
+    const auto item_of = [&](int i) { return group_item(plan, p.groups.groups, tiles_n2, T::kRowsX, i); };
+
+    if (warp == 0) {
+        // ---- loads; the warp stays together, one lane issues
+        const bool one = elect_one();
+        wait_for_kernel_before();                        // x's digits are there
+        asm volatile("fence.proxy.async;" ::: "memory");
+        uint32_t s = 0, phase = 1, loaded = 0;           // (the first wait for a stage is for the phase before the first)
+        unsigned left = p.loads;
+        bool ok = true;
+        for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
+            const GroupItem t = item_of(i);
+            const int halves = halves_of(t), columns = columns_of(t);
+            const long long scales = ((long long)t.group * p.tiles_n + 2 * t.tn) * atoms;
+            for (int kt = 0; kt < p.k_tiles; ++kt) {
+                ok = still_waits(left-- > 0, smem_u32(&empty[s]), phase, &gave_up);      // every lane has seen this phase before the next can begin
+                if (!ok) break;
+                if (one) {
+                    const uint32_t to = smem + s * T::kStageBytes, bar = smem_u32(&full[s]), row = uint32_t(t.group * p.w.rows + t.tn * 2 * kRowsW);
+                    mbar_expect(bar, halves * (T::kBytesW + T::kBytesS) + T::kBytesS + columns * 128);
+                    for (int h = 0; h < halves; ++h) {
+                        tma_load(to + h * T::kBytesW, &map_w, kt * 128, int(row + h * kRowsW), bar);
+                        bulk_load(to + 2 * T::kBytesW + h * T::kBytesS, p.w.scales + (scales + h * atoms + (long long)kt * T::kAtoms) * 512, T::kBytesS, bar);
+                    }
+                    bulk_load(to + 2 * T::kBytesW + 2 * T::kBytesS, p.x + ((long long)t.tile * p.k_tiles + kt) * kRecord, T::kBytesS + columns * 128, bar);
+                }
+                __syncwarp();
+                if (++s == T::kStages) { s = 0; phase ^= 1; }
+                if (loaded < T::kStages) ++loaded;
+            }
+        }
+        wait_for_loads<T::kStages>(full, s, phase, loaded);
+    } else if (warp == 1) {
+        // ---- products; likewise
+        constexpr uint32_t kIdesc = 1u << 7 | 1u << 10 | (FMT == kMxfp4 ? 1u : 0u) << 23 | 1u << 27;
+        const bool one = elect_one();
+        uint32_t s = 0, phase = 0;
+        int n = 0;                                           // buffers of sums taken so far: two an item, a matrix's last one too, so that each waiter sees each phase of its barriers
+        bool ok = true;
+        for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
+            const GroupItem t = item_of(i);
+            const int halves = halves_of(t);
+            const uint32_t idesc0 = kIdesc | uint32_t(columns_of(t) >> 3) << 17;
+            uint32_t d[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int buf = (n + h) % T::kSums, use = (n + h) / T::kSums;
+                d[h] = tmem + buf * T::kNt;
+                if (use > 0) ok = ok && mbar_wait(smem_u32(&sum_empty[buf]), uint32_t(use - 1) & 1, &gave_up);
+            }
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            for (int kt = 0; kt < p.k_tiles; ++kt) {
+                ok = mbar_wait(smem_u32(&full[s]), phase, &gave_up);
+                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t at = smem + s * T::kStageBytes, sw = tmem_scales + s * T::kScaleColumns, sx = sw + 2 * T::kAtoms * 4;
+                const uint64_t dw = desc_rows128(at), dx = desc_rows128(at + 2 * T::kBytesW + 3 * T::kBytesS), ds = desc_rows16(at + 2 * T::kBytesW);
+                if (one) {
+#pragma unroll
+                    for (int j = 0; j < T::kAtoms; ++j) tc_copy_scales(sx + 4 * j, ds + (2 * T::kBytesS >> 4) + 32 * j);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (h >= halves) break;
+#pragma unroll
+                        for (int j = 0; j < T::kAtoms; ++j) tc_copy_scales(sw + h * T::kAtoms * 4 + 4 * j, ds + (h * T::kBytesS >> 4) + 32 * j);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {        // 64 columns: 32 bytes of a row, one word of scales (nvfp4) or half a word (mxfp4)
+                            const int atom = FMT == kNvfp4 ? j : j / 2;
+                            const uint32_t id = FMT == kNvfp4 ? 0u : 2u * (j % 2);
+                            mma_block_scaled<FMT>(d[h], dw + (h * T::kBytesW >> 4) + 2 * j, dx + 2 * j, idesc0 | id << 4 | id << 29, sw + h * T::kAtoms * 4 + 4 * atom, sx + 4 * atom, kt > 0 || j > 0);
+                        }
+                    }
+                    tc_commit(smem_u32(&empty[s]));
+                }
+                __syncwarp();
+                if (++s == T::kStages) { s = 0; phase ^= 1; }
+            }
+            if (ok && one)
+                for (int h = 0; h < 2; ++h) tc_commit(smem_u32(&sum_full[h][(n + h) % T::kSums]));
+            __syncwarp();
+            n += 2;
+        }
+        if (!ok) {                                           // what was issued ends before the tensor memory goes
+            if (one) tc_commit(smem_u32(&drained));
+            __syncwarp();
+            for (long long t0 = clock64(); !mbar_try_wait(smem_u32(&drained), 0) && clock64() - t0 < kMbarWaitCycles;) {}
+        }
+    } else {
+        // ---- results of one half: this warp's lanes are 32 rows of W, so that a store is 32 neighbours in y
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        wait_for_kernel_before();                            // rows' scales
+        bool ok = true;
+        for (int i = blockIdx.x, n = 0; i < items; i += gridDim.x, ++n) {
+            const GroupItem t = item_of(i);
+            const int buf = (2 * n + half) % T::kSums;       // (of each half, every third item: 0, 2, 1 and 1, 0, 2)
+            const long long r = (2ll * t.tn + half) * kRowsW + 32 * quarter + lane, column = (long long)t.group * p.w.rows + r;
+            const bool there = r < p.w.rows;
+            const float fw = FMT == kNvfp4 && there ? __ldg(p.w.row_scale + column) : 1.0f;
+            const float inner = inner_part(fw), outer = outer_part(fw);
+            const float bias = p.out.bias != nullptr && there ? load_as_f32(p.out.bias, p.out.bias_dtype, column) : 0.0f;
+            ok = still_waits(ok, smem_u32(&sum_full[half][buf]), uint32_t(n / T::kSums) & 1, &gave_up);
+            tc_fence_after();
+            const uint32_t from = tmem + buf * T::kNt + (uint32_t(32 * quarter) << 16);
+#pragma unroll 1
+            for (int c = 0; c < t.rows; c += T::kTake) {
+                float h[T::kTake];
+                take_rows<FMT, T::kTake, T::kPieces>(from + c * kPartsX, FMT == kNvfp4 && lane < T::kTake && c + lane < t.rows ? p.x_row[(long long)t.tile * T::kRowsX + c + lane] : 1.0f,
+                                                     inner, outer, ok, h);
+                if (c + T::kTake >= t.rows) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&sum_empty[buf]));
+                }
+#pragma unroll
+                for (int q = 0; q < T::kTake; ++q) h[q] += bias;
+                finish_rows(p.out, h, t.row0 + c, t.rows - c, r, there);
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_free(tmem, 512);
     }
 }
 
@@ -823,14 +1008,23 @@ int columns_for(long long rows, long long groups) {
     return 128;
 }
 
-template <typename T>
-cudaError_t launch_parts(const GroupedCall& c, const PartsArgs& p, cudaStream_t stream) {
+// The rows' scales, then the records, in the scratch.
+size_t parts_bytes(long long rows, long long groups, long long k, int fmt, int nt) {
+    const int per = nt / kPartsX;
+    const long long tiles = most_tiles(rows, groups, per);
+    return size_t((tiles * per * 4 + 255) / 256 * 256) + size_t(tiles) * size_t(ms_tiles_k(k)) * record_bytes(fmt, nt);
+}
+template <int FMT>
+cudaError_t launch_parts(const GroupedCall& c, int nt, void* ws, uint8_t** records, cudaStream_t stream) {
+    const int per = nt / kPartsX, k_tiles = int(ms_tiles_k(c.k));
+    *records = static_cast<uint8_t*>(ws) + (most_tiles(c.groups.rows, c.groups.groups, per) * per * 4 + 255) / 256 * 256;
+    const PartsArgs p{c.x, c.x_rows, c.ldx, c.tokens, c.groups, c.k, k_tiles, per, (long long)record_bytes(FMT, nt), ms_rows_aligned(c.x, c.ldx), *records, static_cast<float*>(ws)};
     // Threads of a row: all of its runs at once while there are few rows; fewer where many rows fill the SMs, since what a row takes of every thread (its group and place, its largest
-    // number) is as much as eight columns do (8192 rows of 2048 columns: 256 threads 73 us).
+    // number) is as much as eight columns do (8192 rows of 2048 columns: 256 threads 73 us, 64 64).
     const int rows = c.groups.rows, sms = ms_sm_count();
     const int threads = std::min(rows <= sms ? 512 : rows <= 4 * sms ? 256 : rows <= 16 * sms ? 128 : 64, p.k_tiles * 32);
     const unsigned grid = unsigned(std::min<long long>(rows, sms * 1536ll / threads));
-    return launch_programmatic(c.fmt == kNvfp4 ? tcq_ms_row_parts_kernel<T, kNvfp4> : tcq_ms_row_parts_kernel<T, kMxfp4>, dim3(grid), dim3(threads), 0, 0, stream, p);
+    return launch_programmatic(c.dtype == kF16 ? tcq_ms_row_parts_kernel<__half, FMT> : tcq_ms_row_parts_kernel<__nv_bfloat16, FMT>, dim3(grid), dim3(threads), 0, 0, stream, p);
 }
 
 // How many CTAs share the columns of an item: as many as leave each an SM of its own, and two pieces of 256 columns or more.
@@ -858,16 +1052,35 @@ cudaError_t launch(const GroupedCall& c, void* ws, cudaStream_t stream) {
     if ((err = make_byte_map(&map_w, c.w.codes, pitch, n * c.groups.groups, pitch, kRowsW)) != cudaSuccess) return err;
     const int k_tiles = int(ms_tiles_k(c.k));
     const long long tiles = most_tiles(c.groups.rows, c.groups.groups, T::kRowsX);
-    uint8_t* const records = static_cast<uint8_t*>(ws) + (tiles * T::kRowsX * 4 + 255) / 256 * 256;
-    const PartsArgs parts{c.x, c.x_rows, c.ldx, c.tokens, c.groups, c.k, k_tiles, T::kRowsX, (long long)record_bytes(FMT, NT),
-                          ms_rows_aligned(c.x, c.ldx), records, static_cast<float*>(ws)};
-    err = c.dtype == kF16 ? launch_parts<__half>(c, parts, stream) : launch_parts<__nv_bfloat16>(c, parts, stream);
-    if (err != cudaSuccess) return err;
+    uint8_t* records;
+    if ((err = launch_parts<FMT>(c, NT, ws, &records, stream)) != cudaSuccess) return err;
     const GroupedArgs p{c.w, c.groups, int((n + kRowsW - 1) / kRowsW), k_tiles, records, static_cast<const float*>(ws), c.out, c.loads};
     const long long items = tiles * p.tiles_n;
     const int splits = splits_for(kept, reinterpret_cast<const void*>(kernel), kThreads, T::kSmem, items, k_tiles);
     // (begins beside the kernel that makes the digits, and waits for it where it needs them)
     return launch_programmatic(kernel, dim3(unsigned(splits > 1 ? items * splits : std::min<long long>(items, ms_sm_count()))), dim3(kThreads), T::kSmem, splits, stream, map_w, p);
+}
+
+template <int FMT>
+cudaError_t launch_wide(const GroupedCall& c, void* ws, cudaStream_t stream) {
+    using T = WideTile<FMT>;
+    const auto kernel = tcq_ms_grouped_wide_kernel<FMT>;
+    static std::atomic<bool> ready[64];
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
+    if (err != cudaSuccess) return err;
+    if (dev >= 64 || !ready[dev]) {
+        if ((err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem)) != cudaSuccess) return err;
+        if (dev < 64) ready[dev] = true;
+    }
+    CUtensorMap map_w;
+    const long long pitch = ms_pitch(c.k), n = c.w.rows;
+    if ((err = make_byte_map(&map_w, c.w.codes, pitch, n * c.groups.groups, pitch, kRowsW)) != cudaSuccess) return err;
+    uint8_t* records;
+    if ((err = launch_parts<FMT>(c, T::kNt, ws, &records, stream)) != cudaSuccess) return err;
+    const GroupedArgs p{c.w, c.groups, int((n + kRowsW - 1) / kRowsW), int(ms_tiles_k(c.k)), records, static_cast<const float*>(ws), c.out, c.loads};
+    const long long items = most_tiles(c.groups.rows, c.groups.groups, T::kRowsX) * ((p.tiles_n + 1) / 2);
+    return launch_programmatic(kernel, dim3(unsigned(std::min<long long>(items, ms_sm_count()))), dim3(kWideThreads), T::kSmem, 0, stream, map_w, p);
 }
 
 template <typename XT, int FMT, int NT>
@@ -894,6 +1107,15 @@ cudaError_t launch_few(const GroupedCall& c, cudaStream_t stream) {
     return launch_programmatic(kernel, dim3(unsigned(splits > 1 ? items * splits : std::min<long long>(items, ms_sm_count()))), dim3(kFewThreads), T::kSmem, splits, stream, map_w, p);
 }
 
+// Whether items of 256 rows of W take fewer of the SMs' turns: one such is as long as 1.75 of 128 rows.  (200 tokens to 4 of 32 experts, 2048 x 2000 mxfp4: 544 items and 26.0 us; 1088 and
+// 28.2.  60 rows through 4096 x 12288 nvfp4: 192 items of 18 rows, two turns, 22.8 us; 288 of 21 rows, two turns, 17.3.)
+bool wide_items(long long rows, long long groups, long long n, int fmt) {
+    if (columns_for(rows, groups) != 128) return false;
+    const long long sms = ms_sm_count(), wide_nt = fmt == kNvfp4 ? WideTile<kNvfp4>::kNt : WideTile<kMxfp4>::kNt;
+    const long long wide = most_tiles(rows, groups, wide_nt / kPartsX) * ((n + 255) / 256), narrow = most_tiles(rows, groups, 128 / kPartsX) * ((n + 127) / 128);
+    return 7 * ((wide + sms - 1) / sms) <= 4 * ((narrow + sms - 1) / sms);
+}
+
 // Whether x is cut up where it is multiplied: one or two rows an item, its columns held by a CTA whatever the split, and few enough items, or only those of the same rows.
 bool cut_in_place(long long rows, long long groups, long long n, long long k, int fmt) {
     const int nt = columns_for(rows, groups);
@@ -911,6 +1133,7 @@ cudaError_t launch_cut(const GroupedCall& c, cudaStream_t stream) {
 
 template <int FMT>
 cudaError_t launch_nt(const GroupedCall& c, void* ws, cudaStream_t stream) {
+    if (wide_items(c.groups.rows, c.groups.groups, c.w.rows, FMT)) return launch_wide<FMT>(c, ws, stream);
     switch (columns_for(c.groups.rows, c.groups.groups)) {
         case 8: return launch<FMT, 8>(c, ws, stream);
         case 16: return launch<FMT, 16>(c, ws, stream);
@@ -924,7 +1147,7 @@ cudaError_t launch_nt(const GroupedCall& c, void* ws, cudaStream_t stream) {
 
 // Whether weights as 16-bit numbers pay: they are made once for up to 256 rows, where digits take six columns a row, and are made anew for each row.  Both forms' times as measured, us: a
 // step of 64 columns of 128 rows of W takes 0.33 to 0.5 with 16-bit weights; 256 columns 0.29 (mxfp4) or 0.35 with digits, which cost 3.2 for a million numbers of x.  (64 rows a group, 2816 x
-// 2048: 132 and 143 in nvfp4, 134 and 123 in mxfp4; 100 rows through 4096 x 4096: 27 and 15, as 16-bit weights have only 32 SMs busy.)
+// 2048: 134 and 134 in nvfp4, 131 and 111 in mxfp4; 96: 143 and 199, 152 and 155; 100 rows through 4096 x 4096: 27 and 15, as 16-bit weights have only 32 SMs busy.)
 static bool many_rows(long long rows, long long groups, long long n, long long k, int dtype, int fmt) {
     if (!ms_grouped_many_takes(dtype, fmt) || rows <= 32 * std::min(groups, rows)) return false;
     const double filled = double(std::min(groups, rows)), sms = ms_sm_count(), across = double((n + kRowsW - 1) / kRowsW);
@@ -941,9 +1164,8 @@ static bool many_rows(long long rows, long long groups, long long n, long long k
 size_t ms_grouped_workspace_bytes(long long rows, long long groups, long long n, long long k, int dtype, int fmt, bool in_order) {
     if (many_rows(rows, groups, n, k, dtype, fmt)) return in_order ? 0 : ms_grouped_many_workspace_bytes(rows, k);
     if (cut_in_place(rows, groups, n, k, fmt)) return 0;
-    const int nt = columns_for(rows, groups), per = nt / kPartsX;
-    const long long tiles = most_tiles(rows, groups, per);
-    return size_t((tiles * per * 4 + 255) / 256 * 256) + size_t(tiles) * size_t(ms_tiles_k(k)) * record_bytes(fmt, nt);
+    const int wide = fmt == kNvfp4 ? WideTile<kNvfp4>::kNt : WideTile<kMxfp4>::kNt;
+    return parts_bytes(rows, groups, k, fmt, wide_items(rows, groups, n, fmt) ? wide : columns_for(rows, groups));
 }
 
 cudaError_t launch_ms_grouped(const GroupedCall& c, void* ws, cudaStream_t stream) {
