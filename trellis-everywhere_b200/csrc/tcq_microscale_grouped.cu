@@ -1145,19 +1145,22 @@ cudaError_t launch_nt(const GroupedCall& c, void* ws, cudaStream_t stream) {
 
 }  // namespace
 
-// Whether weights as 16-bit numbers pay: they are made once for up to 256 rows, where digits take six columns a row, and are made anew for each row.  Both forms' times as measured, us: a
-// step of 64 columns of 128 rows of W takes 0.33 to 0.5 with 16-bit weights; 256 columns 0.29 (mxfp4) or 0.35 with digits, which cost 3.2 for a million numbers of x.  (64 rows a group, 2816 x
-// 2048: 134 and 134 in nvfp4, 131 and 111 in mxfp4; 96: 143 and 199, 152 and 155; 100 rows through 4096 x 4096: 27 and 15, as 16-bit weights have only 32 SMs busy.)
+// Whether weights as 16-bit numbers pay: they are made once for up to 256 rows, where digits take six columns a row, and are made anew for each row.  Both forms' estimated times, us, fitted to
+// 76 pairs of measured ones of 48 to 18000 rows (off by 15 %; the form chosen is 0.4 % slower than the faster one on average, 17 % at most): with 16-bit weights 0.35 a step of 64 columns and
+// 0.025 a row of x; with digits 0.13 (mxfp4) or 0.17 a step of 256 columns, 1.9 an item and 3.2 a million numbers of x.  (64 rows a group, 2816 x 2048: 134 and 134 in nvfp4, 131 and 111 in
+// mxfp4; 96 rows: 143 and 199, 152 and 155; 100 rows through 4096 x 4096 mxfp4: 24 and 13.)  A call whose rows are put in order first takes 2 longer, but the same form.
 static bool many_rows(long long rows, long long groups, long long n, long long k, int dtype, int fmt) {
     if (!ms_grouped_many_takes(dtype, fmt) || rows <= 32 * std::min(groups, rows)) return false;
     const double filled = double(std::min(groups, rows)), sms = ms_sm_count(), across = double((n + kRowsW - 1) / kRowsW);
-    const int per = columns_for(rows, groups) / kPartsX;
-    const auto turns = [&](int per_item) {
-        if (groups == 1) return std::ceil(double((rows + per_item - 1) / per_item) * across / sms);
-        return std::max(filled, double(rows) / per_item + 0.5 * filled) * across / sms + 0.5;
+    const auto turns = [&](int per) {
+        if (groups == 1) return std::ceil(double((rows + per - 1) / per) * across / sms);
+        const double items = std::max(filled, double(rows) / per + 0.5 * filled) * across / sms;
+        return items <= 1 ? 1.0 : items + 0.5;
     };
-    const double many = 6.0 + turns(256) * double((k + 63) / 64) * (0.33 + 0.17 * std::min(1.0, double(rows) / filled / 256));
-    const double digits = 8.0 + turns(per) * double(ms_tiles_k(k)) * (fmt == kNvfp4 ? 0.35 : 0.29) + 3.2e-6 * double(rows) * double(k);
+    const int per = ms_grouped_many_rows(rows, groups, n);
+    const double many = 4.0 + turns(per) * (0.35 * double((k + 63) / 64) + 0.025 * std::min(double(per), double(rows) / filled));
+    const double step = fmt == kNvfp4 ? 0.17 : wide_items(rows, groups, n, fmt) ? 0.11 : 0.13;
+    const double digits = 5.5 + turns(columns_for(rows, groups) / kPartsX) * (step * double(ms_tiles_k(k)) + 1.9) + 3.2e-6 * double(rows) * double(k);
     return many < digits;
 }
 

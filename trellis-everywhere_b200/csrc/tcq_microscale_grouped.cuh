@@ -27,6 +27,7 @@ inline bool ms_rows_aligned(const void* x, long long ldx) { return reinterpret_c
 // tcq_microscale_grouped_many.cu: weights as 16-bit numbers, for many rows a group and x of a type that the weights are numbers of.  Scratch only for rows that are
 // gathered, or that TMA loads cannot start at.
 inline bool ms_grouped_many_takes(int dtype, int fmt) { return dtype == kBf16 || (dtype == kF16 && fmt == kNvfp4); }
+int ms_grouped_many_rows(long long rows, long long groups, long long n);
 size_t ms_grouped_many_workspace_bytes(long long rows, long long k);
 cudaError_t launch_ms_grouped_many(const GroupedCall& c, void* ws, cudaStream_t stream);
 

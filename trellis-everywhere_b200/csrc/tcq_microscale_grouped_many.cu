@@ -5,7 +5,7 @@
 // x are the right operand, by TMA; an item takes as many columns as it has rows.  Rows that are gathered are put in order first.  (TMA loads of four rows of any numbers each took twice as long
 // for all.)
 //
-// Work split: one CTA per SM goes through items of 128 rows of a matrix x up to 256 rows of its group.  One warp loads (codes and scales of 256 columns, x of 64), one issues
+// Work split: one CTA per SM goes through items of 128 rows of a matrix x up to 256 rows of its group, of fewer where there are fewer such than SMs.  One warp loads (codes and scales of 256 columns, x of 64), one issues
 // products, two groups of four make weights in turn, eight take finished sums out of tensor memory.  The sums of 128 rows are a buffer, of which there are three: the next item
 // begins when the first half of the last one's sums has been taken.  x and weights of 64 columns are one stage of one ring, with one barrier that says that both are there and one
 // that they are no longer needed: what a stage takes beside its products is waits and arrivals (0.3 us with neither products nor weights made; a third group of makers makes it longer).
@@ -42,6 +42,7 @@ struct ManyArgs {
     MsMatrix w;
     Groups groups;
     int tiles_n, steps;                          // steps of 64 columns
+    int per;                                     // rows of x an item, at most
     long long atoms;                             // of scales a row group
     Epilogue out;
     unsigned loads;
@@ -102,13 +103,13 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_many_kernel(const 
     if (warp == 1) tmem_alloc(smem_u32(&tmem_at), T::kColumns);
     wait_for_kernel_before();
     launch_dependents();
-    if (warp == 2) plan_groups(p.groups, kNt, plan);
+    if (warp == 2) plan_groups(p.groups, p.per, plan);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_at, tmem_a = tmem + T::kSums * kHalf;
     const int items = plan.tile[p.groups.groups] * p.tiles_n;
-    const auto item_of = [&](int i) { return group_item<true>(plan, p.groups.groups, p.tiles_n, kNt, i); };
+    const auto item_of = [&](int i) { return group_item<true>(plan, p.groups.groups, p.tiles_n, p.per, i); };
 
     if (warp == 0) {
         // ---- loads; the warp stays together, one lane issues
@@ -280,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_many_kernel(const 
     } else {
         // ---- results: this warp's lanes are 32 rows of W, so that a store is 32 neighbours in y
         const int quarter = warp & 3, mine = (warp - kFirstTaker) >> 2;
-        constexpr int kChunk = 16, kShare = kHalf / kTakers;                     // columns of a buffer that are this warp's
+        constexpr int kChunk = 16;
         int n = 0;
         bool ok = true;
         for (int i = blockIdx.x; i < items; i += gridDim.x) {
@@ -294,7 +295,8 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_many_kernel(const 
                 ok = still_waits(ok, smem_u32(&sum_full[buf]), uint32_t(n / T::kSums) & 1, &gave_up);
                 tc_fence_after();
                 const float plus = ok ? bias : __uint_as_float(0x7FC00000u);
-                const int first = mine * kShare, last = min(first + kShare, t.rows - half);
+                const int columns = min(kHalf, t.rows - half), share = (columns + kTakers * kChunk - 1) / (kTakers * kChunk) * kChunk;
+                const int first = mine * share, last = min(first + share, columns);          // those of the buffer that are this warp's
 #pragma unroll 1
                 for (int c0 = first; c0 < last; c0 += kChunk) {
                     uint32_t v[kChunk];
@@ -361,12 +363,22 @@ cudaError_t launch(const GroupedCall& c, cudaStream_t stream) {
     const long long pitch = ms_pitch(c.k), n = c.w.rows;
     if ((err = make_byte_map(&map_w, c.w.codes, pitch, n * c.groups.groups, pitch, kRows)) != cudaSuccess) return err;
     if ((err = make_16bit_map(&map_x, c.x, c.k, c.x_rows, c.ldx, kBoxRows)) != cudaSuccess) return err;
-    const ManyArgs p{c.w, c.groups, int((n + kRows - 1) / kRows), int((c.k + kStepK - 1) / kStepK), ms_tiles_k(c.k) * T::kAtoms, c.out, c.loads};
-    const long long items = most_tiles(c.groups.rows, c.groups.groups, kNt) * p.tiles_n;
+    const ManyArgs p{c.w, c.groups, int((n + kRows - 1) / kRows), int((c.k + kStepK - 1) / kStepK), ms_grouped_many_rows(c.groups.rows, c.groups.groups, n), ms_tiles_k(c.k) * T::kAtoms, c.out, c.loads};
+    const long long items = most_tiles(c.groups.rows, c.groups.groups, p.per) * p.tiles_n;
     return launch_programmatic(kernel, dim3(unsigned(std::min<long long>(items, ms_sm_count()))), dim3(kThreads), T::kSmem, 0, stream, map_w, map_x, p);
 }
 
 }  // namespace
+
+// Rows of x an item: as few (by sixteens, as the products count, and one box of loads at least) as leave no more items than SMs; 256, for which weights are made once, where there are more.
+// (1662 rows of 3 groups, 152 x 347: 32 rows an item 10.4 us, 256 16.9; 1000 rows through 1000 x 1111: 64 rows 13.7, 256 18.2.)
+int ms_grouped_many_rows(long long rows, long long groups, long long n) {
+    const long long filled = std::min(rows, groups), tiles = ms_sm_count() / ((n + kRows - 1) / kRows);      // of rows, that an SM each can have
+    long long per = kNt;
+    if (groups == 1 && tiles > 0) per = (rows + tiles - 1) / tiles;
+    else if (tiles > filled) per = (rows - filled + tiles - filled - 1) / (tiles - filled);                  // most_tiles() of it is `tiles` at most
+    return int(std::min<long long>(kNt, std::max<long long>(kBoxRows, (per + 15) / 16 * 16)));
+}
 
 size_t ms_grouped_many_workspace_bytes(long long rows, long long k) { return size_t(rows) * size_t((k + 7) / 8 * 16); }
 
