@@ -5,10 +5,14 @@
 // x are the right operand, by TMA; an item takes as many columns as it has rows.  Rows that are gathered are put in order first.  (TMA loads of four rows of any numbers each took twice as long
 // for all.)
 //
-// Work split: one CTA per SM goes through items of 128 rows of a matrix x up to 256 rows of its group, of fewer where there are fewer such than SMs.  One warp loads (codes and scales of 256 columns, x of 64), one issues
-// products, two groups of four make weights in turn, eight take finished sums out of tensor memory.  The sums of 128 rows are a buffer, of which there are three: the next item
-// begins when the first half of the last one's sums has been taken.  x and weights of 64 columns are one stage of one ring, with one barrier that says that both are there and one
-// that they are no longer needed: what a stage takes beside its products is waits and arrivals (0.3 us with neither products nor weights made; a third group of makers makes it longer).
+// Work split: one CTA per SM goes through items of 128 rows of a matrix x up to 256 rows of its group, of fewer where there are fewer such than SMs.  One warp loads codes and scales of
+// 256 columns, another x of 64, one issues products, two groups of four make weights in turn, eight take finished sums out of tensor memory.  The sums of 128 rows are a buffer, of which there
+// are three: the next item begins when the first half of the last one's sums has been taken.  x and weights of 64 columns are one stage of one ring, with one barrier that says that both are
+// there and one that they are no longer needed.
+//
+// Measured: 2000 rows through 12288 x 4096 nvfp4 (fp16, GELU) 161 to 177 us, 1.1 to 1.25 PFLOP/s, 2040 tokens to 8 of 64 experts of 2816 x 2048 230 to 250; 15 % longer in long runs, at the power
+// limit.  What a stage takes beside its products is waits and arrivals (0.2 to 0.3 us with neither products nor weights made; x in boxes of 64 or 128 rows, stages of half as many
+// rows and twice as many of them, a third group of makers: no change; a fourth in place of takers 20 % longer).
 //
 // A wait that runs out (kMbarWaitCycles) makes its CTA stop, and its results from there on NaN.
 #include <algorithm>
@@ -23,7 +27,7 @@ namespace tcq {
 namespace {
 
 constexpr int kMakers = 2, kTakers = 2;          // groups of four warps
-constexpr int kFirstTaker = 2, kFirstMaker = 2 + 4 * kTakers, kThreads = 32 * (2 + 4 * kTakers + 4 * kMakers);
+constexpr int kFirstTaker = 2, kFirstMaker = 2 + 4 * kTakers, kLoaderW = kFirstMaker + 4 * kMakers, kThreads = 32 * (kLoaderW + 1);
 constexpr int kRows = 128, kStepK = 64, kNt = 256, kHalf = 128;
 constexpr int kBoxRows = 32;
 
@@ -112,28 +116,14 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_many_kernel(const 
     const auto item_of = [&](int i) { return group_item<true>(plan, p.groups.groups, p.tiles_n, p.per, i); };
 
     if (warp == 0) {
-        // ---- loads; the warp stays together, one lane issues
+        // ---- loads of x; the warp stays together, one lane issues
         const bool one = elect_one();
-        uint32_t sw = 0, pw = 1, s = 0, phase = 1, loaded_w = 0, loaded = 0;      // (the first waits are for the phase before the first)
-        unsigned left = p.loads;
+        uint32_t s = 0, phase = 1, loaded = 0;           // (the first waits are for the phase before the first)
         bool ok = true;
         for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
             const GroupItem t = item_of(i);
             const int boxes = (t.rows + kBoxRows - 1) / kBoxRows;
             for (int step = 0; step < p.steps; ++step) {
-                if (step % 4 == 0) {
-                    ok = still_waits(left-- > 0, smem_u32(&w_empty[sw]), pw, &gave_up) && !__any_sync(0xFFFFFFFFu, gave_up);
-                    if (!ok) break;
-                    if (one) {
-                        const uint32_t to = smem_w + sw * T::kStageW, bar = smem_u32(&w_full[sw]);
-                        mbar_expect(bar, T::kBytesW + T::kBytesS);
-                        tma_load(to, &map_w, step * 32, int(t.group * p.w.rows + t.tn * kRows), bar);
-                        bulk_load(to + T::kBytesW, p.w.scales + (((long long)t.group * p.tiles_n + t.tn) * p.atoms + (long long)(step / 4) * T::kAtoms) * 512, T::kBytesS, bar);
-                    }
-                    __syncwarp();
-                    if (++sw == T::kStagesW) { sw = 0; pw ^= 1; }
-                    if (loaded_w < T::kStagesW) ++loaded_w;
-                }
                 ok = still_waits(ok, smem_u32(&empty[s]), phase, &gave_up);
                 if (!ok) break;
                 if (one) {
@@ -146,8 +136,30 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_many_kernel(const 
                 if (loaded < T::kStages) ++loaded;
             }
         }
-        wait_for_loads<T::kStagesW>(w_full, sw, pw, loaded_w);
         wait_for_loads<T::kStages>(full, s, phase, loaded);
+    } else if (warp == kLoaderW) {
+        // ---- loads of W, which are not held up by those of x: as far ahead as there is room
+        const bool one = elect_one();
+        uint32_t sw = 0, pw = 1, loaded = 0;
+        unsigned left = p.loads;
+        bool ok = true;
+        for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
+            const GroupItem t = item_of(i);
+            for (int step = 0; step < p.steps; step += 4) {
+                ok = still_waits(left-- > 0, smem_u32(&w_empty[sw]), pw, &gave_up) && !__any_sync(0xFFFFFFFFu, gave_up);
+                if (!ok) break;
+                if (one) {
+                    const uint32_t to = smem_w + sw * T::kStageW, bar = smem_u32(&w_full[sw]);
+                    mbar_expect(bar, T::kBytesW + T::kBytesS);
+                    tma_load(to, &map_w, step * 32, int(t.group * p.w.rows + t.tn * kRows), bar);
+                    bulk_load(to + T::kBytesW, p.w.scales + (((long long)t.group * p.tiles_n + t.tn) * p.atoms + (long long)(step / 4) * T::kAtoms) * 512, T::kBytesS, bar);
+                }
+                __syncwarp();
+                if (++sw == T::kStagesW) { sw = 0; pw ^= 1; }
+                if (loaded < T::kStagesW) ++loaded;
+            }
+        }
+        wait_for_loads<T::kStagesW>(w_full, sw, pw, loaded);
     } else if (warp == 1) {
         // ---- products; likewise
         constexpr uint32_t kIdesc = 1u << 4 | (FP16 ? 0u : 1u << 7 | 1u << 10) | uint32_t(kRows >> 4) << 24;      // bf16 x bf16 (or fp16 x fp16), fp32 sums
