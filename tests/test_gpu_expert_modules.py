@@ -104,3 +104,15 @@ def test_linear_with_an_activation(dtype):
                 lambda: MicroscaledLinear(w, b, activations=4)(x, x.new_ones(2, 5, 96))):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_a_linear_layer_saved_without_an_activation():
+    """A module's state as it was before there were activations."""
+    import copy
+
+    from trellis_b200 import quant
+    layer = quant.MicroscaledLinear(rnd(0)(96, 64), rnd(1)(96))
+    old = copy.deepcopy(layer)
+    del old.__dict__["activation"]
+    x = rnd(2)(5, 64).bfloat16()
+    assert torch.equal(old(x), layer(x)) and torch.equal(old(x, x.new_zeros(5, 96)), layer(x, x.new_zeros(5, 96))) and repr(old) == repr(layer)

@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kThreads) tcq_route_choose_kernel(const __grid
     for (int e = threadIdx.x; e < c.experts; e += kThreads) count[e] = 0;
     for (int t = t0 + warp; t < t1; t += kWarps) choose_any(c, t);
     __syncthreads();
-    for (int i = t0 * c.top + threadIdx.x; i < t1 * c.top; i += kThreads) {
+    for (uint32_t i = t0 * c.top + threadIdx.x; i < uint32_t(t1 * c.top); i += kThreads) {      // (of up to 2^31 - 1)
         const int e = c.chosen[i];
         if (e >= 0) atomicAdd(&count[e], 1);
     }

@@ -105,6 +105,8 @@ class MicroscaledLinear(nn.Module):
     applied to the sums of the product, bias included, before they are rounded (``activations=16``).
     """
 
+    activation: Optional[str] = None                        # (of modules that were saved without one)
+
     def __init__(self, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, fmt: str = "nvfp4", activations: int = 16,
                  rotate: int = 0, seed: int = 0, activation: Optional[str] = None):
         super().__init__()
