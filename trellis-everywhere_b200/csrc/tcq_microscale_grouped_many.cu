@@ -338,24 +338,28 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_many_kernel(const 
     }
 }
 
-// Rows of 16-bit numbers in order, zeros up to a multiple of eight columns; rows that x has not are NaN.
-__global__ void __launch_bounds__(256) tcq_ms_grouped_rows_kernel(const uint16_t* __restrict__ x, long long x_rows, long long k, long long ldx, const int* __restrict__ tokens,
-                                                                  long long rows, uint16_t* __restrict__ out, long long runs, bool wide) {
+// Rows of 16-bit numbers in order, zeros up to a multiple of eight columns; rows that x has not are NaN.  Threads in x: eight columns of a row each; in y: rows.
+__global__ void __launch_bounds__(256) tcq_ms_grouped_rows_kernel(const uint16_t* __restrict__ x, long long x_rows, long long k, long long ldx, const int* __restrict__ tokens, int rows,
+                                                                  uint4* __restrict__ out, int runs, bool wide) {
     wait_for_kernel_before();
     launch_dependents();
-    for (long long id = (long long)blockIdx.x * 256 + threadIdx.x; id < rows * runs; id += (long long)gridDim.x * 256) {
-        const long long i = id / runs, c0 = (id - i * runs) * 8, token = tokens != nullptr ? __ldg(tokens + i) : i;
+    for (long long i = (long long)blockIdx.x * blockDim.y + threadIdx.y; i < rows; i += (long long)gridDim.x * blockDim.y) {
+        const long long token = tokens != nullptr ? __ldg(tokens + i) : i;
         const bool there = token >= 0 && token < x_rows;
-        uint32_t w[4] = {};
-        if (wide && there) {
-            const uint4 u = __ldg(reinterpret_cast<const uint4*>(x + token * ldx + c0));
-            w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-        } else {
+        const uint16_t* const from = x + token * ldx;
+        for (int j = threadIdx.x; j < runs; j += blockDim.x) {
+            const long long c0 = 8ll * j;
+            uint32_t w[4] = {};
+            if (wide && there) {
+                const uint4 u = __ldg(reinterpret_cast<const uint4*>(from + c0));
+                w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+            } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (c0 + j < k) w[j / 2] |= (there ? uint32_t(x[token * ldx + c0 + j]) : 0x7FFFu) << (16 * (j & 1));
+                for (int q = 0; q < 8; ++q)
+                    if (c0 + q < k) w[q / 2] |= (there ? uint32_t(from[c0 + q]) : 0x7FFFu) << (16 * (q & 1));
+            }
+            out[i * runs + j] = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        reinterpret_cast<uint4*>(out)[id] = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 
@@ -398,9 +402,11 @@ cudaError_t launch_ms_grouped_many(const GroupedCall& call, void* ws, cudaStream
     GroupedCall c = call;
     if (c.tokens != nullptr || !ms_rows_aligned(c.x, c.ldx)) {      // in order, where TMA loads can start
         const long long runs = (c.k + 7) / 8;
-        const cudaError_t err = launch_programmatic(tcq_ms_grouped_rows_kernel, dim3(unsigned(std::min<long long>((c.groups.rows * runs + 255) / 256, 1 << 20))), dim3(256), 0, 0, stream,
-                                                    static_cast<const uint16_t*>(c.x), c.x_rows, c.k, c.ldx, c.tokens, (long long)c.groups.rows, static_cast<uint16_t*>(ws), runs,
-                                                    c.k % 8 == 0 && ms_rows_aligned(c.x, c.ldx));
+        dim3 block(32, 8);
+        while (block.x < 256 && block.x < runs) { block.x *= 2; block.y /= 2; }
+        const unsigned grid = unsigned(std::min<long long>((c.groups.rows + block.y - 1) / block.y, 1 << 20));
+        const cudaError_t err = launch_programmatic(tcq_ms_grouped_rows_kernel, dim3(grid), block, 0, 0, stream, static_cast<const uint16_t*>(c.x), c.x_rows, c.k, c.ldx, c.tokens,
+                                                    c.groups.rows, static_cast<uint4*>(ws), int(runs), c.k % 8 == 0 && ms_rows_aligned(c.x, c.ldx));
         if (err != cudaSuccess) return err;
         c.x = ws;
         c.x_rows = c.groups.rows;
