@@ -235,3 +235,35 @@ def test_waits_for_matrices_of_many_rows_that_run_out(fmt):
         torch.cuda.synchronize()
         assert bool((y.isnan() | (y == want)).all()) and bool(y.isnan().any()) and (loads < 2 or bool((y == want).any()))
     assert torch.equal(experts.grouped_linear(x, w, offsets), want)
+
+
+@pytest.mark.parametrize("rows,n,k,dtype", [(66000, 33000, 64, torch.bfloat16), (1050000, 40, 2056, torch.float16), (1050000, 130, 2049, torch.bfloat16)])
+def test_more_bytes_than_31_bits_count(rows, n, k, dtype):
+    """Results, or rows of x (where they lie, and put in order), of more than 2^31 bytes: the first and last rows and one between, which are other forms' than a small call's."""
+    from trellis_b200 import experts, microscale as ms
+    fmt = "nvfp4"
+    g = torch.Generator(device=DEV).manual_seed(0)
+    w = experts.quantize_experts(torch.randn(2, n, k, generator=g, device=DEV) * k ** -0.5, fmt)
+    x = torch.empty(rows, k, dtype=dtype, device=DEV)
+    ends = torch.randn(600, k, generator=g, device=DEV).to(dtype)
+    x[:300], x[300:-300], x[-300:] = ends[:300], 1, ends[300:]
+    y = experts.grouped_linear(x, w, torch.tensor([0, 300, rows], device=DEV).int(), activation="swiglu")
+    assert rows * max(n // 2, k) > 2 ** 30
+    for e, at in ((0, slice(0, 300)), (1, slice(rows // 2, rows // 2 + 1)), (1, slice(rows - 300, rows))):
+        one, xd = ms.dequantize(experts.expert(w, e)).double(), x[at].double()
+        want, bound = plain.epilogue(xd @ one.t(), plain.sums_bound(xd, one, fmt), None, "swiglu", None, dtype)
+        assert bool(((y[at].double() - want).abs() <= bound).all())
+
+
+def test_combining_more_numbers_than_31_bits_count():
+    from trellis_b200 import experts
+    for n in (2048, 2051):
+        tokens, g = 1060000, torch.Generator(device=DEV).manual_seed(0)
+        y = torch.randn(64, n, generator=g, device=DEV).bfloat16()
+        places = torch.randint(0, 64, (tokens, 2), generator=g, device=DEV).int()
+        weights = torch.rand(tokens, 2, generator=g, device=DEV)
+        out = experts.combine(y, experts.Routing(weights, places, places, places.flatten(), places.flatten()))
+        assert out.numel() > 2 ** 31
+        for at in (slice(0, 40), slice(tokens // 2, tokens // 2 + 40), slice(tokens - 40, tokens)):
+            p, v = places[at].contiguous(), weights[at].contiguous()
+            assert torch.equal(out[at], experts.combine(y, experts.Routing(v, p, p, p.flatten(), p.flatten())))
