@@ -678,7 +678,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) tcq_ms_grouped_wide_kernel(co
 }
 
 // One or two rows an item, cut up by the CTA that multiplies them: one launch, and x goes from global memory to what the tensor cores read without a way round.  What a CTA's columns of x
-become stays in shared memory while its items are of the same rows.  Bound by latency: one row through 4096 x 4096 nvfp4 6.9 us, one token to 8 of 64 experts of 2048 x 2048 7.5 (2.5 TB/s of weights).
+// become stays in shared memory while its items are of the same rows.  Bound by latency: one row through 4096 x 4096 nvfp4 6.9 us, one token to 8 of 64 experts of 2048 x 2048 7.5 (2.5 TB/s of weights).
 template <int FMT, int NT>
 struct FewTile {
     static constexpr int kAtoms = Ms<FMT>::kAtoms, kRowsX = NT / kPartsX;
