@@ -39,6 +39,8 @@ struct Tile {
     static constexpr int kSums = 3, kColumnsA = kStepK / 2;                                                          // weights in tensor memory
     static constexpr int kColumns = 512;
     static constexpr int kSmem = (kStagesW * kStageW + 1023) / 1024 * 1024 + kStages * kBytesX + 1024;
+    // A maker's wait for the stage of step u is for the products of step u - kStages, and is theirs only if those of u - 2 kStages are done: its wait before was for u - kMakers - kStages.
+    static_assert(kMakers <= kStages);
     static_assert(kSums * kHalf + kStages * kColumnsA <= kColumns && kSmem + sizeof(GroupPlan) + 1024 <= 227 * 1024 && kSmem >= 116 * 1024);
 };
 
