@@ -752,7 +752,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tcq_ms_grouped_few_kernel(cons
     if (warp == 0 && elect_one()) {
         gave_up = 0;
         for (uint32_t s = 0; s < stages; ++s) { mbar_init(smem_u32(&full[s]), 1); mbar_init(smem_u32(&empty[s]), 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&sum_full[s]), 1); mbar_init(smem_u32(&sum_empty[s]), 4); }
+        for (int s = 0; s < 2; ++s) { mbar_init(smem_u32(&sum_full[s]), 1); mbar_init(smem_u32(&sum_empty[s]), kCutters); }
         mbar_init(smem_u32(&x_there), kCutters);
         mbar_init(smem_u32(&drained), 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
@@ -956,7 +956,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) tcq_ms_grouped_few_kernel(cons
                 if (lane == 0) mbar_arrive(smem_u32(&x_there));
             }
             if (!takes) {
+                // (an arrival of its own: the phase after the next of this barrier would answer this wait like the one before it, so it may not begin before this warp has seen its own)
                 ok = still_waits(ok, smem_u32(&sum_full[buf]), uint32_t(n / 2) & 1, &gave_up);
+                if (lane == 0) mbar_arrive(smem_u32(&sum_empty[buf]));
                 continue;
             }
             const long long r = (long long)t.tn * kRowsW + 32 * quarter + lane;
