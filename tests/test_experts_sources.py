@@ -45,3 +45,17 @@ def test_every_warp_that_waits_for_sums_is_counted():
     arrivals = 8 if count == "kCutters" else int(count)
     assert len(re.findall(r"mbar_arrive\(smem_u32\(&sum_empty\[buf\]\)\)", body)) == (2 if arrivals == 8 else 1)
     assert phases_missed(8, 4, 3) and not phases_missed(8, arrivals, 3)
+
+
+def test_kernels_that_begin_early_have_no_read_only_loads():
+    """Read-only loads are defined for memory that nobody writes while the kernel runs, and these kernels run while the one before still writes; what is loaded by assembly stays where it stands."""
+    around = [f for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh")) and ("experts" in f or "grouped" in f or "groups" in f or "epilogue" in f or "programmatic" in f)]
+    assert len(around) >= 8 and {"tcq_experts.cu", "tcq_microscale_grouped.cu", "tcq_microscale_grouped_many.cu", "tcq_microscale_epilogue.cuh", "tcq_microscale_groups.cuh"} <= set(around)
+    for f in os.listdir(CSRC):
+        if f.endswith((".cu", ".cuh")) and "launch_programmatic(" in source(f):
+            assert f in around
+    for f in around:
+        text = source(f)
+        assert not re.search(r"__ldg|\.nc\b|__restrict__", text), f
+        for load in re.finditer(r"asm( volatile)?\((?:\s*\"[^\"]*\")*?\s*\"[^\"]*\bld\.(?:relaxed\.gpu\.)?global[^;]*;", text):
+            assert load.group(1), (f, load.group(0))

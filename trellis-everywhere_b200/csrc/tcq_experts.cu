@@ -276,14 +276,14 @@ __device__ __forceinline__ void to_floats(const Eight<T>& e, float (&v)[8]) {
     for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(reinterpret_cast<const T*>(e.u)[i]);
 }
 __device__ __forceinline__ void load_if(bool there, const void* p, uint4& u) {       // without a branch, so that loads behind it are in flight with it
-    asm("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\t@p ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
-        : "+r"(u.x), "+r"(u.y), "+r"(u.z), "+r"(u.w) : "l"(p), "r"(uint32_t(there)));
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\t@p ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+                 : "+r"(u.x), "+r"(u.y), "+r"(u.z), "+r"(u.w) : "l"(p), "r"(uint32_t(there)) : "memory");
 }
 template <typename T>
 __device__ __forceinline__ Eight<T> load_eight(const T* p) {
     Eight<T> e;
 #pragma unroll
-    for (int q = 0; q < int(sizeof(T) / 2); ++q) e.u[q] = __ldg(reinterpret_cast<const uint4*>(p) + q);
+    for (int q = 0; q < int(sizeof(T) / 2); ++q) e.u[q] = reinterpret_cast<const uint4*>(p)[q];
     return e;
 }
 // Eight numbers at any address: pieces of 16 bytes that start on 16 bytes, one more than they fill, and a shift; single numbers where fewer than eight exist, or in
@@ -354,18 +354,23 @@ __global__ void __launch_bounds__(256, 3) tcq_combine_kernel(const __grid_consta
             for (int j0 = 0; j0 < c.top; j0 += 4) {
                 Row v[4];
                 float w[4];
+                int place[4];
                 bool some[4];
 #pragma unroll
+                for (int q = 0; q < 4; ++q) {            // (all places and weights before the first row: loads that stay where they stand hold up those behind them)
+                    place[q] = j0 + q < c.top ? places[j0 + q] : -1;
+                    w[q] = j0 + q < c.top ? weights[j0 + q] : 0.0f;
+                }
+#pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const int place = j0 + q < c.top ? __ldg(places + j0 + q) : -1;
-                    some[q] = place >= 0 && place < c.rows && there > 0;
-                    w[q] = some[q] ? __ldg(weights + j0 + q) : 0.0f;
-                    const Y* const row = static_cast<const Y*>(c.y) + place * c.ldy + c0;
+                    some[q] = place[q] >= 0 && place[q] < c.rows && there > 0;
+                    if (!some[q]) w[q] = 0.0f;           // (nobody's weight may be anything)
+                    const Y* const row = static_cast<const Y*>(c.y) + place[q] * c.ldy + c0;
                     if constexpr (ALIGNED) {
                         v[q] = {};
                         if (some[q]) v[q] = load_eight<Y>(row);
                     } else {
-                        v[q].load(row, some[q], there, place > 0 && place + 1 < c.rows);
+                        v[q].load(row, some[q], there, place[q] > 0 && place[q] + 1 < c.rows);
                     }
                 }
 #pragma unroll

@@ -42,9 +42,9 @@ __device__ __forceinline__ void activate(int act, float (&h)[N]) {
 }
 
 __device__ __forceinline__ float load_as_f32(const void* p, int dtype, long long at) {
-    if (dtype == kF32) return __ldg(static_cast<const float*>(p) + at);
-    if (dtype == kF16) return __half2float(__ldg(static_cast<const __half*>(p) + at));
-    return __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p) + at));
+    if (dtype == kF32) return static_cast<const float*>(p)[at];
+    if (dtype == kF16) return __half2float(static_cast<const __half*>(p)[at]);
+    return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[at]);
 }
 // N results of one column, in rows row, row + step ...: residual, rounding, stores.  (y may be the residual: read and written by the same thread.)
 template <typename YT, int N>

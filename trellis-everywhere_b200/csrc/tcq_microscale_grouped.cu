@@ -50,7 +50,7 @@ __device__ __forceinline__ float pow2f(int e) { return __uint_as_float(uint32_t(
 // Eight columns of x from c0 on as they are, zeros behind the last.
 template <typename T>
 __device__ __forceinline__ uint4 load8(const T* row, long long c0, long long k, bool wide) {
-    if (wide && c0 + 8 <= k) return __ldg(reinterpret_cast<const uint4*>(row + c0));
+    if (wide && c0 + 8 <= k) return *reinterpret_cast<const uint4*>(row + c0);
     uint32_t w[4] = {};
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(kPartsThreads) tcq_ms_row_parts_kernel(const _
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     bool planned = false;
     for (int i = blockIdx.x, turn = 0; i < p.groups.rows; i += gridDim.x) {
-        const int token = p.tokens != nullptr ? __ldg(p.tokens + i) : i;
+        const int token = p.tokens != nullptr ? p.tokens[i] : i;
         const bool inside = token >= 0 && token < p.x_rows;
         const T* const row = static_cast<const T*>(p.x) + (inside ? token : 0) * p.ldx;
         uint4 u = {};
@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_kernel(const __gri
         const bool one = elect_one();
         wait_for_kernel_before();                        // x's digits are there
         // (the next kernel begins when this one has ended: its warps beside these cost 800 rows of 32 groups of 2000 x 2048 6 %)
-        asm volatile("fence.proxy.async;" ::: "memory");
+        fence_for_bulk_loads();
         uint32_t s = ahead % T::kStages, phase = ahead == T::kStages ? 0 : 1, loaded = ahead;    // (the first wait for a stage is for the phase before the first)
         unsigned left = p.loads - ahead;
         bool ok = true;
@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_kernel(const __gri
             const long long r = (long long)t.tn * kRowsW + 32 * quarter + lane;
             const bool there = r < p.w.rows;
             const long long column = (long long)t.group * p.w.rows + r;
-            const float fw = FMT == kNvfp4 && there ? __ldg(p.w.row_scale + column) : 1.0f;
+            const float fw = FMT == kNvfp4 && there ? p.w.row_scale[column] : 1.0f;
             const float inner = inner_part(fw), outer = outer_part(fw);
             const float bias = p.out.bias != nullptr && there ? load_as_f32(p.out.bias, p.out.bias_dtype, column) : 0.0f;
             ok = still_waits(ok, smem_u32(&sum_full[buf]), uint32_t(n / 2) & 1, &gave_up);
@@ -552,7 +552,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) tcq_ms_grouped_wide_kernel(co
         // ---- loads; the warp stays together, one lane issues
         const bool one = elect_one();
         wait_for_kernel_before();                        // x's digits are there
-        asm volatile("fence.proxy.async;" ::: "memory");
+        fence_for_bulk_loads();
         uint32_t s = 0, phase = 1, loaded = 0;           // (the first wait for a stage is for the phase before the first)
         unsigned left = p.loads;
         bool ok = true;
@@ -646,7 +646,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) tcq_ms_grouped_wide_kernel(co
             const int buf = (2 * n + half) % T::kSums;       // (of each half, every third item: 0, 2, 1 and 1, 0, 2)
             const long long r = (2ll * t.tn + half) * kRowsW + 32 * quarter + lane, column = (long long)t.group * p.w.rows + r;
             const bool there = r < p.w.rows;
-            const float fw = FMT == kNvfp4 && there ? __ldg(p.w.row_scale + column) : 1.0f;
+            const float fw = FMT == kNvfp4 && there ? p.w.row_scale[column] : 1.0f;
             const float inner = inner_part(fw), outer = outer_part(fw);
             const float bias = p.out.bias != nullptr && there ? load_as_f32(p.out.bias, p.out.bias_dtype, column) : 0.0f;
             ok = still_waits(ok, smem_u32(&sum_full[half][buf]), uint32_t(n / T::kSums) & 1, &gave_up);
@@ -741,7 +741,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tcq_ms_grouped_few_kernel(cons
             v[0] = v[1] = v[2] = v[3] = __uint_as_float(0x7FC00000u);
         } else if (p.wide && c0 + 4 <= p.k) {
             uint2 u;
-            asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(u.x), "=r"(u.y) : "l"(from));
+            asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(u.x), "=r"(u.y) : "l"(from) : "memory");
 #pragma unroll
             for (int h = 0; h < 4; ++h) v[h] = to_f32<XT>(reinterpret_cast<const XT*>(&u)[h]);
         } else {
@@ -763,12 +763,12 @@ __global__ void __launch_bounds__(kFewThreads, 1) tcq_ms_grouped_few_kernel(cons
     launch_dependents();
     float v[kRuns][kRun];
     int token[T::kRowsX] = {}, ahead = 0;                // x's rows of the item's rows; of all rows, a lane one, where there are no more than lanes
-    if (p.tokens != nullptr && lane < p.groups.rows && p.groups.rows <= 32) asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(ahead) : "l"(p.tokens + lane));
+    if (p.tokens != nullptr && lane < p.groups.rows && p.groups.rows <= 32) asm volatile("ld.global.u32 %0, [%1];" : "=r"(ahead) : "l"(p.tokens + lane) : "memory");
     const auto fetch_tokens = [&](int row0, int rows) {
 #pragma unroll
         for (int q = 0; q < T::kRowsX; ++q) {
             const int known = __shfl_sync(0xFFFFFFFFu, ahead, (row0 + q) & 31);
-            token[q] = p.tokens == nullptr ? row0 + q : p.groups.rows <= 32 ? known : q < rows ? __ldg(p.tokens + row0 + q) : 0;
+            token[q] = p.tokens == nullptr ? row0 + q : p.groups.rows <= 32 ? known : q < rows ? p.tokens[row0 + q] : 0;
         }
     };
     const auto fetch_all = [&](int j0, int all) {
@@ -795,6 +795,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tcq_ms_grouped_few_kernel(cons
     if (warp == 0) {
         // ---- loads; the warp stays together, one lane issues
         const bool one = elect_one();
+        fence_for_bulk_loads();
         uint32_t s = 0, phase = 1, loaded = 0;           // (the first wait for a stage is for the phase before the first)
         unsigned left = p.loads;
         bool ok = true;
@@ -964,7 +965,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tcq_ms_grouped_few_kernel(cons
             const long long r = (long long)t.tn * kRowsW + 32 * quarter + lane;
             const bool there = r < p.w.rows;
             const long long column = (long long)t.group * p.w.rows + r;
-            const float fw = FMT == kNvfp4 && there ? __ldg(p.w.row_scale + column) : 1.0f;
+            const float fw = FMT == kNvfp4 && there ? p.w.row_scale[column] : 1.0f;
             const float bias = p.out.bias != nullptr && there ? load_as_f32(p.out.bias, p.out.bias_dtype, column) : 0.0f;
             ok = still_waits(ok, smem_u32(&sum_full[buf]), uint32_t(n / 2) & 1, &gave_up);
             tc_fence_after();

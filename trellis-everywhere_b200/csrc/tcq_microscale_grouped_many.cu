@@ -120,6 +120,7 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_many_kernel(const 
     if (warp == 0) {
         // ---- loads of x; the warp stays together, one lane issues
         const bool one = elect_one();
+        fence_for_bulk_loads();
         uint32_t s = 0, phase = 1, loaded = 0;           // (the first waits are for the phase before the first)
         bool ok = true;
         for (int i = blockIdx.x; i < items && ok; i += gridDim.x) {
@@ -142,6 +143,7 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_many_kernel(const 
     } else if (warp == kLoaderW) {
         // ---- loads of W, which are not held up by those of x: as far ahead as there is room
         const bool one = elect_one();
+        fence_for_bulk_loads();
         uint32_t sw = 0, pw = 1, loaded = 0;
         unsigned left = p.loads;
         bool ok = true;
@@ -221,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_many_kernel(const 
             if (FP16 || FMT != kNvfp4 || i >= items) return 1.0f;
             const GroupItem t = item_of(i);
             const long long r = (long long)t.tn * kRows + row;
-            return r < p.w.rows ? __ldg(p.w.row_scale + t.group * p.w.rows + r) : 1.0f;
+            return r < p.w.rows ? p.w.row_scale[t.group * p.w.rows + r] : 1.0f;
         };
         float next = scale_of(blockIdx.x);
         uint32_t sw = 0, pw = 0, s = 0, phase = 1;
@@ -341,19 +343,19 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_many_kernel(const 
 }
 
 // Rows of 16-bit numbers in order, zeros up to a multiple of eight columns; rows that x has not are NaN.  Threads in x: eight columns of a row each; in y: rows.
-__global__ void __launch_bounds__(256) tcq_ms_grouped_rows_kernel(const uint16_t* __restrict__ x, long long x_rows, long long k, long long ldx, const int* __restrict__ tokens, int rows,
-                                                                  uint4* __restrict__ out, int runs, bool wide) {
+__global__ void __launch_bounds__(256) tcq_ms_grouped_rows_kernel(const uint16_t* x, long long x_rows, long long k, long long ldx, const int* tokens, int rows,
+                                                                  uint4* out, int runs, bool wide) {
     wait_for_kernel_before();
     launch_dependents();
     for (long long i = (long long)blockIdx.x * blockDim.y + threadIdx.y; i < rows; i += (long long)gridDim.x * blockDim.y) {
-        const long long token = tokens != nullptr ? __ldg(tokens + i) : i;
+        const long long token = tokens != nullptr ? tokens[i] : i;
         const bool there = token >= 0 && token < x_rows;
         const uint16_t* const from = x + token * ldx;
         for (int j = threadIdx.x; j < runs; j += blockDim.x) {
             const long long c0 = 8ll * j;
             uint32_t w[4] = {};
             if (wide && there) {
-                const uint4 u = __ldg(reinterpret_cast<const uint4*>(from + c0));
+                const uint4 u = *reinterpret_cast<const uint4*>(from + c0);
                 w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
             } else {
 #pragma unroll

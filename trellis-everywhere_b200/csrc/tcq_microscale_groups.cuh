@@ -2,6 +2,7 @@
 #pragma once
 
 #include "tcq_microscale.cuh"
+#include "tcq_programmatic.cuh"
 
 namespace tcq {
 
@@ -19,7 +20,7 @@ struct GroupPlan {
     int begin[kMostGroups + 1], tile[kMostGroups + 1];
 };
 
-// By one whole warp.
+// By one whole warp, which need not have waited for the kernel before where that one does not write offsets.
 __device__ __forceinline__ void plan_groups(const Groups& g, int per, GroupPlan& plan) {
     const int lane = threadIdx.x & 31;
     if (g.offsets == nullptr) {
@@ -35,8 +36,8 @@ __device__ __forceinline__ void plan_groups(const Groups& g, int per, GroupPlan&
         const int mine = at + 4 * lane;
         int v[5];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = mine + q <= g.groups ? __ldg(g.offsets + mine + q) : 0;
-        v[4] = at + 128 <= g.groups ? __ldg(g.offsets + at + 128) : 0;            // what the last lane needs of the next ones
+        for (int q = 0; q < 4; ++q) v[q] = mine + q <= g.groups ? load_before_wait(g.offsets + mine + q) : 0;
+        v[4] = at + 128 <= g.groups ? load_before_wait(g.offsets + at + 128) : 0;            // what the last lane needs of the next ones
 #pragma unroll
         for (int q = 0; q < 5; ++q) v[q] = min(max(v[q], 0), g.rows);
 #pragma unroll
