@@ -19,3 +19,61 @@ def test_many_items_of_the_same_rows(m, k, fmt):
     b = torch.zeros(n, device=DEV)
     got = [ms.linear(x, w, bias=b) for _ in range(20)]
     assert all(torch.equal(y, want) for y in got)
+
+
+def digits_bound(x, w, fmt):
+    """Of fp32 sums of x's 4-bit parts times w (fp64 [m, k], [n, k]).  A number of x is rounded to 21 binary places of the power of two of its block's largest, 2^-22 of that off, or of 2^-17 of the
+    row's largest (nvfp4), 2^-39 of it off.  Its digits' magnitudes are less than three times its own, or than that step; sums of 64 columns each are cut off by 2^-22 of theirs at most."""
+    import moe_plain as plain
+    b, k = plain.BLOCK[fmt], x.shape[1]
+    amax = torch.nn.functional.pad(x.abs(), (0, -k % b)).reshape(x.shape[0], -1, b).amax(2).repeat_interleave(b, 1)[:, :k]
+    step = torch.maximum(amax * 2.0 ** -22, x.abs().amax(1, keepdim=True) * (2.0 ** -39 if fmt == "nvfp4" else 0))
+    return (step + (3 * x.abs() + 2 * step) * (k / 64 + 8) * 2.0 ** -22) @ w.abs().t()
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("m", [1, 2, 3, 7, 15, 30, 130, 700])
+def test_a_channel_far_above_the_others(m, dtype, fmt):
+    """A channel 60000 times the others, in whose column some results have no weight: these are as near to 64 bits as bf16 is (2^-9), the steps of the channel's block, 2^-7, notwithstanding (2^-7 sqrt(32 / 777) at most of the size of all)."""
+    import moe_plain as plain
+    from trellis_b200 import experts, microscale as ms
+    g = torch.Generator(device=DEV).manual_seed(m)
+    for n, k in ((256, 4096), (300, 777)):
+        w = torch.randn(1, n, k, generator=g, device=DEV) * 0.02
+        w[:, ::2, 100] = 0
+        q = experts.quantize_experts(w, fmt)
+        wv = ms.dequantize(experts.expert(q, 0)).double()
+        x = torch.randn(m, k, generator=g, device=DEV)
+        x[:, 100] = 60000.0
+        x = x.to(dtype)
+        y = experts.grouped_linear(x, q, torch.tensor([0, m], device=DEV).int(), dtype=torch.float32)
+        want, bound = plain.epilogue(x.double() @ wv.t(), digits_bound(x.double(), wv, fmt), None, None, None, torch.float32)
+        assert bool(((y.double() - want).abs() <= bound).all())
+        rest = y[:, ::2].double() - want[:, ::2]
+        assert float(rest.norm() / want[:, ::2].norm()) < 2.0 ** -9
+        z = ms.linear(x, experts.expert(q, 0), bias=torch.zeros(n, device=DEV))
+        assert torch.equal(z, y.to(dtype))
+
+
+@pytest.mark.parametrize("dtype,apart", [(torch.bfloat16, 14), (torch.float16, 11)], ids=str)
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("m", [1, 2, 3, 20, 200])
+def test_every_bit_as_far_down_as_the_digits_reach(m, fmt, dtype, apart):
+    """A block's numbers down to 2^-14 (fp16: 2^-11) of its largest count with every bit.  Each result is one number of x times one weight: exact, or (a block's largest may have been rounded up
+    to 2, so that the least are further below it) of the number rounded to 21 places of its block's power of two."""
+    import moe_plain as plain
+    from trellis_b200 import experts, microscale as ms
+    g = torch.Generator(device=DEV).manual_seed(m)
+    k = 256
+    w = torch.eye(k, device=DEV)[None]
+    q = experts.quantize_experts(w, fmt)
+    x = torch.ldexp(torch.rand(m, k, generator=g, device=DEV) + 1, -torch.randint(0, apart + 1, (m, k), generator=g, device=DEV)) * torch.randn(m, k, generator=g, device=DEV).sign()
+    x[:, ::16] = 1.5
+    x = x.to(dtype)
+    y = experts.grouped_linear(x, q, torch.tensor([0, m], device=DEV).int(), dtype=torch.float32)
+    wv, xd, b = ms.dequantize(experts.expert(q, 0)).double().diagonal(), x.double(), plain.BLOCK[fmt]
+    step = torch.exp2(xd.abs().reshape(m, -1, b).amax(2).log2().floor() - 21).repeat_interleave(b, 1)
+    rounded = (xd / step).round() * step
+    assert bool((rounded == xd).float().mean() > 0.99)
+    assert bool(((y.double() == xd * wv) | (y.double() == rounded * wv)).all())

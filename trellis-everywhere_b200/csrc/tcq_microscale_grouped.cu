@@ -1,10 +1,11 @@
 // Rows of 16-bit activations in groups, each group times a 4-bit microscaled matrix of its own, few rows a group: y[i] = act(W[g(i)] x[i] + bias) + residual.
 //
-// The tensor cores multiply 4-bit numbers as they lie in memory, so that a weight costs nothing but its bytes; it is x that is cut up.  With s a power of two, 1.7 s <= amax < 3.4 s for
-// the largest magnitude of a block of 16 (nvfp4) or 32 (mxfp4) columns, x / s rounded to 15 binary places is a number of six digits of base 8, each of -4 .. 3, all of which are e2m1 numbers:
-// x = s (d0 + d1 / 8 + ... + d5 / 8^5).  Each digit is a row of 4-bit numbers with block scales s, s / 8, s / 64 ..., and the product is that of tcgen05.mma with kPartsX columns for
-// each row of x, added up at the end.  Six digits hold every bit of bf16 numbers down to 2^-8 of their block's largest (fp16: 2^-5) and are off by 2^-16.7 of that at most elsewhere;
-// nvfp4's scales, of a token as of a matrix, end 2^-17 below the token's largest one: digits below that are left out (2^-18.5 of its largest number at most).
+// The tensor cores multiply 4-bit numbers as they lie in memory, so that a weight costs nothing but its bytes; it is x that is cut up.  With s the power of two of the
+// largest magnitude of a block of 16 (nvfp4) or 32 (mxfp4) columns, s <= amax < 2 s, x / s rounded to 21 binary places is a number of eight digits of base 8, each of -4 .. 3, all of which are e2m1
+// numbers: x = s (d0 + d1 / 8 + ... + d7 / 8^7).  Each digit is a row of 4-bit numbers with the block scales s, and the product is that of tcgen05.mma with kPartsX columns for each row
+// of x, added up at the end with powers of 1 / 8.  Eight digits hold every bit of bf16 numbers down to 2^-14 of their block's largest (fp16: 2^-11) and are off by 2^-22 of that at most elsewhere,
+// about what sums in fp32 are.  (With six, 2^-17, 12 and 48 tokens took 1 % less and a layer of 200 6 %, and a channel 20000 times the others left 2 % of error in results that have no weight for it.)
+// nvfp4's scales, of a token as of a matrix, end 2^-17 below the token's largest one: blocks below that have its digits (2^-39 of the token's largest number off at most).
 //
 // Work split: one small kernel finds each row's group and place, cuts it up and leaves it as the stages that the products load (codes swizzled as the tensor cores
 // read them, scales in the order of tcgen05.cp).  The other goes through items of 128 rows of a matrix x NT / kPartsX rows of its group, one CTA per SM, and begins
@@ -24,7 +25,7 @@ namespace tcq {
 
 namespace {
 
-constexpr int kPartsX = 6;
+constexpr int kPartsX = 8, kPlaces = 3 * (kPartsX - 1);      // digits, and binary places behind the first
 constexpr int kThreads = 192;                    // loader, issuer, four warps for the results
 constexpr int kRowsW = 128, kMostSplits = 8;
 
@@ -92,56 +93,60 @@ __device__ __forceinline__ uint32_t largest(const float* v) {
     return m;
 }
 
-// The exponent of a block's first scale s, no lower than leaves the last digit a scale of its own.
-__device__ __forceinline__ int first_exponent(uint32_t amax_bits) { return max(int((amax_bits + 0x266667u) >> 23) - 128, -127 + 3 * (kPartsX - 1)); }
+// The exponent of a number's power of two; denormal numbers have that of the least normal one, or less.
+__device__ __forceinline__ int exponent_of(uint32_t bits) { return int(bits >> 23) - 127; }
 
-// A block's first scale as an exponent over 2^base.  nvfp4, base the exponent of the row's scale: digits that would have a scale below 2^-9, the least, are left out, so that the
-// last one is to have this very scale.
+// A block's scale as an exponent over 2^base: mxfp4's no lower than what numbers can be multiplied by 2^kPlaces over, nvfp4's (base: that of the row's scale) than its least scale.
 template <int FMT>
-__device__ __forceinline__ int block_exponent(uint32_t amax_bits, int base) {
-    const int e = first_exponent(amax_bits) - base;
-    if (FMT == kMxfp4 || e >= 3 * (kPartsX - 1) - 9) return e;
-    return (max(e + 9, 0) + 2) / 3 * 3 - 9;
-}
-// Times 2^(15 - e); FAR: in two steps, where e may be below -112 (down to -135: nvfp4, for numbers of fp32's range).
+__device__ __forceinline__ int block_exponent(uint32_t amax_bits, int base) { return FMT == kMxfp4 ? max(exponent_of(amax_bits), kPlaces - 127) : max(exponent_of(amax_bits) - base, -9); }
+// nvfp4: the exponent of a row's scale, with which the largest block's is 2^8.  (FAR: numbers of fp32's range.)
+template <bool FAR>
+__device__ __forceinline__ int row_exponent(uint32_t amax_bits) { return max(exponent_of(amax_bits) - 8, FAR ? -126 : -60); }
+// Times 2^(kPlaces - e); FAR: in two steps, where e may be below kPlaces - 127 (down to -135: nvfp4, for numbers of fp32's range).
 template <bool FAR>
 struct Up {
     float a, b;
-    __device__ __forceinline__ Up(int e) : a(pow2f(FAR ? (15 - e) / 2 : 15 - e)), b(FAR ? pow2f(15 - e - (15 - e) / 2) : 1.0f) {}
+    __device__ __forceinline__ Up(int e) : a(pow2f(FAR ? (kPlaces - e) / 2 : kPlaces - e)), b(FAR ? pow2f(kPlaces - e - (kPlaces - e) / 2) : 1.0f) {}
     __device__ __forceinline__ float operator()(float v) const { return FAR ? v * a * b : v * a; }
 };
 
-// The six digits of v 2^-15, |v| < 3.4 * 2^15, as codes: the first in nibble 5.  Bits 24 and up mean nothing.
-// An addition rounds to a whole number and makes digits 0 .. 7 of -4 .. 3; three bits are spread to four, and all six are looked up as functions of their bits.
+// The eight digits of v 2^-kPlaces, |v| < 2^22, as codes: the first in nibble 7.
+// An addition rounds to a whole number, another makes digits 0 .. 7 of -4 .. 3; three bits are spread to four, and all eight are looked up as functions of their bits.
 __device__ __forceinline__ uint32_t digit_codes(float v) {
-    constexpr float kZero = 12582912.0f + 4.0f * (1 + 8 + 64 + 512 + 4096 + 32768);       // 3 * 2^22, and a digit 4 in every place
-    const uint32_t u = __float_as_uint(v + kZero), two = (u & 0x1FFu) | ((u << 3) & ~0x1FFu);
-    uint32_t d = (two & 0x007007u) | ((two << 1) & ~0x007007u);
-    d = (d & 0x077077u) | ((two << 2) & ~0x077077u);
+    constexpr uint32_t kZero = 4 * ((1u << 24) - 1) / 7;                                     // a digit 4 in every place
+    const uint32_t u = __float_as_uint(v + 12582912.0f) - (0x4B400000u - kZero);             // (3 * 2^22, and its bits)
+    const uint32_t two = (u & 0x00000FFFu) | ((u << 4) & 0xFFFFF000u), four = (two & 0x003F003Fu) | ((two << 2) & ~0x003F003Fu);
+    const uint32_t d = (four & 0x07070707u) | ((four << 1) & ~0x07070707u);
     const uint32_t b1 = d >> 1, b2 = d >> 2;
     const uint32_t c0 = d & ~(b1 ^ b2), c1 = (b2 & ~b1 & d) | (~b2 & ~(b1 ^ d)), c2 = (b2 & b1) | (~b2 & ~(b1 & d));      // 4 3 2 1 0 -1 .. as 6 5 4 2 0 and the sign
-    uint32_t r = (c0 & 0x111111u) | ((c1 << 1) & ~0x111111u);
-    r = (r & 0x333333u) | ((c2 << 2) & ~0x333333u);
-    return (r & 0x777777u) | (~(d << 1) & ~0x777777u);
+    uint32_t r = (c0 & 0x11111111u) | ((c1 << 1) & ~0x11111111u);
+    r = (r & 0x33333333u) | ((c2 << 2) & ~0x33333333u);
+    return (r & 0x77777777u) | (~(d << 1) & ~0x77777777u);
 }
-// The codes of two columns side by side: of part 5 - 2 b in byte b of `even`, of part 4 - 2 b in byte b of `odd`.  kept: of the codes' nibbles.
+// The codes of two columns side by side: of part 7 - 2 b in byte b of `even`, of part 6 - 2 b in byte b of `odd`.
 struct TwoColumns { uint32_t even, odd; };
-__device__ __forceinline__ TwoColumns two_columns(float a, float b, uint32_t kept) {
-    const uint32_t x = digit_codes(a) & kept, y = digit_codes(b) & kept;
-    return {(x & 0x0F0F0Fu) | ((y << 4) & ~0x0F0F0Fu), ((x >> 4) & 0x0F0F0Fu) | (y & ~0x0F0F0Fu)};
+__device__ __forceinline__ TwoColumns two_columns(float a, float b) {
+    const uint32_t x = digit_codes(a), y = digit_codes(b);
+    return {(x & 0x0F0F0F0Fu) | ((y << 4) & ~0x0F0F0F0Fu), ((x >> 4) & 0x0F0F0F0Fu) | (y & ~0x0F0F0F0Fu)};
 }
-__device__ __forceinline__ uint32_t of_part(const TwoColumns& t, int part) { return part & 1 ? t.even : t.odd; }      // (byte (5 - part) / 2 of it)
+__device__ __forceinline__ uint32_t of_part(const TwoColumns& t, int part) { return part & 1 ? t.even : t.odd; }
+__host__ __device__ constexpr int byte_of_part(int part) { return (kPartsX - 1 - part) / 2; }
 
-// The byte of the scale of a part.  e: exponent of the block's first scale (nvfp4: over the row's scale); nan: the block is not finite.
+// The byte of the scale of a part.  e: the block's exponent (nvfp4: over the row's scale); nan: the block is not finite.  mxfp4's parts behind the first have an eighth of it, so that no sum of
+// them is infinite where the first one's is not.
 template <int FMT>
 __device__ __forceinline__ uint32_t part_scale(int e, bool nan, int part) {
-    const int at = e - 3 * part;
-    if constexpr (FMT == kNvfp4) return nan ? 0x7Fu : f32_to_e4m3(pow2f(max(at, -20)));       // (below 2^-10: 0)
-    else return nan ? 0xFFu : uint32_t(at + 127);
+    if constexpr (FMT == kNvfp4) return nan ? 0x7Fu : f32_to_e4m3(pow2f(e));
+    else return nan ? 0xFFu : uint32_t(e + 127 - (part > 0 ? 3 : 0));
 }
-// The nibbles of digits whose scale is no less than the least (all of them but nvfp4's for blocks that are small beside their row's largest).
-template <int FMT>
-__device__ __forceinline__ uint32_t kept_digits(int e) { return FMT == kMxfp4 || e >= 3 * (kPartsX - 1) - 9 ? 0xFFFFFFu : 0xFFFFFFu << (4 * (kPartsX - 1) - (e + 9) / 3 * 4); }
+// A result of its parts' sums, the smallest first.
+template <int FMT, typename SumOf>
+__device__ __forceinline__ float join_parts(SumOf sum_of) {
+    float sum = sum_of(kPartsX - 1);
+#pragma unroll
+    for (int part = kPartsX - 2; part >= 0; --part) sum = __fmaf_rn(sum, FMT == kMxfp4 && part == 0 ? 1.0f : 0.125f, sum_of(part));
+    return sum;
+}
 
 // One CTA takes rows blockIdx.x, blockIdx.x + gridDim.x ...; a thread eight columns at a time (32 of them take a row of 4096 three times as long, and all of many rows no less).
 constexpr int kPartsThreads = 512;
@@ -178,7 +183,7 @@ __global__ void __launch_bounds__(kPartsThreads) tcq_ms_row_parts_kernel(const _
             __syncthreads();
             for (int q = 0; q < int(blockDim.x) / 32; ++q) m = max(m, most[turn][q]);
             turn ^= 1;
-            base = max(first_exponent(as_f32_bits<T>(m)) - 8, -126);             // the largest block's scale is 2^8
+            base = row_exponent<!std::is_same_v<T, __half>>(as_f32_bits<T>(m));
             if (threadIdx.x == 0) p.row_scale[(long long)tile * p.per + place] = pow2f(base);
         }
         uint8_t* const records = p.out + (long long)tile * p.k_tiles * p.record;
@@ -192,18 +197,18 @@ __global__ void __launch_bounds__(kPartsThreads) tcq_ms_row_parts_kernel(const _
             if (nan) u = {};
             const int e = nan ? 0 : block_exponent<FMT>(as_f32_bits<T>(m), base);
             const Up<FMT == kNvfp4 && !std::is_same_v<T, __half>> up(e + base);
-            const uint32_t kept = kept_digits<FMT>(e), w[4] = {u.x, u.y, u.z, u.w};
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
             TwoColumns two[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const T* const pair = reinterpret_cast<const T*>(&w[q]);
-                two[q] = two_columns(up(to_f32<T>(pair[0])), up(to_f32<T>(pair[1])), kept);
+                two[q] = two_columns(up(to_f32<T>(pair[0])), up(to_f32<T>(pair[1])));
             }
             uint8_t* const record = records + (j / 32) * p.record;
             const uint32_t jj = j % 32, block = jj / kLanes, from = kBytesScales<FMT> + column * 128 + 4 * (jj & 3);       // of the 256 columns
 #pragma unroll
             for (int part = 0; part < kPartsX; ++part) {
-                const uint32_t byte = (5 - part) / 2, pick = byte | (4 + byte) << 4;
+                const uint32_t byte = byte_of_part(part), pick = byte | (4 + byte) << 4;
                 *reinterpret_cast<uint32_t*>(record + (from + 128 * part + (((jj >> 2) ^ ((column + part) & 7)) << 4))) =
                     __byte_perm(__byte_perm(of_part(two[0], part), of_part(two[1], part), pick), __byte_perm(of_part(two[2], part), of_part(two[3], part), pick), 0x5410);
             }
@@ -232,9 +237,8 @@ struct Tile {
     // over half of an SM's shared memory: two CTAs never share an SM, so that none waits for another's tensor memory
     static constexpr int kSmem = kStages * kStageBytes + kBytesSum + 1024;
     static_assert(kSmem >= 116 * 1024 && kSmem <= 216 * 1024 && kStages >= 4 && kBytesW % 1024 == 0 && (2 * kBytesS) % 1024 == 0);
-    // rows whose columns are taken out of tensor memory together, in pieces of eight columns
-    static constexpr int kTake = NT <= 8 ? 1 : NT <= 16 ? 2 : 4, kPieces = (kTake * kPartsX + 7) / 8;
-    static_assert(kColumns >= 2 * kSumColumns + 8 * kPieces);                 // a piece behind the last row's lies within what is allocated
+    static constexpr int kTake = NT <= 8 ? 1 : NT <= 16 ? 2 : 4;              // rows whose columns are taken out of tensor memory together
+    static_assert(kRowsX % kTake == 0);
 };
 
 struct GroupedArgs {
@@ -293,18 +297,16 @@ __device__ __forceinline__ void add_up_parts(const Epilogue& out, const GroupIte
     }
 }
 
-// N rows' sums out of tensor memory, six columns each from `from` on in PIECES pieces of eight: added up, smallest first, and scaled.  fx: the scale of row `lane`.
-template <int FMT, int N, int PIECES>
+// N rows' sums out of tensor memory, from column `from` on: added up and scaled.  fx: the scale of row `lane`.
+template <int FMT, int N>
 __device__ __forceinline__ void take_rows(uint32_t from, float fx, float inner, float outer, bool ok, float (&h)[N]) {
-    uint32_t v[PIECES][8];
+    uint32_t v[N][kPartsX];
 #pragma unroll
-    for (int q = 0; q < PIECES; ++q) tmem_load<8>(from + 8 * q, v[q]);
+    for (int q = 0; q < N; ++q) tmem_load<kPartsX>(from + kPartsX * q, v[q]);
     tmem_wait_ld();
 #pragma unroll
     for (int q = 0; q < N; ++q) {
-        float sum = __uint_as_float(v[(q * kPartsX + kPartsX - 1) / 8][(q * kPartsX + kPartsX - 1) % 8]);
-#pragma unroll
-        for (int part = kPartsX - 2; part >= 0; --part) sum += __uint_as_float(v[(q * kPartsX + part) / 8][(q * kPartsX + part) % 8]);
+        float sum = join_parts<FMT>([&](int part) { return __uint_as_float(v[q][part]); });
         if constexpr (FMT == kNvfp4) sum = sum * inner * __shfl_sync(0xFFFFFFFFu, fx, q) * outer;
         h[q] = ok ? sum : __uint_as_float(0x7FC00000u);
     }
@@ -329,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_kernel(const __gri
     const long long atoms = (long long)p.k_tiles * T::kAtoms;
     constexpr long long kRecord = T::kBytesS + NT * 128;
 
-    const auto columns_of = [](const GroupItem& t) { return (t.rows * kPartsX + 7) & ~7; };
+    const auto columns_of = [](const GroupItem& t) { return t.rows * kPartsX; };
     const auto load_w = [&](uint32_t s, const GroupItem& t, int kt) {
         const uint32_t to = smem + s * T::kStageBytes, bar = smem_u32(&full[s]);
         mbar_expect(bar, T::kBytesW + 2 * T::kBytesS + columns_of(t) * 128);
@@ -464,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_kernel(const __gri
 #pragma unroll 1
             for (int c = 0; c < t.rows; c += T::kTake) {
                 float h[T::kTake];
-                take_rows<FMT, T::kTake, T::kPieces>(tmem + buf * T::kSumColumns + c * kPartsX + (uint32_t(32 * quarter) << 16),
+                take_rows<FMT, T::kTake>(tmem + buf * T::kSumColumns + c * kPartsX + (uint32_t(32 * quarter) << 16),
                                                      FMT == kNvfp4 && lane < T::kTake && c + lane < t.rows ? p.x_row[(long long)t.tile * T::kRowsX + c + lane] : 1.0f, inner, outer, ok, h);
                 if (c + T::kTake >= t.rows) {
                     tc_fence_before();
@@ -509,7 +511,8 @@ struct WideTile {
     static constexpr int kSums = 3, kScaleColumns = kAtoms * 4 * 3;
     static constexpr int kSmem = kStages * kStageBytes + 1024;
     static_assert(kSums * kNt + kStages * kScaleColumns <= 512 && kSmem >= 116 * 1024 && kSmem + sizeof(GroupPlan) + 1024 <= 227 * 1024 && (3 * kBytesS) % 1024 == 0);
-    static constexpr int kTake = 4, kPieces = (kTake * kPartsX + 7) / 8;
+    static constexpr int kTake = 4;
+    static_assert(kSums * kNt + kTake * kPartsX <= 512);                      // rows behind the last one's, which are taken too, lie within what is allocated
 };
 constexpr int kWideThreads = 320;                // loader, issuer, four warps for the results of each half
 
@@ -527,7 +530,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) tcq_ms_grouped_wide_kernel(co
     constexpr long long kRecord = T::kBytesS + T::kNt * 128;
     const int tiles_n2 = (p.tiles_n + 1) / 2;
 
-    const auto columns_of = [](const GroupItem& t) { return (t.rows * kPartsX + 7) & ~7; };
+    const auto columns_of = [](const GroupItem& t) { return t.rows * kPartsX; };
     const auto halves_of = [&](const GroupItem& t) { return 2 * t.tn + 1 < p.tiles_n ? 2 : 1; };
     if (warp == 0) {
         if (elect_one()) {
@@ -655,7 +658,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) tcq_ms_grouped_wide_kernel(co
 #pragma unroll 1
             for (int c = 0; c < t.rows; c += T::kTake) {
                 float h[T::kTake];
-                take_rows<FMT, T::kTake, T::kPieces>(from + c * kPartsX, FMT == kNvfp4 && lane < T::kTake && c + lane < t.rows ? p.x_row[(long long)t.tile * T::kRowsX + c + lane] : 1.0f,
+                take_rows<FMT, T::kTake>(from + c * kPartsX, FMT == kNvfp4 && lane < T::kTake && c + lane < t.rows ? p.x_row[(long long)t.tile * T::kRowsX + c + lane] : 1.0f,
                                                      inner, outer, ok, h);
                 if (c + T::kTake >= t.rows) {
                     tc_fence_before();
@@ -820,7 +823,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tcq_ms_grouped_few_kernel(cons
         bool ok = true;
         for (int i = start; i < items && ok; i += clusters, ++n) {
             const GroupItem t = item_of(i);
-            const uint32_t idesc0 = kIdesc | uint32_t((t.rows * kPartsX + 7) / 8) << 17;
+            const uint32_t idesc0 = kIdesc | uint32_t(t.rows * kPartsX / 8) << 17;
             const int buf = n & 1;
             if (n >= 2) ok = mbar_wait(smem_u32(&sum_empty[buf]), uint32_t(n / 2 - 1) & 1, &gave_up);
             if (t.tile != tile) {
@@ -913,7 +916,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tcq_ms_grouped_few_kernel(cons
                     for (int q = 0; q < T::kRowsX; ++q) {
 #pragma unroll
                         for (int h = 0; h < kCutters; ++h) m[q] = max(m[q], most[cut & 1][q][h]);
-                        base[q] = max(first_exponent(m[q]) - 8, -126);           // the largest block's scale is 2^8
+                        base[q] = row_exponent<!std::is_same_v<XT, __half>>(m[q]);
                         fx[q] = pow2f(base[q]);
                     }
                 }
@@ -932,12 +935,11 @@ __global__ void __launch_bounds__(kFewThreads, 1) tcq_ms_grouped_few_kernel(cons
                         const bool nan = m >= 0x7F800000u;
                         const int of_row = q ? base[T::kRowsX - 1] : base[0], from = nan ? 0 : block_exponent<FMT>(m, of_row), block = (run & 63) / kLanes;
                         const Up<FMT == kNvfp4 && !std::is_same_v<XT, __half>> up(from + of_row);
-                        const uint32_t kept = kept_digits<FMT>(from);
-                        const TwoColumns lo = two_columns(nan ? 0.0f : up(v[0][0]), nan ? 0.0f : up(v[0][1]), kept), hi = two_columns(nan ? 0.0f : up(v[0][2]), nan ? 0.0f : up(v[0][3]), kept);
+                        const TwoColumns lo = two_columns(nan ? 0.0f : up(v[0][0]), nan ? 0.0f : up(v[0][1])), hi = two_columns(nan ? 0.0f : up(v[0][2]), nan ? 0.0f : up(v[0][3]));
                         const uint32_t record = smem_x + run / 64 * T::kRecord + q * kPartsX * 128 + 2 * (run & 7), turn = (run & 63) >> 3;
 #pragma unroll
                         for (int part = 0; part < kPartsX; ++part) {
-                            const int byte = (5 - part) / 2;
+                            const int byte = byte_of_part(part);
                             const uint32_t codes = __byte_perm(of_part(lo, part), of_part(hi, part), byte | (4 + byte) << 4);
                             asm volatile("st.shared.u16 [%0], %1;" ::"r"(record + part * 128 + (((turn ^ (q * kPartsX + part)) & 7) << 4)), "h"(uint16_t(codes)) : "memory");
                         }
@@ -978,9 +980,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tcq_ms_grouped_few_kernel(cons
             float h[T::kRowsX];
 #pragma unroll
             for (int q = 0; q < T::kRowsX; ++q) {
-                float sum = __uint_as_float(sum_of[q * kPartsX + kPartsX - 1]);
-#pragma unroll
-                for (int part = kPartsX - 2; part >= 0; --part) sum += __uint_as_float(sum_of[q * kPartsX + part]);   // smallest first
+                float sum = join_parts<FMT>([&](int part) { return __uint_as_float(sum_of[q * kPartsX + part]); });
                 if constexpr (FMT == kNvfp4) sum = sum * inner_part(fw) * fx[q] * outer_part(fw);
                 h[q] = ok ? sum : __uint_as_float(0x7FC00000u);
                 if (splits > 1) sums[q * kRowsW + 32 * quarter + lane] = h[q];
@@ -1150,10 +1150,10 @@ cudaError_t launch_nt(const GroupedCall& c, void* ws, cudaStream_t stream) {
 
 }  // namespace
 
-// Whether weights as 16-bit numbers pay: they are made once for up to 256 rows, where digits take six columns a row, and are made anew for each row.  Both forms' estimated times, us, fitted to
-// 76 pairs of measured ones of 48 to 18000 rows (off by 15 %; the form chosen is 0.4 % slower than the faster one on average, 17 % at most): with 16-bit weights 0.35 a step of 64 columns and
-// 0.025 a row of x; with digits 0.13 (mxfp4) or 0.17 a step of 256 columns, 1.9 an item and 3.2 a million numbers of x.  (64 rows a group, 2816 x 2048: 134 and 134 in nvfp4, 131 and 111 in
-// mxfp4; 96 rows: 143 and 199, 152 and 155; 100 rows through 4096 x 4096 mxfp4: 24 and 13.)  A call whose rows are put in order first takes 2 longer, but the same form.
+// Whether weights as 16-bit numbers pay: they are made once for up to 256 rows, where digits take eight columns a row, and are made anew for each row.  Both forms' estimated times, us, fitted to
+// measured ones of 40 to 18000 rows (63 pairs, off by 15 %; the form chosen is 0.3 % slower than the faster one on average, 14 % at most): with 16-bit weights 0.35 a step of 64 columns and
+// 0.025 a row of x; with digits 0.13 (mxfp4) or 0.17 a step of 256 columns, 1.9 an item and 3.2 a million numbers of x.  (50 rows a group, 2816 x 2048: 125 and 128 in nvfp4, 117 and 102 in
+// mxfp4; 64 rows: 126 and 161, 122 and 125; 100 rows through 4096 x 4096 mxfp4: 23 and 13.)  A call whose rows are put in order first takes 2 longer, but the same form.
 static bool many_rows(long long rows, long long groups, long long n, long long k, int dtype, int fmt) {
     if (!ms_grouped_many_takes(dtype, fmt) || rows <= 32 * std::min(groups, rows)) return false;
     const double filled = double(std::min(groups, rows)), sms = ms_sm_count(), across = double((n + kRowsW - 1) / kRowsW);

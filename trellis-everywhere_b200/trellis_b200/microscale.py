@@ -228,7 +228,7 @@ def linear(x: torch.Tensor, w: Microscaled, bias: Optional[torch.Tensor] = None,
     ``bias [n]`` (fp32, fp16 or bf16), ``activation`` and ``residual [..., n]`` of x's type are applied to the fp32 sums, before the one rounding.
     ``activation``: "relu", "gelu" (with erf), "gelu_tanh", "silu", or gated, "geglu" or "swiglu": rows 2 j and 2 j + 1 of W are the gate and
     the value of result j (``interleave``), ``act(h[2 j]) * h[2 j + 1]``, and n / 2 results come out.  Products of 16-bit x with an epilogue are those of
-    ``experts.grouped_linear`` (bf16 x exact down to 2^-8 of a block's largest magnitude, fp16 x to 2^-5, the rest to 2^-16.7 of that; an infinity in x may give NaN where its sums have an infinity).
+    ``experts.grouped_linear`` (bf16 x exact down to 2^-14 of a block's largest magnitude, fp16 x to 2^-11, the rest to 2^-22 of that; an infinity in x may give NaN where its sums have an infinity).
     """
     if bias is not None or activation is not None or residual is not None:
         short = _lib.short()
