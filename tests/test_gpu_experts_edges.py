@@ -77,3 +77,36 @@ def test_every_bit_as_far_down_as_the_digits_reach(m, fmt, dtype, apart):
     rounded = (xd / step).round() * step
     assert bool((rounded == xd).float().mean() > 0.99)
     assert bool(((y.double() == xd * wv) | (y.double() == rounded * wv)).all())
+
+
+@pytest.mark.parametrize("act", ["silu", "swiglu", "gelu_tanh", "gelu", "geglu"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("m", [1, 40, 400])
+def test_tails_of_activations(m, dtype, act):
+    """Sums that are exact, from far below zero to far above: results to a few ulp of their own size, not of one.  fp32: the function's 8 ulp (an exponential and a quotient 2 each, or erfc 4, and
+    products and sums of 1 / 2), and what the rounding of its argument makes of it: the exponent of the tanh form is off by 4 roundings of itself, |2 z| <= 1.6 |h| + 0.08 |h|^3, erfc's argument
+    by 2, of h^2 / 2 in its exponent and so of h^2 + 1 in the result.  And half a step of the type; below the normal numbers, steps of the least number: the exponential's, times |h|, and
+    the result's."""
+    import moe_plain as plain
+    from trellis_b200 import microscale as ms
+    reach = {"silu": 100, "swiglu": 100, "gelu_tanh": 11, "gelu": 13, "geglu": 13}[act]
+    h = torch.linspace(-reach, 30, m * 16, dtype=torch.float64, device=DEV).to(torch.bfloat16 if dtype != torch.float16 else dtype).reshape(m, 16)
+    x = torch.zeros(m, 64, device=DEV)
+    x[:, 0:32:2], x[:, 33::2] = h.float(), 1.0
+    w = torch.zeros(32 if act in plain.GATED else 16, 64, device=DEV)
+    for j in range(16):
+        if act in plain.GATED:
+            w[2 * j, 2 * j], w[2 * j + 1, 2 * j + 33] = 1.0, 1.0
+        else:
+            w[j, 2 * j] = 1.0
+    q = ms.quantize(w, "mxfp4")
+    assert torch.equal(ms.dequantize(q), w)
+    y = ms.linear(x.to(dtype), q, activation=act).double()
+    hd = h.double()
+    want = plain.activate(hd, plain.GATED.get(act, act))
+    a = hd.abs()
+    grows = {"silu": 0 * a, "gelu_tanh": 4 * (1.6 * a + 0.08 * a ** 3), "gelu": 2 * (a * a + 1)}[plain.GATED.get(act, act)]
+    info = torch.finfo(dtype)
+    bound = want.abs() * (8 * 2.0 ** -23 + grows * 2.0 ** -24 + info.eps / 2) + (a + 2) * 2.0 ** -149 + info.smallest_normal * info.eps / 2
+    off = (y - want).abs()
+    assert bool((off <= bound).all()), (float((off / bound).max()), float(hd.flatten()[(off / bound).argmax()]))

@@ -21,9 +21,13 @@ struct Epilogue {
 
 __host__ __device__ constexpr bool act_gated(int act) { return act >= kActGeglu; }
 
-// N activations at once: one branch for all of them.  The fast exponential and quotient are within a few ulp where results are rounded to 16 bits or follow an fp32 sum
-// that is further off; -h far above 88 gives 1 / infinity, the limit.
-__device__ __forceinline__ float sigmoid(float h) { return __fdividef(1.0f, 1.0f + __expf(-h)); }
+// N activations at once: one branch for all of them.  Tails keep their relative precision, down to where the results are denormal numbers: the exponential is of -|h|, so that
+// what is divided by lies between 1 and 2 (where the fast quotient is within 2 ulp) and nothing overflows, and GELU takes erfc, not 1 + erf, which cancels.  What is left is the rounding of the
+// functions' arguments, which grows with |h|: 2 |h| ulp of GELU's tanh form, h^2 ulp of the other.
+__device__ __forceinline__ float sigmoid(float h) {
+    const float t = expf(-fabsf(h));
+    return __fdividef(h < 0.0f ? t : 1.0f, 1.0f + t);
+}
 template <int N>
 __device__ __forceinline__ void activate(int act, float (&h)[N]) {
     if (act == kActRelu) {
@@ -37,7 +41,7 @@ __device__ __forceinline__ void activate(int act, float (&h)[N]) {
         for (int i = 0; i < N; ++i) h[i] *= sigmoid(1.5957691216057308f * __fmaf_rn(0.044715f * h[i] * h[i], h[i], h[i]));
     } else if (act == kActGelu || act == kActGeglu) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) h[i] *= 0.5f + 0.5f * erff(h[i] * 0.70710678118654752f);
+        for (int i = 0; i < N; ++i) h[i] *= 0.5f * erfcf(h[i] * -0.70710678118654752f);
     }
 }
 
