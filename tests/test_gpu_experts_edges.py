@@ -110,3 +110,16 @@ def test_tails_of_activations(m, dtype, act):
     bound = want.abs() * (8 * 2.0 ** -23 + grows * 2.0 ** -24 + info.eps / 2) + (a + 2) * 2.0 ** -149 + info.smallest_normal * info.eps / 2
     off = (y - want).abs()
     assert bool((off <= bound).all()), (float((off / bound).max()), float(hd.flatten()[(off / bound).argmax()]))
+
+
+@pytest.mark.parametrize("n", [2 ** 31 - 1, 2 ** 31 - 8, 2 ** 31 - 1031])
+def test_combining_rows_of_almost_31_bits_of_columns(n):
+    """The last turn of a row's columns ends behind 2^31; what lies before and behind the result stays as it is."""
+    from trellis_b200 import _lib
+    y = torch.arange(n, dtype=torch.int64, device=DEV).bitwise_and_(255).to(torch.bfloat16)[None]
+    room = torch.full((n + 8192,), -1.0, dtype=torch.bfloat16, device=DEV)
+    out = room[4096:4096 + n][None]
+    weights, places = torch.full((1, 1), 2.0, device=DEV), torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    rc = _lib.lib().tcq_combine(y.data_ptr(), 2, 1, n, n, weights.data_ptr(), places.data_ptr(), 1, 1, None, 0, out.data_ptr(), 2, n, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    assert torch.equal(out, y * 2) and bool((room[:4096] == -1).all()) and bool((room[4096 + n:] == -1).all())

@@ -331,15 +331,16 @@ struct EightAt {
 template <typename Y, typename O, bool ALIGNED>
 __global__ void __launch_bounds__(256, 3) tcq_combine_kernel(const __grid_constant__ CombineCall c) {
     __shared__ uint4 turn[ALIGNED ? 1 : 8][ALIGNED ? 1 : 32 * (sizeof(O) / 2)];      // results of a warp, which stores neighbours
-    const int n = int(c.n), lane = threadIdx.x & 31;
+    const uint32_t n = uint32_t(c.n);                    // less than 2^31, and columns of the last turn may pass that
+    const int lane = threadIdx.x & 31;
     wait_for_kernel_before();
     launch_dependents();
     const long long stride = (long long)gridDim.x * blockDim.y;
     for (long long token = (long long)blockIdx.x * blockDim.y + threadIdx.y; token < c.tokens; token += stride) {
         const int* const places = c.places + token * c.top;
         const float* const weights = c.weights + token * c.top;
-        for (int c0 = 8 * threadIdx.x; c0 - 8 * lane < n; c0 += 8 * blockDim.x) {     // (whole warps stay together)
-            const int there = n - c0;
+        for (uint32_t c0 = 8 * threadIdx.x; c0 - 8 * lane < n; c0 += 8 * blockDim.x) {     // (whole warps stay together)
+            const int there = int(n - c0);
             float out[8] = {};
             const bool add = c.residual != nullptr && there > 0;
             const O* const from = static_cast<const O*>(c.residual) + token * c.ldr + c0;
