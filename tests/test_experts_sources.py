@@ -59,3 +59,12 @@ def test_kernels_that_begin_early_have_no_read_only_loads():
         assert not re.search(r"__ldg|\.nc\b|__restrict__", text), f
         for load in re.finditer(r"asm( volatile)?\((?:\s*\"[^\"]*\")*?\s*\"[^\"]*\bld\.(?:relaxed\.gpu\.)?global[^;]*;", text):
             assert load.group(1), (f, load.group(0))
+
+
+def test_workspaces_of_the_most_tokens():
+    """Counts of every chunk, 148 of them at most, up to the last number of tokens that is taken."""
+    from trellis_b200 import _lib
+    size = _lib.lib().tcq_route_workspace_bytes
+    for tokens in (148 * 32, 148 * 32 + 1, 1 << 30, (1 << 31) - 149, (1 << 31) - 148, (1 << 31) - 147, (1 << 31) - 2, (1 << 31) - 1):
+        chunk = -(-tokens // 148)
+        assert size(tokens, 7) == -(-tokens // chunk) * 7 * 4

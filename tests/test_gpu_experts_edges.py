@@ -123,3 +123,18 @@ def test_combining_rows_of_almost_31_bits_of_columns(n):
     rc = _lib.lib().tcq_combine(y.data_ptr(), 2, 1, n, n, weights.data_ptr(), places.data_ptr(), 1, 1, None, 0, out.data_ptr(), 2, n, torch.cuda.current_stream().cuda_stream)
     assert rc == 0
     assert torch.equal(out, y * 2) and bool((room[:4096] == -1).all()) and bool((room[4096 + n:] == -1).all())
+
+
+def test_routing_as_many_tokens_as_are_taken():
+    """2^31 - 2 tokens of one expert: the last chunk ends where an int does."""
+    from trellis_b200 import experts
+    t = 2 ** 31 - 2
+    r = experts.route(torch.zeros(t, 1, dtype=torch.bfloat16, device=DEV), 1)
+    assert r.offsets.tolist() == [0, t]
+    for at in (0, 1 << 30, t - (1 << 26)):
+        want = torch.arange(at, at + (1 << 26), dtype=torch.int32, device=DEV)
+        part = slice(at, at + (1 << 26))
+        assert torch.equal(r.places[part, 0], want) and torch.equal(r.tokens[part], want)
+        assert bool((r.weights[part] == 1).all()) and bool((r.experts[part] == 0).all())
+    del r
+    torch.cuda.empty_cache()

@@ -211,14 +211,17 @@ __global__ void __launch_bounds__(kThreads) tcq_route_kernel(const __grid_consta
     }
 }
 
+// (up to 2^31 - 1 tokens, where the end of a chunk may pass what an int holds)
+__device__ __forceinline__ int end_of_chunk(const RouteCall& c, int t0, int chunk) { return int(min(uint32_t(c.tokens), uint32_t(t0) + uint32_t(chunk))); }
+
 // A chunk of many: its experts, and how many of each.
 __global__ void __launch_bounds__(kThreads) tcq_route_choose_kernel(const __grid_constant__ RouteCall c, int chunk) {
     __shared__ int count[kMostExperts];
     wait_for_kernel_before();
     launch_dependents();
-    const int warp = threadIdx.x >> 5, t0 = blockIdx.x * chunk, t1 = min(c.tokens, t0 + chunk);
+    const int warp = threadIdx.x >> 5, t0 = blockIdx.x * chunk, t1 = end_of_chunk(c, t0, chunk);
     for (int e = threadIdx.x; e < c.experts; e += kThreads) count[e] = 0;
-    for (int t = t0 + warp; t < t1; t += kWarps) choose_any(c, t);
+    for (uint32_t t = t0 + warp; t < uint32_t(t1); t += kWarps) choose_any(c, int(t));
     __syncthreads();
     for (uint32_t i = t0 * c.top + threadIdx.x; i < uint32_t(t1 * c.top); i += kThreads) {      // (of up to 2^31 - 1)
         const int e = c.chosen[i];
@@ -263,7 +266,7 @@ __global__ void __launch_bounds__(kThreads) tcq_route_place_kernel(const __grid_
     __syncthreads();
     for (int e = threadIdx.x; e < c.experts; e += kThreads) base[e] += before[e];
     __syncthreads();
-    const int t0 = blockIdx.x * chunk, t1 = min(c.tokens, t0 + chunk), entries = (t1 - t0) * c.top;
+    const int t0 = blockIdx.x * chunk, t1 = end_of_chunk(c, t0, chunk), entries = (t1 - t0) * c.top;
     if (entries > kFewEntries) place_chunk(c, (long long)t0 * c.top, entries, base, hist);
     else if (warp == 0) place_few(c, (long long)t0 * c.top, entries, base);
 }
@@ -445,10 +448,11 @@ __global__ void __launch_bounds__(256) tcq_epilogue_kernel(const float* h, long 
 
 }  // namespace
 
+static int tokens_of_chunk(int tokens) { return std::max(32, int((tokens + (kMostChunks - 1ll)) / kMostChunks)); }
 int route_chunks(int tokens) {
     if (tokens <= kOneChunk) return 1;
-    const int chunk = std::max(32, (tokens + kMostChunks - 1) / kMostChunks);
-    return (tokens + chunk - 1) / chunk;
+    const int chunk = tokens_of_chunk(tokens);
+    return int((tokens + (chunk - 1ll)) / chunk);
 }
 
 cudaError_t launch_route(const RouteCall& c, cudaStream_t stream) {
@@ -465,7 +469,7 @@ cudaError_t launch_route(const RouteCall& c, cudaStream_t stream) {
     if (chunks == 1) {
         return launch_programmatic(tcq_route_kernel, dim3(1), dim3(kThreads), smem, 0, stream, c);
     }
-    const int chunk = std::max(32, (c.tokens + kMostChunks - 1) / kMostChunks);
+    const int chunk = tokens_of_chunk(c.tokens);
     if ((err = launch_programmatic(tcq_route_choose_kernel, dim3(unsigned(chunks)), dim3(kThreads), 0, 0, stream, c, chunk)) != cudaSuccess) return err;
     return launch_programmatic(tcq_route_place_kernel, dim3(unsigned(chunks)), dim3(kThreads), size_t(smem), 0, stream, c, chunk);
 }
