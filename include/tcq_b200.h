@@ -58,6 +58,7 @@ extern "C" {
 #define TCQ_E_BAD_FORMAT (-12)   /* microscaled format or element type unknown */
 
 /* Version of this ABI (bumped on any signature change). */
+#define TCQ_ABI_VERSION 7
 TCQ_API int tcq_abi_version(void);
 
 /* Text for a return code.  Never NULL. */

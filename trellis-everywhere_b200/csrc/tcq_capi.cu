@@ -535,7 +535,7 @@ namespace tcq { int report_cuda_error(cudaError_t err, const char* where) { retu
 
 extern "C" {
 
-int tcq_abi_version(void) { return 7; }
+int tcq_abi_version(void) { return TCQ_ABI_VERSION; }
 
 const char* tcq_strerror(int code) {
     switch (code) {

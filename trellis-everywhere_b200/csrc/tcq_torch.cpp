@@ -15,6 +15,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/version.h>
 
 #include "../../include/tcq_b200.h"
 
@@ -320,4 +321,15 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "tcq_torch", "The short way to the 
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit_tcq_torch() { return PyModule_Create(&module); }
+// built_for: what it was compiled against, (ABI of the library, torch, Python); whoever loads it looks before any other call.
+PyMODINIT_FUNC PyInit_tcq_torch() {
+    PyObject* const m = PyModule_Create(&module);
+    if (m == nullptr) return nullptr;
+    PyObject* const built_for = Py_BuildValue("(isi)", TCQ_ABI_VERSION, TORCH_VERSION, PY_VERSION_HEX >> 16);
+    if (built_for == nullptr || PyModule_AddObject(m, "built_for", built_for) < 0) {
+        Py_XDECREF(built_for);
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}

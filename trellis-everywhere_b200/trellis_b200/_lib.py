@@ -12,6 +12,7 @@ import importlib.util
 import os
 import subprocess
 import sys
+import warnings
 
 _CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "csrc")
 LIB_PATH = os.path.join(_CSRC, "libtcq_b200.so")
@@ -75,8 +76,12 @@ class TcqError(RuntimeError):
 
 def build(verbose: bool = False, jobs: int = 8) -> str:
     """Compile the CUDA sources for sm_100a with nvcc (``make`` in ``csrc/``)."""
-    cmd = ["make", "-C", _CSRC, f"-j{jobs}", "libtcq_b200.so", "tcq_torch.so", f"PYTHON={sys.executable}"]
-    subprocess.check_call(cmd, stdout=None if verbose else subprocess.DEVNULL)
+    out = None if verbose else subprocess.DEVNULL
+    subprocess.check_call(["make", "-C", _CSRC, f"-j{jobs}", "libtcq_b200.so"], stdout=out)
+    try:
+        subprocess.check_call(["make", "-C", _CSRC, "tcq_torch.so", f"PYTHON={sys.executable}"], stdout=out)
+    except subprocess.CalledProcessError as e:               # (a torch without its headers or CUDA libraries: all calls work without it)
+        warnings.warn(f"tcq_torch.so was not built ({e}): small calls go through ctypes and take twice the host's time", RuntimeWarning, stacklevel=2)
     return LIB_PATH
 
 
@@ -107,20 +112,29 @@ SHORT_BINDS = ("tcq_ms_grouped_linear_workspace_bytes", "tcq_ms_grouped_linear",
 
 
 def short():
-    """The extension that takes the small calls where all is well (``csrc/tcq_torch.cpp``), bound to the library; False where it was not built: the same calls then go
-    through ctypes, which takes twice as long."""
+    """The extension that takes the small calls where all is well (``csrc/tcq_torch.cpp``), bound to the library; False where it was not built, or (with a warning, once) was built for
+    another library, torch or Python: the same calls then go through ctypes, which takes twice as long."""
     global _short
     if _short is None:
-        handle = lib()
+        handle, _short = lib(), False
         if os.path.exists(SHORT_PATH):
-            loader = importlib.machinery.ExtensionFileLoader("tcq_torch", SHORT_PATH)
-            module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("tcq_torch", SHORT_PATH, loader=loader))
-            loader.exec_module(module)
-            module.bind(*(ctypes.cast(getattr(handle, name), ctypes.c_void_p).value for name in SHORT_BINDS))
-            _short = module
-        else:
-            _short = False
+            try:
+                _short = _load_short(handle)
+            except ImportError as e:
+                warnings.warn(f"{SHORT_PATH} is not used, small calls go through ctypes: {e} (build it anew)", RuntimeWarning, stacklevel=2)
     return _short
+
+
+def _load_short(handle: ctypes.CDLL):
+    import torch
+    loader = importlib.machinery.ExtensionFileLoader("tcq_torch", SHORT_PATH)
+    module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("tcq_torch", SHORT_PATH, loader=loader))
+    loader.exec_module(module)
+    here = (ABI_VERSION, torch.__version__.split("+")[0], sys.hexversion >> 16)
+    if getattr(module, "built_for", None) != here:
+        raise ImportError(f"it was built for {getattr(module, 'built_for', 'an unknown version')}, this is {here}")
+    module.bind(*(ctypes.cast(getattr(handle, name), ctypes.c_void_p).value for name in SHORT_BINDS))
+    return module
 
 
 def check(code: int, what: str) -> None:
