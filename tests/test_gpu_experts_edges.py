@@ -138,3 +138,17 @@ def test_routing_as_many_tokens_as_are_taken():
         assert bool((r.weights[part] == 1).all()) and bool((r.experts[part] == 0).all())
     del r
     torch.cuda.empty_cache()
+
+
+def test_a_routing_as_a_plain_tuple(monkeypatch):
+    """Its parts count, not its type, with the extension and without."""
+    from trellis_b200 import _lib, experts
+    g = torch.Generator(device=DEV).manual_seed(0)
+    r, y = experts.route(torch.randn(6, 5, generator=g, device=DEV), 2), torch.randn(12, 40, generator=g, device=DEV)
+    want = experts.combine(y, r)
+    for way in (_lib.short(), False):
+        monkeypatch.setattr(_lib, "_short", way)
+        assert torch.equal(experts.combine(y, tuple(r)), want) and torch.equal(experts.combine(y, r), want)
+        for bad in (tuple(r)[:4], list(r), r.weights):
+            with pytest.raises(ValueError):
+                experts.combine(y, bad)

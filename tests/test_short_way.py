@@ -80,3 +80,9 @@ def test_make_builds_both():
     csrc = os.path.dirname(_lib.LIB_PATH)
     plan = subprocess.run(["make", "-n", "-B", "-C", csrc], capture_output=True, text=True, check=True).stdout
     assert "libtcq_b200.so" in plan and "tcq_torch.cpp" in plan
+
+
+def test_what_is_no_routing():
+    for bad in ((1, 2, 3), [None] * 5, None, torch.zeros(5)):
+        with pytest.raises(ValueError):
+            experts.combine(torch.zeros(2, 4), bad)

@@ -231,17 +231,19 @@ def grouped_linear(x: torch.Tensor, w: ExpertMatrices, offsets: torch.Tensor, to
 def combine(y: torch.Tensor, routing: Routing, residual: Optional[torch.Tensor] = None, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``sum_j weights[t, j] * y[places[t, j]] + residual[t]`` -> ``[T, n]`` of ``dtype`` (the residual's, else y's): summed in fp32, rounded once.
 
-    ``y [rows, n]`` and ``residual [T, n]`` in fp32, fp16 or bf16; a choice without an expert adds nothing.
+    ``y [rows, n]`` and ``residual [T, n]`` in fp32, fp16 or bf16; a choice without an expert adds nothing.  (Of ``routing``, weights and places are read.)
     """
     short = _lib.short()
     out = short.combine(y, routing, residual, dtype) if short else None
     if out is not None:
         return out
+    if not isinstance(routing, tuple) or len(routing) != 5:
+        raise ValueError(f"routing must be a Routing, or its five parts as a tuple, got {type(routing).__name__}")
     if y.dim() != 2:
         raise ValueError(f"y must be [rows, n], got {tuple(y.shape)}")
     y = _check_x(y, "y")
     dev, n = y.get_device(), y.shape[1]
-    weights, places = routing.weights, routing.places
+    weights, _, places, _, _ = routing
     if weights.dim() != 2 or not 1 <= weights.shape[1] <= MOST_CHOSEN:
         raise ValueError(f"routing.weights must be [tokens, 1 to {MOST_CHOSEN}], got {tuple(weights.shape)}")
     if weights.dtype is not torch.float32 or weights.get_device() != dev or not weights.is_contiguous():
