@@ -152,3 +152,26 @@ def test_a_routing_as_a_plain_tuple(monkeypatch):
         for bad in (tuple(r)[:4], list(r), r.weights):
             with pytest.raises(ValueError):
                 experts.combine(y, bad)
+
+
+@pytest.mark.parametrize("t", [13, 100])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("score,normalize", [("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)])
+def test_weights_of_special_logits(score, normalize, dtype, t):
+    """Weight by weight: a row that is not finite excuses no other.  An exponential of a rounded difference of up to 103 (beyond, it is nothing), 2^-17.3, twice, its own 2 ulp, and a sum of five: 2^-16;
+    below the normal numbers, their steps (2^-126 is more).  Without an expert a weight is 0."""
+    import moe_plain as plain
+    from trellis_b200 import experts
+    inf, nan = float("inf"), float("nan")
+    rows = [[0.0, -0.0, 0.0, -0.0, 1e-45], [-inf] * 5, [-inf, 2.0, -inf, -inf, -inf], [nan, 1.0, 2.0, 3.0, 4.0], [-3e38, 3e38, -inf, -3e38, 3e38], [-200.0, -201.0, -200.0, -inf, -300.0],
+            [-1e-40, -2e-40, 1e-40, 0.0, -inf], [1.0, -inf, -inf, -inf, 1.0], [-29.0, -95.0, -60.0, -88.5, -110.0], [-31.0, -29.5, -94.0, -101.0, -115.0], [0.5, -70.0, -85.0, -87.0, -20.0],
+            [60.0, 20.0, -20.0, -26.0, -16.0], [88.0, 90.0, 87.0, 3.0, -3.0]]
+    logits = torch.tensor(rows, device=DEV).repeat(-(-t // len(rows)), 1)[:t].to(dtype).contiguous()
+    for top in (1, 2, 5):
+        r, want = experts.route(logits, top, score, normalize), plain.route(logits, top, score, normalize)
+        got, weights = r.weights.cpu().double(), want[0]
+        assert torch.equal(r.experts.cpu().long(), want[1])
+        assert torch.equal(got.isnan(), weights.isnan()) and int(weights.isnan().sum()) == (-(-(t - 3) // len(rows)) * (1 if score == "sigmoid" and not normalize else top))
+        assert bool((got[want[1] < 0] == 0).all())
+        off = (got - weights).abs()
+        assert bool(((off <= weights * 2.0 ** -16 + 2.0 ** -126) | weights.isnan()).all())

@@ -85,9 +85,9 @@ __device__ void choose(const RouteCall& c, int token) {
         sum = sum_of_warp(sum);
         w = lane < found ? w / sum : 0.0f;
     } else {
-        // (far below zero a sigmoid is the exponential, and a quotient of two of them needs neither: nothing underflows)
-        const float most = __shfl_sync(0xFFFFFFFFu, value, 0);
-        w = lane >= found ? 0.0f : c.normalize && most < -30.0f ? expf(value - most) : 1.0f / (1.0f + expf(-value));
+        // (below zero a sigmoid is e^v / (1 + e^v); where they are normalised, all of them over e^most where that is below 1, so that nothing underflows that a quotient of two would show)
+        const float most = __shfl_sync(0xFFFFFFFFu, value, 0), over = c.normalize && most < 0.0f ? most : 0.0f;
+        w = lane >= found ? 0.0f : (value < 0.0f ? expf(value - over) : 1.0f) / (1.0f + expf(-fabsf(value)));
         if (c.normalize) {
             const float sum = sum_of_warp(w);
             w = lane < found ? w / sum : 0.0f;
