@@ -175,3 +175,37 @@ def test_weights_of_special_logits(score, normalize, dtype, t):
         assert bool((got[want[1] < 0] == 0).all())
         off = (got - weights).abs()
         assert bool(((off <= weights * 2.0 ** -16 + 2.0 ** -126) | weights.isnan()).all())
+
+
+@pytest.mark.parametrize("fmt,dtype", [("mxfp4", torch.bfloat16), ("nvfp4", torch.bfloat16), ("nvfp4", torch.float16)], ids=str)
+@pytest.mark.parametrize("n,gather", [(1500, False), (20000, True)])
+def test_waits_of_many_rows_that_run_out(n, gather, fmt, dtype):
+    """Loads of weights that never come, in the form that takes hundreds of rows a group (it has no workspace but for rows that it puts in order): the kernel ends, what needed them is NaN, what did
+    not is right, and so is the next call."""
+    from trellis_b200 import _lib, experts
+    g = torch.Generator(device=DEV).manual_seed(0)
+    e, rows, k = 2, 600, 512                                      # two loads an item; one item a CTA, or four and more
+    w = experts.quantize_experts(torch.randn(e, n, k, generator=g, device=DEV) * k ** -0.5, fmt)
+    x = torch.randn(rows, k, generator=g, device=DEV).to(dtype)
+    tokens = torch.randperm(rows, generator=g, device=DEV).int() if gather else None
+    offsets = torch.tensor([0, 290, rows], device=DEV).int()
+    want = experts.grouped_linear(x, w, offsets, tokens)
+    L, f, d = _lib.lib(), 0 if fmt == "mxfp4" else 1, 2 if dtype == torch.bfloat16 else 1
+    assert L.tcq_ms_grouped_linear_workspace_bytes(rows, e, n, k, d, f, 1) == 0 and L.tcq_ms_grouped_linear_workspace_bytes(rows, e, n, k, d, f, 0) == rows * k * 2
+    ws = torch.empty(rows * k * 2, dtype=torch.uint8, device=DEV)
+    for loads in (0, 1, 2, 3, 5, 1000):
+        y = torch.zeros(rows, n, dtype=dtype, device=DEV)
+        rc = L.tcq_selftest_ms_grouped_waits(loads, x.data_ptr(), d, rows, k, None if tokens is None else tokens.data_ptr(), offsets.data_ptr(), e, rows, w.codes.data_ptr(), w.scales.data_ptr(),
+                                             None if w.row_scale is None else w.row_scale.data_ptr(), n, k, f, None, 0, 0, None, 0, y.data_ptr(), d, n, ws.data_ptr(), rows * k * 2,
+                                             torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        torch.cuda.synchronize()
+        right = y == want
+        assert bool((y.isnan() | right).all())
+        if loads < 2:
+            assert bool(y.isnan().all())
+        elif n == 1500 or loads == 1000:
+            assert bool(right.all())
+        else:
+            assert bool(y.isnan().any()) and bool(right.any())
+    assert torch.equal(experts.grouped_linear(x, w, offsets, tokens), want)
