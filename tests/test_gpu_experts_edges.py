@@ -209,3 +209,37 @@ def test_waits_of_many_rows_that_run_out(n, gather, fmt, dtype):
         else:
             assert bool(y.isnan().any()) and bool(right.any())
     assert torch.equal(experts.grouped_linear(x, w, offsets, tokens), want)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("t", [3, 60])
+def test_a_layer_whose_inner_results_leave_fp16(t, fmt):
+    """fp16 tokens whose gated results are beyond 65504, and whose outputs are not: with a bf16 inner type they are right.  Off by the rounding of the inner results, 2^-9, and of the last
+    ones, 2^-12, of each one's size: in norm no more than their sum, taken twice."""
+    import moe_plain as plain
+    from trellis_b200 import experts, microscale as ms
+    from trellis_b200.quant import MicroscaledExperts
+    g = torch.Generator(device=DEV).manual_seed(t)
+    rnd = lambda *s: torch.randn(*s, generator=g, device=DEV)  # noqa: E731
+    e, n, k, out = 3, 64, 96, 40
+    up, gate, down = rnd(e, n, k), rnd(e, n, k), rnd(e, out, n) * 1e-3
+    x, logits = (rnd(t, k) * 60).half(), rnd(t, e)
+    m = MicroscaledExperts(up, down, 2, gate, fmt, inner=torch.bfloat16)
+    y = m(x, logits)
+    weights, chosen, *_ = plain.route(logits, 2, "softmax", True)
+    uv, dv = ([ms.dequantize(experts.expert(q, i)).double() for i in range(e)] for q in (m.up, m.down))
+    want, most = torch.zeros(t, out, dtype=torch.float64, device=DEV), 0.0
+    for i in range(t):
+        for j in range(2):
+            h = x[i].double() @ uv[chosen[i, j]].t()
+            h = plain.activate(h[0::2], "silu") * h[1::2]
+            most = max(most, float(h.abs().max()))
+            want[i] += weights[i, j] * (h @ dv[chosen[i, j]].t())
+    assert most > 70000 and float(want.abs().max()) < 60000 and y.dtype == torch.float16
+    assert bool(y.isfinite().all()) and float((y.double() - want).norm() / want.norm()) < 2 * (2.0 ** -9 + 2.0 ** -12)
+    assert not bool(MicroscaledExperts(up, down, 2, gate, fmt)(x, logits).isfinite().all())
+    old = MicroscaledExperts(up, down, 2, gate, fmt)
+    del old.__dict__["inner"]
+    assert torch.equal(old(x.bfloat16(), logits), MicroscaledExperts(up, down, 2, gate, fmt)(x.bfloat16(), logits))
+    with pytest.raises(ValueError):
+        MicroscaledExperts(up, down, 2, gate, fmt, inner=torch.float32)

@@ -158,13 +158,18 @@ class MicroscaledExperts(nn.Module):
 
     ``up [E, n, k]`` and ``down [E, k_out, n]``; ``gate`` like ``up`` with a gated ``activation`` ("swiglu", "geglu"), None with another (``act(x @ up_e.T)``).  Biases ``[E, n]``,
     ``[E, n]``, ``[E, k_out]`` or None.  The experts and their weights come of logits (``experts.route`` with ``score`` and ``normalize``): ``router(x)``, where one is given, or what
-    ``forward`` is handed.  Sums between the products stay fp32 but for the rounding of the second one's input to x's type.
+    ``forward`` is handed.  Sums between the products stay fp32 but for the rounding of the second one's input to ``inner``, x's type where that is None: fp16 holds inner results up to 65504,
+    beyond which they are infinite, and bfloat16 any.
     """
+
+    inner: Optional[torch.dtype] = None                     # (of modules that were saved without one)
 
     def __init__(self, up: torch.Tensor, down: torch.Tensor, top_k: int, gate: Optional[torch.Tensor] = None, fmt: str = "nvfp4", activation: str = "swiglu",
                  score: str = "softmax", normalize: bool = True, router: Optional[nn.Module] = None, up_bias: Optional[torch.Tensor] = None,
-                 gate_bias: Optional[torch.Tensor] = None, down_bias: Optional[torch.Tensor] = None):
+                 gate_bias: Optional[torch.Tensor] = None, down_bias: Optional[torch.Tensor] = None, inner: Optional[torch.dtype] = None):
         super().__init__()
+        if inner not in (None, torch.float16, torch.bfloat16):
+            raise ValueError(f"inner={inner}: expected None, float16 or bfloat16")
         if up.dim() != 3 or down.dim() != 3 or down.shape[0] != up.shape[0] or down.shape[2] != up.shape[1]:
             raise ValueError(f"up must be [experts, n, k] and down [experts, k_out, n], got {tuple(up.shape)} and {tuple(down.shape)}")
         if (gate is not None) != (activation in microscale.GATED):
@@ -176,7 +181,7 @@ class MicroscaledExperts(nn.Module):
         microscale._check_act(activation, 2)
         if score not in experts.SCORES or not 1 <= top_k <= min(up.shape[0], experts.MOST_CHOSEN):
             raise ValueError(f"score={score!r}, top_k={top_k}: expected one of {sorted(experts.SCORES)} and 1 to {min(up.shape[0], experts.MOST_CHOSEN)}")
-        self.fmt, self.activation, self.top_k, self.score, self.normalize, self.router = fmt, activation, top_k, score, normalize, router
+        self.fmt, self.activation, self.top_k, self.score, self.normalize, self.router, self.inner = fmt, activation, top_k, score, normalize, router, inner
         self.shape = tuple(up.shape) + (down.shape[1],)     # experts, inner, in and out features
         dev = _cuda_device(up)
         with torch.no_grad():
@@ -215,7 +220,7 @@ class MicroscaledExperts(nn.Module):
         tokens = math.prod(x.shape[:-1])
         flat = x.reshape(tokens, k)
         r = experts.route((self.router(flat) if logits is None else logits).reshape(tokens, e), self.top_k, self.score, self.normalize)
-        h = experts.grouped_linear(flat, self.up, r.offsets, r.tokens, self.up_bias, self.activation)
+        h = experts.grouped_linear(flat, self.up, r.offsets, r.tokens, self.up_bias, self.activation, self.inner)
         y = experts.grouped_linear(h, self.down, r.offsets, bias=self.down_bias, dtype=torch.float32)
         return experts.combine(y, r, None if residual is None else residual.reshape(tokens, out), x.dtype).reshape(*x.shape[:-1], out)
 
