@@ -243,3 +243,24 @@ def test_a_layer_whose_inner_results_leave_fp16(t, fmt):
     assert torch.equal(old(x.bfloat16(), logits), MicroscaledExperts(up, down, 2, gate, fmt)(x.bfloat16(), logits))
     with pytest.raises(ValueError):
         MicroscaledExperts(up, down, 2, gate, fmt, inner=torch.float32)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("m", [1, 2, 3, 20, 60, 300])
+def test_the_largest_and_the_least_numbers(m, fmt):
+    """bf16 numbers up to the largest, and down to the least normal ones, times weights of 1: themselves, and nothing infinite on the way."""
+    from trellis_b200 import experts, microscale as ms
+    g = torch.Generator(device=DEV).manual_seed(m)
+    k = 64
+    w = torch.eye(k, device=DEV)[None]
+    q = experts.quantize_experts(w, fmt)
+    wv = ms.dequantize(experts.expert(q, 0)).double().diagonal()
+    q = q._replace(row_scale=q.row_scale / wv.float()) if fmt == "nvfp4" else q          # exactly one, or as near as fp32 comes
+    wv = ms.dequantize(experts.expert(q, 0)).double().diagonal()
+    for low, high in ((1.0, 1.99), (1.40, 1.46), (1.5, 1.75)):
+        for power in (127, 126, 0, -100):
+            x = (torch.rand(m, k, generator=g, device=DEV) * (high - low) + low).bfloat16().double().clamp(max=1.9921875) * 2.0 ** power * torch.randn(m, k, generator=g, device=DEV).sign()
+            x = x.to(torch.bfloat16)
+            y = experts.grouped_linear(x, q, torch.tensor([0, m], device=DEV).int(), dtype=torch.float32)
+            want = x.double() * wv
+            assert bool(x.isfinite().all()) and bool(((y.double() - want).abs() <= want.abs() * 2.0 ** -22).all()), (low, power)

@@ -132,12 +132,12 @@ __device__ __forceinline__ TwoColumns two_columns(float a, float b) {
 __device__ __forceinline__ uint32_t of_part(const TwoColumns& t, int part) { return part & 1 ? t.even : t.odd; }
 __host__ __device__ constexpr int byte_of_part(int part) { return (kPartsX - 1 - part) / 2; }
 
-// The byte of the scale of a part.  e: the block's exponent (nvfp4: over the row's scale); nan: the block is not finite.  mxfp4's parts behind the first have an eighth of it, so that no sum of
-// them is infinite where the first one's is not.
+// The byte of the scale of a part.  e: the block's exponent (nvfp4: over the row's scale); nan: the block is not finite.  mxfp4's are a fourth, and those of parts behind the first an eighth of that, so
+// that a sum of parts is finite where the result is: a first digit is up to 1.4 times the number, the others up to four.
 template <int FMT>
 __device__ __forceinline__ uint32_t part_scale(int e, bool nan, int part) {
     if constexpr (FMT == kNvfp4) return nan ? 0x7Fu : f32_to_e4m3(pow2f(e));
-    else return nan ? 0xFFu : uint32_t(e + 127 - (part > 0 ? 3 : 0));
+    else return nan ? 0xFFu : uint32_t(e + 127 - (part > 0 ? 5 : 2));
 }
 // A result of its parts' sums, the smallest first.
 template <int FMT, typename SumOf>
@@ -145,7 +145,7 @@ __device__ __forceinline__ float join_parts(SumOf sum_of) {
     float sum = sum_of(kPartsX - 1);
 #pragma unroll
     for (int part = kPartsX - 2; part >= 0; --part) sum = __fmaf_rn(sum, FMT == kMxfp4 && part == 0 ? 1.0f : 0.125f, sum_of(part));
-    return sum;
+    return FMT == kMxfp4 ? 4.0f * sum : sum;
 }
 
 // One CTA takes rows blockIdx.x, blockIdx.x + gridDim.x ...; a thread eight columns at a time (32 of them take a row of 4096 three times as long, and all of many rows no less).
