@@ -361,14 +361,11 @@ __global__ void __launch_bounds__(256, 3) tcq_combine_kernel(const __grid_consta
                 int place[4];
                 bool some[4];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {            // (all places and weights before the first row: loads that stay where they stand hold up those behind them)
-                    place[q] = j0 + q < c.top ? places[j0 + q] : -1;
-                    w[q] = j0 + q < c.top ? weights[j0 + q] : 0.0f;
-                }
+                for (int q = 0; q < 4; ++q) place[q] = j0 + q < c.top ? places[j0 + q] : -1;      // (before the first row: loads that stay where they stand hold up those behind them)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     some[q] = place[q] >= 0 && place[q] < c.rows && there > 0;
-                    if (!some[q]) w[q] = 0.0f;           // (nobody's weight may be anything)
+                    w[q] = some[q] ? weights[j0 + q] : 0.0f;
                     const Y* const row = static_cast<const Y*>(c.y) + place[q] * c.ldy + c0;
                     if constexpr (ALIGNED) {
                         v[q] = {};
