@@ -355,7 +355,7 @@ TCQ_API int tcq_ms_matmul(const uint8_t *x_codes, const uint8_t *x_scales, const
  *             row_scale [groups][n]
  *   bias      [groups][n] of type bias_dtype, or NULL;  residual [rows][ldr] of y's type, or NULL;  y [rows][ldy] of type y_dtype.  y may be the residual.
  * Sums, bias, activation and residual in fp32, one rounding.  x is multiplied as it is, or as sums of eight 4-bit parts: exact down to 2^-14 (fp16: 2^-11) of the largest of each 16 (nvfp4)
- * or 32 (mxfp4) columns, 2^-22 of that off at most elsewhere (nvfp4: or 2^-39 of the row's largest).  A row of x with a NaN gives NaN, one with an infinity NaN or what its sums have.  At most 1024 groups and 2^30 rows;
+ * or 32 (mxfp4) columns, 2^-22 of that off at most elsewhere (nvfp4: or 2^-39 of the row's largest; mxfp4: or 2^-128).  A row of x with a NaN gives NaN, one with an infinity NaN or what its sums have.  At most 1024 groups and 2^30 rows;
  * 1 <= k.  A row of y does not depend on the other rows' values; equal calls give equal results.
  *   ws        tcq_ms_grouped_linear_workspace_bytes(...) bytes, 256-byte aligned (may be 0); in_order: tokens is NULL, x 16-byte aligned and ldx a multiple of 8
  */

@@ -4,8 +4,10 @@
 // largest magnitude of a block of 16 (nvfp4) or 32 (mxfp4) columns, s <= amax < 2 s, x / s rounded to 21 binary places is a number of eight digits of base 8, each of -4 .. 3, all of which are e2m1
 // numbers: x = s (d0 + d1 / 8 + ... + d7 / 8^7).  Each digit is a row of 4-bit numbers with the block scales s, and the product is that of tcgen05.mma with kPartsX columns for each row
 // of x, added up at the end with powers of 1 / 8.  Eight digits hold every bit of bf16 numbers down to 2^-14 of their block's largest (fp16: 2^-11) and are off by 2^-22 of that at most elsewhere,
-// about what sums in fp32 are.  (With six, 2^-17, 12 and 48 tokens took 1 % less and a layer of 200 6 %, and a channel 20000 times the others left 2 % of error in results that have no weight for it.)
-// nvfp4's scales, of a token as of a matrix, end 2^-17 below the token's largest one: blocks below that have its digits (2^-39 of the token's largest number off at most).
+// about what sums in fp32 are.  (With six, 2^-17, 12 and 48 tokens took 1 % less, a layer of 200 6 %, 60 tokens through 12288 x 4096, which products bind, 25 %; and a channel 20000 times the others
+// left 2 % of error in results that have no weight for it.)
+// nvfp4's scales, of a token as of a matrix, end 2^-17 below the token's largest one: blocks below that have its digits (2^-39 of the token's largest number off at most).  mxfp4's end at 2^-106: numbers
+// are off by 2^-128 at least.
 //
 // Work split: one small kernel finds each row's group and place, cuts it up and leaves it as the stages that the products load (codes swizzled as the tensor cores
 // read them, scales in the order of tcgen05.cp).  The other goes through items of 128 rows of a matrix x NT / kPartsX rows of its group, one CTA per SM, and begins
@@ -312,8 +314,8 @@ __device__ __forceinline__ void take_rows(uint32_t from, float fx, float inner, 
     }
 }
 
-// Bound by latency with few items (8 rows through 4096 x 4096 nvfp4, the kernel before it included, 9.3 us) and by L2 with many (48 tokens to 8 of 64 experts of 4096 x 1024 mxfp4 33.0, the wide
-// form 29.9: 4.8 TB/s of weights).
+// Bound by latency with few items (8 rows through 4096 x 4096 nvfp4, the kernel before it included, 9.2 us) and by L2 with many (48 tokens to 8 of 64 experts of 4096 x 1024 mxfp4 31.8, the wide
+// form 30.4: 4.7 TB/s of weights).
 template <int FMT, int NT>
 __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ GroupedArgs p) {
     using T = Tile<FMT, NT>;
@@ -502,7 +504,8 @@ __global__ void __launch_bounds__(kThreads, 1) tcq_ms_grouped_kernel(const __gri
 
 // More rows an item than a few, and many items: 256 rows of W an item, two halves of which share a stage's digits of x.  What binds the form above there is what comes out of L2 (9 to 10 TB/s:
 // 17 KB of W and as many of x for 524 clocks of products); here x is read half as often.  Of the sums' buffers there are three, a half of an item each.
-// (256 tokens to 8 of 64 experts, 2048 x 2816 with SwiGLU: mxfp4 71.7 -> 63.4 us, nvfp4, whose x is read for 18 rows an item where the form above has 21, 80.5 -> 78.0.)
+// (256 tokens to 8 of 64 experts, 2816 x 2048 with SwiGLU: mxfp4 82.5 us in the form above, 70.8 in this one; nvfp4, whose x is read for 14 rows an item where the form above has 16, 86.2 and 88.4, and 64 tokens
+// of 4096 x 1024 41.8 and 36.2.)
 template <int FMT>
 struct WideTile {
     static constexpr int kNt = FMT == kMxfp4 ? 128 : 112, kRowsX = kNt / kPartsX;      // (nvfp4's scales take twice the tensor memory)
@@ -681,7 +684,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) tcq_ms_grouped_wide_kernel(co
 }
 
 // One or two rows an item, cut up by the CTA that multiplies them: one launch, and x goes from global memory to what the tensor cores read without a way round.  What a CTA's columns of x
-// become stays in shared memory while its items are of the same rows.  Bound by latency: one row through 4096 x 4096 nvfp4 6.9 us, one token to 8 of 64 experts of 2048 x 2048 7.5 (2.5 TB/s of weights).
+// become stays in shared memory while its items are of the same rows.  Bound by latency: one row through 4096 x 4096 nvfp4 7.0 us, one token to 8 of 64 experts of 2048 x 2048 7.6 (2.5 TB/s of weights).
 template <int FMT, int NT>
 struct FewTile {
     static constexpr int kAtoms = Ms<FMT>::kAtoms, kRowsX = NT / kPartsX;
@@ -1005,7 +1008,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) tcq_ms_grouped_few_kernel(cons
 }
 
 // Columns of sums for the rows of x of one item: what holds all rows of one group, or three times the mean of the groups that may have rows (a group that needs a second item reads its
-// matrix again: 384 rows of 64 groups, 4096 x 1024 mxfp4, with one and a half times the mean 36.7 us, with three times 34.0).
+// matrix again: 256 rows of 64 groups, 4096 x 1024 mxfp4, with one and a half times the mean 30.7 us, with three times 28.2).
 int columns_for(long long rows, long long groups) {
     const long long filled = std::min(rows, groups);
     for (int nt : {8, 16, 32, 64})
@@ -1025,7 +1028,7 @@ cudaError_t launch_parts(const GroupedCall& c, int nt, void* ws, uint8_t** recor
     *records = static_cast<uint8_t*>(ws) + (most_tiles(c.groups.rows, c.groups.groups, per) * per * 4 + 255) / 256 * 256;
     const PartsArgs p{c.x, c.x_rows, c.ldx, c.tokens, c.groups, c.k, k_tiles, per, (long long)record_bytes(FMT, nt), ms_rows_aligned(c.x, c.ldx), *records, static_cast<float*>(ws)};
     // Threads of a row: all of its runs at once while there are few rows; fewer where many rows fill the SMs, since what a row takes of every thread (its group and place, its largest
-    // number) is as much as eight columns do (8192 rows of 2048 columns: 256 threads 73 us, 64 64).
+    // number) is as much as eight columns do (8192 rows through 128 x 2048: 256 threads 58.4 us, 64 55.5).
     const int rows = c.groups.rows, sms = ms_sm_count();
     const int threads = std::min(rows <= sms ? 512 : rows <= 4 * sms ? 256 : rows <= 16 * sms ? 128 : 64, p.k_tiles * 32);
     const unsigned grid = unsigned(std::min<long long>(rows, sms * 1536ll / threads));
@@ -1112,8 +1115,8 @@ cudaError_t launch_few(const GroupedCall& c, cudaStream_t stream) {
     return launch_programmatic(kernel, dim3(unsigned(splits > 1 ? items * splits : std::min<long long>(items, ms_sm_count()))), dim3(kFewThreads), T::kSmem, splits, stream, map_w, p);
 }
 
-// Whether items of 256 rows of W take fewer of the SMs' turns: one such is as long as 1.75 of 128 rows.  (200 tokens to 4 of 32 experts, 2048 x 2000 mxfp4: 544 items and 26.0 us; 1088 and
-// 28.2.  60 rows through 4096 x 12288 nvfp4: 192 items of 18 rows, two turns, 22.8 us; 288 of 21 rows, two turns, 17.3.)
+// Whether items of 256 rows of W take fewer of the SMs' turns: one such is as long as 1.75 of 128 rows.  (200 tokens to 4 of 32 experts, 2000 x 2048 mxfp4: 640 items and 29.2 us; 1280 and
+// 32.0.  60 rows through 12288 x 4096 nvfp4: 240 items of 14 rows, two turns, 22.4 us; 384 of 16 rows, three turns, 20.0.  By the rule 42 such calls were 3 % slower than the other form at most.)
 bool wide_items(long long rows, long long groups, long long n, int fmt) {
     if (columns_for(rows, groups) != 128) return false;
     const long long sms = ms_sm_count(), wide_nt = fmt == kNvfp4 ? WideTile<kNvfp4>::kNt : WideTile<kMxfp4>::kNt;

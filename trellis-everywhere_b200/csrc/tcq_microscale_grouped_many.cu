@@ -10,8 +10,8 @@
 // are three: the next item begins when the first half of the last one's sums has been taken.  x and weights of 64 columns are one stage of one ring, with one barrier that says that both are
 // there and one that they are no longer needed.
 //
-// Measured: 2000 rows through 12288 x 4096 nvfp4 (fp16, GELU) 161 to 177 us, 1.1 to 1.25 PFLOP/s, 2040 tokens to 8 of 64 experts of 2816 x 2048 230 to 250; 15 % longer in long runs, at the power
-// limit.  What a stage takes beside its products is waits and arrivals (0.2 to 0.3 us with neither products nor weights made; x in boxes of 64 or 128 rows, stages of half as many
+// Measured in a graph, in short runs: 2000 rows through 12288 x 4096 nvfp4 (fp16, GELU) 168 to 173 us, 1.2 PFLOP/s, 2040 tokens to 8 of 64 experts of 2816 x 2048 228 to 232, 0.82; in long ones, at the power
+// limit, and as called back to back, 192 to 204 (1.0 PFLOP/s) and 262 to 276 (0.7).  What a stage takes beside its products is waits and arrivals (0.2 to 0.3 us with neither products nor weights made; x in boxes of 64 or 128 rows, stages of half as many
 // rows and twice as many of them, a third group of makers: no change; a fourth in place of takers 20 % longer).
 //
 // A wait that runs out (kMbarWaitCycles) makes its CTA stop, and its results from there on NaN.

@@ -198,7 +198,7 @@ def grouped_linear(x: torch.Tensor, w: ExpertMatrices, offsets: torch.Tensor, to
 
     Sums, bias and activation in fp32, rounded once.  The tensor cores multiply 4-bit numbers, so few rows of x are taken as sums of them: every bit of a bf16 number down to 2^-14
     of the largest of its block of 16 (nvfp4) or 32 (mxfp4) columns (fp16: 2^-11), and 2^-22 of that off at most elsewhere (nvfp4: or 2^-39 of the
-    row's largest); many rows are multiplied as they are.  A row of x with a NaN gives NaN, one with an infinity NaN or what its sums have.  A row's result does not depend on what the others hold, and equal calls give equal results.
+    row's largest; mxfp4: or 2^-128); many rows are multiplied as they are.  A row of x with a NaN gives NaN, one with an infinity NaN or what its sums have.  A row's result does not depend on what the others hold, and equal calls give equal results.
     """
     short = _lib.short()
     y = short.grouped_linear(x, w, offsets, tokens, bias, activation, dtype) if short and isinstance(w, ExpertMatrices) else None
